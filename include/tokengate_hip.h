@@ -422,6 +422,67 @@ int tg_decode_attention(const void *qkv, int64_t qkv_row_stride, const float *ro
 int tg_argmax_rows(const float *x, int64_t x_row_stride, int32_t n_rows, int64_t n_cols, int64_t *out,
                    hipStream_t stream);
 
+/* Next token of every row by sampling, from one given random number u[b] in [0, 1) per row.  With
+ * w_i = exp((x_i - max x) / temperature[b]) and the order "larger logits first, equal ones by index":
+ * S1 = the first top_k[b] (all where top_k <= 0 or no top_k); S2 = the shortest beginning of S1 whose mass
+ * (sum of w) is at least top_p[b] times S1's, at least one element (S1 where top_p >= 1 or no top_p); S3 = the
+ * elements of S2 with w >= min_p[b], at least one (no min_p: S2); token[b] (int64) = the first of S3 whose
+ * cumulated mass exceeds u[b] times S3's, logprob[b] (optional, fp32) = ln(w / mass of S3) of it.
+ * temperature <= 0 or NaN: the first of the order, log probability 0; no temperature: 1.  A NaN logit counts as
+ * -inf; among infinite logits only the equal ones count; a row of -inf gives token 0.  Weights are whole numbers
+ * of 2^-44 (fp32 exponentials, exact sums): the result does not depend on the launch.  x: fp32 rows of any stride
+ * and alignment, at most 262144 columns; the settings and u are dense device arrays with an entry per row.
+ * One launch's counters are zero again when it ends; workspace: tg_sample_rows_workspace_size bytes, zeroed once
+ * when it is allocated, shared by the launches of one stream, of any sizes that it holds (launches that may overlap
+ * need one each). */
+int64_t tg_sample_rows_workspace_size(int32_t n_rows, int64_t n_cols);
+int tg_sample_rows(const float *x, int64_t x_row_stride, int32_t n_rows, int64_t n_cols, const float *u,
+                   const float *temperature, const int32_t *top_k, const float *top_p, const float *min_p,
+                   int64_t *token, float *logprob, void *workspace, int64_t workspace_bytes, hipStream_t stream);
+
+/* ---- KV caches of 4 and 8 bits ----------------------------------------------------------------------------
+ * A row of one head (128 bf16 values) is four groups of 32 consecutive values, each with its least value m and a
+ * step s = bf16((max - m) / L) (L = 15 at 4 bits, 255 at 8; fp32 division), both bf16; a value is held as the whole
+ * number c = rint((x - m) / s) in 0 .. L (fp32 division) and stands for s c + m.  s < 2^-100 is held as 0; a group
+ * whose max - m is not finite in fp32 reads back as NaN (s = m = NaN).
+ * codes: (num_heads_k, head_rows, 16 * bits) bytes, element 16 e + w of a row in nibble (byte) e of its little-endian
+ * word (pair of words) w; meta: (num_heads_k, head_rows, 4, 2) bf16 = (s, m).  A head has cache_rows <= head_rows
+ * rows.  All 16-byte aligned; K and V alike. */
+
+/* n_rows rows of K and V into the cache in one launch: source row src_rows[t] (NULL: t) of source_rows, to cache row
+ * dst_rows[t] (NULL: t).  Entries outside the source or the cache are skipped; other cache rows keep what they hold;
+ * no two entries may name one cache row.  Strides in elements, multiples of 8. */
+int tg_kv_quantize(const void *k, int64_t k_row_stride, int64_t k_head_stride, const void *v, int64_t v_row_stride,
+                   int64_t v_head_stride, int64_t source_rows, const int32_t *src_rows, const int32_t *dst_rows,
+                   int64_t n_rows, int32_t num_heads_k, int32_t head_dim, int32_t bits, void *k_codes, void *k_meta,
+                   void *v_codes, void *v_meta, int64_t cache_rows, int64_t head_rows, hipStream_t stream);
+
+/* Cache rows rows[t] (NULL: t), t < n_rows, as bf16(s c + m) to row t of k_out and v_out; an entry outside the
+ * cache gives zeros. */
+int tg_kv_dequantize(const void *k_codes, const void *k_meta, const void *v_codes, const void *v_meta,
+                     int64_t cache_rows, int64_t head_rows, int32_t num_heads_k, int32_t head_dim, int32_t bits,
+                     const int32_t *rows, int64_t n_rows, void *k_out, int64_t k_row_stride, int64_t k_head_stride,
+                     void *v_out, int64_t v_row_stride, int64_t v_head_stride, hipStream_t stream);
+
+/* tg_decode_attention over a quantised cache, in one launch: q / k norm, rotary embedding and query scale as there;
+ * the new k / v rows (bf16) quantised into cache row kv_start[b] + kv_used[b] - 1; then every head over rows
+ * kv_start[b] .. kv_start[b] + kv_used[b] - 1 as they are held, the new row included, values s c + m not rounded to
+ * bf16.  A bias of -inf hides a row whatever it holds; a head that sees no row gets zeros.  A sequence whose rows
+ * are not all inside the cache, or kv_used[b] <= 0, appends nothing and gets zeros; kv_used[b] > max_seqlen_k: the
+ * first max_seqlen_k rows, of which the last is the new one.  workspace: as for tg_decode_attention,
+ * tg_decode_attention_quant_workspace_size bytes. */
+int64_t tg_decode_attention_quant_workspace_size(int32_t num_seqs, int32_t num_heads, int32_t num_heads_k,
+                                                 int32_t max_seqlen_k);
+int tg_decode_attention_quant(const void *qkv, int64_t qkv_row_stride, const float *rope, int32_t num_seqs,
+                              int32_t num_heads, int32_t num_heads_k, int32_t head_dim, int32_t bits,
+                              const void *q_norm_weight, const void *k_norm_weight, float eps,
+                              const float *q_head_scale, const float *q_row_scale, void *k_codes, void *k_meta,
+                              void *v_codes, void *v_meta, int64_t cache_rows, int64_t head_rows,
+                              const int32_t *kv_start, const int32_t *kv_used, int32_t max_seqlen_k,
+                              const float *bias_raw, int64_t bias_seq_stride, int64_t bias_head_stride,
+                              float softmax_scale, void *out, int64_t out_row_stride, void *workspace,
+                              int64_t workspace_bytes, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

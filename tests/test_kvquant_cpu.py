@@ -1,0 +1,128 @@
+"""Refusals of the quantised caches and of sampling, without a GPU: the argument checks of the Python entry points and
+of the C ABI come before any launch."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+
+def _cache(rows=10, hkv=2, bits=4):
+    from tokengate_amd import kvquant as Q
+    return Q.QuantKV.alloc(rows, hkv, bits, "cpu")
+
+
+def test_quantkv_layout_checks():
+    from tokengate_amd import kvquant as Q
+    c = _cache()
+    assert c.rows == 10 and c.n_kv_heads == 2 and c.head_rows == 10 and c.nbytes == 2 * 10 * 2 * 80
+    assert _cache(bits=8).nbytes == 2 * 10 * 2 * 144
+    with pytest.raises(RuntimeError, match="4 or 8 bits"):
+        Q.QuantKV.alloc(4, 2, 3, "cpu")
+    with pytest.raises(RuntimeError, match="codes"):
+        Q.QuantKV(8, c.k, c.k_meta, c.v, c.v_meta)
+    with pytest.raises(RuntimeError, match="codes"):
+        Q.QuantKV(4, c.k[:, ::2], c.k_meta[:, ::2], c.v[:, ::2], c.v_meta[:, ::2])
+    with pytest.raises(RuntimeError, match="meta"):
+        Q.QuantKV(4, c.k, c.k_meta.float(), c.v, c.v_meta)
+    with pytest.raises(RuntimeError, match="between heads"):
+        Q.QuantKV(4, c.k[:, 2:5], c.k_meta[:, 2:5].clone(), c.v[:, 2:5], c.v_meta[:, 2:5])
+    part = Q.QuantKV(4, c.k[:, 2:5], c.k_meta[:, 2:5], c.v[:, 2:5], c.v_meta[:, 2:5])
+    assert part.rows == 3 and part.head_rows == 10
+
+
+def test_python_refusals():
+    from tokengate_amd import decoder as dec
+    from tokengate_amd import kvquant as Q
+    c = _cache()
+    k = torch.zeros(4, 2, 128, dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match="bf16"):
+        Q.kv_quantize(k.float(), k, c)
+    with pytest.raises(RuntimeError, match="bf16"):
+        Q.kv_quantize(k[:, :1], k[:, :1], c)
+    with pytest.raises(RuntimeError, match="same rows"):
+        Q.kv_quantize(k, k[:3], c)
+    with pytest.raises(RuntimeError, match="row maps"):
+        Q.kv_quantize(k, k, c, dst_rows=torch.zeros(4, dtype=torch.int64))
+    with pytest.raises(RuntimeError, match="row maps"):
+        Q.kv_quantize(k, k, c, dst_rows=torch.zeros(3, dtype=torch.int32), n_rows=4)
+    with pytest.raises(RuntimeError, match="fewer rows"):
+        Q.kv_dequantize(c, n_rows=5, out=(k, k))
+    x = torch.zeros(2, 7)
+    one = torch.zeros(2)
+    for kw, what in ((dict(temperature=one.double()), "temperature"), (dict(top_k=one), "top_k"), (dict(top_p=one[:1]), "top_p"),
+                     (dict(min_p=torch.zeros(4)[::2]), "min_p"), (dict(workspace=one), "workspace")):
+        with pytest.raises(RuntimeError, match=what):
+            dec.sample_rows(x, one, **kw)
+    with pytest.raises(RuntimeError, match="logits"):
+        dec.sample_rows(x.double(), one)
+    with pytest.raises(RuntimeError, match="logits"):
+        dec.sample_rows(x.t(), torch.zeros(7))
+
+
+def test_sampling_settings():
+    from tokengate_amd.decode import Sampling
+    Sampling(0.7, 20, 0.8, 0.0).check(3)
+    Sampling([0.0, 1.0], [0, 5], 1.0, [0.1, 0.0]).check(2)
+    for bad in (dict(temperature=-1.0), dict(temperature=math.nan), dict(temperature=math.inf), dict(top_k=-1),
+                dict(top_k=1.5), dict(top_p=1.1), dict(top_p=-0.1), dict(min_p=2.0), dict(temperature=[1.0] * 3)):
+        with pytest.raises(ValueError):
+            Sampling(**bad).check(2)
+
+
+def _call(name, good, **change):
+    """The error of a C call whose arguments are `good` but for `change`, made before anything is launched."""
+    from tokengate_amd import _lib
+    lib = _lib.load()
+    args = dict(good, **change)
+    assert len(args) == len(_lib.SIGNATURES[name])
+    assert getattr(lib, name)(*args.values()) != 0
+    return lib.tg_last_error().decode()
+
+
+@pytest.fixture(scope="module")
+def ptr():
+    """A 256-byte aligned host address: never read, as the calls are refused."""
+    buf = ctypes.create_string_buffer(1024)
+    return (ctypes.addressof(buf) + 255) // 256 * 256, buf
+
+
+def test_c_abi_refusals(ptr):
+    p = ptr[0]
+    quant = dict(k=p, k_rs=1024, k_hs=128, v=p, v_rs=1024, v_hs=128, source_rows=4, src=None, dst=None, n=4, hkv=8, d=128,
+                 bits=4, kc=p, km=p, vc=p, vm=p, rows=4, head_rows=4, stream=None)
+    for change, text in ((dict(k=None), "null row"), (dict(bits=5), "4 or 8 bits"), (dict(d=64), "head_dim"),
+                         (dict(km=None), "null cache"), (dict(vc=p + 4), "aligned"), (dict(k=p + 2), "aligned"),
+                         (dict(k_rs=1028), "multiples of 8"), (dict(n=5), "more rows"), (dict(source_rows=3), "source"),
+                         (dict(head_rows=3), "head_rows"), (dict(hkv=0), "KV heads"), (dict(n=-1), "row count"),
+                         (dict(rows=1 << 31, head_rows=1 << 31), "cache rows")):
+        assert text in _call("tg_kv_quantize", quant, **change), change
+    read = dict(kc=p, km=p, vc=p, vm=p, rows=4, head_rows=4, hkv=8, d=128, bits=8, map=None, n=4, k=p, k_rs=1024, k_hs=128,
+                v=p, v_rs=1024, v_hs=128, stream=None)
+    for change, text in ((dict(n=5), "more rows"), (dict(v=None), "null row"), (dict(bits=16), "4 or 8"), (dict(v_hs=64), "head strides")):
+        assert text in _call("tg_kv_dequantize", read, **change), change
+    attn = dict(qkv=p, qkv_rs=4096, rope=p, n=1, h=16, hkv=8, d=128, bits=4, qw=p, kw=p, eps=1e-6, qh=None, qr=None, kc=p,
+                km=p, vc=p, vm=p, rows=4, head_rows=4, start=p, used=p, max_k=4, bias=None, bias_s=0, bias_h=0, scale=0.1,
+                out=p, out_rs=2048, ws=p, ws_n=1 << 30, stream=None)
+    for change, text in ((dict(qkv=None), "null pointer"), (dict(h=15), "multiple of the KV heads"), (dict(qkv_rs=4088), "row strides"),
+                         (dict(out_rs=2044), "row strides"), (dict(scale=0.0), "softmax_scale"), (dict(d=64), "head_dim"),
+                         (dict(bits=2), "4 or 8"), (dict(rope=p + 4), "aligned"), (dict(n=-1), "sequence count"),
+                         (dict(max_k=-1), "length"), (dict(h=264), "256")):
+        assert text in _call("tg_decode_attention_quant", attn, **change), change
+    sample = dict(x=p, rs=100, n=1, cols=100, u=p, t=None, k=None, tp=None, mp=None, token=p, lp=None, ws=p, ws_n=1 << 30, stream=None)
+    for change, text in ((dict(u=None), "null pointer"), (dict(rs=99), "row stride"), (dict(cols=0), "columns"),
+                         (dict(cols=262145, rs=262145), "columns"), (dict(n=-1), "rows")):
+        assert text in _call("tg_sample_rows", sample, **change), change
+
+
+def test_workspace_sizes():
+    """Sizes never shrink as a launch grows, and bad sizes ask for nothing."""
+    from tokengate_amd import _lib
+    lib = _lib.load()
+    assert lib.tg_decode_attention_quant_workspace_size(0, 16, 8, 100) == 0
+    assert lib.tg_decode_attention_quant_workspace_size(1, 16, 7, 100) == 0
+    assert lib.tg_sample_rows_workspace_size(0, 100) == 0 and lib.tg_sample_rows_workspace_size(1, 0) == 0
+    sizes = [lib.tg_decode_attention_quant_workspace_size(4, 16, 8, n) for n in (1, 64, 65, 1000, 5000, 40000, 131072)]
+    assert sizes == sorted(sizes)
+    sizes = [lib.tg_sample_rows_workspace_size(n, 151936) for n in (1, 2, 3, 8, 64)]
+    assert sizes == sorted(sizes)

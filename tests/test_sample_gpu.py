@@ -1,0 +1,181 @@
+"""sample_rows against the definition in float64 (numpy, by sorting).
+
+The kernel's weights are good to 2^-40 and rounded to 2^-45 of the largest, and their sums are exact: up to 2^18 such
+roundings come to 2^-27 at worst and 2^-36 at random.  So its choices equal the definition's wherever the numbers that
+decide are apart from their borders by more than 2^-34: u times the kept mass from the cumulated masses around it,
+top_p times the mass from those, and min_p from the weights.  Rows that are nearer (2^18 borders times 2^-33: one in
+thirty thousand at most) are left out, and their number is checked.  Log probabilities are rounded to fp32, 2^-24."""
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+NEAR = 2.0 ** -34
+
+
+def reference(x, u, t, k, p, m):
+    """(token, log probability, near a border) of one row, float64."""
+    x = np.where(np.isnan(x), -np.inf, x.astype(np.float64))
+    order = np.lexsort((np.arange(len(x)), -x))
+    if not t > 0 or x[order[0]] == -np.inf:
+        return int(order[0]), 0.0, False
+    if 0 < k < len(x):
+        order = order[:k]
+    with np.errstate(invalid="ignore"):
+        w = np.where(x[order] == x[order[0]], 1.0, np.exp((x[order] - x[order[0]]) / np.float64(t)))
+    cum, near = np.cumsum(w), False
+    if p < 1:
+        target = np.float64(p) * cum[-1]
+        near |= bool(np.min(np.abs(cum[:-1] - target), initial=np.inf) < NEAR * cum[-1]) if len(cum) > 1 else False
+        n = min(int(np.searchsorted(cum, target)) + 1, len(w))
+        w, order = w[:n], order[:n]
+    if m > 0:
+        near |= bool(np.min(np.abs(w[w != 1] - m), initial=np.inf) < NEAR)      # (weights of 1 are exact)
+        n = max(1, int((w >= np.float64(m)).sum()))
+        w, order = w[:n], order[:n]
+    cum = np.cumsum(w)
+    target = np.float64(u) * cum[-1]
+    near |= bool(np.min(np.abs(cum[:-1] - target), initial=np.inf) < NEAR * cum[-1]) if len(cum) > 1 else False
+    i = min(int(np.searchsorted(cum, target, side="right")), int((w > 0).sum()) - 1)
+    return int(order[i]), float(np.log(w[i] / cum[-1])), near
+
+
+def check(dev, x, u, t, k, p, m, **kw):
+    from tokengate_amd import decoder as dec
+    f = lambda v, dt: None if v is None else torch.tensor(v, dtype=dt, device=dev)
+    x = x.to(dev) if not x.is_cuda else x
+    tok, lp = dec.sample_rows(x, f(u, torch.float32), f(t, torch.float32), f(k, torch.int32), f(p, torch.float32),
+                              f(m, torch.float32), logprob=True, **kw)
+    torch.cuda.synchronize()
+    near = 0
+    n = x.shape[0]
+    f32 = lambda v, d: [d] * n if v is None else [float(np.float32(e)) for e in v]
+    for b, (uu, tt, kk, pp, mm) in enumerate(zip(f32(u, 0), f32(t, 1), k or [0] * n, f32(p, 1), f32(m, 0))):
+        want, wlp, border = reference(x[b].cpu().numpy(), uu, tt, kk, pp, mm)
+        if border:
+            near += 1
+            continue
+        assert int(tok[b]) == want, (b, int(tok[b]), want)
+        assert abs(float(lp[b]) - wlp) <= 2.0 ** -24 * abs(wlp) + 2.0 ** -34, (b, float(lp[b]), wlp)
+    return tok, lp, near
+
+
+def logits(n, v, seed, bf16=True, std=2.0):
+    g = torch.Generator().manual_seed(seed)
+    x = std * torch.randn(n, v, generator=g)
+    x.scatter_add_(1, torch.randint(v, (n, 12), generator=g), 6 * torch.rand(n, 12, generator=g))
+    return x.bfloat16().float() if bf16 else x
+
+
+@pytest.mark.parametrize("n,v,bf16", [(1, 1, True), (3, 2, True), (5, 7, False), (4, 255, True), (2, 1023, False), (3, 1024, True),
+                                      (2, 4097, True), (7, 32001, False), (3, 151936, True), (2, 151935, False), (1, 262144, True)])
+def test_sizes(cuda, n, v, bf16):
+    """Odd sizes (rows that start at any 4-byte address), bf16 logits (many ties) and fp32 ones, all settings."""
+    rng = np.random.default_rng(v + n)
+    near = 0
+    for i, (k, p, m) in enumerate([(0, 1.0, 0.0), (20, 1.0, 0.0), (0, 0.9, 0.0), (0, 1.0, 0.05), (50, 0.8, 0.02), (1, 0.5, 0.5)]):
+        x = logits(n, v, 10 * v + i, bf16)
+        near += check(cuda, x, list(rng.random(n, dtype=np.float32)), list(rng.uniform(0.3, 1.7, n)), [k] * n, [p] * n, [m] * n)[2]
+    assert near == 0
+
+
+def test_many_random_rows(cuda):
+    """Rows with settings of their own."""
+    rng = np.random.default_rng(5)
+    n = 512
+    x = logits(n, 5000, 9)
+    near = check(cuda, x, list(rng.random(n, dtype=np.float32)), list(rng.choice([0.0, 0.2, 0.7, 1.0, 1.5, 5.0], n)),
+                 [int(a) for a in rng.choice([0, 1, 2, 20, 200, 4999, 5000, 9000], n)], list(rng.choice([0.0, 0.1, 0.5, 0.95, 0.999, 1.0], n)),
+                 list(rng.choice([0.0, 0.001, 0.1, 1.0], n)))[2]
+    assert near == 0
+
+
+def test_defaults_and_ends(cuda):
+    """No settings at all; u at both ends of its range (and at 1, which a rounding may give): the first token and the
+    last one with a weight."""
+    x = logits(4, 3000, 1)
+    check(cuda, x, [0.0, 0.25, 0.5, 1 - 2.0 ** -24], None, None, None, None)
+    x[:, 100:] = -float("inf")
+    tok, _, _ = check(cuda, x, [0.0] * 4, [1.0] * 4, None, None, None)
+    assert torch.equal(tok.cpu(), x.argmax(1))
+    tok, _, _ = check(cuda, x, [1.0] * 4, [1.0] * 4, None, None, None)
+    assert bool((tok < 100).all())
+
+
+def test_odd_values(cuda):
+    """Ties everywhere, infinities, NaN (as -inf), rows of -inf, values far apart, signed zeros, tiny temperatures."""
+    inf, nan = float("inf"), float("nan")
+    x = torch.zeros(12, 300)
+    x[1, 7:9] = inf                                     # the two infinite ones, alike
+    x[2] = -inf                                         # token 0
+    x[3] = nan
+    x[4, ::2] = nan                                     # the odd ones
+    x[5] = torch.linspace(-3e38, 3e38, 300)
+    x[6, 100:] = -0.0
+    x[7] = torch.arange(300).float()
+    x[8] = -inf
+    x[8, 250] = -5.0
+    x[9, 3], x[9, 4] = nan, inf
+    x[10] = 1e-30 * torch.arange(300)
+    x[11] = torch.arange(300).flip(0).float() * 1e-3
+    u = [0.999, 0.6, 0.3, 0.9, 0.5, 0.5, 0.7, 0.1, 0.99, 0.5, 0.31, 0.77]
+    for t in (1.0, 1e-3, 100.0, 1e-30, 3e38):
+        tok, _, near = check(cuda, x, u, [t] * 12, None, None, None)
+        assert tok[1] == 8 and tok[2] == 0 and tok[3] == 0 and tok[4] % 2 == 1 and tok[8] == 250 and tok[9] == 4 and tok[0] == 299
+    check(cuda, x, u, [1.0] * 12, [3] * 12, [0.99] * 12, [0.01] * 12)
+    tok, lp, _ = check(cuda, x, u, [0.0] * 12, [3] * 12, [0.9] * 12, [0.1] * 12)
+    assert bool((lp == 0).all()) and tok[7] == 299 and tok[0] == 0 and tok[1] == 7 and tok[9] == 4
+
+
+def test_greedy_is_argmax(cuda):
+    from tokengate_amd import decoder as dec
+    x = logits(6, 151936, 3).to(cuda)
+    t = torch.zeros(6, device=cuda)
+    tok = dec.sample_rows(x, torch.rand(6, device=cuda), t)
+    assert torch.equal(tok, dec.argmax_rows(x))
+    k1 = dec.sample_rows(x, torch.rand(6, device=cuda), t + 1, top_k=torch.ones(6, dtype=torch.int32, device=cuda))
+    assert torch.equal(k1, tok)
+
+
+def test_frequencies(cuda):
+    """65535 stratified random numbers: every token's count is within one of its probability's share."""
+    from tokengate_amd import decoder as dec
+    n = 65535
+    x = torch.tensor([0.0, 1.0, 2.0, -1.0, 1.0, 0.5, -20.0], device=cuda)
+    u = ((torch.arange(n, device=cuda, dtype=torch.float64) + 0.5) / n).float()
+    tok = dec.sample_rows(x.repeat(n, 1), u, torch.full((n,), 0.8, device=cuda))
+    got = torch.bincount(tok, minlength=7).double()
+    want = torch.softmax(x.double() / 0.8, 0) * n
+    assert bool(((got - want).abs() <= 1.5).all()), (got, want)
+
+
+def test_shared_workspace_strides_stream_and_graph(cuda):
+    """One workspace for launches of other sizes, padded rows, a side stream, and a captured launch replayed with
+    other logits and numbers."""
+    from tokengate_amd import decoder as dec
+    ws = dec.sample_rows_workspace(9, 151936, cuda)
+    rng = np.random.default_rng(2)
+    for n, v in ((9, 151936), (1, 50), (3, 40000), (9, 1000), (2, 151936)):
+        wide = torch.full((n, v + 3), float("nan"))
+        wide[:, 1:v + 1] = logits(n, v, n + v)
+        x = wide.to(cuda)[:, 1:v + 1]
+        check(cuda, x, list(rng.random(n, dtype=np.float32)), [0.9] * n, [40] * n, [0.9] * n, None, workspace=ws)
+    x, u, t = logits(4, 30000, 8).to(cuda), torch.rand(4, device=cuda), torch.full((4,), 0.9, device=cuda)
+    p = torch.full((4,), 0.95, device=cuda)
+    want = dec.sample_rows(x, u, t, None, p, workspace=ws)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = dec.sample_rows(x, u, t, None, p, workspace=ws)
+    side.synchronize()
+    assert torch.equal(got, want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        tok, lp = dec.sample_rows(x, u, t, None, p, workspace=ws, logprob=True)
+    for i in range(4):
+        x.copy_(logits(4, 30000, 50 + i))
+        u.copy_(torch.rand(4, generator=torch.Generator().manual_seed(i)))
+        graph.replay()
+        torch.cuda.synchronize()
+        w, l = dec.sample_rows(x, u, t, None, p, workspace=ws, logprob=True)
+        assert torch.equal(tok, w) and torch.equal(lp, l), i

@@ -63,10 +63,18 @@ SIGNATURES = {
                             vp, i64, i64, f32, vp, i64, vp, i64, vp],
     "tg_decode_attention_workspace_size": [i32, i32, i32, i32],
     "tg_argmax_rows": [vp, i64, i32, i64, vp, vp],
+    "tg_kv_quantize": [vp, i64, i64, vp, i64, i64, i64, vp, vp, i64, i32, i32, i32, vp, vp, vp, vp, i64, i64, vp],
+    "tg_kv_dequantize": [vp, vp, vp, vp, i64, i64, i32, i32, i32, vp, i64, vp, i64, i64, vp, i64, i64, vp],
+    "tg_decode_attention_quant": [vp, i64, vp, i32, i32, i32, i32, i32, vp, vp, f32, vp, vp, vp, vp, vp, vp, i64, i64,
+                                  vp, vp, i32, vp, i64, i64, f32, vp, i64, vp, i64, vp],
+    "tg_decode_attention_quant_workspace_size": [i32, i32, i32, i32],
+    "tg_sample_rows": [vp, i64, i32, i64, vp, vp, vp, vp, vp, vp, vp, vp, i64, vp],
+    "tg_sample_rows_workspace_size": [i32, i64],
 }
 RESTYPES = {"tg_last_error": C.c_char_p, "tg_keybias_fwd_workspace_size": C.c_int64,
             "tg_keybias_varlen_fwd_workspace_size": C.c_int64, "tg_keybias_varlen_kv_fwd_workspace_size": C.c_int64,
-            "tg_decode_attention_workspace_size": C.c_int64, "tg_gate_select_pack_workspace_size": C.c_int64}
+            "tg_decode_attention_workspace_size": C.c_int64, "tg_decode_attention_quant_workspace_size": C.c_int64,
+            "tg_sample_rows_workspace_size": C.c_int64, "tg_gate_select_pack_workspace_size": C.c_int64}
 
 
 def lib_path(site: str = None) -> str:

@@ -566,6 +566,43 @@ def argmax_rows(logits: torch.Tensor) -> torch.Tensor:
     return out
 
 
+def sample_rows_workspace(n_rows: int, n_cols: int, device) -> torch.Tensor:
+    """Zeroed workspace for sample_rows calls of up to n_rows rows of n_cols columns (its counters stay zero between
+    calls)."""
+    n = int(_lib.load().tg_sample_rows_workspace_size(int(n_rows), int(n_cols)))
+    return torch.zeros(max(n, 16), dtype=torch.uint8, device=device)
+
+
+def sample_rows(logits: torch.Tensor, u: torch.Tensor, temperature: Optional[torch.Tensor] = None,
+                top_k: Optional[torch.Tensor] = None, top_p: Optional[torch.Tensor] = None,
+                min_p: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None, logprob: bool = False):
+    """Next tokens (B,) int64 of fp32 logits (B, V) sampled with the random numbers u (B,) fp32 in [0, 1)
+    (tg_sample_rows): the logits over temperature, then of the tokens in falling order (equal ones by index) the
+    first top_k, of those the shortest beginning that holds top_p of their mass, of those the ones of at least
+    min_p times the best one's probability; u picks by cumulated mass in that order.  The settings are (B,) tensors
+    (fp32; top_k int32) or None; temperature 0 is greedy, top_k 0, top_p 1 and min_p 0 keep everything.  With
+    logprob also the tokens' log probabilities (B,) fp32 in the distribution that was sampled.  workspace:
+    sample_rows_workspace, kept between calls of one stream (None: a new one)."""
+    if logits.dtype != torch.float32 or logits.dim() != 2 or logits.shape[1] < 1 or logits.stride(1) != 1:
+        raise RuntimeError("sample_rows: logits must be fp32 (B, V) rows")
+    n, V = logits.shape
+    for t, dt, what in ((u, torch.float32, "u"), (temperature, torch.float32, "temperature"), (top_k, torch.int32, "top_k"),
+                        (top_p, torch.float32, "top_p"), (min_p, torch.float32, "min_p")):
+        if t is not None and (t.dtype != dt or not t.is_contiguous() or t.numel() != n or t.device != logits.device):
+            raise RuntimeError(f"sample_rows: {what} must be contiguous {dt} with one entry per row, on the logits' device")
+    if workspace is None:
+        workspace = sample_rows_workspace(n, V, logits.device)
+    elif workspace.dtype != torch.uint8 or not workspace.is_contiguous() or workspace.device != logits.device:
+        raise RuntimeError("sample_rows: workspace must be contiguous bytes on the logits' device")
+    out = torch.empty(n, dtype=torch.int64, device=logits.device)
+    lp = torch.empty(n, dtype=torch.float32, device=logits.device) if logprob else None
+    if n:
+        _lib.call("tg_sample_rows", logits.data_ptr(), logits.stride(0) if n > 1 else V, n, V, u.data_ptr(),
+                  *(t.data_ptr() if t is not None else None for t in (temperature, top_k, top_p, min_p)), out.data_ptr(),
+                  lp.data_ptr() if logprob else None, workspace.data_ptr(), workspace.numel(), _stream(logits))
+    return (out, lp) if logprob else out
+
+
 def logits_last(wts: DecoderWeights, h: torch.Tensor, last_rows: torch.Tensor) -> torch.Tensor:
     """Final norm + LM head on the given rows only (the rows that produce the next token)."""
     rows = h.index_select(0, last_rows)
