@@ -1,4 +1,4 @@
-"""Greedy decode after the gated prefill, over the pruned KV caches.
+"""Decode after the gated prefill, over the pruned KV caches: greedy, or with sampled tokens.
 
 Follows generate_batch (tokengate/e2e_gate/decode/gate_decode.py:88-262) in its default form:
 layers at or below the gate attend over the full prompt cache (prune_below_gate=False) plus the
@@ -18,17 +18,25 @@ every step launches the same kernels with the same arguments: with graph=True th
 later steps replay one captured HIP graph of the whole step (144 launches for 28 layers), whose inputs
 and outputs are static device buffers; the first step runs eagerly and warms every kernel and
 library handle the capture records.
+
+Two options leave the reference's decode.  With kv_bits 4 or 8 every layer's prompt rows are quantised
+into a cache of that many bits (kvquant.QuantKV; the prefill's bf16 caches may then be freed) and each
+layer's launch is tg_decode_attention_quant, which quantises the new rows on the way in.  With a Sampling
+the tokens are drawn by tg_sample_rows from one uniform random number per sequence and step, all of them
+drawn ahead from its seed.
 """
 import math
 from dataclasses import dataclass
-from typing import List, Optional
+from typing import List, Optional, Sequence, Union
 
 import torch
 
 from tokengate_amd.decoder import (CacheGap, DecoderWeights, LayerKV, argmax_rows, decode_attention,
                                    decode_attention_workspace, decode_begin, h2d, linear_rows, linear_rows_norm,
-                                   linear_rows_norm_act, linear_rows_swiglu, logits_last, rmsnorm, silu_mul)
+                                   linear_rows_norm_act, linear_rows_swiglu, logits_last, rmsnorm, sample_rows,
+                                   sample_rows_workspace, silu_mul)
 from tokengate_amd.gate import ScoringHead
+from tokengate_amd.kvquant import (QuantKV, decode_attention_quant, decode_attention_quant_workspace, kv_quantize)
 from tokengate_amd.prefill import PrefillResult
 
 
@@ -38,6 +46,55 @@ class _Group:
     seg: List[int]            # host: segment start per sequence
     n0: List[int]             # host: rows per sequence when decoding starts
     gap: int
+
+
+@dataclass
+class Sampling:
+    """How next tokens are drawn (decoder.sample_rows); every setting a number, or a sequence with one per
+    sequence of the batch.  temperature 0 is greedy, top_k 0, top_p 1 and min_p 0 keep everything."""
+    temperature: Union[float, Sequence[float]] = 1.0
+    top_k: Union[int, Sequence[int]] = 0
+    top_p: Union[float, Sequence[float]] = 1.0
+    min_p: Union[float, Sequence[float]] = 0.0
+    seed: int = 0
+
+    def _values(self, name: str, B: int) -> list:
+        x = getattr(self, name)
+        x = [x] * B if isinstance(x, (int, float)) else list(x)
+        if len(x) != B:
+            raise ValueError(f"Sampling: {name} needs one value per sequence ({B}), got {len(x)}")
+        return x
+
+    def check(self, B: int) -> None:
+        """ValueError unless every setting is a number of its range, one or B of them."""
+        for name, ok, what in (("temperature", lambda v: 0 <= v < math.inf, "a finite number of at least 0"),
+                               ("top_k", lambda v: v == int(v) and 0 <= v < 2 ** 31, "a whole number of at least 0"),
+                               ("top_p", lambda v: 0 <= v <= 1, "in 0..1"), ("min_p", lambda v: 0 <= v <= 1, "in 0..1")):
+            for v in self._values(name, B):
+                if math.isnan(v) or math.isinf(v) or not ok(v):
+                    raise ValueError(f"Sampling: {name} must be {what} (got {v})")
+
+
+class TokenSampler:
+    """The next tokens of a batch's logits: the settings on the device, and every step's random numbers, drawn
+    ahead from the seed."""
+
+    def __init__(self, sampling: Sampling, B: int, vocab: int, n_draws: int, device):
+        sampling.check(B)
+        self.settings = [h2d(torch.tensor(sampling._values(name, B), dtype=dt), device)
+                         for name, dt in (("temperature", torch.float32), ("top_k", torch.int32),
+                                          ("top_p", torch.float32), ("min_p", torch.float32))]
+        g = torch.Generator(device=device).manual_seed(int(sampling.seed))
+        self.draws = torch.rand(n_draws, B, generator=g, dtype=torch.float32, device=device)
+        self.u = torch.empty(B, dtype=torch.float32, device=device)     # this step's
+        self.ws = sample_rows_workspace(B, vocab, device)
+
+    def set_step(self, i: int) -> None:
+        self.u.copy_(self.draws[i])
+
+    def __call__(self, logits: torch.Tensor):
+        """(tokens, log probabilities) with the random numbers of the step that was set."""
+        return sample_rows(logits, self.u, *self.settings, workspace=self.ws, logprob=True)
 
 
 def _relayout(kv: LayerKV, cu: List[int], gap: int) -> LayerKV:
@@ -59,8 +116,16 @@ class DecodeState:
     max_fused_rows: Optional[int] = None
 
     def __init__(self, wts: DecoderWeights, head: ScoringHead, gate_layer: int, pf: PrefillResult,
-                 max_new_tokens: int, prune_below_gate: bool = False, graph: bool = False, fused: bool = True):
+                 max_new_tokens: int, prune_below_gate: bool = False, graph: bool = False, fused: bool = True,
+                 kv_bits: int = 16, sampler: Optional[TokenSampler] = None, release_kv: bool = False):
+        """kv_bits: 16 (the prefill's bf16 caches), 8 or 4 (quantised copies of them).  sampler: draws the tokens
+        (step i takes its random numbers i + 1; the first token's are 0), else greedy.  release_kv: with
+        quantised caches, drops pf's reference to each bf16 cache as soon as it is quantised."""
         shape = wts.shape
+        if kv_bits not in (4, 8, 16):
+            raise ValueError(f"DecodeState: kv_bits must be 16, 8 or 4 (got {kv_bits})")
+        if sampler is not None and sampler.draws.shape[0] < max_new_tokens:
+            raise ValueError("DecodeState: the sampler has fewer random numbers than max_new_tokens")
         self.wts, self.shape = wts, shape
         if self.max_fused_rows is None:
             self.max_fused_rows = 8 if shape.d_model <= 2048 else 2
@@ -70,13 +135,27 @@ class DecodeState:
         self.gate_layer = gate_layer
         L2 = shape.n_layers - gate_layer - 1
         cu_below = pf.cu_prompt if not prune_below_gate else pf.cu_kept
-        in_place = pf.decode_headroom >= max_new_tokens and pf.cache_above is not None \
+        self.kv_bits = kv_bits
+        self.sampler = sampler
+        in_place = kv_bits == 16 and pf.decode_headroom >= max_new_tokens and pf.cache_above is not None \
             and pf.cache_below is not None
         gap = pf.decode_headroom if in_place else max_new_tokens
         self.in_place = in_place
-        self.kv: List[LayerKV] = []
+        self.kv: List[Union[LayerKV, QuantKV]] = []
+        if kv_bits != 16:
+            # where the prompt rows lie in the prefill's caches (None: back to back) and in these
+            src = [c.rows_dev if pf.decode_headroom and c is not None else None for c in (pf.cache_below, pf.cache_above)]
+            dst = [CacheGap.build(cu, gap, dev) for cu in (cu_below, pf.cu_kept)]
         for l in range(shape.n_layers):
-            if in_place:
+            if kv_bits != 16:
+                g = 0 if l <= gate_layer else 1
+                cu = cu_below if g == 0 else pf.cu_kept
+                q = QuantKV.alloc(dst[g].rows, shape.n_kv_heads, kv_bits, dev)
+                kv_quantize(pf.kv[l].k, pf.kv[l].v, q, dst_rows=dst[g].rows_dev, src_rows=src[g], n_rows=cu[-1])
+                self.kv.append(q)
+                if release_kv:
+                    pf.kv[l] = None
+            elif in_place:
                 self.kv.append(pf.kv[l])
             else:                      # the prefill left no room: one copy per layer
                 self.kv.append(_relayout(pf.kv[l], cu_below if l <= gate_layer else pf.cu_kept, gap))
@@ -106,7 +185,8 @@ class DecodeState:
         self.ssmax = pf.kept_ratio is not None
         # cache slots of the Phase-2 layers, the new token's included once a step has begun
         self.slots = h2d(torch.tensor([float(x) for x in pf.n_kept], dtype=torch.float32), dev) if self.ssmax else None
-        self.att_ws = decode_attention_workspace(B, shape, max(self.cap_k), dev)
+        workspace = decode_attention_workspace if kv_bits == 16 else decode_attention_quant_workspace
+        self.att_ws = workspace(B, shape, max(self.cap_k), dev)
         self.rows_b = torch.arange(B, device=dev)
         self.steps = 0
         self.max_new_tokens = max_new_tokens
@@ -117,9 +197,14 @@ class DecodeState:
 
     @torch.no_grad()
     def step(self, tokens: torch.Tensor) -> torch.Tensor:
-        """Appends one token per sequence (tokens (B,) int64) and returns the next greedy tokens."""
+        """Appends one token per sequence (tokens (B,) int64) and returns the next tokens, greedy or sampled
+        (self.last_logprobs then holds their log probabilities, until the next step)."""
         if self.steps >= self.max_new_tokens:
             raise RuntimeError("DecodeState: more steps than max_new_tokens (the caches are full)")
+        if self.sampler is not None:
+            if self.steps + 1 >= self.sampler.draws.shape[0]:
+                raise RuntimeError("DecodeState: the sampler has no random numbers for another step")
+            self.sampler.set_step(self.steps + 1)
         if not self.use_graph or self.steps == 0:
             out = self._body(tokens)
         else:
@@ -174,10 +259,13 @@ class DecodeState:
             if not fused:
                 linear_rows(normed, lw.w_qkv, out=qkv)
             kv = self.kv[l]
-            decode_attention(qkv, rope, lw, s, kv.k, kv.v, self.seg_dev[g], self.used[g],
-                             self.cap_k[g], scale, self.att_ws, self.bias[j] if g else None,
-                             self.qscale[j] if (g and self.qscale is not None) else None,
-                             r_dec if (r_dec is not None and g) else None, out=att)
+            rows = (self.seg_dev[g], self.used[g], self.cap_k[g], scale, self.att_ws, self.bias[j] if g else None,
+                    self.qscale[j] if (g and self.qscale is not None) else None,
+                    r_dec if (r_dec is not None and g) else None)
+            if self.kv_bits == 16:
+                decode_attention(qkv, rope, lw, s, kv.k, kv.v, *rows, out=att)
+            else:
+                decode_attention_quant(qkv, rope, lw, s, kv, *rows, out=att)
             linear_rows(att.view(B, -1), lw.w_o, out=hid)
             if fused:
                 if wide:
@@ -197,4 +285,7 @@ class DecodeState:
         else:
             logits = logits_last(w, hid + res, self.rows_b)
         self.last_logits = logits
+        if self.sampler is not None:
+            tokens, self.last_logprobs = self.sampler(logits)
+            return tokens
         return argmax_rows(logits)

@@ -6,8 +6,8 @@
     out = model.generate([ids], tok, max_kept_prefill_tokens=1000, max_new_tokens=64)
 
 generate() is the gated prefill of tokengate_amd.prefill (one ragged batch: Phase 1 over every
-prompt token, gate, top-K keep, pack, Phase 2 on the kept rows) followed by greedy decode
-(tokengate_amd.decode).  The prompt ids carry the state span as the sentinel ids
+prompt token, gate, top-K keep, pack, Phase 2 on the kept rows) followed by greedy or sampled decode
+(tokengate_amd.decode), over bf16 or quantised caches.  The prompt ids carry the state span as the sentinel ids
 STATE_START_ID / STATE_END_ID, exactly as the reference's apply_chat_template produces them.
 
 Model sources (no network here): "random" / "random:<seed>" builds a seeded Qwen3-1.7B-shaped
@@ -116,6 +116,7 @@ class GenerateOutput:
     prefill_s: float
     decode_s: float
     token_ids: List[List[int]]
+    logprobs: Optional[List[List[float]]] = None    # sampled tokens' log probabilities, as token_ids
 
 
 def _sync():
@@ -151,23 +152,39 @@ class TokenGateModel:
     @torch.no_grad()
     def generate(self, ids: Union[List[int], List[List[int]]], tokenizer=None, *, max_new_tokens: int = 20,
                  max_kept_prefill_tokens: Optional[int] = None, streamer=None,
-                 prune_below_gate: bool = False) -> GenerateOutput:
+                 prune_below_gate: bool = False, kv_bits: int = 16, temperature=0.0, top_k=0, top_p=1.0, min_p=0.0,
+                 seed: int = 0) -> GenerateOutput:
         """Gated prefill + greedy decode (TokenGateModel.generate, inference.py:85-124).  ids: one
         sequence or a batch, each carrying the state sentinels.  max_kept_prefill_tokens: the K of
         the paper (None keeps every state token); a list gives one K per sequence.  tokenizer:
         provides eos_token_id and decode(); without one, no EOS stops generation and answers are
-        empty strings.  streamer: optional object with put(cpu (B, 1) int64) and end()."""
-        from tokengate_amd.decode import DecodeState
+        empty strings.  streamer: optional object with put(cpu (B, 1) int64) and end().
+        kv_bits: 16, or 8 or 4 for caches quantised after the prefill.  temperature (a number or one per
+        sequence, as top_k, top_p and min_p): 0 everywhere is greedy decode, else tokens are sampled
+        (decode.Sampling) from the random numbers that seed gives, and the result has their log
+        probabilities."""
+        from tokengate_amd.decode import DecodeState, Sampling, TokenSampler
         if max_new_tokens < 1:
             raise ValueError("max_new_tokens must be positive")
+        if kv_bits not in (4, 8, 16):
+            raise ValueError(f"kv_bits must be 16, 8 or 4 (got {kv_bits})")
         if ids and isinstance(ids[0], int):
             ids = [ids]
         split = [split_state_span(list(seq)) for seq in ids]
+        sampling = Sampling(temperature, top_k, top_p, min_p, seed)
+        sampling.check(len(split))
+        sampled = any(t > 0 for t in sampling._values("temperature", len(split)))
         _sync()
         t0 = time.perf_counter()
         pf = self.prefill(split, max_kept_prefill_tokens, prune_below_gate,
-                          decode_headroom=max_new_tokens if max_new_tokens > 1 else 0)
+                          decode_headroom=max_new_tokens if max_new_tokens > 1 and kv_bits == 16 else 0)
         first = pf.first_tokens
+        sampler, lps = None, None
+        if sampled:
+            sampler = TokenSampler(sampling, len(split), self.config.vocab, max_new_tokens, first.device)
+            sampler.set_step(0)
+            first, lp = sampler(pf.logits.float())
+            lps = [lp]
         _sync()
         prefill_s = time.perf_counter() - t0
         B = len(split)
@@ -178,7 +195,7 @@ class TokenGateModel:
         t0 = time.perf_counter()
         if max_new_tokens > 1:
             st = DecodeState(self.weights, self.gate, self.gate_layer, pf, max_new_tokens, prune_below_gate,
-                             graph=True)
+                             graph=True, kv_bits=kv_bits, sampler=sampler, release_kv=True)
             cur = first
             done = torch.zeros(B, dtype=torch.bool, device=first.device)
             for _ in range(max_new_tokens - 1):
@@ -188,6 +205,8 @@ class TokenGateModel:
                         break
                 cur = st.step(cur)
                 gen.append(cur)
+                if sampled:
+                    lps.append(st.last_logprobs.clone())
                 if streamer is not None:
                     streamer.put(cur.detach().cpu().view(B, 1))
         _sync()
@@ -207,8 +226,11 @@ class TokenGateModel:
                            if tokenizer is not None and row else "")
         kp = pf.kept_positions.cpu()
         kept_pos = [kp[pf.cu_kept[b]:pf.cu_kept[b + 1]].tolist() for b in range(B)]
+        logprobs = None
+        if sampled:
+            logprobs = [row[:len(t)] for row, t in zip(torch.stack(lps, 1).cpu().tolist(), token_ids)]
         return GenerateOutput(answers, list(pf.n_kept), [e - s for _, s, e in split], kept_pos, prefill_s, decode_s,
-                              token_ids)
+                              token_ids, logprobs)
 
 
 # ---- loading --------------------------------------------------------------------------------
