@@ -11,6 +11,9 @@
 // Layout (head-major, so that the rows that one workgroup reads are contiguous): codes (heads, rows, 16 words of
 // 4 bits x 8 or pairs of words of 8 bits x 8), element 16 e + w in nibble (byte) e of word (pair) w, so that a
 // lane's word holds values of all four groups; meta (heads, rows, 4) x (s, m).
+#include <algorithm>
+#include <type_traits>
+
 #include "tg_common.h"
 #include "../../include/tokengate_hip.h"
 
@@ -167,11 +170,28 @@ __global__ __launch_bounds__(256) void kv_dequantize_kernel(QuantCache c, RowTar
 }
 
 // ---- attention of a decode step ---------------------------------------------------------------------
+// z_j = scale (q . k_j + bias_j), out = sum_j p_j v_j / sum_j p_j, p_j = exp(z_j - max z), with k_j = s c + m by groups
+// of 32 (g): q . k_j = sum_g s_jg (q . c_j)_g + m_jg Q_g,  Q_g the sum of q over the group, and
+// out = sum_g (p_j s_jg) c_j + sum_j p_j m_jg.  Bound by the bytes of the cache (80 or 144 per key and kv head, K and
+// V each), so a workgroup takes one kv head of one sequence, up to four query heads of its group at once, and a
+// stretch of keys: chunks of chunk_tiles tiles of 64 keys, its four waves a tile each in turn.  Nothing is staged
+// through LDS: a wave's matrix instructions take the codes from the registers that the loads fill.
+//   * S = Q C^T on v_mfma_f32_16x16x32_bf16, one instruction per 16 keys and group.  A: row 4 r + i holds query head i
+//     (each head four times), so that every lane group gets all heads' sums and lane l keeps those of key l: the
+//     softmax's work is one key per lane and head, and a lane applies its own key's s and m.  B: lane (n, G) holds the
+//     words 4 G .. 4 G + 3 of key n.
+//   * At 4 bits codes become bf16 by their bits: 0x4300 | c is 128 + c (two per and-or).  The sums start from
+//     -128 Q_g (C operand); the output's part is taken off at the end.  At 8 bits they are converted.
+//   * O += P C with P = bf16(p s) per group (8 significant bits, as the bf16 cache's kernel weights; the least values'
+//     part is summed in fp32), from LDS in A's layout; B: lane (n, G) holds word n of keys 4 j + G, whose nibble
+//     (byte) e is element 16 e + n: eight keys of one element, and the element's group depends on e alone.
+//   * The running maximum moves only when a logit passes it by 2^8.  Waves merge in LDS, chunks through the
+//     workspace in the workgroup that arrives last.
 struct QuantAttnArgs {
   const bf16_t *qkv;
   int64_t qkv_rs;
   const float *rope;
-  int h, hkv;
+  int h, hkv, group, hgroups;
   const bf16_t *qw, *kw;
   float eps;
   const float *q_head_scale, *q_row_scale;
@@ -183,107 +203,436 @@ struct QuantAttnArgs {
   float scale_log2;
   bf16_t *out;
   int64_t out_rs;
+  int units, chunk_tiles, ns;    // (sequence, kv head, head set); tiles per chunk; chunks of the longest sequence
+  uint32_t *counters;            // per unit: chunks arrived; zero between launches
+  uint64_t *ml;                  // [unit][chunk][head]: running max (log2 units) and sum
+  uint64_t *po;                  // [unit][chunk][head][64]: O, pairs of fp32
 };
 
-// One workgroup per (query head, sequence); 16 lanes take a key at a time, every 16th of the sequence, each with a
-// running maximum and sum of its own; the 16 results meet in LDS.
-template <int BITS>
-__global__ __launch_bounds__(256) void decode_attn_quant_kernel(QuantAttnArgs a) {
-  const int h = blockIdx.x, b = blockIdx.y, kh = h / (a.h / a.hkv);
-  const int grp = threadIdx.x >> 4, j = threadIdx.x & 15;
-  __shared__ float qs[kHeadDim];
-  __shared__ uint32_t new_w[2][row_words<BITS>()], new_m[2][kGroups];
-  __shared__ float part[16][kHeadDim], pm[16], pl[16];
+constexpr int kWaves = 4;
+constexpr int kTile = 64;        // keys of a wave's step
+constexpr float kRescaleTau = 8.f;
+
+template <typename T>
+__device__ __forceinline__ void st_agent(T *p, T v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+template <typename T>
+__device__ __forceinline__ T ld_agent(const T *p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+
+// 0 * x = 0, whatever x is.  (The builtin: an asm statement right behind the exponential that feeds it would read the
+// register too early, as the compiler keeps the wait that such a pair needs from its own instructions only.)
+extern "C" __device__ float tg_fmul_legacy(float, float) __asm("llvm.amdgcn.fmul.legacy");
+__device__ __forceinline__ float mul_zero(float a, float b) { return tg_fmul_legacy(a, b); }
+template <int CTRL>
+__device__ __forceinline__ float dpp(float x) {
+  const int i = __builtin_bit_cast(int, x);
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(i, i, CTRL, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float wave_max(float x) {
+  x = fmaxf(x, dpp<0xB1>(x));    // quad_perm 1 0 3 2
+  x = fmaxf(x, dpp<0x4E>(x));    // quad_perm 2 3 0 1
+  x = fmaxf(x, dpp<0x141>(x));   // row_half_mirror
+  x = fmaxf(x, dpp<0x140>(x));   // row_mirror
+  return quad_swap_max(x);
+}
+
+// bf16 pairs of eight codes from four words (4 bits) or pairs of words (8) of as many rows, nibbles (bytes) e of each:
+// low half a, high half b of code pairs (a, b).
+constexpr uint32_t kNibbles = 0x000F000Fu, kBf128 = 0x43004300u;
+
+// (a's code e, b's code e) as a bf16 pair; at 4 bits from the halves' merger y = lo/hi16(a) | lo/hi16(b) << 16
+__device__ __forceinline__ uint32_t merge_half(uint32_t a, uint32_t b, int hi) {
+  return __builtin_amdgcn_perm(b, a, hi ? 0x07060302u : 0x05040100u);
+}
+__device__ __forceinline__ uint32_t nibble_pair(uint32_t y, int e) { return ((y >> (4 * (e & 3))) & kNibbles) | kBf128; }
+__device__ __forceinline__ uint32_t byte_pair(uint32_t a, uint32_t b, int byte) {
+  const float fa = (float)((a >> (8 * byte)) & 255u), fb = (float)((b >> (8 * byte)) & 255u);
+  return __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, fb), __builtin_bit_cast(uint32_t, fa), 0x07060302u);
+}
+
+template <int BITS, int HP, bool HAS_BIAS>
+__global__ __launch_bounds__(64 * kWaves) void decode_attn_quant_kernel(QuantAttnArgs a) {
+  constexpr int kRow = 16 * BITS;                 // bytes of a row's codes
+  constexpr int KW = BITS;                        // words of a row that one lane takes for S: 16 B or 32 B
+  constexpr int VW = BITS / 4;                    // and for O
+  const int tid = threadIdx.x, wave = wave_id(), lane = tid & 63, n16 = lane & 15, G = lane >> 4;
+  const int unit = blockIdx.x % a.units, chunk = blockIdx.x / a.units;
+  const int kh = unit % a.hkv, hg = (unit / a.hkv) % a.hgroups, b = unit / (a.hkv * a.hgroups);
+  const int h0 = kh * a.group + hg * HP, nh = min(HP, a.group - hg * HP);   // heads h0 .. h0 + nh - 1
+
+  __shared__ __attribute__((aligned(16))) bf16_t qs[HP][kHeadDim];
+  __shared__ __attribute__((aligned(16))) uint32_t new_w[2][row_words<BITS>()], new_m[2][kGroups];
+  __shared__ __attribute__((aligned(16))) bf16_t ps[kWaves][kGroups][HP][kTile];
+  __shared__ float part_o[kWaves][HP][kHeadDim], part_ml[kWaves][HP][2];
+
   const int64_t start = a.kv_start[b];
-  int sk = min(a.kv_used[b], a.max_k);
+  int sk = max(0, min(a.kv_used[b], a.max_k));
   if (start < 0 || start + sk > a.c.rows) sk = 0;
-  if (grp < 3) {          // this head's query, and the new key and value
-    const int head = grp == 0 ? h : grp == 1 ? a.h + kh : a.h + a.hkv + kh;
-    float x[8], y[8], wf[8];
-    unpack8(ld16(a.qkv + b * a.qkv_rs + (int64_t)head * kHeadDim + 8 * j), x);
-    if (grp < 2) {
-      unpack8(ld16((grp == 0 ? a.qw : a.kw) + 8 * j), wf);
-      const float hs = grp == 0 ? (float)(__bf16)((a.q_head_scale ? a.q_head_scale[h] : 1.f) *
-                                                  (a.q_row_scale ? a.q_row_scale[b] : 1.f))
-                                : 1.f;
-      norm_rope8(x, wf, a.eps, reinterpret_cast<const float(*)[2]>(a.rope) + b * (kHeadDim / 2) + 8 * (j & 7), j, hs, y);
+  const int n_tiles = (sk + kTile - 1) / kTile, n_parts = max(1, (n_tiles + a.chunk_tiles - 1) / a.chunk_tiles);
+  if (chunk >= n_parts) return;
+  const int t_lo = chunk * a.chunk_tiles, t_hi = min(n_tiles, t_lo + a.chunk_tiles);
+  const bool has_new = t_hi == n_tiles && n_tiles > 0;
+
+  // ---- loads of a tile: rows past sk read as zero (codes, s and m) ----
+  const int64_t row0 = kh * a.c.head_rows + start;
+  const brsrc_t krs = make_rsrc(a.c.k + row0 * row_words<BITS>(), (uint32_t)sk * kRow);
+  const brsrc_t vrs = make_rsrc(a.c.v + row0 * row_words<BITS>(), (uint32_t)sk * kRow);
+  const brsrc_t kmrs = make_rsrc(a.c.km + row0 * kGroups, (uint32_t)sk * 16);
+  const brsrc_t vmrs = make_rsrc(a.c.vm + row0 * kGroups, (uint32_t)sk * 16);
+  uint32_t kx[4][KW], vx[2][8][VW];
+  u32x4 kmeta, vmeta;
+  float bias[HP];
+  auto load_k = [&](int t) {
+    const uint32_t at = (uint32_t)t * (kTile * kRow) + n16 * kRow + G * (kRow / 4);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = (float)(__bf16)y[i];
-    }
-    if (grp == 0) {
+    for (int kb = 0; kb < 4; ++kb)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) qs[8 * j + i] = x[i];
-    } else {
-      uint32_t w[BITS / 4], meta;
-      quant_row<BITS>(x, j, w, meta);
-      const int64_t row = kh * a.c.head_rows + start + sk - 1;
-      const bool write = sk > 0 && h % (a.h / a.hkv) == 0;
-      uint32_t *codes = grp == 1 ? a.c.k : a.c.v, *metas = grp == 1 ? a.c.km : a.c.vm;
+      for (int i = 0; i < KW / 4; ++i) {
+        const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(krs, at + kb * 16 * kRow + 16 * i, 0, 0);
 #pragma unroll
-      for (int i = 0; i < BITS / 4; ++i) {
-        const int at = word_of(j) * (BITS / 4) + i;
-        new_w[grp - 1][at] = w[i];
-        if (write) codes[row * row_words<BITS>() + at] = w[i];
+        for (int e = 0; e < 4; ++e) kx[kb][4 * i + e] = v[e];
       }
-      if ((j & 3) == 0) {
-        new_m[grp - 1][j >> 2] = meta;
-        if (write) metas[row * kGroups + (j >> 2)] = meta;
+    const uint32_t key = (uint32_t)t * kTile + lane;
+    kmeta = __builtin_amdgcn_raw_buffer_load_b128(kmrs, key * 16, 0, 0);
+    if constexpr (HAS_BIAS) {
+#pragma unroll
+      for (int i = 0; i < HP; ++i) {
+        const float *p = a.bias + (int64_t)b * a.bias_bs + (int64_t)(h0 + min(i, nh - 1)) * a.bias_hs;
+        bias[i] = u32_as_f32(__builtin_amdgcn_raw_buffer_load_b32(make_rsrc(p, (uint32_t)sk * 4), key * 4, 0, 0));
       }
-    }
-  }
-  __syncthreads();
-  float q[8], acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, m = -INFINITY, l = 0.f;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) q[e] = qs[16 * e + j];
-  auto load = [&](const uint32_t *w, const uint32_t *meta, float (&x)[8]) {   // elements 16 e + j of a row
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const uint32_t c = (w[j * (BITS / 4) + e * BITS / 32] >> (BITS * e % 32)) & ((1u << BITS) - 1u);
-      x[e] = fmaf((float)c, u32_as_f32(meta[e >> 1] << 16), u32_as_f32(meta[e >> 1] & 0xffff0000u));
     }
   };
-  for (int k = grp; k < sk; k += 16) {
-    const int64_t row = kh * a.c.head_rows + start + k;
-    const bool is_new = k == sk - 1;
-    float x[8], z = 0.f;
-    load(is_new ? new_w[0] : a.c.k + row * row_words<BITS>(), is_new ? new_m[0] : a.c.km + row * kGroups, x);
+  auto load_v = [&](int t) {
+    const uint32_t at = (uint32_t)t * (kTile * kRow) + G * kRow + n16 * (4 * VW);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) z = fmaf(q[e], x[e], z);
-    z += __shfl_xor(z, 1);
-    z += __shfl_xor(z, 2);
-    z += __shfl_xor(z, 4);
-    z += __shfl_xor(z, 8);
-    const float bias = a.bias ? a.bias[b * a.bias_bs + h * a.bias_hs + k] : 0.f;
-    if (bias == -INFINITY) continue;             // hidden, whatever the row holds
-    z = (z + bias) * a.scale_log2;
-    asm("" : "+v"(z));   // rounded: contracted into z - m below, a bias near the lowest float leaves the rounding's rest
-    load(is_new ? new_w[1] : a.c.v + row * row_words<BITS>(), is_new ? new_m[1] : a.c.vm + row * kGroups, x);
-    const float mn = fmaxf(m, z), keep = m == -INFINITY ? 0.f : fast_exp2(m - mn);
-    const float p = z == -INFINITY ? 0.f : fast_exp2(z - mn);   // (NaN where z is)
-    l = l * keep + p;
+    for (int st = 0; st < 2; ++st)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) acc[e] = acc[e] * keep + (p == 0.f ? 0.f : p * x[e]);
-    m = mn;
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t p = at + (32 * st + 4 * j) * kRow;
+        if constexpr (BITS == 4) {
+          vx[st][j][0] = __builtin_amdgcn_raw_buffer_load_b32(vrs, p, 0, 0);
+        } else {
+          const u32x2 v = __builtin_amdgcn_raw_buffer_load_b64(vrs, p, 0, 0);
+          vx[st][j][0] = v[0];
+          vx[st][j][1] = v[1];
+        }
+      }
+    vmeta = __builtin_amdgcn_raw_buffer_load_b128(vmrs, ((uint32_t)t * kTile + lane) * 16, 0, 0);
+  };
+  int t = t_lo + wave;
+  const bool works = t < t_hi;
+  if (works) {
+    load_k(t);
+    load_v(t);
   }
+
+  // ---- the query heads' rows, and the new key and value ----
+  if (wave == 0) {                               // 16 lanes a head
+    if (G < HP) {
+      const int head = h0 + min(G, nh - 1);
+      float x[8], wf[8], y[8];
+      unpack8(ld16(a.qkv + b * a.qkv_rs + (int64_t)head * kHeadDim + 8 * n16), x);
+      unpack8(ld16(a.qw + 8 * n16), wf);
+      const float hs = (float)(__bf16)((a.q_head_scale ? a.q_head_scale[head] : 1.f) * (a.q_row_scale ? a.q_row_scale[b] : 1.f));
+      norm_rope8(x, wf, a.eps, reinterpret_cast<const float(*)[2]>(a.rope) + b * (kHeadDim / 2) + 8 * (n16 & 7), n16, hs, y);
+      st16(&qs[G][8 * n16], pack8(y));
+    }
+  } else if (wave == 1 && has_new && G < 2) {    // lanes 0..15 the key, 16..31 the value
+    const int head = G == 0 ? a.h + kh : a.h + a.hkv + kh;
+    float x[8], wf[8], y[8];
+    const u32x4 raw = ld16(a.qkv + b * a.qkv_rs + (int64_t)head * kHeadDim + 8 * n16);
+    unpack8(raw, x);
+    unpack8(ld16(a.kw + 8 * n16), wf);
+    norm_rope8(x, wf, a.eps, reinterpret_cast<const float(*)[2]>(a.rope) + b * (kHeadDim / 2) + 8 * (n16 & 7), n16, 1.f, y);
+    const u32x4 turned = pack8(y);
+    unpack8(G == 0 ? turned : raw, x);
+    uint32_t w[BITS / 4], meta;
+    quant_row<BITS>(x, n16, w, meta);
+    const int64_t row = row0 + sk - 1;
+    uint32_t *codes = G == 0 ? a.c.k : a.c.v, *metas = G == 0 ? a.c.km : a.c.vm;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) part[grp][16 * e + j] = acc[e];
-  if (j == 0) {
-    pm[grp] = m;
-    pl[grp] = l;
+    for (int i = 0; i < BITS / 4; ++i) {
+      const int at = word_of(n16) * (BITS / 4) + i;
+      new_w[G][at] = w[i];
+      if (hg == 0) codes[row * row_words<BITS>() + at] = w[i];
+    }
+    if ((n16 & 3) == 0) {
+      new_m[G][n16 >> 2] = meta;
+      if (hg == 0) metas[row * kGroups + (n16 >> 2)] = meta;
+    }
   }
   __syncthreads();
-  if (threadIdx.x < kHeadDim) {
-    float mm = -INFINITY, sum = 0.f, o = 0.f;
-    for (int g = 0; g < 16; ++g) mm = fmaxf(mm, pm[g]);
-    for (int g = 0; g < 16; ++g) {
-      const float w = pm[g] == -INFINITY ? 0.f : fast_exp2(pm[g] - mm);
-      sum += w * pl[g];
-      o += w == 0.f ? 0.f : w * part[g][threadIdx.x];
-    }
-    // (a row whose scores are NaN: pl is NaN, and so is the output)
-    const float y = sum == 0.f ? 0.f : o / sum;
-    a.out[b * a.out_rs + (int64_t)h * kHeadDim + threadIdx.x] = __builtin_bit_cast(uint16_t, (__bf16)y);
+
+  // ---- Q in A's layout, and its sums by group ----
+  bf16x8 qf[kGroups];
+  float qsum[kGroups][HP];
+#pragma unroll
+  for (int g = 0; g < kGroups; ++g) {
+    const bf16_t *p = &qs[n16 & (HP - 1)][32 * g + 4 * G];
+    const u32x2 lo = *reinterpret_cast<const u32x2 *>(p), hi = *reinterpret_cast<const u32x2 *>(p + 16);
+    const u32x4 q = {lo[0], lo[1], hi[0], hi[1]};
+    qf[g] = __builtin_bit_cast(bf16x8, q);
+    float f[8], s = 0.f;
+    unpack8(q, f);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s += f[i];
+    s = quad_sum(s);
+#pragma unroll
+    for (int i = 0; i < HP; ++i) qsum[g][i] = u32_as_f32(__builtin_amdgcn_readlane(__builtin_bit_cast(uint32_t, s), i));
   }
+
+  f32x4 oacc[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) oacc[e] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float mrun[HP], lsum[HP], rest[HP][kGroups];   // rest: what the output's sums lack, by lane
+#pragma unroll
+  for (int i = 0; i < HP; ++i) {
+    mrun[i] = -INFINITY;
+    lsum[i] = 0.f;
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) rest[i][g] = 0.f;
+  }
+  // position of this lane's key in A's order of keys: lane (m, G) takes keys 4 j + G, j = 0 .. 7, of 32
+  bf16_t *const pw = &ps[wave][0][0][32 * (lane >> 5) + 8 * (lane & 3) + ((lane & 31) >> 2)];
+
+  for (; t < t_hi; t += kWaves) {
+    if (t == n_tiles - 1) {                      // the new row, in place of what the cache held there
+      const int key = (sk - 1) & 63;
+#pragma unroll
+      for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+        for (int i = 0; i < KW; ++i) {
+          const uint32_t w = new_w[0][KW * G + i];
+          kx[kb][i] = key == 16 * kb + n16 ? w : kx[kb][i];
+        }
+#pragma unroll
+      for (int st = 0; st < 2; ++st)
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+          for (int i = 0; i < VW; ++i) {
+            const uint32_t w = new_w[1][VW * n16 + i];
+            vx[st][j][i] = key == 32 * st + 4 * j + G ? w : vx[st][j][i];
+          }
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g) {
+        const uint32_t k1 = new_m[0][g], v1 = new_m[1][g];
+        kmeta[g] = key == lane ? k1 : kmeta[g];
+        vmeta[g] = key == lane ? v1 : vmeta[g];
+      }
+    }
+    // ---- logits of key `lane` ----
+    float z[HP];
+#pragma unroll
+    for (int i = 0; i < HP; ++i) z[i] = HAS_BIAS ? bias[i] : 0.f;
+    uint32_t ky[4][4];                           // 4 bits: merged halves (words 0 1 lo, 0 1 hi, 2 3 lo, 2 3 hi)
+    if constexpr (BITS == 4) {
+#pragma unroll
+      for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+          ky[kb][2 * p] = merge_half(kx[kb][2 * p], kx[kb][2 * p + 1], 0);
+          ky[kb][2 * p + 1] = merge_half(kx[kb][2 * p], kx[kb][2 * p + 1], 1);
+        }
+    }
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+      f32x4 init = {0.f, 0.f, 0.f, 0.f};
+      if constexpr (BITS == 4) {
+#pragma unroll
+        for (int i = 0; i < HP; ++i) init[i] = -128.f * qsum[g][i];
+      }
+      f32x4 s[4];
+#pragma unroll
+      for (int kb = 0; kb < 4; ++kb) {
+        u32x4 c;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {            // codes e = 2 g (w < 2) and 2 g + 1 of words 0 1 or 2 3
+          const int e = 2 * g + (w >> 1), p = w & 1;
+          if constexpr (BITS == 4)
+            c[w] = nibble_pair(ky[kb][2 * p + (e >> 2)], e);
+          else
+            c[w] = byte_pair(kx[kb][4 * p + (e >> 2)], kx[kb][4 * p + 2 + (e >> 2)], e & 3);
+        }
+        s[kb] = mfma16(qf[g], __builtin_bit_cast(bf16x8, c), init);
+      }
+      const float step = u32_as_f32(kmeta[g] << 16), least = u32_as_f32(kmeta[g] & 0xffff0000u);
+#pragma unroll
+      for (int i = 0; i < HP; ++i) {
+        const float s01 = G & 1 ? s[1][i] : s[0][i], s23 = G & 1 ? s[3][i] : s[2][i];
+        z[i] = fmaf(G & 2 ? s23 : s01, step, fmaf(qsum[g][i], least, z[i]));
+      }
+    }
+    const bool there = t * kTile + lane < sk;
+    bool up = false;
+#pragma unroll
+    for (int i = 0; i < HP; ++i) {
+      z[i] *= a.scale_log2;
+      asm("" : "+v"(z[i]));   // rounded: contracted into z - m below, a bias near the lowest float leaves the rounding's rest
+      if (!there) z[i] = -INFINITY;
+      if constexpr (HAS_BIAS) z[i] = bias[i] == -INFINITY ? -INFINITY : z[i];   // hidden, whatever the row holds
+      up |= z[i] > mrun[i] + kRescaleTau;
+    }
+    if (t + kWaves < t_hi) load_k(t + kWaves);
+    if (__builtin_amdgcn_ballot_w64(up)) {
+#pragma unroll
+      for (int i = 0; i < HP; ++i) {
+        const float m = fmaxf(mrun[i], wave_max(z[i])), f = mrun[i] == -INFINITY ? 0.f : fast_exp2(mrun[i] - m);
+        mrun[i] = m;
+        lsum[i] *= f;
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) rest[i][g] *= f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) oacc[e][i] *= f;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < HP; ++i) {
+      const float p = fast_exp2(z[i] - (mrun[i] == -INFINITY ? 0.f : mrun[i]));
+      lsum[i] += p;
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g) {
+        const float step = u32_as_f32(vmeta[g] << 16), least = u32_as_f32(vmeta[g] & 0xffff0000u);
+        const __bf16 w = (__bf16)mul_zero(p, step);   // (a weight of 0 is 0, whatever the row holds)
+        pw[(g * HP + i) * kTile] = __builtin_bit_cast(uint16_t, w);
+        rest[i][g] += mul_zero(p, least);
+        if constexpr (BITS == 4) rest[i][g] = fmaf(-128.f, (float)w, rest[i][g]);
+      }
+    }
+    // ---- O += P C ----
+#pragma unroll
+    for (int st = 0; st < 2; ++st) {
+      uint32_t vy[4][2];
+      if constexpr (BITS == 4) {
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          vy[w][0] = merge_half(vx[st][2 * w][0], vx[st][2 * w + 1][0], 0);
+          vy[w][1] = merge_half(vx[st][2 * w][0], vx[st][2 * w + 1][0], 1);
+        }
+      }
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g) {
+        const bf16x8 pf = *reinterpret_cast<const bf16x8 *>(&ps[wave][g][n16 & (HP - 1)][32 * st + 8 * G]);
+#pragma unroll
+        for (int e = 2 * g; e < 2 * g + 2; ++e) {
+          u32x4 c;
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            if constexpr (BITS == 4)
+              c[w] = nibble_pair(vy[w][e >> 2], e);
+            else
+              c[w] = byte_pair(vx[st][2 * w][e >> 2], vx[st][2 * w + 1][e >> 2], e & 3);
+          }
+          oacc[e] = mfma16(pf, __builtin_bit_cast(bf16x8, c), oacc[e]);
+        }
+      }
+    }
+    if (t + kWaves < t_hi) load_v(t + kWaves);
+  }
+
+  // ---- the waves' results meet in LDS ----
+#pragma unroll
+  for (int i = 0; i < HP; ++i) {
+    const float l = wave_sum(lsum[i]);
+    if (lane == 0) {
+      part_ml[wave][i][0] = mrun[i];
+      part_ml[wave][i][1] = l;
+    }
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+      const float r = wave_sum(rest[i][g]);
+      if (G == g) {                              // lane group g writes group g's elements
+        part_o[wave][i][32 * g + n16] = oacc[2 * g][i] + r;
+        part_o[wave][i][32 * g + 16 + n16] = oacc[2 * g + 1][i] + r;
+      }
+    }
+  }
+  __syncthreads();
+  constexpr int kOuts = HP * kHeadDim / 2;       // pairs of output elements
+  bf16_t *const orow = a.out + b * a.out_rs + (int64_t)h0 * kHeadDim;
+  auto put = [&](int item, float o0, float o1, float l) {   // a row that saw no key: 0
+    const float f = l == 0.f ? 0.f : 1.f / l;
+    if (item / 64 < nh)
+      *reinterpret_cast<uint32_t *>(orow + 2 * item) = l == 0.f ? 0u : pack_bf16x2(o0 * f, o1 * f);
+  };
+  for (int item = tid; item < kOuts; item += 64 * kWaves) {
+    const int i = item / 64, d = 2 * (item % 64);
+    float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) m = fmaxf(m, part_ml[w][i][0]);
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const float mw = part_ml[w][i][0], f = mw == -INFINITY ? (part_ml[w][i][1] == 0.f ? 0.f : 1.f) : fast_exp2(mw - m);
+      l += f * part_ml[w][i][1];
+      o0 += mul_zero(f, part_o[w][i][d]);
+      o1 += mul_zero(f, part_o[w][i][d + 1]);
+    }
+    if (n_parts == 1) {
+      put(item, o0, o1, l);
+    } else {
+      // (agent-scope accesses write through and read past the XCD's L2, where a release would write all of it back)
+      const int64_t at = ((int64_t)unit * a.ns + chunk) * HP + i;
+      const float2 o = {o0, o1}, mlv = {m, l};
+      st_agent(a.po + at * 64 + item % 64, __builtin_bit_cast(uint64_t, o));
+      if (d == 0) st_agent(a.ml + at, __builtin_bit_cast(uint64_t, mlv));
+    }
+  }
+  if (n_parts == 1) return;
+  __shared__ int last_s;
+  wait_all_mem();                                // this wave's stores are done
+  __syncthreads();
+  if (tid == 0)
+    last_s = __hip_atomic_fetch_add(a.counters + unit, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)n_parts - 1u;
+  __syncthreads();
+  if (!last_s) return;
+  if (tid == 0) st_agent(a.counters + unit, 0u);
+  // ---- the last workgroup of the unit merges its chunks, in their order ----
+  for (int item = tid; item < kOuts; item += 64 * kWaves) {
+    const int i = item / 64;
+    float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
+    constexpr int kAhead = 8;
+    for (int c0 = 0; c0 < n_parts; c0 += kAhead) {
+      uint64_t ml[kAhead], o[kAhead];
+#pragma unroll
+      for (int r = 0; r < kAhead; ++r) {         // (every load is made, past the end the last's)
+        const int64_t at = ((int64_t)unit * a.ns + min(c0 + r, n_parts - 1)) * HP + i;
+        ml[r] = ld_agent(a.ml + at);
+        o[r] = ld_agent(a.po + at * 64 + item % 64);
+      }
+#pragma unroll
+      for (int r = 0; r < kAhead; ++r) {
+        const float2 mc = __builtin_bit_cast(float2, ml[r]), oc = __builtin_bit_cast(float2, o[r]);
+        if (c0 + r >= n_parts || mc.y == 0.f) continue;   // saw no key
+        const float mn = fmaxf(m, mc.x), f0 = m == -INFINITY ? 0.f : fast_exp2(m - mn);
+        const float f1 = mc.x == -INFINITY ? 1.f : fast_exp2(mc.x - mn);
+        l = l * f0 + mc.y * f1;
+        o0 = o0 * f0 + oc.x * f1;
+        o1 = o1 * f0 + oc.y * f1;
+        m = mn;
+      }
+    }
+    put(item, o0, o1, l);
+  }
+}
+
+// Chunks: as many as make two workgroups per CU for the longest sequence, each of whole rounds of its waves.
+struct QuantPlan {
+  int hp, hgroups, units, chunk_tiles, ns;
+};
+QuantPlan plan_quant(int num_seqs, int num_heads, int num_heads_k, int max_k) {
+  QuantPlan p;
+  const int group = num_heads / num_heads_k;
+  p.hp = group >= 3 ? 4 : group;
+  p.hgroups = (group + p.hp - 1) / p.hp;
+  p.units = num_seqs * num_heads_k * p.hgroups;
+  const int tiles = std::max(1, (max_k + kTile - 1) / kTile), want = std::max(1, 2 * device_cus() / p.units);
+  p.chunk_tiles = ((tiles + want - 1) / want + kWaves - 1) / kWaves * kWaves;
+  p.ns = (tiles + p.chunk_tiles - 1) / p.chunk_tiles;
+  return p;
+}
+// The counters' region is the same for every launch, so that no launch writes partial results where another counts.
+int64_t quant_counter_bytes() { return ((int64_t)device_cus() * 2 * 4 + 255) / 256 * 256; }
+int64_t quant_bytes(int64_t parts, int hp) {   // counters, (max, sum), O
+  return quant_counter_bytes() + (parts * hp * 8 + 255) / 256 * 256 + parts * hp * kHeadDim * 4;
 }
 
 int check_cache(const char *what, int32_t num_heads_k, int32_t head_dim, int32_t bits, const void *k_codes,
@@ -365,9 +714,14 @@ extern "C" int tg_kv_dequantize(const void *k_codes, const void *k_meta, const v
   return 0;
 }
 
+// (enough for fewer sequences and keys too: those may be cut into more chunks, never into more parts in all than two
+// per CU or one per round of four tiles)
 extern "C" int64_t tg_decode_attention_quant_workspace_size(int32_t num_seqs, int32_t num_heads, int32_t num_heads_k,
                                                             int32_t max_seqlen_k) {
-  return 0;
+  if (num_seqs <= 0 || num_heads <= 0 || num_heads_k <= 0 || num_heads % num_heads_k != 0 || max_seqlen_k <= 0) return 0;
+  const QuantPlan p = plan_quant(num_seqs, num_heads, num_heads_k, max_seqlen_k);
+  const int64_t rounds = ((int64_t)max_seqlen_k + kWaves * kTile - 1) / (kWaves * kTile);
+  return rounds == 1 ? 0 : quant_bytes(std::min<int64_t>(2 * device_cus(), p.units * rounds), p.hp);
 }
 
 extern "C" int tg_decode_attention_quant(const void *qkv, int64_t qkv_row_stride, const float *rope, int32_t num_seqs,
@@ -388,7 +742,8 @@ extern "C" int tg_decode_attention_quant(const void *qkv, int64_t qkv_row_stride
   TG_CHECK(qkv && rope && q_norm_weight && k_norm_weight && kv_start && kv_used && out, "%s: null pointer", what);
   TG_CHECK(num_heads > 0 && num_heads <= 256 && num_heads % num_heads_k == 0,
            "%s: heads must be in 1..256 and a multiple of the KV heads", what);
-  TG_CHECK(num_seqs >= 0 && num_seqs < 65536 && max_seqlen_k >= 0, "%s: bad sequence count or length", what);
+  TG_CHECK(num_seqs >= 0 && (int64_t)num_seqs * num_heads < (1 << 24) && max_seqlen_k >= 0,
+           "%s: bad sequence count or length", what);
   TG_CHECK(qkv_row_stride % 8 == 0 && out_row_stride % 8 == 0 &&
                qkv_row_stride >= (int64_t)(num_heads + 2 * num_heads_k) * kHeadDim &&
                out_row_stride >= (int64_t)num_heads * kHeadDim,
@@ -397,8 +752,10 @@ extern "C" int tg_decode_attention_quant(const void *qkv, int64_t qkv_row_stride
                aligned16(workspace),
            "%s: pointers must be 16-byte aligned", what);
   TG_CHECK(softmax_scale > 0.f, "%s: softmax_scale must be positive", what);
+  TG_CHECK(max_seqlen_k < (1 << 24), "%s: max_seqlen_k must be less than 2^24", what);   // spans of under 4 GiB
   TG_CHECK(!bias_raw || (bias_seq_stride >= 0 && bias_head_stride >= 0), "%s: negative bias stride", what);
   if (num_seqs == 0) return 0;
+  const QuantPlan p = plan_quant(num_seqs, num_heads, num_heads_k, max_seqlen_k);
   a.qkv = static_cast<const bf16_t *>(qkv);
   a.qkv_rs = qkv_row_stride;
   a.rope = rope;
@@ -418,9 +775,36 @@ extern "C" int tg_decode_attention_quant(const void *qkv, int64_t qkv_row_stride
   a.scale_log2 = softmax_scale * 1.4426950408889634f;
   a.out = static_cast<bf16_t *>(out);
   a.out_rs = out_row_stride;
-  const dim3 grid((unsigned)num_heads, (unsigned)num_seqs), block(256);
-  if (bits == 4) hipLaunchKernelGGL(decode_attn_quant_kernel<4>, grid, block, 0, stream, a);
-  else hipLaunchKernelGGL(decode_attn_quant_kernel<8>, grid, block, 0, stream, a);
+  a.group = num_heads / num_heads_k;
+  a.hgroups = p.hgroups;
+  a.units = p.units;
+  a.chunk_tiles = p.chunk_tiles;
+  a.ns = p.ns;
+  const int64_t parts = (int64_t)p.units * p.ns;
+  if (p.ns > 1) {
+    TG_CHECK(workspace != nullptr && workspace_bytes >= quant_bytes(parts, p.hp),
+             "%s: needs a workspace of %lld bytes (got %lld)", what, (long long)quant_bytes(parts, p.hp),
+             (long long)workspace_bytes);
+    char *ws = static_cast<char *>(workspace);
+    a.counters = reinterpret_cast<uint32_t *>(ws);
+    a.ml = reinterpret_cast<uint64_t *>(ws + quant_counter_bytes());
+    a.po = reinterpret_cast<uint64_t *>(ws + quant_bytes(parts, p.hp) - parts * p.hp * kHeadDim * 4);
+  }
+  const dim3 grid((unsigned)parts), block(64 * kWaves);
+  auto launch = [&](auto bits_c, auto hp_c) {
+    constexpr int BITS = decltype(bits_c)::value, HP = decltype(hp_c)::value;
+    if (bias_raw)
+      hipLaunchKernelGGL((decode_attn_quant_kernel<BITS, HP, true>), grid, block, 0, stream, a);
+    else
+      hipLaunchKernelGGL((decode_attn_quant_kernel<BITS, HP, false>), grid, block, 0, stream, a);
+  };
+  auto with_heads = [&](auto bits_c) {
+    if (p.hp == 1) launch(bits_c, std::integral_constant<int, 1>());
+    else if (p.hp == 2) launch(bits_c, std::integral_constant<int, 2>());
+    else launch(bits_c, std::integral_constant<int, 4>());
+  };
+  if (bits == 4) with_heads(std::integral_constant<int, 4>());
+  else with_heads(std::integral_constant<int, 8>());
   TG_HIP_CHECK(hipGetLastError());
   return 0;
 }
