@@ -70,9 +70,10 @@ __device__ __forceinline__ int word_of(int j) { return 8 * (j & 1) + (j >> 1); }
 
 // Quantises a row held by 16 lanes, lane j its elements 8 j .. 8 j + 7: word (pair) word_of(j) of its codes, and the
 // (s, m) pair of its group j / 4.  The quotient is the correctly rounded one of a division: q = d (1/s) and one
-// correction by its remainder.
+// correction by its remainder.  held: the values that the codes stand for.
 template <int BITS>
-__device__ __forceinline__ void quant_row(const float (&x)[8], int j, uint32_t (&w)[BITS / 4], uint32_t &meta) {
+__device__ __forceinline__ void quant_row(const float (&x)[8], int j, uint32_t (&w)[BITS / 4], uint32_t &meta,
+                                          float (&held)[8]) {
   float mn = min3_nan(min3_nan(x[0], x[1], x[2]), min3_nan(x[3], x[4], x[5]), min3_nan(x[6], x[7], x[7]));
   float mx = max3_nan(max3_nan(x[0], x[1], x[2]), max3_nan(x[3], x[4], x[5]), max3_nan(x[6], x[7], x[7]));
 #pragma unroll
@@ -94,6 +95,7 @@ __device__ __forceinline__ void quant_row(const float (&x)[8], int j, uint32_t (
     q = fmaf(fmaf(-q, s, d), inv, q);
     q = fminf(fmaxf(rintf(q), 0.f), top_code<BITS>());   // (a NaN gives 0)
     c[i] = (uint32_t)q;
+    held[i] = fine ? fmaf(q, s, mn) : NAN;
   }
 #pragma unroll
   for (int k = 0; k < BITS / 4; ++k) {
@@ -137,7 +139,8 @@ __global__ __launch_bounds__(256) void kv_quantize_kernel(RowSource a, QuantCach
   float x[8];
   unpack8(ld16(p + 8 * j), x);
   uint32_t w[BITS / 4], meta;
-  quant_row<BITS>(x, j, w, meta);
+  float held[8];
+  quant_row<BITS>(x, j, w, meta, held);
   const int64_t row = head * c.head_rows + dst;
   uint32_t *out = (is_v ? c.v : c.k) + row * row_words<BITS>() + word_of(j) * (BITS / 4);
 #pragma unroll
@@ -185,6 +188,7 @@ __global__ __launch_bounds__(256) void kv_dequantize_kernel(QuantCache c, RowTar
 //   * O += P C with P = bf16(p s) per group (8 significant bits, as the bf16 cache's kernel weights; the least values'
 //     part is summed in fp32), from LDS in A's layout; B: lane (n, G) holds word n of keys 4 j + G, whose nibble
 //     (byte) e is element 16 e + n: eight keys of one element, and the element's group depends on e alone.
+//   * The new key is not in the tiles: it is a part of its own beside the waves', from registers.
 //   * The running maximum moves only when a logit passes it by 2^8.  Waves merge in LDS, chunks through the
 //     workspace in the workgroup that arrives last.
 struct QuantAttnArgs {
@@ -211,6 +215,9 @@ struct QuantAttnArgs {
 
 constexpr int kWaves = 4;
 constexpr int kTile = 64;        // keys of a wave's step
+// Tiles that a wave holds or has on their way, and workgroups per CU, by the registers
+constexpr int depth(int bits, int hp) { return bits == 4 && hp <= 2 ? 2 : 1; }
+__host__ __device__ constexpr int per_cu(int bits, int hp) { return depth(bits, hp) == 2 || hp == 4 ? 2 : 3; }
 constexpr float kRescaleTau = 8.f;
 
 template <typename T>
@@ -234,6 +241,19 @@ __device__ __forceinline__ float wave_max(float x) {
   x = fmaxf(x, dpp<0x140>(x));   // row_mirror
   return quad_swap_max(x);
 }
+__device__ __forceinline__ float wave_add(float x) {
+  x += dpp<0xB1>(x);
+  x += dpp<0x4E>(x);
+  x += dpp<0x141>(x);
+  x += dpp<0x140>(x);
+  const uint32_t u = __builtin_bit_cast(uint32_t, x);
+  const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  const uint32_t a0 = a[0], a1 = a[1];
+  const uint32_t v = __builtin_bit_cast(uint32_t, u32_as_f32(a0) + u32_as_f32(a1));
+  const auto c = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  const uint32_t c0 = c[0], c1 = c[1];
+  return u32_as_f32(c0) + u32_as_f32(c1);
+}
 
 // bf16 pairs of eight codes from four words (4 bits) or pairs of words (8) of as many rows, nibbles (bytes) e of each:
 // low half a, high half b of code pairs (a, b).
@@ -243,45 +263,54 @@ constexpr uint32_t kNibbles = 0x000F000Fu, kBf128 = 0x43004300u;
 __device__ __forceinline__ uint32_t merge_half(uint32_t a, uint32_t b, int hi) {
   return __builtin_amdgcn_perm(b, a, hi ? 0x07060302u : 0x05040100u);
 }
-__device__ __forceinline__ uint32_t nibble_pair(uint32_t y, int e) { return ((y >> (4 * (e & 3))) & kNibbles) | kBf128; }
+// (mask and bias in registers: as literals they cost an instruction each)
+__device__ __forceinline__ uint32_t nibble_pair(uint32_t y, int e, uint32_t nibbles, uint32_t bf128) {
+  return ((y >> (4 * (e & 3))) & nibbles) | bf128;
+}
 __device__ __forceinline__ uint32_t byte_pair(uint32_t a, uint32_t b, int byte) {
   const float fa = (float)((a >> (8 * byte)) & 255u), fb = (float)((b >> (8 * byte)) & 255u);
   return __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, fb), __builtin_bit_cast(uint32_t, fa), 0x07060302u);
 }
 
 template <int BITS, int HP, bool HAS_BIAS>
-__global__ __launch_bounds__(64 * kWaves) void decode_attn_quant_kernel(QuantAttnArgs a) {
+__global__ __launch_bounds__(64 * kWaves, per_cu(BITS, HP)) void decode_attn_quant_kernel(QuantAttnArgs a) {
   constexpr int kRow = 16 * BITS;                 // bytes of a row's codes
   constexpr int KW = BITS;                        // words of a row that one lane takes for S: 16 B or 32 B
   constexpr int VW = BITS / 4;                    // and for O
+  constexpr int kDepth = depth(BITS, HP);         // tiles in registers
   const int tid = threadIdx.x, wave = wave_id(), lane = tid & 63, n16 = lane & 15, G = lane >> 4;
   const int unit = blockIdx.x % a.units, chunk = blockIdx.x / a.units;
   const int kh = unit % a.hkv, hg = (unit / a.hkv) % a.hgroups, b = unit / (a.hkv * a.hgroups);
   const int h0 = kh * a.group + hg * HP, nh = min(HP, a.group - hg * HP);   // heads h0 .. h0 + nh - 1
 
   __shared__ __attribute__((aligned(16))) bf16_t qs[HP][kHeadDim];
-  __shared__ __attribute__((aligned(16))) uint32_t new_w[2][row_words<BITS>()], new_m[2][kGroups];
+  __shared__ __attribute__((aligned(16))) float new_x[2][kHeadDim];   // the new key and value as they are held
   __shared__ __attribute__((aligned(16))) bf16_t ps[kWaves][kGroups][HP][kTile];
-  __shared__ float part_o[kWaves][HP][kHeadDim], part_ml[kWaves][HP][2];
+  __shared__ __attribute__((aligned(16))) float part_o[kWaves + 1][HP][kHeadDim], part_ml[kWaves + 1][HP][2];
 
   const int64_t start = a.kv_start[b];
   int sk = max(0, min(a.kv_used[b], a.max_k));
   if (start < 0 || start + sk > a.c.rows) sk = 0;
-  const int n_tiles = (sk + kTile - 1) / kTile, n_parts = max(1, (n_tiles + a.chunk_tiles - 1) / a.chunk_tiles);
+  const int nk = max(0, sk - 1);                 // keys in the cache; the new one is apart
+  const int n_tiles = (nk + kTile - 1) / kTile, n_parts = max(1, (n_tiles + a.chunk_tiles - 1) / a.chunk_tiles);
   if (chunk >= n_parts) return;
   const int t_lo = chunk * a.chunk_tiles, t_hi = min(n_tiles, t_lo + a.chunk_tiles);
-  const bool has_new = t_hi == n_tiles && n_tiles > 0;
+  const bool has_new = chunk == n_parts - 1 && sk > 0;
 
-  // ---- loads of a tile: rows past sk read as zero (codes, s and m) ----
+  // ---- loads of a tile: rows past nk read as zero (codes, s and m) ----
   const int64_t row0 = kh * a.c.head_rows + start;
-  const brsrc_t krs = make_rsrc(a.c.k + row0 * row_words<BITS>(), (uint32_t)sk * kRow);
-  const brsrc_t vrs = make_rsrc(a.c.v + row0 * row_words<BITS>(), (uint32_t)sk * kRow);
-  const brsrc_t kmrs = make_rsrc(a.c.km + row0 * kGroups, (uint32_t)sk * 16);
-  const brsrc_t vmrs = make_rsrc(a.c.vm + row0 * kGroups, (uint32_t)sk * 16);
-  uint32_t kx[4][KW], vx[2][8][VW];
-  u32x4 kmeta, vmeta;
-  float bias[HP];
-  auto load_k = [&](int t) {
+  const brsrc_t krs = make_rsrc(a.c.k + row0 * row_words<BITS>(), (uint32_t)nk * kRow);
+  const brsrc_t vrs = make_rsrc(a.c.v + row0 * row_words<BITS>(), (uint32_t)nk * kRow);
+  const brsrc_t kmrs = make_rsrc(a.c.km + row0 * kGroups, (uint32_t)nk * 16);
+  const brsrc_t vmrs = make_rsrc(a.c.vm + row0 * kGroups, (uint32_t)nk * 16);
+  struct Tile {
+    uint32_t kx[4][KW], vx[2][8][VW];
+    u32x4 kmeta, vmeta;
+    float bias[HP];
+  } tiles[kDepth];
+  // (past the chunk's end a tile past the rows: zeros, and no access)
+  auto load_k = [&](Tile &l, int tile) {
+    const int t = tile < t_hi ? tile : n_tiles;
     const uint32_t at = (uint32_t)t * (kTile * kRow) + n16 * kRow + G * (kRow / 4);
 #pragma unroll
     for (int kb = 0; kb < 4; ++kb)
@@ -289,19 +318,20 @@ __global__ __launch_bounds__(64 * kWaves) void decode_attn_quant_kernel(QuantAtt
       for (int i = 0; i < KW / 4; ++i) {
         const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(krs, at + kb * 16 * kRow + 16 * i, 0, 0);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) kx[kb][4 * i + e] = v[e];
+        for (int e = 0; e < 4; ++e) l.kx[kb][4 * i + e] = v[e];
       }
     const uint32_t key = (uint32_t)t * kTile + lane;
-    kmeta = __builtin_amdgcn_raw_buffer_load_b128(kmrs, key * 16, 0, 0);
+    l.kmeta = __builtin_amdgcn_raw_buffer_load_b128(kmrs, key * 16, 0, 0);
     if constexpr (HAS_BIAS) {
 #pragma unroll
       for (int i = 0; i < HP; ++i) {
         const float *p = a.bias + (int64_t)b * a.bias_bs + (int64_t)(h0 + min(i, nh - 1)) * a.bias_hs;
-        bias[i] = u32_as_f32(__builtin_amdgcn_raw_buffer_load_b32(make_rsrc(p, (uint32_t)sk * 4), key * 4, 0, 0));
+        l.bias[i] = u32_as_f32(__builtin_amdgcn_raw_buffer_load_b32(make_rsrc(p, (uint32_t)nk * 4), key * 4, 0, 0));
       }
     }
   };
-  auto load_v = [&](int t) {
+  auto load_v = [&](Tile &l, int tile) {
+    const int t = tile < t_hi ? tile : n_tiles;
     const uint32_t at = (uint32_t)t * (kTile * kRow) + G * kRow + n16 * (4 * VW);
 #pragma unroll
     for (int st = 0; st < 2; ++st)
@@ -309,58 +339,90 @@ __global__ __launch_bounds__(64 * kWaves) void decode_attn_quant_kernel(QuantAtt
       for (int j = 0; j < 8; ++j) {
         const uint32_t p = at + (32 * st + 4 * j) * kRow;
         if constexpr (BITS == 4) {
-          vx[st][j][0] = __builtin_amdgcn_raw_buffer_load_b32(vrs, p, 0, 0);
+          l.vx[st][j][0] = __builtin_amdgcn_raw_buffer_load_b32(vrs, p, 0, 0);
         } else {
           const u32x2 v = __builtin_amdgcn_raw_buffer_load_b64(vrs, p, 0, 0);
-          vx[st][j][0] = v[0];
-          vx[st][j][1] = v[1];
+          l.vx[st][j][0] = v[0];
+          l.vx[st][j][1] = v[1];
         }
       }
-    vmeta = __builtin_amdgcn_raw_buffer_load_b128(vmrs, ((uint32_t)t * kTile + lane) * 16, 0, 0);
+    l.vmeta = __builtin_amdgcn_raw_buffer_load_b128(vmrs, ((uint32_t)t * kTile + lane) * 16, 0, 0);
   };
-  int t = t_lo + wave;
-  const bool works = t < t_hi;
-  if (works) {
-    load_k(t);
-    load_v(t);
-  }
-
-  // ---- the query heads' rows, and the new key and value ----
-  if (wave == 0) {                               // 16 lanes a head
-    if (G < HP) {
-      const int head = h0 + min(G, nh - 1);
-      float x[8], wf[8], y[8];
-      unpack8(ld16(a.qkv + b * a.qkv_rs + (int64_t)head * kHeadDim + 8 * n16), x);
-      unpack8(ld16(a.qw + 8 * n16), wf);
-      const float hs = (float)(__bf16)((a.q_head_scale ? a.q_head_scale[head] : 1.f) * (a.q_row_scale ? a.q_row_scale[b] : 1.f));
-      norm_rope8(x, wf, a.eps, reinterpret_cast<const float(*)[2]>(a.rope) + b * (kHeadDim / 2) + 8 * (n16 & 7), n16, hs, y);
-      st16(&qs[G][8 * n16], pack8(y));
-    }
-  } else if (wave == 1 && has_new && G < 2) {    // lanes 0..15 the key, 16..31 the value
-    const int head = G == 0 ? a.h + kh : a.h + a.hkv + kh;
-    float x[8], wf[8], y[8];
-    const u32x4 raw = ld16(a.qkv + b * a.qkv_rs + (int64_t)head * kHeadDim + 8 * n16);
-    unpack8(raw, x);
-    unpack8(ld16(a.kw + 8 * n16), wf);
-    norm_rope8(x, wf, a.eps, reinterpret_cast<const float(*)[2]>(a.rope) + b * (kHeadDim / 2) + 8 * (n16 & 7), n16, 1.f, y);
-    const u32x4 turned = pack8(y);
-    unpack8(G == 0 ? turned : raw, x);
-    uint32_t w[BITS / 4], meta;
-    quant_row<BITS>(x, n16, w, meta);
-    const int64_t row = row0 + sk - 1;
-    uint32_t *codes = G == 0 ? a.c.k : a.c.v, *metas = G == 0 ? a.c.km : a.c.vm;
+  // ---- the rows to form: 16 lanes a row; wave 0 the query heads, wave 1 the new key (lanes 0 .. 15) and value.  Their
+  // loads come before the tiles': loads complete in issue order ----
+  const bool forms = wave == 0 ? G < HP : wave == 1 && has_new && G < 2;
+  const int head = wave == 0 ? h0 + min(G, nh - 1) : (G == 0 ? a.h : a.h + a.hkv) + kh;
+  u32x4 raw = {0u, 0u, 0u, 0u}, norm_w = raw;
+  f32x4 turn[4] = {};
+  float q_scale = 1.f;
+  if (forms) {
+    raw = ld16(a.qkv + b * a.qkv_rs + (int64_t)head * kHeadDim + 8 * n16);
+    norm_w = ld16((wave == 0 ? a.qw : a.kw) + 8 * n16);
+    const f32x4 *rp = reinterpret_cast<const f32x4 *>(a.rope + b * kHeadDim + 16 * (n16 & 7));
 #pragma unroll
-    for (int i = 0; i < BITS / 4; ++i) {
-      const int at = word_of(n16) * (BITS / 4) + i;
-      new_w[G][at] = w[i];
-      if (hg == 0) codes[row * row_words<BITS>() + at] = w[i];
+    for (int i = 0; i < 4; ++i) turn[i] = rp[i];
+    if (wave == 0)
+      q_scale = (float)(__bf16)((a.q_head_scale ? a.q_head_scale[head] : 1.f) * (a.q_row_scale ? a.q_row_scale[b] : 1.f));
+  }
+  float new_bias = 0.f;
+  if (HAS_BIAS && has_new && wave == kWaves - 1 && G < HP)
+    new_bias = a.bias[(int64_t)b * a.bias_bs + (int64_t)(h0 + min(G, nh - 1)) * a.bias_hs + nk];
+  int t = t_lo + wave;
+  if (t < t_hi) {
+#pragma unroll
+    for (int d = 0; d < kDepth; ++d) {
+      load_k(tiles[d], t + d * kWaves);
+      // (the loop's loads and these in one order: at its head the compiler waits for whatever either order has last)
+      __builtin_amdgcn_sched_barrier(0);
+      load_v(tiles[d], t + d * kWaves);
+      __builtin_amdgcn_sched_barrier(0);
     }
-    if ((n16 & 3) == 0) {
-      new_m[G][n16 >> 2] = meta;
-      if (hg == 0) metas[row * kGroups + (n16 >> 2)] = meta;
+  }
+  if (forms) {
+    float x[8], wf[8], y[8], cs[8][2];
+    unpack8(raw, x);
+    unpack8(norm_w, wf);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) cs[i >> 1][i & 1] = turn[i >> 2][i & 3];
+    norm_rope8(x, wf, a.eps, cs, n16, q_scale, y);
+    const u32x4 turned = pack8(y);
+    if (wave == 0) {
+      st16(&qs[G][8 * n16], turned);
+    } else {
+      unpack8(G == 0 ? turned : raw, x);
+      uint32_t w[BITS / 4], meta;
+      quant_row<BITS>(x, n16, w, meta, y);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) new_x[G][8 * n16 + i] = y[i];
+      if (hg == 0) {
+        const int64_t row = row0 + nk;
+        uint32_t *codes = G == 0 ? a.c.k : a.c.v, *metas = G == 0 ? a.c.km : a.c.vm;
+#pragma unroll
+        for (int i = 0; i < BITS / 4; ++i) codes[row * row_words<BITS>() + word_of(n16) * (BITS / 4) + i] = w[i];
+        if ((n16 & 3) == 0) metas[row * kGroups + (n16 >> 2)] = meta;
+      }
     }
   }
   __syncthreads();
+  // ---- the new key: a part of its own, 16 lanes a head ----
+  if (has_new && wave == kWaves - 1 && G < HP) {
+    float q[8], z = 0.f;
+    unpack8(*reinterpret_cast<const u32x4 *>(&qs[G][8 * n16]), q);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      z = fmaf(q[i], new_x[0][8 * n16 + i], z);
+      part_o[kWaves][G][8 * n16 + i] = new_x[1][8 * n16 + i];
+    }
+    z += dpp<0xB1>(z);
+    z += dpp<0x4E>(z);
+    z += dpp<0x141>(z);
+    z += dpp<0x140>(z);
+    const bool hidden = new_bias == -INFINITY;
+    if (n16 == 0) {
+      part_ml[kWaves][G][0] = hidden ? -INFINITY : (z + new_bias) * a.scale_log2;
+      part_ml[kWaves][G][1] = hidden ? 0.f : 1.f;
+    }
+  }
 
   // ---- Q in A's layout, and its sums by group ----
   bf16x8 qf[kGroups];
@@ -394,44 +456,21 @@ __global__ __launch_bounds__(64 * kWaves) void decode_attn_quant_kernel(QuantAtt
   // position of this lane's key in A's order of keys: lane (m, G) takes keys 4 j + G, j = 0 .. 7, of 32
   bf16_t *const pw = &ps[wave][0][0][32 * (lane >> 5) + 8 * (lane & 3) + ((lane & 31) >> 2)];
 
-  for (; t < t_hi; t += kWaves) {
-    if (t == n_tiles - 1) {                      // the new row, in place of what the cache held there
-      const int key = (sk - 1) & 63;
-#pragma unroll
-      for (int kb = 0; kb < 4; ++kb)
-#pragma unroll
-        for (int i = 0; i < KW; ++i) {
-          const uint32_t w = new_w[0][KW * G + i];
-          kx[kb][i] = key == 16 * kb + n16 ? w : kx[kb][i];
-        }
-#pragma unroll
-      for (int st = 0; st < 2; ++st)
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-#pragma unroll
-          for (int i = 0; i < VW; ++i) {
-            const uint32_t w = new_w[1][VW * n16 + i];
-            vx[st][j][i] = key == 32 * st + 4 * j + G ? w : vx[st][j][i];
-          }
-#pragma unroll
-      for (int g = 0; g < kGroups; ++g) {
-        const uint32_t k1 = new_m[0][g], v1 = new_m[1][g];
-        kmeta[g] = key == lane ? k1 : kmeta[g];
-        vmeta[g] = key == lane ? v1 : vmeta[g];
-      }
-    }
+  uint32_t nibbles = kNibbles, bf128 = kBf128;
+  asm("" : "+v"(nibbles), "+v"(bf128));
+  auto step = [&](Tile &l) {
     // ---- logits of key `lane` ----
     float z[HP];
 #pragma unroll
-    for (int i = 0; i < HP; ++i) z[i] = HAS_BIAS ? bias[i] : 0.f;
+    for (int i = 0; i < HP; ++i) z[i] = HAS_BIAS ? l.bias[i] : 0.f;
     uint32_t ky[4][4];                           // 4 bits: merged halves (words 0 1 lo, 0 1 hi, 2 3 lo, 2 3 hi)
     if constexpr (BITS == 4) {
 #pragma unroll
       for (int kb = 0; kb < 4; ++kb)
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
-          ky[kb][2 * p] = merge_half(kx[kb][2 * p], kx[kb][2 * p + 1], 0);
-          ky[kb][2 * p + 1] = merge_half(kx[kb][2 * p], kx[kb][2 * p + 1], 1);
+          ky[kb][2 * p] = merge_half(l.kx[kb][2 * p], l.kx[kb][2 * p + 1], 0);
+          ky[kb][2 * p + 1] = merge_half(l.kx[kb][2 * p], l.kx[kb][2 * p + 1], 1);
         }
     }
 #pragma unroll
@@ -449,30 +488,30 @@ __global__ __launch_bounds__(64 * kWaves) void decode_attn_quant_kernel(QuantAtt
         for (int w = 0; w < 4; ++w) {            // codes e = 2 g (w < 2) and 2 g + 1 of words 0 1 or 2 3
           const int e = 2 * g + (w >> 1), p = w & 1;
           if constexpr (BITS == 4)
-            c[w] = nibble_pair(ky[kb][2 * p + (e >> 2)], e);
+            c[w] = nibble_pair(ky[kb][2 * p + (e >> 2)], e, nibbles, bf128);
           else
-            c[w] = byte_pair(kx[kb][4 * p + (e >> 2)], kx[kb][4 * p + 2 + (e >> 2)], e & 3);
+            c[w] = byte_pair(l.kx[kb][4 * p + (e >> 2)], l.kx[kb][4 * p + 2 + (e >> 2)], e & 3);
         }
         s[kb] = mfma16(qf[g], __builtin_bit_cast(bf16x8, c), init);
       }
-      const float step = u32_as_f32(kmeta[g] << 16), least = u32_as_f32(kmeta[g] & 0xffff0000u);
+      const float step = u32_as_f32(l.kmeta[g] << 16), least = u32_as_f32(l.kmeta[g] & 0xffff0000u);
 #pragma unroll
       for (int i = 0; i < HP; ++i) {
         const float s01 = G & 1 ? s[1][i] : s[0][i], s23 = G & 1 ? s[3][i] : s[2][i];
         z[i] = fmaf(G & 2 ? s23 : s01, step, fmaf(qsum[g][i], least, z[i]));
       }
     }
-    const bool there = t * kTile + lane < sk;
     bool up = false;
 #pragma unroll
     for (int i = 0; i < HP; ++i) {
       z[i] *= a.scale_log2;
       asm("" : "+v"(z[i]));   // rounded: contracted into z - m below, a bias near the lowest float leaves the rounding's rest
-      if (!there) z[i] = -INFINITY;
-      if constexpr (HAS_BIAS) z[i] = bias[i] == -INFINITY ? -INFINITY : z[i];   // hidden, whatever the row holds
+      if (t * kTile + lane >= nk) z[i] = -INFINITY;
+      if constexpr (HAS_BIAS) z[i] = l.bias[i] == -INFINITY ? -INFINITY : z[i];   // hidden, whatever the row holds
       up |= z[i] > mrun[i] + kRescaleTau;
     }
-    if (t + kWaves < t_hi) load_k(t + kWaves);
+    load_k(l, t + kDepth * kWaves);
+    __builtin_amdgcn_sched_barrier(0);
     if (__builtin_amdgcn_ballot_w64(up)) {
 #pragma unroll
       for (int i = 0; i < HP; ++i) {
@@ -491,7 +530,7 @@ __global__ __launch_bounds__(64 * kWaves) void decode_attn_quant_kernel(QuantAtt
       lsum[i] += p;
 #pragma unroll
       for (int g = 0; g < kGroups; ++g) {
-        const float step = u32_as_f32(vmeta[g] << 16), least = u32_as_f32(vmeta[g] & 0xffff0000u);
+        const float step = u32_as_f32(l.vmeta[g] << 16), least = u32_as_f32(l.vmeta[g] & 0xffff0000u);
         const __bf16 w = (__bf16)mul_zero(p, step);   // (a weight of 0 is 0, whatever the row holds)
         pw[(g * HP + i) * kTile] = __builtin_bit_cast(uint16_t, w);
         rest[i][g] += mul_zero(p, least);
@@ -505,8 +544,8 @@ __global__ __launch_bounds__(64 * kWaves) void decode_attn_quant_kernel(QuantAtt
       if constexpr (BITS == 4) {
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-          vy[w][0] = merge_half(vx[st][2 * w][0], vx[st][2 * w + 1][0], 0);
-          vy[w][1] = merge_half(vx[st][2 * w][0], vx[st][2 * w + 1][0], 1);
+          vy[w][0] = merge_half(l.vx[st][2 * w][0], l.vx[st][2 * w + 1][0], 0);
+          vy[w][1] = merge_half(l.vx[st][2 * w][0], l.vx[st][2 * w + 1][0], 1);
         }
       }
 #pragma unroll
@@ -518,28 +557,40 @@ __global__ __launch_bounds__(64 * kWaves) void decode_attn_quant_kernel(QuantAtt
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
             if constexpr (BITS == 4)
-              c[w] = nibble_pair(vy[w][e >> 2], e);
+              c[w] = nibble_pair(vy[w][e >> 2], e, nibbles, bf128);
             else
-              c[w] = byte_pair(vx[st][2 * w][e >> 2], vx[st][2 * w + 1][e >> 2], e & 3);
+              c[w] = byte_pair(l.vx[st][2 * w][e >> 2], l.vx[st][2 * w + 1][e >> 2], e & 3);
           }
           oacc[e] = mfma16(pf, __builtin_bit_cast(bf16x8, c), oacc[e]);
         }
       }
     }
-    if (t + kWaves < t_hi) load_v(t + kWaves);
+    load_v(l, t + kDepth * kWaves);
+    __builtin_amdgcn_sched_barrier(0);
+    t += kWaves;
+  };
+  if constexpr (kDepth == 2) {
+    // (an exit between the two steps would leave the compiler a path on which the second tile's loads are the older)
+    while (t + kWaves < t_hi) {
+      step(tiles[0]);
+      step(tiles[1]);
+    }
+    if (t < t_hi) step(tiles[0]);
+  } else {
+    while (t < t_hi) step(tiles[0]);
   }
 
   // ---- the waves' results meet in LDS ----
 #pragma unroll
   for (int i = 0; i < HP; ++i) {
-    const float l = wave_sum(lsum[i]);
+    const float l = wave_add(lsum[i]);
     if (lane == 0) {
       part_ml[wave][i][0] = mrun[i];
       part_ml[wave][i][1] = l;
     }
 #pragma unroll
     for (int g = 0; g < kGroups; ++g) {
-      const float r = wave_sum(rest[i][g]);
+      const float r = wave_add(rest[i][g]);
       if (G == g) {                              // lane group g writes group g's elements
         part_o[wave][i][32 * g + n16] = oacc[2 * g][i] + r;
         part_o[wave][i][32 * g + 16 + n16] = oacc[2 * g + 1][i] + r;
@@ -558,9 +609,11 @@ __global__ __launch_bounds__(64 * kWaves) void decode_attn_quant_kernel(QuantAtt
     const int i = item / 64, d = 2 * (item % 64);
     float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) m = fmaxf(m, part_ml[w][i][0]);
+    for (int w = 0; w < kWaves + 1; ++w)
+      if (w < kWaves || has_new) m = fmaxf(m, part_ml[w][i][0]);
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
+    for (int w = 0; w < kWaves + 1; ++w) {
+      if (w == kWaves && !has_new) break;
       const float mw = part_ml[w][i][0], f = mw == -INFINITY ? (part_ml[w][i][1] == 0.f ? 0.f : 1.f) : fast_exp2(mw - m);
       l += f * part_ml[w][i][1];
       o0 += mul_zero(f, part_o[w][i][d]);
@@ -585,52 +638,70 @@ __global__ __launch_bounds__(64 * kWaves) void decode_attn_quant_kernel(QuantAtt
   __syncthreads();
   if (!last_s) return;
   if (tid == 0) st_agent(a.counters + unit, 0u);
-  // ---- the last workgroup of the unit merges its chunks, in their order ----
-  for (int item = tid; item < kOuts; item += 64 * kWaves) {
-    const int i = item / 64;
-    float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
-    constexpr int kAhead = 8;
-    for (int c0 = 0; c0 < n_parts; c0 += kAhead) {
-      uint64_t ml[kAhead], o[kAhead];
+  // ---- the last workgroup of the unit merges its chunks: four output elements per thread, every kSets-th chunk,
+  // as many loads in flight as chunks; then the sets in turn ----
+  constexpr int kItems = HP * 32, kSets = 64 * kWaves / kItems, kAhead = 8;
+  const int item = tid % kItems, set = tid / kItems, i = item / 32;
+  float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+  auto fold = [&](float mc, float lc, const float (&oc)[4]) {
+    const float mn = fmaxf(m, mc), f0 = m == -INFINITY ? 0.f : fast_exp2(m - mn), f1 = mc == -INFINITY ? 1.f : fast_exp2(mc - mn);
+    l = l * f0 + lc * f1;
 #pragma unroll
-      for (int r = 0; r < kAhead; ++r) {         // (every load is made, past the end the last's)
-        const int64_t at = ((int64_t)unit * a.ns + min(c0 + r, n_parts - 1)) * HP + i;
-        ml[r] = ld_agent(a.ml + at);
-        o[r] = ld_agent(a.po + at * 64 + item % 64);
-      }
+    for (int e = 0; e < 4; ++e) o[e] = o[e] * f0 + oc[e] * f1;
+    m = mn;
+  };
+  for (int c0 = set; c0 < n_parts; c0 += kAhead * kSets) {
+    uint64_t ml[kAhead], ow[kAhead][2];
 #pragma unroll
-      for (int r = 0; r < kAhead; ++r) {
-        const float2 mc = __builtin_bit_cast(float2, ml[r]), oc = __builtin_bit_cast(float2, o[r]);
-        if (c0 + r >= n_parts || mc.y == 0.f) continue;   // saw no key
-        const float mn = fmaxf(m, mc.x), f0 = m == -INFINITY ? 0.f : fast_exp2(m - mn);
-        const float f1 = mc.x == -INFINITY ? 1.f : fast_exp2(mc.x - mn);
-        l = l * f0 + mc.y * f1;
-        o0 = o0 * f0 + oc.x * f1;
-        o1 = o1 * f0 + oc.y * f1;
-        m = mn;
-      }
+    for (int r = 0; r < kAhead; ++r) {           // (every load is made, past the end the last's)
+      const int64_t at = ((int64_t)unit * a.ns + min(c0 + r * kSets, n_parts - 1)) * HP + i;
+      ml[r] = ld_agent(a.ml + at);
+      ow[r][0] = ld_agent(a.po + at * 64 + 2 * (item % 32));
+      ow[r][1] = ld_agent(a.po + at * 64 + 2 * (item % 32) + 1);
     }
-    put(item, o0, o1, l);
+#pragma unroll
+    for (int r = 0; r < kAhead; ++r) {
+      const float2 mc = __builtin_bit_cast(float2, ml[r]), a0 = __builtin_bit_cast(float2, ow[r][0]), a1 = __builtin_bit_cast(float2, ow[r][1]);
+      const float oc[4] = {a0.x, a0.y, a1.x, a1.y};
+      if (c0 + r * kSets < n_parts && mc.y != 0.f) fold(mc.x, mc.y, oc);   // (0: saw no key)
+    }
   }
+  __shared__ float set_s[kSets > 1 ? kSets - 1 : 1][6][kItems];
+  if (set > 0) {
+    set_s[set - 1][0][item] = m;
+    set_s[set - 1][1][item] = l;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) set_s[set - 1][2 + e][item] = o[e];
+  }
+  __syncthreads();
+  if (set > 0) return;
+#pragma unroll
+  for (int s = 0; s < kSets - 1; ++s) {
+    const float oc[4] = {set_s[s][2][item], set_s[s][3][item], set_s[s][4][item], set_s[s][5][item]};
+    if (set_s[s][1][item] != 0.f) fold(set_s[s][0][item], set_s[s][1][item], oc);
+  }
+  put(2 * item, o[0], o[1], l);
+  put(2 * item + 1, o[2], o[3], l);
 }
 
 // Chunks: as many as make two workgroups per CU for the longest sequence, each of whole rounds of its waves.
 struct QuantPlan {
-  int hp, hgroups, units, chunk_tiles, ns;
+  int bits, hp, hgroups, units, chunk_tiles, ns;
 };
-QuantPlan plan_quant(int num_seqs, int num_heads, int num_heads_k, int max_k) {
+QuantPlan plan_quant(int bits, int num_seqs, int num_heads, int num_heads_k, int max_k) {
   QuantPlan p;
+  p.bits = bits;
   const int group = num_heads / num_heads_k;
   p.hp = group >= 3 ? 4 : group;
   p.hgroups = (group + p.hp - 1) / p.hp;
   p.units = num_seqs * num_heads_k * p.hgroups;
-  const int tiles = std::max(1, (max_k + kTile - 1) / kTile), want = std::max(1, 2 * device_cus() / p.units);
+  const int tiles = std::max(1, (max_k + kTile - 1) / kTile), want = std::max(1, per_cu(p.bits, p.hp) * device_cus() / p.units);
   p.chunk_tiles = ((tiles + want - 1) / want + kWaves - 1) / kWaves * kWaves;
   p.ns = (tiles + p.chunk_tiles - 1) / p.chunk_tiles;
   return p;
 }
 // The counters' region is the same for every launch, so that no launch writes partial results where another counts.
-int64_t quant_counter_bytes() { return ((int64_t)device_cus() * 2 * 4 + 255) / 256 * 256; }
+int64_t quant_counter_bytes() { return ((int64_t)device_cus() * 3 * 4 + 255) / 256 * 256; }
 int64_t quant_bytes(int64_t parts, int hp) {   // counters, (max, sum), O
   return quant_counter_bytes() + (parts * hp * 8 + 255) / 256 * 256 + parts * hp * kHeadDim * 4;
 }
@@ -719,9 +790,9 @@ extern "C" int tg_kv_dequantize(const void *k_codes, const void *k_meta, const v
 extern "C" int64_t tg_decode_attention_quant_workspace_size(int32_t num_seqs, int32_t num_heads, int32_t num_heads_k,
                                                             int32_t max_seqlen_k) {
   if (num_seqs <= 0 || num_heads <= 0 || num_heads_k <= 0 || num_heads % num_heads_k != 0 || max_seqlen_k <= 0) return 0;
-  const QuantPlan p = plan_quant(num_seqs, num_heads, num_heads_k, max_seqlen_k);
+  const QuantPlan p = plan_quant(8, num_seqs, num_heads, num_heads_k, max_seqlen_k);
   const int64_t rounds = ((int64_t)max_seqlen_k + kWaves * kTile - 1) / (kWaves * kTile);
-  return rounds == 1 ? 0 : quant_bytes(std::min<int64_t>(2 * device_cus(), p.units * rounds), p.hp);
+  return rounds == 1 ? 0 : quant_bytes(std::min<int64_t>(per_cu(p.bits, p.hp) * device_cus(), p.units * rounds), p.hp);
 }
 
 extern "C" int tg_decode_attention_quant(const void *qkv, int64_t qkv_row_stride, const float *rope, int32_t num_seqs,
@@ -755,7 +826,7 @@ extern "C" int tg_decode_attention_quant(const void *qkv, int64_t qkv_row_stride
   TG_CHECK(max_seqlen_k < (1 << 24), "%s: max_seqlen_k must be less than 2^24", what);   // spans of under 4 GiB
   TG_CHECK(!bias_raw || (bias_seq_stride >= 0 && bias_head_stride >= 0), "%s: negative bias stride", what);
   if (num_seqs == 0) return 0;
-  const QuantPlan p = plan_quant(num_seqs, num_heads, num_heads_k, max_seqlen_k);
+  const QuantPlan p = plan_quant(bits, num_seqs, num_heads, num_heads_k, max_seqlen_k);
   a.qkv = static_cast<const bf16_t *>(qkv);
   a.qkv_rs = qkv_row_stride;
   a.rope = rope;
