@@ -107,7 +107,8 @@ def test_c_abi_refusals(ptr):
     for change, text in ((dict(qkv=None), "null pointer"), (dict(h=15), "multiple of the KV heads"), (dict(qkv_rs=4088), "row strides"),
                          (dict(out_rs=2044), "row strides"), (dict(scale=0.0), "softmax_scale"), (dict(d=64), "head_dim"),
                          (dict(bits=2), "4 or 8"), (dict(rope=p + 4), "aligned"), (dict(n=-1), "sequence count"),
-                         (dict(max_k=-1), "length"), (dict(h=264), "256")):
+                         (dict(max_k=-1), "length"), (dict(h=264), "256"), (dict(max_k=1000, ws_n=1000), "workspace"),
+                         (dict(max_k=1000, ws=None), "workspace"), (dict(max_k=1 << 24), "2^24")):
         assert text in _call("tg_decode_attention_quant", attn, **change), change
     sample = dict(x=p, rs=100, n=1, cols=100, u=p, t=None, k=None, tp=None, mp=None, token=p, lp=None, ws=p, ws_n=1 << 30, stream=None)
     for change, text in ((dict(u=None), "null pointer"), (dict(rs=99), "row stride"), (dict(cols=0), "columns"),

@@ -5,8 +5,9 @@ rounding there are IEEE's, as the kernel's are; code times step is exact in fp32
 
 Attention is compared with float64 over the values s c + m that the cache holds.  With P the weights and z the
 logits, the kernel may be off by (a rounding to bf16, of 8 significant bits, by 2^-8 relative)
-  * the weights' rounding to bf16 before the value product, 2^-8 each, where a value counts by its code's part s c
-    (the least values' part is summed in fp32): 2^-8 sum P s c;
+  * the weights' rounding before the value product, to two bf16 numbers, 2^-16 each, where a value counts by its code's
+    part s c (the least values' part is summed in fp32): 2^-16 sum P s c; at 4 bits codes are held as 128 + c here too,
+    taken off at the end, and the sums of 128 + L times a step are good to 2^-18;
   * the logits' fp32 sums: a group's 32 products of a bf16 query value and a code are summed from -128 sum q on (at 4
     bits codes are held as 128 + c), at most 2^-20 (128 + L) sum |q| a group (16 roundings), so
     dz = scale max_j sum_g s_jg 2^-20 (128 + L) sum_{d in g} |q_d| + 2^-20 max |z|, and 2 dz sum P |v|;
@@ -208,6 +209,7 @@ def check_attn(c, out, cache, skip=()):
         assert torch.equal(a.view(torch.uint8), b.view(torch.uint8)), "cache after the append"
     kk, vv = (t.to(out.device) for t in values_of(want))
     ks, vm = want.k_meta[..., 0].double(), want.v_meta[..., 1].double().repeat_interleave(32, -1)
+    vs = want.v_meta[..., 0].double().repeat_interleave(32, -1)
     L = 2 ** bits - 1
     for b in range(B):
         s, n = int(c["start"][b]), int(c["used"][b])
@@ -224,9 +226,10 @@ def check_attn(c, out, cache, skip=()):
             p = torch.softmax(z, 0)
             ref, mass = p @ v, p @ v.abs()
             coded = p @ (v - vm[kh, s:s + n])
+            steps = p @ vs[kh, s:s + n]
             dz = SCALE * 2.0 ** -20 * (128 + L) * float((ks[kh, s:s + n] * qd.abs().view(4, 32).sum(1)).sum(1).max()) \
                 + 2.0 ** -20 * float(z[torch.isfinite(z)].abs().max())
-            tol = 2.0 ** -8 * coded + 2.0 ** -8 * ref.abs() + (2 * dz + 2.0 ** -18) * mass + 1e-30
+            tol = 2.0 ** -16 * coded + 2.0 ** -18 * (128 + L) * steps + 2.0 ** -8 * ref.abs() + (2 * dz + 2.0 ** -18) * mass + 1e-30
             err = (out[b, h].double() - ref).abs()
             assert bool((err <= tol).all()), (b, h, float((err / tol).max()))
 

@@ -185,9 +185,11 @@ __global__ __launch_bounds__(256) void kv_dequantize_kernel(QuantCache c, RowTar
 //     words 4 G .. 4 G + 3 of key n.
 //   * At 4 bits codes become bf16 by their bits: 0x4300 | c is 128 + c (two per and-or).  The sums start from
 //     -128 Q_g (C operand); the output's part is taken off at the end.  At 8 bits they are converted.
-//   * O += P C with P = bf16(p s) per group (8 significant bits, as the bf16 cache's kernel weights; the least values'
-//     part is summed in fp32), from LDS in A's layout; B: lane (n, G) holds word n of keys 4 j + G, whose nibble
-//     (byte) e is element 16 e + n: eight keys of one element, and the element's group depends on e alone.
+//   * O += P C with P = p s per group, from LDS in A's layout, as two bf16 numbers of 16 bits together: rounded to
+//     one, the weights of keys that cancel left errors of 0.4 % of the output.  The second takes rows of A that would
+//     repeat the heads, so no more instructions.  The least values' part is summed in fp32.  B: lane (n, G) holds word
+//     n of keys 4 j + G, whose nibble (byte) e is element 16 e + n: eight keys of one element, and the element's
+//     group depends on e alone.
 //   * The new key is not in the tiles: it is a part of its own beside the waves', from registers.
 //   * The running maximum moves only when a logit passes it by 2^8.  Waves merge in LDS, chunks through the
 //     workspace in the workgroup that arrives last.
@@ -195,7 +197,7 @@ struct QuantAttnArgs {
   const bf16_t *qkv;
   int64_t qkv_rs;
   const float *rope;
-  int h, hkv, group, hgroups;
+  int h, hkv, group;
   const bf16_t *qw, *kw;
   float eps;
   const float *q_head_scale, *q_row_scale;
@@ -207,13 +209,15 @@ struct QuantAttnArgs {
   float scale_log2;
   bf16_t *out;
   int64_t out_rs;
-  int units, chunk_tiles, ns;    // (sequence, kv head, head set); tiles per chunk; chunks of the longest sequence
+  int nseq, sets;                // kv heads times head sets
+  int slots, least;              // workgroups that are resident at once; fewest tiles per chunk
   uint32_t *counters;            // per unit: chunks arrived; zero between launches
-  uint64_t *ml;                  // [unit][chunk][head]: running max (log2 units) and sum
-  uint64_t *po;                  // [unit][chunk][head][64]: O, pairs of fp32
+  uint64_t *ml;                  // [workgroup][head]: running max (log2 units) and sum
+  uint64_t *po;                  // [workgroup][head][64]: O, pairs of fp32
 };
 
 constexpr int kWaves = 4;
+constexpr int kRounds = 2;
 constexpr int kTile = 64;        // keys of a wave's step
 // Tiles that a wave holds or has on their way, and workgroups per CU, by the registers
 constexpr int depth(int bits, int hp) { return bits == 4 && hp <= 2 ? 2 : 1; }
@@ -272,6 +276,78 @@ __device__ __forceinline__ uint32_t byte_pair(uint32_t a, uint32_t b, int byte) 
   return __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, fb), __builtin_bit_cast(uint32_t, fa), 0x07060302u);
 }
 
+// The chunk that a workgroup takes: the q-th of all sequences' chunks in turn.  A sequence of n tiles is cut into
+// ceil(n / T) chunks of even length, with one T for all, from their tiles, which only the device knows: the least that
+// makes no more workgroups than are resident at once (a workgroup's fixed costs, 5 us, and a second round's uneven
+// end cost more than idle places), or, where the sequences' remainders alone would fill most of these, two
+// rounds.  16 / 8 heads, T for one round of the longest sequence / two rounds / as here, us: 64 sequences of 512 .. 4099
+// at 8 bits 84.7 / 84.3 / 79.8; 8 of 16k .. 128k at 4 bits 183 / 170 / 159; 16 of 4k .. 30k - / 63 / 57; 64 alike of
+// 4096 70 / 77 / 70.
+struct Chunk {
+  int seq, chunk, chunks, tiles, sk;
+  int64_t start;
+};
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int scan_step(int x) { return x + __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xf, false); }
+__device__ __forceinline__ int wave_scan(int x) {   // sum over the lanes up to this one
+  x = scan_step<0x111, 0xf>(x);   // row_shr 1, 2, 4, 8
+  x = scan_step<0x112, 0xf>(x);
+  x = scan_step<0x114, 0xf>(x);
+  x = scan_step<0x118, 0xf>(x);
+  x = scan_step<0x142, 0xa>(x);   // row_bcast 15: the first row's sum to the second, the third's to the fourth
+  return scan_step<0x143, 0xc>(x);   // row_bcast 31: the first half's to the second
+}
+// ceil(n / T), n and T below 2^22: the quotient's float is off by less than 1 / T
+__device__ __forceinline__ int ceil_div(int n, float inv) { return (int)(((float)n - 0.5f) * inv) + 1; }
+__device__ __forceinline__ Chunk find_chunk(const QuantAttnArgs &a, int q, int lane) {
+  int sk = 0, start = 0, tiles = 0;
+  auto read = [&](int s) {                       // of sequence s, this lane's
+    start = s < a.nseq ? a.kv_start[s] : 0;
+    sk = s < a.nseq ? max(0, min(a.kv_used[s], a.max_k)) : 0;
+    if (start < 0 || (int64_t)start + sk > a.c.rows) sk = 0;
+    tiles = (max(0, sk - 1) + kTile - 1) / kTile;
+  };
+  auto count = [&](int T, bool all) {            // chunks of all sequences, or their tiles
+    int n = 0;
+    const float inv = 1.f / (float)T;
+    for (int s0 = 0; s0 < a.nseq; s0 += 64) {
+      if (s0 > 0 || all) read(s0 + lane);
+      n += wave_sum_int(all ? tiles : s0 + lane < a.nseq ? max(1, ceil_div(tiles, inv)) : 0);
+    }
+    if (a.nseq > 64) read(lane);
+    return __builtin_amdgcn_readfirstlane(n);
+  };
+  const float work = (float)count(1, true) * (float)a.sets, slots = (float)a.slots;
+  float target = slots;
+  int T = max(a.least, (int)(work / target) + 1);
+  for (int i = 0; i < 3 && T > a.least; ++i) {
+    const float over = (float)count(T, false) * (float)a.sets - slots;
+    if (over <= 0.f) break;
+    if (over > 0.75f * slots) {
+      T = max(a.least, (int)(work / (kRounds * slots)) + 1);
+      break;
+    }
+    target = fmaxf(target - over, 0.25f * slots);
+    T = (int)(work / target) + 1;
+  }
+  const float inv = 1.f / (float)T;
+  int before = 0;
+  for (int s0 = 0; s0 < a.nseq; s0 += 64) {
+    if (s0 > 0) read(s0 + lane);
+    const int n = s0 + lane < a.nseq ? max(1, ceil_div(tiles, inv)) : 0;
+    const int up_to = wave_scan(n) + before;
+    const uint64_t in = __builtin_amdgcn_ballot_w64(up_to > q);
+    if (in) {
+      const int l = (int)__builtin_ctzll(in);
+      const int chunks = __builtin_amdgcn_readlane(n, l);
+      return Chunk{s0 + l, q - (__builtin_amdgcn_readlane(up_to, l) - chunks), chunks, __builtin_amdgcn_readlane(tiles, l),
+                   __builtin_amdgcn_readlane(sk, l), __builtin_amdgcn_readlane(start, l)};
+    }
+    before = __builtin_amdgcn_readlane(up_to, 63);
+  }
+  return Chunk{-1, 0, 0, 0, 0, 0};
+}
+
 template <int BITS, int HP, bool HAS_BIAS>
 __global__ __launch_bounds__(64 * kWaves, per_cu(BITS, HP)) void decode_attn_quant_kernel(QuantAttnArgs a) {
   constexpr int kRow = 16 * BITS;                 // bytes of a row's codes
@@ -279,23 +355,21 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(BITS, HP)) void decode_attn_qua
   constexpr int VW = BITS / 4;                    // and for O
   constexpr int kDepth = depth(BITS, HP);         // tiles in registers
   const int tid = threadIdx.x, wave = wave_id(), lane = tid & 63, n16 = lane & 15, G = lane >> 4;
-  const int unit = blockIdx.x % a.units, chunk = blockIdx.x / a.units;
-  const int kh = unit % a.hkv, hg = (unit / a.hkv) % a.hgroups, b = unit / (a.hkv * a.hgroups);
+  const int set = blockIdx.x % a.sets, kh = set % a.hkv, hg = set / a.hkv;
   const int h0 = kh * a.group + hg * HP, nh = min(HP, a.group - hg * HP);   // heads h0 .. h0 + nh - 1
 
   __shared__ __attribute__((aligned(16))) bf16_t qs[HP][kHeadDim];
   __shared__ __attribute__((aligned(16))) float new_x[2][kHeadDim];   // the new key and value as they are held
-  __shared__ __attribute__((aligned(16))) bf16_t ps[kWaves][kGroups][HP][kTile];
+  __shared__ __attribute__((aligned(16))) bf16_t ps[kWaves][kGroups][2 * HP][kTile];
   __shared__ __attribute__((aligned(16))) float part_o[kWaves + 1][HP][kHeadDim], part_ml[kWaves + 1][HP][2];
 
-  const int64_t start = a.kv_start[b];
-  int sk = max(0, min(a.kv_used[b], a.max_k));
-  if (start < 0 || start + sk > a.c.rows) sk = 0;
-  const int nk = max(0, sk - 1);                 // keys in the cache; the new one is apart
-  const int n_tiles = (nk + kTile - 1) / kTile, n_parts = max(1, (n_tiles + a.chunk_tiles - 1) / a.chunk_tiles);
-  if (chunk >= n_parts) return;
-  const int t_lo = chunk * a.chunk_tiles, t_hi = min(n_tiles, t_lo + a.chunk_tiles);
-  const bool has_new = chunk == n_parts - 1 && sk > 0;
+  const Chunk ck = find_chunk(a, blockIdx.x / a.sets, lane);
+  if (ck.seq < 0) return;                        // workgroup-uniform: past the last chunk
+  const int b = ck.seq, nk = max(0, ck.sk - 1);  // keys in the cache; the new one is apart
+  const int64_t start = ck.start;
+  const int n_tiles = ck.tiles, n_parts = ck.chunks, chunk = ck.chunk;
+  const int t_lo = (int)((int64_t)n_tiles * chunk / n_parts), t_hi = (int)((int64_t)n_tiles * (chunk + 1) / n_parts);
+  const bool has_new = chunk == n_parts - 1 && ck.sk > 0;
 
   // ---- loads of a tile: rows past nk read as zero (codes, s and m) ----
   const int64_t row0 = kh * a.c.head_rows + start;
@@ -521,7 +595,10 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(BITS, HP)) void decode_attn_qua
 #pragma unroll
         for (int g = 0; g < kGroups; ++g) rest[i][g] *= f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) oacc[e][i] *= f;
+        for (int e = 0; e < 8; ++e) {
+          oacc[e][i] *= f;
+          if constexpr (HP <= 2) oacc[e][i + HP] *= f;   // the low parts' rows
+        }
       }
     }
 #pragma unroll
@@ -531,10 +608,12 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(BITS, HP)) void decode_attn_qua
 #pragma unroll
       for (int g = 0; g < kGroups; ++g) {
         const float step = u32_as_f32(l.vmeta[g] << 16), least = u32_as_f32(l.vmeta[g] & 0xffff0000u);
-        const __bf16 w = (__bf16)mul_zero(p, step);   // (a weight of 0 is 0, whatever the row holds)
-        pw[(g * HP + i) * kTile] = __builtin_bit_cast(uint16_t, w);
+        const float w = mul_zero(p, step);       // (a weight of 0 is 0, whatever the row holds)
+        const __bf16 hi = (__bf16)w, lo = (__bf16)(w - (float)hi);
+        pw[(2 * HP * g + i) * kTile] = __builtin_bit_cast(uint16_t, hi);
+        pw[(2 * HP * g + HP + i) * kTile] = __builtin_bit_cast(uint16_t, lo);
         rest[i][g] += mul_zero(p, least);
-        if constexpr (BITS == 4) rest[i][g] = fmaf(-128.f, (float)w, rest[i][g]);
+        if constexpr (BITS == 4) rest[i][g] = fmaf(-128.f, (float)hi + (float)lo, rest[i][g]);
       }
     }
     // ---- O += P C ----
@@ -550,7 +629,7 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(BITS, HP)) void decode_attn_qua
       }
 #pragma unroll
       for (int g = 0; g < kGroups; ++g) {
-        const bf16x8 pf = *reinterpret_cast<const bf16x8 *>(&ps[wave][g][n16 & (HP - 1)][32 * st + 8 * G]);
+        const bf16x8 pf = *reinterpret_cast<const bf16x8 *>(&ps[wave][g][n16 & (2 * HP - 1)][32 * st + 8 * G]);
 #pragma unroll
         for (int e = 2 * g; e < 2 * g + 2; ++e) {
           u32x4 c;
@@ -591,9 +670,17 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(BITS, HP)) void decode_attn_qua
 #pragma unroll
     for (int g = 0; g < kGroups; ++g) {
       const float r = wave_add(rest[i][g]);
+      float o0 = oacc[2 * g][i], o1 = oacc[2 * g + 1][i];
+      if constexpr (HP <= 2) {
+        o0 += oacc[2 * g][i + HP];
+        o1 += oacc[2 * g + 1][i + HP];
+      } else {                                   // the low parts' rows are the neighbour lane group's
+        o0 += __shfl_xor(o0, 16);
+        o1 += __shfl_xor(o1, 16);
+      }
       if (G == g) {                              // lane group g writes group g's elements
-        part_o[wave][i][32 * g + n16] = oacc[2 * g][i] + r;
-        part_o[wave][i][32 * g + 16 + n16] = oacc[2 * g + 1][i] + r;
+        part_o[wave][i][32 * g + n16] = o0 + r;
+        part_o[wave][i][32 * g + 16 + n16] = o1 + r;
       }
     }
   }
@@ -623,7 +710,7 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(BITS, HP)) void decode_attn_qua
       put(item, o0, o1, l);
     } else {
       // (agent-scope accesses write through and read past the XCD's L2, where a release would write all of it back)
-      const int64_t at = ((int64_t)unit * a.ns + chunk) * HP + i;
+      const int64_t at = (int64_t)blockIdx.x * HP + i;
       const float2 o = {o0, o1}, mlv = {m, l};
       st_agent(a.po + at * 64 + item % 64, __builtin_bit_cast(uint64_t, o));
       if (d == 0) st_agent(a.ml + at, __builtin_bit_cast(uint64_t, mlv));
@@ -631,17 +718,18 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(BITS, HP)) void decode_attn_qua
   }
   if (n_parts == 1) return;
   __shared__ int last_s;
+  uint32_t *const counter = a.counters + (int64_t)b * a.sets + set;
   wait_all_mem();                                // this wave's stores are done
   __syncthreads();
   if (tid == 0)
-    last_s = __hip_atomic_fetch_add(a.counters + unit, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)n_parts - 1u;
+    last_s = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)n_parts - 1u;
   __syncthreads();
   if (!last_s) return;
-  if (tid == 0) st_agent(a.counters + unit, 0u);
+  if (tid == 0) st_agent(counter, 0u);
   // ---- the last workgroup of the unit merges its chunks: four output elements per thread, every kSets-th chunk,
   // as many loads in flight as chunks; then the sets in turn ----
   constexpr int kItems = HP * 32, kSets = 64 * kWaves / kItems, kAhead = 8;
-  const int item = tid % kItems, set = tid / kItems, i = item / 32;
+  const int item = tid % kItems, cs = tid / kItems, i = item / 32;
   float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
   auto fold = [&](float mc, float lc, const float (&oc)[4]) {
     const float mn = fmaxf(m, mc), f0 = m == -INFINITY ? 0.f : fast_exp2(m - mn), f1 = mc == -INFINITY ? 1.f : fast_exp2(mc - mn);
@@ -650,11 +738,11 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(BITS, HP)) void decode_attn_qua
     for (int e = 0; e < 4; ++e) o[e] = o[e] * f0 + oc[e] * f1;
     m = mn;
   };
-  for (int c0 = set; c0 < n_parts; c0 += kAhead * kSets) {
+  for (int c0 = cs; c0 < n_parts; c0 += kAhead * kSets) {
     uint64_t ml[kAhead], ow[kAhead][2];
 #pragma unroll
     for (int r = 0; r < kAhead; ++r) {           // (every load is made, past the end the last's)
-      const int64_t at = ((int64_t)unit * a.ns + min(c0 + r * kSets, n_parts - 1)) * HP + i;
+      const int64_t at = ((int64_t)blockIdx.x + (min(c0 + r * kSets, n_parts - 1) - chunk) * a.sets) * HP + i;
       ml[r] = ld_agent(a.ml + at);
       ow[r][0] = ld_agent(a.po + at * 64 + 2 * (item % 32));
       ow[r][1] = ld_agent(a.po + at * 64 + 2 * (item % 32) + 1);
@@ -667,14 +755,14 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(BITS, HP)) void decode_attn_qua
     }
   }
   __shared__ float set_s[kSets > 1 ? kSets - 1 : 1][6][kItems];
-  if (set > 0) {
-    set_s[set - 1][0][item] = m;
-    set_s[set - 1][1][item] = l;
+  if (cs > 0) {
+    set_s[cs - 1][0][item] = m;
+    set_s[cs - 1][1][item] = l;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) set_s[set - 1][2 + e][item] = o[e];
+    for (int e = 0; e < 4; ++e) set_s[cs - 1][2 + e][item] = o[e];
   }
   __syncthreads();
-  if (set > 0) return;
+  if (cs > 0) return;
 #pragma unroll
   for (int s = 0; s < kSets - 1; ++s) {
     const float oc[4] = {set_s[s][2][item], set_s[s][3][item], set_s[s][4][item], set_s[s][5][item]};
@@ -684,26 +772,27 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(BITS, HP)) void decode_attn_qua
   put(2 * item + 1, o[2], o[3], l);
 }
 
-// Chunks: as many as make two workgroups per CU for the longest sequence, each of whole rounds of its waves.
+// Workgroups of a launch: units of (sequence, kv head, head set), cut into chunks on the device.
 struct QuantPlan {
-  int bits, hp, hgroups, units, chunk_tiles, ns;
+  int hp, sets, slots, least;
+  int64_t grid, bytes;
 };
-QuantPlan plan_quant(int bits, int num_seqs, int num_heads, int num_heads_k, int max_k) {
+// The counters' region is the same for every launch, so that no launch writes partial results where another counts;
+// launches of more units cut none.
+constexpr int64_t kCounters = 1 << 14;
+QuantPlan plan_quant(int bits, int64_t num_seqs, int num_heads, int num_heads_k, int max_k) {
   QuantPlan p;
-  p.bits = bits;
   const int group = num_heads / num_heads_k;
   p.hp = group >= 3 ? 4 : group;
-  p.hgroups = (group + p.hp - 1) / p.hp;
-  p.units = num_seqs * num_heads_k * p.hgroups;
-  const int tiles = std::max(1, (max_k + kTile - 1) / kTile), want = std::max(1, per_cu(p.bits, p.hp) * device_cus() / p.units);
-  p.chunk_tiles = ((tiles + want - 1) / want + kWaves - 1) / kWaves * kWaves;
-  p.ns = (tiles + p.chunk_tiles - 1) / p.chunk_tiles;
+  p.sets = num_heads_k * ((group + p.hp - 1) / p.hp);
+  p.slots = per_cu(bits, p.hp) * device_cus();
+  const int64_t units = num_seqs * p.sets, tiles = std::max(1, (max_k + kTile - 1) / kTile);
+  // (a wave's first tile: 2320 keys 10.5 us in chunks of four tiles at least, 13.1 of eight)
+  p.least = units <= kCounters ? kWaves : 1 << 22;
+  p.grid = std::min<int64_t>(units * ((tiles + p.least - 1) / p.least), units + kRounds * p.slots);
+  // counters, (max, sum), O
+  p.bytes = p.grid == units ? 0 : kCounters * 4 + (p.grid * p.hp * 8 + 255) / 256 * 256 + p.grid * p.hp * kHeadDim * 4;
   return p;
-}
-// The counters' region is the same for every launch, so that no launch writes partial results where another counts.
-int64_t quant_counter_bytes() { return ((int64_t)device_cus() * 3 * 4 + 255) / 256 * 256; }
-int64_t quant_bytes(int64_t parts, int hp) {   // counters, (max, sum), O
-  return quant_counter_bytes() + (parts * hp * 8 + 255) / 256 * 256 + parts * hp * kHeadDim * 4;
 }
 
 int check_cache(const char *what, int32_t num_heads_k, int32_t head_dim, int32_t bits, const void *k_codes,
@@ -785,14 +874,12 @@ extern "C" int tg_kv_dequantize(const void *k_codes, const void *k_meta, const v
   return 0;
 }
 
-// (enough for fewer sequences and keys too: those may be cut into more chunks, never into more parts in all than two
-// per CU or one per round of four tiles)
+// (for the bits with more workgroups; enough for fewer sequences and keys too)
 extern "C" int64_t tg_decode_attention_quant_workspace_size(int32_t num_seqs, int32_t num_heads, int32_t num_heads_k,
                                                             int32_t max_seqlen_k) {
   if (num_seqs <= 0 || num_heads <= 0 || num_heads_k <= 0 || num_heads % num_heads_k != 0 || max_seqlen_k <= 0) return 0;
-  const QuantPlan p = plan_quant(8, num_seqs, num_heads, num_heads_k, max_seqlen_k);
-  const int64_t rounds = ((int64_t)max_seqlen_k + kWaves * kTile - 1) / (kWaves * kTile);
-  return rounds == 1 ? 0 : quant_bytes(std::min<int64_t>(per_cu(p.bits, p.hp) * device_cus(), p.units * rounds), p.hp);
+  const int64_t fits = kCounters / plan_quant(8, 1, num_heads, num_heads_k, 1).sets;   // sequences that may be cut
+  return plan_quant(8, std::min<int64_t>(num_seqs, fits), num_heads, num_heads_k, max_seqlen_k).bytes;
 }
 
 extern "C" int tg_decode_attention_quant(const void *qkv, int64_t qkv_row_stride, const float *rope, int32_t num_seqs,
@@ -847,21 +934,19 @@ extern "C" int tg_decode_attention_quant(const void *qkv, int64_t qkv_row_stride
   a.out = static_cast<bf16_t *>(out);
   a.out_rs = out_row_stride;
   a.group = num_heads / num_heads_k;
-  a.hgroups = p.hgroups;
-  a.units = p.units;
-  a.chunk_tiles = p.chunk_tiles;
-  a.ns = p.ns;
-  const int64_t parts = (int64_t)p.units * p.ns;
-  if (p.ns > 1) {
-    TG_CHECK(workspace != nullptr && workspace_bytes >= quant_bytes(parts, p.hp),
-             "%s: needs a workspace of %lld bytes (got %lld)", what, (long long)quant_bytes(parts, p.hp),
-             (long long)workspace_bytes);
+  a.nseq = num_seqs;
+  a.sets = p.sets;
+  a.slots = p.slots;
+  a.least = p.least;
+  if (p.bytes > 0) {
+    TG_CHECK(workspace != nullptr && workspace_bytes >= p.bytes, "%s: needs a workspace of %lld bytes (got %lld)", what,
+             (long long)p.bytes, (long long)workspace_bytes);
     char *ws = static_cast<char *>(workspace);
     a.counters = reinterpret_cast<uint32_t *>(ws);
-    a.ml = reinterpret_cast<uint64_t *>(ws + quant_counter_bytes());
-    a.po = reinterpret_cast<uint64_t *>(ws + quant_bytes(parts, p.hp) - parts * p.hp * kHeadDim * 4);
+    a.ml = reinterpret_cast<uint64_t *>(ws + kCounters * 4);
+    a.po = reinterpret_cast<uint64_t *>(ws + p.bytes - p.grid * p.hp * kHeadDim * 4);
   }
-  const dim3 grid((unsigned)parts), block(64 * kWaves);
+  const dim3 grid((unsigned)p.grid), block(64 * kWaves);
   auto launch = [&](auto bits_c, auto hp_c) {
     constexpr int BITS = decltype(bits_c)::value, HP = decltype(hp_c)::value;
     if (bias_raw)
