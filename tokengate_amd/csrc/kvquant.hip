@@ -42,67 +42,108 @@ __device__ __forceinline__ float min3_nan(float a, float b, float c) {
   return d;
 }
 
-// Lanes j = 2 e + p of 16 lanes hold element i of an 8 x 8 table (e, i) in nibble (byte) i of w: transposed among
-// the eight lanes of the same p.  Its own inverse.
-__device__ __forceinline__ uint32_t swap_parts(uint32_t x, uint32_t mask, int shift, int lanes, bool up) {
-  const uint32_t y = __shfl_xor(x, lanes);
-  return up ? (x & ~mask) | ((y >> shift) & mask) : (x & mask) | ((y & mask) << shift);
+// x of lane l ^ M, of 16 lanes, without the LDS crossbar
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp(uint32_t x) {
+  return (uint32_t)__builtin_amdgcn_update_dpp((int)x, (int)x, CTRL, 0xf, 0xf, true);
+}
+template <int CTRL>
+__device__ __forceinline__ float dpp(float x) {
+  return u32_as_f32(dpp<CTRL>(__builtin_bit_cast(uint32_t, x)));
+}
+template <int M>
+__device__ __forceinline__ uint32_t lane_xor(uint32_t x) {
+  static_assert(M == 1 || M == 2 || M == 4 || M == 8, "a row of 16 lanes");
+  if constexpr (M == 1) return dpp<0xB1>(x);                 // quad_perm 1 0 3 2
+  else if constexpr (M == 2) return dpp<0x4E>(x);            // quad_perm 2 3 0 1
+  else if constexpr (M == 4) return dpp<0x1B>(dpp<0x141>(x));   // row_half_mirror (l ^ 7), quad_perm 3 2 1 0 (l ^ 3)
+  else return dpp<0x128>(x);                                 // row_ror 8
+}
+template <int M>
+__device__ __forceinline__ float lane_xor(float x) {
+  return u32_as_f32(lane_xor<M>(__builtin_bit_cast(uint32_t, x)));
+}
+
+// Lanes j = 2 e + p of 16 lanes hold element i of an 8 x 8 table (e, i) in byte i of the pair w (4 bits: nibble i of
+// w): transposed among the eight lanes of the same p, part by part: a lane whose bit of e is 0 keeps its parts of
+// that bit 0 and takes its partner's, the partner those of bit 1.
+__device__ __forceinline__ uint32_t swap_bytes(uint32_t x, uint32_t y, bool up) {    // of 16
+  return __builtin_amdgcn_perm(y, x, up ? 0x03070105u : 0x06020400u);
+}
+__device__ __forceinline__ uint32_t swap_halves(uint32_t x, uint32_t y, bool up) {   // of 32
+  return __builtin_amdgcn_perm(y, x, up ? 0x03020706u : 0x05040100u);
+}
+__device__ __forceinline__ uint32_t swap_nibbles(uint32_t x, uint32_t y, bool up) {  // of 8
+  const uint32_t keep = up ? 0xF0F0F0F0u : 0x0F0F0F0Fu, moved = up ? y >> 4 : y << 4;
+  return (x & keep) | (moved & ~keep);
 }
 template <int BITS>
 __device__ __forceinline__ void transpose8(uint32_t (&w)[BITS / 4], int j) {
   if constexpr (BITS == 4) {
-    w[0] = swap_parts(w[0], 0x0F0F0F0Fu, 4, 2, j & 2);
-    w[0] = swap_parts(w[0], 0x00FF00FFu, 8, 4, j & 4);
-    w[0] = swap_parts(w[0], 0x0000FFFFu, 16, 8, j & 8);
+    w[0] = swap_halves(w[0], lane_xor<8>(w[0]), j & 8);
+    w[0] = swap_bytes(w[0], lane_xor<4>(w[0]), j & 4);
+    w[0] = swap_nibbles(w[0], lane_xor<2>(w[0]), j & 2);
   } else {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      w[i] = swap_parts(w[i], 0x00FF00FFu, 8, 2, j & 2);
-      w[i] = swap_parts(w[i], 0x0000FFFFu, 16, 4, j & 4);
-    }
-    const uint32_t give = j & 8 ? w[0] : w[1], got = __shfl_xor(give, 8);
+    const uint32_t got = lane_xor<8>(j & 8 ? w[0] : w[1]);
     w[0] = j & 8 ? got : w[0];
     w[1] = j & 8 ? w[1] : got;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      w[i] = swap_halves(w[i], lane_xor<4>(w[i]), j & 4);
+      w[i] = swap_bytes(w[i], lane_xor<2>(w[i]), j & 2);
+    }
   }
 }
 // The word (pair) that lane j of a row holds after transpose8
 __device__ __forceinline__ int word_of(int j) { return 8 * (j & 1) + (j >> 1); }
 
 // Quantises a row held by 16 lanes, lane j its elements 8 j .. 8 j + 7: word (pair) word_of(j) of its codes, and the
-// (s, m) pair of its group j / 4.  The quotient is the correctly rounded one of a division: q = d (1/s) and one
-// correction by its remainder.  held: the values that the codes stand for.
+// (s, m) pair of its group j / 4.  Quotients are a division's: q = d r with r about 1 / s, and one correction by the
+// remainder, which makes quotients that lie between two codes exact (others are 2^-16 and more away from there:
+// d and s have 16 and 8 significant bits, and the correction's error is 2^-40).  held: the values that the codes
+// stand for.
 template <int BITS>
 __device__ __forceinline__ void quant_row(const float (&x)[8], int j, uint32_t (&w)[BITS / 4], uint32_t &meta,
                                           float (&held)[8]) {
+  constexpr float L = top_code<BITS>(), kInvL = 1.f / L;
   float mn = min3_nan(min3_nan(x[0], x[1], x[2]), min3_nan(x[3], x[4], x[5]), min3_nan(x[6], x[7], x[7]));
   float mx = max3_nan(max3_nan(x[0], x[1], x[2]), max3_nan(x[3], x[4], x[5]), max3_nan(x[6], x[7], x[7]));
-#pragma unroll
-  for (int o = 1; o <= 2; o <<= 1) {
-    const float a = __shfl_xor(mn, o), b = __shfl_xor(mx, o);
-    mn = min3_nan(mn, a, a);
-    mx = max3_nan(mx, b, b);
-  }
+  float a = lane_xor<1>(mn), b = lane_xor<1>(mx);
+  mn = min3_nan(mn, a, a);
+  mx = max3_nan(mx, b, b);
+  a = lane_xor<2>(mn), b = lane_xor<2>(mx);
+  mn = min3_nan(mn, a, a);
+  mx = max3_nan(mx, b, b);
   const float span = mx - mn;
   const bool fine = span < INFINITY;             // neither NaN nor infinite
-  float s = (float)(__bf16)(span / top_code<BITS>());
+  float s = span * kInvL;
+  s = (float)(__bf16)fmaf(fmaf(-s, L, span), kInvL, s);
   s = s < kLeastStep ? 0.f : s;
-  const float inv = fine && s > 0.f ? 1.f / s : 0.f;
+  const float inv = fine && s > 0.f ? __builtin_amdgcn_rcpf(s) : 0.f;
   uint32_t c[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const float d = x[i] - mn;
     float q = d * inv;
     q = fmaf(fmaf(-q, s, d), inv, q);
-    q = fminf(fmaxf(rintf(q), 0.f), top_code<BITS>());   // (a NaN gives 0)
-    c[i] = (uint32_t)q;
-    held[i] = fine ? fmaf(q, s, mn) : NAN;
+    // (the step's rounding takes q to 15 (1 + 2^-8) at most, which rounds to 15, and to 256)
+    if constexpr (BITS == 8) q = fminf(q, L);
+    const float r = q + 0x1p23f;                 // rounded to a whole number, in its low bits
+    c[i] = __builtin_bit_cast(uint32_t, r);
+    held[i] = fine ? fmaf(r - 0x1p23f, s, mn) : NAN;
+  }
+  auto bytes = [](uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {   // their low bytes
+    return __builtin_amdgcn_perm(__builtin_amdgcn_perm(a3, a2, 0x0c0c0400u), __builtin_amdgcn_perm(a1, a0, 0x0c0c0400u),
+                                 0x05040100u);
+  };
+  if constexpr (BITS == 4) {
+    w[0] = bytes(c[0], c[2], c[4], c[6]) | (bytes(c[1], c[3], c[5], c[7]) << 4);
+  } else {
+    w[0] = bytes(c[0], c[1], c[2], c[3]);
+    w[1] = bytes(c[4], c[5], c[6], c[7]);
   }
 #pragma unroll
-  for (int k = 0; k < BITS / 4; ++k) {
-    w[k] = 0;
-#pragma unroll
-    for (int i = 0; i < 32 / BITS; ++i) w[k] |= c[k * (32 / BITS) + i] << (BITS * i);
-  }
+  for (int k = 0; k < BITS / 4; ++k) w[k] = fine ? w[k] : 0u;
   transpose8<BITS>(w, j);
   meta = fine ? pack_bf16x2(s, mn) : 0x7FC07FC0u;
 }
@@ -126,26 +167,40 @@ struct RowSource {
   int64_t rows;
   const int32_t *src_rows, *dst_rows;
 };
-// One (row, head, K or V) per 16 lanes.
+// A wave takes one head of K or V of 16 rows (kRows = 4 at a time: 4 rows of 16 lanes, 16 bytes each, all four
+// requested at once; their codes are stored as 256 contiguous bytes).  Blocks go by head first, so that the rows that
+// are read at one time are whole.
+constexpr int kRows = 4;
 template <int BITS>
-__global__ __launch_bounds__(256) void kv_quantize_kernel(RowSource a, QuantCache c, int64_t n) {
-  const int64_t t = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
-  const int j = threadIdx.x & 15, head = blockIdx.y;
-  const bool is_v = blockIdx.z;
-  if (t >= n) return;
-  const int64_t src = a.src_rows ? a.src_rows[t] : t, dst = a.dst_rows ? a.dst_rows[t] : t;
-  if (src < 0 || src >= a.rows || dst < 0 || dst >= c.rows) return;   // alike in the 16 lanes
-  const bf16_t *p = is_v ? a.v + src * a.v_rs + head * a.v_hs : a.k + src * a.k_rs + head * a.k_hs;
-  float x[8];
-  unpack8(ld16(p + 8 * j), x);
-  uint32_t w[BITS / 4], meta;
-  float held[8];
-  quant_row<BITS>(x, j, w, meta, held);
-  const int64_t row = head * c.head_rows + dst;
-  uint32_t *out = (is_v ? c.v : c.k) + row * row_words<BITS>() + word_of(j) * (BITS / 4);
+__global__ __launch_bounds__(256) void kv_quantize_kernel(RowSource a, QuantCache c, int64_t n, int heads) {
+  const int x = blockIdx.x % (2 * heads), head = x >> 1, j = threadIdx.x & 15;
+  const bool is_v = x & 1;
+  const int64_t t0 = ((int64_t)(blockIdx.x / (2 * heads)) * 4 + (threadIdx.x >> 6)) * (4 * kRows) + ((threadIdx.x >> 4) & 3);
+  int64_t dst[kRows];
+  u32x4 raw[kRows];
 #pragma unroll
-  for (int i = 0; i < BITS / 4; ++i) out[i] = w[i];
-  if ((j & 3) == 0) (is_v ? c.vm : c.km)[row * kGroups + (j >> 2)] = meta;
+  for (int r = 0; r < kRows; ++r) {              // alike in the 16 lanes
+    const int64_t t = t0 + 4 * r;
+    const bool in = t < n;
+    const int64_t src = in && a.src_rows ? a.src_rows[t] : t;
+    dst[r] = in && a.dst_rows ? a.dst_rows[t] : t;
+    const bool ok = in && src >= 0 && src < a.rows && dst[r] >= 0 && dst[r] < c.rows;
+    raw[r] = gload16((is_v ? a.v + src * a.v_rs + head * a.v_hs : a.k + src * a.k_rs + head * a.k_hs) + 8 * j, ok);
+    dst[r] = ok ? dst[r] : -1;
+  }
+#pragma unroll
+  for (int r = 0; r < kRows; ++r) {
+    float x[8], held[8];
+    unpack8(raw[r], x);
+    uint32_t w[BITS / 4], meta;
+    quant_row<BITS>(x, j, w, meta, held);
+    if (dst[r] < 0) continue;
+    const int64_t row = head * c.head_rows + dst[r];
+    uint32_t *out = (is_v ? c.v : c.k) + row * row_words<BITS>() + word_of(j) * (BITS / 4);
+    if constexpr (BITS == 4) *out = w[0];
+    else *reinterpret_cast<u32x2 *>(out) = u32x2{w[0], w[1]};
+    if ((j & 3) == 0) (is_v ? c.vm : c.km)[row * kGroups + (j >> 2)] = meta;
+  }
 }
 
 struct RowTarget {
@@ -154,22 +209,33 @@ struct RowTarget {
   const int32_t *rows;
 };
 template <int BITS>
-__global__ __launch_bounds__(256) void kv_dequantize_kernel(QuantCache c, RowTarget a, int64_t n) {
-  const int64_t t = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
-  const int j = threadIdx.x & 15, head = blockIdx.y;
-  const bool is_v = blockIdx.z;
-  if (t >= n) return;
-  const int64_t src = a.rows ? a.rows[t] : t;
-  float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  if (src >= 0 && src < c.rows) {
-    const int64_t row = head * c.head_rows + src;
-    const uint32_t *in = (is_v ? c.v : c.k) + row * row_words<BITS>() + word_of(j) * (BITS / 4);
-    uint32_t w[BITS / 4];
+__global__ __launch_bounds__(256) void kv_dequantize_kernel(QuantCache c, RowTarget a, int64_t n, int heads) {
+  const int x = blockIdx.x % (2 * heads), head = x >> 1, j = threadIdx.x & 15;
+  const bool is_v = x & 1;
+  const int64_t t0 = ((int64_t)(blockIdx.x / (2 * heads)) * 4 + (threadIdx.x >> 6)) * (4 * kRows) + ((threadIdx.x >> 4) & 3);
+  uint32_t w[kRows][BITS / 4], meta[kRows];
 #pragma unroll
-    for (int i = 0; i < BITS / 4; ++i) w[i] = in[i];
-    read_row<BITS>(w, (is_v ? c.vm : c.km)[row * kGroups + (j >> 2)], j, x);
+  for (int r = 0; r < kRows; ++r) {
+    const int64_t t = t0 + 4 * r, src = t < n && a.rows ? a.rows[t] : t;
+    const bool ok = t < n && src >= 0 && src < c.rows;
+    const int64_t row = head * c.head_rows + (ok ? src : 0);
+#pragma unroll
+    for (int i = 0; i < BITS / 4; ++i) w[r][i] = 0;
+    meta[r] = 0;
+    if (ok) {
+      const uint32_t *in = (is_v ? c.v : c.k) + row * row_words<BITS>() + word_of(j) * (BITS / 4);
+#pragma unroll
+      for (int i = 0; i < BITS / 4; ++i) w[r][i] = in[i];
+      meta[r] = (is_v ? c.vm : c.km)[row * kGroups + (j >> 2)];
+    }
   }
-  st16((is_v ? a.v + t * a.v_rs + head * a.v_hs : a.k + t * a.k_rs + head * a.k_hs) + 8 * j, pack8(x));
+#pragma unroll
+  for (int r = 0; r < kRows; ++r) {
+    const int64_t t = t0 + 4 * r;
+    float x[8];
+    read_row<BITS>(w[r], meta[r], j, x);
+    if (t < n) st16((is_v ? a.v + t * a.v_rs + head * a.v_hs : a.k + t * a.k_rs + head * a.k_hs) + 8 * j, pack8(x));
+  }
 }
 
 // ---- attention of a decode step ---------------------------------------------------------------------
@@ -233,11 +299,6 @@ __device__ __forceinline__ T ld_agent(const T *p) { return __hip_atomic_load(p, 
 // register too early, as the compiler keeps the wait that such a pair needs from its own instructions only.)
 extern "C" __device__ float tg_fmul_legacy(float, float) __asm("llvm.amdgcn.fmul.legacy");
 __device__ __forceinline__ float mul_zero(float a, float b) { return tg_fmul_legacy(a, b); }
-template <int CTRL>
-__device__ __forceinline__ float dpp(float x) {
-  const int i = __builtin_bit_cast(int, x);
-  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(i, i, CTRL, 0xf, 0xf, true));
-}
 __device__ __forceinline__ float wave_max(float x) {
   x = fmaxf(x, dpp<0xB1>(x));    // quad_perm 1 0 3 2
   x = fmaxf(x, dpp<0x4E>(x));    // quad_perm 2 3 0 1
@@ -814,10 +875,12 @@ int check_cache(const char *what, int32_t num_heads_k, int32_t head_dim, int32_t
   c->head_rows = head_rows;
   return 0;
 }
+// workgroups of the row kernels: 16 rows per wave
+int64_t row_blocks(int64_t n_rows, int heads) { return (n_rows + 16 * kRows - 1) / (16 * kRows) * 2 * heads; }
 int check_rows(const char *what, const void *k, int64_t k_rs, int64_t k_hs, const void *v, int64_t v_rs, int64_t v_hs,
-               int64_t n_rows) {
+               int64_t n_rows, int heads) {
   TG_CHECK(k && v, "%s: null row pointer", what);
-  TG_CHECK(n_rows >= 0 && (n_rows + 15) / 16 < (1ll << 31), "%s: bad row count", what);
+  TG_CHECK(n_rows >= 0 && n_rows < (1ll << 31) && row_blocks(n_rows, heads) < (1ll << 31), "%s: bad row count", what);
   TG_CHECK(k_rs >= 0 && v_rs >= 0 && k_hs >= kHeadDim && v_hs >= kHeadDim && k_rs % 8 == 0 && v_rs % 8 == 0 &&
                k_hs % 8 == 0 && v_hs % 8 == 0,
            "%s: strides must be multiples of 8 elements, head strides at least 128", what);
@@ -839,15 +902,15 @@ extern "C" int tg_kv_quantize(const void *k, int64_t k_row_stride, int64_t k_hea
   QuantCache c;
   if (int e = check_cache("kv_quantize", num_heads_k, head_dim, bits, k_codes, k_meta, v_codes, v_meta, cache_rows, head_rows, &c))
     return e;
-  if (int e = check_rows("kv_quantize", k, k_row_stride, k_head_stride, v, v_row_stride, v_head_stride, n_rows)) return e;
+  if (int e = check_rows("kv_quantize", k, k_row_stride, k_head_stride, v, v_row_stride, v_head_stride, n_rows, num_heads_k)) return e;
   TG_CHECK(source_rows >= 0 && (src_rows || n_rows <= source_rows), "kv_quantize: more rows than the source holds");
   TG_CHECK(dst_rows || n_rows <= cache_rows, "kv_quantize: more rows than the cache holds");
   if (n_rows == 0) return 0;
   const RowSource a{static_cast<const bf16_t *>(k), static_cast<const bf16_t *>(v), k_row_stride, k_head_stride,
                     v_row_stride, v_head_stride, source_rows, src_rows, dst_rows};
-  const dim3 grid((unsigned)((n_rows + 15) / 16), (unsigned)num_heads_k, 2), block(256);
-  if (bits == 4) hipLaunchKernelGGL(kv_quantize_kernel<4>, grid, block, 0, stream, a, c, n_rows);
-  else hipLaunchKernelGGL(kv_quantize_kernel<8>, grid, block, 0, stream, a, c, n_rows);
+  const dim3 grid((unsigned)row_blocks(n_rows, num_heads_k)), block(256);
+  if (bits == 4) hipLaunchKernelGGL(kv_quantize_kernel<4>, grid, block, 0, stream, a, c, n_rows, num_heads_k);
+  else hipLaunchKernelGGL(kv_quantize_kernel<8>, grid, block, 0, stream, a, c, n_rows, num_heads_k);
   TG_HIP_CHECK(hipGetLastError());
   return 0;
 }
@@ -861,15 +924,15 @@ extern "C" int tg_kv_dequantize(const void *k_codes, const void *k_meta, const v
   QuantCache c;
   if (int e = check_cache("kv_dequantize", num_heads_k, head_dim, bits, k_codes, k_meta, v_codes, v_meta, cache_rows, head_rows, &c))
     return e;
-  if (int e = check_rows("kv_dequantize", k_out, k_row_stride, k_head_stride, v_out, v_row_stride, v_head_stride, n_rows))
+  if (int e = check_rows("kv_dequantize", k_out, k_row_stride, k_head_stride, v_out, v_row_stride, v_head_stride, n_rows, num_heads_k))
     return e;
   TG_CHECK(rows || n_rows <= cache_rows, "kv_dequantize: more rows than the cache holds");
   if (n_rows == 0) return 0;
   const RowTarget a{static_cast<bf16_t *>(k_out), static_cast<bf16_t *>(v_out), k_row_stride, k_head_stride, v_row_stride,
                     v_head_stride, rows};
-  const dim3 grid((unsigned)((n_rows + 15) / 16), (unsigned)num_heads_k, 2), block(256);
-  if (bits == 4) hipLaunchKernelGGL(kv_dequantize_kernel<4>, grid, block, 0, stream, c, a, n_rows);
-  else hipLaunchKernelGGL(kv_dequantize_kernel<8>, grid, block, 0, stream, c, a, n_rows);
+  const dim3 grid((unsigned)row_blocks(n_rows, num_heads_k)), block(256);
+  if (bits == 4) hipLaunchKernelGGL(kv_dequantize_kernel<4>, grid, block, 0, stream, c, a, n_rows, num_heads_k);
+  else hipLaunchKernelGGL(kv_dequantize_kernel<8>, grid, block, 0, stream, c, a, n_rows, num_heads_k);
   TG_HIP_CHECK(hipGetLastError());
   return 0;
 }
