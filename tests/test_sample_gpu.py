@@ -67,7 +67,7 @@ def logits(n, v, seed, bf16=True, std=2.0):
     return x.bfloat16().float() if bf16 else x
 
 
-@pytest.mark.parametrize("n,v,bf16", [(1, 1, True), (3, 2, True), (5, 7, False), (4, 255, True), (2, 1023, False), (3, 1024, True),
+@pytest.mark.parametrize("n,v,bf16", [(1, 1, True), (3, 2, True), (5, 7, False), (4, 255, True), (2, 1023, False), (3, 1024, True), (2, 8192, True), (3, 8193, False),
                                       (2, 4097, True), (7, 32001, False), (3, 151936, True), (2, 151935, False), (1, 262144, True)])
 def test_sizes(cuda, n, v, bf16):
     """Odd sizes (rows that start at any 4-byte address), bf16 logits (many ties) and fp32 ones, all settings."""
@@ -100,6 +100,41 @@ def test_defaults_and_ends(cuda):
     assert torch.equal(tok.cpu(), x.argmax(1))
     tok, _, _ = check(cuda, x, [1.0] * 4, [1.0] * 4, None, None, None)
     assert bool((tok < 100).all())
+
+
+@pytest.mark.parametrize("v", [151936, 20001])
+def test_flat_and_wide_rows(cuda, v):
+    """Rows whose deciding bins hold more elements than are sorted (all equal, two values, nearly flat, high
+    temperatures), rows with most of their mass far below their largest logit, and ones spread over all floats."""
+    g = torch.Generator().manual_seed(v)
+    x = torch.randn(10, v, generator=g)
+    x[0] = 0.25
+    x[1] = (torch.arange(v) % 3 == 0).float()
+    x[2] *= 0.01
+    x[3] = x[3] * 2 - 60
+    x[3, 77] = 3.0                                      # 1e-24 of the mass below it, and at temperature 5 much more
+    x[4] = -40 + 0.1 * x[4]
+    x[4, 5], x[4, 9] = 6.0, 5.9
+    x[5] = torch.linspace(-3e38, 3e38, v)
+    x[6] = x[6] * 1e-30
+    x[7, v // 2:] = -float("inf")
+    x[8] = -float("inf")
+    x[9, 1::2] = float("inf")
+    rng = np.random.default_rng(v)
+    near = 0
+    for t, k, p, m in ((1.0, 0, 1.0, 0.0), (5.0, 0, 1.0, 0.0), (0.01, 0, 0.9, 0.0), (1.0, v // 2, 0.9, 0.0), (5.0, v - 7, 0.99, 1e-9),
+                       (40.0, 0, 0.5, 0.3), (1.0, 9000, 1.0, 0.9), (0.0, 0, 1.0, 0.0), (300.0, 0, 0.999, 0.001)):
+        near += check(cuda, x, list(rng.random(10, dtype=np.float32)), [t] * 10, [k] * 10, [p] * 10, [m] * 10)[2]
+    # (half the mass of an even number of equal weights lies on a border: v // 2 of them in row 9, v in row 0 and, but
+    # for 1e-30, in row 6)
+    assert v // 2 % 2 == 0 and near <= (3 if v % 2 == 0 else 1)
+
+
+def test_more_rows_than_a_launch(cuda):
+    rng = np.random.default_rng(1)
+    n = 300
+    near = check(cuda, logits(n, 9000, 2), list(rng.random(n, dtype=np.float32)), [1.0] * n, [50] * n, [0.9] * n, None)[2]
+    assert near == 0
 
 
 def test_odd_values(cuda):

@@ -3,17 +3,32 @@
 // With w_i = exp((x_i - max x) / T) and the order "larger logits first, equal ones by index": S1 = the first k;
 // S2 = the shortest beginning of S1 whose mass (sum of w) is at least top_p times S1's, one at least; S3 = those
 // of S2 with w >= min_p, one at least; the token is the first of S3 whose cumulated mass exceeds u times S3's, and
-// its log probability is ln(w / mass(S3)).  Every set is a beginning of the same order, so nothing is sorted: the
-// element at which a count or a mass is reached is found by its bits, most significant digit first.  Masses are
-// whole numbers (units of 2^-44): their sums are exact and the same in any order.
+// its log probability is ln(w / mass(S3)).  Every set is a beginning of the same order, so the row is not sorted:
+//   * sample_hist_kernel, several workgroups per row: logits in units of y = cc x (cc = 8 log2 e, or 4 log2 e / T for
+//     T < 0.5) fall into bins of width one, 512 from the chunk's largest down.  A bin's count and the sum of its
+//     elements' e^t, t = (the fraction of y - 1/2) T-scaled, need no common maximum, and as whole numbers (one 64-bit
+//     LDS addition per logit) no order of additions.  The workgroup that arrives last merges the row's bins and finds
+//     those in which the ends of S1, S2, S3 and the token must lie;
+//   * sample_pick_kernel collects the elements of these bins (some hundred), and the last workgroup sorts them and
+//     walks them with the masses of the bins above.
+// Rows of up to 8192 logits take one workgroup and one launch, which sorts them all.  Where the bins hold more than
+// 8192 elements (flat rows), the last workgroup finds the places digit by digit over the whole row instead.
+// Double throughout: a row has so many borders between tokens that sums good to 2^-24 would move one row in a hundred
+// across one; here they are good to 2^-36.
+// Bound by latency (two launches, two merges) for few rows and by the exponentials and LDS additions for many.
+#include <algorithm>
+
 #include "tg_common.h"
 #include "../../include/tokengate_hip.h"
 
 namespace tg {
 namespace {
 
-constexpr double kMassUnit = 0x1p44;
-constexpr double kLog2e = 1.4426950408889634;
+constexpr double kLog2e = 1.4426950408889634, kLn2 = 0.6931471805599453;
+constexpr int kThreads = 1024;
+constexpr int kBins = 512;
+constexpr int kList = 8192;                      // elements that one workgroup sorts
+constexpr int kRowsPerLaunch = 256;
 
 struct SampleArgs {
   const float *x;
@@ -25,33 +40,500 @@ struct SampleArgs {
   float *logprob;
 };
 
+// One workgroup's bins
+struct Part {
+  double top;                                    // bin 0 holds y in [top, top + 1)
+  uint64_t tail;                                 // mass below the bins, in units of 2^-44 of 2^(top / q)
+  uint32_t best, tail_count;                     // order bits of the largest logit
+  uint64_t hist[kBins];                          // count << 48 | sum of (e^t - 0.9) 2^36
+};
+// What the first launch leaves for the second, per row
+struct State {
+  double top, mass, m_mass;                      // of the row's bins; mass of the whole row; as Walk's
+  uint64_t mask[kBins / 64];                     // bins to collect
+  uint32_t best, slow, m_bin, pad;
+  uint32_t before_count[kBins];                  // of bin j: elements above it, less those of collected bins
+  double before_mass[kBins];                     // and masses
+};
+struct Counters {
+  uint32_t hist, pick, listed, pad;              // zero between launches
+};
+
+template <typename T>
+__device__ __forceinline__ void st_agent(T *p, T v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+template <typename T>
+__device__ __forceinline__ T ld_agent(const T *p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ uint64_t bits_of(double x) { return __builtin_bit_cast(uint64_t, x); }
+__device__ __forceinline__ double double_of(uint64_t x) { return __builtin_bit_cast(double, x); }
+
 // Order-preserving bits of a float: larger floats, larger numbers; NaN is -inf, -0 is 0.
 __device__ __forceinline__ uint32_t order_bits(float x) {
   x = x != x ? -INFINITY : x + 0.f;
   const uint32_t b = __builtin_bit_cast(uint32_t, x);
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
-__device__ __forceinline__ float order_float(uint32_t o) {
-  return u32_as_f32(o & 0x80000000u ? o & 0x7fffffffu : ~o);
+__device__ __forceinline__ float order_float(uint32_t o) { return u32_as_f32(o & 0x80000000u ? o & 0x7fffffffu : ~o); }
+constexpr uint32_t kNone = 0x007FFFFFu;          // order bits of -inf
+
+// A row's settings.  Bins per octave of w: q; y = cc x.
+struct Row {
+  double q, cc;
+  float temp;
+  bool greedy;
+  __device__ Row(const SampleArgs &a, int b) {
+    const float t = a.temperature ? a.temperature[b] : 1.f;
+    greedy = !(t > 0.f);
+    temp = greedy ? 1.f : t;
+    q = fmax(4.0, 8.0 * (double)temp);
+    cc = q * kLog2e / (double)temp;
+  }
+  // (+inf: so far above every finite one that those weigh nothing)
+  __device__ double y(float x) const { return x == INFINITY ? 0x1p1000 : (double)x * cc; }
+  __device__ double weight(double y, double top) const { return exp2((y - top) / q); }
+};
+
+// e^t for |t| <= 0.087, to 2^-49
+__device__ __forceinline__ double exp_small(double t) {
+  double p = 1.0 / 40320;
+  p = fma(p, t, 1.0 / 5040);
+  p = fma(p, t, 1.0 / 720);
+  p = fma(p, t, 1.0 / 120);
+  p = fma(p, t, 1.0 / 24);
+  p = fma(p, t, 1.0 / 6);
+  p = fma(p, t, 0.5);
+  p = fma(p, t, 1.0);
+  return fma(p, t, 1.0);
 }
-// exp((x - top) / T) for x <= top, scale = log2(e) / T; in units of 2^-44.  Double: a row has so many borders
-// between tokens that sums good to 2^-24 would move one row in a hundred across one.
-__device__ __forceinline__ double weight_of(float x, float top, double scale) {
-  return x == top ? 1.0 : exp2(((double)x - (double)top) * scale);   // (both may be infinite)
+constexpr double kHistBase = 0.9, kHistUnit = 0x1p36;
+
+__device__ __forceinline__ uint32_t block_max(uint32_t v, uint32_t *tmp) {   // tmp: 16 words
+  const int tid = threadIdx.x;
+#pragma unroll
+  for (int o = 32; o; o >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o));
+  __syncthreads();
+  if ((tid & 63) == 0) tmp[tid >> 6] = v;
+  __syncthreads();
+  v = tmp[tid & 15];
+#pragma unroll
+  for (int o = 8; o; o >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o));
+  return v;
 }
-__device__ __forceinline__ uint64_t mass_of(float x, float top, double scale) {
-  return (uint64_t)(weight_of(x, top, scale) * kMassUnit + 0.5);
+// Sums over the threads up to this one; total: over all.  tmp: 16 of T.
+template <typename T>
+__device__ __forceinline__ T block_scan(T v, T *tmp, T &total) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const T y = __shfl_up(v, o);
+    v += lane >= o ? y : T(0);
+  }
+  __syncthreads();
+  if (lane == 63) tmp[wave] = v;
+  __syncthreads();
+  T s = lane < 16 ? tmp[lane] : T(0);
+#pragma unroll
+  for (int o = 1; o < 16; o <<= 1) {
+    const T y = __shfl_up(s, o);
+    s += lane >= o ? y : T(0);
+  }
+  total = __shfl(s, 15);
+  return v + (wave ? __shfl(s, wave - 1) : T(0));
 }
 
+// ---- the elements of one list, in order ----------------------------------------------------------------
+// list: n <= kList entries (~order bits) << 32 | index; ascending is the row's order.
+__device__ __forceinline__ int sort_list(uint64_t *list, int n) {
+  const int tid = threadIdx.x;
+  int size = 64;
+  while (size < n) size *= 2;
+  for (int i = n + tid; i < size; i += kThreads) list[i] = ~0ull;
+  for (int k = 2; k <= size; k *= 2)
+    for (int j = k / 2; j >= 1; j /= 2) {
+      __syncthreads();
+      for (int i = tid; i < size / 2; i += kThreads) {
+        const int lo = 2 * i - (i & (j - 1)), hi = lo + j;
+        const uint64_t a = list[lo], b = list[hi];
+        if ((a > b) == ((lo & k) == 0)) {
+          list[lo] = b;
+          list[hi] = a;
+        }
+      }
+    }
+  __syncthreads();
+  return size;
+}
+
+// What comes before an element of the list that is not in it: counts and masses by bin (null: the list is the whole
+// row).
+struct Walk {
+  double top, mass;                              // unit of the masses: 2^(top / q); mass of the row
+  const uint32_t *before_count;
+  const double *before_mass;
+  int m_bin;                                     // the last bin that may hold min_p's end
+  double m_mass;                                 // mass up to and with it
+};
+struct WalkShared {
+  double scan[16], end_mass[3];                  // of S1, of S2 and of min_p alone
+  uint32_t place, last;
+};
+__device__ void finish_row(const SampleArgs &a, int b, const Row &row, uint64_t *list, int n, const Walk &w, uint32_t best,
+                           WalkShared &sh) {
+  const int tid = threadIdx.x;
+  const int size = sort_list(list, n), per = (size + kThreads - 1) / kThreads;   // per thread, in order
+  if (row.greedy || best == kNone) {
+    if (tid == 0) {
+      a.token[b] = (uint32_t)list[0];
+      if (a.logprob) a.logprob[b] = 0.f;
+    }
+    return;
+  }
+  constexpr int kPer = kList / kThreads;
+  double wt[kPer], cum[kPer], sum = 0.0;
+  uint32_t rank[kPer];
+  const double y_best = row.y(order_float(best));
+#pragma unroll
+  for (int r = 0; r < kPer; ++r) {
+    const int i = tid * per + r;
+    wt[r] = 0.0;
+    if (r < per && i < n) {
+      const float x = order_float(~(uint32_t)(list[i] >> 32));
+      wt[r] = x == -INFINITY ? 0.0 : row.weight(row.y(x), w.top);
+    }
+    sum += wt[r];
+  }
+  double total;
+  double before = block_scan(sum, sh.scan, total) - sum;
+#pragma unroll
+  for (int r = 0; r < kPer; ++r) {
+    const int i = tid * per + r;
+    before += wt[r];
+    cum[r] = before;
+    rank[r] = i + 1;
+    if (w.before_count && r < per && i < n) {
+      const double bin = w.top - floor(row.y(order_float(~(uint32_t)(list[i] >> 32))));
+      const int j = (int)bin;
+      cum[r] += w.before_mass[j];
+      rank[r] += w.before_count[j];
+    }
+  }
+  auto each = [&](auto f) {
+#pragma unroll
+    for (int r = 0; r < kPer; ++r)
+      if (r < per && tid * per + r < n) f(tid * per + r, r);
+  };
+  const double mass = w.before_count ? w.mass : total;
+  const uint32_t k = a.top_k && a.top_k[b] > 0 && a.top_k[b] < a.n ? (uint32_t)a.top_k[b] : 0xffffffffu;
+  const float tp = a.top_p ? a.top_p[b] : 1.f, mp = a.min_p ? a.min_p[b] : 0.f;
+  // (the sets are beginnings of one order, so the shortest is the one of the least mass)
+  if (tid == 0) {
+    sh.end_mass[0] = sh.end_mass[1] = sh.end_mass[2] = mass;
+    sh.place = sh.last = 0xffffffffu;
+  }
+  __syncthreads();
+  each([&](int, int r) {
+    if (rank[r] == k) sh.end_mass[0] = cum[r];
+  });
+  __syncthreads();
+  if (tp < 1.f) {
+    const double target = (double)fmaxf(tp, 0.f) * sh.end_mass[0];
+    each([&](int i, int r) {
+      if (cum[r] >= target) atomicMin(&sh.place, (uint32_t)i);
+    });
+    __syncthreads();
+    each([&](int i, int r) {
+      if ((uint32_t)i == sh.place) sh.end_mass[1] = cum[r];
+    });
+  }
+  if (mp > 0.f) {
+    const double least = fmin((double)mp, 1.0);
+    // (weights of the largest logit's are 1 in any case)
+    each([&](int i, int r) {
+      const float x = order_float(~(uint32_t)(list[i] >> 32));
+      const bool under = x != order_float(best) && (x == -INFINITY || exp2((row.y(x) - y_best) / row.q) < least);
+      if (under && (!w.before_count || w.top - floor(row.y(x)) <= w.m_bin)) atomicMin(&sh.last, (uint32_t)i);
+    });
+    __syncthreads();
+    const uint32_t first = sh.last;
+    if (first == 0xffffffffu) {                  // every element of those bins reaches it
+      if (tid == 0 && w.before_count) sh.end_mass[2] = w.m_mass;
+    } else {
+      each([&](int i, int r) {
+        if ((uint32_t)i == first) sh.end_mass[2] = cum[r] - wt[r];
+      });
+    }
+  }
+  __syncthreads();
+  const double s3 = fmin(fmin(sh.end_mass[0], sh.end_mass[1]), sh.end_mass[2]);
+  const double target = fmin(fmax((double)a.u[b], 0.0), 1.0) * s3;
+  if (tid == 0) {
+    sh.place = 0xffffffffu;
+    sh.last = 0;
+  }
+  __syncthreads();
+  each([&](int i, int r) {
+    if (cum[r] > target && wt[r] > 0.0) atomicMin(&sh.place, (uint32_t)i);
+    if (wt[r] > 0.0 && cum[r] <= s3) atomicMax(&sh.last, (uint32_t)i);   // u = 1: the last with a weight
+  });
+  __syncthreads();
+  const uint32_t at = min(sh.place, sh.last);
+  each([&](int i, int r) {
+    if ((uint32_t)i == at) {
+      a.token[b] = (uint32_t)list[i];
+      if (a.logprob) a.logprob[b] = (float)log(wt[r] / s3);
+    }
+  });
+}
+
+// ---- rows of up to kList logits --------------------------------------------------------------------------
+__global__ __launch_bounds__(kThreads) void sample_small_kernel(SampleArgs a) {
+  __shared__ uint64_t list[kList];
+  __shared__ uint32_t tmp[16];
+  __shared__ WalkShared sh;
+  const int b = blockIdx.x, tid = threadIdx.x;
+  const float *x = a.x + b * a.rs;
+  const Row row(a, b);
+  uint32_t best = 0;
+  for (int i = tid; i < a.n; i += kThreads) {
+    const uint32_t key = order_bits(x[i]);
+    list[i] = (uint64_t)~key << 32 | (uint32_t)i;
+    best = max(best, key);
+  }
+  best = block_max(best, tmp);
+  Walk w{};
+  w.top = best == kNone ? 0.0 : row.y(order_float(best));
+  finish_row(a, b, row, list, a.n, w, best, sh);
+}
+
+// ---- longer rows -------------------------------------------------------------------------------------------
+struct SampleWork {
+  Counters *counters;                            // per row
+  State *states;
+  uint64_t *lists;                               // kList per row
+  Part *parts;                                   // gridDim.x per row
+};
+
+template <int E>
+__global__ __launch_bounds__(kThreads) void sample_hist_kernel(SampleArgs a, SampleWork ws) {
+  const int b = blockIdx.y, g = blockIdx.x, parts = gridDim.x, tid = threadIdx.x;
+  const float *x = a.x + b * a.rs;
+  __shared__ uint64_t hist[kBins];
+  __shared__ uint32_t tmp[16];
+  __shared__ unsigned long long tail_s;
+  __shared__ uint32_t last_s;
+  float v[E];
+  uint32_t best = kNone;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const int i = (g * E + e) * kThreads + tid;
+    v[e] = i < a.n ? x[i] : -INFINITY;
+    best = max(best, order_bits(v[e]));
+  }
+  const Row row(a, b);
+  if (tid < kBins) hist[tid] = 0;
+  if (tid == 0) tail_s = 0;
+  best = block_max(best, tmp);                   // (its barriers cover the bins)
+  const double top = best == kNone ? 0.0 : floor(row.y(order_float(best)));
+  const double scale = kLn2 / row.q;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    if (!(v[e] > -INFINITY)) continue;
+    const double y = row.y(v[e]), f = floor(y), j = top - f;
+    if (j < kBins) {
+      const double t = (y - f - 0.5) * scale;
+      atomicAdd((unsigned long long *)&hist[(int)j], (1ull << 48) + (unsigned long long)((exp_small(t) - kHistBase) * kHistUnit + 0.5));
+    } else {
+      const double w = row.weight(y, top);
+      if (w > 0x1p-46) atomicAdd(&tail_s, (unsigned long long)(w * 0x1p44 + 0.5));
+    }
+  }
+  __syncthreads();
+  Part *const part = ws.parts + (int64_t)b * parts;
+  if (tid < kBins) st_agent(&part[g].hist[tid], hist[tid]);
+  if (tid == 0) {
+    st_agent((uint64_t *)&part[g].top, bits_of(top));
+    st_agent(&part[g].tail, (uint64_t)tail_s);
+    st_agent(&part[g].best, best);
+  }
+  wait_all_mem();
+  __syncthreads();
+  if (tid == 0)
+    last_s = __hip_atomic_fetch_add(&ws.counters[b].hist, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)parts - 1u;
+  __syncthreads();
+  if (!last_s) return;
+
+  // ---- the row's bins ----
+  __shared__ double tops[64], mass_s[kBins], scan_d[16], edge_s[4];
+  __shared__ uint64_t sums[kBins];
+  __shared__ uint32_t counts[kBins], count_s[kBins], scan_u[16], bests[64];
+  __shared__ int first_s[4];
+  if (tid < parts) {
+    tops[tid] = double_of(ld_agent((const uint64_t *)&part[tid].top));
+    bests[tid] = ld_agent(&part[tid].best);
+  }
+  __syncthreads();
+  best = kNone;
+  for (int i = 0; i < parts; ++i) best = max(best, bests[i]);
+  State *const st = ws.states + b;
+  if (best == kNone) {                           // nothing but -inf: token 0, by the slow way
+    if (tid == 0) {
+      st->slow = 1;
+      for (int i = 0; i < kBins / 64; ++i) st->mask[i] = 0;
+      st_agent(&ws.counters[b].hist, 0u);
+    }
+    return;
+  }
+  const double gtop = floor(row.y(order_float(best)));
+  const int j = tid & (kBins - 1), half = tid / kBins;
+  uint64_t sum = 0;
+  uint32_t count = 0;
+  double tail = 0.0;
+  constexpr int kAhead = 8;
+  for (int i0 = half; i0 < parts; i0 += 2 * kAhead) {
+    uint64_t h[kAhead];
+#pragma unroll
+    for (int r = 0; r < kAhead; ++r) {
+      const int i = min(i0 + 2 * r, parts - 1);
+      h[r] = ld_agent(&part[i].hist[j]);         // of the part's bin j
+    }
+#pragma unroll
+    for (int r = 0; r < kAhead; ++r) {
+      const int i = i0 + 2 * r;
+      if (i >= parts || bests[i] == kNone) continue;
+      const double off = gtop - tops[i];
+      if (h[r] && off + j >= kBins)
+        tail += exp2((0.5 - off - j) / row.q) * (kHistBase * (double)(h[r] >> 48) + (double)(h[r] & 0xffffffffffffull) / kHistUnit);
+    }
+  }
+  __syncthreads();
+  // (two passes: a part's bin j is the row's bin j + off, and reads of the same lines are cached by then)
+  for (int i0 = half; i0 < parts; i0 += 2 * kAhead) {
+    uint64_t h[kAhead];
+#pragma unroll
+    for (int r = 0; r < kAhead; ++r) {
+      const int i = min(i0 + 2 * r, parts - 1);
+      const double off = gtop - tops[i];
+      const int at = off <= (double)j ? j - (int)off : -1;
+      h[r] = at >= 0 && i0 + 2 * r < parts && bests[i] != kNone ? ld_agent(&part[i].hist[at]) : 0;
+    }
+#pragma unroll
+    for (int r = 0; r < kAhead; ++r) {
+      count += (uint32_t)(h[r] >> 48);
+      sum += h[r] & 0xffffffffffffull;
+    }
+  }
+  if (tid < parts && bests[tid] != kNone) tail += exp2((tops[tid] - gtop) / row.q) * ((double)ld_agent(&part[tid].tail) * 0x1p-44);
+  if (half == 1) {
+    sums[j] = sum;
+    counts[j] = count;
+  }
+  __syncthreads();
+  double m = 0.0;
+  if (half == 0) {
+    sum += sums[j];
+    count += counts[j];
+    m = exp2((0.5 - j) / row.q) * (kHistBase * (double)count + (double)sum / kHistUnit);
+  } else {
+    count = 0;
+  }
+  double in_bins, tail_all;
+  uint32_t n_bins;
+  const double upto = block_scan(m, scan_d, in_bins);
+  const uint32_t upto_count = block_scan(count, scan_u, n_bins);
+  block_scan(tail, scan_d, tail_all);
+  const double mass = in_bins + tail_all;
+  const bool tail_counts = tail_all > 0x1p-42 * mass;
+  if (half == 0) {
+    mass_s[j] = upto;
+    count_s[j] = upto_count;
+  }
+  if (tid < 4) first_s[tid] = kBins;
+  __syncthreads();
+  auto first_mass = [&](int slot, double target) {   // the first bin up to which the mass reaches target
+    if (half == 0 && upto >= target && (j == 0 || mass_s[j - 1] < target)) first_s[slot] = j;
+  };
+  constexpr double kEps = 0x1p-34;
+  const uint32_t k = row.greedy ? 1u : a.top_k && a.top_k[b] > 0 && a.top_k[b] < a.n ? (uint32_t)a.top_k[b] : 0u;
+  const float tp = a.top_p && !row.greedy ? a.top_p[b] : 1.f, mp = a.min_p && !row.greedy ? a.min_p[b] : 0.f;
+  bool slow = false;
+  if (half == 0 && k && upto_count >= k && (j == 0 || count_s[j - 1] < k)) first_s[0] = j;
+  __syncthreads();
+  const int k_bin = k ? first_s[0] : kBins;
+  double lo = mass, hi = mass;                   // bounds of S1's mass, then of S3's
+  if (k && k_bin < kBins) {
+    lo = k_bin ? mass_s[k_bin - 1] : 0.0;
+    hi = mass_s[k_bin];
+  } else if (k) {
+    lo = in_bins;
+    slow |= tail_counts;
+  }
+  const double p = fmax((double)tp, 0.0);
+  if (tp < 1.f) {
+    first_mass(1, p * lo * (1.0 - kEps));
+    first_mass(2, p * hi * (1.0 + kEps));
+  }
+  __syncthreads();
+  int p_lo = kBins, p_hi = kBins, m_lo = kBins, m_hi = kBins;
+  if (tp < 1.f) {
+    p_lo = min(first_s[1], kBins - 1);
+    p_hi = min(first_s[2], kBins - 1);
+    slow |= tail_counts && first_s[2] == kBins;
+    lo = fmin(lo, p_lo ? mass_s[p_lo - 1] : 0.0);
+    hi = fmin(hi, mass_s[p_hi]);
+  }
+  double m_mass = mass;
+  if (mp > 0.f) {
+    const double thr = row.y(order_float(best)) + row.q * log2(fmin((double)mp, 1.0)), d0 = gtop - floor(thr + 1e-6),
+                 d1 = gtop - floor(thr - 1e-6);
+    m_lo = d0 < 0.0 ? 0 : d0 < kBins ? (int)d0 : kBins;
+    m_hi = d1 < 0.0 ? 0 : d1 < kBins ? (int)d1 : kBins;
+    slow |= tail_counts && m_hi == kBins;
+    if (m_lo < kBins) lo = fmin(lo, m_lo ? mass_s[m_lo - 1] : 0.0);
+    if (m_hi < kBins) hi = fmin(hi, m_mass = mass_s[m_hi]);
+  }
+  const double u = fmin(fmax((double)a.u[b], 0.0), 1.0);
+  __syncthreads();
+  if (tid < 4) first_s[tid] = kBins;
+  __syncthreads();
+  first_mass(0, u * lo * (1.0 - kEps));
+  first_mass(1, u * hi * (1.0 + kEps));
+  __syncthreads();
+  int t_lo = min(first_s[0], kBins - 1), t_hi = min(first_s[1], kBins - 1);
+  slow |= tail_counts && first_s[1] == kBins;
+  if (row.greedy) t_lo = t_hi = 0;
+  auto in = [&](int lo_, int hi_) { return j >= lo_ && j <= hi_; };
+  const bool wanted = half == 0 && (j == k_bin || (tp < 1.f && in(p_lo, p_hi)) || (mp > 0.f && in(m_lo, min(m_hi, kBins - 1))) || in(t_lo, t_hi));
+  uint32_t listed;
+  double unused;
+  const uint32_t before_c = block_scan(wanted ? count : 0u, scan_u, listed);
+  const double before_m = block_scan(wanted ? m : 0.0, scan_d, unused);
+  slow |= listed > kList;
+  const uint64_t bits = __builtin_amdgcn_ballot_w64(wanted && !slow);
+  if (half == 0) {
+    st->before_count[j] = upto_count - before_c;
+    st->before_mass[j] = upto - before_m;
+    if ((tid & 63) == 0) st->mask[j >> 6] = bits;
+  }
+  if (tid == 0) {
+    st->top = gtop;
+    st->mass = mass;
+    st->m_mass = m_mass;
+    st->best = best;
+    st->slow = slow;
+    st->m_bin = (uint32_t)min(m_hi, kBins - 1);
+    st_agent(&ws.counters[b].hist, 0u);
+  }
+}
+// ---- a flat row: the places found digit by digit ----------------------------------------------------------
 // A place in the order: the elements above `key`, and the first `ties` of those equal to it.
 struct Place {
   uint32_t key;
   uint32_t ties;
   uint64_t above;   // count or mass of the elements above key
 };
-
-__global__ __launch_bounds__(1024) void sample_rows_kernel(SampleArgs a) {
-  const int b = blockIdx.x, tid = threadIdx.x;
+// Masses as whole numbers, in units of 2^-44 of the largest weight.
+__device__ void slow_row(const SampleArgs &a, int b) {
+  constexpr double kMassUnit = 0x1p44;
+  const int tid = threadIdx.x;
   const float *x = a.x + b * a.rs;
   __shared__ uint64_t hist[256], red[16];
   __shared__ uint32_t found;
@@ -65,13 +547,14 @@ __global__ __launch_bounds__(1024) void sample_rows_kernel(SampleArgs a) {
     return v;
   };
   uint32_t best = 0;
-  for (int i = tid; i < a.n; i += 1024) best = max(best, order_bits(x[i]));
+  for (int i = tid; i < a.n; i += kThreads) best = max(best, order_bits(x[i]));
   best = reduce_max(best);
   const float top = order_float(best);
   const float temp = a.temperature ? a.temperature[b] : 1.f;
   const bool greedy = !(temp > 0.f) || top == -INFINITY;
   const double scale = greedy ? 1.0 : kLog2e / temp;
-  auto mass = [&](uint32_t key) { return mass_of(order_float(key), top, scale); };
+  auto weight = [&](float x) { return x == top ? 1.0 : exp2(((double)x - (double)top) * scale); };   // (both may be infinite)
+  auto mass = [&](uint32_t key) { return (uint64_t)(weight(order_float(key)) * kMassUnit + 0.5); };
   // The first place at which the sum of value(key) over the elements up to it reaches target (> 0).
   auto find = [&](uint64_t target, bool by_mass) {
     uint32_t prefix = 0;
@@ -79,7 +562,7 @@ __global__ __launch_bounds__(1024) void sample_rows_kernel(SampleArgs a) {
     for (int shift = 24; shift >= 0; shift -= 8) {
       if (tid < 256) hist[tid] = 0;
       __syncthreads();
-      for (int i = tid; i < a.n; i += 1024) {
+      for (int i = tid; i < a.n; i += kThreads) {
         const uint32_t key = order_bits(x[i]);
         if (shift == 24 || (key >> (shift + 8)) == (prefix >> (shift + 8)))
           atomicAdd((unsigned long long *)&hist[(key >> shift) & 255], (unsigned long long)(by_mass ? mass(key) : 1));
@@ -103,7 +586,7 @@ __global__ __launch_bounds__(1024) void sample_rows_kernel(SampleArgs a) {
   };
   auto sum_mass = [&](Place p) {                 // of the elements of a place's beginning
     uint64_t s = 0;
-    for (int i = tid; i < a.n; i += 1024) {
+    for (int i = tid; i < a.n; i += kThreads) {
       const uint32_t key = order_bits(x[i]);
       if (key > p.key) s += mass(key);
     }
@@ -117,7 +600,7 @@ __global__ __launch_bounds__(1024) void sample_rows_kernel(SampleArgs a) {
   };
   auto index_of = [&](Place p) {                 // the ties-th element equal to key, by index
     uint32_t seen = 0;
-    for (int i0 = 0; i0 < a.n; i0 += 1024) {
+    for (int i0 = 0; i0 < a.n; i0 += kThreads) {
       const int i = i0 + tid;
       const bool eq = i < a.n && order_bits(x[i]) == p.key;
       const uint64_t m = __ballot(eq);
@@ -163,9 +646,9 @@ __global__ __launch_bounds__(1024) void sample_rows_kernel(SampleArgs a) {
     uint64_t s = 0;                              // mass of what reaches min_p (a beginning as well)
     const double least = fmin((double)mp, 1.0);
     uint32_t end = 0xffffffffu;
-    for (int i = tid; i < a.n; i += 1024) {
+    for (int i = tid; i < a.n; i += kThreads) {
       const uint32_t key = order_bits(x[i]);
-      if (weight_of(x[i], top, scale) >= least) end = min(end, key);
+      if (weight(order_float(key)) >= least) end = min(end, key);
     }
     end = ~reduce_max(~end);
     if (end > last.key) {
@@ -185,12 +668,106 @@ __global__ __launch_bounds__(1024) void sample_rows_kernel(SampleArgs a) {
   }
 }
 
+template <int E>
+__global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleArgs a, SampleWork ws) {
+  const int b = blockIdx.y, g = blockIdx.x, parts = gridDim.x, tid = threadIdx.x;
+  const State *const st = ws.states + b;
+  if (st->slow) {
+    if (g == 0) slow_row(a, b);
+    return;
+  }
+  __shared__ uint64_t list[kList];
+  __shared__ uint32_t n_s, base_s, last_s;
+  __shared__ WalkShared sh;
+  const float *x = a.x + b * a.rs;
+  float v[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const int i = (g * E + e) * kThreads + tid;
+    v[e] = i < a.n ? x[i] : -INFINITY;
+  }
+  const Row row(a, b);
+  uint64_t mask[kBins / 64];
+#pragma unroll
+  for (int i = 0; i < kBins / 64; ++i) mask[i] = st->mask[i];
+  const double top = st->top;
+  if (tid == 0) n_s = 0;
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    if (!(v[e] > -INFINITY)) continue;
+    const double j = top - floor(row.y(v[e]));
+    if (!(j < kBins)) continue;
+    const int bin = (int)j;
+    uint64_t m = mask[0];
+#pragma unroll
+    for (int i = 1; i < kBins / 64; ++i) m = bin >> 6 == i ? mask[i] : m;
+    if (m >> (bin & 63) & 1) {
+      const uint32_t at = atomicAdd(&n_s, 1u);   // (all collected bins together hold at most kList)
+      if (at < kList) list[at] = (uint64_t)~order_bits(v[e]) << 32 | (uint32_t)((g * E + e) * kThreads + tid);
+    }
+  }
+  __syncthreads();
+  uint64_t *const all = ws.lists + (int64_t)b * kList;
+  Counters *const c = ws.counters + b;
+  if (n_s > 0) {
+    if (tid == 0) base_s = __hip_atomic_fetch_add(&c->listed, n_s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    for (uint32_t i = tid; i < n_s && base_s + i < kList; i += kThreads) st_agent(all + base_s + i, list[i]);
+  }
+  wait_all_mem();
+  __syncthreads();
+  if (tid == 0)
+    last_s = __hip_atomic_fetch_add(&c->pick, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)parts - 1u;
+  __syncthreads();
+  if (!last_s) return;
+  const int n = (int)min(ld_agent(&c->listed), (uint32_t)kList);
+  for (int i = tid; i < n; i += kThreads) list[i] = ld_agent(all + i);
+  Walk w;
+  w.top = top;
+  w.mass = st->mass;
+  w.before_count = st->before_count;
+  w.before_mass = st->before_mass;
+  w.m_bin = (int)st->m_bin;
+  w.m_mass = st->m_mass;
+  __syncthreads();
+  if (tid == 0) {
+    st_agent(&c->listed, 0u);
+    st_agent(&c->pick, 0u);
+  }
+  finish_row(a, b, row, list, n, w, st->best, sh);
+}
+
+struct SamplePlan {
+  int parts, e;
+  int64_t states, lists, parts_at, bytes;        // byte offsets; the counters come first, for any launch
+};
+int sample_parts(int64_t n, int e) { return (int)((n + e * kThreads - 1) / (e * kThreads)); }
+// rows: of one launch.  4 logits per thread while that makes at most two workgroups per CU, else 16.
+SamplePlan plan_sample(int64_t rows, int64_t n) {
+  SamplePlan p;
+  p.e = rows * sample_parts(n, 4) <= 2 * device_cus() ? 4 : 16;
+  p.parts = sample_parts(n, p.e);
+  p.states = kRowsPerLaunch * sizeof(Counters);
+  p.lists = p.states + rows * (int64_t)sizeof(State);
+  p.parts_at = p.lists + rows * kList * 8;
+  p.bytes = p.parts_at + rows * p.parts * (int64_t)sizeof(Part);
+  return p;
+}
+
 }  // namespace
 }  // namespace tg
 
 using namespace tg;
 
-extern "C" int64_t tg_sample_rows_workspace_size(int32_t n_rows, int64_t n_cols) { return 0; }
+// (enough for fewer rows and columns: those may take 4 logits per thread, but then no more parts than two per CU)
+extern "C" int64_t tg_sample_rows_workspace_size(int32_t n_rows, int64_t n_cols) {
+  if (n_rows <= 0 || n_cols <= kList || n_cols > (1 << 18)) return 0;
+  const int64_t rows = std::min<int32_t>(n_rows, kRowsPerLaunch);
+  const int64_t parts = std::max(std::min<int64_t>(rows * sample_parts(n_cols, 4), 2 * device_cus()), rows * sample_parts(n_cols, 16));
+  const SamplePlan p = plan_sample(rows, n_cols);
+  return p.parts_at + parts * (int64_t)sizeof(Part);
+}
 
 extern "C" int tg_sample_rows(const float *x, int64_t x_row_stride, int32_t n_rows, int64_t n_cols, const float *u,
                               const float *temperature, const int32_t *top_k, const float *top_p, const float *min_p,
@@ -201,8 +778,33 @@ extern "C" int tg_sample_rows(const float *x, int64_t x_row_stride, int32_t n_ro
   TG_CHECK(n_rows >= 0 && n_rows < 65536 && n_cols > 0 && n_cols <= (1 << 18), "sample_rows: 0..65535 rows of 1..262144 columns");
   TG_CHECK(x_row_stride >= n_cols, "sample_rows: row stride must be >= n_cols");
   if (n_rows == 0) return 0;
-  const SampleArgs a{x, x_row_stride, (int)n_cols, u, temperature, top_p, min_p, top_k, token, logprob};
-  hipLaunchKernelGGL(sample_rows_kernel, dim3((unsigned)n_rows), dim3(1024), 0, stream, a);
-  TG_HIP_CHECK(hipGetLastError());
+  if (n_cols <= kList) {
+    const SampleArgs a{x, x_row_stride, (int)n_cols, u, temperature, top_p, min_p, top_k, token, logprob};
+    hipLaunchKernelGGL(sample_small_kernel, dim3((unsigned)n_rows), dim3(kThreads), 0, stream, a);
+    TG_HIP_CHECK(hipGetLastError());
+    return 0;
+  }
+  const int64_t need = plan_sample(std::min<int32_t>(n_rows, kRowsPerLaunch), n_cols).bytes;
+  TG_CHECK(workspace != nullptr && aligned16(workspace) && workspace_bytes >= need,
+           "sample_rows: needs a 16-byte aligned workspace of %lld bytes (got %lld)", (long long)need, (long long)workspace_bytes);
+  for (int32_t r0 = 0; r0 < n_rows; r0 += kRowsPerLaunch) {
+    const int32_t rows = std::min<int32_t>(n_rows - r0, kRowsPerLaunch);
+    auto at = [r0](auto *p) { return p ? p + r0 : p; };
+    const SampleArgs a{x + r0 * x_row_stride, x_row_stride, (int)n_cols, u + r0, at(temperature), at(top_p), at(min_p),
+                       at(top_k), token + r0, at(logprob)};
+    const SamplePlan p = plan_sample(rows, n_cols);
+    char *ws = static_cast<char *>(workspace);
+    const SampleWork w{reinterpret_cast<Counters *>(ws), reinterpret_cast<State *>(ws + p.states),
+                       reinterpret_cast<uint64_t *>(ws + p.lists), reinterpret_cast<Part *>(ws + p.parts_at)};
+    const dim3 grid((unsigned)p.parts, (unsigned)rows), block(kThreads);
+    if (p.e == 4) {
+      hipLaunchKernelGGL(sample_hist_kernel<4>, grid, block, 0, stream, a, w);
+      hipLaunchKernelGGL(sample_pick_kernel<4>, grid, block, 0, stream, a, w);
+    } else {
+      hipLaunchKernelGGL(sample_hist_kernel<16>, grid, block, 0, stream, a, w);
+      hipLaunchKernelGGL(sample_pick_kernel<16>, grid, block, 0, stream, a, w);
+    }
+    TG_HIP_CHECK(hipGetLastError());
+  }
   return 0;
 }

@@ -51,6 +51,10 @@ class QuantKV:
             raise RuntimeError("QuantKV: codes and meta must have the same rows between heads")
         if len({t.device for t in (self.k, self.v, self.k_meta, self.v_meta)}) != 1:
             raise RuntimeError("QuantKV: tensors on different devices")
+        # what every call passes on (the tensors of a cache are not replaced, resized or moved)
+        self.rows, self.n_kv_heads, self.device_index = rows, hkv, self.k.get_device()
+        self._args = (self.k.data_ptr(), self.k_meta.data_ptr(), self.v.data_ptr(), self.v_meta.data_ptr(), rows,
+                      self.head_rows)
 
     @staticmethod
     def alloc(rows: int, n_kv_heads: int, bits: int, device) -> "QuantKV":
@@ -62,36 +66,27 @@ class QuantKV:
         return QuantKV(bits, c[0], m[0], c[1], m[1])
 
     @property
-    def rows(self) -> int:
-        return self.k.shape[1]
-
-    @property
-    def n_kv_heads(self) -> int:
-        return self.k.shape[0]
-
-    @property
     def nbytes(self) -> int:
         return sum(t.numel() * t.element_size() for t in (self.k, self.k_meta, self.v, self.v_meta))
 
-    def _args(self):
-        return (self.k.data_ptr(), self.k_meta.data_ptr(), self.v.data_ptr(), self.v_meta.data_ptr(), self.rows,
-                self.head_rows)
 
-
-def _row_map(what: str, t: Optional[torch.Tensor], n: int, device):
+def _row_map(what: str, t: Optional[torch.Tensor], n: int, cache: QuantKV):
     if t is None:
         return None
-    if t.dtype != torch.int32 or not t.is_contiguous() or t.numel() < n or t.device != device:
+    if t.dtype is not torch.int32 or not t.is_contiguous() or t.numel() < n or t.get_device() != cache.device_index:
         raise RuntimeError(f"{what}: row maps must be contiguous int32 on the cache's device, an entry per row")
     return t.data_ptr()
 
 
-def _bf16_rows(what: str, k: torch.Tensor, v: torch.Tensor, cache: QuantKV):
-    for t in (k, v):
-        if t.dtype != torch.bfloat16 or t.dim() != 3 or tuple(t.shape[1:]) != (cache.n_kv_heads, HEAD_DIM) \
-                or t.stride(2) != 1 or t.device != cache.k.device:
-            raise RuntimeError(f"{what}: k and v must be bf16 (rows, {cache.n_kv_heads}, 128) on the cache's device, "
-                               "values contiguous")
+def _bf16_rows(what: str, t: torch.Tensor, cache: QuantKV):
+    """(pointer, row stride, head stride) and the rows of k or v."""
+    if t.dtype is torch.bfloat16 and t.dim() == 3 and t.get_device() == cache.device_index:
+        n, hkv, d = t.shape
+        rs, hs, es = t.stride()
+        if hkv == cache.n_kv_heads and d == HEAD_DIM and es == 1:
+            return (t.data_ptr(), rs, hs if hkv > 1 else HEAD_DIM), n
+    raise RuntimeError(f"{what}: k and v must be bf16 (rows, {cache.n_kv_heads}, 128) on the cache's device, values "
+                       "contiguous")
 
 
 def kv_quantize(k: torch.Tensor, v: torch.Tensor, cache: QuantKV, dst_rows: Optional[torch.Tensor] = None,
@@ -100,18 +95,18 @@ def kv_quantize(k: torch.Tensor, v: torch.Tensor, cache: QuantKV, dst_rows: Opti
     launch (tg_kv_quantize): source row src_rows[t] (int32; default t) to cache row dst_rows[t] (int32; default
     t), t < n_rows (default: an entry of the maps, else every source row).  Entries outside the source or the cache
     are skipped; cache rows that no entry names keep what they hold; two entries may not name the same cache row."""
-    _bf16_rows("kv_quantize", k, v, cache)
-    if k.shape[0] != v.shape[0]:
+    k_args, n = _bf16_rows("kv_quantize", k, cache)
+    v_args, n_v = _bf16_rows("kv_quantize", v, cache)
+    if n != n_v:
         raise RuntimeError("kv_quantize: k and v must have the same rows")
     if n_rows is None:
-        n_rows = src_rows.numel() if src_rows is not None else dst_rows.numel() if dst_rows is not None else k.shape[0]
-    src = _row_map("kv_quantize", src_rows, n_rows, k.device)
-    dst = _row_map("kv_quantize", dst_rows, n_rows, k.device)
+        n_rows = src_rows.numel() if src_rows is not None else dst_rows.numel() if dst_rows is not None else n
+    src = _row_map("kv_quantize", src_rows, n_rows, cache)
+    dst = _row_map("kv_quantize", dst_rows, n_rows, cache)
     if n_rows == 0:
         return
-    _lib.call("tg_kv_quantize", k.data_ptr(), k.stride(0), k.stride(1) if k.shape[1] > 1 else HEAD_DIM,
-              v.data_ptr(), v.stride(0), v.stride(1) if v.shape[1] > 1 else HEAD_DIM, k.shape[0], src, dst, n_rows,
-              cache.n_kv_heads, HEAD_DIM, cache.bits, *cache._args(), _lib.stream_of(k))
+    _lib.call("tg_kv_quantize", *k_args, *v_args, n, src, dst, n_rows, cache.n_kv_heads, HEAD_DIM, cache.bits,
+              *cache._args, _lib.stream_of(k))
 
 
 def kv_dequantize(cache: QuantKV, rows: Optional[torch.Tensor] = None, n_rows: Optional[int] = None,
@@ -121,19 +116,20 @@ def kv_dequantize(cache: QuantKV, rows: Optional[torch.Tensor] = None, n_rows: O
     the cache reads as 0.  out: two bf16 tensors to write to (at least n_rows rows)."""
     if n_rows is None:
         n_rows = rows.numel() if rows is not None else cache.rows
-    ptr = _row_map("kv_dequantize", rows, n_rows, cache.k.device)
+    ptr = _row_map("kv_dequantize", rows, n_rows, cache)
     if out is None:
-        out = tuple(torch.empty(n_rows, cache.n_kv_heads, HEAD_DIM, dtype=torch.bfloat16, device=cache.k.device)
-                    for _ in range(2))
+        shape = (n_rows, cache.n_kv_heads, HEAD_DIM)
+        out = (torch.empty(shape, dtype=torch.bfloat16, device=cache.k.device),
+               torch.empty(shape, dtype=torch.bfloat16, device=cache.k.device))
     k, v = out
-    _bf16_rows("kv_dequantize", k, v, cache)
-    if k.shape[0] < n_rows or v.shape[0] < n_rows:
+    k_args, n = _bf16_rows("kv_dequantize", k, cache)
+    v_args, n_v = _bf16_rows("kv_dequantize", v, cache)
+    if n < n_rows or n_v < n_rows:
         raise RuntimeError("kv_dequantize: out holds fewer rows than are read")
     if n_rows == 0:
         return k, v
-    _lib.call("tg_kv_dequantize", *cache._args(), cache.n_kv_heads, HEAD_DIM, cache.bits, ptr, n_rows,
-              k.data_ptr(), k.stride(0), k.stride(1) if k.shape[1] > 1 else HEAD_DIM,
-              v.data_ptr(), v.stride(0), v.stride(1) if v.shape[1] > 1 else HEAD_DIM, _lib.stream_of(cache.k))
+    _lib.call("tg_kv_dequantize", *cache._args, cache.n_kv_heads, HEAD_DIM, cache.bits, ptr, n_rows, *k_args, *v_args,
+              _lib.stream_of(cache.k))
     return k, v
 
 
@@ -153,41 +149,41 @@ def decode_attention_quant(qkv: torch.Tensor, rope: torch.Tensor, lw: LayerWeigh
     value of sequence b are quantised into cache row kv_start[b] + kv_used[b] - 1, and its query attends over rows
     kv_start[b] .. kv_start[b] + kv_used[b] - 1 as they are held (s c + m, not rounded to bf16); bias_raw
     (nseq, H, >= max_k) as decode_attention; a bias of -inf hides a row whatever it holds."""
-    B = qkv.shape[0]
     H, Hkv, D = shape.n_heads, shape.n_kv_heads, shape.head_dim
-    dev = qkv.device
-    if qkv.dtype != torch.bfloat16 or qkv.dim() != 2 or qkv.shape[1] < (H + 2 * Hkv) * D or qkv.stride(1) != 1:
+    dev = qkv.get_device()
+    if qkv.dtype is not torch.bfloat16 or qkv.dim() != 2 or qkv.shape[1] < (H + 2 * Hkv) * D or qkv.stride(1) != 1:
         raise RuntimeError("decode_attention_quant: qkv must be bf16 rows of every head's q, k and v")
-    if cache.n_kv_heads != Hkv or cache.k.device != dev:
+    B = qkv.shape[0]
+    if cache.n_kv_heads != Hkv or cache.device_index != dev:
         raise RuntimeError("decode_attention_quant: the cache has other KV heads or is on another device")
-    if rope.dtype != torch.float32 or rope.numel() != B * D or not rope.is_contiguous():
-        raise RuntimeError("decode_attention_quant: rope must be contiguous fp32 (B, 64, 2)")
-    for t in (kv_start, kv_used):
-        if t.dtype != torch.int32 or not t.is_contiguous() or t.numel() < B:
-            raise RuntimeError("decode_attention_quant: kv_start and kv_used must be contiguous int32, an entry per "
-                               "sequence")
-    for t, n, which in ((q_head_scale, H, "q_head_scale must be contiguous fp32 with one entry per head"),
-                        (q_row_scale, B, "q_row_scale must be contiguous fp32 with one entry per sequence")):
-        if t is not None and (t.dtype != torch.float32 or not t.is_contiguous() or t.numel() < n):
-            raise RuntimeError("decode_attention_quant: " + which)
-    if bias_raw is not None and (bias_raw.dtype != torch.float32 or tuple(bias_raw.shape[:2]) != (B, H)
-                                 or bias_raw.stride(-1) != 1 or bias_raw.shape[-1] < max_k):
-        raise RuntimeError("decode_attention_quant: bias must be fp32 (B, H, >= max_k) with a contiguous key axis")
+    # (contiguous, dtype and device of each, and its least size)
+    for t, dt, n, which in ((rope, torch.float32, B * D, "rope must be contiguous fp32 (B, 64, 2)"),
+                            (kv_start, torch.int32, B, "kv_start must be contiguous int32, an entry per sequence"),
+                            (kv_used, torch.int32, B, "kv_used must be contiguous int32, an entry per sequence"),
+                            (q_head_scale, torch.float32, H, "q_head_scale must be contiguous fp32, an entry per head"),
+                            (q_row_scale, torch.float32, B, "q_row_scale must be contiguous fp32, an entry per sequence"),
+                            (workspace, torch.uint8, 0, "workspace must be contiguous bytes")):
+        if t is not None and (t.dtype is not dt or t.numel() < n or not t.is_contiguous() or t.get_device() != dev):
+            raise RuntimeError(f"decode_attention_quant: {which}, on qkv's device")
+    bias_args = (None, 0, 0)
+    if bias_raw is not None:
+        if bias_raw.dtype is not torch.float32 or bias_raw.dim() != 3 or bias_raw.get_device() != dev:
+            raise RuntimeError("decode_attention_quant: bias must be fp32 (B, H, >= max_k) on qkv's device")
+        nb, nh, nk = bias_raw.shape
+        sb, sh, sk = bias_raw.stride()
+        if nb != B or nh != H or nk < max_k or (sk != 1 and nk > 1):
+            raise RuntimeError("decode_attention_quant: bias must be fp32 (B, H, >= max_k) with a contiguous key axis")
+        bias_args = (bias_raw.data_ptr(), sb, sh)
     if out is None:
-        out = torch.empty(B, H, D, dtype=torch.bfloat16, device=dev)
-    elif out.dtype != torch.bfloat16 or tuple(out.shape) != (B, H, D) or out.stride(-1) != 1 or out.stride(-2) != D:
-        raise RuntimeError("decode_attention_quant: out must be bf16 (B, H, 128) rows")
-    for t in (rope, kv_start, kv_used, q_head_scale, q_row_scale, bias_raw, out, workspace):
-        if t is not None and t.device != dev:
-            raise RuntimeError("decode_attention_quant: tensors on different devices")
+        out = torch.empty((B, H, D), dtype=torch.bfloat16, device=qkv.device)
+    elif out.dtype is not torch.bfloat16 or out.shape != (B, H, D) or out.stride()[1:] != (D, 1) or out.get_device() != dev:
+        raise RuntimeError("decode_attention_quant: out must be bf16 (B, H, 128) rows on qkv's device")
     if B == 0:
         return out
     _lib.call("tg_decode_attention_quant", qkv.data_ptr(), qkv.stride(0), rope.data_ptr(), B, H, Hkv, D, cache.bits,
-              lw.q_norm.data_ptr(), lw.k_norm.data_ptr(), float(shape.rms_eps),
-              q_head_scale.data_ptr() if q_head_scale is not None else None,
-              q_row_scale.data_ptr() if q_row_scale is not None else None,
-              *cache._args(), kv_start.data_ptr(), kv_used.data_ptr(), int(max_k),
-              bias_raw.data_ptr() if bias_raw is not None else None,
-              bias_raw.stride(0) if bias_raw is not None else 0, bias_raw.stride(1) if bias_raw is not None else 0,
-              float(scale), out.data_ptr(), out.stride(0), workspace.data_ptr(), workspace.numel(), _lib.stream_of(qkv))
+              lw.q_norm.data_ptr(), lw.k_norm.data_ptr(), shape.rms_eps,
+              None if q_head_scale is None else q_head_scale.data_ptr(),
+              None if q_row_scale is None else q_row_scale.data_ptr(), *cache._args, kv_start.data_ptr(),
+              kv_used.data_ptr(), max_k, *bias_args, scale, out.data_ptr(), out.stride(0), workspace.data_ptr(),
+              workspace.numel(), _lib.stream_of(qkv))
     return out
