@@ -29,7 +29,7 @@ constexpr int kThreads = 1024;
 constexpr int kBins = 512;
 constexpr int kSort = 2048;                      // elements that one workgroup sorts
 constexpr int kList = 16384;                     // elements that are collected
-constexpr int kTiny = 1024;                      // elements that are compared with one another
+constexpr int kTiny = 64;                        // elements that are compared with one another
 constexpr int kRowsPerLaunch = 256;
 
 struct SampleArgs {
@@ -47,7 +47,7 @@ struct Part {
   double top;
   uint64_t tail;                                 // mass below the bins, in units of 2^-44 of 2^(top / q)
   uint32_t best, pad;                            // order bits of the largest logit
-  uint64_t hist[kBins];                          // count << 48 | sum of (e^t - 0.9) 2^36
+  uint64_t hist[kBins];                          // count << 48 | sum of (e^t - 0.9) 2^33
 };
 // What the first launch leaves for the second, per row; bin j: y in [top - j, top - j + 1)
 struct State {
@@ -101,30 +101,38 @@ struct Row {
 // u[b]; a one, which a rounded number may be, takes the last element of a mass of more than 2^-30
 __device__ __forceinline__ double draw(const SampleArgs &a, int b) { return fmin(fmax((double)a.u[b], 0.0), 1.0 - 0x1p-30); }
 
-// e^t for |t| <= 0.087, to 2^-49
-__device__ __forceinline__ double exp_small(double t) {
-  double p = 1.0 / 40320;
-  p = fma(p, t, 1.0 / 5040);
+// What an element adds to its bin: 1 << 48 | (e^t - 0.9) 2^33 for |t| <= 0.087, e^t to 2^-43.  The sum's whole number
+// comes out of the fraction bits of 2^52 + it.
+constexpr double kHistBase = 0.9, kHistUnit = 0x1p33;
+constexpr int kMostChunk = 0xffff;               // elements whose sums and counts the fields hold
+__device__ __forceinline__ uint64_t hist_add(double t) {
+  double p = 1.0 / 5040;
   p = fma(p, t, 1.0 / 720);
   p = fma(p, t, 1.0 / 120);
   p = fma(p, t, 1.0 / 24);
   p = fma(p, t, 1.0 / 6);
   p = fma(p, t, 0.5);
   p = fma(p, t, 1.0);
-  return fma(p, t, 1.0);
+  p = fma(p, t, 1.0);
+  return bits_of(fma(p, kHistUnit, 0x1p52 - kHistBase * kHistUnit)) - (bits_of(0x1p52) - (1ull << 48));
 }
-constexpr double kHistBase = 0.9, kHistUnit = 0x1p36;
 
 __device__ __forceinline__ uint32_t block_max(uint32_t v, uint32_t *tmp) {   // tmp: 16 words
   const int tid = threadIdx.x;
-#pragma unroll
-  for (int o = 32; o; o >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o));
+  auto step = [](uint32_t x, uint32_t y) { return x > y ? x : y; };
+  v = step(v, (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, 0xB1, 0xf, 0xf, true));    // quad_perm 1 0 3 2
+  v = step(v, (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, 0x4E, 0xf, 0xf, true));    // quad_perm 2 3 0 1
+  v = step(v, (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, 0x141, 0xf, 0xf, true));   // row_half_mirror
+  v = step(v, (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, 0x140, 0xf, 0xf, true));   // row_mirror
+  const auto p = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = step(p[0], p[1]);
+  const auto q = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  v = step(q[0], q[1]);
   __syncthreads();
   if ((tid & 63) == 0) tmp[tid >> 6] = v;
   __syncthreads();
-  v = tmp[tid & 15];
 #pragma unroll
-  for (int o = 8; o; o >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o));
+  for (int i = 0; i < kThreads / 64; ++i) v = step(v, tmp[i]);
   return v;
 }
 // Sums over the lanes up to this one, without the LDS crossbar
@@ -273,41 +281,56 @@ struct SampleWork {
 
 __device__ __forceinline__ int slot_of(double f) { return (int)(f - kBins * floor(f / kBins)); }
 
-template <int E>
-__global__ __launch_bounds__(kThreads, E == 4 ? 4 : 8) void sample_hist_kernel(SampleArgs a, SampleWork ws) {
+// A workgroup's logits: x[first], x[first + kThreads] and so on, while below end
+struct Share {
+  int first, end;
+  __device__ Share(int n) {
+    const int chunk = (n + gridDim.x - 1) / gridDim.x;
+    first = blockIdx.x * chunk + threadIdx.x;
+    end = min(n, (int)(blockIdx.x + 1) * chunk);
+  }
+  // f(value, its number), four loads at a time
+  template <typename F>
+  __device__ __forceinline__ void each(const float *x, F f) const {
+    int i = first, k = 0;
+    for (; i + 3 * kThreads < end; i += 4 * kThreads, k += 4) {
+      float v[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) v[r] = x[i + r * kThreads];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) f(v[r], k + r);
+    }
+    for (; i < end; i += kThreads, ++k) f(x[i], k);
+  }
+};
+
+__global__ __launch_bounds__(kThreads, 4) void sample_hist_kernel(SampleArgs a, SampleWork ws) {
   const int b = blockIdx.y, g = blockIdx.x, parts = gridDim.x, tid = threadIdx.x;
   const float *x = a.x + b * a.rs;
   __shared__ uint64_t hist[kBins];
   __shared__ uint32_t tmp[16];
   __shared__ unsigned long long tail_s;
   __shared__ uint32_t last_s;
-  float v[E];
-  uint32_t best = kNone;
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    const int i = (g * E + e) * kThreads + tid;
-    v[e] = i < a.n ? x[i] : -INFINITY;
-    best = max(best, order_bits(v[e]));
-  }
+  const Share share(a.n);
+  float most = -INFINITY;                        // (maxima of pairs drop NaN)
+  share.each(x, [&](float v, int) { most = fmaxf(most, v); });
   const Row row(a, b);
   if (tid < kBins) hist[tid] = 0;
   if (tid == 0) tail_s = 0;
-  best = block_max(best, tmp);                   // (its barriers cover the bins)
+  uint32_t best = block_max(order_bits(most), tmp);   // (its barriers cover the bins)
   const double top = best == kNone ? 0.0 : floor(row.y(order_float(best)));
   const double scale = kLn2 / row.q;
   const int top_slot = slot_of(top);
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    if (!(v[e] > -INFINITY)) continue;
-    const double y = row.y(v[e]), f = floor(y), j = top - f;
+  share.each(x, [&](float v, int) {
+    if (!(v > -INFINITY)) return;
+    const double y = row.y(v), f = floor(y), j = top - f;
     if (j < kBins) {
-      const double t = (y - f - 0.5) * scale;
-      atomicAdd((unsigned long long *)&hist[(top_slot - (int)j) & (kBins - 1)], (1ull << 48) + (unsigned long long)((exp_small(t) - kHistBase) * kHistUnit + 0.5));
+      atomicAdd((unsigned long long *)&hist[(top_slot - (int)j) & (kBins - 1)], (unsigned long long)hist_add((y - f - 0.5) * scale));
     } else {
       const double w = row.weight(y, top);
       if (w > 0x1p-46) atomicAdd(&tail_s, (unsigned long long)(w * 0x1p44 + 0.5));
     }
-  }
+  });
   __syncthreads();
   Part *const part = ws.parts + (int64_t)b * parts;
   if (tid < kBins) st_agent(&part[g].hist[tid], hist[tid]);
@@ -351,7 +374,7 @@ __global__ __launch_bounds__(kThreads, E == 4 ? 4 : 8) void sample_hist_kernel(S
   uint64_t sum = 0;
   uint32_t count = 0;
   double tail = 0.0;
-  constexpr int kAhead = E == 4 ? 20 : 8;
+  constexpr int kAhead = 20;
   for (int i0 = half; i0 < parts; i0 += 2 * kAhead) {
     uint64_t h[kAhead];
 #pragma unroll
@@ -614,145 +637,20 @@ __device__ void slow_row(const SampleArgs &a, int b) {
   }
 }
 
-// The collected elements of a row, in any order: kList / kThreads per thread, and what they are searched with.
+// What the collected elements of a row are searched with
 struct PickShared {
-  uint64_t mass[kBins];                          // of a bin's 512 parts, in units of 2^-44 of the bin's lower end
+  uint64_t mass[kBins];                          // of 512 parts of an interval of keys, in units of 2^-44 of the bin's lower end
   uint32_t count[kBins];
   uint64_t key[kTiny], weight[kTiny];            // elements that are compared with one another
-  uint64_t got_key;
-  double scan[16], got_cum, got_weight, above;
-  uint32_t scan_u[16], n, bin, part, above_n, place;
-};
-struct Picked {
-  uint64_t key;
-  double cum, weight;                            // mass up to and with it, and its own
-  bool ok;
-};
-template <int R>
-struct Collected {
-  const Row &row;
-  const State *st;
-  PickShared &sh;
-  uint64_t key[R];
-  int n;
-  double top, upto;                              // upto: mass up to and with bin tid
-  uint32_t upto_n;
-
-  template <typename F>
-  __device__ __forceinline__ void each(F f) const {
-#pragma unroll
-    for (int r = 0; r < R; ++r)
-      if (r * kThreads + (int)threadIdx.x < n) f(key[r]);
-  }
-  // The first element up to which the count, or the mass, reaches target (strictly: passes it).
-  __device__ Picked find(bool by_mass, double target, bool strictly) {
-    const int tid = threadIdx.x;
-    auto reaches = [&](double c) { return strictly ? c > target : c >= target; };
-    __syncthreads();
-    if (tid == 0) {
-      sh.bin = kBins;
-      sh.n = 0;
-      sh.place = ~0u;
-    }
-    __syncthreads();
-    if (tid < kBins) {
-      const double c = by_mass ? upto : (double)upto_n, p = tid == 0 ? -1.0 : by_mass ? st->upto_mass[tid - 1] : (double)st->upto_count[tid - 1];
-      if (reaches(c) && (tid == 0 || !reaches(p))) {
-        sh.bin = tid;
-        sh.above = tid ? st->upto_mass[tid - 1] : 0.0;
-        sh.above_n = tid ? st->upto_count[tid - 1] : 0;
-        sh.part = upto_n - sh.above_n;           // elements of the bin
-      }
-    }
-    __syncthreads();
-    const uint32_t bin = sh.bin, in_bin = sh.part;
-    if (bin == kBins) return Picked{0, 0.0, 0.0, false};
-    const double low = top - (double)bin;        // the bin's lower end
-    const double unit = exp2(-(double)bin / row.q) * 0x1p-44;
-    auto mine = [&](uint64_t e) { return floor(row.y(list_value(e))) == low; };
-    auto part_of = [&](uint64_t e) { return min(kBins - 1, (int)((low + 1.0 - row.y(list_value(e))) * kBins)); };
-    auto units = [&](uint64_t e) { return (uint64_t)(row.weight(row.y(list_value(e)), low) * 0x1p44 + 0.5); };
-    double above = sh.above;
-    uint32_t above_n = sh.above_n, part = kBins;   // kBins: the whole bin
-    if (in_bin > kTiny / 2) {                    // its 512 parts
-      if (tid < kBins) {
-        sh.mass[tid] = 0;
-        sh.count[tid] = 0;
-      }
-      __syncthreads();
-      each([&](uint64_t e) {
-        if (!mine(e)) return;
-        const int p = part_of(e);
-        atomicAdd((unsigned long long *)&sh.mass[p], (unsigned long long)units(e));
-        atomicAdd(&sh.count[p], 1u);
-      });
-      __syncthreads();
-      const uint32_t c = tid < kBins ? sh.count[tid] : 0;
-      const double m = tid < kBins ? (double)sh.mass[tid] * unit : 0.0;
-      uint32_t all_n;
-      double all;
-      const uint32_t c_upto = above_n + block_scan(c, sh.scan_u, all_n);
-      const double m_upto = above + block_scan(m, sh.scan, all);
-      const bool here = c > 0 && reaches(by_mass ? m_upto : (double)c_upto);
-      // (the last of the bin where rounding leaves none)
-      if (here || (c > 0 && c_upto == above_n + all_n)) atomicMin(&sh.place, (uint32_t)tid);
-      __syncthreads();
-      part = sh.place;
-      __syncthreads();
-      if ((uint32_t)tid == part) {
-        sh.above = m_upto - m;
-        sh.above_n = c_upto - c;
-      }
-      if (tid == 0) sh.place = ~0u;
-      __syncthreads();
-      above = sh.above;
-      above_n = sh.above_n;
-    }
-    each([&](uint64_t e) {
-      if (!mine(e) || (part < kBins && part_of(e) != (int)part)) return;
-      const uint32_t at = atomicAdd(&sh.n, 1u);
-      if (at < kTiny) {
-        sh.key[at] = e;
-        sh.weight[at] = units(e);
-      }
-    });
-    __syncthreads();
-    const uint32_t m = sh.n;
-    if (m == 0 || m > kTiny) return Picked{0, 0.0, 0.0, false};
-    uint64_t own = 0, cum = 0;
-    uint32_t rank = 0;
-    if ((uint32_t)tid < m) {
-      own = sh.key[tid];
-      for (uint32_t i = 0; i < m; ++i) {
-        const bool upto_me = sh.key[i] <= own;
-        rank += upto_me;
-        cum += upto_me ? sh.weight[i] : 0;
-      }
-      const double c = by_mass ? above + (double)cum * unit : (double)(above_n + rank);
-      if (reaches(c) || rank == m) atomicMin(&sh.place, rank);
-    }
-    __syncthreads();
-    if ((uint32_t)tid < m && rank == sh.place) {
-      sh.got_key = own;
-      sh.got_cum = above + (double)cum * unit;
-      sh.got_weight = row.weight_of(list_value(own), top);
-    }
-    __syncthreads();
-    return Picked{sh.got_key, sh.got_cum, sh.got_weight, true};
-  }
+  uint64_t got_key, low[16], high[16];
+  double scan[16], above, got_cum, got_weight;
+  uint32_t scan_u[16], n, bin, above_n, in, place;
 };
 
-template <int E>
 __global__ __launch_bounds__(kThreads, 4) void sample_pick_kernel(SampleArgs a, SampleWork ws) {
   const int b = blockIdx.y, g = blockIdx.x, parts = gridDim.x, tid = threadIdx.x, lane = tid & 63;
   const State *const st = ws.states + b;
   const float *x = a.x + b * a.rs;
-  float v[E];
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    const int i = (g * E + e) * kThreads + tid;
-    v[e] = i < a.n ? x[i] : -INFINITY;
-  }
   if (st->slow) {
     if (g == 0) slow_row(a, b);
     return;
@@ -765,29 +663,27 @@ __global__ __launch_bounds__(kThreads, 4) void sample_pick_kernel(SampleArgs a, 
   const double top = st->top;
   if (tid == 0) n_s = 0;
   __syncthreads();
-  uint32_t wanted = 0;
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    const double j = v[e] > -INFINITY ? top - floor(row.y(v[e])) : (double)kBins;
-    if (j < kBins && (mask[(int)j >> 6] >> ((int)j & 63) & 1)) wanted |= 1u << e;
-  }
+  const Share share(a.n);
+  uint64_t wanted = 0;                           // (at most 64 of a thread)
+  share.each(x, [&](float v, int i) {
+    const double j = v > -INFINITY ? top - floor(row.y(v)) : (double)kBins;
+    if (j < kBins && (mask[(int)j >> 6] >> ((int)j & 63) & 1)) wanted |= (uint64_t)1 << i;
+  });
   uint64_t *const all = ws.lists + (int64_t)b * kList;
   Counters *const c = ws.counters + b;
   // places in the row's list: of the thread in the workgroup, of the workgroup in the row
-  const uint32_t mine = (uint32_t)__builtin_popcount(wanted);
+  const uint32_t mine = (uint32_t)__builtin_popcountll(wanted);
   uint32_t n_mine, at = 0;
   if (__syncthreads_or(wanted != 0)) {
     at = block_scan(mine, sh.scan_u, n_mine) - mine;
     if (tid == 0) base_s = __hip_atomic_fetch_add(&c->listed, n_mine, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     __syncthreads();
     at += base_s;
-#pragma unroll
-    for (int e = 0; e < E; ++e)
-      if (wanted >> e & 1) {
-        // (all collected bins together hold at most kList)
-        if (at < kList) st_agent(all + at, (uint64_t)~order_bits(v[e]) << 32 | (uint32_t)((g * E + e) * kThreads + tid));
-        ++at;
-      }
+    for (; wanted; wanted &= wanted - 1, ++at) {
+      const int i = share.first + __builtin_ctzll(wanted) * kThreads;
+      // (all collected bins together hold at most kList)
+      if (at < kList) st_agent(all + at, (uint64_t)~order_bits(x[i]) << 32 | (uint32_t)i);
+    }
   }
   wait_all_mem();
   __syncthreads();
@@ -795,72 +691,199 @@ __global__ __launch_bounds__(kThreads, 4) void sample_pick_kernel(SampleArgs a, 
     last_s = __hip_atomic_fetch_add(&c->pick, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)parts - 1u;
   __syncthreads();
   if (!last_s) return;
-  constexpr int R = kList / kThreads;
-  Collected<R> col{row, st, sh};
-  col.n = (int)min(ld_agent(&c->listed), (uint32_t)kList);
-  col.top = top;
-  col.upto = tid < kBins ? st->upto_mass[tid] : 0.0;
-  col.upto_n = tid < kBins ? st->upto_count[tid] : 0;
-#pragma unroll
-  for (int r = 0; r < R; ++r) col.key[r] = r * kThreads < col.n ? ld_agent(all + min(r * kThreads + tid, kList - 1)) : 0;
+  // ---- the row's elements, in any order ----
+  // (loops over LDS: unrolled over registers, their doubles' code was fetched for longer than it ran)
+  __shared__ uint64_t list[kList];
+  const int n = (int)min(ld_agent(&c->listed), (uint32_t)kList), wave = tid >> 6;
+  for (int i = tid; i < n; i += kThreads) list[i] = ld_agent(all + i);
+  auto each = [&](auto f) {                      // (a thread's own)
+#pragma unroll 1
+    for (int i = tid; i < n; i += kThreads) f(list[i]);
+  };
+  // up to and with bin tid, and above it
+  double upto = 0.0, over = 0.0;
+  uint32_t upto_n = 0, over_n = 0;
+  if (tid < kBins) {
+    upto = st->upto_mass[tid];
+    upto_n = st->upto_count[tid];
+    if (tid > 0) {
+      over = st->upto_mass[tid - 1];
+      over_n = st->upto_count[tid - 1];
+    }
+  }
+  const uint32_t in_bins = st->upto_count[kBins - 1];
+  const int m_lo = (int)st->m_lo, m_hi = (int)st->m_hi;
+  const float best = order_float(st->best);
+  double s3 = st->mass;                          // of S1, of S2, of S3
   __syncthreads();
   if (tid == 0) {
     st_agent(&c->listed, 0u);
     st_agent(&c->pick, 0u);
   }
-  const double mass = st->mass;
   const float tp = a.top_p ? a.top_p[b] : 1.f, mp = a.min_p ? a.min_p[b] : 0.f;
   const int k = row.greedy ? 1 : a.top_k && a.top_k[b] > 0 && a.top_k[b] < a.n ? a.top_k[b] : 0;
-  bool ok = true;
-  double s3 = mass;                              // of S1, then of S3
-  Picked p{0, 0.0, 0.0, true};
-  if (k && (uint32_t)k <= st->upto_count[kBins - 1]) {
-    p = col.find(false, (double)k, false);
-    ok &= p.ok;
-    s3 = p.cum;
-  }
-  if (!row.greedy) {
-    double end = s3;
-    if (tp < 1.f) {
-      p = col.find(true, (double)fmaxf(tp, 0.f) * s3, false);
-      ok &= p.ok;
-      end = fmin(end, p.cum);
-    }
-    if (mp > 0.f && (int)st->m_lo < kBins) {     // what reaches min_p: the bins above m_lo and elements of m_lo .. m_hi
-      const float best = order_float(st->best);
-      const double lo = (double)st->m_lo, hi = (double)st->m_hi;
-      uint64_t sum = 0;
-      const double unit = exp2(-lo / row.q) * 0x1p-44;
-      col.each([&](uint64_t e) {
-        const float y = list_value(e);
-        const double j = top - floor(row.y(y));
-        if (j >= lo && j <= hi && !row.under(y, best, mp)) sum += (uint64_t)(row.weight(row.y(y), top - lo) * 0x1p44 + 0.5);
+  // S1's end, S2's end, the token: each the first element up to which a count, or the mass, reaches a target (the
+  // token's: passes it).  Its bin first; then, as long as an interval of keys holds more than kTiny elements, 512 parts
+  // of what its least and largest key span (a few values, each of many elements, where logits are bf16: then the parts
+  // are of indices); then element by element.
+#pragma unroll 1
+  for (int stage = 0; stage < 3; ++stage) {
+    if (stage == 0 && !(k && (uint32_t)k <= in_bins)) continue;
+    if (stage == 1 && !(tp < 1.f)) continue;
+    if (stage == 2 && mp > 0.f && m_lo < kBins) {   // S3: also what reaches min_p, the bins above m_lo and elements of m_lo .. m_hi
+      uint64_t sum = 0, all_sum;
+      each([&](uint64_t e) {
+        const float v = list_value(e);
+        const double y = row.y(v), j = top - floor(y);
+        if (j >= (double)m_lo && j <= (double)m_hi && !row.under(v, best, mp))
+          sum += (uint64_t)(row.weight(y, top - (double)m_lo) * 0x1p44 + 0.5);
       });
-      uint64_t all_sum;
       block_scan(sum, reinterpret_cast<uint64_t *>(sh.scan), all_sum);
-      end = fmin(end, (st->m_lo ? st->upto_mass[st->m_lo - 1] : 0.0) + (double)all_sum * unit);
+      const double above = m_lo ? st->upto_mass[m_lo - 1] : 0.0;
+      s3 = fmin(s3, above + (double)all_sum * (exp2(-(double)m_lo / row.q) * 0x1p-44));
     }
-    s3 = end;
-    p = col.find(true, draw(a, b) * s3, true);
-    ok &= p.ok;
+    const bool by_mass = stage > 0;
+    const double target = stage == 0 ? (double)k : stage == 1 ? (double)fmaxf(tp, 0.f) * s3 : draw(a, b) * s3;
+    auto reaches = [&](double x) { return stage == 2 ? x > target : x >= target; };
+    __syncthreads();
+    if (tid == 0) {
+      sh.bin = kBins - 1;                        // (where rounding leaves none)
+      sh.place = ~0u;
+      sh.n = 0;
+    }
+    __syncthreads();
+    if (tid < kBins && reaches(by_mass ? upto : (double)upto_n) && (tid == 0 || !reaches(by_mass ? over : (double)over_n))) sh.bin = tid;
+    __syncthreads();
+    const uint32_t bin = sh.bin;
+    if ((uint32_t)tid == bin) {
+      sh.above = over;
+      sh.above_n = over_n;
+      sh.in = upto_n - over_n;
+    }
+    __syncthreads();
+    double above = sh.above;
+    uint32_t above_n = sh.above_n, in = sh.in;
+    const double low = top - (double)bin;        // the bin's lower end
+    const double unit = exp2(-(double)bin / row.q) * 0x1p-44;
+    auto units = [&](uint64_t e) { return (uint64_t)(row.weight(row.y(list_value(e)), low) * 0x1p44 + 0.5); };
+    uint64_t lo = 0, hi = ~0ull;                 // the interval: elements of the bin with lo <= key <= hi
+    bool whole = true;
+    auto mine = [&](uint64_t e) { return whole ? floor(row.y(list_value(e))) == low : e >= lo && e <= hi; };
+#pragma unroll 1
+    for (int round = 0; round < 8 && in > kTiny; ++round) {   // (64 bits of keys, 9 and more a round)
+      uint64_t l = ~0ull, h = 0;
+      each([&](uint64_t e) {
+        if (!mine(e)) return;
+        l = e < l ? e : l;
+        h = e > h ? e : h;
+      });
+#pragma unroll
+      for (int o = 32; o; o >>= 1) {
+        const uint64_t l2 = __shfl_xor((unsigned long long)l, o), h2 = __shfl_xor((unsigned long long)h, o);
+        l = l2 < l ? l2 : l;
+        h = h2 > h ? h2 : h;
+      }
+      if (lane == 0) {
+        sh.low[wave] = l;
+        sh.high[wave] = h;
+      }
+      if (tid < kBins) {
+        sh.mass[tid] = 0;
+        sh.count[tid] = 0;
+      }
+      __syncthreads();
+      lo = ~0ull;
+      hi = 0;
+#pragma unroll
+      for (int i = 0; i < kThreads / 64; ++i) {
+        lo = sh.low[i] < lo ? sh.low[i] : lo;
+        hi = sh.high[i] > hi ? sh.high[i] : hi;
+      }
+      whole = false;
+      if (lo >= hi) break;                       // (not with more than one element)
+      const int bits = 64 - __builtin_clzll(hi - lo), shift = bits > 9 ? bits - 9 : 0;
+      each([&](uint64_t e) {
+        if (!mine(e)) return;
+        const int p = (int)((e - lo) >> shift);
+        atomicAdd((unsigned long long *)&sh.mass[p], (unsigned long long)units(e));
+        atomicAdd(&sh.count[p], 1u);
+      });
+      __syncthreads();
+      const uint32_t cnt = tid < kBins ? sh.count[tid] : 0;
+      const double m = tid < kBins ? (double)sh.mass[tid] * unit : 0.0;
+      uint32_t all_n;
+      double all_m;
+      const uint32_t c_upto = above_n + block_scan(cnt, sh.scan_u, all_n);
+      const double m_upto = above + block_scan(m, sh.scan, all_m);
+      // (the last where rounding leaves none)
+      if (cnt > 0 && (reaches(by_mass ? m_upto : (double)c_upto) || c_upto == above_n + all_n)) atomicMin(&sh.place, (uint32_t)tid);
+      __syncthreads();
+      const uint32_t part = sh.place;
+      if ((uint32_t)tid == part) {
+        sh.above = m_upto - m;
+        sh.above_n = c_upto - cnt;
+        sh.in = cnt;
+      }
+      __syncthreads();
+      if (tid == 0) sh.place = ~0u;
+      above = sh.above;
+      above_n = sh.above_n;
+      in = sh.in;
+      lo += (uint64_t)part << shift;
+      const uint64_t end = lo + (((uint64_t)1 << shift) - 1);
+      hi = end < hi ? end : hi;
+    }
+    each([&](uint64_t e) {
+      if (!mine(e)) return;
+      const uint32_t at = atomicAdd(&sh.n, 1u);
+      if (at < kTiny) {
+        sh.key[at] = e;
+        sh.weight[at] = units(e);
+      }
+    });
+    __syncthreads();
+    const uint32_t m = min(sh.n, (uint32_t)kTiny);
+    uint64_t own = 0, cum = 0;
+    uint32_t rank = 0;
+    if ((uint32_t)tid < m) {
+      own = sh.key[tid];
+#pragma unroll 4
+      for (uint32_t i = 0; i < m; ++i) {
+        const bool upto_me = sh.key[i] <= own;
+        rank += upto_me;
+        cum += upto_me ? sh.weight[i] : 0;
+      }
+      if (reaches(by_mass ? above + (double)cum * unit : (double)(above_n + rank)) || rank == m) atomicMin(&sh.place, rank);
+    }
+    __syncthreads();
+    if ((uint32_t)tid < m && rank == sh.place) {
+      sh.got_key = own;
+      sh.got_cum = above + (double)cum * unit;
+      sh.got_weight = row.weight_of(list_value(own), top);
+    }
+    __syncthreads();
+    if (row.greedy) break;
+    if (stage < 2) s3 = fmin(s3, sh.got_cum);
   }
-  if (!ok) return slow_row(a, b);                // more than kTiny elements in 1/512 of a bin
   if (tid == 0) {
-    a.token[b] = (uint32_t)p.key;
-    if (a.logprob) a.logprob[b] = row.greedy ? 0.f : (float)log(fmin(1.0, p.weight / s3));
+    a.token[b] = (uint32_t)sh.got_key;
+    if (a.logprob) a.logprob[b] = row.greedy ? 0.f : (float)log(fmin(1.0, sh.got_weight / s3));
   }
 }
 
 struct SamplePlan {
-  int parts, e;
+  int parts;
   int64_t states, lists, parts_at, bytes;        // byte offsets; the counters come first, for any launch
 };
-int sample_parts(int64_t n, int e) { return (int)((n + e * kThreads - 1) / (e * kThreads)); }
-// rows: of one launch.  4 logits per thread while that makes at most two workgroups per CU, else 16.
+// rows: of one launch.  Parts of 4096 logits, fewer and larger ones where that would make more than one workgroup per CU,
+// but for what a bin's fields hold.
+int sample_parts(int64_t rows, int64_t n) {
+  const int64_t least = (n + kMostChunk - 1) / kMostChunk, most = (n + 4 * kThreads - 1) / (4 * kThreads);
+  return (int)std::max(least, std::min(most, device_cus() / rows));
+}
 SamplePlan plan_sample(int64_t rows, int64_t n) {
   SamplePlan p;
-  p.e = rows * sample_parts(n, 4) <= 2 * device_cus() ? 4 : 16;
-  p.parts = sample_parts(n, p.e);
+  p.parts = sample_parts(rows, n);
   p.states = kRowsPerLaunch * sizeof(Counters);
   p.lists = p.states + rows * (int64_t)sizeof(State);
   p.parts_at = p.lists + rows * kList * 8;
@@ -873,13 +896,12 @@ SamplePlan plan_sample(int64_t rows, int64_t n) {
 
 using namespace tg;
 
-// (enough for fewer rows and columns: those may take 4 logits per thread, but then no more parts than two per CU)
+// (enough for fewer rows and columns: those may be cut into more parts, but then into no more than one per CU in all)
 extern "C" int64_t tg_sample_rows_workspace_size(int32_t n_rows, int64_t n_cols) {
   if (n_rows <= 0 || n_cols <= kSort || n_cols > (1 << 18)) return 0;
   const int64_t rows = std::min<int32_t>(n_rows, kRowsPerLaunch);
-  const int64_t parts = std::max(std::min<int64_t>(rows * sample_parts(n_cols, 4), 2 * device_cus()), rows * sample_parts(n_cols, 16));
-  const SamplePlan p = plan_sample(rows, n_cols);
-  return p.parts_at + parts * (int64_t)sizeof(Part);
+  const int64_t parts = std::max(std::min<int64_t>(rows * sample_parts(1, n_cols), device_cus()), rows * sample_parts(rows, n_cols));
+  return plan_sample(rows, n_cols).parts_at + parts * (int64_t)sizeof(Part);
 }
 
 extern "C" int tg_sample_rows(const float *x, int64_t x_row_stride, int32_t n_rows, int64_t n_cols, const float *u,
@@ -910,13 +932,8 @@ extern "C" int tg_sample_rows(const float *x, int64_t x_row_stride, int32_t n_ro
     const SampleWork w{reinterpret_cast<Counters *>(ws), reinterpret_cast<State *>(ws + p.states),
                        reinterpret_cast<uint64_t *>(ws + p.lists), reinterpret_cast<Part *>(ws + p.parts_at)};
     const dim3 grid((unsigned)p.parts, (unsigned)rows), block(kThreads);
-    if (p.e == 4) {
-      hipLaunchKernelGGL(sample_hist_kernel<4>, grid, block, 0, stream, a, w);
-      hipLaunchKernelGGL(sample_pick_kernel<4>, grid, block, 0, stream, a, w);
-    } else {
-      hipLaunchKernelGGL(sample_hist_kernel<16>, grid, block, 0, stream, a, w);
-      hipLaunchKernelGGL(sample_pick_kernel<16>, grid, block, 0, stream, a, w);
-    }
+    hipLaunchKernelGGL(sample_hist_kernel, grid, block, 0, stream, a, w);
+    hipLaunchKernelGGL(sample_pick_kernel, grid, block, 0, stream, a, w);
     TG_HIP_CHECK(hipGetLastError());
   }
   return 0;
