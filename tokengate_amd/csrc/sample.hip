@@ -46,7 +46,8 @@ struct SampleArgs {
 struct Part {
   double top;
   uint64_t tail;                                 // mass below the bins, in units of 2^-44 of 2^(top / q)
-  uint32_t best, pad;                            // order bits of the largest logit
+  uint32_t best, least;                          // order bits of the largest logit, and of the smallest within reach
+  uint32_t fine, pad;                            // Row's
   uint64_t hist[kBins];                          // count << 48 | sum of (e^t - 0.9) 2^33
 };
 // What the first launch leaves for the second, per row; bin j: y in [top - j, top - j + 1)
@@ -54,9 +55,11 @@ struct State {
   double top, mass;                              // mass of the whole row, in units of 2^(top / q), as all
   uint64_t mask[kBins / 64];                     // bins to collect
   uint32_t best, slow, m_lo, m_hi;               // bins that may hold min_p's end
+  uint32_t fine, pad;                            // Row's
   double upto_mass[kBins];                       // up to and with bin j
   uint32_t upto_count[kBins];
 };
+enum : uint32_t { kUsual, kSlow, kDone };        // State::slow
 struct Counters {
   uint32_t hist, pick, listed, pad;              // zero between launches
 };
@@ -77,21 +80,52 @@ __device__ __forceinline__ uint32_t order_bits(float x) {
 __device__ __forceinline__ float order_float(uint32_t o) { return u32_as_f32(o & 0x80000000u ? o & 0x7fffffffu : ~o); }
 constexpr uint32_t kNone = 0x007FFFFFu;          // order bits of -inf
 
-// A row's settings.  Bins per octave of w: q; y = cc x.
+// 2^z, to 2^-46, for z of up to some hundreds (the exponential's series over half an octave either way)
+__device__ __forceinline__ double exp2_of(double z) {
+  z = fmax(z, -1100.0);
+  const double n = rint(z), t = (z - n) * kLn2;
+  double p = 1.0 / 39916800;
+  p = fma(p, t, 1.0 / 3628800);
+  p = fma(p, t, 1.0 / 362880);
+  p = fma(p, t, 1.0 / 40320);
+  p = fma(p, t, 1.0 / 5040);
+  p = fma(p, t, 1.0 / 720);
+  p = fma(p, t, 1.0 / 120);
+  p = fma(p, t, 1.0 / 24);
+  p = fma(p, t, 1.0 / 6);
+  p = fma(p, t, 0.5);
+  p = fma(p, t, 1.0);
+  p = fma(p, t, 1.0);
+  return ldexp(p, (int)n);
+}
+
+// A row's settings.  Bins per octave of w: q; y = cc x.  Both are 2^fine times what lets the bins reach 64 octaves (at
+// T <= 1) down: with 2^fine as large as the spread of the logits allows, a bin of a flat row holds no more than one of a
+// steep row.
+constexpr int kFinest = 12;
 struct Row {
-  double q, cc;
-  float temp;
+  double q, per_q, cc;
   bool greedy;
-  __device__ Row(const SampleArgs &a, int b) {
+  __device__ Row(const SampleArgs &a, int b, int fine) {
     const float t = a.temperature ? a.temperature[b] : 1.f;
     greedy = !(t > 0.f);
-    temp = greedy ? 1.f : t;
-    q = fmax(4.0, 8.0 * (double)temp);
-    cc = q * kLog2e / (double)temp;
+    const double temp = greedy ? 1.0 : (double)t;
+    q = ldexp(fmax(4.0, 8.0 * temp), fine);
+    per_q = 1.0 / q;
+    cc = ldexp(temp >= 0.5 ? 8.0 * kLog2e : 4.0 * kLog2e / temp, fine);
+  }
+  // the bins' reach, in logits; the finest bins (of a row of fine 0) that reach from most down to least
+  __device__ float reach() const { return (float)(kBins / cc); }
+  __device__ int finest(float most, float least) const {
+    const double span = ((double)most - (double)least) * cc;
+    int fine = 0;
+    if (span >= 0.0)                             // (not where nothing is within reach, or both are infinite)
+      while (fine < kFinest && ldexp(span, fine + 1) < kBins - 2) ++fine;
+    return fine;
   }
   // (+inf: so far above every finite one that those weigh nothing)
   __device__ double y(float x) const { return x == INFINITY ? 0x1p1000 : (double)x * cc; }
-  __device__ double weight(double y, double top) const { return exp2((y - top) / q); }
+  __device__ double weight(double y, double top) const { return exp2_of((y - top) * per_q); }
   __device__ double weight_of(float x, double top) const { return x == -INFINITY ? 0.0 : weight(y(x), top); }
   // whether x has less than least times the largest logit's weight
   __device__ bool under(float x, float best, float least) const {
@@ -105,7 +139,7 @@ __device__ __forceinline__ double draw(const SampleArgs &a, int b) { return fmin
 // comes out of the fraction bits of 2^52 + it.
 constexpr double kHistBase = 0.9, kHistUnit = 0x1p33;
 constexpr int kMostChunk = 0xffff;               // elements whose sums and counts the fields hold
-__device__ __forceinline__ uint64_t hist_add(double t) {
+__device__ __forceinline__ double exp_small(double t) {
   double p = 1.0 / 5040;
   p = fma(p, t, 1.0 / 720);
   p = fma(p, t, 1.0 / 120);
@@ -113,12 +147,18 @@ __device__ __forceinline__ uint64_t hist_add(double t) {
   p = fma(p, t, 1.0 / 6);
   p = fma(p, t, 0.5);
   p = fma(p, t, 1.0);
-  p = fma(p, t, 1.0);
-  return bits_of(fma(p, kHistUnit, 0x1p52 - kHistBase * kHistUnit)) - (bits_of(0x1p52) - (1ull << 48));
+  return fma(p, t, 1.0);
+}
+__device__ __forceinline__ uint64_t hist_add(double t) {
+  return bits_of(fma(exp_small(t), kHistUnit, 0x1p52 - kHistBase * kHistUnit)) - (bits_of(0x1p52) - (1ull << 48));
 }
 
-__device__ __forceinline__ uint32_t block_max(uint32_t v, uint32_t *tmp) {   // tmp: 16 words
-  const int tid = threadIdx.x;
+// Mass of a bin, in units of 2^(its middle / q)
+__device__ __forceinline__ double hist_mass(uint64_t h) {
+  return kHistBase * (double)(uint32_t)(h >> 48) + (double)(h & 0xffffffffffffull) * (1.0 / kHistUnit);
+}
+
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
   auto step = [](uint32_t x, uint32_t y) { return x > y ? x : y; };
   v = step(v, (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, 0xB1, 0xf, 0xf, true));    // quad_perm 1 0 3 2
   v = step(v, (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, 0x4E, 0xf, 0xf, true));    // quad_perm 2 3 0 1
@@ -127,12 +167,16 @@ __device__ __forceinline__ uint32_t block_max(uint32_t v, uint32_t *tmp) {   // 
   const auto p = __builtin_amdgcn_permlane16_swap(v, v, false, false);
   v = step(p[0], p[1]);
   const auto q = __builtin_amdgcn_permlane32_swap(v, v, false, false);
-  v = step(q[0], q[1]);
+  return step(q[0], q[1]);
+}
+__device__ __forceinline__ uint32_t block_max(uint32_t v, uint32_t *tmp) {   // tmp: 16 words
+  const int tid = threadIdx.x;
+  v = wave_max(v);
   __syncthreads();
   if ((tid & 63) == 0) tmp[tid >> 6] = v;
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < kThreads / 64; ++i) v = step(v, tmp[i]);
+  for (int i = 0; i < kThreads / 64; ++i) v = v > tmp[i] ? v : tmp[i];
   return v;
 }
 // Sums over the lanes up to this one, without the LDS crossbar
@@ -214,7 +258,7 @@ __global__ __launch_bounds__(kThreads) void sample_small_kernel(SampleArgs a) {
   __shared__ double scan[16], mass_s[2];
   const int b = blockIdx.x, tid = threadIdx.x, n = a.n;
   const float *x = a.x + b * a.rs;
-  const Row row(a, b);
+  const Row row(a, b, 0);
   for (int i = tid; i < n; i += kThreads) list[i] = (uint64_t)~order_bits(x[i]) << 32 | (uint32_t)i;
   const int per = (sort_list(list, n) + kThreads - 1) / kThreads;   // elements of a thread, in order
   const float best = list_value(list[0]);
@@ -312,14 +356,24 @@ __global__ __launch_bounds__(kThreads, 4) void sample_hist_kernel(SampleArgs a, 
   __shared__ unsigned long long tail_s;
   __shared__ uint32_t last_s;
   const Share share(a.n);
-  float most = -INFINITY;                        // (maxima of pairs drop NaN)
-  share.each(x, [&](float v, int) { most = fmaxf(most, v); });
-  const Row row(a, b);
+  float most = -INFINITY, least = INFINITY;      // (maxima of pairs drop NaN)
+  const Row coarse(a, b, 0);
+  const float reach = coarse.reach();
+  // least: of what lies within reach of the largest; what lies below, as a finite mask does, may not count
+  share.each(x, [&](float v, int) {
+    most = fmaxf(most, v);
+    const float end = most - reach;
+    least = least > end ? least : INFINITY;
+    least = v > end ? fminf(least, v) : least;
+  });
   if (tid < kBins) hist[tid] = 0;
   if (tid == 0) tail_s = 0;
   uint32_t best = block_max(order_bits(most), tmp);   // (its barriers cover the bins)
+  const uint32_t low_bits = ~block_max(least > order_float(best) - reach ? ~order_bits(least) : 0u, tmp);
+  const int fine = low_bits == ~0u ? 0 : coarse.finest(order_float(best), order_float(low_bits));
+  const Row row(a, b, fine);
   const double top = best == kNone ? 0.0 : floor(row.y(order_float(best)));
-  const double scale = kLn2 / row.q;
+  const double scale = kLn2 * row.per_q;
   const int top_slot = slot_of(top);
   share.each(x, [&](float v, int) {
     if (!(v > -INFINITY)) return;
@@ -337,7 +391,8 @@ __global__ __launch_bounds__(kThreads, 4) void sample_hist_kernel(SampleArgs a, 
   if (tid == 0) {
     st_agent((uint64_t *)&part[g].top, bits_of(top));
     st_agent(&part[g].tail, (uint64_t)tail_s);
-    st_agent(&part[g].best, best);
+    st_agent((uint64_t *)&part[g].best, (uint64_t)low_bits << 32 | best);
+    st_agent(&part[g].fine, (uint32_t)fine);
   }
   wait_all_mem();
   __syncthreads();
@@ -347,28 +402,48 @@ __global__ __launch_bounds__(kThreads, 4) void sample_hist_kernel(SampleArgs a, 
   if (!last_s) return;
 
   // ---- the row's bins ----
-  __shared__ double tops[64], mass_s[kBins], scan_d[16];
+  __shared__ double mass_s[kBins], scan_d[16];
   __shared__ uint64_t sums[2][kBins];
-  __shared__ uint32_t counts[2][kBins], count_s[kBins], scan_u[16], bests[64];
-  __shared__ int first_s[4], slots[64];
-  if (tid < parts) {
-    tops[tid] = double_of(ld_agent((const uint64_t *)&part[tid].top));
-    slots[tid] = slot_of(tops[tid]);
-    bests[tid] = ld_agent(&part[tid].best);
+  __shared__ uint32_t counts[2][kBins], count_s[kBins], scan_u[16];
+  __shared__ int first_s[4], slots[64], finer_s[64], depth[64];
+  // every wave: a part per lane (at most 64)
+  const int lane = tid & 63;
+  double part_top = 0.0;
+  uint32_t part_best = kNone, part_least = ~0u, part_fine = kFinest;
+  if (lane < parts) {
+    part_top = double_of(ld_agent((const uint64_t *)&part[lane].top));
+    const uint64_t ends = ld_agent((const uint64_t *)&part[lane].best);
+    part_best = (uint32_t)ends;
+    part_least = (uint32_t)(ends >> 32);
+    part_fine = ld_agent(&part[lane].fine);
   }
-  __syncthreads();
-  best = kNone;
-  for (int i = 0; i < parts; ++i) best = max(best, bests[i]);
+  (&sums[0][0])[tid] = 0;
+  (&counts[0][0])[tid] = 0;
+  best = wave_max(part_best);
   State *const st = ws.states + b;
-  if (best == kNone) {                           // nothing but -inf: token 0, by the slow way
+  if (best == kNone) {                           // nothing but -inf
     if (tid == 0) {
-      st->slow = 1;
-      for (int i = 0; i < kBins / 64; ++i) st->mask[i] = 0;
+      a.token[b] = 0;
+      if (a.logprob) a.logprob[b] = 0.f;
+      st->slow = kDone;
       st_agent(&ws.counters[b].hist, 0u);
     }
     return;
   }
-  const double gtop = floor(row.y(order_float(best)));
+  // the finest bins that the row's span and every part's allow
+  const bool near_top = part_best != kNone && order_float(part_least) > order_float(best) - reach;
+  const uint32_t least_row = ~wave_max(near_top ? ~part_least : 0u);
+  int fine_row = kFinest - (int)wave_max(part_best == kNone ? 0u : kFinest - part_fine);
+  fine_row = least_row == ~0u ? 0 : min(fine_row, coarse.finest(order_float(best), order_float(least_row)));
+  const Row whole(a, b, fine_row);
+  const double gtop = floor(whole.y(order_float(best))), scale_row = kLn2 * whole.per_q;
+  const int part_finer = part_best == kNone ? 0 : (int)part_fine - fine_row;
+  if (tid < parts) {
+    slots[tid] = slot_of(part_top);
+    finer_s[tid] = part_finer;
+    depth[tid] = (int)fmin(ldexp(gtop, part_finer) - part_top, 0x1p29);   // of its first bin below the row's, in its bins
+  }
+  __syncthreads();
   // thread: one slot of every other part
   const int slot = tid & (kBins - 1), half = tid / kBins;
   uint64_t sum = 0;
@@ -383,20 +458,31 @@ __global__ __launch_bounds__(kThreads, 4) void sample_hist_kernel(SampleArgs a, 
     for (int r = 0; r < kAhead; ++r) {
       const int i = i0 + 2 * r;
       if (i >= parts || h[r] == 0) continue;
-      const double below = gtop - tops[i] + ((slots[i] - slot) & (kBins - 1));   // the row's bin, if less than kBins
-      if (below < kBins) {
-        count += (uint32_t)(h[r] >> 48);
-        sum += h[r] & 0xffffffffffffull;
+      const int finer = finer_s[i], d = depth[i] + ((slots[i] - slot) & (kBins - 1)), below = (d + (1 << finer) - 1) >> finer;
+      const uint32_t c = (uint32_t)(h[r] >> 48);
+      uint64_t s = h[r] & 0xffffffffffffull;
+      if (finer) {                               // 2^finer of the part's bins are one of the row's: from one middle to another's
+        const double off = ldexp((double)((below << finer) - d) + 0.5, -finer) - 0.5;
+        s = (uint64_t)((hist_mass(h[r]) * exp_small(off * scale_row) - kHistBase * (double)c) * kHistUnit + 0.5);
+      }
+      if (below >= kBins) {
+        tail += exp2_of((0.5 - below) * whole.per_q) * hist_mass((uint64_t)c << 48 | s);
+      } else if (finer) {
+        atomicAdd((unsigned long long *)&sums[half][below], (unsigned long long)s);
+        atomicAdd(&counts[half][below], c);
       } else {
-        tail += exp2((0.5 - below) / row.q) * (kHistBase * (double)(h[r] >> 48) + (double)(h[r] & 0xffffffffffffull) / kHistUnit);
+        count += c;
+        sum += s;
       }
     }
   }
-  if (tid < parts && bests[tid] != kNone) tail += exp2((tops[tid] - gtop) / row.q) * ((double)ld_agent(&part[tid].tail) * 0x1p-44);
+  if (tid < parts && part_best != kNone)
+    tail += exp2_of((ldexp(part_top, -part_finer) - gtop) * whole.per_q) * ((double)ld_agent(&part[tid].tail) * 0x1p-44);
+  __syncthreads();
   {
     const int j = (slot_of(gtop) - slot) & (kBins - 1);
-    sums[half][j] = sum;
-    counts[half][j] = count;
+    sums[half][j] += sum;
+    counts[half][j] += count;
   }
   __syncthreads();
   const int j = slot;                            // from here on a bin
@@ -404,7 +490,7 @@ __global__ __launch_bounds__(kThreads, 4) void sample_hist_kernel(SampleArgs a, 
   count = 0;
   if (half == 0) {
     count = counts[0][j] + counts[1][j];
-    m = exp2((0.5 - j) / row.q) * (kHistBase * (double)count + (double)(sums[0][j] + sums[1][j]) / kHistUnit);
+    m = exp2_of((0.5 - j) * whole.per_q) * (kHistBase * (double)count + (double)(sums[0][j] + sums[1][j]) * (1.0 / kHistUnit));
   }
   double in_bins, tail_all;
   uint32_t n_bins;
@@ -452,7 +538,7 @@ __global__ __launch_bounds__(kThreads, 4) void sample_hist_kernel(SampleArgs a, 
     hi = fmin(hi, mass_s[p_hi]);
   }
   if (mp > 0.f) {
-    const double thr = row.y(order_float(best)) + row.q * log2(fmin((double)mp, 1.0)), d0 = gtop - floor(thr + 1e-6),
+    const double thr = whole.y(order_float(best)) + whole.q * log2(fmin((double)mp, 1.0)), d0 = gtop - floor(thr + 1e-6),
                  d1 = gtop - floor(thr - 1e-6);
     m_lo = d0 < 0.0 ? 0 : d0 < kBins ? (int)d0 : kBins;
     m_hi = d1 < 0.0 ? 0 : d1 < kBins ? (int)d1 : kBins;
@@ -485,9 +571,10 @@ __global__ __launch_bounds__(kThreads, 4) void sample_hist_kernel(SampleArgs a, 
     st->top = gtop;
     st->mass = mass;
     st->best = best;
-    st->slow = slow;
+    st->slow = slow ? kSlow : kUsual;
     st->m_lo = (uint32_t)m_lo;
     st->m_hi = (uint32_t)m_hi;
+    st->fine = (uint32_t)fine_row;
     st_agent(&ws.counters[b].hist, 0u);
   }
 }
@@ -625,7 +712,7 @@ __device__ void slow_row(const SampleArgs &a, int b) {
       total = sum_mass(last);
     }
   }
-  const double t = (double)a.u[b] * (double)total;
+  const double t = draw(a, b) * (double)total;
   const uint64_t target = min((uint64_t)t + 1, total);
   const Place p = find(target, true);
   const uint32_t i = index_of(p);
@@ -637,10 +724,11 @@ __device__ void slow_row(const SampleArgs &a, int b) {
   }
 }
 
-// What the collected elements of a row are searched with
+// What the collected elements of a row are searched with.  Copies of the bins: elements of one value, hundreds where
+// logits are bf16, add to one bin.
+constexpr int kCopies = 4;
 struct PickShared {
-  uint64_t mass[kBins];                          // of 512 parts of an interval of keys, in units of 2^-44 of the bin's lower end
-  uint32_t count[kBins];
+  uint64_t hist[kCopies][kBins];                 // of 512 parts of an interval of keys, as Part's
   uint64_t key[kTiny], weight[kTiny];            // elements that are compared with one another
   uint64_t got_key, low[16], high[16];
   double scan[16], above, got_cum, got_weight;
@@ -651,14 +739,14 @@ __global__ __launch_bounds__(kThreads, 4) void sample_pick_kernel(SampleArgs a, 
   const int b = blockIdx.y, g = blockIdx.x, parts = gridDim.x, tid = threadIdx.x, lane = tid & 63;
   const State *const st = ws.states + b;
   const float *x = a.x + b * a.rs;
-  if (st->slow) {
-    if (g == 0) slow_row(a, b);
+  if (st->slow != kUsual) {
+    if (g == 0 && st->slow == kSlow) slow_row(a, b);
     return;
   }
   __shared__ PickShared sh;
   __shared__ uint64_t mask[kBins / 64];
   __shared__ uint32_t n_s, base_s, last_s;
-  const Row row(a, b);
+  const Row row(a, b, (int)st->fine);
   if (tid < kBins / 64) mask[tid] = st->mask[tid];
   const double top = st->top;
   if (tid == 0) n_s = 0;
@@ -720,6 +808,7 @@ __global__ __launch_bounds__(kThreads, 4) void sample_pick_kernel(SampleArgs a, 
     st_agent(&c->listed, 0u);
     st_agent(&c->pick, 0u);
   }
+  const double scale = kLn2 * row.per_q;
   const float tp = a.top_p ? a.top_p[b] : 1.f, mp = a.min_p ? a.min_p[b] : 0.f;
   const int k = row.greedy ? 1 : a.top_k && a.top_k[b] > 0 && a.top_k[b] < a.n ? a.top_k[b] : 0;
   // S1's end, S2's end, the token: each the first element up to which a count, or the mass, reaches a target (the
@@ -740,7 +829,7 @@ __global__ __launch_bounds__(kThreads, 4) void sample_pick_kernel(SampleArgs a, 
       });
       block_scan(sum, reinterpret_cast<uint64_t *>(sh.scan), all_sum);
       const double above = m_lo ? st->upto_mass[m_lo - 1] : 0.0;
-      s3 = fmin(s3, above + (double)all_sum * (exp2(-(double)m_lo / row.q) * 0x1p-44));
+      s3 = fmin(s3, above + (double)all_sum * (exp2_of(-(double)m_lo * row.per_q) * 0x1p-44));
     }
     const bool by_mass = stage > 0;
     const double target = stage == 0 ? (double)k : stage == 1 ? (double)fmaxf(tp, 0.f) * s3 : draw(a, b) * s3;
@@ -764,33 +853,30 @@ __global__ __launch_bounds__(kThreads, 4) void sample_pick_kernel(SampleArgs a, 
     double above = sh.above;
     uint32_t above_n = sh.above_n, in = sh.in;
     const double low = top - (double)bin;        // the bin's lower end
-    const double unit = exp2(-(double)bin / row.q) * 0x1p-44;
+    const double unit = exp2_of(-(double)bin * row.per_q) * 0x1p-44, mid = exp2_of((0.5 - (double)bin) * row.per_q);
     auto units = [&](uint64_t e) { return (uint64_t)(row.weight(row.y(list_value(e)), low) * 0x1p44 + 0.5); };
     uint64_t lo = 0, hi = ~0ull;                 // the interval: elements of the bin with lo <= key <= hi
     bool whole = true;
     auto mine = [&](uint64_t e) { return whole ? floor(row.y(list_value(e))) == low : e >= lo && e <= hi; };
 #pragma unroll 1
     for (int round = 0; round < 8 && in > kTiny; ++round) {   // (64 bits of keys, 9 and more a round)
-      uint64_t l = ~0ull, h = 0;
+      uint64_t l = ~0ull, r = 0;
       each([&](uint64_t e) {
         if (!mine(e)) return;
         l = e < l ? e : l;
-        h = e > h ? e : h;
+        r = e > r ? e : r;
       });
 #pragma unroll
       for (int o = 32; o; o >>= 1) {
-        const uint64_t l2 = __shfl_xor((unsigned long long)l, o), h2 = __shfl_xor((unsigned long long)h, o);
+        const uint64_t l2 = __shfl_xor((unsigned long long)l, o), r2 = __shfl_xor((unsigned long long)r, o);
         l = l2 < l ? l2 : l;
-        h = h2 > h ? h2 : h;
+        r = r2 > r ? r2 : r;
       }
       if (lane == 0) {
         sh.low[wave] = l;
-        sh.high[wave] = h;
+        sh.high[wave] = r;
       }
-      if (tid < kBins) {
-        sh.mass[tid] = 0;
-        sh.count[tid] = 0;
-      }
+      for (int i = tid; i < kCopies * kBins; i += kThreads) sh.hist[i / kBins][i % kBins] = 0;
       __syncthreads();
       lo = ~0ull;
       hi = 0;
@@ -804,13 +890,15 @@ __global__ __launch_bounds__(kThreads, 4) void sample_pick_kernel(SampleArgs a, 
       const int bits = 64 - __builtin_clzll(hi - lo), shift = bits > 9 ? bits - 9 : 0;
       each([&](uint64_t e) {
         if (!mine(e)) return;
-        const int p = (int)((e - lo) >> shift);
-        atomicAdd((unsigned long long *)&sh.mass[p], (unsigned long long)units(e));
-        atomicAdd(&sh.count[p], 1u);
+        atomicAdd((unsigned long long *)&sh.hist[lane % kCopies][(e - lo) >> shift],
+                  (unsigned long long)hist_add((row.y(list_value(e)) - low - 0.5) * scale));
       });
       __syncthreads();
-      const uint32_t cnt = tid < kBins ? sh.count[tid] : 0;
-      const double m = tid < kBins ? (double)sh.mass[tid] * unit : 0.0;
+      uint64_t h = 0;
+      if (tid < kBins)
+        for (int i = 0; i < kCopies; ++i) h += sh.hist[i][tid];
+      const uint32_t cnt = (uint32_t)(h >> 48);
+      const double m = hist_mass(h) * mid;
       uint32_t all_n;
       double all_m;
       const uint32_t c_upto = above_n + block_scan(cnt, sh.scan_u, all_n);
