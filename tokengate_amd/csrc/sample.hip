@@ -78,7 +78,7 @@ __device__ __forceinline__ uint32_t order_bits(float x) {
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ float order_float(uint32_t o) { return u32_as_f32(o & 0x80000000u ? o & 0x7fffffffu : ~o); }
-constexpr uint32_t kNone = 0x007FFFFFu;          // order bits of -inf
+constexpr uint32_t kNone = 0x007FFFFFu, kMost = 0xFF800000u;   // order bits of -inf, of +inf
 
 // 2^z, to 2^-46, for z of up to some hundreds (the exponential's series over half an octave either way)
 __device__ __forceinline__ double exp2_of(double z) {
@@ -104,7 +104,7 @@ __device__ __forceinline__ double exp2_of(double z) {
 // steep row.
 constexpr int kFinest = 12;
 struct Row {
-  double q, per_q, cc;
+  double q, per_q, cc, per_cc;
   bool greedy;
   __device__ Row(const SampleArgs &a, int b, int fine) {
     const float t = a.temperature ? a.temperature[b] : 1.f;
@@ -113,9 +113,10 @@ struct Row {
     q = ldexp(fmax(4.0, 8.0 * temp), fine);
     per_q = 1.0 / q;
     cc = ldexp(temp >= 0.5 ? 8.0 * kLog2e : 4.0 * kLog2e / temp, fine);
+    per_cc = ldexp(temp >= 0.5 ? 0.125 * kLn2 : 0.25 * kLn2 * temp, -fine);
   }
   // the bins' reach, in logits; the finest bins (of a row of fine 0) that reach from most down to least
-  __device__ float reach() const { return (float)(kBins / cc); }
+  __device__ float reach() const { return (float)(kBins * per_cc); }
   __device__ int finest(float most, float least) const {
     const double span = ((double)most - (double)least) * cc;
     int fine = 0;
@@ -127,6 +128,14 @@ struct Row {
   __device__ double y(float x) const { return x == INFINITY ? 0x1p1000 : (double)x * cc; }
   __device__ double weight(double y, double top) const { return exp2_of((y - top) * per_q); }
   __device__ double weight_of(float x, double top) const { return x == -INFINITY ? 0.0 : weight(y(x), top); }
+  // order bits of the first value, from below, of a bin not under low (above: not of low either)
+  __device__ uint32_t first(double low, bool above) const {
+    auto in = [&](uint32_t o) { return above ? floor(y(order_float(o))) > low : y(order_float(o)) >= low; };
+    uint32_t o = order_bits((float)((above ? low + 1.0 : low) * per_cc));   // (off by its roundings)
+    while (o > kNone && in(o - 1)) --o;
+    while (o <= kMost && !in(o)) ++o;
+    return o;
+  }
   // whether x has less than least times the largest logit's weight
   __device__ bool under(float x, float best, float least) const {
     return x != best && (x == -INFINITY || weight(y(x), y(best)) < fmin((double)least, 1.0));
@@ -724,11 +733,9 @@ __device__ void slow_row(const SampleArgs &a, int b) {
   }
 }
 
-// What the collected elements of a row are searched with.  Copies of the bins: elements of one value, hundreds where
-// logits are bf16, add to one bin.
-constexpr int kCopies = 4;
+// What the collected elements of a row are searched with
 struct PickShared {
-  uint64_t hist[kCopies][kBins];                 // of 512 parts of an interval of keys, as Part's
+  uint64_t hist[kBins];                          // of 512 parts of an interval of keys, as Part's
   uint64_t key[kTiny], weight[kTiny];            // elements that are compared with one another
   uint64_t got_key, low[16], high[16];
   double scan[16], above, got_cum, got_weight;
@@ -739,16 +746,18 @@ __global__ __launch_bounds__(kThreads, 4) void sample_pick_kernel(SampleArgs a, 
   const int b = blockIdx.y, g = blockIdx.x, parts = gridDim.x, tid = threadIdx.x, lane = tid & 63;
   const State *const st = ws.states + b;
   const float *x = a.x + b * a.rs;
-  if (st->slow != kUsual) {
-    if (g == 0 && st->slow == kSlow) slow_row(a, b);
+  const uint32_t slow = st->slow;
+  const double top = st->top;
+  const uint64_t mask_bits = st->mask[tid & (kBins / 64 - 1)];
+  const Row row(a, b, (int)st->fine);
+  if (slow != kUsual) {
+    if (g == 0 && slow == kSlow) slow_row(a, b);
     return;
   }
   __shared__ PickShared sh;
   __shared__ uint64_t mask[kBins / 64];
   __shared__ uint32_t n_s, base_s, last_s;
-  const Row row(a, b, (int)st->fine);
-  if (tid < kBins / 64) mask[tid] = st->mask[tid];
-  const double top = st->top;
+  if (tid < kBins / 64) mask[tid] = mask_bits;
   if (tid == 0) n_s = 0;
   __syncthreads();
   const Share share(a.n);
@@ -773,22 +782,7 @@ __global__ __launch_bounds__(kThreads, 4) void sample_pick_kernel(SampleArgs a, 
       if (at < kList) st_agent(all + at, (uint64_t)~order_bits(x[i]) << 32 | (uint32_t)i);
     }
   }
-  wait_all_mem();
-  __syncthreads();
-  if (tid == 0)
-    last_s = __hip_atomic_fetch_add(&c->pick, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)parts - 1u;
-  __syncthreads();
-  if (!last_s) return;
-  // ---- the row's elements, in any order ----
-  // (loops over LDS: unrolled over registers, their doubles' code was fetched for longer than it ran)
-  __shared__ uint64_t list[kList];
-  const int n = (int)min(ld_agent(&c->listed), (uint32_t)kList), wave = tid >> 6;
-  for (int i = tid; i < n; i += kThreads) list[i] = ld_agent(all + i);
-  auto each = [&](auto f) {                      // (a thread's own)
-#pragma unroll 1
-    for (int i = tid; i < n; i += kThreads) f(list[i]);
-  };
-  // up to and with bin tid, and above it
+  // up to and with bin tid, and above it (for the last workgroup: here their loads take no time of their own)
   double upto = 0.0, over = 0.0;
   uint32_t upto_n = 0, over_n = 0;
   if (tid < kBins) {
@@ -802,6 +796,23 @@ __global__ __launch_bounds__(kThreads, 4) void sample_pick_kernel(SampleArgs a, 
   const uint32_t in_bins = st->upto_count[kBins - 1];
   const int m_lo = (int)st->m_lo, m_hi = (int)st->m_hi;
   const float best = order_float(st->best);
+  wait_all_mem();
+  __syncthreads();
+  if (tid == 0)
+    last_s = __hip_atomic_fetch_add(&c->pick, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)parts - 1u;
+  __syncthreads();
+  if (!last_s) return;
+  // ---- the row's elements, in any order ----
+  // (loops over LDS: unrolled over registers, their doubles' code was fetched for longer than it ran)
+  __shared__ uint64_t list[kList];
+  const uint64_t first_entry = ld_agent(all + tid);
+  const int n = (int)min(ld_agent(&c->listed), (uint32_t)kList), wave = tid >> 6;
+  if (tid < n) list[tid] = first_entry;
+  for (int i = tid + kThreads; i < n; i += kThreads) list[i] = ld_agent(all + i);
+  auto each = [&](auto f) {                      // (a thread's own)
+#pragma unroll 1
+    for (int i = tid; i < n; i += kThreads) f(list[i]);
+  };
   double s3 = st->mass;                          // of S1, of S2, of S3
   __syncthreads();
   if (tid == 0) {
@@ -855,48 +866,49 @@ __global__ __launch_bounds__(kThreads, 4) void sample_pick_kernel(SampleArgs a, 
     const double low = top - (double)bin;        // the bin's lower end
     const double unit = exp2_of(-(double)bin * row.per_q) * 0x1p-44, mid = exp2_of((0.5 - (double)bin) * row.per_q);
     auto units = [&](uint64_t e) { return (uint64_t)(row.weight(row.y(list_value(e)), low) * 0x1p44 + 0.5); };
-    uint64_t lo = 0, hi = ~0ull;                 // the interval: elements of the bin with lo <= key <= hi
-    bool whole = true;
-    auto mine = [&](uint64_t e) { return whole ? floor(row.y(list_value(e))) == low : e >= lo && e <= hi; };
+    // the interval: elements with lo <= key <= hi, at first those of the bin
+    uint64_t lo = (uint64_t)~(row.first(low, true) - 1u) << 32, hi = (uint64_t)~row.first(low, false) << 32 | 0xffffffffu;
+    auto mine = [&](uint64_t e) { return e >= lo && e <= hi; };
 #pragma unroll 1
     for (int round = 0; round < 8 && in > kTiny; ++round) {   // (64 bits of keys, 9 and more a round)
-      uint64_t l = ~0ull, r = 0;
-      each([&](uint64_t e) {
-        if (!mine(e)) return;
-        l = e < l ? e : l;
-        r = e > r ? e : r;
-      });
+      if (tid < kBins) sh.hist[tid] = 0;
+      if (round > 0) {                           // what the elements span
+        uint64_t l = ~0ull, r = 0;
+        each([&](uint64_t e) {
+          if (!mine(e)) return;
+          l = e < l ? e : l;
+          r = e > r ? e : r;
+        });
 #pragma unroll
-      for (int o = 32; o; o >>= 1) {
-        const uint64_t l2 = __shfl_xor((unsigned long long)l, o), r2 = __shfl_xor((unsigned long long)r, o);
-        l = l2 < l ? l2 : l;
-        r = r2 > r ? r2 : r;
-      }
-      if (lane == 0) {
-        sh.low[wave] = l;
-        sh.high[wave] = r;
-      }
-      for (int i = tid; i < kCopies * kBins; i += kThreads) sh.hist[i / kBins][i % kBins] = 0;
-      __syncthreads();
-      lo = ~0ull;
-      hi = 0;
+        for (int o = 32; o; o >>= 1) {
+          const uint64_t l2 = __shfl_xor((unsigned long long)l, o), r2 = __shfl_xor((unsigned long long)r, o);
+          l = l2 < l ? l2 : l;
+          r = r2 > r ? r2 : r;
+        }
+        if (lane == 0) {
+          sh.low[wave] = l;
+          sh.high[wave] = r;
+        }
+        __syncthreads();
+        lo = ~0ull;
+        hi = 0;
 #pragma unroll
-      for (int i = 0; i < kThreads / 64; ++i) {
-        lo = sh.low[i] < lo ? sh.low[i] : lo;
-        hi = sh.high[i] > hi ? sh.high[i] : hi;
+        for (int i = 0; i < kThreads / 64; ++i) {
+          lo = sh.low[i] < lo ? sh.low[i] : lo;
+          hi = sh.high[i] > hi ? sh.high[i] : hi;
+        }
+      } else {
+        __syncthreads();
       }
-      whole = false;
       if (lo >= hi) break;                       // (not with more than one element)
       const int bits = 64 - __builtin_clzll(hi - lo), shift = bits > 9 ? bits - 9 : 0;
       each([&](uint64_t e) {
         if (!mine(e)) return;
-        atomicAdd((unsigned long long *)&sh.hist[lane % kCopies][(e - lo) >> shift],
+        atomicAdd((unsigned long long *)&sh.hist[(e - lo) >> shift],
                   (unsigned long long)hist_add((row.y(list_value(e)) - low - 0.5) * scale));
       });
       __syncthreads();
-      uint64_t h = 0;
-      if (tid < kBins)
-        for (int i = 0; i < kCopies; ++i) h += sh.hist[i][tid];
+      const uint64_t h = tid < kBins ? sh.hist[tid] : 0;
       const uint32_t cnt = (uint32_t)(h >> 48);
       const double m = hist_mass(h) * mid;
       uint32_t all_n;
