@@ -458,7 +458,7 @@ __global__ __launch_bounds__(kThreads, 4) void sample_hist_kernel(SampleArgs a, 
   uint64_t sum = 0;
   uint32_t count = 0;
   double tail = 0.0;
-  constexpr int kAhead = 20;
+  constexpr int kAhead = 10;
   for (int i0 = half; i0 < parts; i0 += 2 * kAhead) {
     uint64_t h[kAhead];
 #pragma unroll
@@ -975,10 +975,12 @@ struct SamplePlan {
   int parts;
   int64_t states, lists, parts_at, bytes;        // byte offsets; the counters come first, for any launch
 };
-// rows: of one launch.  Parts of 4096 logits, fewer and larger ones where that would make more than one workgroup per CU,
-// but for what a bin's fields hold.
+// rows: of one launch.  Parts of 8192 logits, fewer and larger ones where that would make more than one workgroup per CU,
+// but for what a bin's fields hold.  (Parts of 4096, 8192, 12288 and 16384, both launches: 4 rows of 151936 44, 41, 41 and
+// 43 us, 1 row of them 36, 37, 39 and 40: a part costs its logits' time twice over, and 4 KB of the merge.)
+constexpr int64_t kPart = 8 * kThreads;
 int sample_parts(int64_t rows, int64_t n) {
-  const int64_t least = (n + kMostChunk - 1) / kMostChunk, most = (n + 4 * kThreads - 1) / (4 * kThreads);
+  const int64_t least = (n + kMostChunk - 1) / kMostChunk, most = (n + kPart - 1) / kPart;
   return (int)std::max(least, std::min(most, device_cus() / rows));
 }
 SamplePlan plan_sample(int64_t rows, int64_t n) {
