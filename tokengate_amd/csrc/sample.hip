@@ -611,14 +611,28 @@ __device__ void slow_row(const SampleArgs &a, int b) {
     __syncthreads();
     return v;
   };
+  auto each = [&](auto f) {                      // f(order bits), eight loads at a time
+    for (int i0 = tid; i0 < a.n; i0 += 8 * kThreads) {
+      float v[8];
+#pragma unroll
+      for (int r = 0; r < 8; ++r) v[r] = x[min(i0 + r * kThreads, a.n - 1)];
+#pragma unroll 1
+      for (int r = 0; r < 8; ++r) {
+        float w = v[0];                          // (shifted down: no indexed registers)
+#pragma unroll
+        for (int q = 0; q < 7; ++q) v[q] = v[q + 1];
+        if (i0 + r * kThreads < a.n) f(order_bits(w));
+      }
+    }
+  };
   uint32_t best = 0;
-  for (int i = tid; i < a.n; i += kThreads) best = max(best, order_bits(x[i]));
+  each([&](uint32_t key) { best = max(best, key); });
   best = reduce_max(best);
   const float top = order_float(best);
   const float temp = a.temperature ? a.temperature[b] : 1.f;
   const bool greedy = !(temp > 0.f) || top == -INFINITY;
   const double scale = greedy ? 1.0 : kLog2e / temp;
-  auto weight = [&](float x) { return x == top ? 1.0 : exp2(((double)x - (double)top) * scale); };   // (both may be infinite)
+  auto weight = [&](float x) { return x == top ? 1.0 : exp2_of(((double)x - (double)top) * scale); };   // (both may be infinite)
   auto mass = [&](uint32_t key) { return (uint64_t)(weight(order_float(key)) * kMassUnit + 0.5); };
   // The first place at which the sum of value(key) over the elements up to it reaches target (> 0).
   auto find = [&](uint64_t target, bool by_mass) {
@@ -627,11 +641,17 @@ __device__ void slow_row(const SampleArgs &a, int b) {
     for (int shift = 24; shift >= 0; shift -= 8) {
       if (tid < 256) hist[tid] = 0;
       __syncthreads();
-      for (int i = tid; i < a.n; i += kThreads) {
-        const uint32_t key = order_bits(x[i]);
-        if (shift == 24 || (key >> (shift + 8)) == (prefix >> (shift + 8)))
-          atomicAdd((unsigned long long *)&hist[(key >> shift) & 255], (unsigned long long)(by_mass ? mass(key) : 1));
-      }
+      each([&](uint32_t key) {
+        if (shift != 24 && (key >> (shift + 8)) != (prefix >> (shift + 8))) return;
+        uint64_t m = by_mass ? mass(key) : 1;
+        const uint32_t first = (uint32_t)__builtin_amdgcn_readfirstlane((int)key);
+        const uint64_t here = __ballot(1), same = __ballot(key == first);
+        if (here == same) {                      // (many equal ones make such a row: one addition for all of a wave's)
+          m *= (uint64_t)__popcll(here);
+          if ((tid & 63) != __builtin_ctzll(here)) return;
+        }
+        atomicAdd((unsigned long long *)&hist[(key >> shift) & 255], (unsigned long long)m);
+      });
       __syncthreads();
       if (tid == 0) {
         uint64_t c = above;
@@ -651,10 +671,9 @@ __device__ void slow_row(const SampleArgs &a, int b) {
   };
   auto sum_mass = [&](Place p) {                 // of the elements of a place's beginning
     uint64_t s = 0;
-    for (int i = tid; i < a.n; i += kThreads) {
-      const uint32_t key = order_bits(x[i]);
+    each([&](uint32_t key) {
       if (key > p.key) s += mass(key);
-    }
+    });
     for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o);
     if ((tid & 63) == 0) red[tid >> 6] = s;
     __syncthreads();
@@ -711,10 +730,9 @@ __device__ void slow_row(const SampleArgs &a, int b) {
     uint64_t s = 0;                              // mass of what reaches min_p (a beginning as well)
     const double least = fmin((double)mp, 1.0);
     uint32_t end = 0xffffffffu;
-    for (int i = tid; i < a.n; i += kThreads) {
-      const uint32_t key = order_bits(x[i]);
-      if (weight(order_float(key)) >= least) end = min(end, key);
-    }
+    each([&](uint32_t key) {
+      if (key < end && weight(order_float(key)) >= least) end = key;
+    });
     end = ~reduce_max(~end);
     if (end > last.key) {
       last = Place{end - 1, 0, 0};
