@@ -214,3 +214,27 @@ def test_shared_workspace_strides_stream_and_graph(cuda):
         torch.cuda.synchronize()
         w, l = dec.sample_rows(x, u, t, None, p, workspace=ws, logprob=True)
         assert torch.equal(tok, w) and torch.equal(lp, l), i
+
+
+def test_log_probability_of_nearly_all_the_mass(cuda):
+    """A token with all of the mass has log probability 0 exactly, by every setting that leaves it alone; one whose rival
+    has 2^-30 .. 2^-40 of it keeps a relative error of 2^-24 for its rounding, 2^-33 for the rivals' bins, and an absolute one of
+    2^-43 for its own weight and its sum."""
+    inf = float("inf")
+    for v in (2048, 5000, 151936):
+        x = torch.full((5, v), -inf)
+        x[:, v // 3] = torch.tensor([0.3, -7.1, 100.7, 1e-3, 3e4])
+        for k, p, m in ((0, 1.0, 0.0), (1, 1.0, 0.0), (3, 0.5, 0.0), (0, 1.0, 0.9)):
+            lp = check(cuda, x, [0.3] * 5, [0.7] * 5, [k] * 5, [p] * 5, [m] * 5)[1]
+            assert bool((lp == 0).all()), (v, k, p, m, lp)
+        y = logits(5, v, v)
+        y[:, v // 2] = 40.3
+        for k, p, m in ((1, 1.0, 0.0), (0, 0.5, 0.0), (0, 1.0, 0.9)):
+            lp = check(cuda, y, [0.3] * 5, [0.9] * 5, [k] * 5, [p] * 5, [m] * 5)[1]
+            assert bool((lp == 0).all()), (v, k, p, m, lp)
+        z = torch.full((5, v), -inf)
+        z[:, 4] = 1.7
+        z[:, v - 5] = 1.7 - torch.tensor([20.5, 21.0, 23.3, 25.0, 28.0])
+        lp = check(cuda, z, [0.4] * 5, None, None, None, None)[1].cpu().double()
+        want = -torch.log1p(torch.exp(z[:, v - 5].double() - z[:, 4].double()))
+        assert bool(((lp - want).abs() <= (2.0 ** -24 + 2.0 ** -33) * want.abs() + 2.0 ** -43).all()), (lp, want)

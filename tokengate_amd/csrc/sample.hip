@@ -756,7 +756,7 @@ struct PickShared {
   uint64_t hist[kBins];                          // of 512 parts of an interval of keys, as Part's
   uint64_t key[kTiny], weight[kTiny];            // elements that are compared with one another
   uint64_t got_key, low[16], high[16];
-  double scan[16], above, got_cum, got_weight;
+  double scan[16], above, got_cum, got_weight, bin_mass, bin_upto, bin_over;
   uint32_t scan_u[16], n, bin, above_n, in, place;
 };
 
@@ -831,7 +831,8 @@ __global__ __launch_bounds__(kThreads, 4) void sample_pick_kernel(SampleArgs a, 
 #pragma unroll 1
     for (int i = tid; i < n; i += kThreads) f(list[i]);
   };
-  double s3 = st->mass;                          // of S1, of S2, of S3
+  double s3 = st->mass;                          // of S1, of S2, of S3: bins 0 .. from_hist - 1 as the first launch has them
+  uint32_t from_hist = kBins;
   __syncthreads();
   if (tid == 0) {
     st_agent(&c->listed, 0u);
@@ -858,7 +859,11 @@ __global__ __launch_bounds__(kThreads, 4) void sample_pick_kernel(SampleArgs a, 
       });
       block_scan(sum, reinterpret_cast<uint64_t *>(sh.scan), all_sum);
       const double above = m_lo ? st->upto_mass[m_lo - 1] : 0.0;
-      s3 = fmin(s3, above + (double)all_sum * (exp2_of(-(double)m_lo * row.per_q) * 0x1p-44));
+      const double sum_m = above + (double)all_sum * (exp2_of(-(double)m_lo * row.per_q) * 0x1p-44);
+      if (sum_m < s3) {
+        s3 = sum_m;
+        from_hist = (uint32_t)m_lo;
+      }
     }
     const bool by_mass = stage > 0;
     const double target = stage == 0 ? (double)k : stage == 1 ? (double)fmaxf(tp, 0.f) * s3 : draw(a, b) * s3;
@@ -877,10 +882,13 @@ __global__ __launch_bounds__(kThreads, 4) void sample_pick_kernel(SampleArgs a, 
       sh.above = over;
       sh.above_n = over_n;
       sh.in = upto_n - over_n;
+      sh.bin_upto = upto;
+      sh.bin_over = over;
     }
     __syncthreads();
     double above = sh.above;
     uint32_t above_n = sh.above_n, in = sh.in;
+    const uint32_t first_in = in;
     const double low = top - (double)bin;        // the bin's lower end
     const double unit = exp2_of(-(double)bin * row.per_q) * 0x1p-44, mid = exp2_of((0.5 - (double)bin) * row.per_q);
     auto units = [&](uint64_t e) { return (uint64_t)(row.weight(row.y(list_value(e)), low) * 0x1p44 + 0.5); };
@@ -977,11 +985,21 @@ __global__ __launch_bounds__(kThreads, 4) void sample_pick_kernel(SampleArgs a, 
     if ((uint32_t)tid < m && rank == sh.place) {
       sh.got_key = own;
       sh.got_cum = above + (double)cum * unit;
-      sh.got_weight = row.weight_of(list_value(own), top);
+      sh.got_weight = (double)sh.weight[tid] * unit;
     }
+    if ((uint32_t)tid < m && rank == m) sh.bin_mass = (double)cum * unit;
     __syncthreads();
     if (row.greedy) break;
-    if (stage < 2) s3 = fmin(s3, sh.got_cum);
+    if (stage < 2) {
+      if (sh.got_cum < s3) {
+        s3 = sh.got_cum;
+        from_hist = bin;
+      }
+    } else if (first_in <= kTiny && bin < from_hist) {
+      // the whole bin is S3's: its sum from its elements' 2^-44 instead of 2^-34, so that the logarithm of a token with
+      // nearly all of the mass, which may be alone, has few wrong digits
+      s3 += sh.bin_mass - (sh.bin_upto - sh.bin_over);
+    }
   }
   if (tid == 0) {
     a.token[b] = (uint32_t)sh.got_key;
