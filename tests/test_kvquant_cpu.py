@@ -127,3 +127,46 @@ def test_workspace_sizes():
     assert sizes == sorted(sizes)
     sizes = [lib.tg_sample_rows_workspace_size(n, 151936) for n in (1, 2, 3, 8, 64)]
     assert sizes == sorted(sizes)
+
+
+def test_more_refusals(ptr):
+    """Workspaces of sampling; tensors that are on no GPU."""
+    from tokengate_amd import _lib
+    from tokengate_amd import decoder as dec
+    from tokengate_amd import kvquant as Q
+    p = ptr[0]
+    lib = _lib.load()
+    for n, cols in ((1, 2049), (7, 40000), (300, 262144)):
+        need = lib.tg_sample_rows_workspace_size(n, cols)
+        sample = dict(x=p, rs=cols, n=n, cols=cols, u=p, t=None, k=None, tp=None, mp=None, token=p, lp=None, ws=p, ws_n=need, stream=None)
+        for change in (dict(ws=None), dict(ws=p + 4), dict(ws_n=1000)):
+            assert "workspace" in _call("tg_sample_rows", sample, **change), (n, cols, change)
+    c = _cache()
+    k = torch.zeros(4, 2, 128, dtype=torch.bfloat16)
+    for f in (lambda: Q.kv_quantize(k, k, c), lambda: Q.kv_dequantize(c, n_rows=2),
+              lambda: dec.sample_rows(torch.zeros(2, 7), torch.zeros(2))):
+        with pytest.raises(RuntimeError, match="on a GPU"):
+            f()
+
+
+def test_calls_on_another_device(monkeypatch):
+    """A call whose tensors are not on the current device is made on theirs, with its stream."""
+    from tokengate_amd import _lib
+    seen, on = [], [0]
+
+    class Device:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            on.append(self.index)
+
+        def __exit__(self, *e):
+            on.pop()
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda i: 100 + i, raising=False)
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: on[-1], raising=False)
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(_lib, "call", lambda name, *args: seen.append((name, args, on[-1])))
+    _lib.call_on(0, "a", 1)
+    _lib.call_on(3, "b", 2)
+    assert seen == [("a", (1, 100), 0), ("b", (2, 103), 3)] and on == [0]

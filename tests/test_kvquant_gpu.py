@@ -431,3 +431,31 @@ def test_read_back_for_other_query_counts(cuda):
         p = torch.softmax(torch.einsum("hd,nhd->hn", q[i].double(), a) * SCALE, -1)
         ref, mass = torch.einsum("hn,nhd->hd", p, b), torch.einsum("hn,nhd->hd", p, b.abs())
         assert bool(((out[i].double() - ref).abs() <= 2.0 ** -8 * mass + 2.0 ** -8 * ref.abs() + 2e-5).all())
+
+
+@pytest.mark.parametrize("used,H,Hkv,checked", [
+    ([100 + 37 * i for i in range(130)], 8, 8, 7),          # more sequences than a wave has lanes; two rounds
+    ([300 + 997 * i % 5000 for i in range(70)], 16, 8, 5),  # a cut that is corrected
+    ([1 + 61 * i % 700 for i in range(2100)], 8, 8, 400),   # more units than counters: nothing is cut
+    ([0, 5, 0, 3000, 1], 16, 8, 1)])                        # sequences of no key among others
+def test_many_ragged_sequences(cuda, used, H, Hkv, checked):
+    """Cuts of every kind: all sequences in one launch, and every `checked`-th one in a launch of its own, which cuts
+    them in another way and is compared in float64.  Both are off by half a step of bf16, 2^-8 of an element, for the
+    last rounding and by less than 2^-8 of the head's largest for everything else."""
+    from tokengate_amd import kvquant as Q
+    c = attn_case(cuda, used, 2, H, Hkv, 4, 77 + len(used), False, False)
+    ws = Q.decode_attention_quant_workspace(len(used), c["shape"], c["max_k"], cuda)
+    cache = clone_cache(c["cache"])
+    for _ in range(2):
+        out = run_attn(c, cache, ws)
+    torch.cuda.synchronize()
+    B = len(used)
+    some = [b for b in range(0, B, checked) if used[b] > 0]
+    part = dict(c, qkv=c["qkv"][some], pos=c["pos"][some], start=c["start"][some], used=c["used"][some])
+    alone = clone_cache(c["cache"])
+    got = run_attn(part, alone, ws)
+    torch.cuda.synchronize()
+    check_attn(part, got, alone)
+    a, b = got.float(), out[some].float()
+    assert bool(((a - b).abs() <= 2.0 ** -7 * a.abs() + 2.0 ** -7 * a.abs().amax(-1, keepdim=True)).all())
+    assert all(bool((out[i] == 0).all()) for i in range(B) if used[i] == 0)

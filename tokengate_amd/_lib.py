@@ -6,6 +6,7 @@ Nothing here falls back to another implementation: a missing library is an error
 """
 import ctypes as C
 import os
+import sys
 import threading
 
 from tokengate_amd.fa2bias.site_path import LIB_NAME, SITE
@@ -118,6 +119,20 @@ def stream_of(t) -> int:
     """The current stream of the tensor's device, as the handle the library takes."""
     import torch
     return torch._C._cuda_getCurrentRawStream(t.device.index)
+
+
+def call_on(index: int, name: str, *args) -> None:
+    """`name` with args and, as its last argument, the current stream of device `index`, on that device whatever the
+    current one is."""
+    if index < 0:
+        raise RuntimeError(f"{name}: tensors must be on a GPU")
+    torch = sys.modules["torch"]                 # (the caller has tensors)
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if torch._C._cuda_getDevice() == index:
+        call(name, *args, stream)
+    else:
+        with torch.cuda.device(index):
+            call(name, *args, stream)
 
 
 def fwd_plan(B, Sq, Sk, H, Hkv, causal, workspace_bytes):

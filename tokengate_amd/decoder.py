@@ -597,9 +597,9 @@ def sample_rows(logits: torch.Tensor, u: torch.Tensor, temperature: Optional[tor
     out = torch.empty(n, dtype=torch.int64, device=logits.device)
     lp = torch.empty(n, dtype=torch.float32, device=logits.device) if logprob else None
     if n:
-        _lib.call("tg_sample_rows", logits.data_ptr(), logits.stride(0) if n > 1 else V, n, V, u.data_ptr(),
-                  *(t.data_ptr() if t is not None else None for t in (temperature, top_k, top_p, min_p)), out.data_ptr(),
-                  lp.data_ptr() if logprob else None, workspace.data_ptr(), workspace.numel(), _stream(logits))
+        _lib.call_on(logits.get_device(), "tg_sample_rows", logits.data_ptr(), logits.stride(0) if n > 1 else V, n, V,
+                     u.data_ptr(), *(t.data_ptr() if t is not None else None for t in (temperature, top_k, top_p, min_p)),
+                     out.data_ptr(), lp.data_ptr() if logprob else None, workspace.data_ptr(), workspace.numel())
     return (out, lp) if logprob else out
 
 

@@ -105,8 +105,8 @@ def kv_quantize(k: torch.Tensor, v: torch.Tensor, cache: QuantKV, dst_rows: Opti
     dst = _row_map("kv_quantize", dst_rows, n_rows, cache)
     if n_rows == 0:
         return
-    _lib.call("tg_kv_quantize", *k_args, *v_args, n, src, dst, n_rows, cache.n_kv_heads, HEAD_DIM, cache.bits,
-              *cache._args, _lib.stream_of(k))
+    _lib.call_on(cache.device_index, "tg_kv_quantize", *k_args, *v_args, n, src, dst, n_rows, cache.n_kv_heads,
+                 HEAD_DIM, cache.bits, *cache._args)
 
 
 def kv_dequantize(cache: QuantKV, rows: Optional[torch.Tensor] = None, n_rows: Optional[int] = None,
@@ -128,8 +128,8 @@ def kv_dequantize(cache: QuantKV, rows: Optional[torch.Tensor] = None, n_rows: O
         raise RuntimeError("kv_dequantize: out holds fewer rows than are read")
     if n_rows == 0:
         return k, v
-    _lib.call("tg_kv_dequantize", *cache._args, cache.n_kv_heads, HEAD_DIM, cache.bits, ptr, n_rows, *k_args, *v_args,
-              _lib.stream_of(cache.k))
+    _lib.call_on(cache.device_index, "tg_kv_dequantize", *cache._args, cache.n_kv_heads, HEAD_DIM, cache.bits, ptr,
+                 n_rows, *k_args, *v_args)
     return k, v
 
 
@@ -180,10 +180,10 @@ def decode_attention_quant(qkv: torch.Tensor, rope: torch.Tensor, lw: LayerWeigh
         raise RuntimeError("decode_attention_quant: out must be bf16 (B, H, 128) rows on qkv's device")
     if B == 0:
         return out
-    _lib.call("tg_decode_attention_quant", qkv.data_ptr(), qkv.stride(0), rope.data_ptr(), B, H, Hkv, D, cache.bits,
-              lw.q_norm.data_ptr(), lw.k_norm.data_ptr(), shape.rms_eps,
-              None if q_head_scale is None else q_head_scale.data_ptr(),
-              None if q_row_scale is None else q_row_scale.data_ptr(), *cache._args, kv_start.data_ptr(),
-              kv_used.data_ptr(), max_k, *bias_args, scale, out.data_ptr(), out.stride(0), workspace.data_ptr(),
-              workspace.numel(), _lib.stream_of(qkv))
+    _lib.call_on(dev, "tg_decode_attention_quant", qkv.data_ptr(), qkv.stride(0), rope.data_ptr(), B, H, Hkv, D,
+                 cache.bits, lw.q_norm.data_ptr(), lw.k_norm.data_ptr(), shape.rms_eps,
+                 None if q_head_scale is None else q_head_scale.data_ptr(),
+                 None if q_row_scale is None else q_row_scale.data_ptr(), *cache._args, kv_start.data_ptr(),
+                 kv_used.data_ptr(), max_k, *bias_args, scale, out.data_ptr(), out.stride(0), workspace.data_ptr(),
+                 workspace.numel())
     return out
