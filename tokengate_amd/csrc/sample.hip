@@ -167,6 +167,25 @@ __device__ __forceinline__ double hist_mass(uint64_t h) {
   return kHistBase * (double)(uint32_t)(h >> 48) + (double)(h & 0xffffffffffffull) * (1.0 / kHistUnit);
 }
 
+template <int CTRL>
+__device__ __forceinline__ uint64_t dpp(uint64_t x) {
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp((int)(uint32_t)x, (int)(uint32_t)x, CTRL, 0xf, 0xf, true);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp((int)(uint32_t)(x >> 32), (int)(uint32_t)(x >> 32), CTRL, 0xf, 0xf, true);
+  return (uint64_t)hi << 32 | lo;
+}
+__device__ __forceinline__ uint64_t wave_max(uint64_t v) {
+  auto step = [](uint64_t x, uint64_t y) { return x > y ? x : y; };
+  v = step(v, dpp<0xB1>(v));     // quad_perm 1 0 3 2
+  v = step(v, dpp<0x4E>(v));     // quad_perm 2 3 0 1
+  v = step(v, dpp<0x141>(v));    // row_half_mirror
+  v = step(v, dpp<0x140>(v));    // row_mirror
+  auto p = __builtin_amdgcn_permlane16_swap((uint32_t)v, (uint32_t)v, false, false);
+  auto q = __builtin_amdgcn_permlane16_swap((uint32_t)(v >> 32), (uint32_t)(v >> 32), false, false);
+  v = step((uint64_t)q[0] << 32 | p[0], (uint64_t)q[1] << 32 | p[1]);
+  p = __builtin_amdgcn_permlane32_swap((uint32_t)v, (uint32_t)v, false, false);
+  q = __builtin_amdgcn_permlane32_swap((uint32_t)(v >> 32), (uint32_t)(v >> 32), false, false);
+  return step((uint64_t)q[0] << 32 | p[0], (uint64_t)q[1] << 32 | p[1]);
+}
 __device__ __forceinline__ uint32_t wave_max(uint32_t v) {
   auto step = [](uint32_t x, uint32_t y) { return x > y ? x : y; };
   v = step(v, (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, 0xB1, 0xf, 0xf, true));    // quad_perm 1 0 3 2
@@ -215,20 +234,43 @@ __device__ __forceinline__ T wave_scan(T x) {
   x = scan_step<0x142, 0xa>(x);   // row_bcast 15: the first row's sum to the second, the third's to the fourth
   return scan_step<0x143, 0xc>(x);   // row_bcast 31: the first half's to the second
 }
-// Sums over the threads up to this one; total: over all.  tmp: 16 of T.
+template <typename T>
+__device__ __forceinline__ T row_scan(T x) {     // of 16 lanes
+  x = scan_step<0x111, 0xf>(x);
+  x = scan_step<0x112, 0xf>(x);
+  x = scan_step<0x114, 0xf>(x);
+  return scan_step<0x118, 0xf>(x);
+}
+__device__ __forceinline__ uint32_t read_lane(uint32_t x, int lane) { return (uint32_t)__builtin_amdgcn_readlane((int)x, lane); }
+__device__ __forceinline__ uint64_t read_lane(uint64_t x, int lane) {
+  return (uint64_t)read_lane((uint32_t)(x >> 32), lane) << 32 | read_lane((uint32_t)x, lane);
+}
+// Sums over the threads up to this one; total: over all.  tmp: 16 of T.  Whole numbers: every wave adds the waves' sums
+// up for itself, one per lane.
 template <typename T>
 __device__ __forceinline__ T block_scan(T v, T *tmp, T &total) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int lane = threadIdx.x & 63, wave = wave_id();
   v = wave_scan(v);
   __syncthreads();
   if (lane == 63) tmp[wave] = v;
   __syncthreads();
-  T before = T(0);
-  total = T(0);
+  const T s = row_scan(tmp[lane & 15]);
+  total = read_lane(s, 15);
+  return v + (wave ? read_lane(s, wave - 1) : T(0));
+}
+// Doubles, for rows that are sorted
+__device__ __forceinline__ double block_scan(double v, double *tmp, double &total) {
+  const int lane = threadIdx.x & 63, wave = wave_id();
+  v = wave_scan(v);
+  __syncthreads();
+  if (lane == 63) tmp[wave] = v;
+  __syncthreads();
+  double before = 0.0;
+  total = 0.0;
 #pragma unroll
   for (int i = 0; i < kThreads / 64; ++i) {
-    const T s = tmp[i];
-    before += i < wave ? s : T(0);
+    const double s = tmp[i];
+    before += i < wave ? s : 0.0;
     total += s;
   }
   return v + before;
@@ -411,7 +453,8 @@ __global__ __launch_bounds__(kThreads, 4) void sample_hist_kernel(SampleArgs a, 
   if (!last_s) return;
 
   // ---- the row's bins ----
-  __shared__ double mass_s[kBins], scan_d[16];
+  __shared__ double mass_s[kBins];
+  __shared__ uint64_t scan_m[16];
   __shared__ uint64_t sums[2][kBins];
   __shared__ uint32_t counts[2][kBins], count_s[kBins], scan_u[16];
   __shared__ int first_s[4], slots[64], finer_s[64], depth[64];
@@ -501,12 +544,13 @@ __global__ __launch_bounds__(kThreads, 4) void sample_hist_kernel(SampleArgs a, 
     count = counts[0][j] + counts[1][j];
     m = exp2_of((0.5 - j) * whole.per_q) * (kHistBase * (double)count + (double)(sums[0][j] + sums[1][j]) * (1.0 / kHistUnit));
   }
-  double in_bins, tail_all;
+  // (as whole numbers: no bin's sum is less than the one's before it, as roundings could make it)
   uint32_t n_bins;
-  const double upto = block_scan(m, scan_d, in_bins);
+  uint64_t in_bins_u, tail_u;
+  const double upto = (double)block_scan((uint64_t)(m * 0x1p44 + 0.5), scan_m, in_bins_u) * 0x1p-44;
   const uint32_t upto_count = block_scan(count, scan_u, n_bins);
-  block_scan(tail, scan_d, tail_all);
-  const double mass = in_bins + tail_all;
+  block_scan((uint64_t)(tail * 0x1p44), scan_m, tail_u);
+  const double in_bins = (double)in_bins_u * 0x1p-44, tail_all = (double)tail_u * 0x1p-44, mass = in_bins + tail_all;
   const bool tail_counts = tail_all > 0x1p-42 * mass;
   if (half == 0) {
     mass_s[j] = upto;
@@ -756,7 +800,9 @@ struct PickShared {
   uint64_t hist[kBins];                          // of 512 parts of an interval of keys, as Part's
   uint64_t key[kTiny], weight[kTiny];            // elements that are compared with one another
   uint64_t got_key, low[16], high[16];
-  double scan[16], above, got_cum, got_weight, bin_mass, bin_upto, bin_over;
+  uint64_t scan[16];
+  double above, got_cum, got_weight, bin_mass, bin_upto, bin_over, unit, mid;
+  uint64_t ends[2];
   uint32_t scan_u[16], n, bin, above_n, in, place;
 };
 
@@ -824,7 +870,7 @@ __global__ __launch_bounds__(kThreads, 4) void sample_pick_kernel(SampleArgs a, 
   // (loops over LDS: unrolled over registers, their doubles' code was fetched for longer than it ran)
   __shared__ uint64_t list[kList];
   const uint64_t first_entry = ld_agent(all + tid);
-  const int n = (int)min(ld_agent(&c->listed), (uint32_t)kList), wave = tid >> 6;
+  const int n = (int)min(ld_agent(&c->listed), (uint32_t)kList), wave = wave_id();
   if (tid < n) list[tid] = first_entry;
   for (int i = tid + kThreads; i < n; i += kThreads) list[i] = ld_agent(all + i);
   auto each = [&](auto f) {                      // (a thread's own)
@@ -857,7 +903,7 @@ __global__ __launch_bounds__(kThreads, 4) void sample_pick_kernel(SampleArgs a, 
         if (j >= (double)m_lo && j <= (double)m_hi && !row.under(v, best, mp))
           sum += (uint64_t)(row.weight(y, top - (double)m_lo) * 0x1p44 + 0.5);
       });
-      block_scan(sum, reinterpret_cast<uint64_t *>(sh.scan), all_sum);
+      block_scan(sum, sh.scan, all_sum);
       const double above = m_lo ? st->upto_mass[m_lo - 1] : 0.0;
       const double sum_m = above + (double)all_sum * (exp2_of(-(double)m_lo * row.per_q) * 0x1p-44);
       if (sum_m < s3) {
@@ -868,32 +914,46 @@ __global__ __launch_bounds__(kThreads, 4) void sample_pick_kernel(SampleArgs a, 
     const bool by_mass = stage > 0;
     const double target = stage == 0 ? (double)k : stage == 1 ? (double)fmaxf(tp, 0.f) * s3 : draw(a, b) * s3;
     auto reaches = [&](double x) { return stage == 2 ? x > target : x >= target; };
+    // the first bin that reaches it (where rounding leaves none, the last), from its thread
     __syncthreads();
+    if (tid < kBins) {
+      const bool here = reaches(by_mass ? upto : (double)upto_n), before = tid > 0 && reaches(by_mass ? over : (double)over_n);
+      if (tid == kBins - 1 ? !before : here && !before) {
+        sh.bin = tid;
+        sh.above = over;
+        sh.above_n = over_n;
+        sh.in = upto_n - over_n;
+        sh.bin_upto = upto;
+        sh.bin_over = over;
+      }
+    }
     if (tid == 0) {
-      sh.bin = kBins - 1;                        // (where rounding leaves none)
       sh.place = ~0u;
       sh.n = 0;
     }
     __syncthreads();
-    if (tid < kBins && reaches(by_mass ? upto : (double)upto_n) && (tid == 0 || !reaches(by_mass ? over : (double)over_n))) sh.bin = tid;
-    __syncthreads();
-    const uint32_t bin = sh.bin;
-    if ((uint32_t)tid == bin) {
-      sh.above = over;
-      sh.above_n = over_n;
-      sh.in = upto_n - over_n;
-      sh.bin_upto = upto;
-      sh.bin_over = over;
+    const uint32_t bin = sh.bin, first_in = sh.in;
+    const double low = top - (double)bin;        // the bin's lower end
+    // what all threads need of the bin, each from one wave (of one SIMD each)
+    if (wave == 0) {
+      const uint32_t o = row.first(low, true);
+      if (lane == 0) sh.ends[0] = (uint64_t)~(o - 1u) << 32;
+    } else if (wave == 1) {
+      const uint32_t o = row.first(low, false);
+      if (lane == 0) sh.ends[1] = (uint64_t)~o << 32 | 0xffffffffu;
+    } else if (wave == 2) {
+      const double w = exp2_of(-(double)bin * row.per_q);
+      if (lane == 0) sh.unit = w * 0x1p-44;
+    } else if (wave == 3) {
+      const double w = exp2_of((0.5 - (double)bin) * row.per_q);
+      if (lane == 0) sh.mid = w;
     }
     __syncthreads();
     double above = sh.above;
-    uint32_t above_n = sh.above_n, in = sh.in;
-    const uint32_t first_in = in;
-    const double low = top - (double)bin;        // the bin's lower end
-    const double unit = exp2_of(-(double)bin * row.per_q) * 0x1p-44, mid = exp2_of((0.5 - (double)bin) * row.per_q);
-    auto units = [&](uint64_t e) { return (uint64_t)(row.weight(row.y(list_value(e)), low) * 0x1p44 + 0.5); };
+    uint32_t above_n = sh.above_n, in = first_in;
+    const double unit = sh.unit, mid = sh.mid;
     // the interval: elements with lo <= key <= hi, at first those of the bin
-    uint64_t lo = (uint64_t)~(row.first(low, true) - 1u) << 32, hi = (uint64_t)~row.first(low, false) << 32 | 0xffffffffu;
+    uint64_t lo = sh.ends[0], hi = sh.ends[1];
     auto mine = [&](uint64_t e) { return e >= lo && e <= hi; };
 #pragma unroll 1
     for (int round = 0; round < 8 && in > kTiny; ++round) {   // (64 bits of keys, 9 and more a round)
@@ -905,24 +965,15 @@ __global__ __launch_bounds__(kThreads, 4) void sample_pick_kernel(SampleArgs a, 
           l = e < l ? e : l;
           r = e > r ? e : r;
         });
-#pragma unroll
-        for (int o = 32; o; o >>= 1) {
-          const uint64_t l2 = __shfl_xor((unsigned long long)l, o), r2 = __shfl_xor((unsigned long long)r, o);
-          l = l2 < l ? l2 : l;
-          r = r2 > r ? r2 : r;
-        }
+        l = ~wave_max(~l);
+        r = wave_max(r);
         if (lane == 0) {
           sh.low[wave] = l;
           sh.high[wave] = r;
         }
         __syncthreads();
-        lo = ~0ull;
-        hi = 0;
-#pragma unroll
-        for (int i = 0; i < kThreads / 64; ++i) {
-          lo = sh.low[i] < lo ? sh.low[i] : lo;
-          hi = sh.high[i] > hi ? sh.high[i] : hi;
-        }
+        lo = ~wave_max(~sh.low[lane & 15]);
+        hi = wave_max(sh.high[lane & 15]);
       } else {
         __syncthreads();
       }
@@ -936,17 +987,17 @@ __global__ __launch_bounds__(kThreads, 4) void sample_pick_kernel(SampleArgs a, 
       __syncthreads();
       const uint64_t h = tid < kBins ? sh.hist[tid] : 0;
       const uint32_t cnt = (uint32_t)(h >> 48);
-      const double m = hist_mass(h) * mid;
+      const double m = hist_mass(h);
       uint32_t all_n;
-      double all_m;
+      uint64_t all_m;
       const uint32_t c_upto = above_n + block_scan(cnt, sh.scan_u, all_n);
-      const double m_upto = above + block_scan(m, sh.scan, all_m);
+      const double m_upto = above + (double)block_scan((uint64_t)(m * 0x1p44), sh.scan, all_m) * (mid * 0x1p-44);
       // (the last where rounding leaves none)
       if (cnt > 0 && (reaches(by_mass ? m_upto : (double)c_upto) || c_upto == above_n + all_n)) atomicMin(&sh.place, (uint32_t)tid);
       __syncthreads();
       const uint32_t part = sh.place;
       if ((uint32_t)tid == part) {
-        sh.above = m_upto - m;
+        sh.above = m_upto - m * mid;
         sh.above_n = c_upto - cnt;
         sh.in = cnt;
       }
@@ -962,32 +1013,36 @@ __global__ __launch_bounds__(kThreads, 4) void sample_pick_kernel(SampleArgs a, 
     each([&](uint64_t e) {
       if (!mine(e)) return;
       const uint32_t at = atomicAdd(&sh.n, 1u);
-      if (at < kTiny) {
-        sh.key[at] = e;
-        sh.weight[at] = units(e);
-      }
+      if (at < kTiny) sh.key[at] = e;
     });
     __syncthreads();
-    const uint32_t m = min(sh.n, (uint32_t)kTiny);
-    uint64_t own = 0, cum = 0;
-    uint32_t rank = 0;
-    if ((uint32_t)tid < m) {
-      own = sh.key[tid];
+    if (wave == 0) {                             // one element per lane
+      const uint32_t m = min(sh.n, (uint32_t)kTiny);
+      const uint64_t own = (uint32_t)lane < m ? sh.key[lane] : ~0ull;
+      const uint64_t weight = (uint32_t)lane < m ? (uint64_t)(row.weight(row.y(list_value(own)), low) * 0x1p44 + 0.5) : 0;
+      sh.weight[lane] = weight;
+      sh.key[lane] = own;
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      uint64_t cum = 0;
+      uint32_t rank = 0;
 #pragma unroll 4
       for (uint32_t i = 0; i < m; ++i) {
         const bool upto_me = sh.key[i] <= own;
         rank += upto_me;
         cum += upto_me ? sh.weight[i] : 0;
       }
-      if (reaches(by_mass ? above + (double)cum * unit : (double)(above_n + rank)) || rank == m) atomicMin(&sh.place, rank);
+      const double mass = above + (double)cum * unit;
+      const bool ok = (uint32_t)lane < m && (reaches(by_mass ? mass : (double)(above_n + rank)) || rank == m);
+      const uint32_t place = ~wave_max(ok ? ~rank : 0u);
+      if ((uint32_t)lane < m) {
+        if (rank == place) {
+          sh.got_key = own;
+          sh.got_cum = mass;
+          sh.got_weight = (double)weight * unit;
+        }
+        if (rank == m) sh.bin_mass = (double)cum * unit;
+      }
     }
-    __syncthreads();
-    if ((uint32_t)tid < m && rank == sh.place) {
-      sh.got_key = own;
-      sh.got_cum = above + (double)cum * unit;
-      sh.got_weight = (double)sh.weight[tid] * unit;
-    }
-    if ((uint32_t)tid < m && rank == m) sh.bin_mass = (double)cum * unit;
     __syncthreads();
     if (row.greedy) break;
     if (stage < 2) {
