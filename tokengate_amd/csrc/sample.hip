@@ -106,23 +106,29 @@ constexpr int kFinest = 12;
 struct Row {
   double q, per_q, cc, per_cc;
   bool greedy;
-  __device__ Row(const SampleArgs &a, int b, int fine) {
+  __device__ Row(const SampleArgs &a, int b) {
     const float t = a.temperature ? a.temperature[b] : 1.f;
     greedy = !(t > 0.f);
     const double temp = greedy ? 1.0 : (double)t;
-    q = ldexp(fmax(4.0, 8.0 * temp), fine);
+    q = fmax(4.0, 8.0 * temp);
     per_q = 1.0 / q;
-    cc = ldexp(temp >= 0.5 ? 8.0 * kLog2e : 4.0 * kLog2e / temp, fine);
-    per_cc = ldexp(temp >= 0.5 ? 0.125 * kLn2 : 0.25 * kLn2 * temp, -fine);
+    cc = temp >= 0.5 ? 8.0 * kLog2e : 4.0 * kLog2e / temp;
+    per_cc = temp >= 0.5 ? 0.125 * kLn2 : 0.25 * kLn2 * temp;
   }
   // the bins' reach, in logits; the finest bins (of a row of fine 0) that reach from most down to least
   __device__ float reach() const { return (float)(kBins * per_cc); }
   __device__ int finest(float most, float least) const {
     const double span = ((double)most - (double)least) * cc;
-    int fine = 0;
-    if (span >= 0.0)                             // (not where nothing is within reach, or both are infinite)
-      while (fine < kFinest && ldexp(span, fine + 1) < kBins - 2) ++fine;
-    return fine;
+    if (!(span >= 0.0)) return 0;                // (nothing is within reach, or both are infinite)
+    static_assert(kBins == 512, "9 bits");
+    const int bits = span > 0.0 ? __builtin_amdgcn_frexp_exp(span) : -64;   // span < 2^bits
+    return max(0, min(kFinest, 9 - bits - (ldexp(span, 9 - bits) < kBins - 2 ? 0 : 1)));
+  }
+  __device__ Row(const Row &coarse, int fine) : Row(coarse) {
+    q = ldexp(q, fine);
+    per_q = ldexp(per_q, -fine);
+    cc = ldexp(cc, fine);
+    per_cc = ldexp(per_cc, -fine);
   }
   // (+inf: so far above every finite one that those weigh nothing)
   __device__ double y(float x) const { return x == INFINITY ? 0x1p1000 : (double)x * cc; }
@@ -309,7 +315,7 @@ __global__ __launch_bounds__(kThreads) void sample_small_kernel(SampleArgs a) {
   __shared__ double scan[16], mass_s[2];
   const int b = blockIdx.x, tid = threadIdx.x, n = a.n;
   const float *x = a.x + b * a.rs;
-  const Row row(a, b, 0);
+  const Row row(a, b);
   for (int i = tid; i < n; i += kThreads) list[i] = (uint64_t)~order_bits(x[i]) << 32 | (uint32_t)i;
   const int per = (sort_list(list, n) + kThreads - 1) / kThreads;   // elements of a thread, in order
   const float best = list_value(list[0]);
@@ -408,7 +414,7 @@ __global__ __launch_bounds__(kThreads, 4) void sample_hist_kernel(SampleArgs a, 
   __shared__ uint32_t last_s;
   const Share share(a.n);
   float most = -INFINITY, least = INFINITY;      // (maxima of pairs drop NaN)
-  const Row coarse(a, b, 0);
+  const Row coarse(a, b);
   const float reach = coarse.reach();
   // least: of what lies within reach of the largest; what lies below, as a finite mask does, may not count
   share.each(x, [&](float v, int) {
@@ -422,7 +428,7 @@ __global__ __launch_bounds__(kThreads, 4) void sample_hist_kernel(SampleArgs a, 
   uint32_t best = block_max(order_bits(most), tmp);   // (its barriers cover the bins)
   const uint32_t low_bits = ~block_max(least > order_float(best) - reach ? ~order_bits(least) : 0u, tmp);
   const int fine = low_bits == ~0u ? 0 : coarse.finest(order_float(best), order_float(low_bits));
-  const Row row(a, b, fine);
+  const Row row(coarse, fine);
   const double top = best == kNone ? 0.0 : floor(row.y(order_float(best)));
   const double scale = kLn2 * row.per_q;
   const int top_slot = slot_of(top);
@@ -487,7 +493,7 @@ __global__ __launch_bounds__(kThreads, 4) void sample_hist_kernel(SampleArgs a, 
   const uint32_t least_row = ~wave_max(near_top ? ~part_least : 0u);
   int fine_row = kFinest - (int)wave_max(part_best == kNone ? 0u : kFinest - part_fine);
   fine_row = least_row == ~0u ? 0 : min(fine_row, coarse.finest(order_float(best), order_float(least_row)));
-  const Row whole(a, b, fine_row);
+  const Row whole(coarse, fine_row);
   const double gtop = floor(whole.y(order_float(best))), scale_row = kLn2 * whole.per_q;
   const int part_finer = part_best == kNone ? 0 : (int)part_fine - fine_row;
   if (tid < parts) {
@@ -813,7 +819,7 @@ __global__ __launch_bounds__(kThreads, 4) void sample_pick_kernel(SampleArgs a, 
   const uint32_t slow = st->slow;
   const double top = st->top;
   const uint64_t mask_bits = st->mask[tid & (kBins / 64 - 1)];
-  const Row row(a, b, (int)st->fine);
+  const Row row(Row(a, b), (int)st->fine);
   if (slow != kUsual) {
     if (g == 0 && slow == kSlow) slow_row(a, b);
     return;
