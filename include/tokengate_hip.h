@@ -429,11 +429,13 @@ int tg_argmax_rows(const float *x, int64_t x_row_stride, int32_t n_rows, int64_t
  * elements of S2 with w >= min_p[b], at least one (no min_p: S2); token[b] (int64) = the first of S3 whose
  * cumulated mass exceeds u[b] times S3's, logprob[b] (optional, fp32) = ln(w / mass of S3) of it.
  * temperature <= 0 or NaN: the first of the order, log probability 0; no temperature: 1.  A NaN logit counts as
- * -inf; among infinite logits only the equal ones count; a row of -inf gives token 0.  Weights are whole numbers
- * of 2^-44 (fp32 exponentials, exact sums): the result does not depend on the launch.  x: fp32 rows of any stride
- * and alignment, at most 262144 columns; the settings and u are dense device arrays with an entry per row.
- * One launch's counters are zero again when it ends; workspace: tg_sample_rows_workspace_size bytes, zeroed once
- * when it is allocated, shared by the launches of one stream, of any sizes that it holds (launches that may overlap
+ * -inf; among infinite logits only the equal ones count; a row of -inf gives token 0.  Weights are doubles, a logit's
+ * share of a sum is rounded to 2^-34 of it, and sums are whole numbers of any order: the result does not depend on the
+ * launch.  x: fp32 rows of any stride >= n_cols and alignment, at most 65535 of at most 262144 columns; the settings and
+ * u (below 0 counts as 0, 1 and more as just below 1) are dense device arrays with an entry per row.  Rows of up to 2048
+ * columns take one launch and no workspace, longer ones two per 256 rows.  workspace: tg_sample_rows_workspace_size bytes,
+ * 16-byte aligned, zeroed once when it is allocated (its counters are zero again when a call's launches end), shared by
+ * the calls of one stream, of any sizes that it holds (calls that may overlap, from two streams or two replayed graphs,
  * need one each). */
 int64_t tg_sample_rows_workspace_size(int32_t n_rows, int64_t n_cols);
 int tg_sample_rows(const float *x, int64_t x_row_stride, int32_t n_rows, int64_t n_cols, const float *u,
@@ -469,8 +471,10 @@ int tg_kv_dequantize(const void *k_codes, const void *k_meta, const void *v_code
  * kv_start[b] .. kv_start[b] + kv_used[b] - 1 as they are held, the new row included, values s c + m not rounded to
  * bf16.  A bias of -inf hides a row whatever it holds; a head that sees no row gets zeros.  A sequence whose rows
  * are not all inside the cache, or kv_used[b] <= 0, appends nothing and gets zeros; kv_used[b] > max_seqlen_k: the
- * first max_seqlen_k rows, of which the last is the new one.  workspace: as for tg_decode_attention,
- * tg_decode_attention_quant_workspace_size bytes. */
+ * first max_seqlen_k rows, of which the last is the new one.  No sequence may append a row that another one reads or
+ * appends.  workspace: tg_decode_attention_quant_workspace_size bytes (0: NULL will do), 16-byte aligned, zeroed once
+ * when it is allocated, shared by the launches of one stream, of any sizes that it holds; launches that may overlap, from
+ * two streams or two replayed graphs, need one each.  max_seqlen_k < 2^24. */
 int64_t tg_decode_attention_quant_workspace_size(int32_t num_seqs, int32_t num_heads, int32_t num_heads_k,
                                                  int32_t max_seqlen_k);
 int tg_decode_attention_quant(const void *qkv, int64_t qkv_row_stride, const float *rope, int32_t num_seqs,

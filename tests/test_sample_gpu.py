@@ -1,10 +1,11 @@
 """sample_rows against the definition in float64 (numpy, by sorting).
 
-The kernel's weights are good to 2^-40 and rounded to 2^-45 of the largest, and their sums are exact: up to 2^18 such
-roundings come to 2^-27 at worst and 2^-36 at random.  So its choices equal the definition's wherever the numbers that
-decide are apart from their borders by more than 2^-34: u times the kept mass from the cumulated masses around it,
-top_p times the mass from those, and min_p from the weights.  Rows that are nearer (2^18 borders times 2^-33: one in
-thirty thousand at most) are left out, and their number is checked.  Log probabilities are rounded to fp32, 2^-24."""
+The kernel's sums are exact but for the rounding of every logit's share to a whole number: of 2^-33 of the largest that
+its bin can hold, or of 2^-44 in the bins that decide, so at most 2^-34 of the share and of the sum.  So its choices equal
+the definition's wherever the numbers that decide are apart from their borders by more than 2^-34: u times the kept mass
+from the cumulated masses around it, top_p times the mass from those, and min_p from the weights.  Rows that are nearer
+(2^18 borders times 2^-33: one in thirty thousand at most) are left out, and their number is checked.  Log probabilities
+are rounded to fp32, 2^-24."""
 import numpy as np
 import pytest
 import torch

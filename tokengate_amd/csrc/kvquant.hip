@@ -169,7 +169,8 @@ struct RowSource {
 };
 // A wave takes one head of K or V of 16 rows (kRows = 4 at a time: 4 rows of 16 lanes, 16 bytes each, all four
 // requested at once; their codes are stored as 256 contiguous bytes).  Blocks go by head first, so that the rows that
-// are read at one time are whole.
+// are read at one time are whole.  Bound by the bytes: 98765 rows of 8 heads at 4 bits (K and V, 534 MB) 108 to 126 us,
+// 4.9 to 4.2 TB/s, and read back 109 to 120, by the box; 4096 rows at 8 bits (26 MB) 7.3 and 6.6; one launch, 3 us, for a few.
 constexpr int kRows = 4;
 template <int BITS>
 __global__ __launch_bounds__(256) void kv_quantize_kernel(RowSource a, QuantCache c, int64_t n, int heads) {
@@ -259,6 +260,10 @@ __global__ __launch_bounds__(256) void kv_dequantize_kernel(QuantCache c, RowTar
 //   * The new key is not in the tiles: it is a part of its own beside the waves', from registers.
 //   * The running maximum moves only when a logit passes it by 2^8.  Waves merge in LDS, chunks through the
 //     workspace in the workgroup that arrives last.
+// Measured, 16 / 8 heads: 4 bits, one sequence of 1, 300, 2320, 32769, 131072 keys 6.0, 9.7, 10.5, 22, 44 us (over a bf16
+// cache by tg_decode_attention 2320 13, 32769 36); 64 x 4096 71 (4.7 TB/s; bf16 191), 8 x 80000 152 (5.4 TB/s); 8 bits
+// 6.0, 10.6, 11.8, 27, 64; 113 (5.4), 259 (5.7).  A short sequence is bound by its chain of latencies: launch, lengths
+// and norms 4.9 us, the waves' merge 1.5, arrival 1.8, the chunks' merge 2.7, beside the tiles.
 struct QuantAttnArgs {
   const bf16_t *qkv;
   int64_t qkv_rs;
@@ -285,7 +290,10 @@ struct QuantAttnArgs {
 constexpr int kWaves = 4;
 constexpr int kRounds = 2;
 constexpr int kTile = 64;        // keys of a wave's step
-// Tiles that a wave holds or has on their way, and workgroups per CU, by the registers
+// Tiles that a wave holds or has on their way, and workgroups per CU, by the registers.  16 / 8 heads (two at once), 4
+// bits, two tiles and 2 workgroups / one and 3: 32769 keys 22.0 / 23.3 us, 64 x 4096 71.4 / 70.6, with bias 72.9 /
+// 73.8; 8 bits, where two tiles spill: 28.7 / 26.9, 119.4 / 112.6, 137 / 118.  Four heads at once, one tile, 2 / 3
+// workgroups (spills): 4 x 8192 keys of 16 / 2 heads 20.5 / 24.4 at 4 bits, 22.4 / 32.5 at 8.
 constexpr int depth(int bits, int hp) { return bits == 4 && hp <= 2 ? 2 : 1; }
 __host__ __device__ constexpr int per_cu(int bits, int hp) { return depth(bits, hp) == 2 || hp == 4 ? 2 : 3; }
 constexpr float kRescaleTau = 8.f;
@@ -341,7 +349,8 @@ __device__ __forceinline__ uint32_t byte_pair(uint32_t a, uint32_t b, int byte) 
 // ceil(n / T) chunks of even length, with one T for all, from their tiles, which only the device knows: the least that
 // makes no more workgroups than are resident at once (a workgroup's fixed costs, 5 us, and a second round's uneven
 // end cost more than idle places), or, where the sequences' remainders alone would fill most of these, two
-// rounds.  16 / 8 heads, T for one round of the longest sequence / two rounds / as here, us: 64 sequences of 512 .. 4099
+// rounds.  (64 sequences of 300 at 8 bits in chunks of four tiles, a round and a third: 24.9 us; cut for one round: 17.5.)
+// 16 / 8 heads, T for one round of the longest sequence / two rounds / as here, us: 64 sequences of 512 .. 4099
 // at 8 bits 84.7 / 84.3 / 79.8; 8 of 16k .. 128k at 4 bits 183 / 170 / 159; 16 of 4k .. 30k - / 63 / 57; 64 alike of
 // 4096 70 / 77 / 70.
 struct Chunk {
@@ -381,7 +390,8 @@ __device__ __forceinline__ Chunk find_chunk(const QuantAttnArgs &a, int q, int l
   const float work = (float)count(1, true) * (float)a.sets, slots = (float)a.slots;
   float target = slots;
   int T = max(a.least, (int)(work / target) + 1);
-  for (int i = 0; i < 3 && T > a.least; ++i) {
+  // (where not even an even cut of every sequence would fill one round, nothing is counted)
+  for (int i = 0; i < 3 && work / (float)T + (float)a.nseq * (float)a.sets > slots; ++i) {
     const float over = (float)count(T, false) * (float)a.sets - slots;
     if (over <= 0.f) break;
     if (over > 0.75f * slots) {
@@ -389,7 +399,7 @@ __device__ __forceinline__ Chunk find_chunk(const QuantAttnArgs &a, int q, int l
       break;
     }
     target = fmaxf(target - over, 0.25f * slots);
-    T = (int)(work / target) + 1;
+    T = max(T + 1, (int)(work / target) + 1);
   }
   const float inv = 1.f / (float)T;
   int before = 0;

@@ -582,7 +582,8 @@ def sample_rows(logits: torch.Tensor, u: torch.Tensor, temperature: Optional[tor
     min_p times the best one's probability; u picks by cumulated mass in that order.  The settings are (B,) tensors
     (fp32; top_k int32) or None; temperature 0 is greedy, top_k 0, top_p 1 and min_p 0 keep everything.  With
     logprob also the tokens' log probabilities (B,) fp32 in the distribution that was sampled.  workspace:
-    sample_rows_workspace, kept between calls of one stream (None: a new one)."""
+    sample_rows_workspace, kept between calls of one stream (None: a new one); calls that may overlap, and graphs
+    that may be replayed at once, need one each."""
     if logits.dtype != torch.float32 or logits.dim() != 2 or logits.shape[1] < 1 or logits.stride(1) != 1:
         raise RuntimeError("sample_rows: logits must be fp32 (B, V) rows")
     n, V = logits.shape

@@ -135,7 +135,7 @@ def kv_dequantize(cache: QuantKV, rows: Optional[torch.Tensor] = None, n_rows: O
 
 def decode_attention_quant_workspace(n_seqs: int, shape: DecoderShape, max_k: int, device) -> torch.Tensor:
     """Zeroed workspace for decode_attention_quant calls of up to n_seqs sequences and max_k keys (its counters
-    stay zero between calls)."""
+    stay zero between calls), for one stream: calls that may overlap need one each."""
     n = int(_lib.load().tg_decode_attention_quant_workspace_size(n_seqs, shape.n_heads, shape.n_kv_heads, int(max_k)))
     return torch.zeros(max(n, 16), dtype=torch.uint8, device=device)
 
@@ -148,7 +148,8 @@ def decode_attention_quant(qkv: torch.Tensor, rope: torch.Tensor, lw: LayerWeigh
     """decoder.decode_attention over a quantised cache in one launch (tg_decode_attention_quant): the new key and
     value of sequence b are quantised into cache row kv_start[b] + kv_used[b] - 1, and its query attends over rows
     kv_start[b] .. kv_start[b] + kv_used[b] - 1 as they are held (s c + m, not rounded to bf16); bias_raw
-    (nseq, H, >= max_k) as decode_attention; a bias of -inf hides a row whatever it holds."""
+    (nseq, H, >= max_k) as decode_attention; a bias of -inf hides a row whatever it holds.  No sequence may append
+    a row that another one reads or appends."""
     H, Hkv, D = shape.n_heads, shape.n_kv_heads, shape.head_dim
     dev = qkv.get_device()
     if qkv.dtype is not torch.bfloat16 or qkv.dim() != 2 or qkv.shape[1] < (H + 2 * Hkv) * D or qkv.stride(1) != 1:
