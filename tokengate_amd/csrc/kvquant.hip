@@ -169,7 +169,7 @@ struct RowSource {
 };
 // A wave takes one head of K or V of 16 rows (kRows = 4 at a time: 4 rows of 16 lanes, 16 bytes each, all four
 // requested at once; their codes are stored as 256 contiguous bytes).  Blocks go by head first, so that the rows that
-// are read at one time are whole.  Bound by the bytes: 98765 rows of 8 heads at 4 bits (K and V, 534 MB) 108 to 126 us,
+// are read at one time are whole.  Bound by the bytes: 98765 rows of 8 heads at 4 bits (K and V, 531 MB) 108 to 126 us,
 // 4.9 to 4.2 TB/s, and read back 109 to 120, by the box; 4096 rows at 8 bits (26 MB) 7.3 and 6.6; one launch, 3 us, for a few.
 constexpr int kRows = 4;
 template <int BITS>
