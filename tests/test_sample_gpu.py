@@ -239,3 +239,15 @@ def test_log_probability_of_nearly_all_the_mass(cuda):
         lp = check(cuda, z, [0.4] * 5, None, None, None, None)[1].cpu().double()
         want = -torch.log1p(torch.exp(z[:, v - 5].double() - z[:, 4].double()))
         assert bool(((lp - want).abs() <= (2.0 ** -24 + 2.0 ** -33) * want.abs() + 2.0 ** -43).all()), (lp, want)
+
+
+@pytest.mark.parametrize("v", [2049, 13117, 31947])
+def test_one_token_left_of_many_that_weigh_little(cuda, v):
+    """top_k leaves some tokens with 2^-30 .. 2^-45 of the mass beside the best one, top_p or min_p then leaves it alone:
+    its log probability is 0, whichever of the masses a rounding makes the larger."""
+    n = 64
+    x = logits(n, v, v, std=0.5)
+    x[torch.arange(n), (torch.arange(n) * 997) % v] = 14.0 + torch.linspace(0, 3, n)
+    for k, p, m in ((50, 0.0, 0.0), (0, 0.3, 0.0), (1000, 0.8, 1.0), (0, 1.0, 1.0), (20, 1.0, 0.5)):
+        lp = check(cuda, x, [0.6] * n, [0.45] * n, [k] * n, [p] * n, [m] * n)[1]
+        assert bool((lp == 0).all()), (k, p, m, lp)

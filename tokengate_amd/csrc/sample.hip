@@ -893,6 +893,7 @@ __global__ __launch_bounds__(kThreads, 4) void sample_pick_kernel(SampleArgs a, 
   };
   double s3 = st->mass;                          // of S1, of S2, of S3: bins 0 .. from_hist - 1 as the first launch has them
   uint32_t from_hist = kBins;
+  uint64_t end_key = ~0ull;                      // its last element
   __syncthreads();
   if (tid == 0) {
     st_agent(&c->listed, 0u);
@@ -910,17 +911,23 @@ __global__ __launch_bounds__(kThreads, 4) void sample_pick_kernel(SampleArgs a, 
     if (stage == 0 && !(k && (uint32_t)k <= in_bins)) continue;
     if (stage == 1 && !(tp < 1.f)) continue;
     if (stage == 2 && mp > 0.f && m_lo < kBins) {   // S3: also what reaches min_p, the bins above m_lo and elements of m_lo .. m_hi
-      uint64_t sum = 0, all_sum;
+      uint64_t sum = 0, all_sum, end_m = 0;
       each([&](uint64_t e) {
         const float v = list_value(e);
         const double y = row.y(v), j = top - floor(y);
-        if (j >= (double)m_lo && j <= (double)m_hi && !row.under(v, best, mp))
+        if (j >= (double)m_lo && j <= (double)m_hi && !row.under(v, best, mp)) {
           sum += (uint64_t)(row.weight(y, top - (double)m_lo) * 0x1p44 + 0.5);
+          end_m = e > end_m ? e : end_m;
+        }
       });
+      end_m = wave_max(end_m);
+      if (lane == 0) sh.high[wave] = end_m;      // (the scan's barriers stand before and behind its reads)
       block_scan(sum, sh.scan, all_sum);
       const double above = m_lo ? st->upto_mass[m_lo - 1] : 0.0;
       const double sum_m = above + (double)all_sum * (exp2_of(-(double)m_lo * row.per_q) * 0x1p-44);
-      if (sum_m < s3) {
+      end_m = wave_max(sh.high[lane & 15]);      // 0: what reaches min_p ends above m_lo
+      const uint64_t first_m = (uint64_t)~(row.first(top - (double)m_lo, true) - 1u) << 32;   // the least key of m_lo
+      if ((end_m ? end_m : first_m - 1) < end_key) {
         s3 = sum_m;
         from_hist = (uint32_t)m_lo;
       }
@@ -1060,9 +1067,10 @@ __global__ __launch_bounds__(kThreads, 4) void sample_pick_kernel(SampleArgs a, 
     __syncthreads();
     if (row.greedy) break;
     if (stage < 2) {
-      if (sh.got_cum < s3) {
+      if (sh.got_key <= end_key) {               // (a rounding could put S2's behind S1's)
         s3 = sh.got_cum;
         from_hist = bin;
+        end_key = sh.got_key;
       }
     } else if (first_in <= kTiny && bin < from_hist) {
       // the whole bin is S3's: its sum from its elements' 2^-44 instead of 2^-34, so that the logarithm of a token with
