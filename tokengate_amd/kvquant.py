@@ -118,14 +118,15 @@ def kv_dequantize(cache: QuantKV, rows: Optional[torch.Tensor] = None, n_rows: O
         n_rows = rows.numel() if rows is not None else cache.rows
     ptr = _row_map("kv_dequantize", rows, n_rows, cache)
     if out is None:
-        shape = (n_rows, cache.n_kv_heads, HEAD_DIM)
-        out = (torch.empty(shape, dtype=torch.bfloat16, device=cache.k.device),
-               torch.empty(shape, dtype=torch.bfloat16, device=cache.k.device))
-    k, v = out
-    k_args, n = _bf16_rows("kv_dequantize", k, cache)
-    v_args, n_v = _bf16_rows("kv_dequantize", v, cache)
-    if n < n_rows or n_v < n_rows:
-        raise RuntimeError("kv_dequantize: out holds fewer rows than are read")
+        shape, dev, stride = (n_rows, cache.n_kv_heads, HEAD_DIM), cache.k.device, cache.n_kv_heads * HEAD_DIM
+        k, v = (torch.empty(shape, dtype=torch.bfloat16, device=dev), torch.empty(shape, dtype=torch.bfloat16, device=dev))
+        k_args, v_args = (k.data_ptr(), stride, HEAD_DIM), (v.data_ptr(), stride, HEAD_DIM)
+    else:
+        k, v = out
+        k_args, n = _bf16_rows("kv_dequantize", k, cache)
+        v_args, n_v = _bf16_rows("kv_dequantize", v, cache)
+        if n < n_rows or n_v < n_rows:
+            raise RuntimeError("kv_dequantize: out holds fewer rows than are read")
     if n_rows == 0:
         return k, v
     _lib.call_on(cache.device_index, "tg_kv_dequantize", *cache._args, cache.n_kv_heads, HEAD_DIM, cache.bits, ptr,
