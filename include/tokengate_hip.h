@@ -460,7 +460,7 @@ int tg_kv_quantize(const void *k, int64_t k_row_stride, int64_t k_head_stride, c
                    void *v_codes, void *v_meta, int64_t cache_rows, int64_t head_rows, hipStream_t stream);
 
 /* Cache rows rows[t] (NULL: t), t < n_rows, as bf16(s c + m) to row t of k_out and v_out; an entry outside the
- * cache gives zeros. */
+ * cache gives zeros.  Strides as there; the rows of an output may not overlap. */
 int tg_kv_dequantize(const void *k_codes, const void *k_meta, const void *v_codes, const void *v_meta,
                      int64_t cache_rows, int64_t head_rows, int32_t num_heads_k, int32_t head_dim, int32_t bits,
                      const int32_t *rows, int64_t n_rows, void *k_out, int64_t k_row_stride, int64_t k_head_stride,

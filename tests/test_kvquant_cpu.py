@@ -170,3 +170,12 @@ def test_calls_on_another_device(monkeypatch):
     _lib.call_on(0, "a", 1)
     _lib.call_on(3, "b", 2)
     assert seen == [("a", (1, 100), 0), ("b", (2, 103), 3)] and on == [0]
+
+
+def test_outputs_that_overlap(ptr):
+    """Read-back into rows that share memory is refused."""
+    p = ptr[0]
+    read = dict(kc=p, km=p, vc=p, vm=p, rows=4, head_rows=4, hkv=2, d=128, bits=8, map=None, n=4, k=p, k_rs=256, k_hs=128,
+                v=p, v_rs=128, v_hs=512, stream=None)
+    for change in (dict(k_rs=0), dict(v_rs=64), dict(k_rs=128), dict(v_hs=384), dict(v_rs=0, v_hs=128)):
+        assert "overlap" in _call("tg_kv_dequantize", read, **change), change

@@ -459,3 +459,30 @@ def test_many_ragged_sequences(cuda, used, H, Hkv, checked):
     a, b = got.float(), out[some].float()
     assert bool(((a - b).abs() <= 2.0 ** -7 * a.abs() + 2.0 ** -7 * a.abs().amax(-1, keepdim=True)).all())
     assert all(bool((out[i] == 0).all()) for i in range(B) if used[i] == 0)
+
+
+def test_strides_of_single_rows(cuda):
+    """A dimension of one entry may have any stride; head-major and padded outputs."""
+    from tokengate_amd import kvquant as Q
+    g = torch.Generator(device=cuda).manual_seed(5)
+    k, v = (torch.randn(6, 3, 128, generator=g, device=cuda).bfloat16() for _ in range(2))
+    c = Q.QuantKV.alloc(6, 3, 8, cuda)
+    Q.kv_quantize(k, v, c)
+    want = Q.kv_dequantize(c)
+    heads = tuple(torch.empty(3, 6, 128, dtype=torch.bfloat16, device=cuda).transpose(0, 1) for _ in range(2))
+    wide = tuple(torch.empty(6, 4, 136, dtype=torch.bfloat16, device=cuda)[:, 1:, :128] for _ in range(2))
+    for out in (heads, wide):
+        got = Q.kv_dequantize(c, out=out)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    one = Q.QuantKV.alloc(1, 3, 8, cuda)
+    odd = lambda t: t[:1].contiguous().as_strided((1, 3, 128), (3, 128, 1))
+    Q.kv_quantize(odd(k), odd(v), one)
+    got = Q.kv_dequantize(one, out=tuple(odd(torch.empty_like(t)) for t in (k, v)))
+    assert all(torch.equal(a, b[:1]) for a, b in zip(got, want))
+    # a decode step of one sequence whose row has a stride of nothing
+    case = attn_case(cuda, [70], 1, 16, 8, 4, 9, False, False)
+    ws = Q.decode_attention_quant_workspace(1, case["shape"], case["max_k"], cuda)
+    a = run_attn(case, clone_cache(case["cache"]), ws)
+    row = case["qkv"][0].clone()
+    b = run_attn(dict(case, qkv=row.as_strided((1, row.numel()), (3, 1))), clone_cache(case["cache"]), ws)
+    assert torch.equal(a, b)

@@ -170,7 +170,7 @@ struct RowSource {
 // A wave takes one head of K or V of 16 rows (kRows = 4 at a time: 4 rows of 16 lanes, 16 bytes each, all four
 // requested at once; their codes are stored as 256 contiguous bytes).  Blocks go by head first, so that the rows that
 // are read at one time are whole.  Bound by the bytes: 98765 rows of 8 heads at 4 bits (K and V, 531 MB) 108 to 126 us,
-// 4.9 to 4.2 TB/s, and read back 109 to 120, by the box; 4096 rows at 8 bits (26 MB) 7.3 and 6.6; one launch, 3 us, for a few.
+// 4.9 to 4.2 TB/s, and read back 109 to 120, by the card; 4096 rows at 8 bits (26 MB) 7.3 and 6.6; one launch, 3 us, for a few.
 constexpr int kRows = 4;
 template <int BITS>
 __global__ __launch_bounds__(256) void kv_quantize_kernel(RowSource a, QuantCache c, int64_t n, int heads) {
@@ -937,6 +937,10 @@ extern "C" int tg_kv_dequantize(const void *k_codes, const void *k_meta, const v
   if (int e = check_rows("kv_dequantize", k_out, k_row_stride, k_head_stride, v_out, v_row_stride, v_head_stride, n_rows, num_heads_k))
     return e;
   TG_CHECK(rows || n_rows <= cache_rows, "kv_dequantize: more rows than the cache holds");
+  auto apart = [&](int64_t rs, int64_t hs) {     // rows of all heads, or heads of all rows, one behind another
+    return (n_rows <= 1 || rs >= kHeadDim) && (n_rows <= 1 || num_heads_k == 1 || rs >= num_heads_k * hs || hs >= n_rows * rs);
+  };
+  TG_CHECK(apart(k_row_stride, k_head_stride) && apart(v_row_stride, v_head_stride), "kv_dequantize: rows of the outputs overlap");
   if (n_rows == 0) return 0;
   const RowTarget a{static_cast<bf16_t *>(k_out), static_cast<bf16_t *>(v_out), k_row_stride, k_head_stride, v_row_stride,
                     v_head_stride, rows};

@@ -84,7 +84,7 @@ def _bf16_rows(what: str, t: torch.Tensor, cache: QuantKV):
         n, hkv, d = t.shape
         rs, hs, es = t.stride()
         if hkv == cache.n_kv_heads and d == HEAD_DIM and es == 1:
-            return (t.data_ptr(), rs, hs if hkv > 1 else HEAD_DIM), n
+            return (t.data_ptr(), rs if n > 1 else hkv * HEAD_DIM, hs if hkv > 1 else HEAD_DIM), n
     raise RuntimeError(f"{what}: k and v must be bf16 (rows, {cache.n_kv_heads}, 128) on the cache's device, values "
                        "contiguous")
 
@@ -113,7 +113,7 @@ def kv_dequantize(cache: QuantKV, rows: Optional[torch.Tensor] = None, n_rows: O
                   out: Optional[Tuple[torch.Tensor, torch.Tensor]] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """(k, v) (n_rows, Hkv, 128) bf16 of the cache rows rows[t] (int32; default t) in one launch
     (tg_kv_dequantize): bf16(s c + m).  n_rows defaults to an entry of the map, else every row; an entry outside
-    the cache reads as 0.  out: two bf16 tensors to write to (at least n_rows rows)."""
+    the cache reads as 0.  out: two bf16 tensors to write to (at least n_rows rows, none of which overlap)."""
     if n_rows is None:
         n_rows = rows.numel() if rows is not None else cache.rows
     ptr = _row_map("kv_dequantize", rows, n_rows, cache)
@@ -182,10 +182,10 @@ def decode_attention_quant(qkv: torch.Tensor, rope: torch.Tensor, lw: LayerWeigh
         raise RuntimeError("decode_attention_quant: out must be bf16 (B, H, 128) rows on qkv's device")
     if B == 0:
         return out
-    _lib.call_on(dev, "tg_decode_attention_quant", qkv.data_ptr(), qkv.stride(0), rope.data_ptr(), B, H, Hkv, D,
-                 cache.bits, lw.q_norm.data_ptr(), lw.k_norm.data_ptr(), shape.rms_eps,
+    _lib.call_on(dev, "tg_decode_attention_quant", qkv.data_ptr(), qkv.stride(0) if B > 1 else (H + 2 * Hkv) * D,
+                 rope.data_ptr(), B, H, Hkv, D, cache.bits, lw.q_norm.data_ptr(), lw.k_norm.data_ptr(), shape.rms_eps,
                  None if q_head_scale is None else q_head_scale.data_ptr(),
                  None if q_row_scale is None else q_row_scale.data_ptr(), *cache._args, kv_start.data_ptr(),
-                 kv_used.data_ptr(), max_k, *bias_args, scale, out.data_ptr(), out.stride(0), workspace.data_ptr(),
-                 workspace.numel())
+                 kv_used.data_ptr(), max_k, *bias_args, scale, out.data_ptr(),
+                 out.stride(0) if B > 1 else H * D, workspace.data_ptr(), workspace.numel())
     return out
