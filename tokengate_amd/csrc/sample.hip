@@ -155,6 +155,20 @@ struct Row {
     return x != best && (x == -INFINITY || weight(y(x), y(best)) < fmin((double)least, 1.0));
   }
 };
+// The other settings: top_k as 0 where it leaves everything, 1 where the row is greedy
+struct Settings {
+  int k;
+  float tp, mp;
+  double u;
+  __device__ Settings(const SampleArgs &a, int b, bool greedy) {
+    const int top_k = a.top_k ? a.top_k[b] : 0;
+    const float top_p = a.top_p ? a.top_p[b] : 1.f, min_p = a.min_p ? a.min_p[b] : 0.f, u0 = a.u[b];
+    k = greedy ? 1 : top_k > 0 && top_k < a.n ? top_k : 0;
+    tp = greedy ? 1.f : top_p;
+    mp = greedy ? 0.f : min_p;
+    u = fmin(fmax((double)u0, 0.0), 1.0 - 0x1p-30);
+  }
+};
 // u[b]; a one, which a rounded number may be, takes the last element of a mass of more than 2^-30
 __device__ __forceinline__ double draw(const SampleArgs &a, int b) { return fmin(fmax((double)a.u[b], 0.0), 1.0 - 0x1p-30); }
 
@@ -271,6 +285,29 @@ __device__ __forceinline__ T block_scan(T v, T *tmp, T &total) {
   const T s = row_scan(tmp[lane & 15]);
   total = read_lane(s, 15);
   return v + (wave ? read_lane(s, wave - 1) : T(0));
+}
+// Three at once: of u and v the sums up to this thread, of w the sum of all; total: u's of all.
+__device__ __forceinline__ void block_scan3(uint64_t &u, uint32_t &v, uint64_t &w, uint64_t *tmp_u, uint32_t *tmp_v, uint64_t *tmp_w,
+                                            uint64_t &total) {
+  const int lane = threadIdx.x & 63, wave = wave_id();
+  u = wave_scan(u);
+  v = wave_scan(v);
+  w = wave_scan(w);
+  __syncthreads();
+  if (lane == 63) {
+    tmp_u[wave] = u;
+    tmp_v[wave] = v;
+    tmp_w[wave] = w;
+  }
+  __syncthreads();
+  const uint64_t su = row_scan(tmp_u[lane & 15]), sw = row_scan(tmp_w[lane & 15]);
+  const uint32_t sv = row_scan(tmp_v[lane & 15]);
+  total = read_lane(su, 15);
+  w = read_lane(sw, 15);
+  if (wave) {
+    u += read_lane(su, wave - 1);
+    v += read_lane(sv, wave - 1);
+  }
 }
 // Doubles, for rows that are sorted
 __device__ __forceinline__ double block_scan(double v, double *tmp, double &total) {
@@ -423,6 +460,7 @@ __global__ __launch_bounds__(kThreads, 4) void sample_hist_kernel(SampleArgs a, 
   const Share share(a.n);
   float most = -INFINITY, least = INFINITY;      // (maxima of pairs drop NaN)
   const Row coarse(a, b);
+  const Settings set(a, b, coarse.greedy);       // (for the last workgroup: here their loads take no time of their own)
   const float reach = coarse.reach();
   // least: of what lies within reach of the largest; what lies below, as a finite mask does, may not count
   share.each(x, [&](float v, int) {
@@ -468,10 +506,18 @@ __global__ __launch_bounds__(kThreads, 4) void sample_hist_kernel(SampleArgs a, 
 
   // ---- the row's bins ----
   __shared__ double mass_s[kBins];
-  __shared__ uint64_t scan_m[16];
+  __shared__ uint64_t scan_m[16], scan_t[16];
   __shared__ uint64_t sums[2][kBins];
   __shared__ uint32_t counts[2][kBins], count_s[kBins], scan_u[16];
-  __shared__ int first_s[4], slots[64], finer_s[64], depth[64];
+  __shared__ int first_s[4];
+  // thread: one slot of every other part, requested before what they are merged by is formed
+  constexpr int kAhead = 10;
+  const int slot = tid & (kBins - 1), half = wave_id() / (kBins / 64);
+  uint64_t h[kAhead];
+  auto request = [&](int i0) {
+#pragma unroll
+    for (int r = 0; r < kAhead; ++r) h[r] = ld_agent(&part[min(i0 + 2 * r, parts - 1)].hist[slot]);
+  };
   // every wave: a part per lane (at most 64)
   const int lane = tid & 63;
   double part_top = 0.0;
@@ -483,6 +529,7 @@ __global__ __launch_bounds__(kThreads, 4) void sample_hist_kernel(SampleArgs a, 
     part_least = (uint32_t)(ends >> 32);
     part_fine = ld_agent(&part[lane].fine);
   }
+  request(half);
   (&sums[0][0])[tid] = 0;
   (&counts[0][0])[tid] = 0;
   best = wave_max(part_best);
@@ -503,28 +550,22 @@ __global__ __launch_bounds__(kThreads, 4) void sample_hist_kernel(SampleArgs a, 
   fine_row = least_row == ~0u ? 0 : min(fine_row, coarse.finest(order_float(best), order_float(least_row)));
   const Row whole(coarse, fine_row);
   const double gtop = floor(whole.y(order_float(best))), scale_row = kLn2 * whole.per_q;
-  const int part_finer = part_best == kNone ? 0 : (int)part_fine - fine_row;
-  if (tid < parts) {
-    slots[tid] = slot_of(part_top);
-    finer_s[tid] = part_finer;
-    depth[tid] = (int)fmin(ldexp(gtop, part_finer) - part_top, 0x1p29);   // of its first bin below the row's, in its bins
-  }
-  __syncthreads();
-  // thread: one slot of every other part
-  const int slot = tid & (kBins - 1), half = tid / kBins;
+  const int part_finer = part_best == kNone ? 0 : (int)part_fine - fine_row, part_slot = slot_of(part_top),
+            part_depth = (int)fmin(ldexp(gtop, part_finer) - part_top, 0x1p29);   // of its first bin below the row's, in its bins
+  __syncthreads();                               // (the sums are cleared)
   uint64_t sum = 0;
   uint32_t count = 0;
   double tail = 0.0;
-  constexpr int kAhead = 10;
   for (int i0 = half; i0 < parts; i0 += 2 * kAhead) {
-    uint64_t h[kAhead];
-#pragma unroll
-    for (int r = 0; r < kAhead; ++r) h[r] = ld_agent(&part[min(i0 + 2 * r, parts - 1)].hist[slot]);
+    if (i0 > half) request(i0);
 #pragma unroll
     for (int r = 0; r < kAhead; ++r) {
       const int i = i0 + 2 * r;
-      if (i >= parts || h[r] == 0) continue;
-      const int finer = finer_s[i], d = depth[i] + ((slots[i] - slot) & (kBins - 1)), below = (d + (1 << finer) - 1) >> finer;
+      if (i >= parts) continue;
+      const int finer = __builtin_amdgcn_readlane(part_finer, i),   // (by all lanes, ahead of what only some do)
+                d = __builtin_amdgcn_readlane(part_depth, i) + ((__builtin_amdgcn_readlane(part_slot, i) - slot) & (kBins - 1)),
+                below = (d + (1 << finer) - 1) >> finer;
+      if (h[r] == 0) continue;
       const uint32_t c = (uint32_t)(h[r] >> 48);
       uint64_t s = h[r] & 0xffffffffffffull;
       if (finer) {                               // 2^finer of the part's bins are one of the row's: from one middle to another's
@@ -559,11 +600,10 @@ __global__ __launch_bounds__(kThreads, 4) void sample_hist_kernel(SampleArgs a, 
     m = exp2_of((0.5 - j) * whole.per_q) * (kHistBase * (double)count + (double)(sums[0][j] + sums[1][j]) * (1.0 / kHistUnit));
   }
   // (as whole numbers: no bin's sum is less than the one's before it, as roundings could make it)
-  uint32_t n_bins;
-  uint64_t in_bins_u, tail_u;
-  const double upto = (double)block_scan((uint64_t)(m * 0x1p44 + 0.5), scan_m, in_bins_u) * 0x1p-44;
-  const uint32_t upto_count = block_scan(count, scan_u, n_bins);
-  block_scan((uint64_t)(tail * 0x1p44), scan_m, tail_u);
+  uint32_t upto_count = count;
+  uint64_t upto_u = (uint64_t)(m * 0x1p44 + 0.5), tail_u = (uint64_t)(tail * 0x1p44), in_bins_u;
+  block_scan3(upto_u, upto_count, tail_u, scan_m, scan_u, scan_t, in_bins_u);
+  const double upto = (double)upto_u * 0x1p-44;
   const double in_bins = (double)in_bins_u * 0x1p-44, tail_all = (double)tail_u * 0x1p-44, mass = in_bins + tail_all;
   const bool tail_counts = tail_all > 0x1p-42 * mass;
   if (half == 0) {
@@ -576,8 +616,8 @@ __global__ __launch_bounds__(kThreads, 4) void sample_hist_kernel(SampleArgs a, 
     if (half == 0 && upto >= target && (j == 0 || mass_s[j - 1] < target)) first_s[slot] = j;
   };
   constexpr double kEps = 0x1p-34;
-  const uint32_t k = row.greedy ? 1u : a.top_k && a.top_k[b] > 0 && a.top_k[b] < a.n ? (uint32_t)a.top_k[b] : 0u;
-  const float tp = a.top_p && !row.greedy ? a.top_p[b] : 1.f, mp = a.min_p && !row.greedy ? a.min_p[b] : 0.f;
+  const uint32_t k = (uint32_t)set.k;
+  const float tp = set.tp, mp = set.mp;
   bool slow = false;
   if (half == 0 && k && upto_count >= k && (j == 0 || count_s[j - 1] < k)) first_s[0] = j;
   __syncthreads();
@@ -613,7 +653,7 @@ __global__ __launch_bounds__(kThreads, 4) void sample_hist_kernel(SampleArgs a, 
     if (m_lo < kBins) lo = fmin(lo, m_lo ? mass_s[m_lo - 1] : 0.0);
     if (m_hi < kBins) hi = fmin(hi, mass_s[m_hi]);
   }
-  const double u = fmin(fmax((double)a.u[b], 0.0), 1.0);
+  const double u = set.u;
   __syncthreads();
   if (tid < 4) first_s[tid] = kBins;
   __syncthreads();
@@ -828,6 +868,7 @@ __global__ __launch_bounds__(kThreads, 4) void sample_pick_kernel(SampleArgs a, 
   const double top = st->top;
   const uint64_t mask_bits = st->mask[tid & (kBins / 64 - 1)];
   const Row row(Row(a, b), (int)st->fine);
+  const Settings set(a, b, row.greedy);
   if (slow != kUsual) {
     if (g == 0 && slow == kSlow) slow_row(a, b);
     return;
@@ -900,8 +941,8 @@ __global__ __launch_bounds__(kThreads, 4) void sample_pick_kernel(SampleArgs a, 
     st_agent(&c->pick, 0u);
   }
   const double scale = kLn2 * row.per_q;
-  const float tp = a.top_p ? a.top_p[b] : 1.f, mp = a.min_p ? a.min_p[b] : 0.f;
-  const int k = row.greedy ? 1 : a.top_k && a.top_k[b] > 0 && a.top_k[b] < a.n ? a.top_k[b] : 0;
+  const float tp = set.tp, mp = set.mp;
+  const int k = set.k;
   // S1's end, S2's end, the token: each the first element up to which a count, or the mass, reaches a target (the
   // token's: passes it).  Its bin first; then, as long as an interval of keys holds more than kTiny elements, 512 parts
   // of what its least and largest key span (a few values, each of many elements, where logits are bf16: then the parts
@@ -933,7 +974,7 @@ __global__ __launch_bounds__(kThreads, 4) void sample_pick_kernel(SampleArgs a, 
       }
     }
     const bool by_mass = stage > 0;
-    const double target = stage == 0 ? (double)k : stage == 1 ? (double)fmaxf(tp, 0.f) * s3 : draw(a, b) * s3;
+    const double target = stage == 0 ? (double)k : stage == 1 ? (double)fmaxf(tp, 0.f) * s3 : set.u * s3;
     auto reaches = [&](double x) { return stage == 2 ? x > target : x >= target; };
     // the first bin that reaches it (where rounding leaves none, the last), from its thread
     __syncthreads();
