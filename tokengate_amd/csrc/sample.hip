@@ -825,9 +825,8 @@ __device__ void slow_row(const SampleArgs &a, int b) {
   }
   const float mp = a.min_p ? a.min_p[b] : 0.f;
   if (mp > 0.f) {
-    uint64_t s = 0;                              // mass of what reaches min_p (a beginning as well)
     const double least = fmin((double)mp, 1.0);
-    uint32_t end = 0xffffffffu;
+    uint32_t end = 0xffffffffu;                  // the least that reaches min_p (a beginning as well)
     each([&](uint32_t key) {
       if (key < end && weight(order_float(key)) >= least) end = key;
     });
@@ -875,9 +874,8 @@ __global__ __launch_bounds__(kThreads, 4) void sample_pick_kernel(SampleArgs a, 
   }
   __shared__ PickShared sh;
   __shared__ uint64_t mask[kBins / 64];
-  __shared__ uint32_t n_s, base_s, last_s;
+  __shared__ uint32_t base_s, last_s;
   if (tid < kBins / 64) mask[tid] = mask_bits;
-  if (tid == 0) n_s = 0;
   __syncthreads();
   const Share share(a.n);
   uint64_t wanted = 0;                           // (at most 64 of a thread)
