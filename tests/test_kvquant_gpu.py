@@ -486,3 +486,46 @@ def test_strides_of_single_rows(cuda):
     row = case["qkv"][0].clone()
     b = run_attn(dict(case, qkv=row.as_strided((1, row.numel()), (3, 1))), clone_cache(case["cache"]), ws)
     assert torch.equal(a, b)
+
+
+def mirrored_case(dev, used, H, Hkv, bits, seed, bias_std):
+    """A case whose cached keys come in pairs 2 i, 2 i + 1 of the same key and bias and of values s c - s L / 2 of opposite
+    signs, with a new value of 0: every output is 0 exactly.  (s = 1; L / 2 is a bf16 number.)"""
+    c = attn_case(dev, used, 1, H, Hkv, bits, seed, True, False)
+    assert all(n % 2 == 1 for n in used)
+    cache, g = c["cache"], torch.Generator(device=dev).manual_seed(seed)
+    L = 2 ** bits - 1
+    cache.v.copy_(torch.randint(256, cache.v.shape, generator=g, device=dev, dtype=torch.uint8))
+    cache.v_meta[..., 0] = 1.0
+    cache.v_meta[..., 1] = -L / 2
+    c["bias"] = torch.empty(c["bias"].shape, device=dev).normal_(generator=g).mul_(bias_std)
+    c["qkv"][:, (H + Hkv) * 128:] = 0.0
+    for b, n in enumerate(used):
+        s = int(c["start"][b])
+        for t in (cache.k, cache.k_meta, cache.v):
+            t[:, s + 1:s + n - 1:2] = t[:, s:s + n - 2:2]
+        cache.v[:, s + 1:s + n - 1:2] ^= 255                # every code c to L - c
+        c["bias"][b, :, 1:n - 1:2] = c["bias"][b, :, 0:n - 2:2]
+    return c
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_long_sequences_whose_values_cancel(cuda, bits):
+    """16384 keys in pairs.  A block of 32 keys goes through two instructions, of 32 additions each, that round at sizes of
+    at most O = 16 + (L + 1) / 2 + 16 + L times the block's weights, and the sum before a block is next to nothing: as
+    independent roundings of 2^-24 of that at most, the outputs' errors have a root mean square below
+    2^-24 sqrt(64 blocks) O 32 max P.  (An offset that is carried from block to block is rounded at the size of all
+    the blocks' weights.)"""
+    from tokengate_amd import kvquant as Q
+    n, B = 16385, 32
+    c = mirrored_case(cuda, [n] * B, 16, 8, bits, 4, 0.3)
+    c["qkv"][:, :16 * 128] *= 0.01
+    c["lw"].q_norm.mul_(0.01)                              # (logits from the bias: weights within a factor of ten)
+    ws = Q.decode_attention_quant_workspace(B, c["shape"], c["max_k"], cuda)
+    out = run_attn(c, clone_cache(c["cache"]), ws).double()
+    L = 2 ** bits - 1
+    z = c["bias"][..., :n - 1].double() * SCALE
+    most = float(torch.softmax(z, -1).max()) * 1.5          # (the products' part of z is below 0.2)
+    tol = 2.0 ** -24 * (64 * n / 32) ** 0.5 * (32 + (L + 1) / 2 + L) * 32 * most
+    rms = float(out.square().mean().sqrt())
+    assert rms <= tol, (rms, tol)

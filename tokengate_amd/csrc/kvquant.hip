@@ -242,7 +242,9 @@ __global__ __launch_bounds__(256) void kv_dequantize_kernel(QuantCache c, RowTar
 // ---- attention of a decode step ---------------------------------------------------------------------
 // z_j = scale (q . k_j + bias_j), out = sum_j p_j v_j / sum_j p_j, p_j = exp(z_j - max z), with k_j = s c + m by groups
 // of 32 (g): q . k_j = sum_g s_jg (q . c_j)_g + m_jg Q_g,  Q_g the sum of q over the group, and
-// out = sum_g (p_j s_jg) c_j + sum_j p_j m_jg.  Bound by the bytes of the cache (80 or 144 per key and kv head, K and
+// out = sum_g (p_j s_jg) c'_j + sum_j p_j m'_jg with c' = c - C, m' = m + C s, C the middle code (8 or 128): values of
+// either sign have codes around the middle, so the sums over the keys are as small as the values', where those of p s c
+// and p m would grow with every key and cancel at the end.  Bound by the bytes of the cache (80 or 144 per key and kv head, K and
 // V each), so a workgroup takes one kv head of one sequence, up to four query heads of its group at once, and a
 // stretch of keys: chunks of chunk_tiles tiles of 64 keys, its four waves a tile each in turn.  Nothing is staged
 // through LDS: a wave's matrix instructions take the codes from the registers that the loads fill.
@@ -250,11 +252,13 @@ __global__ __launch_bounds__(256) void kv_dequantize_kernel(QuantCache c, RowTar
 //     (each head four times), so that every lane group gets all heads' sums and lane l keeps those of key l: the
 //     softmax's work is one key per lane and head, and a lane applies its own key's s and m.  B: lane (n, G) holds the
 //     words 4 G .. 4 G + 3 of key n.
-//   * At 4 bits codes become bf16 by their bits: 0x4300 | c is 128 + c (two per and-or).  The sums start from
-//     -128 Q_g (C operand); the output's part is taken off at the end.  At 8 bits they are converted.
+//   * At 4 bits codes become bf16 by their bits: 0x4180 | c << 3 is 16 + c (two per and-or).  At 8 bits they are
+//     converted.  S starts from -16 Q_g (C operand).  O gets -24 P or -128 P, P times a constant B, ahead of every 32 keys, so
+//     that its sums are of c' and no more than the 32 keys' offset is rounded with them.  (At 128 + c, the 128 taken off at
+//     the end, outputs over 131072 keys were off by 5e-4 of their size.)
 //   * O += P C with P = p s per group, from LDS in A's layout, as two bf16 numbers of 16 bits together: rounded to
 //     one, the weights of keys that cancel left errors of 0.4 % of the output.  The second takes rows of A that would
-//     repeat the heads, so no more instructions.  The least values' part is summed in fp32.  B: lane (n, G) holds word
+//     repeat the heads, so no more instructions.  The middles' part is summed in fp32.  B: lane (n, G) holds word
 //     n of keys 4 j + G, whose nibble (byte) e is element 16 e + n: eight keys of one element, and the element's
 //     group depends on e alone.
 //   * The new key is not in the tiles: it is a part of its own beside the waves', from registers.
@@ -330,15 +334,17 @@ __device__ __forceinline__ float wave_add(float x) {
 
 // bf16 pairs of eight codes from four words (4 bits) or pairs of words (8) of as many rows, nibbles (bytes) e of each:
 // low half a, high half b of code pairs (a, b).
-constexpr uint32_t kNibbles = 0x000F000Fu, kBf128 = 0x43004300u;
+constexpr uint32_t kNibbles = 0x00780078u, kBf16 = 0x41804180u;   // (a nibble three bits up, 16)
+template <int BITS> constexpr float mid_code() { return BITS == 4 ? 8.f : 128.f; }
+template <int BITS> constexpr uint32_t kMinusOffset = BITS == 4 ? 0xC1C0C1C0u : 0xC300C300u;   // -24, -128: c' less the pairs
 
 // (a's code e, b's code e) as a bf16 pair; at 4 bits from the halves' merger y = lo/hi16(a) | lo/hi16(b) << 16
 __device__ __forceinline__ uint32_t merge_half(uint32_t a, uint32_t b, int hi) {
   return __builtin_amdgcn_perm(b, a, hi ? 0x07060302u : 0x05040100u);
 }
 // (mask and bias in registers: as literals they cost an instruction each)
-__device__ __forceinline__ uint32_t nibble_pair(uint32_t y, int e, uint32_t nibbles, uint32_t bf128) {
-  return ((y >> (4 * (e & 3))) & nibbles) | bf128;
+__device__ __forceinline__ uint32_t nibble_pair(uint32_t y, int e, uint32_t nibbles, uint32_t bf16) {
+  return (((e & 3) == 0 ? y << 3 : y >> (4 * (e & 3) - 3)) & nibbles) | bf16;
 }
 __device__ __forceinline__ uint32_t byte_pair(uint32_t a, uint32_t b, int byte) {
   const float fa = (float)((a >> (8 * byte)) & 255u), fb = (float)((b >> (8 * byte)) & 255u);
@@ -590,7 +596,7 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(BITS, HP)) void decode_attn_qua
   f32x4 oacc[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) oacc[e] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float mrun[HP], lsum[HP], rest[HP][kGroups];   // rest: what the output's sums lack, by lane
+  float mrun[HP], lsum[HP], rest[HP][kGroups];   // rest: sums of p m', by lane
 #pragma unroll
   for (int i = 0; i < HP; ++i) {
     mrun[i] = -INFINITY;
@@ -601,8 +607,10 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(BITS, HP)) void decode_attn_qua
   // position of this lane's key in A's order of keys: lane (m, G) takes keys 4 j + G, j = 0 .. 7, of 32
   bf16_t *const pw = &ps[wave][0][0][32 * (lane >> 5) + 8 * (lane & 3) + ((lane & 31) >> 2)];
 
-  uint32_t nibbles = kNibbles, bf128 = kBf128;
-  asm("" : "+v"(nibbles), "+v"(bf128));
+  uint32_t nibbles = kNibbles, bf16 = kBf16;
+  asm("" : "+v"(nibbles), "+v"(bf16));
+  constexpr uint32_t kOff = kMinusOffset<BITS>;
+  const bf16x8 minus_offset = __builtin_bit_cast(bf16x8, u32x4{kOff, kOff, kOff, kOff});
   auto step = [&](Tile &l) {
     // ---- logits of key `lane` ----
     float z[HP];
@@ -623,7 +631,7 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(BITS, HP)) void decode_attn_qua
       f32x4 init = {0.f, 0.f, 0.f, 0.f};
       if constexpr (BITS == 4) {
 #pragma unroll
-        for (int i = 0; i < HP; ++i) init[i] = -128.f * qsum[g][i];
+        for (int i = 0; i < HP; ++i) init[i] = -16.f * qsum[g][i];
       }
       f32x4 s[4];
 #pragma unroll
@@ -633,7 +641,7 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(BITS, HP)) void decode_attn_qua
         for (int w = 0; w < 4; ++w) {            // codes e = 2 g (w < 2) and 2 g + 1 of words 0 1 or 2 3
           const int e = 2 * g + (w >> 1), p = w & 1;
           if constexpr (BITS == 4)
-            c[w] = nibble_pair(ky[kb][2 * p + (e >> 2)], e, nibbles, bf128);
+            c[w] = nibble_pair(ky[kb][2 * p + (e >> 2)], e, nibbles, bf16);
           else
             c[w] = byte_pair(l.kx[kb][4 * p + (e >> 2)], l.kx[kb][4 * p + 2 + (e >> 2)], e & 3);
         }
@@ -678,13 +686,12 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(BITS, HP)) void decode_attn_qua
       lsum[i] += p;
 #pragma unroll
       for (int g = 0; g < kGroups; ++g) {
-        const float step = u32_as_f32(l.vmeta[g] << 16), least = u32_as_f32(l.vmeta[g] & 0xffff0000u);
+        const float step = u32_as_f32(l.vmeta[g] << 16), mid = fmaf(mid_code<BITS>(), step, u32_as_f32(l.vmeta[g] & 0xffff0000u));
         const float w = mul_zero(p, step);       // (a weight of 0 is 0, whatever the row holds)
         const __bf16 hi = (__bf16)w, lo = (__bf16)(w - (float)hi);
         pw[(2 * HP * g + i) * kTile] = __builtin_bit_cast(uint16_t, hi);
         pw[(2 * HP * g + HP + i) * kTile] = __builtin_bit_cast(uint16_t, lo);
-        rest[i][g] += mul_zero(p, least);
-        if constexpr (BITS == 4) rest[i][g] = fmaf(-128.f, (float)hi + (float)lo, rest[i][g]);
+        rest[i][g] += mul_zero(p, mid);
       }
     }
     // ---- O += P C ----
@@ -702,12 +709,14 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(BITS, HP)) void decode_attn_qua
       for (int g = 0; g < kGroups; ++g) {
         const bf16x8 pf = *reinterpret_cast<const bf16x8 *>(&ps[wave][g][n16 & (2 * HP - 1)][32 * st + 8 * G]);
 #pragma unroll
+        for (int e = 2 * g; e < 2 * g + 2; ++e) oacc[e] = mfma16(pf, minus_offset, oacc[e]);
+#pragma unroll
         for (int e = 2 * g; e < 2 * g + 2; ++e) {
           u32x4 c;
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
             if constexpr (BITS == 4)
-              c[w] = nibble_pair(vy[w][e >> 2], e, nibbles, bf128);
+              c[w] = nibble_pair(vy[w][e >> 2], e, nibbles, bf16);
             else
               c[w] = byte_pair(l.vx[st][2 * w][e >> 2], l.vx[st][2 * w + 1][e >> 2], e & 3);
           }
