@@ -529,3 +529,31 @@ def test_long_sequences_whose_values_cancel(cuda, bits):
     tol = 2.0 ** -24 * (64 * n / 32) ** 0.5 * (32 + (L + 1) / 2 + L) * 32 * most
     rms = float(out.square().mean().sqrt())
     assert rms <= tol, (rms, tol)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("H,Hkv", [(8, 8), (16, 8), (16, 2), (12, 4)])
+def test_weights_of_two_keys_that_cancel(cuda, bits, H, Hkv):
+    """Two keys of opposite values, one of the largest logit whose value is 0, and the new one: the outputs, 0, are off by
+    the rounding of the two's weight w times L.  In 24 bits that is less than the sums' roundings: two products and their
+    offsets, at sizes of at most 2 (16 + (L + 1) / 2) w or 16 + L + as much, four of them of 2^-24; and as much again for
+    the weights' smaller parts, the least values' sum and the merge.  (A weight of 16 bits is off by up to 2^-17, times L.)"""
+    from tokengate_amd import kvquant as Q
+    used = [4] * 12
+    c = mirrored_case(cuda, [3] * 12, H, Hkv, bits, 3, 1.0)
+    c["used"] += 1                                          # (a free row after each)
+    c["qkv"][:, :H * 128] *= 0.01
+    c["lw"].q_norm.mul_(0.01)
+    for b, s in enumerate(c["start"].tolist()):
+        for t in (c["cache"].v, c["cache"].v_meta):
+            t[:, s + 2] = 0                                 # the third key's value
+        c["bias"][b, :, 0] = 20 * torch.rand(H, generator=torch.Generator().manual_seed(b)).to(cuda)
+        c["bias"][b, :, 1] = c["bias"][b, :, 0]
+        c["bias"][b, :, 2] = 20.0
+        c["bias"][b, :, 3] = 0.0
+    ws = Q.decode_attention_quant_workspace(len(used), c["shape"], c["max_k"], cuda)
+    out = run_attn(c, clone_cache(c["cache"]), ws).double().abs()
+    w = torch.softmax(c["bias"][..., :4].double() * SCALE, -1)[..., 0]      # (products of q and k are below 0.02)
+    L = 2 ** bits - 1
+    tol = 1.05 * w[..., None] * 2 * 4 * 2.0 ** -24 * (2 * (16 + (L + 1) / 2) + 16 + L)
+    assert bool((out <= tol).all()), float((out / tol).max())

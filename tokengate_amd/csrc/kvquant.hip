@@ -256,9 +256,9 @@ __global__ __launch_bounds__(256) void kv_dequantize_kernel(QuantCache c, RowTar
 //     converted.  S starts from -16 Q_g (C operand).  O gets -24 P or -128 P, P times a constant B, ahead of every 32 keys, so
 //     that its sums are of c' and no more than the 32 keys' offset is rounded with them.  (At 128 + c, the 128 taken off at
 //     the end, outputs over 131072 keys were off by 5e-4 of their size.)
-//   * O += P C with P = p s per group, from LDS in A's layout, as two bf16 numbers of 16 bits together: rounded to
-//     one, the weights of keys that cancel left errors of 0.4 % of the output.  The second takes rows of A that would
-//     repeat the heads, so no more instructions.  The middles' part is summed in fp32.  B: lane (n, G) holds word
+//   * O += P C with P = p s per group, from LDS in A's layout, as three bf16 numbers, 24 bits together as fp32's:
+//     rounded to one, the weights of keys that cancel left errors of 0.4 % of the output, to two of 2^-18 L steps.  The
+//     others take rows of A that would repeat the heads, so no more instructions.  The middles' part is summed in fp32.  B: lane (n, G) holds word
 //     n of keys 4 j + G, whose nibble (byte) e is element 16 e + n: eight keys of one element, and the element's
 //     group depends on e alone.
 //   * The new key is not in the tiles: it is a part of its own beside the waves', from registers.
@@ -301,6 +301,7 @@ constexpr int kTile = 64;        // keys of a wave's step
 constexpr int depth(int bits, int hp) { return bits == 4 && hp <= 2 ? 2 : 1; }
 __host__ __device__ constexpr int per_cu(int bits, int hp) { return depth(bits, hp) == 2 || hp == 4 ? 2 : 3; }
 constexpr float kRescaleTau = 8.f;
+constexpr int kParts = 3;        // bf16 numbers of a weight
 
 template <typename T>
 __device__ __forceinline__ void st_agent(T *p, T v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
@@ -318,18 +319,24 @@ __device__ __forceinline__ float wave_max(float x) {
   x = fmaxf(x, dpp<0x140>(x));   // row_mirror
   return quad_swap_max(x);
 }
+__device__ __forceinline__ float add_row_pair(float x) {   // x of lanes l and l ^ 16
+  const uint32_t u = __builtin_bit_cast(uint32_t, x);
+  const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  const uint32_t a0 = a[0], a1 = a[1];
+  return u32_as_f32(a0) + u32_as_f32(a1);
+}
+__device__ __forceinline__ float add_rows(float x) {       // x of lanes l, l ^ 16, l ^ 32, l ^ 48
+  const uint32_t v = __builtin_bit_cast(uint32_t, add_row_pair(x));
+  const auto c = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  const uint32_t c0 = c[0], c1 = c[1];
+  return u32_as_f32(c0) + u32_as_f32(c1);
+}
 __device__ __forceinline__ float wave_add(float x) {
   x += dpp<0xB1>(x);
   x += dpp<0x4E>(x);
   x += dpp<0x141>(x);
   x += dpp<0x140>(x);
-  const uint32_t u = __builtin_bit_cast(uint32_t, x);
-  const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-  const uint32_t a0 = a[0], a1 = a[1];
-  const uint32_t v = __builtin_bit_cast(uint32_t, u32_as_f32(a0) + u32_as_f32(a1));
-  const auto c = __builtin_amdgcn_permlane32_swap(v, v, false, false);
-  const uint32_t c0 = c[0], c1 = c[1];
-  return u32_as_f32(c0) + u32_as_f32(c1);
+  return add_rows(x);
 }
 
 // bf16 pairs of eight codes from four words (4 bits) or pairs of words (8) of as many rows, nibbles (bytes) e of each:
@@ -437,7 +444,7 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(BITS, HP)) void decode_attn_qua
 
   __shared__ __attribute__((aligned(16))) bf16_t qs[HP][kHeadDim];
   __shared__ __attribute__((aligned(16))) float new_x[2][kHeadDim];   // the new key and value as they are held
-  __shared__ __attribute__((aligned(16))) bf16_t ps[kWaves][kGroups][2 * HP][kTile];
+  __shared__ __attribute__((aligned(16))) bf16_t ps[kWaves][kGroups][kParts * HP][kTile];
   __shared__ __attribute__((aligned(16))) float part_o[kWaves + 1][HP][kHeadDim], part_ml[kWaves + 1][HP][2];
 
   const Chunk ck = find_chunk(a, blockIdx.x / a.sets, lane);
@@ -605,6 +612,9 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(BITS, HP)) void decode_attn_qua
     for (int g = 0; g < kGroups; ++g) rest[i][g] = 0.f;
   }
   // position of this lane's key in A's order of keys: lane (m, G) takes keys 4 j + G, j = 0 .. 7, of 32
+  // row of the weights that this lane holds in A: heads' first parts, second, third and as many rows of these again, which
+  // no sum is taken of
+  const int a_row = (n16 & (4 * HP - 1)) < kParts * HP ? n16 & (4 * HP - 1) : (n16 & (4 * HP - 1)) - HP;
   bf16_t *const pw = &ps[wave][0][0][32 * (lane >> 5) + 8 * (lane & 3) + ((lane & 31) >> 2)];
 
   uint32_t nibbles = kNibbles, bf16 = kBf16;
@@ -675,8 +685,8 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(BITS, HP)) void decode_attn_qua
         for (int g = 0; g < kGroups; ++g) rest[i][g] *= f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          oacc[e][i] *= f;
-          if constexpr (HP <= 2) oacc[e][i + HP] *= f;   // the low parts' rows
+#pragma unroll
+          for (int r = i; r < 4; r += HP) oacc[e][r] *= f;   // the head's parts
         }
       }
     }
@@ -688,9 +698,10 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(BITS, HP)) void decode_attn_qua
       for (int g = 0; g < kGroups; ++g) {
         const float step = u32_as_f32(l.vmeta[g] << 16), mid = fmaf(mid_code<BITS>(), step, u32_as_f32(l.vmeta[g] & 0xffff0000u));
         const float w = mul_zero(p, step);       // (a weight of 0 is 0, whatever the row holds)
-        const __bf16 hi = (__bf16)w, lo = (__bf16)(w - (float)hi);
-        pw[(2 * HP * g + i) * kTile] = __builtin_bit_cast(uint16_t, hi);
-        pw[(2 * HP * g + HP + i) * kTile] = __builtin_bit_cast(uint16_t, lo);
+        const __bf16 w0 = (__bf16)w, w1 = (__bf16)(w - (float)w0), w2 = (__bf16)(w - (float)w0 - (float)w1);
+        pw[(kParts * HP * g + i) * kTile] = __builtin_bit_cast(uint16_t, w0);
+        pw[(kParts * HP * g + HP + i) * kTile] = __builtin_bit_cast(uint16_t, w1);
+        pw[(kParts * HP * g + 2 * HP + i) * kTile] = __builtin_bit_cast(uint16_t, w2);
         rest[i][g] += mul_zero(p, mid);
       }
     }
@@ -707,7 +718,7 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(BITS, HP)) void decode_attn_qua
       }
 #pragma unroll
       for (int g = 0; g < kGroups; ++g) {
-        const bf16x8 pf = *reinterpret_cast<const bf16x8 *>(&ps[wave][g][n16 & (2 * HP - 1)][32 * st + 8 * G]);
+        const bf16x8 pf = *reinterpret_cast<const bf16x8 *>(&ps[wave][g][a_row][32 * st + 8 * G]);
 #pragma unroll
         for (int e = 2 * g; e < 2 * g + 2; ++e) oacc[e] = mfma16(pf, minus_offset, oacc[e]);
 #pragma unroll
@@ -750,14 +761,12 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(BITS, HP)) void decode_attn_qua
 #pragma unroll
     for (int g = 0; g < kGroups; ++g) {
       const float r = wave_add(rest[i][g]);
-      float o0 = oacc[2 * g][i], o1 = oacc[2 * g + 1][i];
-      if constexpr (HP <= 2) {
-        o0 += oacc[2 * g][i + HP];
-        o1 += oacc[2 * g + 1][i + HP];
-      } else {                                   // the low parts' rows are the neighbour lane group's
-        o0 += __shfl_xor(o0, 16);
-        o1 += __shfl_xor(o1, 16);
-      }
+      auto sum_parts = [&](const f32x4 &o) {     // (lane group G holds A's rows 4 G .. 4 G + 3)
+        if constexpr (HP == 1) return o[0] + (o[1] + o[2]);
+        else if constexpr (HP == 2) return add_row_pair(G & 1 ? o[i] : o[i] + o[i + 2]);
+        else return add_rows(G < kParts ? o[i] : 0.f);
+      };
+      const float o0 = sum_parts(oacc[2 * g]), o1 = sum_parts(oacc[2 * g + 1]);
       if (G == g) {                              // lane group g writes group g's elements
         part_o[wave][i][32 * g + n16] = o0 + r;
         part_o[wave][i][32 * g + 16 + n16] = o1 + r;
