@@ -251,3 +251,33 @@ def test_one_token_left_of_many_that_weigh_little(cuda, v):
     for k, p, m in ((50, 0.0, 0.0), (0, 0.3, 0.0), (1000, 0.8, 1.0), (0, 1.0, 1.0), (20, 1.0, 0.5)):
         lp = check(cuda, x, [0.6] * n, [0.45] * n, [k] * n, [p] * n, [m] * n)[1]
         assert bool((lp == 0).all()), (k, p, m, lp)
+
+
+def test_a_logit_behind_a_larger_one(cuda):
+    """One thread's logits 0, -42, 4, in its order, and two of another part: the -42 leaves the reach of the bins when the
+    4 arrives, the 0 does not, and its 0.018 of the mass decides."""
+    x = torch.full((1, 16384), -float("inf"))
+    for i, v in ((0, 0.0), (1024, -42.0), (2048, 4.0), (8192, -30.0), (8269, -1.0)):
+        x[0, i] = v
+    tok, _, near = check(cuda, x, [0.98], None, None, None, None)
+    assert near == 0 and tok[0] == 0
+
+
+@pytest.mark.parametrize("v", [16384, 50001, 151936])
+@pytest.mark.parametrize("masked", [-float("inf"), -1e4, -3e38])
+def test_few_logits_that_are_not_masked(cuda, v, masked):
+    """Rows of 3 to 50 logits among masked ones, far apart, the largest anywhere, at temperatures down to 0.05."""
+    n = 48
+    rng = np.random.default_rng(v)
+    for t in (0.05, 0.1, 0.3, 1.0, 2.0):
+        x = np.full((n, v), masked, dtype=np.float32)
+        for b in range(n):
+            some = rng.choice(v, int(rng.integers(3, 51)), replace=False)
+            # (half of them together in a few threads' columns)
+            some[::2] = some[0] % 1024 + 1024 * rng.choice(v // 1024, len(some[::2]), replace=False) if v // 1024 >= len(some[::2]) else some[::2]
+            x[b, some] = -np.abs(rng.standard_normal(len(some))) * t * rng.choice([3.0, 20.0, 60.0]) + rng.uniform(-20, 20)
+        near = 0
+        for k, p, m in ((0, 1.0, 0.0), (3, 1.0, 0.0), (10, 0.97, 0.0), (0, 0.9, 1e-3)):
+            u = list(1 - 10.0 ** -rng.uniform(0.1, 6, n))
+            near += check(cuda, torch.from_numpy(x), u, [t] * n, [k] * n, [p] * n, [m] * n)[2]
+        assert near == 0

@@ -458,21 +458,31 @@ __global__ __launch_bounds__(kThreads, 4) void sample_hist_kernel(SampleArgs a, 
   __shared__ unsigned long long tail_s;
   __shared__ uint32_t last_s;
   const Share share(a.n);
-  float most = -INFINITY, least = INFINITY;      // (maxima of pairs drop NaN)
+  float most = -INFINITY, least = INFINITY;      // (maxima of pairs drop NaN; -inf has no weight)
   const Row coarse(a, b);
   const Settings set(a, b, coarse.greedy);       // (for the last workgroup: here their loads take no time of their own)
   const float reach = coarse.reach();
-  // least: of what lies within reach of the largest; what lies below, as a finite mask does, may not count
   share.each(x, [&](float v, int) {
     most = fmaxf(most, v);
-    const float end = most - reach;
-    least = least > end ? least : INFINITY;
-    least = v > end ? fminf(least, v) : least;
+    least = v > -INFINITY ? fminf(least, v) : least;
   });
   if (tid < kBins) hist[tid] = 0;
   if (tid == 0) tail_s = 0;
   uint32_t best = block_max(order_bits(most), tmp);   // (its barriers cover the bins)
-  const uint32_t low_bits = ~block_max(least > order_float(best) - reach ? ~order_bits(least) : 0u, tmp);
+  uint32_t low_bits = ~block_max(~order_bits(least), tmp);
+  const float end = order_float(best) - reach;
+  // the least of what lies within reach of the largest: what lies below, as a finite mask does, may not count, and takes
+  // another pass (which logits are within reach is known only when the largest is)
+  if (!(order_float(low_bits) > end)) {
+    least = INFINITY;
+    bool any = false;
+    share.each(x, [&](float v, int) {
+      const bool near = v > end;
+      least = near ? fminf(least, v) : least;
+      any |= near;
+    });
+    low_bits = ~block_max(any ? ~order_bits(least) : 0u, tmp);
+  }
   const int fine = low_bits == ~0u ? 0 : coarse.finest(order_float(best), order_float(low_bits));
   const Row row(coarse, fine);
   const double top = best == kNone ? 0.0 : floor(row.y(order_float(best)));
