@@ -281,3 +281,30 @@ def test_few_logits_that_are_not_masked(cuda, v, masked):
             u = list(1 - 10.0 ** -rng.uniform(0.1, 6, n))
             near += check(cuda, torch.from_numpy(x), u, [t] * n, [k] * n, [p] * n, [m] * n)[2]
         assert near == 0
+
+
+def test_parts_far_apart_at_high_temperatures(cuda):
+    """Logits more than 2^29 bins below the row's largest, whole parts of them: an infinity in one part alone, and spreads of
+    1e7 to 1e9, at temperatures at which they weigh nothing, something and nearly as much as the largest."""
+    v, inf = 40000, float("inf")
+    rng = np.random.default_rng(7)
+    x = np.zeros((6, v), dtype=np.float32)
+    x[0] = rng.standard_normal(v)
+    x[0, [5, 77]] = inf
+    x[1] = rng.standard_normal(v)
+    x[1, [39000, 39999]] = inf
+    for b, spread in ((2, 1e7), (3, 1e8), (4, 1e9)):
+        x[b] = -spread * (1 + 0.1 * rng.random(v))
+        x[b, :300] = rng.standard_normal(300)
+    x[5] = -inf
+    x[5, 20000:] = -1e8 + 1e6 * rng.standard_normal(20000)
+    x[5, 9] = 1.0
+    x = torch.from_numpy(x)
+    near = 0
+    for t in (1.0, 1e6, 1e7, 3e7, 1e9, 3e38):
+        for k, p, m in ((0, 1.0, 0.0), (20000, 1.0, 0.0), (0, 0.6, 0.0), (0, 1.0, 0.9)):
+            for u in (0.01, 0.4, 0.97):
+                tok, _, border = check(cuda, x, [u] * 6, [t] * 6, [k] * 6, [p] * 6, [m] * 6)
+                near += border
+                assert tok[0] in (5, 77) and tok[1] in (39000, 39999)
+    assert near == 0

@@ -273,6 +273,7 @@ __device__ __forceinline__ uint32_t read_lane(uint32_t x, int lane) { return (ui
 __device__ __forceinline__ uint64_t read_lane(uint64_t x, int lane) {
   return (uint64_t)read_lane((uint32_t)(x >> 32), lane) << 32 | read_lane((uint32_t)x, lane);
 }
+__device__ __forceinline__ double read_lane(double x, int lane) { return double_of(read_lane(bits_of(x), lane)); }
 // Sums over the threads up to this one; total: over all.  tmp: 16 of T.  Whole numbers: every wave adds the waves' sums
 // up for itself, one per lane.
 template <typename T>
@@ -560,8 +561,12 @@ __global__ __launch_bounds__(kThreads, 4) void sample_hist_kernel(SampleArgs a, 
   fine_row = least_row == ~0u ? 0 : min(fine_row, coarse.finest(order_float(best), order_float(least_row)));
   const Row whole(coarse, fine_row);
   const double gtop = floor(whole.y(order_float(best))), scale_row = kLn2 * whole.per_q;
-  const int part_finer = part_best == kNone ? 0 : (int)part_fine - fine_row, part_slot = slot_of(part_top),
-            part_depth = (int)fmin(ldexp(gtop, part_finer) - part_top, 0x1p29);   // of its first bin below the row's, in its bins
+  const int part_finer = part_best == kNone ? 0 : (int)part_fine - fine_row, part_slot = slot_of(part_top);
+  // its first bin lies so many of its bins below the row's first; past 2^29 in two numbers, part_beyond of the row's bins and
+  // the rest (at high temperatures no distance is so large that it weighs nothing by itself)
+  const double depth = ldexp(gtop, part_finer) - part_top;
+  const double part_beyond = depth > 0x1p29 ? floor(ldexp(depth - 0x1p29, -part_finer)) : 0.0;
+  const int part_depth = depth > 0x1p29 ? (int)fmin(fmax(depth - ldexp(part_beyond, part_finer), 0x1p28), 0x1p30) : (int)depth;
   __syncthreads();                               // (the sums are cleared)
   uint64_t sum = 0;
   uint32_t count = 0;
@@ -575,6 +580,7 @@ __global__ __launch_bounds__(kThreads, 4) void sample_hist_kernel(SampleArgs a, 
       const int finer = __builtin_amdgcn_readlane(part_finer, i),   // (by all lanes, ahead of what only some do)
                 d = __builtin_amdgcn_readlane(part_depth, i) + ((__builtin_amdgcn_readlane(part_slot, i) - slot) & (kBins - 1)),
                 below = (d + (1 << finer) - 1) >> finer;
+      const double beyond = read_lane(part_beyond, i);
       if (h[r] == 0) continue;
       const uint32_t c = (uint32_t)(h[r] >> 48);
       uint64_t s = h[r] & 0xffffffffffffull;
@@ -583,7 +589,7 @@ __global__ __launch_bounds__(kThreads, 4) void sample_hist_kernel(SampleArgs a, 
         s = (uint64_t)((hist_mass(h[r]) * exp_small(off * scale_row) - kHistBase * (double)c) * kHistUnit + 0.5);
       }
       if (below >= kBins) {
-        tail += exp2_of((0.5 - below) * whole.per_q) * hist_mass((uint64_t)c << 48 | s);
+        tail += exp2_of((0.5 - below - beyond) * whole.per_q) * hist_mass((uint64_t)c << 48 | s);
       } else if (finer) {
         atomicAdd((unsigned long long *)&sums[half][below], (unsigned long long)s);
         atomicAdd(&counts[half][below], c);
