@@ -179,3 +179,32 @@ def test_outputs_that_overlap(ptr):
                 v=p, v_rs=128, v_hs=512, stream=None)
     for change in (dict(k_rs=0), dict(v_rs=64), dict(k_rs=128), dict(v_hs=384), dict(v_rs=0, v_hs=128)):
         assert "overlap" in _call("tg_kv_dequantize", read, **change), change
+
+
+def test_copies_of_a_cache_are_their_own(monkeypatch):
+    """A cache that was copied, pickled or moved passes its own tensors on; its fields cannot be replaced."""
+    import copy
+    import dataclasses
+    import io
+    from tokengate_amd import _lib
+    from tokengate_amd import kvquant as Q
+    calls = []
+    monkeypatch.setattr(_lib, "call_on", lambda index, name, *args: calls.append((index, name, args)))
+    whole = _cache(rows=20)
+    cut = Q.QuantKV(4, *(t[:, 3:13] for t in (whole.k, whole.k_meta, whole.v, whole.v_meta)))
+    buf = io.BytesIO()
+    torch.save(cut, buf)
+    buf.seek(0)
+    x = torch.zeros(4, 2, 128, dtype=torch.bfloat16)
+    for c in (copy.deepcopy(cut), torch.load(buf, weights_only=False), copy.copy(cut), dataclasses.replace(cut, v=whole.v.clone()[:, 3:13])):
+        calls.clear()
+        Q.kv_quantize(x, x, c)
+        Q.kv_dequantize(c, n_rows=2)
+        assert len(calls) == 2 and c.rows == 10 and c.n_kv_heads == 2 and c.device_index == -1
+        ptrs = [t.data_ptr() for t in (c.k, c.k_meta, c.v, c.v_meta)] + [c.rows, c.head_rows]
+        assert list(calls[0][2][-6:]) == ptrs and list(calls[1][2][:6]) == ptrs
+    assert copy.copy(cut).k is cut.k and copy.deepcopy(cut).k.data_ptr() != cut.k.data_ptr()
+    with pytest.raises(AttributeError):
+        cut.k = whole.v[:, 3:13]
+    with pytest.raises(AttributeError):
+        cut.bits = 8

@@ -23,11 +23,12 @@ HEAD_DIM = 128
 GROUPS = 4
 
 
-@dataclass
+@dataclass(frozen=True)
 class QuantKV:
     """One layer's cache: codes (Hkv, rows, 16 * bits) uint8 and meta (Hkv, rows, 4, 2) bf16 = (s, m) of each
     group, for K and for V.  Element 16 e + w of a row is nibble (byte) e of its word (pair of words) w.  The
-    rows of a head are contiguous; the heads may be further apart (a slice of rows of a longer cache)."""
+    rows of a head are contiguous; the heads may be further apart (a slice of rows of a longer cache).  The fields of
+    a cache are not replaced (dataclasses.replace makes another one); a copy has the copied tensors."""
     bits: int
     k: torch.Tensor
     k_meta: torch.Tensor
@@ -45,16 +46,23 @@ class QuantKV:
         for t in (self.k_meta, self.v_meta):
             if t.dtype != torch.bfloat16 or tuple(t.shape) != (hkv, rows, GROUPS, 2) or t.stride()[1:] != (8, 2, 1):
                 raise RuntimeError("QuantKV: meta must be bf16 (heads, rows, 4, 2) with contiguous rows")
-        self.head_rows = self.k.stride(0) // n if hkv > 1 else rows
-        if hkv > 1 and (any(t.stride(0) != self.head_rows * n for t in (self.k, self.v))
-                        or any(t.stride(0) != self.head_rows * 8 for t in (self.k_meta, self.v_meta))):
+        head_rows = self.k.stride(0) // n if hkv > 1 else rows
+        if hkv > 1 and (any(t.stride(0) != head_rows * n for t in (self.k, self.v))
+                        or any(t.stride(0) != head_rows * 8 for t in (self.k_meta, self.v_meta))):
             raise RuntimeError("QuantKV: codes and meta must have the same rows between heads")
         if len({t.device for t in (self.k, self.v, self.k_meta, self.v_meta)}) != 1:
             raise RuntimeError("QuantKV: tensors on different devices")
-        # what every call passes on (the tensors of a cache are not replaced, resized or moved)
-        self.rows, self.n_kv_heads, self.device_index = rows, hkv, self.k.get_device()
-        self._args = (self.k.data_ptr(), self.k_meta.data_ptr(), self.v.data_ptr(), self.v_meta.data_ptr(), rows,
-                      self.head_rows)
+        self.__dict__.update(rows=rows, n_kv_heads=hkv, head_rows=head_rows, device_index=self.k.get_device())
+
+    def __setstate__(self, state):               # copies and unpickled caches: of the tensors that they got
+        self.__dict__.update(state)
+        self.__post_init__()
+
+    @property
+    def _args(self) -> tuple:
+        """What every call passes on."""
+        return (self.k.data_ptr(), self.k_meta.data_ptr(), self.v.data_ptr(), self.v_meta.data_ptr(), self.rows,
+                self.head_rows)
 
     @staticmethod
     def alloc(rows: int, n_kv_heads: int, bits: int, device) -> "QuantKV":
