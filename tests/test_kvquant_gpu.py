@@ -557,3 +557,36 @@ def test_weights_of_two_keys_that_cancel(cuda, bits, H, Hkv):
     L = 2 ** bits - 1
     tol = 1.05 * w[..., None] * 2 * 4 * 2.0 ** -24 * (2 * (16 + (L + 1) / 2) + 16 + L)
     assert bool((out <= tol).all()), float((out / tol).max())
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("H,Hkv", [(8, 8), (16, 8), (16, 2)])
+def test_values_near_the_largest_float(cuda, bits, H, Hkv):
+    """Value groups whose values and steps reach up to fp32's largest, some keys or all of them, in one group or all, with
+    the largest logits late: the weighted means are finite, as in float64."""
+    from tokengate_amd import kvquant as Q
+    used = [5, 300, 700, 1500, 64]
+    c = attn_case(cuda, used, 3, H, Hkv, bits, 91, True, False)
+    c["bias"] += torch.linspace(0, 200, c["bias"].shape[-1], device=cuda)    # (logits rise by up to 18)
+    s = c["start"].tolist()
+    g = torch.Generator(device=cuda).manual_seed(1)
+    v = torch.randn(c["cache"].rows, Hkv, 4, 32, generator=g, device=cuda)
+    big = torch.rand(v.shape, generator=g, device=cuda) * 2 - 1
+    v[s[0]:s[0] + 4] = 1.6e38 * big[s[0]:s[0] + 4]
+    v[s[1]:s[1] + 300, :, 1] = 1.6e38 * big[s[1]:s[1] + 300, :, 1]           # one group of every key
+    v[s[2] + 650] = 1.6e38 * big[s[2] + 650]                                 # one key late in its sequence
+    v[s[3]:s[3] + 1500] = 3e36 * big[s[3]:s[3] + 1500]
+    v[s[3]:s[3] + 1500, :, 2] = 3.2e38 - 1e37 * big[s[3]:s[3] + 1500, :, 2].abs()   # all near the largest, of one sign
+    v[s[4] + 10] = 3.3e38
+    Q.kv_quantize(v.flatten(2).bfloat16(), v.flatten(2).bfloat16(), c["cache"])
+    k = torch.randn(v.flatten(2).shape, generator=g, device=cuda).bfloat16()
+    keys = Q.QuantKV.alloc(c["cache"].rows, Hkv, bits, cuda)
+    Q.kv_quantize(k, k, keys)
+    c["cache"].k.copy_(keys.k)
+    c["cache"].k_meta.copy_(keys.k_meta)
+    ws = Q.decode_attention_quant_workspace(len(used), c["shape"], c["max_k"], cuda)
+    cache = clone_cache(c["cache"])
+    out = run_attn(c, cache, ws)
+    torch.cuda.synchronize()
+    assert bool(torch.isfinite(out).all())
+    check_attn(c, out, cache)

@@ -262,8 +262,9 @@ __global__ __launch_bounds__(256) void kv_dequantize_kernel(QuantCache c, RowTar
 //     n of keys 4 j + G, whose nibble (byte) e is element 16 e + n: eight keys of one element, and the element's
 //     group depends on e alone.
 //   * The new key is not in the tiles: it is a part of its own beside the waves', from registers.
-//   * The running maximum moves only when a logit passes it by 2^8.  Waves merge in LDS, chunks through the
-//     workspace in the workgroup that arrives last.
+//   * The running maximum moves only when a logit passes it by 2^8.  Values near the largest float would
+//     pass fp32's range in these sums: a wave whose sums come near it takes its tiles once more, with weights 2^-64 of these.
+//     Waves merge in LDS, chunks through the workspace in the workgroup that arrives last.
 // Measured, 16 / 8 heads: 4 bits, one sequence of 1, 300, 2320, 32769, 131072 keys 6.0, 9.7, 10.5, 22, 44 us (over a bf16
 // cache by tg_decode_attention 2320 13, 32769 36); 64 x 4096 71 (4.7 TB/s; bf16 191), 8 x 80000 152 (5.4 TB/s); 8 bits
 // 6.0, 10.6, 11.8, 27, 64; 113 (5.4), 259 (5.7).  A short sequence is bound by its chain of latencies: launch, lengths
@@ -301,6 +302,9 @@ constexpr int kTile = 64;        // keys of a wave's step
 constexpr int depth(int bits, int hp) { return bits == 4 && hp <= 2 ? 2 : 1; }
 __host__ __device__ constexpr int per_cu(int bits, int hp) { return depth(bits, hp) == 2 || hp == 4 ? 2 : 3; }
 constexpr float kRescaleTau = 8.f;
+// A wave whose sums pass kLargeSum takes its tiles once more with weights 2^-kLift of these: 2^8 p s (c + 24) over 2^24 keys
+// stays below it up to steps of 2^60, and then up to the largest.
+constexpr float kLargeSum = 0x1p100f, kLift = 64.f;
 constexpr int kParts = 3;        // bf16 numbers of a weight
 
 template <typename T>
@@ -525,8 +529,10 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(BITS, HP)) void decode_attn_qua
   float new_bias = 0.f;
   if (HAS_BIAS && has_new && wave == kWaves - 1 && G < HP)
     new_bias = a.bias[(int64_t)b * a.bias_bs + (int64_t)(h0 + min(G, nh - 1)) * a.bias_hs + nk];
-  int t = t_lo + wave;
-  if (t < t_hi) {
+  int t = 0;
+  auto first_loads = [&] {
+    t = t_lo + wave;
+    if (t >= t_hi) return;
 #pragma unroll
     for (int d = 0; d < kDepth; ++d) {
       load_k(tiles[d], t + d * kWaves);
@@ -535,7 +541,8 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(BITS, HP)) void decode_attn_qua
       load_v(tiles[d], t + d * kWaves);
       __builtin_amdgcn_sched_barrier(0);
     }
-  }
+  };
+  first_loads();
   if (forms) {
     float x[8], wf[8], y[8], cs[8][2];
     unpack8(raw, x);
@@ -601,16 +608,8 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(BITS, HP)) void decode_attn_qua
   }
 
   f32x4 oacc[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) oacc[e] = f32x4{0.f, 0.f, 0.f, 0.f};
   float mrun[HP], lsum[HP], rest[HP][kGroups];   // rest: sums of p m', by lane
-#pragma unroll
-  for (int i = 0; i < HP; ++i) {
-    mrun[i] = -INFINITY;
-    lsum[i] = 0.f;
-#pragma unroll
-    for (int g = 0; g < kGroups; ++g) rest[i][g] = 0.f;
-  }
+  float lift = 0.f;                              // the running maximum is so far above the logits' (alike in the wave)
   // position of this lane's key in A's order of keys: lane (m, G) takes keys 4 j + G, j = 0 .. 7, of 32
   // row of the weights that this lane holds in A: heads' first parts, second, third and as many rows of these again, which
   // no sum is taken of
@@ -671,14 +670,14 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(BITS, HP)) void decode_attn_qua
       asm("" : "+v"(z[i]));   // rounded: contracted into z - m below, a bias near the lowest float leaves the rounding's rest
       if (t * kTile + lane >= nk) z[i] = -INFINITY;
       if constexpr (HAS_BIAS) z[i] = l.bias[i] == -INFINITY ? -INFINITY : z[i];   // hidden, whatever the row holds
-      up |= z[i] > mrun[i] + kRescaleTau;
+      up |= z[i] > mrun[i] + (kRescaleTau - lift);
     }
     load_k(l, t + kDepth * kWaves);
     __builtin_amdgcn_sched_barrier(0);
     if (__builtin_amdgcn_ballot_w64(up)) {
 #pragma unroll
       for (int i = 0; i < HP; ++i) {
-        const float m = fmaxf(mrun[i], wave_max(z[i])), f = mrun[i] == -INFINITY ? 0.f : fast_exp2(mrun[i] - m);
+        const float m = fmaxf(mrun[i], wave_max(z[i]) + lift), f = mrun[i] == -INFINITY ? 0.f : fast_exp2(mrun[i] - m);
         mrun[i] = m;
         lsum[i] *= f;
 #pragma unroll
@@ -739,39 +738,56 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(BITS, HP)) void decode_attn_qua
     __builtin_amdgcn_sched_barrier(0);
     t += kWaves;
   };
-  if constexpr (kDepth == 2) {
-    // (an exit between the two steps would leave the compiler a path on which the second tile's loads are the older)
-    while (t + kWaves < t_hi) {
-      step(tiles[0]);
-      step(tiles[1]);
+  for (;;) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) oacc[e] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < HP; ++i) {
+      mrun[i] = -INFINITY;
+      lsum[i] = 0.f;
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g) rest[i][g] = 0.f;
     }
-    if (t < t_hi) step(tiles[0]);
-  } else {
-    while (t < t_hi) step(tiles[0]);
-  }
+    if constexpr (kDepth == 2) {
+      // (an exit between the two steps would leave the compiler a path on which the second tile's loads are the older)
+      while (t + kWaves < t_hi) {
+        step(tiles[0]);
+        step(tiles[1]);
+      }
+      if (t < t_hi) step(tiles[0]);
+    } else {
+      while (t < t_hi) step(tiles[0]);
+    }
 
-  // ---- the waves' results meet in LDS ----
+    // ---- the waves' results meet in LDS ----
+    bool fine = true;
 #pragma unroll
-  for (int i = 0; i < HP; ++i) {
-    const float l = wave_add(lsum[i]);
-    if (lane == 0) {
-      part_ml[wave][i][0] = mrun[i];
-      part_ml[wave][i][1] = l;
-    }
+    for (int i = 0; i < HP; ++i) {
+      const float l = wave_add(lsum[i]);
+      if (lane == 0) {
+        part_ml[wave][i][0] = mrun[i];
+        part_ml[wave][i][1] = l;
+      }
 #pragma unroll
-    for (int g = 0; g < kGroups; ++g) {
-      const float r = wave_add(rest[i][g]);
-      auto sum_parts = [&](const f32x4 &o) {     // (lane group G holds A's rows 4 G .. 4 G + 3)
-        if constexpr (HP == 1) return o[0] + (o[1] + o[2]);
-        else if constexpr (HP == 2) return add_row_pair(G & 1 ? o[i] : o[i] + o[i + 2]);
-        else return add_rows(G < kParts ? o[i] : 0.f);
-      };
-      const float o0 = sum_parts(oacc[2 * g]), o1 = sum_parts(oacc[2 * g + 1]);
-      if (G == g) {                              // lane group g writes group g's elements
-        part_o[wave][i][32 * g + n16] = o0 + r;
-        part_o[wave][i][32 * g + 16 + n16] = o1 + r;
+      for (int g = 0; g < kGroups; ++g) {
+        const float r = wave_add(rest[i][g]);
+        auto sum_parts = [&](const f32x4 &o) {     // (lane group G holds A's rows 4 G .. 4 G + 3)
+          if constexpr (HP == 1) return o[0] + (o[1] + o[2]);
+          else if constexpr (HP == 2) return add_row_pair(G & 1 ? o[i] : o[i] + o[i + 2]);
+          else return add_rows(G < kParts ? o[i] : 0.f);
+        };
+        const float o0 = sum_parts(oacc[2 * g]), o1 = sum_parts(oacc[2 * g + 1]);
+        if (G == g) {                              // lane group g writes group g's elements
+          part_o[wave][i][32 * g + n16] = o0 + r;
+          part_o[wave][i][32 * g + 16 + n16] = o1 + r;
+          fine &= fabsf(o0 + r) < kLargeSum && fabsf(o1 + r) < kLargeSum;
+        }
       }
     }
+    // (a NaN that a key holds comes again)
+    if (lift != 0.f || !__builtin_amdgcn_ballot_w64(!fine)) break;
+    lift = kLift;
+    first_loads();
   }
   __syncthreads();
   constexpr int kOuts = HP * kHeadDim / 2;       // pairs of output elements
