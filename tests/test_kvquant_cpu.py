@@ -208,3 +208,17 @@ def test_copies_of_a_cache_are_their_own(monkeypatch):
         cut.k = whole.v[:, 3:13]
     with pytest.raises(AttributeError):
         cut.bits = 8
+
+
+def test_outputs_that_overlap_in_part(ptr):
+    """Strides by which some row of some head shares memory with another one's, neither of which is contained in the
+    other: refused, against a list of every element's address."""
+    p = ptr[0]
+    read = dict(kc=p, km=p, vc=p, vm=p, rows=9, head_rows=9, hkv=4, d=128, bits=8, map=None, n=6, k=p, k_rs=1024, k_hs=128,
+                v=p, v_rs=1024, v_hs=128, stream=None)
+    for rs, hs in ((256, 256), (384, 256), (128, 640), (640, 384), (136, 128), (256, 392), (512, 1016), (8, 704), (1024, 336)):
+        for n, hkv in ((6, 4), (3, 2)):
+            at = torch.arange(n)[:, None, None] * rs + torch.arange(hkv)[:, None] * hs + torch.arange(128)
+            if at.unique().numel() < at.numel():
+                assert "overlap" in _call("tg_kv_dequantize", read, n=n, hkv=hkv, k_rs=rs, k_hs=hs), (rs, hs, n, hkv)
+                assert "overlap" in _call("tg_kv_dequantize", read, n=n, hkv=hkv, v_rs=rs, v_hs=hs), (rs, hs, n, hkv)

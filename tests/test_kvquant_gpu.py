@@ -590,3 +590,28 @@ def test_values_near_the_largest_float(cuda, bits, H, Hkv):
     torch.cuda.synchronize()
     assert bool(torch.isfinite(out).all())
     check_attn(c, out, cache)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_interleaved_outputs(cuda, bits):
+    """Rows to read back into whose heads lie among those of other tensors, to the last element that may be written."""
+    from tokengate_amd import kvquant as Q
+    n, hkv = 6, 4
+    k, v = rand_rows(cuda, n, hkv, 12)
+    c = Q.QuantKV.alloc(n, hkv, bits, cuda)
+    Q.kv_quantize(k, v, c)
+    want = Q.kv_dequantize(c)
+
+    def check(view):
+        """view: of a flat buffer, (n, hkv, 128); the rest of the buffer is left as it was."""
+        flat = [torch.full((16 * n * hkv * 128,), 9.0, dtype=torch.bfloat16, device=cuda) for _ in range(2)]
+        got = Q.kv_dequantize(c, out=tuple(view(f) for f in flat))
+        for f, g, w in zip(flat, got, want):
+            assert torch.equal(g, w)
+            g.fill_(9.0)
+            assert bool((f == 9.0).all())
+    check(lambda f: f[:n * (2 * hkv - 1) * 128].view(n, 2 * hkv - 1, 128)[:, ::2])            # every second head
+    check(lambda f: f[:hkv * (2 * n - 1) * 128].view(hkv, 2 * n - 1, 128)[:, ::2].transpose(0, 1))   # every second row of a head
+    check(lambda f: f.as_strided((n, hkv, 128), (3 * 128, 19 * 128, 1)))                      # rows of one head among another's
+    check(lambda f: f.as_strided((n, hkv, 128), (9 * 128, 2 * 128, 1)))
+    check(lambda f: f.as_strided((n, hkv, 128), (5 * 128, 7 * 128, 1)))                       # neither within the other

@@ -971,8 +971,16 @@ extern "C" int tg_kv_dequantize(const void *k_codes, const void *k_meta, const v
   if (int e = check_rows("kv_dequantize", k_out, k_row_stride, k_head_stride, v_out, v_row_stride, v_head_stride, n_rows, num_heads_k))
     return e;
   TG_CHECK(rows || n_rows <= cache_rows, "kv_dequantize: more rows than the cache holds");
-  auto apart = [&](int64_t rs, int64_t hs) {     // rows of all heads, or heads of all rows, one behind another
-    return (n_rows <= 1 || rs >= kHeadDim) && (n_rows <= 1 || num_heads_k == 1 || rs >= num_heads_k * hs || hs >= n_rows * rs);
+  // no row of a head within 128 elements of another: of the same head, or of the one h heads on, whose nearest rows are the
+  // two around h hs / rs
+  auto apart = [&](int64_t rs, int64_t hs) {
+    if (n_rows <= 1) return true;
+    if (rs < kHeadDim) return false;
+    for (int64_t h = 1; h < num_heads_k; ++h) {
+      const int64_t d = std::min(h * hs / rs, n_rows - 1);
+      if (h * hs - d * rs < kHeadDim || (d + 1 < n_rows && (d + 1) * rs - h * hs < kHeadDim)) return false;
+    }
+    return true;
   };
   TG_CHECK(apart(k_row_stride, k_head_stride) && apart(v_row_stride, v_head_stride), "kv_dequantize: rows of the outputs overlap");
   if (n_rows == 0) return 0;
