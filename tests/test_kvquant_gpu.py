@@ -615,3 +615,18 @@ def test_interleaved_outputs(cuda, bits):
     check(lambda f: f.as_strided((n, hkv, 128), (3 * 128, 19 * 128, 1)))                      # rows of one head among another's
     check(lambda f: f.as_strided((n, hkv, 128), (9 * 128, 2 * 128, 1)))
     check(lambda f: f.as_strided((n, hkv, 128), (5 * 128, 7 * 128, 1)))                       # neither within the other
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_sources_of_any_strides(cuda, bits):
+    """One row for every head (a head stride of 0), one for every place (a row stride of 0), heads that overlap."""
+    from tokengate_amd import kvquant as Q
+    k, v = rand_rows(cuda, 7, 1, 8)
+    flat = torch.randn(4096, generator=torch.Generator(device=cuda).manual_seed(2), device=cuda).bfloat16()
+    for a, b in ((k.expand(7, 5, 128), v.expand(7, 5, 128)), (k[:1].expand(7, 5, 128), v[:1].expand(7, 5, 128)),
+                 (flat.as_strided((7, 5, 128), (256, 64, 1)), flat.as_strided((7, 5, 128), (8, 16, 1)))):
+        c, d = (Q.QuantKV.alloc(7, 5, bits, cuda) for _ in range(2))
+        Q.kv_quantize(a, b, c)
+        Q.kv_quantize(a.contiguous(), b.contiguous(), d)
+        assert torch.equal(c.k, d.k) and torch.equal(c.v, d.v)
+        assert torch.equal(c.k_meta, d.k_meta) and torch.equal(c.v_meta, d.v_meta) and bool(c.k.any())

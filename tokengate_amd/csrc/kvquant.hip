@@ -925,9 +925,8 @@ int check_rows(const char *what, const void *k, int64_t k_rs, int64_t k_hs, cons
                int64_t n_rows, int heads) {
   TG_CHECK(k && v, "%s: null row pointer", what);
   TG_CHECK(n_rows >= 0 && n_rows < (1ll << 31) && row_blocks(n_rows, heads) < (1ll << 31), "%s: bad row count", what);
-  TG_CHECK(k_rs >= 0 && v_rs >= 0 && k_hs >= kHeadDim && v_hs >= kHeadDim && k_rs % 8 == 0 && v_rs % 8 == 0 &&
-               k_hs % 8 == 0 && v_hs % 8 == 0,
-           "%s: strides must be multiples of 8 elements, head strides at least 128", what);
+  TG_CHECK(k_rs >= 0 && v_rs >= 0 && k_hs >= 0 && v_hs >= 0 && k_rs % 8 == 0 && v_rs % 8 == 0 && k_hs % 8 == 0 && v_hs % 8 == 0,
+           "%s: strides must be multiples of 8 elements", what);
   TG_CHECK(aligned16(k) && aligned16(v), "%s: rows must be 16-byte aligned", what);
   return 0;
 }
@@ -971,6 +970,7 @@ extern "C" int tg_kv_dequantize(const void *k_codes, const void *k_meta, const v
   if (int e = check_rows("kv_dequantize", k_out, k_row_stride, k_head_stride, v_out, v_row_stride, v_head_stride, n_rows, num_heads_k))
     return e;
   TG_CHECK(rows || n_rows <= cache_rows, "kv_dequantize: more rows than the cache holds");
+  TG_CHECK(k_head_stride >= kHeadDim && v_head_stride >= kHeadDim, "kv_dequantize: head strides of outputs must be at least 128");
   // no row of a head within 128 elements of another: of the same head, or of the one h heads on, whose nearest rows are the
   // two around h hs / rs
   auto apart = [&](int64_t rs, int64_t hs) {
