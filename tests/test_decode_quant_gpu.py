@@ -155,3 +155,24 @@ def test_release_and_refusals(cuda):
         n = st.groups[0].n0[b]
         assert torch.equal(st.kv[0].k[:, s:s + n], first.k[:, s:s + n]) and bool(st.kv[0].k[:, s + n].any())
         assert not bool(st.kv[0].k[:, s + n + 1:s + n + 4].any())
+
+
+@pytest.mark.parametrize("draws,steps", [(4, 3), (5, 4), (9, 4)])
+def test_steps_that_a_sampler_allows(cuda, draws, steps):
+    """A state takes max_steps steps, one less than its sampler has random numbers for (the first are the first token's), and
+    max_new_tokens at most; each with its own."""
+    from tokengate_amd import decode as D
+    m = _model(cuda, seed=4)
+    pf = _prefill(m, False, 4)
+    sam = D.TokenSampler(D.Sampling(1.3, seed=5), 3, m.config.vocab, draws, cuda)
+    st = D.DecodeState(m.weights, m.gate, m.gate_layer, pf, 4, kv_bits=8, sampler=sam)
+    assert st.max_steps == steps
+    sam.set_step(0)
+    cur, _ = sam(pf.logits.float())
+    for i in range(steps):
+        cur = st.step(cur)
+        assert torch.equal(sam.u, sam.draws[i + 1])
+        assert torch.equal(cur, sam(st.last_logits)[0])
+    with pytest.raises(RuntimeError, match="random numbers" if draws == 4 else "full"):
+        st.step(cur)
+    assert D.DecodeState(m.weights, m.gate, m.gate_layer, pf, 4, kv_bits=8).max_steps == 4

@@ -120,7 +120,10 @@ class DecodeState:
                  kv_bits: int = 16, sampler: Optional[TokenSampler] = None, release_kv: bool = False):
         """kv_bits: 16 (the prefill's bf16 caches), 8 or 4 (quantised copies of them).  sampler: draws the tokens
         (step i takes its random numbers i + 1; the first token's are 0), else greedy.  release_kv: with
-        quantised caches, drops pf's reference to each bf16 cache as soon as it is quantised."""
+        quantised caches, drops pf's reference to each bf16 cache as soon as it is quantised.
+
+        max_steps, the steps that the state takes: max_new_tokens, for which the caches have room; with a sampler of
+        n random numbers per sequence n - 1 at most (n = max_new_tokens tokens in all, the first among them)."""
         shape = wts.shape
         if kv_bits not in (4, 8, 16):
             raise ValueError(f"DecodeState: kv_bits must be 16, 8 or 4 (got {kv_bits})")
@@ -190,6 +193,7 @@ class DecodeState:
         self.rows_b = torch.arange(B, device=dev)
         self.steps = 0
         self.max_new_tokens = max_new_tokens
+        self.max_steps = max_new_tokens if sampler is None else min(max_new_tokens, sampler.draws.shape[0] - 1)
         self.use_graph = graph
         self.fused = fused
         self._graph = None
@@ -201,9 +205,9 @@ class DecodeState:
         (self.last_logprobs then holds their log probabilities, until the next step)."""
         if self.steps >= self.max_new_tokens:
             raise RuntimeError("DecodeState: more steps than max_new_tokens (the caches are full)")
+        if self.steps >= self.max_steps:
+            raise RuntimeError("DecodeState: more steps than max_steps (the sampler has no random numbers for another)")
         if self.sampler is not None:
-            if self.steps + 1 >= self.sampler.draws.shape[0]:
-                raise RuntimeError("DecodeState: the sampler has no random numbers for another step")
             self.sampler.set_step(self.steps + 1)
         if not self.use_graph or self.steps == 0:
             out = self._body(tokens)
