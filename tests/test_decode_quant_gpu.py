@@ -176,3 +176,15 @@ def test_steps_that_a_sampler_allows(cuda, draws, steps):
     with pytest.raises(RuntimeError, match="random numbers" if draws == 4 else "full"):
         st.step(cur)
     assert D.DecodeState(m.weights, m.gate, m.gate_layer, pf, 4, kv_bits=8).max_steps == 4
+
+
+def test_samplers_of_another_batch(cuda):
+    """A sampler for other sequences or fewer tokens than the state's is refused before anything is appended."""
+    from tokengate_amd import decode as D
+    m = _model(cuda, seed=4)
+    pf = _prefill(m, False, 4)
+    for b, vocab in ((2, m.config.vocab), (4, m.config.vocab), (3, m.config.vocab - 1)):
+        sam = D.TokenSampler(D.Sampling(), b, vocab, 6, cuda)
+        with pytest.raises(ValueError, match="sampler is for"):
+            D.DecodeState(m.weights, m.gate, m.gate_layer, pf, 4, sampler=sam)
+    D.DecodeState(m.weights, m.gate, m.gate_layer, pf, 4, sampler=D.TokenSampler(D.Sampling(), 3, m.config.vocab, 6, cuda))

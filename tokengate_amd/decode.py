@@ -81,6 +81,7 @@ class TokenSampler:
 
     def __init__(self, sampling: Sampling, B: int, vocab: int, n_draws: int, device):
         sampling.check(B)
+        self.batch, self.vocab = B, vocab
         self.settings = [h2d(torch.tensor(sampling._values(name, B), dtype=dt), device)
                          for name, dt in (("temperature", torch.float32), ("top_k", torch.int32),
                                           ("top_p", torch.float32), ("min_p", torch.float32))]
@@ -129,6 +130,9 @@ class DecodeState:
             raise ValueError(f"DecodeState: kv_bits must be 16, 8 or 4 (got {kv_bits})")
         if sampler is not None and sampler.draws.shape[0] < max_new_tokens:
             raise ValueError("DecodeState: the sampler has fewer random numbers than max_new_tokens")
+        if sampler is not None and (sampler.batch != len(pf.n_kept) or sampler.vocab < wts.lm_head.shape[0]):
+            raise ValueError(f"DecodeState: the sampler is for {sampler.batch} sequences and {sampler.vocab} tokens, the model's "
+                             f"are {len(pf.n_kept)} and {wts.lm_head.shape[0]}")
         self.wts, self.shape = wts, shape
         if self.max_fused_rows is None:
             self.max_fused_rows = 8 if shape.d_model <= 2048 else 2
