@@ -222,3 +222,16 @@ def test_outputs_that_overlap_in_part(ptr):
             if at.unique().numel() < at.numel():
                 assert "overlap" in _call("tg_kv_dequantize", read, n=n, hkv=hkv, k_rs=rs, k_hs=hs), (rs, hs, n, hkv)
                 assert "overlap" in _call("tg_kv_dequantize", read, n=n, hkv=hkv, v_rs=rs, v_hs=hs), (rs, hs, n, hkv)
+
+
+def test_temperatures_of_fp32():
+    """Temperatures are passed on as fp32 numbers: those that would be infinite there are refused, those that would be 0 are
+    greedy."""
+    from tokengate_amd.decode import Sampling
+    most = torch.finfo(torch.float32).max
+    Sampling([most, 1e-60, 0.0]).check(3)
+    for t in (2 * most, 1e39, 1e300):
+        with pytest.raises(ValueError, match="temperature"):
+            Sampling(t).check(2)
+        with pytest.raises(ValueError, match="temperature"):
+            Sampling([1.0, t]).check(2)

@@ -48,6 +48,9 @@ class _Group:
     gap: int
 
 
+MAX_TEMPERATURE = torch.finfo(torch.float32).max
+
+
 @dataclass
 class Sampling:
     """How next tokens are drawn (decoder.sample_rows); every setting a number, or a sequence with one per
@@ -67,7 +70,7 @@ class Sampling:
 
     def check(self, B: int) -> None:
         """ValueError unless every setting is a number of its range, one or B of them."""
-        for name, ok, what in (("temperature", lambda v: 0 <= v < math.inf, "a finite number of at least 0"),
+        for name, ok, what in (("temperature", lambda v: 0 <= v <= MAX_TEMPERATURE, "a finite fp32 number of at least 0"),
                                ("top_k", lambda v: v == int(v) and 0 <= v < 2 ** 31, "a whole number of at least 0"),
                                ("top_p", lambda v: 0 <= v <= 1, "in 0..1"), ("min_p", lambda v: 0 <= v <= 1, "in 0..1")):
             for v in self._values(name, B):
