@@ -308,3 +308,23 @@ def test_parts_far_apart_at_high_temperatures(cuda):
                 near += border
                 assert tok[0] in (5, 77) and tok[1] in (39000, 39999)
     assert near == 0
+
+
+@pytest.mark.parametrize("v", [20000, 151936, 262144])
+def test_tails_that_decide(cuda, v):
+    """One logit with nearly all of the mass and the rest, of few values as bf16 logits have, far below it: tokens and top_p's
+    ends among the rest, which together weigh 2^-8 .. 2^-24 of it, and the log probabilities that their sum makes."""
+    n = 12
+    g = torch.Generator().manual_seed(v)
+    rng = np.random.default_rng(v)
+    near = 0
+    for t in (1.0, 2.0, 3.0, 8.0, 40.0):
+        x = torch.randn(n, v, generator=g).bfloat16().float()
+        x[::3] = 0.375                                  # all alike
+        x[1::3] = (x[1::3] * 0.25).bfloat16().float()
+        peak = t * (np.log(v) + rng.uniform(6, 16, n))
+        x[torch.arange(n), torch.arange(n) * 997 % v] = torch.from_numpy(peak).float()
+        for k, p, m in ((0, 1.0, 0.0), (v // 2, 1.0, 0.0), (0, 1 - 2.0 ** -19, 0.0), (0, 1.0, 2.0 ** -50)):
+            for u in (0.3, 1 - 2.0 ** -16):
+                near += check(cuda, x, [u] * n, [t] * n, [k] * n, [p] * n, [m] * n)[2]
+    assert near < n * 5 * 4 * 2 / 2                     # (the rest's borders are nearer to one another than 2^-34 in many rows)

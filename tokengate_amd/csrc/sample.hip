@@ -53,7 +53,7 @@ struct SampleArgs {
 // One workgroup's bins: [f, f + 1) of y for f in top - 511 .. top, at f mod 512
 struct Part {
   double top;
-  uint64_t tail;                                 // mass below the bins, in units of 2^-44 of 2^(top / q)
+  double tail;                                   // mass below the bins, in units of 2^(top / q)
   uint32_t best, least;                          // order bits of the largest logit, and of the smallest within reach
   uint32_t fine, pad;                            // Row's
   uint64_t hist[kBins];                          // count << 48 | sum of (e^t - 0.9) 2^33
@@ -288,7 +288,7 @@ __device__ __forceinline__ T block_scan(T v, T *tmp, T &total) {
   return v + (wave ? read_lane(s, wave - 1) : T(0));
 }
 // Three at once: of u and v the sums up to this thread, of w the sum of all; total: u's of all.
-__device__ __forceinline__ void block_scan3(uint64_t &u, uint32_t &v, uint64_t &w, uint64_t *tmp_u, uint32_t *tmp_v, uint64_t *tmp_w,
+__device__ __forceinline__ void block_scan3(uint64_t &u, uint32_t &v, double &w, uint64_t *tmp_u, uint32_t *tmp_v, double *tmp_w,
                                             uint64_t &total) {
   const int lane = threadIdx.x & 63, wave = wave_id();
   u = wave_scan(u);
@@ -301,7 +301,8 @@ __device__ __forceinline__ void block_scan3(uint64_t &u, uint32_t &v, uint64_t &
     tmp_w[wave] = w;
   }
   __syncthreads();
-  const uint64_t su = row_scan(tmp_u[lane & 15]), sw = row_scan(tmp_w[lane & 15]);
+  const uint64_t su = row_scan(tmp_u[lane & 15]);
+  const double sw = row_scan(tmp_w[lane & 15]);
   const uint32_t sv = row_scan(tmp_v[lane & 15]);
   total = read_lane(su, 15);
   w = read_lane(sw, 15);
@@ -456,7 +457,7 @@ __global__ __launch_bounds__(kThreads, 4) void sample_hist_kernel(SampleArgs a, 
   const float *x = a.x + b * a.rs;
   __shared__ uint64_t hist[kBins];
   __shared__ uint32_t tmp[16];
-  __shared__ unsigned long long tail_s;
+  __shared__ double tail_s[16];
   __shared__ uint32_t last_s;
   const Share share(a.n);
   float most = -INFINITY, least = INFINITY;      // (maxima of pairs drop NaN; -inf has no weight)
@@ -468,7 +469,6 @@ __global__ __launch_bounds__(kThreads, 4) void sample_hist_kernel(SampleArgs a, 
     least = v > -INFINITY ? fminf(least, v) : least;
   });
   if (tid < kBins) hist[tid] = 0;
-  if (tid == 0) tail_s = 0;
   uint32_t best = block_max(order_bits(most), tmp);   // (its barriers cover the bins)
   uint32_t low_bits = ~block_max(~order_bits(least), tmp);
   const float end = order_float(best) - reach;
@@ -487,6 +487,7 @@ __global__ __launch_bounds__(kThreads, 4) void sample_hist_kernel(SampleArgs a, 
   const int fine = low_bits == ~0u ? 0 : coarse.finest(order_float(best), order_float(low_bits));
   const Row row(coarse, fine);
   const double top = best == kNone ? 0.0 : floor(row.y(order_float(best)));
+  double tail_mine = 0.0;                        // (a double: weights of any size, in an order that the launch gives)
   const double scale = kLn2 * row.per_q;
   const int top_slot = slot_of(top);
   share.each(x, [&](float v, int) {
@@ -496,15 +497,18 @@ __global__ __launch_bounds__(kThreads, 4) void sample_hist_kernel(SampleArgs a, 
       atomicAdd((unsigned long long *)&hist[(top_slot - (int)j) & (kBins - 1)], (unsigned long long)hist_add((y - f - 0.5) * scale));
     } else {
       const double w = row.weight(y, top);
-      if (w > 0x1p-46) atomicAdd(&tail_s, (unsigned long long)(w * 0x1p44 + 0.5));
+      if (w > 0x1p-72) tail_mine += w;           // (2^18 of less: 2^-54)
     }
   });
+  tail_mine = wave_scan(tail_mine);
+  if ((tid & 63) == 63) tail_s[wave_id()] = tail_mine;
   __syncthreads();
   Part *const part = ws.parts + (int64_t)b * parts;
   if (tid < kBins) st_agent(&part[g].hist[tid], hist[tid]);
+  const double tail_part = read_lane(row_scan(tail_s[tid & 15]), 15);
   if (tid == 0) {
     st_agent((uint64_t *)&part[g].top, bits_of(top));
-    st_agent(&part[g].tail, (uint64_t)tail_s);
+    st_agent((uint64_t *)&part[g].tail, bits_of(tail_part));
     st_agent((uint64_t *)&part[g].best, (uint64_t)low_bits << 32 | best);
     st_agent(&part[g].fine, (uint32_t)fine);
   }
@@ -517,7 +521,8 @@ __global__ __launch_bounds__(kThreads, 4) void sample_hist_kernel(SampleArgs a, 
 
   // ---- the row's bins ----
   __shared__ double mass_s[kBins];
-  __shared__ uint64_t scan_m[16], scan_t[16];
+  __shared__ uint64_t scan_m[16];
+  __shared__ double scan_t[16];
   __shared__ uint64_t sums[2][kBins];
   __shared__ uint32_t counts[2][kBins], count_s[kBins], scan_u[16];
   __shared__ int first_s[4];
@@ -600,7 +605,7 @@ __global__ __launch_bounds__(kThreads, 4) void sample_hist_kernel(SampleArgs a, 
     }
   }
   if (tid < parts && part_best != kNone)
-    tail += exp2_of((ldexp(part_top, -part_finer) - gtop) * whole.per_q) * ((double)ld_agent(&part[tid].tail) * 0x1p-44);
+    tail += exp2_of((ldexp(part_top, -part_finer) - gtop) * whole.per_q) * double_of(ld_agent((const uint64_t *)&part[tid].tail));
   __syncthreads();
   {
     const int j = (slot_of(gtop) - slot) & (kBins - 1);
@@ -617,10 +622,11 @@ __global__ __launch_bounds__(kThreads, 4) void sample_hist_kernel(SampleArgs a, 
   }
   // (as whole numbers: no bin's sum is less than the one's before it, as roundings could make it)
   uint32_t upto_count = count;
-  uint64_t upto_u = (uint64_t)(m * 0x1p44 + 0.5), tail_u = (uint64_t)(tail * 0x1p44), in_bins_u;
-  block_scan3(upto_u, upto_count, tail_u, scan_m, scan_u, scan_t, in_bins_u);
+  uint64_t upto_u = (uint64_t)(m * 0x1p44 + 0.5), in_bins_u;
+  double tail_all = tail;
+  block_scan3(upto_u, upto_count, tail_all, scan_m, scan_u, scan_t, in_bins_u);
   const double upto = (double)upto_u * 0x1p-44;
-  const double in_bins = (double)in_bins_u * 0x1p-44, tail_all = (double)tail_u * 0x1p-44, mass = in_bins + tail_all;
+  const double in_bins = (double)in_bins_u * 0x1p-44, mass = in_bins + tail_all;
   const bool tail_counts = tail_all > 0x1p-42 * mass;
   if (half == 0) {
     mass_s[j] = upto;
@@ -709,9 +715,10 @@ struct Place {
   uint32_t ties;
   uint64_t above;   // count or mass of the elements above key
 };
-// Masses as whole numbers, in units of 2^-44 of the largest weight.
-__device__ void slow_row(const SampleArgs &a, int b) {
-  constexpr double kMassUnit = 0x1p44;
+// Masses as whole numbers, in units of 2^-mass_bits of the largest weight: as small as the row's mass, in the same units
+// at most row_mass, allows (2^18 roundings of 2^-62 of the whole).
+__device__ void slow_row(const SampleArgs &a, int b, double row_mass) {
+  const int mass_bits = 61 - __builtin_amdgcn_frexp_exp(row_mass);
   const int tid = threadIdx.x;
   const float *x = a.x + b * a.rs;
   __shared__ uint64_t hist[256], red[16];
@@ -747,7 +754,7 @@ __device__ void slow_row(const SampleArgs &a, int b) {
   const bool greedy = !(temp > 0.f) || top == -INFINITY;
   const double scale = greedy ? 1.0 : kLog2e / temp;
   auto weight = [&](float x) { return x == top ? 1.0 : exp2_of(((double)x - (double)top) * scale); };   // (both may be infinite)
-  auto mass = [&](uint32_t key) { return (uint64_t)(weight(order_float(key)) * kMassUnit + 0.5); };
+  auto mass = [&](uint32_t key) { return (uint64_t)(ldexp(weight(order_float(key)), mass_bits) + 0.5); };
   // The first place at which the sum of value(key) over the elements up to it reaches target (> 0).
   auto find = [&](uint64_t target, bool by_mass) {
     uint32_t prefix = 0;
@@ -860,7 +867,7 @@ __device__ void slow_row(const SampleArgs &a, int b) {
     a.token[b] = i;
     const float v = order_float(p.key);
     const double d = v == top ? 0.0 : ((double)v - (double)top) / (double)temp;
-    if (a.logprob) a.logprob[b] = (float)(d - log((double)total / kMassUnit));
+    if (a.logprob) a.logprob[b] = (float)(d - log(ldexp((double)total, -mass_bits)));
   }
 }
 
@@ -885,7 +892,7 @@ __global__ __launch_bounds__(kThreads, 4) void sample_pick_kernel(SampleArgs a, 
   const Row row(Row(a, b), (int)st->fine);
   const Settings set(a, b, row.greedy);
   if (slow != kUsual) {
-    if (g == 0 && slow == kSlow) slow_row(a, b);
+    if (g == 0 && slow == kSlow) slow_row(a, b, st->mass);
     return;
   }
   __shared__ PickShared sh;
