@@ -429,9 +429,10 @@ int tg_argmax_rows(const float *x, int64_t x_row_stride, int32_t n_rows, int64_t
  * elements of S2 with w >= min_p[b], at least one (no min_p: S2); token[b] (int64) = the first of S3 whose
  * cumulated mass exceeds u[b] times S3's, logprob[b] (optional, fp32) = ln(w / mass of S3) of it.
  * temperature <= 0 or NaN: the first of the order, log probability 0; no temperature: 1.  A NaN logit counts as
- * -inf; among infinite logits only the equal ones count; a row of -inf gives token 0.  Weights are doubles, a logit's
- * share of a sum is rounded to 2^-34 of it, and sums are whole numbers of any order: the result does not depend on the
- * launch.  x: fp32 rows of any stride >= n_cols and alignment, at most 65535 of at most 262144 columns; the settings and
+ * -inf; among infinite logits only the equal ones count; a row of -inf gives token 0.  Weights are doubles and
+ * a logit's share of a sum is rounded to 2^-34 of it, so sums are good to 2^-33: a token may be another where u, top_p or
+ * min_p is as near to a border.  One call's result is the same every time; how a row is cut depends on the rows of the
+ * call, so that a row alone and in a batch may differ within these bounds.  x: fp32 rows of any stride >= n_cols and alignment, at most 65535 of at most 262144 columns; the settings and
  * u (below 0 counts as 0, 1 and more as just below 1) are dense device arrays with an entry per row.  Rows of up to 2048
  * columns take one launch and no workspace, longer ones two per 256 rows.  workspace: tg_sample_rows_workspace_size bytes,
  * 16-byte aligned, zeroed once when it is allocated (its counters are zero again when a call's launches end), shared by

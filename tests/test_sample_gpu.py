@@ -328,3 +328,29 @@ def test_tails_that_decide(cuda, v):
             for u in (0.3, 1 - 2.0 ** -16):
                 near += check(cuda, x, [u] * n, [t] * n, [k] * n, [p] * n, [m] * n)[2]
     assert near < n * 5 * 4 * 2 / 2                     # (the rest's borders are nearer to one another than 2^-34 in many rows)
+
+
+def test_rows_alone_and_in_a_batch(cuda):
+    """A row's result alone, in a small batch and in a large one, which cut it into other parts: the same tokens where
+    they are not near a border, and log probabilities within the bounds of both (2^-24 of the value for its rounding,
+    2^-34 for the sums, on either side)."""
+    from tokengate_amd import decoder as dec
+    v, n = 151936, 64
+    rng = np.random.default_rng(3)
+    x = rng.standard_normal((n, v)).astype(np.float32) * rng.choice([0.01, 1.0, 3.0], (n, 1)).astype(np.float32)
+    for b in range(n):                                  # stretches of other spreads and maxima
+        a, e = sorted(rng.integers(0, v, 2))
+        x[b, a:e] = x[b, a:e] * rng.choice([1e-3, 5.0]) + rng.uniform(-12, 6)
+    x = torch.from_numpy(x).to(cuda)
+    u = torch.from_numpy(rng.random(n, dtype=np.float32)).to(cuda)
+    t = torch.from_numpy(rng.uniform(0.3, 1.7, n).astype(np.float32)).to(cuda)
+    p = torch.from_numpy(rng.choice([0.5, 0.9, 1.0], n).astype(np.float32)).to(cuda)
+    tok, lp = dec.sample_rows(x, u, t, top_p=p, logprob=True)
+    near = 0
+    for rows in [slice(b, b + 1) for b in range(0, n, 7)] + [slice(8, 13)]:
+        tok1, lp1, border = check(cuda, x[rows], u[rows].tolist(), t[rows].tolist(), None, p[rows].tolist(), None)
+        near += border
+        if border == 0:
+            assert torch.equal(tok1, tok[rows])
+            assert bool(((lp1 - lp[rows]).abs().double() <= 2.0 ** -23 * lp1.abs() + 2.0 ** -33).all())
+    assert near == 0

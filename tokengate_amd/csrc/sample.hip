@@ -7,7 +7,8 @@
 //   * sample_hist_kernel, several workgroups per row: logits in units of y = cc x (cc = 8 log2 e, or 4 log2 e / T for
 //     T < 0.5, times 2^fine where they lie close together) fall into bins of width one, 512 from the part's largest down.
 //     A bin's count and the sum of its elements' e^t, t = (the fraction of y - 1/2) T-scaled, need no common maximum,
-//     and as whole numbers (one 64-bit LDS addition per logit) no order of additions.  The workgroup that arrives last
+//     and as whole numbers (one 64-bit LDS addition per logit) no order of additions.  (How wide the bins are depends on what
+//     a part holds: cut into other parts, a row's sums differ within their roundings.)  The workgroup that arrives last
 //     merges the row's bins and finds those in which the ends of S1, S2, S3 and the token must lie;
 //   * sample_pick_kernel collects the elements of these bins (up to 16384), and the last workgroup finds each end in its
 //     bin: by 512 parts of the bin's interval of keys (value and index), again in the part that decides, and from 64
