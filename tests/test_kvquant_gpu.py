@@ -630,3 +630,24 @@ def test_sources_of_any_strides(cuda, bits):
         Q.kv_quantize(a.contiguous(), b.contiguous(), d)
         assert torch.equal(c.k, d.k) and torch.equal(c.v, d.v)
         assert torch.equal(c.k_meta, d.k_meta) and torch.equal(c.v_meta, d.v_meta) and bool(c.k.any())
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_groups_of_many_binary_orders(cuda, bits):
+    """Groups whose least value and values differ by many binary orders, so that x - m has up to 24 bits or is rounded,
+    bit for bit."""
+    from tokengate_amd import kvquant as Q
+    g = torch.Generator().manual_seed(9)
+    n = 4096
+    x = torch.randn(n, 4, 32, generator=g) * 2.0 ** torch.randint(-24, 3, (n, 4, 32), generator=g)
+    x[:, 0] = x[:, 0].abs()
+    x[:, 1, 0] = -(1 + 2.0 ** -7) * 2.0 ** -16          # a least value far below the others' last bit
+    x[:, 1, 1:] = x[:, 1, 1:].abs() + 0.5
+    x[:, 2] = 1.0 + x[:, 2].abs() * 2.0 ** -6
+    x[0, 3] = torch.tensor([1.0, -(1 + 2.0 ** -7) * 2.0 ** -16] * 16)
+    k = x.flatten(1)[:, None].bfloat16().to(cuda)
+    v = (k.float() * 2.0 ** 60).bfloat16()
+    cache = Q.QuantKV.alloc(n, 1, bits, cuda)
+    Q.kv_quantize(k, v, cache)
+    torch.cuda.synchronize()
+    check_quantized(cache, k, v, slice(None))

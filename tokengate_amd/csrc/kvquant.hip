@@ -98,10 +98,10 @@ __device__ __forceinline__ void transpose8(uint32_t (&w)[BITS / 4], int j) {
 __device__ __forceinline__ int word_of(int j) { return 8 * (j & 1) + (j >> 1); }
 
 // Quantises a row held by 16 lanes, lane j its elements 8 j .. 8 j + 7: word (pair) word_of(j) of its codes, and the
-// (s, m) pair of its group j / 4.  Quotients are a division's: q = d r with r about 1 / s, and one correction by the
-// remainder, which makes quotients that lie between two codes exact (others are 2^-16 and more away from there:
-// d and s have 16 and 8 significant bits, and the correction's error is 2^-40).  held: the values that the codes
-// stand for.
+// (s, m) pair of its group j / 4.  Quotients are fp32 division's: q = d r with r about 1 / s, and one correction by the
+// remainder, which is off by 2^-45 of q before its rounding.  d has 24 significant bits at most (values may differ by many
+// binary orders) and s has 8, so d / s is no nearer than 2^-33 of itself to a number half way between two floats, and never
+// one: that would have 25 bits, and s times it as many.  So too span / L.  held: the values that the codes stand for.
 template <int BITS>
 __device__ __forceinline__ void quant_row(const float (&x)[8], int j, uint32_t (&w)[BITS / 4], uint32_t &meta,
                                           float (&held)[8]) {
