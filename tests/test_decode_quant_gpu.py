@@ -188,3 +188,42 @@ def test_samplers_of_another_batch(cuda):
         with pytest.raises(ValueError, match="sampler is for"):
             D.DecodeState(m.weights, m.gate, m.gate_layer, pf, 4, sampler=sam)
     D.DecodeState(m.weights, m.gate, m.gate_layer, pf, 4, sampler=D.TokenSampler(D.Sampling(), 3, m.config.vocab, 6, cuda))
+
+
+@pytest.mark.parametrize("B,bits", [(3, 4), (8, 16), (11, 8), (11, 16)])
+def test_long_vocabularies_and_batches(cuda, B, bits):
+    """A vocabulary whose sampling takes two launches and a workspace, inside the captured step, and batches of more rows than
+    the fused projections take: every replay equals the eager step, and every token is what the definition draws from
+    the step's logits."""
+    import numpy as np
+    from tests.test_inference_gpu import SMALL
+    from tests.test_sample_gpu import reference
+    from tokengate_amd import decode as D
+    from tokengate_amd import decoder as dec
+    from tokengate_amd import inference as I
+    m = I.load_model("random:9", gate_layer=1, device=cuda, shape=dec.DecoderShape(**dict(SMALL, vocab=20480)))
+    lens = [70 + 41 * b for b in range(B)]
+    split = [I.split_state_span(p) for p in _prompts(lens, [(5, n - 10) for n in lens], 6)]
+    steps = 4
+    pfs = [m.prefill(split, [40] * B, decode_headroom=steps + 1) for _ in range(2)]
+    kind = [b % 4 for b in range(B)]
+    s = D.Sampling([0.0 if k == 0 else 0.7 + 0.1 * k for k in kind], [20 if k == 1 else 0 for k in kind],
+                   [0.9 if k == 2 else 1.0 for k in kind], [0.02 if k == 3 else 0.0 for k in kind], seed=4)
+    sam = [D.TokenSampler(s, B, 20480, steps + 1, cuda) for _ in range(2)]
+    eager = D.DecodeState(m.weights, m.gate, m.gate_layer, pfs[0], steps, kv_bits=bits, sampler=sam[0])
+    graph = D.DecodeState(m.weights, m.gate, m.gate_layer, pfs[1], steps, graph=True, kv_bits=bits, sampler=sam[1])
+    ce = cg = pfs[0].first_tokens
+    near = 0
+    for i in range(steps):
+        ce, cg = eager.step(ce), graph.step(cg)
+        junk = torch.randn(1 << 20, device=cuda).sum()
+        torch.cuda.synchronize()
+        assert torch.equal(ce, cg) and torch.equal(eager.last_logits, graph.last_logits), i
+        assert torch.equal(eager.last_logprobs, graph.last_logprobs) and bool(torch.isfinite(junk))
+        for b in range(B):
+            t, k, p, mp = (float(np.float32(v[b])) for v in (s.temperature, s.top_k, s.top_p, s.min_p))
+            tok, lp, border = reference(eager.last_logits[b].cpu().numpy(), float(sam[0].u[b]), t, int(k), p, mp)
+            near += border
+            if not border:
+                assert int(ce[b]) == tok and abs(float(eager.last_logprobs[b]) - lp) <= 2.0 ** -24 * abs(lp) + 2.0 ** -34
+    assert near <= 1

@@ -651,3 +651,33 @@ def test_groups_of_many_binary_orders(cuda, bits):
     Q.kv_quantize(k, v, cache)
     torch.cuda.synchronize()
     check_quantized(cache, k, v, slice(None))
+
+
+@pytest.mark.parametrize("bits,used,H,Hkv", [(4, [1 + 61 * i % 700 for i in range(2100)], 8, 8),   # nothing is cut
+                                             (8, [100 + 37 * i for i in range(130)], 8, 8),        # two rounds
+                                             (8, [300 + 997 * i % 5000 for i in range(70)], 12, 4)])
+def test_rows_that_a_large_launch_appends(cuda, bits, used, H, Hkv):
+    """Every sequence's new row as kv_quantize has it, every other row as it was, and outputs of sequences all over the
+    batch in float64."""
+    from tokengate_amd import decoder as dec
+    from tokengate_amd import kvquant as Q
+    c = attn_case(cuda, used, 2, H, Hkv, bits, 5 + len(used), True, True)
+    B = len(used)
+    ws = Q.decode_attention_quant_workspace(B, c["shape"], c["max_k"], cuda)
+    cache, want = clone_cache(c["cache"]), clone_cache(c["cache"])
+    out = run_attn(c, cache, ws)
+    k1, v1 = (torch.empty(B, Hkv, 128, dtype=torch.bfloat16, device=cuda) for _ in range(2))
+    dec.qk_norm_rope(c["qkv"].clone(), c["pos"], c["lw"], c["shape"], c["inv"], k1, v1, c["qs"], c["rs"])
+    Q.kv_quantize(k1, v1, want, dst_rows=c["start"] + c["used"] - 1)
+    torch.cuda.synchronize()
+    for a, b in ((cache.k, want.k), (cache.v, want.v), (cache.k_meta, want.k_meta), (cache.v_meta, want.v_meta)):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+    some = list(range(0, B, max(1, B // 30)))
+    rows = lambda t: t[some].contiguous()
+    part = dict(c, qkv=rows(c["qkv"]), pos=rows(c["pos"]), start=rows(c["start"]), used=rows(c["used"]), bias=rows(c["bias"]),
+                rs=rows(c["rs"]))
+    view = clone_cache(c["cache"])                      # (check_attn appends only these sequences' rows)
+    new = (part["start"] + part["used"] - 1).long()
+    for a, b in ((view.k, cache.k), (view.v, cache.v), (view.k_meta, cache.k_meta), (view.v_meta, cache.v_meta)):
+        a[:, new] = b[:, new]
+    check_attn(part, rows(out), view)
