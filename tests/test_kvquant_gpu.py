@@ -12,6 +12,8 @@ logits, the kernel may be off by (a rounding to bf16, of 8 significant bits, by 
     bits codes are held as 128 + c), at most 2^-20 (128 + L) sum |q| a group (16 roundings), so
     dz = scale max_j sum_g s_jg 2^-20 (128 + L) sum_{d in g} |q_d| + 2^-20 max |z|, and 2 dz sum P |v|;
   * the output's rounding to bf16: 2^-8 |out|; and 2^-18 sum P |v| for the fp32 sums of the values.
+(The kernel's weights have 24 bits and its codes are 16 + c, the offset taken off every 32 keys: these bounds are those of
+16 bits and of 128 + c taken off at the end, which it stays well below; the tests of keys that cancel hold it to its own.)
 """
 import pytest
 import torch

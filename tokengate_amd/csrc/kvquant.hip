@@ -244,9 +244,9 @@ __global__ __launch_bounds__(256) void kv_dequantize_kernel(QuantCache c, RowTar
 // of 32 (g): q . k_j = sum_g s_jg (q . c_j)_g + m_jg Q_g,  Q_g the sum of q over the group, and
 // out = sum_g (p_j s_jg) c'_j + sum_j p_j m'_jg with c' = c - C, m' = m + C s, C the middle code (8 or 128): values of
 // either sign have codes around the middle, so the sums over the keys are as small as the values', where those of p s c
-// and p m would grow with every key and cancel at the end.  Bound by the bytes of the cache (80 or 144 per key and kv head, K and
-// V each), so a workgroup takes one kv head of one sequence, up to four query heads of its group at once, and a
-// stretch of keys: chunks of chunk_tiles tiles of 64 keys, its four waves a tile each in turn.  Nothing is staged
+// and p m would grow with every key and cancel at the end.  Bound by the bytes of the cache (80 or 144 per key and kv
+// head, K and V each), so a workgroup takes one kv head of one sequence, up to four query heads of its group at once,
+// and a stretch of keys: chunks of chunk_tiles tiles of 64 keys, its four waves a tile each in turn.  Nothing is staged
 // through LDS: a wave's matrix instructions take the codes from the registers that the loads fill.
 //   * S = Q C^T on v_mfma_f32_16x16x32_bf16, one instruction per 16 keys and group.  A: row 4 r + i holds query head i
 //     (each head four times), so that every lane group gets all heads' sums and lane l keeps those of key l: the
@@ -258,17 +258,18 @@ __global__ __launch_bounds__(256) void kv_dequantize_kernel(QuantCache c, RowTar
 //     the end, outputs over 131072 keys were off by 5e-4 of their size.)
 //   * O += P C with P = p s per group, from LDS in A's layout, as three bf16 numbers, 24 bits together as fp32's:
 //     rounded to one, the weights of keys that cancel left errors of 0.4 % of the output, to two of 2^-18 L steps.  The
-//     others take rows of A that would repeat the heads, so no more instructions.  The middles' part is summed in fp32.  B: lane (n, G) holds word
-//     n of keys 4 j + G, whose nibble (byte) e is element 16 e + n: eight keys of one element, and the element's
-//     group depends on e alone.
+//     others take rows of A that would repeat the heads, so no more instructions.  The middles' part is summed in fp32.
+//     B: lane (n, G) holds word n of keys 4 j + G, whose nibble (byte) e is element 16 e + n: eight keys of one element,
+//     and the element's group depends on e alone.
 //   * The new key is not in the tiles: it is a part of its own beside the waves', from registers.
 //   * The running maximum moves only when a logit passes it by 2^8.  Values near the largest float would
 //     pass fp32's range in these sums: a wave whose sums come near it takes its tiles once more, with weights 2^-64 of these.
 //     Waves merge in LDS, chunks through the workspace in the workgroup that arrives last.
-// Measured, 16 / 8 heads: 4 bits, one sequence of 1, 300, 2320, 32769, 131072 keys 6.0, 9.7, 10.5, 22, 44 us (over a bf16
-// cache by tg_decode_attention 2320 13, 32769 36); 64 x 4096 71 (4.7 TB/s; bf16 191), 8 x 80000 152 (5.4 TB/s); 8 bits
-// 6.0, 10.6, 11.8, 27, 64; 113 (5.4), 259 (5.7).  A short sequence is bound by its chain of latencies: launch, lengths
-// and norms 4.9 us, the waves' merge 1.5, arrival 1.8, the chunks' merge 2.7, beside the tiles.
+// Measured, 16 / 8 heads: 4 bits, one sequence of 1, 300, 2320, 32769, 131072 keys 6.5, 10.4, 11.3, 23, 47 us (over a bf16
+// cache by tg_decode_attention 2320 13, 32769 36); 64 x 4096 76 (4.4 TB/s; bf16 191), 8 x 80000 157 (5.2 TB/s); 8 bits
+// 6.4, 11.4, 12.4, 28, 66; 116 (5.2), 257 (5.7).  (With weights of 16 bits, 128 + c and sums that may pass fp32's range
+// 6.0, 9.7, 10.5, 22, 44; 71, 152 and 6.0, 10.6, 11.8, 27, 64; 113, 251.)  A short sequence is bound by its chain of
+// latencies: launch, lengths and norms 4.9 us, the waves' merge 2, arrival 1.8, the chunks' merge 2.7, beside the tiles.
 struct QuantAttnArgs {
   const bf16_t *qkv;
   int64_t qkv_rs;
@@ -296,9 +297,9 @@ constexpr int kWaves = 4;
 constexpr int kRounds = 2;
 constexpr int kTile = 64;        // keys of a wave's step
 // Tiles that a wave holds or has on their way, and workgroups per CU, by the registers.  16 / 8 heads (two at once), 4
-// bits, two tiles and 2 workgroups / one and 3: 32769 keys 22.0 / 23.3 us, 64 x 4096 71.4 / 70.6, with bias 72.9 /
-// 73.8; 8 bits, where two tiles spill: 28.7 / 26.9, 119.4 / 112.6, 137 / 118.  Four heads at once, one tile, 2 / 3
-// workgroups (spills): 4 x 8192 keys of 16 / 2 heads 20.5 / 24.4 at 4 bits, 22.4 / 32.5 at 8.
+// bits, two tiles and 2 workgroups / one and 3: 32769 keys 23.5 / 24.5 us, 64 x 4096 79 / 77, with bias 73.4 / 72.6, 64 x
+// 300 15.3 / 14.9; 8 bits, where two tiles spill: 34 / 28, 134 / 118, 148 / 113, 22.5 / 18.1.  Four heads at once, one
+// tile, 2 / 3 workgroups (spills): 4 x 8192 keys of 16 / 2 heads 21.5 / 26.8 at 4 bits, 22.5 / 36.6 at 8.
 constexpr int depth(int bits, int hp) { return bits == 4 && hp <= 2 ? 2 : 1; }
 __host__ __device__ constexpr int per_cu(int bits, int hp) { return depth(bits, hp) == 2 || hp == 4 ? 2 : 3; }
 constexpr float kRescaleTau = 8.f;
@@ -366,10 +367,10 @@ __device__ __forceinline__ uint32_t byte_pair(uint32_t a, uint32_t b, int byte) 
 // ceil(n / T) chunks of even length, with one T for all, from their tiles, which only the device knows: the least that
 // makes no more workgroups than are resident at once (a workgroup's fixed costs, 5 us, and a second round's uneven
 // end cost more than idle places), or, where the sequences' remainders alone would fill most of these, two
-// rounds.  (64 sequences of 300 at 8 bits in chunks of four tiles, a round and a third: 24.9 us; cut for one round: 17.5.)
-// 16 / 8 heads, T for one round of the longest sequence / two rounds / as here, us: 64 sequences of 512 .. 4099
-// at 8 bits 84.7 / 84.3 / 79.8; 8 of 16k .. 128k at 4 bits 183 / 170 / 159; 16 of 4k .. 30k - / 63 / 57; 64 alike of
-// 4096 70 / 77 / 70.
+// rounds.
+// 16 / 8 heads, T for one round as far as it goes / two rounds / as here, us: 64 sequences of 512 .. 4099 at 8 bits 76 / 78
+// / 76; 64 alike of 300 18.3 / 25.5 / 18.0; 8 of 16k .. 128k at 4 bits 162 / 178 / 161; 16 of 4k .. 30k 82 / 91 / 82; 64
+// alike of 4096 69 / 78 / 69; 300 of 300 .. 3000 168 / 154 / 154; 120 of 50 .. 20000 323 / 298 / 297.
 struct Chunk {
   int seq, chunk, chunks, tiles, sk;
   int64_t start;

@@ -18,10 +18,10 @@
 // digit over the whole row.
 // Double throughout: a row has so many borders between tokens that sums good to 2^-24 would move one row in a hundred
 // across one; here a logit's part of its bin is rounded to 2^-34, those of the bins that decide to 2^-45.
-// Measured, 151936 columns, both launches: 1 row 30 us, 4 rows 36, 8 rows of top_p 47, 64 rows 61 (their bytes once:
+// Measured, 151936 columns, both launches: 1 row 30 us, 4 rows 36, 8 rows of top_p 47, 64 rows 59 (their bytes once:
 // 0.1, 0.4, 0.8 and 6.3).  Bound by latency for few rows (7 us until the last part has arrived, 8 to merge 4 KB per part
 // and find the bins; then 6 to collect, and 3 to 11 for every end), and for many by the double arithmetic of the
-// second pass over a part (30 instructions a logit: 12 of 64 rows' 33 us; a copy of the logits in LDS or of the
+// second pass over a part (30 instructions a logit: 12 of 64 rows' 30 us; a copy of the logits in LDS or of the
 // bins for every fourth lane changed nothing).  Rows whose logits are all alike: 0.4 to 0.8 ms.
 #include <algorithm>
 
