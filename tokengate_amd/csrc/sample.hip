@@ -716,10 +716,10 @@ struct Place {
   uint32_t ties;
   uint64_t above;   // count or mass of the elements above key
 };
-// Masses as whole numbers, in units of 2^-mass_bits of the largest weight: as small as the row's mass, in the same units
-// at most row_mass, allows (2^18 roundings of 2^-62 of the whole).
+// Masses as whole numbers, `unit` the largest weight's: as large as the row's mass, at most row_mass of that weight,
+// allows (2^18 roundings of 2^-62 of the whole).
 __device__ void slow_row(const SampleArgs &a, int b, double row_mass) {
-  const int mass_bits = 61 - __builtin_amdgcn_frexp_exp(row_mass);
+  const double unit = ldexp(1.0, 61 - __builtin_amdgcn_frexp_exp(row_mass));
   const int tid = threadIdx.x;
   const float *x = a.x + b * a.rs;
   __shared__ uint64_t hist[256], red[16];
@@ -755,7 +755,7 @@ __device__ void slow_row(const SampleArgs &a, int b, double row_mass) {
   const bool greedy = !(temp > 0.f) || top == -INFINITY;
   const double scale = greedy ? 1.0 : kLog2e / temp;
   auto weight = [&](float x) { return x == top ? 1.0 : exp2_of(((double)x - (double)top) * scale); };   // (both may be infinite)
-  auto mass = [&](uint32_t key) { return (uint64_t)(ldexp(weight(order_float(key)), mass_bits) + 0.5); };
+  auto mass = [&](uint32_t key) { return (uint64_t)(weight(order_float(key)) * unit + 0.5); };
   // The first place at which the sum of value(key) over the elements up to it reaches target (> 0).
   auto find = [&](uint64_t target, bool by_mass) {
     uint32_t prefix = 0;
@@ -868,7 +868,7 @@ __device__ void slow_row(const SampleArgs &a, int b, double row_mass) {
     a.token[b] = i;
     const float v = order_float(p.key);
     const double d = v == top ? 0.0 : ((double)v - (double)top) / (double)temp;
-    if (a.logprob) a.logprob[b] = (float)(d - log(ldexp((double)total, -mass_bits)));
+    if (a.logprob) a.logprob[b] = (float)(d - log((double)total / unit));
   }
 }
 
