@@ -227,3 +227,17 @@ def test_long_vocabularies_and_batches(cuda, B, bits):
             if not border:
                 assert int(ce[b]) == tok and abs(float(eager.last_logprobs[b]) - lp) <= 2.0 ** -24 * abs(lp) + 2.0 ** -34
     assert near <= 1
+
+
+def test_generate_with_a_padded_vocabulary(cuda):
+    """A head of more rows than the configuration's vocabulary (padded ones): sampling is over the head's."""
+    import dataclasses
+    from tests.test_inference_gpu import SMALL
+    from tokengate_amd import decoder as dec
+    from tokengate_amd import inference as I
+    m = I.load_model("random:9", gate_layer=1, device=cuda, shape=dec.DecoderShape(**dict(SMALL, vocab=20480)))
+    prompts = _prompts([90, 120], [(5, 80), (10, 100)], 3)
+    want = m.generate(prompts, None, max_new_tokens=4, temperature=1.2, seed=2)
+    m.weights.shape = dataclasses.replace(m.config, vocab=2000)
+    got = m.generate(prompts, None, max_new_tokens=4, temperature=1.2, seed=2)
+    assert got.token_ids == want.token_ids and got.logprobs == want.logprobs

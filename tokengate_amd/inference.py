@@ -181,7 +181,7 @@ class TokenGateModel:
         first = pf.first_tokens
         sampler, lps = None, None
         if sampled:
-            sampler = TokenSampler(sampling, len(split), self.config.vocab, max_new_tokens, first.device)
+            sampler = TokenSampler(sampling, len(split), pf.logits.shape[1], max_new_tokens, first.device)
             sampler.set_step(0)
             first, lp = sampler(pf.logits.float())
             lps = [lp]
