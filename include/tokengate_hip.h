@@ -488,6 +488,73 @@ int tg_decode_attention_quant(const void *qkv, int64_t qkv_row_stride, const flo
                               float softmax_scale, void *out, int64_t out_row_stride, void *workspace,
                               int64_t workspace_bytes, hipStream_t stream);
 
+/* ---- a KV cache in pages ------------------------------------------------------------------------------------
+ * A layer's cache is num_pages pages of page_rows rows (a power of two, 16 .. 65536) of every KV head, bf16, head_dim 128:
+ * row r of head h in page p lies p * page_stride + h * head_stride + r * row_stride elements behind k_pages (v_pages), strides
+ * multiples of 8, pointers 16-byte aligned, no two rows overlapping; less than 2^31 rows.  Key j of sequence b is row
+ * j % page_rows of page page_table[b * table_stride + j / page_rows] (int32; table_cols columns).  An entry outside
+ * 0 .. num_pages - 1 names no page: its keys weigh nothing and nothing is written to them (columns past a sequence's
+ * keys are not used).  Sequences may share pages that none of them appends to.
+ *
+ * Start of a step for n_rows packed rows (row t of sequence b: cu_seqlens[b] <= t < cu_seqlens[b + 1], the last of kv_used[b]
+ * keys): slots[t] = page * page_rows + row of the row's key, or -1 where it has none (rows of no sequence, keys past the
+ * table's columns, entries that name no page); rope[t][64][2] = (cos, sin)(float(positions[t]) * inv_freq), as
+ * tg_decode_begin's. */
+int tg_paged_begin(const int64_t *positions, int64_t n_rows, const float *inv_freq, const int32_t *cu_seqlens,
+                   const int32_t *kv_used, int32_t num_seqs, const int32_t *page_table, int64_t table_stride,
+                   int32_t table_cols, int32_t num_pages, int32_t page_rows, int32_t *slots, float *rope,
+                   hipStream_t stream);
+
+/* tg_qk_norm_rope (same roundings and bits, with the rotation from a table rope[t][64][2] of (cos, sin)) into pages: q head h
+ * of row t to q_out + t * q_row_stride + h * q_head_stride (qkv's own q columns, or rows that do not overlap qkv), k and
+ * v heads to cache row slots[t] (int32, page * page_rows + row); rows with a slot outside the cache get their q only.  No two
+ * rows may name one slot. */
+int tg_paged_append(const void *qkv, int64_t qkv_row_stride, const float *rope, int64_t n_tokens, int32_t num_heads,
+                    int32_t num_heads_k, int32_t head_dim, const void *q_norm_weight, const void *k_norm_weight, float eps,
+                    const float *q_head_scale, const float *q_row_scale, void *q_out, int64_t q_row_stride,
+                    int64_t q_head_stride, const int32_t *slots, void *k_pages, int64_t k_page_stride,
+                    int64_t k_head_stride, int64_t k_row_stride, void *v_pages, int64_t v_page_stride,
+                    int64_t v_head_stride, int64_t v_row_stride, int32_t num_pages, int32_t page_rows, hipStream_t stream);
+
+/* Causal attention of every packed query segment over its sequence's pages: query i of n_q = cu_seqlens_q[b + 1] -
+ * cu_seqlens_q[b] (at most max_seqlen_q) sees keys j <= i + n_k - n_q of n_k = min(kv_used[b], max_seqlen_k), logits softmax_scale *
+ * (q . k_j + bias_raw[b, h, j]).  Rows that see no key get zeros; rows of no sequence keep what out holds.  A bias of -inf hides a
+ * key from the head whatever its row holds, as does an entry that names no page; the rows of keys that a query
+ * only comes before have to be finite.  Weights in bf16, fp32 sums; workspace: tg_paged_attention_workspace_size bytes
+ * for the key-range split of small launches (NULL or fewer bytes: no split), contents need no initialisation, shared by
+ * stream-ordered calls.  max_seqlen_k < 2^24 and at most table_cols * page_rows. */
+int64_t tg_paged_attention_workspace_size(int32_t num_seqs, int32_t max_seqlen_q, int32_t max_seqlen_k, int32_t num_heads,
+                                          int32_t num_heads_k);
+int tg_paged_attention(const void *q, int64_t q_row_stride, int64_t q_head_stride, const void *k_pages,
+                       int64_t k_page_stride, int64_t k_head_stride, int64_t k_row_stride, const void *v_pages,
+                       int64_t v_page_stride, int64_t v_head_stride, int64_t v_row_stride, int32_t num_pages,
+                       int32_t page_rows, const int32_t *page_table, int64_t table_stride, int32_t table_cols,
+                       const int32_t *cu_seqlens_q, const int32_t *kv_used, int32_t num_seqs, int32_t max_seqlen_q,
+                       int32_t max_seqlen_k, int32_t total_q, int32_t num_heads, int32_t num_heads_k, int32_t head_dim,
+                       const float *bias_raw, int64_t bias_seq_stride, int64_t bias_head_stride, float softmax_scale,
+                       void *out, int64_t out_row_stride, int64_t out_head_stride, void *workspace,
+                       int64_t workspace_bytes, hipStream_t stream);
+
+/* tg_decode_attention over pages, in one launch: q / k norm, rotary embedding and query scale as there; the new k / v rows
+ * written to key kv_used[b] - 1 of sequence b; then every head over keys 0 .. kv_used[b] - 1.  Weights of 16 bits, fp32
+ * sums.  A bias of -inf hides a key whatever its row holds, as does an entry that names no page; a head that sees no key gets
+ * zeros.  kv_used[b] <= 0 appends nothing and gets zeros; kv_used[b] > max_seqlen_k: the first max_seqlen_k keys, of which the
+ * last is the new one.  No sequence may append a row that another one reads or appends.  workspace:
+ * tg_paged_decode_attention_workspace_size bytes (0: NULL will do), 16-byte aligned, zeroed once when it is allocated,
+ * shared by the launches of one stream, of any sizes that it holds; launches that may overlap, from two streams or two
+ * replayed graphs, need one each.  max_seqlen_k < 2^24 and at most table_cols * page_rows. */
+int64_t tg_paged_decode_attention_workspace_size(int32_t num_seqs, int32_t num_heads, int32_t num_heads_k,
+                                                 int32_t max_seqlen_k);
+int tg_paged_decode_attention(const void *qkv, int64_t qkv_row_stride, const float *rope, int32_t num_seqs,
+                              int32_t num_heads, int32_t num_heads_k, int32_t head_dim, const void *q_norm_weight,
+                              const void *k_norm_weight, float eps, const float *q_head_scale, const float *q_row_scale,
+                              void *k_pages, int64_t k_page_stride, int64_t k_head_stride, int64_t k_row_stride,
+                              void *v_pages, int64_t v_page_stride, int64_t v_head_stride, int64_t v_row_stride,
+                              int32_t num_pages, int32_t page_rows, const int32_t *page_table, int64_t table_stride,
+                              int32_t table_cols, const int32_t *kv_used, int32_t max_seqlen_k, const float *bias_raw,
+                              int64_t bias_seq_stride, int64_t bias_head_stride, float softmax_scale, void *out,
+                              int64_t out_row_stride, void *workspace, int64_t workspace_bytes, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

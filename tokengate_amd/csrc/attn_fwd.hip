@@ -45,6 +45,7 @@
 #include <mutex>
 #include <type_traits>
 
+#include "paged.h"
 #include "tg_common.h"
 #include "../../include/tokengate_hip.h"
 
@@ -111,6 +112,13 @@ struct DecArgs {
   uint64_t *po;                // [unit][chunk][head][16 pieces of 8 bf16]: O / l, 32 words
 };
 struct NoDec {};
+// Keys in pages: key j of sequence b is row j % page of page table[b][j / page] (PagePool), FwdArgs' k, v and their row
+// and head strides those of a page's rows.
+struct PagedArgs {
+  const int32_t *table;
+  int64_t table_rs, k_ps, v_ps;
+  int cols, lg, n_pages;
+};
 template <typename T>
 __device__ __forceinline__ void st_agent(T *p, T v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 template <typename T>
@@ -169,7 +177,8 @@ struct Fold {
   float mmax = -INFINITY, wsum = 0.f;
   float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 };
-__device__ __forceinline__ void fold_chunk(Fold &f, float2 mc, u32x4 pv) {
+template <typename Value>   // value(e): the e-th of the chunk's eight
+__device__ __forceinline__ void fold_values(Fold &f, float2 mc, Value value) {
   if (!(mc.y > 0.f)) return;
   if (mc.x > f.mmax) {
     const float sc = fast_exp2(f.mmax - mc.x);   // 0 while nothing has been added yet
@@ -181,10 +190,10 @@ __device__ __forceinline__ void fold_chunk(Fold &f, float2 mc, u32x4 pv) {
   const float w = mc.y * fast_exp2(mc.x - f.mmax);
   f.wsum += w;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    f.acc[2 * e] += w * __builtin_bit_cast(float, pv[e] << 16);
-    f.acc[2 * e + 1] += w * __builtin_bit_cast(float, pv[e] & 0xffff0000u);
-  }
+  for (int e = 0; e < 8; ++e) f.acc[e] += w * value(e);
+}
+__device__ __forceinline__ void fold_chunk(Fold &f, float2 mc, u32x4 pv) {
+  fold_values(f, mc, [&](int e) { return u32_as_f32(e & 1 ? pv[e >> 1] & 0xffff0000u : pv[e >> 1] << 16); });
 }
 // p: another group's (mmax, wsum, acc), `stride` floats apart
 __device__ __forceinline__ void merge_fold(Fold &f, const float *p, int stride) {
@@ -210,10 +219,13 @@ __host__ __device__ __forceinline__ int combine_groups(int ns) {
   return n;
 }
 
-template <int NW, int KS, int HP, bool CAUSAL, bool HAS_BIAS, bool VARLEN, bool DEC = false>
-__global__ __launch_bounds__(64 * NW, 8 / NW) void keybias_fwd_kernel(FwdArgs a,
-                                                                      std::conditional_t<DEC, DecArgs, NoDec> dec) {
+template <bool DEC, bool PAGED>
+using MoreArgs = std::conditional_t<DEC, DecArgs, std::conditional_t<PAGED, PagedArgs, NoDec>>;
+
+template <int NW, int KS, int HP, bool CAUSAL, bool HAS_BIAS, bool VARLEN, bool DEC = false, bool PAGED = false>
+__global__ __launch_bounds__(64 * NW, 8 / NW) void keybias_fwd_kernel(FwdArgs a, MoreArgs<DEC, PAGED> dec) {
   static_assert(!DEC || (VARLEN && NW == 4 && KS == 1), "the decode step's form");
+  static_assert(!PAGED || (VARLEN && CAUSAL && KS == 1 && !DEC), "the paged form");
   constexpr int kWaves = NW;
   constexpr int CW = col_waves<NW, KS>();
   constexpr int BM = bm<CW, HP>();
@@ -292,7 +304,9 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void keybias_fwd_kernel(FwdArgs a,
   } else if constexpr (VARLEN) {
     row0 = seq_row0;
     sq = seq_len;
-    if (a.cu_k != nullptr) {
+    if constexpr (PAGED) {
+      sk = max(0, min(a.used_k[b], a.sk));
+    } else if (a.cu_k != nullptr) {
       krow0 = a.cu_k[b];
       const int nk = a.used_k != nullptr ? a.used_k[b] : a.cu_k[b + 1] - a.cu_k[b];
       sk = max(0, min(nk, a.sk));
@@ -401,7 +415,43 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void keybias_fwd_kernel(FwdArgs a,
     const int vc = (lane & 15) ^ vswz(vkey);
     voff[it] = (uint32_t)(vkey * a.v_rs * 2 + vc * 16);
   }
+  // Pages: the entries of the next tile to be issued, its 16-key quarters in lanes 0 .. 3 (loaded while the tile before it
+  // is computed), and which quarters of the issued tile have no page.
+  [[maybe_unused]] int32_t entry = 0;
+  [[maybe_unused]] uint32_t no_page = 0;
+  [[maybe_unused]] auto load_entries = [&](int tile) {
+    if constexpr (PAGED)
+      entry = dec.table[b * dec.table_rs + min((tile * SK + 16 * (lane & 3)) >> dec.lg, dec.cols - 1)];
+  };
+  [[maybe_unused]] auto issue_paged = [&](int tile, auto buf_c) {
+    if constexpr (PAGED) {
+      char *kd = kslot(buf_c), *vd = vslot(buf_c);
+      const int wv = __builtin_amdgcn_readfirstlane(wave), mask = (1 << dec.lg) - 1;
+      // a load brings four keys, of one page, through a descriptor of exactly those that are there
+      auto rows_of = [&](const bf16_t *base, int64_t ps, int64_t rs, int key) {
+        const int32_t page = __builtin_amdgcn_readlane(entry, (key >> 4) & 3);
+        const bool there = (uint32_t)page < (uint32_t)dec.n_pages;
+        const int n = there ? max(0, min(4, sk - key)) : 0;
+        const bf16_t *p = base + (there ? page : 0) * ps + (int64_t)(key & mask) * rs;
+        return make_rsrc(p, n > 0 ? (uint32_t)((n - 1) * (int)rs + kD) * 2u : 0u);
+      };
+      const bf16_t *kh_base = a.k + (int64_t)kh * a.k_hs, *vh_base = a.v + (int64_t)kh * a.v_hs;
+#pragma unroll
+      for (int it = 0; it < kLoads; ++it) {
+        const int slot = wv + it * kWaves, lr = 4 * slot + (lane >> 4);
+        dma16(rows_of(kh_base, dec.k_ps, a.k_rs, tile * SK + kperm(4 * slot)), kd + slot * 1024,
+              (uint32_t)((lane >> 4) * (int)a.k_rs * 2 + ((lane & 15) ^ (lr & 15)) * 16));
+        dma16(rows_of(vh_base, dec.v_ps, a.v_rs, tile * SK + 4 * slot), vd + slot * 1024,
+              (uint32_t)((lane >> 4) * (int)a.v_rs * 2 + ((lane & 15) ^ vswz(lr)) * 16));
+      }
+      no_page = (uint32_t)__builtin_amdgcn_ballot_w64((uint32_t)entry >= (uint32_t)dec.n_pages) & 15u;
+      load_entries(tile + 1);
+    }
+  };
   auto issue_tile = [&](int tile, auto buf_c) {
+    if constexpr (PAGED) {
+      issue_paged(tile, buf_c);
+    } else {
     const uint32_t kb0 = (uint32_t)((int64_t)tile * SK * a.k_rs * 2);
     const uint32_t vb0 = (uint32_t)((int64_t)tile * SK * a.v_rs * 2);
     char *kd = kslot(buf_c), *vd = vslot(buf_c);
@@ -412,6 +462,7 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void keybias_fwd_kernel(FwdArgs a,
     for (int it = 0; it < kLoads; ++it) {
       dma16(krs, kd + (wv + it * kWaves) * 1024, kb0 + koff[it]);
       dma16(vrs, vd + (wv + it * kWaves) * 1024, vb0 + voff[it]);
+    }
     }
     if constexpr (HAS_BIAS) {
       if (wave < HP * BP)
@@ -467,6 +518,7 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void keybias_fwd_kernel(FwdArgs a,
         ring_barrier();
       }
     }
+    [[maybe_unused]] const uint32_t gone = no_page;   // of this tile
     if (t + 1 < t_hi) issue_tile(t + 1, std::integral_constant<int, 1 - BUF>());
     if (!wave_has_rows || (CAUSAL && n0 > qw_hi + off)) return;
 
@@ -505,6 +557,41 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void keybias_fwd_kernel(FwdArgs a,
       }
     }
 
+    // Pages: keys that a bias of -inf hides or that have no page weigh nothing whatever their rows hold, and where a bias is
+    // as large as a mask's (2^30 and more) the weights' exponents are formed without contraction, whose rest would be
+    // a large number there.  One test per tile of the lane's 16 biases.
+    [[maybe_unused]] bool far = false;
+    [[maybe_unused]] uint32_t hidden = 0;   // by bit 4 kb + i
+    if constexpr (PAGED) {
+      if constexpr (HAS_BIAS) {
+        const float *bp = &bslot(buf_c)[hw][8 * G];
+        f32x4 bv[KB];
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) bv[kb] = *reinterpret_cast<const f32x4 *>(bp + 32 * (kb >> 1) + 4 * (kb & 1));
+        float big = 0.f;
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) big = fmaxf(big, fabsf(bv[kb][i]));
+        far = __builtin_amdgcn_ballot_w64(!(big < 0x1p30f)) != 0;
+        if (far) {
+#pragma unroll
+          for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) hidden |= bv[kb][i] == -INFINITY ? 1u << (4 * kb + i) : 0u;
+        }
+      }
+      if (gone) hidden |= ((gone >> (G >> 1)) & 1 ? 0xffu : 0u) | ((gone >> (2 + (G >> 1))) & 1 ? 0xff00u : 0u);
+      if (__builtin_amdgcn_ballot_w64(hidden != 0)) {
+#pragma unroll
+        for (int cb = 0; cb < 2; ++cb)
+#pragma unroll
+          for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sacc[cb][kb][i] = (hidden >> (4 * kb + i)) & 1 ? -INFINITY : sacc[cb][kb][i];
+      }
+    }
+
     // ---- online softmax: lane holds KN/4 keys of one column per block; the other keys of that
     // column sit in lanes l^16, l^32, l^48 ----
     const bool need_mask = (n0 + KN > sk) || (CAUSAL && n0 + KN - 1 > qw0 + off);
@@ -523,8 +610,13 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void keybias_fwd_kernel(FwdArgs a,
           for (int i = 0; i < 4; ++i) {
             int sgn;
             asm("v_ashrrev_i32 %0, 31, %1" : "=v"(sgn) : "v"(rel - i));   // -1 where key > lim
-            const float pen = __builtin_bit_cast(float, (uint32_t)sgn & 0xFF800000u);
-            sacc[cb][kb][i] += pen;
+            if constexpr (PAGED) {   // (replaced, not added to: the row behind the mask may hold anything)
+              const uint32_t s = __builtin_bit_cast(uint32_t, (float)sacc[cb][kb][i]);
+              sacc[cb][kb][i] = u32_as_f32(((uint32_t)sgn & 0xFF800000u) | (~(uint32_t)sgn & s));
+            } else {
+              const float pen = __builtin_bit_cast(float, (uint32_t)sgn & 0xFF800000u);
+              sacc[cb][kb][i] += pen;
+            }
           }
         }
       }
@@ -586,6 +678,20 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void keybias_fwd_kernel(FwdArgs a,
         }
       }
     }
+    if constexpr (PAGED && HAS_BIAS) {
+      if (far) {
+#pragma unroll
+        for (int cb = 0; cb < 2; ++cb)
+#pragma unroll
+          for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int i = 0; i < 4; i += 2) {
+              float z0 = sacc[cb][kb][i] * a.scale_log2, z1 = sacc[cb][kb][i + 1] * a.scale_log2;
+              asm("" : "+v"(z0), "+v"(z1));   // rounded, as the running maximum is
+              pk[cb][kb][i >> 1] = pack_bf16x2(fast_exp2(z0 + mneg[cb]), fast_exp2(z1 + mneg[cb]));
+            }
+      }
+    }
 
     // ---- O^T += V^T P^T: ST key steps x 8 d-blocks x 2 column blocks ----
 #pragma unroll
@@ -604,12 +710,24 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void keybias_fwd_kernel(FwdArgs a,
         const char *vbuf = vslot(buf_c) + KN * kg * kKRowBytes;
         const s16x4 lo = lds_read_tr16(vbuf + krow + vch[dblk]);
         const s16x4 hi = lds_read_tr16(vbuf + krow + 4 * kKRowBytes + vch[dblk]);
-        const bf16x8 vf = __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+        bf16x8 vf = __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+        if constexpr (PAGED && HAS_BIAS) {
+          if (far) {   // rows that the bias hides from this wave's head: 0
+            u32x4 w = __builtin_bit_cast(u32x4, vf);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const uint32_t two = hidden >> (8 * st + 2 * j);
+              w[j] &= (two & 1 ? 0u : 0xffffu) | (two & 2 ? 0u : 0xffff0000u);
+            }
+            vf = __builtin_bit_cast(bf16x8, w);
+          }
+        }
 #pragma unroll
         for (int cb = 0; cb < 2; ++cb) oacc[cb][dblk] = mfma16(vf, pb[cb], oacc[cb][dblk]);
       }
     }
   };
+  if constexpr (PAGED) load_entries(t_lo);
   if (t_lo < t_hi) issue_tile(t_lo, std::integral_constant<int, 0>());
   if constexpr (DEC) {
     if (wave_has_rows || is_k) {
@@ -772,13 +890,18 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void keybias_fwd_kernel(FwdArgs a,
     // column block cb; each piece a coalesced 1 KB wave store) and, per column block, (running max
     // in log2 units, row sum l)
     const int64_t pw = (hunit * a.ns + chunk) * CW + cw;
-    u32x4 *po = reinterpret_cast<u32x4 *>(a.ws_o) + pw * (8 * 64) + lane;
+    u32x4 *po = reinterpret_cast<u32x4 *>(a.ws_o) + pw * (8 * 64 * (PAGED ? 2 : 1)) + lane;
 #pragma unroll
     for (int cb = 0; cb < 2; ++cb)
 #pragma unroll
       for (int p = 0; p < DB / 2; ++p) {
         const f32x4 &o0 = oacc[cb][2 * p], &o1 = oacc[cb][2 * p + 1];
         const float s = inv[cb];
+        if constexpr (PAGED) {   // in fp32, the second half of a piece 64 lanes on
+          po[(8 * cb + 2 * p) * 64] = __builtin_bit_cast(u32x4, o0 * s);
+          po[(8 * cb + 2 * p + 1) * 64] = __builtin_bit_cast(u32x4, o1 * s);
+          continue;
+        }
         const u32x4 w = {pack_bf16x2(o0[0] * s, o0[1] * s), pack_bf16x2(o0[2] * s, o0[3] * s),
                          pack_bf16x2(o1[0] * s, o1[1] * s), pack_bf16x2(o1[2] * s, o1[3] * s)};
         po[(4 * cb + db0 / 2 + p) * 64] = w;
@@ -807,7 +930,7 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void keybias_fwd_kernel(FwdArgs a,
       const u32x2 w = {pack_bf16x2(o[0] * s, o[1] * s), pack_bf16x2(o[2] * s, o[3] * s)};
       *reinterpret_cast<u32x2 *>(orow + 16 * (db0 + d) + 4 * G) = w;
     }
-    if (!DEC && G == 0 && kg == 0) {
+    if (!DEC && !PAGED && G == 0 && kg == 0) {
       const float lse = l[cb] > 0.f ? (mrun[cb] + __log2f(l[cb])) * kLn2 : INFINITY;
       const int hh = h0 + hl;
       if constexpr (VARLEN)
@@ -823,7 +946,7 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void keybias_fwd_kernel(FwdArgs a,
 // tile; per piece, thread (group cg, lane) folds chunks cg, cg + CG, ... of its column and group 0
 // merges the CG partial results through LDS, so that a long chunk list (a decode row over a long
 // cache) is walked CG ways in parallel.
-template <int CW, int HP, bool VARLEN>
+template <int CW, int HP, bool VARLEN, bool PAGED = false>   // PAGED: partial results in fp32, no LSE
 __global__ __launch_bounds__(512) void keybias_fwd_combine_kernel(FwdArgs a, int CG) {
   constexpr int BM = bm<CW, HP>();
   // (m, wsum, acc[8]) of groups 1..CG-1 of each piece: PP * (CG - 1) < 8 slots
@@ -866,8 +989,14 @@ __global__ __launch_bounds__(512) void keybias_fwd_combine_kernel(FwdArgs a, int
     for (int c = cg; c < a.ns; c += CG) {
       const int64_t pw = pw0 + (int64_t)c * CW;
       const float2 mc = ml[pw * 128 + cb * 64 + lane];
-      const u32x4 pv = po[pw * (8 * 64) + j * 64 + lane];
-      fold_chunk(f, mc, pv);
+      if constexpr (PAGED) {
+        const f32x4 *pf = reinterpret_cast<const f32x4 *>(po) + pw * (16 * 64) + 2 * j * 64 + lane;
+        const f32x4 v0 = pf[0], v1 = pf[64];
+        fold_values(f, mc, [&](int e) { return e < 4 ? v0[e & 3] : v1[e & 3]; });
+      } else {
+        const u32x4 pv = po[pw * (8 * 64) + j * 64 + lane];
+        fold_chunk(f, mc, pv);
+      }
     }
   }
   if (cg > 0) store_fold(f, &mypart[cg - 1][0][lane], 64);
@@ -886,7 +1015,7 @@ __global__ __launch_bounds__(512) void keybias_fwd_combine_kernel(FwdArgs a, int
   const u32x2 w1 = {pack_bf16x2(acc[4] * inv, acc[5] * inv), pack_bf16x2(acc[6] * inv, acc[7] * inv)};
   *reinterpret_cast<u32x2 *>(orow + d0) = w0;
   *reinterpret_cast<u32x2 *>(orow + d0 + 16) = w1;
-  if (p == 0 && G == 0) {
+  if (!PAGED && p == 0 && G == 0) {
     const float lse = wsum > 0.f ? (mmax + __log2f(wsum)) * kLn2 : INFINITY;
     const int hh = h0 + hl;
     if constexpr (VARLEN)
@@ -934,6 +1063,17 @@ void dispatch_fwd(const FwdArgs &a, int nw, int ks, int hp, bool causal, bool ha
 #undef TG_FWD_CASE
 }
 
+template <int NW, int HP, bool HAS_BIAS>
+void launch_paged(const FwdArgs &a, const PagedArgs &pages, int nblocks, hipStream_t stream) {
+  hipLaunchKernelGGL((keybias_fwd_kernel<NW, 1, HP, true, HAS_BIAS, true, false, true>), dim3(nblocks), dim3(64 * NW), 0,
+                     stream, a, pages);
+  if (a.heavy_blocks > 0) {
+    const int cgroups = combine_groups(a.ns);
+    hipLaunchKernelGGL((keybias_fwd_combine_kernel<NW, HP, true, true>), dim3((unsigned)(a.heavy_blocks / a.ns * NW * cgroups)),
+                       dim3(512), 0, stream, a, cgroups);
+  }
+}
+
 // The four forms of the kernel: waves per workgroup and key groups.  A CU holds one workgroup of eight
 // waves or two of four.
 struct Form {
@@ -960,13 +1100,15 @@ struct Tiles {
 // longest tiles while the chip idles: the tiles whose key range exceeds 1/ns of the longest are split
 // into ns chunks of consecutive key steps (ns from the free slots), merged by the combine kernel.
 // Returns ns = 1 when nothing is split.
+// A lane's part of a chunk's result: 64 values of O / l, bf16 (over pages fp32), then (m, l) per column block.
 struct SplitPlan {
   int ns = 1, n_heavy = 0;
   int64_t heavy_units = 0, bytes = 0;
+  int o_bytes = 128;
 };
-constexpr int64_t kPartialBytesPerLane = 8 * 16 + 2 * 8;   // O / l as 64 bf16, then (m, l) per column block
-SplitPlan plan_split(const Form &f, const Tiles &t, int64_t units) {
+SplitPlan plan_split(const Form &f, const Tiles &t, int64_t units, int o_bytes = 128) {
   SplitPlan p;
+  p.o_bytes = o_bytes;
   const int64_t slots = (int64_t)device_cus() * (8 / f.nw);
   const int64_t nblocks = (int64_t)t.n_qtiles * units;
   if (nblocks <= 0 || 4 * nblocks > 3 * slots || t.sk <= 0) return p;
@@ -982,13 +1124,13 @@ SplitPlan plan_split(const Form &f, const Tiles &t, int64_t units) {
   // that, extra chunks only queue behind the others.  ns <= slots / nblocks already ensures it
   // unless ns was raised to 2 for a grid of more than half the slots; then only the heaviest tiles
   // that fit are split.  Hence heavy_units * ns <= slots, and the partials take at most
-  // CUs x 8 waves x 64 lanes x kPartialBytesPerLane bytes.
+  // CUs x 8 waves x 64 lanes x (o_bytes + 16) bytes.
   n_heavy = (int)std::min<int64_t>(n_heavy, (slots - nblocks) / ((int64_t)(ns - 1) * units));
   if (n_heavy <= 0) return p;
   p.ns = ns;
   p.n_heavy = n_heavy;
   p.heavy_units = (int64_t)n_heavy * units;
-  p.bytes = p.heavy_units * ns * (f.nw / f.ks) * 64 * kPartialBytesPerLane;
+  p.bytes = p.heavy_units * ns * (f.nw / f.ks) * 64 * (o_bytes + 2 * 8);
   return p;
 }
 
@@ -1090,13 +1232,13 @@ FwdPlan plan_dense_in(int hp, int sq, int sk, int64_t units, bool causal, int64_
 // here, and key groups would change the order in which a column's keys are summed: of a whole gated
 // prefill at 2320 kept rows they took 0.5 % off the time and moved the logits by 2.6 %, the noise
 // of 26 bf16 layers rounded otherwise, so packed launches keep one key group.
-FwdPlan plan_varlen(int hp, int max_sq, int max_sk, int64_t units, bool causal, int64_t workspace_bytes) {
+FwdPlan plan_varlen(int hp, int max_sq, int max_sk, int64_t units, bool causal, int64_t workspace_bytes, int o_bytes = 128) {
   FwdPlan plan;
   const Tiles wide(kForms[0], hp, max_sq, max_sk, causal), narrow(kForms[1], hp, max_sq, max_sk, causal);
   const bool w = wide.n_qtiles * units >= 2 * (int64_t)device_cus();
   plan.nw = w ? 8 : 4;
   plan.n_qtiles = w ? wide.n_qtiles : narrow.n_qtiles;
-  plan.split = plan_split(kForms[w ? 0 : 1], w ? wide : narrow, units);
+  plan.split = plan_split(kForms[w ? 0 : 1], w ? wide : narrow, units, o_bytes);
   if (plan.split.bytes > workspace_bytes) plan.split = SplitPlan{};
   return plan;
 }
@@ -1110,7 +1252,7 @@ int64_t apply_plan(FwdArgs &a, const FwdPlan &f, int64_t units, void *workspace)
   a.heavy_blocks = p.heavy_units * p.ns;
   a.ws_o = static_cast<bf16_t *>(workspace);
   a.ws_ml = workspace ? reinterpret_cast<float *>(static_cast<char *>(workspace) +
-                                                  p.heavy_units * p.ns * (f.nw / f.ks) * 64 * 128)
+                                                  p.heavy_units * p.ns * (f.nw / f.ks) * 64 * p.o_bytes)
                       : nullptr;
   return a.heavy_blocks + (int64_t)(a.n_qtiles - a.n_heavy) * units;
 }
@@ -1280,6 +1422,28 @@ extern "C" int tg_keybias_fwd_noalloc(const void *q, const void *k, const void *
 
 namespace tg {
 namespace {
+// Workgroups of a varlen launch, its plan and the order of its tiles put into the arguments.
+//
+// Sequence-major where level order has nothing to give.  Where every tile has a CU of its own the order decides
+// nothing (16 sequences of 21 to 80 tokens: 8.7 us, in level order 10.1); it does where two four-wave workgroups
+// share one (level / sequence-major, us: 20 of up to 200, 16 / 8 heads, 13.8 / 17.3, 23 of up to 370, 8 / 8, 15.7 /
+// 16.9, 60 of up to 90, 8 / 2, 9.8 / 12.1; 8 of up to 150, 32 / 8, 9.3 / 8.5).  Sequences of one length finish
+// evenly by themselves; with up to three tiles each, level order then parts the few workgroups that share a
+// sequence's keys and mends no tail (level / sequence-major, 14 shapes of 8 to 32 heads: 22 x 360 tokens 1.17,
+// 54 x 378 1.13, 18 x 367 1.10, in the mean 1.05), with more there are long tiles to put first (64 x 500 with 16
+// heads 0.88, 8 x 2048 0.86, 30 x 1000 0.92; 52 x 609 1.08; in the mean of 19 0.99).
+int64_t varlen_grid(FwdArgs &a, const FwdPlan &plan, int64_t units, void *workspace, bool causal, int64_t total_q,
+                    int64_t key_rows) {
+  const int64_t nblocks = apply_plan(a, plan, units, workspace);
+  const int hp = a.group % 2 == 0 ? 2 : 1;
+  const int64_t level_blocks = level_tiles(a.batch, total_q, plan.nw * 32 / hp) * (a.h / hp);
+  const bool own_cu = level_blocks <= device_cus();
+  const bool few_even_tiles = a.n_qtiles < 4 && total_q == (int64_t)a.batch * a.sq;
+  a.level_order = a.n_heavy == 0 && a.n_qtiles > 1 && !own_cu && !few_even_tiles &&
+                  varlen_level_order(causal, a.batch, key_rows, a.hkv);
+  return a.level_order ? level_blocks : nblocks;
+}
+
 // The varlen forward behind tg_keybias_varlen_fwd (keys = the query rows) and
 // tg_keybias_varlen_kv_fwd (keys at cu_k / used_k).
 int keybias_fwd_varlen(const void *q, const void *k, const void *v, const float *bias_raw, void *out, float *lse,
@@ -1327,22 +1491,8 @@ int keybias_fwd_varlen(const void *q, const void *k, const void *v, const float 
   const int64_t units = (int64_t)num_seqs * (num_heads / hp);
   TG_CHECK(workspace == nullptr || aligned16(workspace), "workspace must be 16-byte aligned");
   const FwdPlan plan = plan_varlen(hp, max_seqlen_q, max_seqlen_k, units, causal != 0, workspace ? workspace_bytes : 0);
-  int64_t nblocks = apply_plan(a, plan, units, workspace);
-  // Sequence-major where level order has nothing to give.  Where every tile has a CU of its own the order decides
-  // nothing (16 sequences of 21 to 80 tokens: 8.7 us, in level order 10.1); it does where two four-wave workgroups
-  // share one (level / sequence-major, us: 20 of up to 200, 16 / 8 heads, 13.8 / 17.3, 23 of up to 370, 8 / 8, 15.7 /
-  // 16.9, 60 of up to 90, 8 / 2, 9.8 / 12.1; 8 of up to 150, 32 / 8, 9.3 / 8.5).  Sequences of one length finish
-  // evenly by themselves; with up to three tiles each, level order then parts the few workgroups that share a
-  // sequence's keys and mends no tail (level / sequence-major, 14 shapes of 8 to 32 heads: 22 x 360 tokens 1.17,
-  // 54 x 378 1.13, 18 x 367 1.10, in the mean 1.05), with more there are long tiles to put first (64 x 500 with 16
-  // heads 0.88, 8 x 2048 0.86, 30 x 1000 0.92; 52 x 609 1.08; in the mean of 19 0.99).
-  const int64_t level_blocks = level_tiles(num_seqs, total_q, plan.nw * 32 / hp) * (num_heads / hp);
-  const bool own_cu = level_blocks <= device_cus();
-  const bool few_even_tiles = a.n_qtiles < 4 && total_q == (int64_t)num_seqs * max_seqlen_q;
-  a.level_order = a.n_heavy == 0 && a.n_qtiles > 1 && !own_cu && !few_even_tiles &&
-                  varlen_level_order(causal != 0, num_seqs, cu_k != nullptr ? (int64_t)num_seqs * max_seqlen_k : total_q,
-                                     num_heads_k);
-  if (a.level_order) nblocks = level_blocks;
+  const int64_t nblocks = varlen_grid(a, plan, units, workspace, causal != 0, total_q,
+                                      cu_k != nullptr ? (int64_t)num_seqs * max_seqlen_k : total_q);
   TG_CHECK(nblocks < (1ll << 31), "grid too large");
   dispatch_fwd<true>(a, plan.nw, plan.ks, hp, causal != 0, bias_raw != nullptr, (int)nblocks, stream);
   TG_HIP_CHECK(hipPeekAtLastError());
@@ -1528,5 +1678,81 @@ extern "C" int tg_decode_attention(const void *qkv, int64_t qkv_row_stride, cons
   else
     hipLaunchKernelGGL((keybias_fwd_kernel<4, 1, 1, true, false, true, true>), grid, block, 0, stream, a, d);
   TG_HIP_CHECK(hipGetLastError());
+  return 0;
+}
+
+extern "C" int64_t tg_paged_attention_workspace_size(int32_t num_seqs, int32_t max_seqlen_q, int32_t max_seqlen_k,
+                                                     int32_t num_heads, int32_t num_heads_k) {
+  if (num_seqs <= 0 || max_seqlen_q <= 0 || max_seqlen_k <= 0 || num_heads <= 0 || num_heads_k <= 0 || num_heads % num_heads_k != 0)
+    return 0;
+  const int hp = (num_heads / num_heads_k) % 2 == 0 ? 2 : 1;
+  return plan_varlen(hp, max_seqlen_q, max_seqlen_k, (int64_t)num_seqs * (num_heads / hp), true, INT64_MAX, 256).split.bytes;
+}
+
+extern "C" int tg_paged_attention(const void *q, int64_t q_row_stride, int64_t q_head_stride, const void *k_pages,
+                                  int64_t k_page_stride, int64_t k_head_stride, int64_t k_row_stride, const void *v_pages,
+                                  int64_t v_page_stride, int64_t v_head_stride, int64_t v_row_stride, int32_t num_pages,
+                                  int32_t page_rows, const int32_t *page_table, int64_t table_stride, int32_t table_cols,
+                                  const int32_t *cu_seqlens_q, const int32_t *kv_used, int32_t num_seqs,
+                                  int32_t max_seqlen_q, int32_t max_seqlen_k, int32_t total_q, int32_t num_heads,
+                                  int32_t num_heads_k, int32_t head_dim, const float *bias_raw, int64_t bias_seq_stride,
+                                  int64_t bias_head_stride, float softmax_scale, void *out, int64_t out_row_stride,
+                                  int64_t out_head_stride, void *workspace, int64_t workspace_bytes, hipStream_t stream) {
+  clear_error();
+  const char *what = "paged_attention";
+  PagePool c;
+  if (int e = check_pool(what, k_pages, v_pages, {k_page_stride, k_head_stride, k_row_stride},
+                         {v_page_stride, v_head_stride, v_row_stride}, num_pages, page_rows, num_heads_k, head_dim, &c))
+    return e;
+  if (int e = check_table(what, page_table, table_stride, table_cols, num_seqs)) return e;
+  TG_CHECK(q && out && cu_seqlens_q && kv_used, "%s: null pointer", what);
+  TG_CHECK(aligned16(q) && aligned16(out) && aligned16(workspace), "%s: pointers must be 16-byte aligned", what);
+  TG_CHECK(num_heads > 0 && num_heads <= 256 && num_heads % num_heads_k == 0,
+           "%s: heads must be in 1..256 and a multiple of the KV heads", what);
+  TG_CHECK(num_seqs >= 0 && max_seqlen_q >= 0 && total_q >= 0, "%s: negative size", what);
+  TG_CHECK(max_seqlen_k >= 0 && max_seqlen_k < (1 << 24), "%s: max_seqlen_k must be in 0..2^24 - 1", what);
+  TG_CHECK(max_seqlen_k <= (int64_t)table_cols * page_rows, "%s: max_seqlen_k is more than the page table's columns hold", what);
+  TG_CHECK(strides_ok({q_row_stride, q_head_stride, out_row_stride, out_head_stride}),
+           "%s: q and out strides must be multiples of 8 elements", what);
+  TG_CHECK(softmax_scale > 0.f, "%s: softmax_scale must be positive", what);
+  TG_CHECK(!bias_raw || (bias_seq_stride >= 0 && bias_head_stride >= 0), "%s: negative bias stride", what);
+  if (num_seqs == 0 || max_seqlen_q == 0 || total_q == 0) return 0;
+  FwdArgs a{};
+  a.q = static_cast<const bf16_t *>(q);
+  a.k = c.k;
+  a.v = c.v;
+  a.bias = bias_raw;
+  a.o = static_cast<bf16_t *>(out);
+  a.cu_seqlens = cu_seqlens_q;
+  a.used_k = kv_used;
+  a.q_rs = q_row_stride; a.q_hs = q_head_stride;
+  a.k_rs = c.k_rs; a.k_hs = c.k_hs;
+  a.v_rs = c.v_rs; a.v_hs = c.v_hs;
+  a.o_rs = out_row_stride; a.o_hs = out_head_stride;
+  a.bias_bs = bias_seq_stride; a.bias_hs = bias_head_stride;
+  a.lse_total = total_q;
+  a.batch = num_seqs; a.sq = max_seqlen_q; a.sk = max_seqlen_k;
+  a.h = num_heads; a.hkv = num_heads_k; a.group = num_heads / num_heads_k;
+  a.scale_log2 = softmax_scale * kLog2e;
+  const PagedArgs pages{page_table, table_stride, c.k_ps, c.v_ps, table_cols, c.lg, c.n_pages};
+  const int hp = a.group % 2 == 0 ? 2 : 1;
+  const int64_t units = (int64_t)num_seqs * (num_heads / hp);
+  const FwdPlan plan = plan_varlen(hp, max_seqlen_q, max_seqlen_k, units, true, workspace ? workspace_bytes : 0, 256);
+  const int64_t nblocks = varlen_grid(a, plan, units, workspace, true, total_q, (int64_t)num_seqs * max_seqlen_k);
+  TG_CHECK(nblocks < (1ll << 31), "%s: grid too large", what);
+  auto launch = [&](auto nw_c, auto hp_c) {
+    constexpr int NW = decltype(nw_c)::value, HP = decltype(hp_c)::value;
+    if (bias_raw) launch_paged<NW, HP, true>(a, pages, (int)nblocks, stream);
+    else launch_paged<NW, HP, false>(a, pages, (int)nblocks, stream);
+  };
+  const std::integral_constant<int, 1> one;
+  const std::integral_constant<int, 2> two;
+  const std::integral_constant<int, 4> four;
+  const std::integral_constant<int, 8> eight;
+  if (plan.nw == 4 && hp == 2) launch(four, two);
+  else if (plan.nw == 4) launch(four, one);
+  else if (hp == 2) launch(eight, two);
+  else launch(eight, one);
+  TG_HIP_CHECK(hipPeekAtLastError());
   return 0;
 }

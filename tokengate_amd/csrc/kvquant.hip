@@ -14,6 +14,7 @@
 #include <algorithm>
 #include <type_traits>
 
+#include "decode_split.h"
 #include "tg_common.h"
 #include "../../include/tokengate_hip.h"
 
@@ -43,14 +44,6 @@ __device__ __forceinline__ float min3_nan(float a, float b, float c) {
 }
 
 // x of lane l ^ M, of 16 lanes, without the LDS crossbar
-template <int CTRL>
-__device__ __forceinline__ uint32_t dpp(uint32_t x) {
-  return (uint32_t)__builtin_amdgcn_update_dpp((int)x, (int)x, CTRL, 0xf, 0xf, true);
-}
-template <int CTRL>
-__device__ __forceinline__ float dpp(float x) {
-  return u32_as_f32(dpp<CTRL>(__builtin_bit_cast(uint32_t, x)));
-}
 template <int M>
 __device__ __forceinline__ uint32_t lane_xor(uint32_t x) {
   static_assert(M == 1 || M == 2 || M == 4 || M == 8, "a row of 16 lanes");
@@ -295,7 +288,6 @@ struct QuantAttnArgs {
 };
 
 constexpr int kWaves = 4;
-constexpr int kRounds = 2;
 constexpr int kTile = 64;        // keys of a wave's step
 // Tiles that a wave holds or has on their way, and workgroups per CU, by the registers.  16 / 8 heads (two at once), 4
 // bits, two tiles and 2 workgroups / one and 3: 32769 keys 23.5 / 24.5 us, 64 x 4096 79 / 77, with bias 73.4 / 72.6, 64 x
@@ -308,42 +300,6 @@ constexpr float kRescaleTau = 8.f;
 // stays below it up to steps of 2^60, and then up to the largest.
 constexpr float kLargeSum = 0x1p100f, kLift = 64.f;
 constexpr int kParts = 3;        // bf16 numbers of a weight
-
-template <typename T>
-__device__ __forceinline__ void st_agent(T *p, T v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
-template <typename T>
-__device__ __forceinline__ T ld_agent(const T *p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
-
-// 0 * x = 0, whatever x is.  (The builtin: an asm statement right behind the exponential that feeds it would read the
-// register too early, as the compiler keeps the wait that such a pair needs from its own instructions only.)
-extern "C" __device__ float tg_fmul_legacy(float, float) __asm("llvm.amdgcn.fmul.legacy");
-__device__ __forceinline__ float mul_zero(float a, float b) { return tg_fmul_legacy(a, b); }
-__device__ __forceinline__ float wave_max(float x) {
-  x = fmaxf(x, dpp<0xB1>(x));    // quad_perm 1 0 3 2
-  x = fmaxf(x, dpp<0x4E>(x));    // quad_perm 2 3 0 1
-  x = fmaxf(x, dpp<0x141>(x));   // row_half_mirror
-  x = fmaxf(x, dpp<0x140>(x));   // row_mirror
-  return quad_swap_max(x);
-}
-__device__ __forceinline__ float add_row_pair(float x) {   // x of lanes l and l ^ 16
-  const uint32_t u = __builtin_bit_cast(uint32_t, x);
-  const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-  const uint32_t a0 = a[0], a1 = a[1];
-  return u32_as_f32(a0) + u32_as_f32(a1);
-}
-__device__ __forceinline__ float add_rows(float x) {       // x of lanes l, l ^ 16, l ^ 32, l ^ 48
-  const uint32_t v = __builtin_bit_cast(uint32_t, add_row_pair(x));
-  const auto c = __builtin_amdgcn_permlane32_swap(v, v, false, false);
-  const uint32_t c0 = c[0], c1 = c[1];
-  return u32_as_f32(c0) + u32_as_f32(c1);
-}
-__device__ __forceinline__ float wave_add(float x) {
-  x += dpp<0xB1>(x);
-  x += dpp<0x4E>(x);
-  x += dpp<0x141>(x);
-  x += dpp<0x140>(x);
-  return add_rows(x);
-}
 
 // bf16 pairs of eight codes from four words (4 bits) or pairs of words (8) of as many rows, nibbles (bytes) e of each:
 // low half a, high half b of code pairs (a, b).
@@ -364,80 +320,6 @@ __device__ __forceinline__ uint32_t byte_pair(uint32_t a, uint32_t b, int byte) 
   return __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, fb), __builtin_bit_cast(uint32_t, fa), 0x07060302u);
 }
 
-// The chunk that a workgroup takes: the q-th of all sequences' chunks in turn.  A sequence of n tiles is cut into
-// ceil(n / T) chunks of even length, with one T for all, from their tiles, which only the device knows: the least that
-// makes no more workgroups than are resident at once (a workgroup's fixed costs, 5 us, and a second round's uneven
-// end cost more than idle places), or, where the sequences' remainders alone would fill most of these, two
-// rounds.
-// 16 / 8 heads, T for one round as far as it goes / two rounds / as here, us: 64 sequences of 512 .. 4099 at 8 bits 76 / 78
-// / 76; 64 alike of 300 18.3 / 25.5 / 18.0; 8 of 16k .. 128k at 4 bits 162 / 178 / 161; 16 of 4k .. 30k 82 / 91 / 82; 64
-// alike of 4096 69 / 78 / 69; 300 of 300 .. 3000 168 / 154 / 154; 120 of 50 .. 20000 323 / 298 / 297.
-struct Chunk {
-  int seq, chunk, chunks, tiles, sk;
-  int64_t start;
-};
-template <int CTRL, int ROWS>
-__device__ __forceinline__ int scan_step(int x) { return x + __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xf, false); }
-__device__ __forceinline__ int wave_scan(int x) {   // sum over the lanes up to this one
-  x = scan_step<0x111, 0xf>(x);   // row_shr 1, 2, 4, 8
-  x = scan_step<0x112, 0xf>(x);
-  x = scan_step<0x114, 0xf>(x);
-  x = scan_step<0x118, 0xf>(x);
-  x = scan_step<0x142, 0xa>(x);   // row_bcast 15: the first row's sum to the second, the third's to the fourth
-  return scan_step<0x143, 0xc>(x);   // row_bcast 31: the first half's to the second
-}
-// ceil(n / T), n and T below 2^22: the quotient's float is off by less than 1 / T
-__device__ __forceinline__ int ceil_div(int n, float inv) { return (int)(((float)n - 0.5f) * inv) + 1; }
-__device__ __forceinline__ Chunk find_chunk(const QuantAttnArgs &a, int q, int lane) {
-  int sk = 0, start = 0, tiles = 0;
-  auto read = [&](int s) {                       // of sequence s, this lane's
-    start = s < a.nseq ? a.kv_start[s] : 0;
-    sk = s < a.nseq ? max(0, min(a.kv_used[s], a.max_k)) : 0;
-    if (start < 0 || (int64_t)start + sk > a.c.rows) sk = 0;
-    tiles = (max(0, sk - 1) + kTile - 1) / kTile;
-  };
-  auto count = [&](int T, bool all) {            // chunks of all sequences, or their tiles
-    int n = 0;
-    const float inv = 1.f / (float)T;
-    for (int s0 = 0; s0 < a.nseq; s0 += 64) {
-      if (s0 > 0 || all) read(s0 + lane);
-      n += wave_sum_int(all ? tiles : s0 + lane < a.nseq ? max(1, ceil_div(tiles, inv)) : 0);
-    }
-    if (a.nseq > 64) read(lane);
-    return __builtin_amdgcn_readfirstlane(n);
-  };
-  const float work = (float)count(1, true) * (float)a.sets, slots = (float)a.slots;
-  float target = slots;
-  int T = max(a.least, (int)(work / target) + 1);
-  // (where not even an even cut of every sequence would fill one round, nothing is counted)
-  for (int i = 0; i < 3 && work / (float)T + (float)a.nseq * (float)a.sets > slots; ++i) {
-    const float over = (float)count(T, false) * (float)a.sets - slots;
-    if (over <= 0.f) break;
-    if (over > 0.75f * slots) {
-      T = max(a.least, (int)(work / (kRounds * slots)) + 1);
-      break;
-    }
-    target = fmaxf(target - over, 0.25f * slots);
-    T = max(T + 1, (int)(work / target) + 1);
-  }
-  const float inv = 1.f / (float)T;
-  int before = 0;
-  for (int s0 = 0; s0 < a.nseq; s0 += 64) {
-    if (s0 > 0) read(s0 + lane);
-    const int n = s0 + lane < a.nseq ? max(1, ceil_div(tiles, inv)) : 0;
-    const int up_to = wave_scan(n) + before;
-    const uint64_t in = __builtin_amdgcn_ballot_w64(up_to > q);
-    if (in) {
-      const int l = (int)__builtin_ctzll(in);
-      const int chunks = __builtin_amdgcn_readlane(n, l);
-      return Chunk{s0 + l, q - (__builtin_amdgcn_readlane(up_to, l) - chunks), chunks, __builtin_amdgcn_readlane(tiles, l),
-                   __builtin_amdgcn_readlane(sk, l), __builtin_amdgcn_readlane(start, l)};
-    }
-    before = __builtin_amdgcn_readlane(up_to, 63);
-  }
-  return Chunk{-1, 0, 0, 0, 0, 0};
-}
-
 template <int BITS, int HP, bool HAS_BIAS>
 __global__ __launch_bounds__(64 * kWaves, per_cu(BITS, HP)) void decode_attn_quant_kernel(QuantAttnArgs a) {
   constexpr int kRow = 16 * BITS;                 // bytes of a row's codes
@@ -453,7 +335,11 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(BITS, HP)) void decode_attn_qua
   __shared__ __attribute__((aligned(16))) bf16_t ps[kWaves][kGroups][kParts * HP][kTile];
   __shared__ __attribute__((aligned(16))) float part_o[kWaves + 1][HP][kHeadDim], part_ml[kWaves + 1][HP][2];
 
-  const Chunk ck = find_chunk(a, blockIdx.x / a.sets, lane);
+  const Chunk ck = find_chunk<kTile>({a.nseq, a.sets, a.slots, a.least}, blockIdx.x / a.sets, lane, [&](int s) {
+    const int64_t start = a.kv_start[s];
+    const int sk = max(0, min(a.kv_used[s], a.max_k));
+    return Keys{start, start < 0 || start + sk > a.c.rows ? 0 : sk};
+  });
   if (ck.seq < 0) return;                        // workgroup-uniform: past the last chunk
   const int b = ck.seq, nk = max(0, ck.sk - 1);  // keys in the cache; the new one is apart
   const int64_t start = ck.start;

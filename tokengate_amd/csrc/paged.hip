@@ -1,0 +1,583 @@
+// KV caches in pages: rows appended on the way out of the projection, and the attention of a decode step over them.
+#include <algorithm>
+#include <type_traits>
+
+#include "decode_split.h"
+#include "paged.h"
+#include "tg_common.h"
+#include "../../include/tokengate_hip.h"
+
+namespace tg {
+namespace {
+
+// ---- start of a step: the packed rows' slots and rotary table -----------------------------------------
+// One wave a row.  The row's sequence is the last one that begins at or before it (a bisection over cu_seqlens, whose
+// values the lanes read alike).  Angles as tg_decode_begin's and tg_qk_norm_rope's: position * inv_freq in fp32.
+struct BeginArgs {
+  const int64_t *pos;
+  int64_t n;
+  const float *inv_freq;
+  const int32_t *cu, *used;
+  int nseq;
+  const int32_t *table;
+  int64_t table_rs;
+  int cols, lg, n_pages;
+  int32_t *slots;
+  float2 *rope;
+};
+__global__ __launch_bounds__(256) void paged_begin_kernel(BeginArgs a) {
+  const int64_t t = (int64_t)blockIdx.x * 4 + wave_id();
+  if (t >= a.n) return;
+  const int lane = threadIdx.x & 63;
+  float s, c;
+  sincosf((float)a.pos[t] * a.inv_freq[lane], &s, &c);
+  a.rope[t * (kHeadDim / 2) + lane] = float2{c, s};
+  if (lane != 0) return;
+  int lo = 0, hi = a.nseq;                       // cu[lo] <= t < cu[hi], where the row has a sequence
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (a.cu[mid] <= t) lo = mid;
+    else hi = mid;
+  }
+  const int64_t first = a.cu[lo], end = a.cu[lo + 1], key = a.used[lo] - end + t;
+  int32_t slot = -1;
+  if (t >= first && t < end && key >= 0 && key >> a.lg < a.cols) {
+    const int32_t page = a.table[lo * a.table_rs + (key >> a.lg)];
+    if ((uint32_t)page < (uint32_t)a.n_pages) slot = (page << a.lg) + (int32_t)(key & ((1 << a.lg) - 1));
+  }
+  a.slots[t] = slot;
+}
+
+// ---- append: q/k RMSNorm, rotary embedding, k and v rows into their slots ------------------------------------
+// 16 lanes a row of one head, 8 elements a lane (the rotate-half partner sits in lane j ^ 8); a group of 16 lanes takes up
+// to kRowsPer rows of one token, so that its (cos, sin) are read once for them and as many rows are in flight.
+struct AppendArgs {
+  const bf16_t *qkv;
+  int64_t qkv_rs;
+  const float *rope;
+  int64_t n;
+  int h, hkv;
+  const bf16_t *qw, *kw;
+  float eps;
+  const float *q_head_scale, *q_row_scale;
+  bf16_t *q;
+  int64_t q_rs, q_hs;
+  const int32_t *slots;
+  PagePool c;
+  int groups;                    // of 16 lanes per token
+};
+constexpr int kRowsPer = 4;
+
+__global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a) {
+  const int j = threadIdx.x & 15;
+  const int64_t id = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
+  const int64_t t = id / a.groups;
+  const int sub = (int)(id - t * a.groups), rows = a.h + 2 * a.hkv;
+  if (t >= a.n) return;          // uniform over the 16 lanes
+  const bf16_t *src = a.qkv + t * a.qkv_rs + 8 * j;
+  u32x4 raw[kRowsPer];
+#pragma unroll
+  for (int i = 0; i < kRowsPer; ++i) {
+    const int r = sub + i * a.groups;
+    if (r < rows) raw[i] = ld16(src + (int64_t)r * kHeadDim);
+  }
+  const f32x4 *rp = reinterpret_cast<const f32x4 *>(a.rope + t * kHeadDim + 16 * (j & 7));
+  float cs[8][2];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const f32x4 x = rp[i];
+    cs[2 * i][0] = x[0];
+    cs[2 * i][1] = x[1];
+    cs[2 * i + 1][0] = x[2];
+    cs[2 * i + 1][1] = x[3];
+  }
+  const int32_t slot = a.slots[t];
+  const bool keep = (uint32_t)slot < (uint32_t)a.c.n_pages << a.c.lg;
+  const int64_t page = slot >> a.c.lg, off = slot & ((1 << a.c.lg) - 1);
+#pragma unroll
+  for (int i = 0; i < kRowsPer; ++i) {
+    const int r = sub + i * a.groups;
+    if (r >= rows) break;
+    if (r >= a.h + a.hkv) {      // a value
+      if (keep) st16(a.c.v + page * a.c.v_ps + (r - a.h - a.hkv) * a.c.v_hs + off * a.c.v_rs + 8 * j, raw[i]);
+      continue;
+    }
+    const bool is_q = r < a.h;
+    float x[8], wf[8], y[8];
+    unpack8(raw[i], x);
+    unpack8(ld16((is_q ? a.qw : a.kw) + 8 * j), wf);
+    const float hs = is_q ? (float)(__bf16)((a.q_head_scale ? a.q_head_scale[r] : 1.f) * (a.q_row_scale ? a.q_row_scale[t] : 1.f))
+                          : 1.f;
+    norm_rope8(x, wf, a.eps, cs, j, hs, y);
+    if (is_q) st16(a.q + t * a.q_rs + r * a.q_hs + 8 * j, pack8(y));
+    else if (keep) st16(a.c.k + page * a.c.k_ps + (r - a.h) * a.c.k_hs + off * a.c.k_rs + 8 * j, pack8(y));
+  }
+}
+
+// ---- attention of a decode step ---------------------------------------------------------------------
+//   z_j = scale (q . k_j + bias_j),   out = sum_j e^(z_j - m) v_j / sum_j e^(z_j - m)
+// One workgroup per (sequence, KV head and up to 16 of its query heads); a wave takes 32 keys at a time, straight from
+// the pages to registers in the layouts that the matrix cores read, so nothing waits at a barrier:
+//   * S^T = K Q^T (v_mfma_f32_16x16x32_bf16): A holds keys, lane (n, G) (n = lane % 16, G = lane / 16) elements 32 i + 8 G
+//     .. + 7 of key 8 (n / 4) + 4 t + n % 4 of instruction t (0, 1); B the query heads, head n % HP in column n.  So lane
+//     (n, G) ends up with the logits of keys 8 G .. 8 G + 7 of its head: in the order that the weights have as O's A.
+//   * O = P V: a lane reads 16 bytes (elements 8 n .. 8 n + 7) of keys 8 G .. 8 G + 7; instruction e takes element 8 n + e of
+//     the eight, one byte permutation per two.
+//   * A weight is two bf16 numbers, 16 bits together (relative error 2^-17; rounded to one it would be 2^-9, as much as
+//     the output's own rounding): columns repeat the heads, and every other repetition holds the second numbers.  With 16
+//     heads there is no repetition, and the second numbers are a second product.
+//   * The new key is not in the tiles: it is a part of its own beside the waves', from registers.
+//   * Keys past the sequence's last, or of no page, are of weight 0 and their values 0, whatever the rows hold.  A key that a
+//     bias of -inf hides from a head may hold anything too: a wave whose sums are not finite takes its tiles once more,
+//     each head by itself with the rows it does not see left out, and with weights 2^-64 of these (values near the largest
+//     float pass fp32's range in the first sums).
+struct PagedAttnArgs {
+  const bf16_t *qkv;
+  int64_t qkv_rs;
+  const float *rope;
+  int h, hkv, group;
+  const bf16_t *qw, *kw;
+  float eps;
+  const float *q_head_scale, *q_row_scale;
+  PagePool c;
+  const int32_t *table;
+  int64_t table_rs;
+  int cols;
+  const int32_t *used;
+  int max_k;
+  const float *bias;
+  int64_t bias_bs, bias_hs;
+  float scale_log2;
+  bf16_t *out;
+  int64_t out_rs;
+  int nseq, sets;                // kv heads times head sets
+};
+
+constexpr int kWaves = 4;
+constexpr int kTile = 32;        // keys of a wave's step
+constexpr float kRescaleTau = 8.f;               // the running maximum moves only when a logit passes it by 2^8
+constexpr float kLargeSum = 0x1p100f, kLift = 64.f;
+
+template <int HP, bool HAS_BIAS>
+__global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_kernel(PagedAttnArgs a) {
+  const int tid = threadIdx.x, wave = wave_id(), lane = tid & 63, n16 = lane & 15, G = lane >> 4;
+  const int set = blockIdx.x % a.sets, kh = set % a.hkv, hg = set / a.hkv;
+  const int h0 = kh * a.group + hg * HP, nh = min(HP, a.group - hg * HP);   // heads h0 .. h0 + nh - 1
+
+  __shared__ __attribute__((aligned(16))) bf16_t qs[HP][kHeadDim];
+  __shared__ __attribute__((aligned(16))) bf16_t new_x[2][kHeadDim];   // the new key and value
+  __shared__ __attribute__((aligned(16))) float part_o[kWaves + 1][HP][kHeadDim], part_ml[kWaves + 1][HP][2];
+
+  const int b = blockIdx.x / a.sets;
+  const int sk = max(0, min(a.used[b], a.max_k)), nk = max(0, sk - 1);   // keys in the pages; the new one is apart
+  const int t_lo = 0, t_hi = (nk + kTile - 1) / kTile;
+  const int32_t *const trow = a.table + b * a.table_rs;
+  const int lg = a.c.lg, mask = (1 << lg) - 1;
+  auto page_of = [&](int key) { return trow[min(key >> lg, a.cols - 1)]; };
+  const bool has_new = sk > 0 && (uint32_t)page_of(nk) < (uint32_t)a.c.n_pages;
+
+  // ---- the rows to form: 16 lanes a row: query heads, then the new key and the new value ----
+  for (int r = tid >> 4; r < HP + 2; r += 4 * kWaves) {
+    if (r >= HP && !has_new) break;
+    const int head = r < HP ? h0 + min(r, nh - 1) : r == HP ? a.h + kh : a.h + a.hkv + kh;
+    const u32x4 raw = ld16(a.qkv + b * a.qkv_rs + (int64_t)head * kHeadDim + 8 * n16);
+    u32x4 y8 = raw;
+    if (r <= HP) {
+      const float *rp = a.rope + b * kHeadDim + 16 * (n16 & 7);
+      float x[8], wf[8], y[8], cs[8][2];
+      unpack8(raw, x);
+      unpack8(ld16((r < HP ? a.qw : a.kw) + 8 * n16), wf);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) cs[i >> 1][i & 1] = rp[i];
+      const float hs = r < HP ? (float)(__bf16)((a.q_head_scale ? a.q_head_scale[head] : 1.f) * (a.q_row_scale ? a.q_row_scale[b] : 1.f))
+                              : 1.f;
+      norm_rope8(x, wf, a.eps, cs, n16, hs, y);
+      y8 = pack8(y);
+    }
+    if (r < HP) {
+      st16(&qs[r][8 * n16], y8);
+    } else {
+      st16(&new_x[r - HP][8 * n16], y8);
+      if (hg == 0) {
+        const int64_t page = page_of(nk), off = nk & mask;
+        st16((r == HP ? a.c.k + page * a.c.k_ps + kh * a.c.k_hs + off * a.c.k_rs
+                      : a.c.v + page * a.c.v_ps + kh * a.c.v_hs + off * a.c.v_rs) + 8 * n16, y8);
+      }
+    }
+  }
+  __syncthreads();
+  // ---- the new key: a part of its own, 16 lanes a head ----
+  if (has_new && wave == kWaves - 1) {
+    for (int i = G; i < HP; i += 4) {
+      float q[8], k[8], v[8], z = 0.f;
+      unpack8(*reinterpret_cast<const u32x4 *>(&qs[i][8 * n16]), q);
+      unpack8(*reinterpret_cast<const u32x4 *>(&new_x[0][8 * n16]), k);
+      unpack8(*reinterpret_cast<const u32x4 *>(&new_x[1][8 * n16]), v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        z = fmaf(q[e], k[e], z);
+        part_o[kWaves][i][8 * n16 + e] = v[e];
+      }
+      z += dpp<0xB1>(z);
+      z += dpp<0x4E>(z);
+      z += dpp<0x141>(z);
+      z += dpp<0x140>(z);
+      const float bias = HAS_BIAS ? a.bias[(int64_t)b * a.bias_bs + (int64_t)(h0 + min(i, nh - 1)) * a.bias_hs + nk] : 0.f;
+      const bool hidden = bias == -INFINITY;
+      if (n16 == 0) {
+        part_ml[kWaves][i][0] = hidden ? -INFINITY : (z + bias) * a.scale_log2;
+        part_ml[kWaves][i][1] = hidden ? 0.f : 1.f;
+      }
+    }
+  }
+
+  bf16x8 qf[4];                  // lane (n, G): elements 32 i + 8 G .. + 7 of head n % HP
+#pragma unroll
+  for (int i = 0; i < 4; ++i) qf[i] = *reinterpret_cast<const bf16x8 *>(&qs[n16 & (HP - 1)][32 * i + 8 * G]);
+  const bool second = HP < 16 && (n16 & HP);     // this column holds the weights' second numbers
+
+  struct Tile {
+    u32x4 k[2][4], v[8];
+    float bias[8];
+    int valid;                   // of this lane's keys 8 G .. 8 G + 7, those that are there
+  };
+  const bf16_t *const kbase = a.c.k + kh * a.c.k_hs + 8 * G, *const vbase = a.c.v + kh * a.c.v_hs + 8 * n16;
+  const float *const bias_row = HAS_BIAS ? a.bias + (int64_t)b * a.bias_bs + (int64_t)(h0 + min(n16 & (HP - 1), nh - 1)) * a.bias_hs : nullptr;
+  auto load = [&](Tile &l, int tile) {
+    const int key0 = tile * kTile, kk = key0 + 8 * (n16 >> 2), vk = key0 + 8 * G;
+    const int kp = page_of(kk), vp = page_of(vk);
+    const bool there = (uint32_t)vp < (uint32_t)a.c.n_pages;
+    l.valid = there ? max(0, min(8, nk - vk)) : 0;
+    const int64_t kpage = (uint32_t)kp < (uint32_t)a.c.n_pages ? kp : 0, vpage = there ? vp : 0;   // (any row will do)
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const bf16_t *p = kbase + kpage * a.c.k_ps + (int64_t)((kk & mask) + 4 * t + (n16 & 3)) * a.c.k_rs;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) l.k[t][i] = ld16(p + 32 * i);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) l.v[j] = ld16(vbase + vpage * a.c.v_ps + (int64_t)((vk & mask) + j) * a.c.v_rs);
+    if constexpr (HAS_BIAS) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) l.bias[j] = vk + j < nk ? bias_row[vk + j] : 0.f;
+    }
+  };
+
+  f32x4 oacc[8];                 // lane (n, G): rows (columns of S^T) 4 G .. 4 G + 3, elements 8 n + e
+  float mrun, lsum;
+  auto step = [&](Tile &l, auto careful_c, float lift) {
+    constexpr bool CAREFUL = decltype(careful_c)::value;
+    f32x4 s[2] = {};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) s[t] = mfma16(__builtin_bit_cast(bf16x8, l.k[t][i]), qf[i], s[t]);
+    float z[8], most = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      z[j] = (HAS_BIAS ? s[j >> 2][j & 3] + l.bias[j] : s[j >> 2][j & 3]) * a.scale_log2;
+      asm("" : "+v"(z[j]));   // rounded: contracted into z - m below, a bias near the lowest float leaves the rounding's rest
+      if (j >= l.valid) z[j] = -INFINITY;
+      if constexpr (HAS_BIAS) z[j] = l.bias[j] == -INFINITY ? -INFINITY : z[j];   // hidden, whatever the row holds
+      most = fmaxf(most, z[j]);
+    }
+    if (__builtin_amdgcn_ballot_w64(most > mrun + (kRescaleTau - lift))) {
+      const float m = fmaxf(mrun, quad_swap_max(most) + lift), f = mrun == -INFINITY ? 0.f : fast_exp2(mrun - m);
+      mrun = m;
+      lsum *= f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float fr = __shfl(f, 4 * G + i);   // of the row's head
+#pragma unroll
+        for (int e = 0; e < 8; ++e) oacc[e][i] *= fr;
+      }
+    }
+    const float base = mrun == -INFINITY ? 0.f : mrun;
+    u32x4 w0, w1;
+    float p[8];
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+      p[j] = fast_exp2(z[j] - base);
+      p[j + 1] = fast_exp2(z[j + 1] - base);
+      lsum += p[j] + p[j + 1];
+      const uint32_t hi = pack_bf16x2(p[j], p[j + 1]);
+      const uint32_t lo = pack_bf16x2(p[j] - u32_as_f32(hi << 16), p[j + 1] - u32_as_f32(hi & 0xffff0000u));
+      w0[j >> 1] = second && !CAREFUL ? lo : hi;
+      w1[j >> 1] = lo;
+    }
+    if (__builtin_amdgcn_ballot_w64(l.valid < 8)) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (j >= l.valid) l.v[j] = u32x4{0u, 0u, 0u, 0u};
+    }
+    auto column = [&](const u32x4 (&v)[8], int e) {   // element 8 n + e of keys 8 G .. 8 G + 7
+      u32x4 c;
+#pragma unroll
+      for (int m = 0; m < 4; ++m)
+        c[m] = __builtin_amdgcn_perm(v[2 * m + 1][e >> 1], v[2 * m][e >> 1], e & 1 ? 0x07060302u : 0x05040100u);
+      return __builtin_bit_cast(bf16x8, c);
+    };
+    const bf16x8 pa = __builtin_bit_cast(bf16x8, w0), pb = __builtin_bit_cast(bf16x8, w1);
+    if constexpr (!CAREFUL) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const bf16x8 v = column(l.v, e);
+        oacc[e] = mfma16(pa, v, oacc[e]);
+        if constexpr (HP == 16) oacc[e] = mfma16(pb, v, oacc[e]);
+      }
+    } else {
+      // (the second numbers times the finite values alone: such a number may be 0)
+      auto finite = [](uint32_t x) {
+        const uint32_t lo = (x & 0x7f80u) == 0x7f80u ? 0u : x & 0xffffu, hi = (x & 0x7f800000u) == 0x7f800000u ? 0u : x & 0xffff0000u;
+        return lo | hi;
+      };
+#pragma unroll 1
+      for (int hd = 0; hd < HP; ++hd) {
+        u32x4 v[8], u[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          v[j] = __shfl(p[j], 16 * G + hd) == 0.f ? u32x4{0u, 0u, 0u, 0u} : l.v[j];
+#pragma unroll
+          for (int x = 0; x < 4; ++x) u[j][x] = finite(v[j][x]);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const f32x4 o = mfma16(pb, column(u, e), mfma16(pa, column(v, e), f32x4{0.f, 0.f, 0.f, 0.f}));
+#pragma unroll
+          for (int i = 0; i < 4; ++i) oacc[e][i] += 4 * G + i == hd ? o[i] : 0.f;
+        }
+      }
+    }
+  };
+  auto tiles = [&](auto careful_c, float lift) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) oacc[e] = f32x4{0.f, 0.f, 0.f, 0.f};
+    mrun = -INFINITY;
+    lsum = 0.f;
+    for (int t = t_lo + wave; t < t_hi; t += kWaves) {
+      Tile l;
+      load(l, t);
+      step(l, careful_c, lift);
+    }
+  };
+  // elements 8 n .. 8 n + 7 of head i, i = 0 .. 3 of the lane group that holds the head's first rows, the numbers' sums
+  auto sums = [&](int i, float (&o)[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if constexpr (HP == 1) o[e] = oacc[e][0] + oacc[e][1];
+      else if constexpr (HP == 2) o[e] = oacc[e][i] + oacc[e][i + 2];
+      else if constexpr (HP == 4) o[e] = add_row_pair(oacc[e][i]);
+      else if constexpr (HP == 8) o[e] = pair_sum(oacc[e][i]);
+      else o[e] = oacc[e][i];
+    }
+  };
+  constexpr int kHere = HP < 4 ? HP : 4;         // heads of a lane group
+  auto fine = [&] {
+    bool ok = true;
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) ok &= fabsf(oacc[e][i]) < kLargeSum;
+    return !__builtin_amdgcn_ballot_w64(!ok);
+  };
+  tiles(std::false_type(), 0.f);
+  if (!fine()) tiles(std::true_type(), kLift);   // (a NaN that a visible key holds comes again)
+
+  // ---- the waves' results meet in LDS ----
+  {
+    const float l = add_rows(lsum);
+    if (G == 0 && n16 < HP) {
+      part_ml[wave][n16][0] = mrun;
+      part_ml[wave][n16][1] = l;
+    }
+#pragma unroll
+    for (int i = 0; i < kHere; ++i) {
+      float o[8];
+      sums(i, o);
+      const int hd = 4 * G + i;
+      if (hd < HP) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) part_o[wave][hd][8 * n16 + e] = o[e];
+      }
+    }
+  }
+  __syncthreads();
+  bf16_t *const orow = a.out + b * a.out_rs + (int64_t)h0 * kHeadDim;
+  for (int item = tid; item < HP * kHeadDim / 2; item += 64 * kWaves) {
+    const int i = item / 64, d = 2 * (item % 64);
+    float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWaves + 1; ++w)
+      if (w < kWaves || has_new) m = fmaxf(m, part_ml[w][i][0]);
+#pragma unroll
+    for (int w = 0; w < kWaves + 1; ++w) {
+      if (w == kWaves && !has_new) break;
+      const float mw = part_ml[w][i][0], f = mw == -INFINITY ? (part_ml[w][i][1] == 0.f ? 0.f : 1.f) : fast_exp2(mw - m);
+      l += f * part_ml[w][i][1];
+      o0 += mul_zero(f, part_o[w][i][d]);
+      o1 += mul_zero(f, part_o[w][i][d + 1]);
+    }
+    const float f = l == 0.f ? 0.f : 1.f / l;
+    if (i < nh)                  // a row that saw no key: 0
+      *reinterpret_cast<uint32_t *>(orow + 2 * item) = l == 0.f ? 0u : pack_bf16x2(o0 * f, o1 * f);
+  }
+}
+
+// Query heads of a workgroup: the KV head's, up to a power of two that holds them, at most 16.
+int heads_per(int group) {
+  int hp = 1;
+  while (hp < group && hp < 16) hp *= 2;
+  return hp;
+}
+
+}  // namespace
+}  // namespace tg
+
+using namespace tg;
+
+extern "C" int tg_paged_begin(const int64_t *positions, int64_t n_rows, const float *inv_freq, const int32_t *cu_seqlens,
+                              const int32_t *kv_used, int32_t num_seqs, const int32_t *page_table, int64_t table_stride,
+                              int32_t table_cols, int32_t num_pages, int32_t page_rows, int32_t *slots, float *rope,
+                              hipStream_t stream) {
+  clear_error();
+  const char *what = "paged_begin";
+  TG_CHECK(positions && inv_freq && cu_seqlens && kv_used && slots && rope, "%s: null pointer", what);
+  TG_CHECK(n_rows >= 0 && n_rows < (1ll << 31) && num_seqs > 0, "%s: bad row or sequence count", what);
+  TG_CHECK(num_pages >= 0 && page_rows >= 16 && page_rows <= 65536 && (page_rows & (page_rows - 1)) == 0 &&
+               (int64_t)num_pages * page_rows < (1ll << 31),
+           "%s: page rows must be a power of two from 16 to 65536, of less than 2^31 rows in all", what);
+  if (int e = check_table(what, page_table, table_stride, table_cols, num_seqs)) return e;
+  if (n_rows == 0) return 0;
+  const BeginArgs a{positions, n_rows, inv_freq, cu_seqlens, kv_used, num_seqs, page_table, table_stride, table_cols,
+                    __builtin_ctz((unsigned)page_rows), num_pages, slots, reinterpret_cast<float2 *>(rope)};
+  hipLaunchKernelGGL(paged_begin_kernel, dim3((unsigned)((n_rows + 3) / 4)), dim3(256), 0, stream, a);
+  TG_HIP_CHECK(hipGetLastError());
+  return 0;
+}
+
+extern "C" int tg_paged_append(const void *qkv, int64_t qkv_row_stride, const float *rope, int64_t n_tokens,
+                               int32_t num_heads, int32_t num_heads_k, int32_t head_dim, const void *q_norm_weight,
+                               const void *k_norm_weight, float eps, const float *q_head_scale, const float *q_row_scale,
+                               void *q_out, int64_t q_row_stride, int64_t q_head_stride, const int32_t *slots,
+                               void *k_pages, int64_t k_page_stride, int64_t k_head_stride, int64_t k_row_stride,
+                               void *v_pages, int64_t v_page_stride, int64_t v_head_stride, int64_t v_row_stride,
+                               int32_t num_pages, int32_t page_rows, hipStream_t stream) {
+  clear_error();
+  const char *what = "paged_append";
+  AppendArgs a{};
+  if (int e = check_pool(what, k_pages, v_pages, {k_page_stride, k_head_stride, k_row_stride},
+                         {v_page_stride, v_head_stride, v_row_stride}, num_pages, page_rows, num_heads_k, head_dim, &a.c))
+    return e;
+  TG_CHECK(qkv && rope && q_norm_weight && k_norm_weight && q_out && slots, "%s: null pointer", what);
+  TG_CHECK(num_heads > 0 && num_heads <= 256, "%s: heads must be in 1..256", what);
+  TG_CHECK(n_tokens >= 0 && n_tokens < (1ll << 31), "%s: bad token count", what);
+  TG_CHECK(qkv_row_stride % 8 == 0 && qkv_row_stride >= (int64_t)(num_heads + 2 * num_heads_k) * kHeadDim,
+           "%s: qkv rows must hold q, k and v of every head, strides be multiples of 8 elements", what);
+  TG_CHECK(q_row_stride % 8 == 0 && q_head_stride % 8 == 0 && q_head_stride >= kHeadDim && q_row_stride >= 0,
+           "%s: q strides must be multiples of 8 elements, heads apart", what);
+  TG_CHECK(aligned16(qkv) && aligned16(q_norm_weight) && aligned16(k_norm_weight) && aligned16(rope) && aligned16(q_out),
+           "%s: pointers must be 16-byte aligned", what);
+  if (n_tokens == 0) return 0;
+  a.qkv = static_cast<const bf16_t *>(qkv);
+  a.qkv_rs = qkv_row_stride;
+  a.rope = rope;
+  a.n = n_tokens;
+  a.h = num_heads;
+  a.hkv = num_heads_k;
+  a.qw = static_cast<const bf16_t *>(q_norm_weight);
+  a.kw = static_cast<const bf16_t *>(k_norm_weight);
+  a.eps = eps;
+  a.q_head_scale = q_head_scale;
+  a.q_row_scale = q_row_scale;
+  a.q = static_cast<bf16_t *>(q_out);
+  a.q_rs = q_row_stride;
+  a.q_hs = q_head_stride;
+  a.slots = slots;
+  a.groups = (num_heads + 2 * num_heads_k + kRowsPer - 1) / kRowsPer;
+  const int64_t blocks = (n_tokens * a.groups + 15) / 16;
+  TG_CHECK(blocks < (1ll << 31), "%s: too many tokens", what);
+  hipLaunchKernelGGL(paged_append_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, a);
+  TG_HIP_CHECK(hipGetLastError());
+  return 0;
+}
+
+extern "C" int64_t tg_paged_decode_attention_workspace_size(int32_t num_seqs, int32_t num_heads, int32_t num_heads_k,
+                                                            int32_t max_seqlen_k) {
+  (void)num_seqs; (void)num_heads; (void)num_heads_k; (void)max_seqlen_k;
+  return 0;
+}
+
+extern "C" int tg_paged_decode_attention(const void *qkv, int64_t qkv_row_stride, const float *rope, int32_t num_seqs,
+                                         int32_t num_heads, int32_t num_heads_k, int32_t head_dim,
+                                         const void *q_norm_weight, const void *k_norm_weight, float eps,
+                                         const float *q_head_scale, const float *q_row_scale, void *k_pages,
+                                         int64_t k_page_stride, int64_t k_head_stride, int64_t k_row_stride,
+                                         void *v_pages, int64_t v_page_stride, int64_t v_head_stride,
+                                         int64_t v_row_stride, int32_t num_pages, int32_t page_rows,
+                                         const int32_t *page_table, int64_t table_stride, int32_t table_cols,
+                                         const int32_t *kv_used, int32_t max_seqlen_k, const float *bias_raw,
+                                         int64_t bias_seq_stride, int64_t bias_head_stride, float softmax_scale,
+                                         void *out, int64_t out_row_stride, void *workspace, int64_t workspace_bytes,
+                                         hipStream_t stream) {
+  clear_error();
+  const char *what = "paged_decode_attention";
+  PagedAttnArgs a{};
+  if (int e = check_pool(what, k_pages, v_pages, {k_page_stride, k_head_stride, k_row_stride},
+                         {v_page_stride, v_head_stride, v_row_stride}, num_pages, page_rows, num_heads_k, head_dim, &a.c))
+    return e;
+  if (int e = check_table(what, page_table, table_stride, table_cols, num_seqs)) return e;
+  TG_CHECK(qkv && rope && q_norm_weight && k_norm_weight && kv_used && out, "%s: null pointer", what);
+  TG_CHECK(num_heads > 0 && num_heads <= 256 && num_heads % num_heads_k == 0,
+           "%s: heads must be in 1..256 and a multiple of the KV heads", what);
+  TG_CHECK(num_seqs >= 0 && (int64_t)num_seqs * num_heads < (1 << 24), "%s: bad sequence count", what);
+  TG_CHECK(max_seqlen_k >= 0 && max_seqlen_k < (1 << 24), "%s: max_seqlen_k must be in 0..2^24 - 1", what);
+  TG_CHECK(max_seqlen_k <= (int64_t)table_cols * page_rows, "%s: max_seqlen_k is more than the page table's columns hold", what);
+  TG_CHECK(qkv_row_stride % 8 == 0 && out_row_stride % 8 == 0 &&
+               qkv_row_stride >= (int64_t)(num_heads + 2 * num_heads_k) * kHeadDim &&
+               out_row_stride >= (int64_t)num_heads * kHeadDim,
+           "%s: row strides must be multiples of 8 elements that hold every head", what);
+  TG_CHECK(aligned16(qkv) && aligned16(q_norm_weight) && aligned16(k_norm_weight) && aligned16(rope) && aligned16(out) &&
+               aligned16(workspace),
+           "%s: pointers must be 16-byte aligned", what);
+  TG_CHECK(softmax_scale > 0.f, "%s: softmax_scale must be positive", what);
+  TG_CHECK(!bias_raw || (bias_seq_stride >= 0 && bias_head_stride >= 0), "%s: negative bias stride", what);
+  if (num_seqs == 0) return 0;
+  a.qkv = static_cast<const bf16_t *>(qkv);
+  a.qkv_rs = qkv_row_stride;
+  a.rope = rope;
+  a.h = num_heads;
+  a.hkv = num_heads_k;
+  a.group = num_heads / num_heads_k;
+  a.qw = static_cast<const bf16_t *>(q_norm_weight);
+  a.kw = static_cast<const bf16_t *>(k_norm_weight);
+  a.eps = eps;
+  a.q_head_scale = q_head_scale;
+  a.q_row_scale = q_row_scale;
+  a.table = page_table;
+  a.table_rs = table_stride;
+  a.cols = table_cols;
+  a.used = kv_used;
+  a.max_k = max_seqlen_k;
+  a.bias = bias_raw;
+  a.bias_bs = bias_seq_stride;
+  a.bias_hs = bias_head_stride;
+  a.scale_log2 = softmax_scale * 1.4426950408889634f;
+  a.out = static_cast<bf16_t *>(out);
+  a.out_rs = out_row_stride;
+  a.nseq = num_seqs;
+  const int hp = heads_per(a.group);
+  a.sets = num_heads_k * ((a.group + hp - 1) / hp);
+  const dim3 grid((unsigned)(num_seqs * a.sets)), block(64 * kWaves);
+  auto launch = [&](auto hp_c) {
+    constexpr int HP = decltype(hp_c)::value;
+    if (bias_raw) hipLaunchKernelGGL((paged_decode_kernel<HP, true>), grid, block, 0, stream, a);
+    else hipLaunchKernelGGL((paged_decode_kernel<HP, false>), grid, block, 0, stream, a);
+  };
+  if (hp == 1) launch(std::integral_constant<int, 1>());
+  else if (hp == 2) launch(std::integral_constant<int, 2>());
+  else if (hp == 4) launch(std::integral_constant<int, 4>());
+  else if (hp == 8) launch(std::integral_constant<int, 8>());
+  else launch(std::integral_constant<int, 16>());
+  TG_HIP_CHECK(hipGetLastError());
+  return 0;
+}
