@@ -151,15 +151,19 @@ struct PagedAttnArgs {
   bf16_t *out;
   int64_t out_rs;
   int nseq, sets;                // kv heads times head sets
+  int slots, least;              // workgroups that are resident at once; fewest tiles per chunk
+  uint32_t *counters;            // per unit: chunks arrived; zero between launches
+  uint64_t *ml;                  // [workgroup][head]: running max (log2 units) and sum
+  uint64_t *po;                  // [workgroup][head][64]: O, pairs of fp32
 };
 
-constexpr int kWaves = 4;
+constexpr int kWaves = 4, kPerCu = 3;
 constexpr int kTile = 32;        // keys of a wave's step
 constexpr float kRescaleTau = 8.f;               // the running maximum moves only when a logit passes it by 2^8
 constexpr float kLargeSum = 0x1p100f, kLift = 64.f;
 
 template <int HP, bool HAS_BIAS>
-__global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_kernel(PagedAttnArgs a) {
+__global__ __launch_bounds__(64 * kWaves, kPerCu) void paged_decode_kernel(PagedAttnArgs a) {
   const int tid = threadIdx.x, wave = wave_id(), lane = tid & 63, n16 = lane & 15, G = lane >> 4;
   const int set = blockIdx.x % a.sets, kh = set % a.hkv, hg = set / a.hkv;
   const int h0 = kh * a.group + hg * HP, nh = min(HP, a.group - hg * HP);   // heads h0 .. h0 + nh - 1
@@ -168,13 +172,16 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_kernel(PagedAttnA
   __shared__ __attribute__((aligned(16))) bf16_t new_x[2][kHeadDim];   // the new key and value
   __shared__ __attribute__((aligned(16))) float part_o[kWaves + 1][HP][kHeadDim], part_ml[kWaves + 1][HP][2];
 
-  const int b = blockIdx.x / a.sets;
-  const int sk = max(0, min(a.used[b], a.max_k)), nk = max(0, sk - 1);   // keys in the pages; the new one is apart
-  const int t_lo = 0, t_hi = (nk + kTile - 1) / kTile;
+  const Chunk ck = find_chunk<kTile>({a.nseq, a.sets, a.slots, a.least}, blockIdx.x / a.sets, lane,
+                                     [&](int s) { return Keys{0, max(0, min(a.used[s], a.max_k))}; });
+  if (ck.seq < 0) return;                        // workgroup-uniform: past the last chunk
+  const int b = ck.seq, sk = ck.sk, nk = max(0, sk - 1);   // keys in the pages; the new one is apart
+  const int n_parts = ck.chunks, chunk = ck.chunk;
+  const int t_lo = (int)((int64_t)ck.tiles * chunk / n_parts), t_hi = (int)((int64_t)ck.tiles * (chunk + 1) / n_parts);
   const int32_t *const trow = a.table + b * a.table_rs;
   const int lg = a.c.lg, mask = (1 << lg) - 1;
   auto page_of = [&](int key) { return trow[min(key >> lg, a.cols - 1)]; };
-  const bool has_new = sk > 0 && (uint32_t)page_of(nk) < (uint32_t)a.c.n_pages;
+  const bool has_new = chunk == n_parts - 1 && sk > 0 && (uint32_t)page_of(nk) < (uint32_t)a.c.n_pages;
 
   // ---- the rows to form: 16 lanes a row: query heads, then the new key and the new value ----
   for (int r = tid >> 4; r < HP + 2; r += 4 * kWaves) {
@@ -243,30 +250,40 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_kernel(PagedAttnA
   };
   const bf16_t *const kbase = a.c.k + kh * a.c.k_hs + 8 * G, *const vbase = a.c.v + kh * a.c.v_hs + 8 * n16;
   const float *const bias_row = HAS_BIAS ? a.bias + (int64_t)b * a.bias_bs + (int64_t)(h0 + min(n16 & (HP - 1), nh - 1)) * a.bias_hs : nullptr;
-  auto load = [&](Tile &l, int tile) {
-    const int key0 = tile * kTile, kk = key0 + 8 * (n16 >> 2), vk = key0 + 8 * G;
-    const int kp = page_of(kk), vp = page_of(vk);
-    const bool there = (uint32_t)vp < (uint32_t)a.c.n_pages;
-    l.valid = there ? max(0, min(8, nk - vk)) : 0;
-    const int64_t kpage = (uint32_t)kp < (uint32_t)a.c.n_pages ? kp : 0, vpage = there ? vp : 0;   // (any row will do)
+  // the page entries of the tile after the one whose loads are on their way
+  int32_t kp = 0, vp = 0;
+  auto load_entries = [&](int tile) {
+    kp = page_of(tile * kTile + 8 * (n16 >> 2));
+    vp = page_of(tile * kTile + 8 * G);
+  };
+  auto load_k = [&](Tile &l, int tile) {
+    const int kk = tile * kTile + 8 * (n16 >> 2), vk = tile * kTile + 8 * G;
+    const int64_t page = (uint32_t)kp < (uint32_t)a.c.n_pages ? kp : 0;   // (no page: any row will do)
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      const bf16_t *p = kbase + kpage * a.c.k_ps + (int64_t)((kk & mask) + 4 * t + (n16 & 3)) * a.c.k_rs;
+      const bf16_t *p = kbase + page * a.c.k_ps + (int64_t)((kk & mask) + 4 * t + (n16 & 3)) * a.c.k_rs;
 #pragma unroll
       for (int i = 0; i < 4; ++i) l.k[t][i] = ld16(p + 32 * i);
     }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) l.v[j] = ld16(vbase + vpage * a.c.v_ps + (int64_t)((vk & mask) + j) * a.c.v_rs);
     if constexpr (HAS_BIAS) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) l.bias[j] = vk + j < nk ? bias_row[vk + j] : 0.f;
     }
   };
+  auto load_v = [&](Tile &l, int tile) {
+    const int vk = tile * kTile + 8 * G;
+    const bool there = (uint32_t)vp < (uint32_t)a.c.n_pages;
+    const int64_t page = there ? vp : 0;
+    l.valid = there ? max(0, min(8, nk - vk)) : 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) l.v[j] = ld16(vbase + page * a.c.v_ps + (int64_t)((vk & mask) + j) * a.c.v_rs);
+  };
 
   f32x4 oacc[8];                 // lane (n, G): rows (columns of S^T) 4 G .. 4 G + 3, elements 8 n + e
   float mrun, lsum;
-  auto step = [&](Tile &l, auto careful_c, float lift) {
-    constexpr bool CAREFUL = decltype(careful_c)::value;
+  // tile t; with NEXT the loads of the wave's next one are made as its registers fall free
+  auto step = [&](Tile &l, int t, auto careful_c, auto next_c, float lift) {
+    constexpr bool CAREFUL = decltype(careful_c)::value, NEXT = decltype(next_c)::value;
     f32x4 s[2] = {};
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -281,6 +298,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_kernel(PagedAttnA
       if constexpr (HAS_BIAS) z[j] = l.bias[j] == -INFINITY ? -INFINITY : z[j];   // hidden, whatever the row holds
       most = fmaxf(most, z[j]);
     }
+    if constexpr (NEXT) load_k(l, t + kWaves);
+    __builtin_amdgcn_sched_barrier(0);
     if (__builtin_amdgcn_ballot_w64(most > mrun + (kRescaleTau - lift))) {
       const float m = fmaxf(mrun, quad_swap_max(most) + lift), f = mrun == -INFINITY ? 0.f : fast_exp2(mrun - m);
       mrun = m;
@@ -310,18 +329,17 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_kernel(PagedAttnA
       for (int j = 0; j < 8; ++j)
         if (j >= l.valid) l.v[j] = u32x4{0u, 0u, 0u, 0u};
     }
-    auto column = [&](const u32x4 (&v)[8], int e) {   // element 8 n + e of keys 8 G .. 8 G + 7
+    auto column = [&](auto word, int odd) {        // the low or high halves of word(j), j = 0 .. 7
       u32x4 c;
 #pragma unroll
-      for (int m = 0; m < 4; ++m)
-        c[m] = __builtin_amdgcn_perm(v[2 * m + 1][e >> 1], v[2 * m][e >> 1], e & 1 ? 0x07060302u : 0x05040100u);
+      for (int m = 0; m < 4; ++m) c[m] = __builtin_amdgcn_perm(word(2 * m + 1), word(2 * m), odd ? 0x07060302u : 0x05040100u);
       return __builtin_bit_cast(bf16x8, c);
     };
     const bf16x8 pa = __builtin_bit_cast(bf16x8, w0), pb = __builtin_bit_cast(bf16x8, w1);
     if constexpr (!CAREFUL) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const bf16x8 v = column(l.v, e);
+        const bf16x8 v = column([&](int j) { return (uint32_t)l.v[j][e >> 1]; }, e & 1);   // element 8 n + e of keys 8 G .. 8 G + 7
         oacc[e] = mfma16(pa, v, oacc[e]);
         if constexpr (HP == 16) oacc[e] = mfma16(pb, v, oacc[e]);
       }
@@ -333,32 +351,46 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_kernel(PagedAttnA
       };
 #pragma unroll 1
       for (int hd = 0; hd < HP; ++hd) {
-        u32x4 v[8], u[8];
+        bool sees[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          v[j] = __shfl(p[j], 16 * G + hd) == 0.f ? u32x4{0u, 0u, 0u, 0u} : l.v[j];
+        for (int j = 0; j < 8; ++j) sees[j] = __shfl(p[j], 16 * G + hd) != 0.f;
 #pragma unroll
-          for (int x = 0; x < 4; ++x) u[j][x] = finite(v[j][x]);
-        }
+        for (int x = 0; x < 4; ++x) {
+          uint32_t v[8], u[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const f32x4 o = mfma16(pb, column(u, e), mfma16(pa, column(v, e), f32x4{0.f, 0.f, 0.f, 0.f}));
+          for (int j = 0; j < 8; ++j) {
+            v[j] = sees[j] ? l.v[j][x] : 0u;
+            u[j] = finite(v[j]);
+          }
 #pragma unroll
-          for (int i = 0; i < 4; ++i) oacc[e][i] += 4 * G + i == hd ? o[i] : 0.f;
+          for (int odd = 0; odd < 2; ++odd) {
+            const f32x4 first = mfma16(pa, column([&](int j) { return v[j]; }, odd), f32x4{0.f, 0.f, 0.f, 0.f});
+            const f32x4 o = mfma16(pb, column([&](int j) { return u[j]; }, odd), first);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) oacc[2 * x + odd][i] += 4 * G + i == hd ? o[i] : 0.f;
+          }
+          __builtin_amdgcn_sched_barrier(0);
         }
       }
     }
+    if constexpr (NEXT) {
+      load_v(l, t + kWaves);
+      load_entries(t + 2 * kWaves);
+    }
+    __builtin_amdgcn_sched_barrier(0);
   };
-  auto tiles = [&](auto careful_c, float lift) {
+  Tile l;
+  auto first_loads = [&](int t) {
+    load_entries(t);
+    load_k(l, t);
+    load_v(l, t);
+    load_entries(t + kWaves);
+  };
+  auto clear = [&] {
 #pragma unroll
     for (int e = 0; e < 8; ++e) oacc[e] = f32x4{0.f, 0.f, 0.f, 0.f};
     mrun = -INFINITY;
     lsum = 0.f;
-    for (int t = t_lo + wave; t < t_hi; t += kWaves) {
-      Tile l;
-      load(l, t);
-      step(l, careful_c, lift);
-    }
   };
   // elements 8 n .. 8 n + 7 of head i, i = 0 .. 3 of the lane group that holds the head's first rows, the numbers' sums
   auto sums = [&](int i, float (&o)[8]) {
@@ -380,8 +412,20 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_kernel(PagedAttnA
       for (int i = 0; i < 4; ++i) ok &= fabsf(oacc[e][i]) < kLargeSum;
     return !__builtin_amdgcn_ballot_w64(!ok);
   };
-  tiles(std::false_type(), 0.f);
-  if (!fine()) tiles(std::true_type(), kLift);   // (a NaN that a visible key holds comes again)
+  clear();
+  int t = t_lo + wave;
+  if (t < t_hi) {
+    first_loads(t);
+    for (; t + kWaves < t_hi; t += kWaves) step(l, t, std::false_type(), std::true_type(), 0.f);
+    step(l, t, std::false_type(), std::false_type(), 0.f);
+  }
+  if (!fine()) {                                 // (a NaN that a visible key holds comes again)
+    clear();
+    for (t = t_lo + wave; t < t_hi; t += kWaves) {
+      first_loads(t);
+      step(l, t, std::true_type(), std::false_type(), kLift);
+    }
+  }
 
   // ---- the waves' results meet in LDS ----
   {
@@ -403,6 +447,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_kernel(PagedAttnA
   }
   __syncthreads();
   bf16_t *const orow = a.out + b * a.out_rs + (int64_t)h0 * kHeadDim;
+  auto put = [&](int item, float o0, float o1, float l) {   // a row that saw no key: 0
+    const float f = l == 0.f ? 0.f : 1.f / l;
+    if (item / 64 < nh)
+      *reinterpret_cast<uint32_t *>(orow + 2 * item) = l == 0.f ? 0u : pack_bf16x2(o0 * f, o1 * f);
+  };
   for (int item = tid; item < HP * kHeadDim / 2; item += 64 * kWaves) {
     const int i = item / 64, d = 2 * (item % 64);
     float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
@@ -417,17 +466,98 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_kernel(PagedAttnA
       o0 += mul_zero(f, part_o[w][i][d]);
       o1 += mul_zero(f, part_o[w][i][d + 1]);
     }
-    const float f = l == 0.f ? 0.f : 1.f / l;
-    if (i < nh)                  // a row that saw no key: 0
-      *reinterpret_cast<uint32_t *>(orow + 2 * item) = l == 0.f ? 0u : pack_bf16x2(o0 * f, o1 * f);
+    if (n_parts == 1) {
+      put(item, o0, o1, l);
+    } else {
+      // (agent-scope accesses write through and read past the XCD's L2, where a release would write all of it back)
+      const int64_t at = (int64_t)blockIdx.x * HP + i;
+      const float2 o = {o0, o1}, mlv = {m, l};
+      st_agent(a.po + at * 64 + item % 64, __builtin_bit_cast(uint64_t, o));
+      if (d == 0) st_agent(a.ml + at, __builtin_bit_cast(uint64_t, mlv));
+    }
+  }
+  if (n_parts == 1) return;
+  __shared__ int last_s;
+  uint32_t *const counter = a.counters + (int64_t)b * a.sets + set;
+  wait_all_mem();                                // this wave's stores are done
+  __syncthreads();
+  if (tid == 0)
+    last_s = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)n_parts - 1u;
+  __syncthreads();
+  if (!last_s) return;
+  if (tid == 0) st_agent(counter, 0u);
+  // ---- the last workgroup of the unit merges its chunks: four output elements per thread, every kSets-th chunk,
+  // as many loads in flight as chunks; then the sets in turn ----
+  constexpr int kThreads = 64 * kWaves, kAll = HP * 32, kItems = kAll < kThreads ? kAll : kThreads, kSets = kThreads / kItems, kAhead = 8;
+  __shared__ float set_s[kSets > 1 ? kSets - 1 : 1][6][kItems];
+  const int cs = tid / kItems;
+#pragma unroll 1
+  for (int item = tid % kItems; item < kAll; item += kItems) {
+    const int i = item / 32;
+    float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+    auto fold = [&](float mc, float lc, const float (&oc)[4]) {
+      const float mn = fmaxf(m, mc), f0 = m == -INFINITY ? 0.f : fast_exp2(m - mn), f1 = mc == -INFINITY ? 1.f : fast_exp2(mc - mn);
+      l = l * f0 + lc * f1;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = o[e] * f0 + oc[e] * f1;
+      m = mn;
+    };
+    for (int c0 = cs; c0 < n_parts; c0 += kAhead * kSets) {
+      uint64_t ml[kAhead], ow[kAhead][2];
+#pragma unroll
+      for (int r = 0; r < kAhead; ++r) {           // (every load is made, past the end the last's)
+        const int64_t at = ((int64_t)blockIdx.x + (min(c0 + r * kSets, n_parts - 1) - chunk) * a.sets) * HP + i;
+        ml[r] = ld_agent(a.ml + at);
+        ow[r][0] = ld_agent(a.po + at * 64 + 2 * (item % 32));
+        ow[r][1] = ld_agent(a.po + at * 64 + 2 * (item % 32) + 1);
+      }
+#pragma unroll
+      for (int r = 0; r < kAhead; ++r) {
+        const float2 mc = __builtin_bit_cast(float2, ml[r]), a0 = __builtin_bit_cast(float2, ow[r][0]), a1 = __builtin_bit_cast(float2, ow[r][1]);
+        const float oc[4] = {a0.x, a0.y, a1.x, a1.y};
+        if (c0 + r * kSets < n_parts && mc.y != 0.f) fold(mc.x, mc.y, oc);   // (0: saw no key)
+      }
+    }
+    if constexpr (kSets > 1) {                     // (one item per thread)
+      if (cs > 0) {
+        set_s[cs - 1][0][item] = m;
+        set_s[cs - 1][1][item] = l;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) set_s[cs - 1][2 + e][item] = o[e];
+      }
+      __syncthreads();
+      if (cs > 0) return;
+#pragma unroll
+      for (int s = 0; s < kSets - 1; ++s) {
+        const float oc[4] = {set_s[s][2][item], set_s[s][3][item], set_s[s][4][item], set_s[s][5][item]};
+        if (set_s[s][1][item] != 0.f) fold(set_s[s][0][item], set_s[s][1][item], oc);
+      }
+    }
+    put(2 * item, o[0], o[1], l);
+    put(2 * item + 1, o[2], o[3], l);
   }
 }
 
-// Query heads of a workgroup: the KV head's, up to a power of two that holds them, at most 16.
-int heads_per(int group) {
-  int hp = 1;
-  while (hp < group && hp < 16) hp *= 2;
-  return hp;
+// Workgroups of a launch: units of (sequence, kv head, head set), cut into chunks on the device.
+struct DecodePlan {
+  int hp, sets, slots, least;    // query heads of a workgroup: a power of two that holds the KV head's, at most 16
+  int64_t grid, bytes;
+};
+// The counters' region is the same for every launch, so that no launch writes partial results where another counts;
+// launches of more units cut none.
+constexpr int64_t kCounters = 1 << 14;
+DecodePlan plan_decode(int64_t num_seqs, int num_heads, int num_heads_k, int max_k) {
+  DecodePlan p;
+  const int group = num_heads / num_heads_k;
+  for (p.hp = 1; p.hp < group && p.hp < 16;) p.hp *= 2;
+  p.sets = num_heads_k * ((group + p.hp - 1) / p.hp);
+  p.slots = kPerCu * device_cus();
+  const int64_t units = num_seqs * p.sets, tiles = std::max(1, (max_k + kTile - 1) / kTile);
+  p.least = units <= kCounters ? kWaves : 1 << 22;
+  p.grid = std::min<int64_t>(units * ((tiles + p.least - 1) / p.least), units + kRounds * p.slots);
+  // counters, (max, sum), O
+  p.bytes = p.grid == units ? 0 : kCounters * 4 + (p.grid * p.hp * 8 + 255) / 256 * 256 + p.grid * p.hp * kHeadDim * 4;
+  return p;
 }
 
 }  // namespace
@@ -503,8 +633,9 @@ extern "C" int tg_paged_append(const void *qkv, int64_t qkv_row_stride, const fl
 
 extern "C" int64_t tg_paged_decode_attention_workspace_size(int32_t num_seqs, int32_t num_heads, int32_t num_heads_k,
                                                             int32_t max_seqlen_k) {
-  (void)num_seqs; (void)num_heads; (void)num_heads_k; (void)max_seqlen_k;
-  return 0;
+  if (num_seqs <= 0 || num_heads <= 0 || num_heads_k <= 0 || num_heads % num_heads_k != 0 || max_seqlen_k <= 0) return 0;
+  const int64_t fits = kCounters / plan_decode(1, num_heads, num_heads_k, 1).sets;   // sequences that may be cut
+  return plan_decode(std::min<int64_t>(num_seqs, fits), num_heads, num_heads_k, max_seqlen_k).bytes;
 }
 
 extern "C" int tg_paged_decode_attention(const void *qkv, int64_t qkv_row_stride, const float *rope, int32_t num_seqs,
@@ -565,9 +696,20 @@ extern "C" int tg_paged_decode_attention(const void *qkv, int64_t qkv_row_stride
   a.out = static_cast<bf16_t *>(out);
   a.out_rs = out_row_stride;
   a.nseq = num_seqs;
-  const int hp = heads_per(a.group);
-  a.sets = num_heads_k * ((a.group + hp - 1) / hp);
-  const dim3 grid((unsigned)(num_seqs * a.sets)), block(64 * kWaves);
+  const DecodePlan p = plan_decode(num_seqs, num_heads, num_heads_k, max_seqlen_k);
+  const int hp = p.hp;
+  a.sets = p.sets;
+  a.slots = p.slots;
+  a.least = p.least;
+  if (p.bytes > 0) {
+    TG_CHECK(workspace != nullptr && workspace_bytes >= p.bytes, "%s: needs a workspace of %lld bytes (got %lld)", what,
+             (long long)p.bytes, (long long)workspace_bytes);
+    char *ws = static_cast<char *>(workspace);
+    a.counters = reinterpret_cast<uint32_t *>(ws);
+    a.ml = reinterpret_cast<uint64_t *>(ws + kCounters * 4);
+    a.po = reinterpret_cast<uint64_t *>(ws + p.bytes - p.grid * p.hp * kHeadDim * 4);
+  }
+  const dim3 grid((unsigned)p.grid), block(64 * kWaves);
   auto launch = [&](auto hp_c) {
     constexpr int HP = decltype(hp_c)::value;
     if (bias_raw) hipLaunchKernelGGL((paged_decode_kernel<HP, true>), grid, block, 0, stream, a);
