@@ -160,6 +160,12 @@ __device__ __forceinline__ float vmax3(float a, float b, float c) {
   return d;
 }
 
+__device__ __forceinline__ float vmax3_abs(float a, float b, float c) {   // max(a, |b|, |c|)
+  float d;
+  asm("v_max3_f32 %0, %1, abs(%2), abs(%3)" : "=v"(d) : "v"(a), "v"(b), "v"(c));
+  return d;
+}
+
 // Column wave w (of the CW in a key group) owns head wave_head(w) of the workgroup's HP heads (column
 // waves 0 .. CW/2-1 the first of a pair, the others the second) at positions wave_pos(w) .. +31 of
 // the workgroup's query tile; its column block cb (0, 1) is positions 16 cb .. 16 cb + 15 of those,
@@ -219,11 +225,13 @@ __host__ __device__ __forceinline__ int combine_groups(int ns) {
   return n;
 }
 
-template <bool DEC, bool PAGED>
-using MoreArgs = std::conditional_t<DEC, DecArgs, std::conditional_t<PAGED, PagedArgs, NoDec>>;
+template <bool DEC, int PAGES>
+using MoreArgs = std::conditional_t<DEC, DecArgs, std::conditional_t<PAGES != 0, PagedArgs, NoDec>>;
 
-template <int NW, int KS, int HP, bool CAUSAL, bool HAS_BIAS, bool VARLEN, bool DEC = false, bool PAGED = false>
-__global__ __launch_bounds__(64 * NW, 8 / NW) void keybias_fwd_kernel(FwdArgs a, MoreArgs<DEC, PAGED> dec) {
+// PAGES: 0 none, 1 of 16 or 32 rows, 2 of 64 and more (a tile lies in one page).
+template <int NW, int KS, int HP, bool CAUSAL, bool HAS_BIAS, bool VARLEN, bool DEC = false, int PAGES = 0>
+__global__ __launch_bounds__(64 * NW, 8 / NW) void keybias_fwd_kernel(FwdArgs a, MoreArgs<DEC, PAGES> dec) {
+  constexpr bool PAGED = PAGES != 0;
   static_assert(!DEC || (VARLEN && NW == 4 && KS == 1), "the decode step's form");
   static_assert(!PAGED || (VARLEN && CAUSAL && KS == 1 && !DEC), "the paged form");
   constexpr int kWaves = NW;
@@ -405,6 +413,7 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void keybias_fwd_kernel(FwdArgs a,
   // A tile of SK rows is SK/4 wave-loads of 1 KB; wave w issues loads w, w + kWaves, ...
   constexpr int kLoads = kKTileBytes / 1024 / kWaves;
   uint32_t koff[kLoads], voff[kLoads];
+  [[maybe_unused]] uint32_t koff4[kLoads], voff4[kLoads];   // within the four rows of a load
 #pragma unroll
   for (int it = 0; it < kLoads; ++it) {
     const int slot = wave + it * kWaves;                  // 1 KB slot = 4 rows
@@ -414,6 +423,8 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void keybias_fwd_kernel(FwdArgs a,
     const int vkey = slot * 4 + (lane >> 4);              // V LDS row (= key) written by this lane
     const int vc = (lane & 15) ^ vswz(vkey);
     voff[it] = (uint32_t)(vkey * a.v_rs * 2 + vc * 16);
+    koff4[it] = (uint32_t)((lane >> 4) * a.k_rs * 2 + kc * 16);
+    voff4[it] = (uint32_t)((lane >> 4) * a.v_rs * 2 + vc * 16);
   }
   // Pages: the entries of the next tile to be issued, its 16-key quarters in lanes 0 .. 3 (loaded while the tile before it
   // is computed), and which quarters of the issued tile have no page.
@@ -421,30 +432,49 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void keybias_fwd_kernel(FwdArgs a,
   [[maybe_unused]] uint32_t no_page = 0;
   [[maybe_unused]] auto load_entries = [&](int tile) {
     if constexpr (PAGED)
-      entry = dec.table[b * dec.table_rs + min((tile * SK + 16 * (lane & 3)) >> dec.lg, dec.cols - 1)];
+      entry = dec.table[b * dec.table_rs + min((tile * SK + (PAGES == 1 ? 16 * (lane & 3) : 0)) >> dec.lg, dec.cols - 1)];
   };
   [[maybe_unused]] auto issue_paged = [&](int tile, auto buf_c) {
     if constexpr (PAGED) {
       char *kd = kslot(buf_c), *vd = vslot(buf_c);
-      const int wv = __builtin_amdgcn_readfirstlane(wave), mask = (1 << dec.lg) - 1;
-      // a load brings four keys, of one page, through a descriptor of exactly those that are there
-      auto rows_of = [&](const bf16_t *base, int64_t ps, int64_t rs, int key) {
-        const int32_t page = __builtin_amdgcn_readlane(entry, (key >> 4) & 3);
-        const bool there = (uint32_t)page < (uint32_t)dec.n_pages;
-        const int n = there ? max(0, min(4, sk - key)) : 0;
-        const bf16_t *p = base + (there ? page : 0) * ps + (int64_t)(key & mask) * rs;
-        return make_rsrc(p, n > 0 ? (uint32_t)((n - 1) * (int)rs + kD) * 2u : 0u);
-      };
+      const int wv = __builtin_amdgcn_readfirstlane(wave), mask = (1 << dec.lg) - 1, left = sk - tile * SK;
       const bf16_t *kh_base = a.k + (int64_t)kh * a.k_hs, *vh_base = a.v + (int64_t)kh * a.v_hs;
+      auto bytes = [&](int n, int64_t rs) { return n > 0 ? (uint32_t)((n - 1) * (int)rs + kD) * 2u : 0u; };   // of n rows
+      if constexpr (PAGES == 2) {
+        const int32_t page = __builtin_amdgcn_readfirstlane(entry);
+        const bool there = (uint32_t)page < (uint32_t)dec.n_pages;
+        const int64_t p = there ? page : 0, row = (tile * SK) & mask;
+        const int n = there ? min(left, SK) : 0;
+        const brsrc_t kr = make_rsrc(kh_base + p * dec.k_ps + row * a.k_rs, bytes(n, a.k_rs));
+        const brsrc_t vr = make_rsrc(vh_base + p * dec.v_ps + row * a.v_rs, bytes(n, a.v_rs));
+        no_page = there ? 0u : 15u;
 #pragma unroll
-      for (int it = 0; it < kLoads; ++it) {
-        const int slot = wv + it * kWaves, lr = 4 * slot + (lane >> 4);
-        dma16(rows_of(kh_base, dec.k_ps, a.k_rs, tile * SK + kperm(4 * slot)), kd + slot * 1024,
-              (uint32_t)((lane >> 4) * (int)a.k_rs * 2 + ((lane & 15) ^ (lr & 15)) * 16));
-        dma16(rows_of(vh_base, dec.v_ps, a.v_rs, tile * SK + 4 * slot), vd + slot * 1024,
-              (uint32_t)((lane >> 4) * (int)a.v_rs * 2 + ((lane & 15) ^ vswz(lr)) * 16));
+        for (int it = 0; it < kLoads; ++it) {
+          dma16(kr, kd + (wv + it * kWaves) * 1024, koff[it]);
+          dma16(vr, vd + (wv + it * kWaves) * 1024, voff[it]);
+        }
+      } else {
+        // lane q holds where quarter q begins; a load brings four keys of a quarter, through a descriptor of exactly those that
+        // are there
+        const bool there = (uint32_t)entry < (uint32_t)dec.n_pages;
+        const int64_t p = there ? entry : 0, row = (tile * SK + 16 * (lane & 3)) & mask;
+        const uint64_t ka = (uint64_t)(kh_base + p * dec.k_ps + row * a.k_rs), va = (uint64_t)(vh_base + p * dec.v_ps + row * a.v_rs);
+        no_page = (uint32_t)__builtin_amdgcn_ballot_w64(!there) & 15u;
+        auto quarter = [&](uint64_t at, int key, int64_t rs, uint32_t n_bytes) {
+          const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)at, key >> 4), hi = __builtin_amdgcn_readlane((uint32_t)(at >> 32), key >> 4);
+          return make_rsrc((const char *)(((uint64_t)hi << 32 | lo) + (uint32_t)((key & 15) * (int)rs * 2)), n_bytes);
+        };
+        auto issue = [&](auto rows) {              // rows(key): those of the four keys from `key` on that are there
+#pragma unroll
+          for (int it = 0; it < kLoads; ++it) {
+            const int slot = wv + it * kWaves, kk = kperm(4 * slot), vk = 4 * slot;
+            dma16(quarter(ka, kk, a.k_rs, bytes(rows(kk), a.k_rs)), kd + slot * 1024, koff4[it]);
+            dma16(quarter(va, vk, a.v_rs, bytes(rows(vk), a.v_rs)), vd + slot * 1024, voff4[it]);
+          }
+        };
+        if (no_page == 0 && left >= SK) issue([](int) { return 4; });
+        else issue([&](int key) { return (no_page >> (key >> 4)) & 1 ? 0 : max(0, min(4, left - key)); });
       }
-      no_page = (uint32_t)__builtin_amdgcn_ballot_w64((uint32_t)entry >= (uint32_t)dec.n_pages) & 15u;
       load_entries(tile + 1);
     }
   };
@@ -525,6 +555,10 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void keybias_fwd_kernel(FwdArgs a,
     // ---- S^T = K Q^T + bias: 2 column blocks x KB key blocks x 4 d-steps.  The accumulators start
     // from the bias of their keys (raw-score units), so the bias add costs no VALU work. ----
     f32x4 sacc[2][KB];
+    // Pages: keys that a bias of -inf hides or that have no page weigh nothing whatever their rows hold, and where a bias is
+    // as large as a mask's (2^30 and more) the weights' exponents are formed without contraction, whose rest would be
+    // a large number there.  One test per tile of the lane's 16 biases.
+    [[maybe_unused]] float big = 0.f;
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
       if constexpr (HAS_BIAS) {
@@ -535,6 +569,10 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void keybias_fwd_kernel(FwdArgs a,
         sacc[0][kb] = f32x4{0.f, 0.f, 0.f, 0.f};
       }
       sacc[1][kb] = sacc[0][kb];
+      if constexpr (PAGED && HAS_BIAS) {
+        big = vmax3_abs(big, sacc[0][kb][0], sacc[0][kb][1]);
+        big = vmax3_abs(big, sacc[0][kb][2], sacc[0][kb][3]);
+      }
     }
     // all K fragments of the wave's keys are read before the first MFMA, so LDS latency is paid once
     bf16x8 kfr[KB][4];
@@ -557,38 +595,23 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void keybias_fwd_kernel(FwdArgs a,
       }
     }
 
-    // Pages: keys that a bias of -inf hides or that have no page weigh nothing whatever their rows hold, and where a bias is
-    // as large as a mask's (2^30 and more) the weights' exponents are formed without contraction, whose rest would be
-    // a large number there.  One test per tile of the lane's 16 biases.
     [[maybe_unused]] bool far = false;
     [[maybe_unused]] uint32_t hidden = 0;   // by bit 4 kb + i
     if constexpr (PAGED) {
-      if constexpr (HAS_BIAS) {
-        const float *bp = &bslot(buf_c)[hw][8 * G];
-        f32x4 bv[KB];
+      if constexpr (HAS_BIAS) far = __builtin_amdgcn_ballot_w64(!(big < 0x1p30f)) != 0;
+      if (far || gone != 0) {
+        if constexpr (HAS_BIAS) {
+          const float *bp = &bslot(buf_c)[hw][8 * G];
 #pragma unroll
-        for (int kb = 0; kb < KB; ++kb) bv[kb] = *reinterpret_cast<const f32x4 *>(bp + 32 * (kb >> 1) + 4 * (kb & 1));
-        float big = 0.f;
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) big = fmaxf(big, fabsf(bv[kb][i]));
-        far = __builtin_amdgcn_ballot_w64(!(big < 0x1p30f)) != 0;
-        if (far) {
-#pragma unroll
-          for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) hidden |= bv[kb][i] == -INFINITY ? 1u << (4 * kb + i) : 0u;
+          for (int e = 0; e < 4 * KB; ++e)
+            hidden |= bp[32 * (e >> 3) + 4 * ((e >> 2) & 1) + (e & 3)] == -INFINITY ? 1u << e : 0u;
         }
-      }
-      if (gone) hidden |= ((gone >> (G >> 1)) & 1 ? 0xffu : 0u) | ((gone >> (2 + (G >> 1))) & 1 ? 0xff00u : 0u);
-      if (__builtin_amdgcn_ballot_w64(hidden != 0)) {
+        hidden |= ((gone >> (G >> 1)) & 1 ? 0xffu : 0u) | ((gone >> (2 + (G >> 1))) & 1 ? 0xff00u : 0u);
 #pragma unroll
         for (int cb = 0; cb < 2; ++cb)
 #pragma unroll
-          for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) sacc[cb][kb][i] = (hidden >> (4 * kb + i)) & 1 ? -INFINITY : sacc[cb][kb][i];
+          for (int e = 0; e < 4 * KB; ++e)
+            sacc[cb][e >> 2][e & 3] = (hidden >> e) & 1 ? -INFINITY : sacc[cb][e >> 2][e & 3];
       }
     }
 
@@ -694,6 +717,7 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void keybias_fwd_kernel(FwdArgs a,
     }
 
     // ---- O^T += V^T P^T: ST key steps x 8 d-blocks x 2 column blocks ----
+    auto add_values = [&](auto some_hidden) {
 #pragma unroll
     for (int st = 0; st < ST; ++st) {
       bf16x8 pb[2];
@@ -711,21 +735,27 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void keybias_fwd_kernel(FwdArgs a,
         const s16x4 lo = lds_read_tr16(vbuf + krow + vch[dblk]);
         const s16x4 hi = lds_read_tr16(vbuf + krow + 4 * kKRowBytes + vch[dblk]);
         bf16x8 vf = __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-        if constexpr (PAGED && HAS_BIAS) {
-          if (far) {   // rows that the bias hides from this wave's head: 0
-            u32x4 w = __builtin_bit_cast(u32x4, vf);
+        if constexpr (decltype(some_hidden)::value) {   // rows that the bias hides from this wave's head: 0
+          u32x4 w = __builtin_bit_cast(u32x4, vf);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const uint32_t two = hidden >> (8 * st + 2 * j);
-              w[j] &= (two & 1 ? 0u : 0xffffu) | (two & 2 ? 0u : 0xffff0000u);
-            }
-            vf = __builtin_bit_cast(bf16x8, w);
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t two = hidden >> (8 * st + 2 * j);
+            w[j] &= (two & 1 ? 0u : 0xffffu) | (two & 2 ? 0u : 0xffff0000u);
           }
+          vf = __builtin_bit_cast(bf16x8, w);
         }
 #pragma unroll
         for (int cb = 0; cb < 2; ++cb) oacc[cb][dblk] = mfma16(vf, pb[cb], oacc[cb][dblk]);
       }
     }
+    };
+    if constexpr (PAGED && HAS_BIAS) {
+      if (far) {
+        add_values(std::true_type());
+        return;
+      }
+    }
+    add_values(std::false_type());
   };
   if constexpr (PAGED) load_entries(t_lo);
   if (t_lo < t_hi) issue_tile(t_lo, std::integral_constant<int, 0>());
@@ -1063,9 +1093,9 @@ void dispatch_fwd(const FwdArgs &a, int nw, int ks, int hp, bool causal, bool ha
 #undef TG_FWD_CASE
 }
 
-template <int NW, int HP, bool HAS_BIAS>
+template <int NW, int HP, bool HAS_BIAS, int PAGES>
 void launch_paged(const FwdArgs &a, const PagedArgs &pages, int nblocks, hipStream_t stream) {
-  hipLaunchKernelGGL((keybias_fwd_kernel<NW, 1, HP, true, HAS_BIAS, true, false, true>), dim3(nblocks), dim3(64 * NW), 0,
+  hipLaunchKernelGGL((keybias_fwd_kernel<NW, 1, HP, true, HAS_BIAS, true, false, PAGES>), dim3(nblocks), dim3(64 * NW), 0,
                      stream, a, pages);
   if (a.heavy_blocks > 0) {
     const int cgroups = combine_groups(a.ns);
@@ -1742,8 +1772,10 @@ extern "C" int tg_paged_attention(const void *q, int64_t q_row_stride, int64_t q
   TG_CHECK(nblocks < (1ll << 31), "%s: grid too large", what);
   auto launch = [&](auto nw_c, auto hp_c) {
     constexpr int NW = decltype(nw_c)::value, HP = decltype(hp_c)::value;
-    if (bias_raw) launch_paged<NW, HP, true>(a, pages, (int)nblocks, stream);
-    else launch_paged<NW, HP, false>(a, pages, (int)nblocks, stream);
+    if (bias_raw && c.lg >= 6) launch_paged<NW, HP, true, 2>(a, pages, (int)nblocks, stream);
+    else if (bias_raw) launch_paged<NW, HP, true, 1>(a, pages, (int)nblocks, stream);
+    else if (c.lg >= 6) launch_paged<NW, HP, false, 2>(a, pages, (int)nblocks, stream);
+    else launch_paged<NW, HP, false, 1>(a, pages, (int)nblocks, stream);
   };
   const std::integral_constant<int, 1> one;
   const std::integral_constant<int, 2> two;

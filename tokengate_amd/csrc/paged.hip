@@ -157,6 +157,7 @@ struct PagedAttnArgs {
   uint64_t *po;                  // [workgroup][head][64]: O, pairs of fp32
 };
 
+typedef float f32x4_u __attribute__((ext_vector_type(4), aligned(4)));
 constexpr int kWaves = 4, kPerCu = 3;
 constexpr int kTile = 32;        // keys of a wave's step
 constexpr float kRescaleTau = 8.f;               // the running maximum moves only when a logit passes it by 2^8
@@ -266,8 +267,17 @@ __global__ __launch_bounds__(64 * kWaves, kPerCu) void paged_decode_kernel(Paged
       for (int i = 0; i < 4; ++i) l.k[t][i] = ld16(p + 32 * i);
     }
     if constexpr (HAS_BIAS) {
+      if (tile * kTile + kTile <= nk) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) l.bias[j] = vk + j < nk ? bias_row[vk + j] : 0.f;
+        for (int i = 0; i < 2; ++i) {
+          const f32x4_u x = *reinterpret_cast<const f32x4_u *>(bias_row + vk + 4 * i);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) l.bias[4 * i + j] = x[j];
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) l.bias[j] = vk + j < nk ? bias_row[vk + j] : 0.f;
+      }
     }
   };
   auto load_v = [&](Tile &l, int tile) {
