@@ -160,12 +160,6 @@ __device__ __forceinline__ float vmax3(float a, float b, float c) {
   return d;
 }
 
-__device__ __forceinline__ float vmax3_abs(float a, float b, float c) {   // max(a, |b|, |c|)
-  float d;
-  asm("v_max3_f32 %0, %1, abs(%2), abs(%3)" : "=v"(d) : "v"(a), "v"(b), "v"(c));
-  return d;
-}
-
 // Column wave w (of the CW in a key group) owns head wave_head(w) of the workgroup's HP heads (column
 // waves 0 .. CW/2-1 the first of a pair, the others the second) at positions wave_pos(w) .. +31 of
 // the workgroup's query tile; its column block cb (0, 1) is positions 16 cb .. 16 cb + 15 of those,
@@ -228,25 +222,34 @@ __host__ __device__ __forceinline__ int combine_groups(int ns) {
 template <bool DEC, int PAGES>
 using MoreArgs = std::conditional_t<DEC, DecArgs, std::conditional_t<PAGES != 0, PagedArgs, NoDec>>;
 
-// PAGES: 0 none, 1 of 16 or 32 rows, 2 of 64 and more (a tile lies in one page).
-template <int NW, int KS, int HP, bool CAUSAL, bool HAS_BIAS, bool VARLEN, bool DEC = false, int PAGES = 0>
-__global__ __launch_bounds__(64 * NW, 8 / NW) void keybias_fwd_kernel(FwdArgs a, MoreArgs<DEC, PAGES> dec) {
+// Ring slots in LDS.  One __shared__ object per ring slot: the compiler separates LDS-DMA writes from LDS reads only
+// across distinct objects, so the DMA of tile t+1 does not hold up the reads of tile t.
+template <int KS> constexpr int tile_bytes() { return step_keys<KS>() * kKRowBytes; }
+// bias rows padded by 4 floats so that the two heads' rows fall on different banks
+template <int KS> constexpr int bias_row() { return step_keys<KS>() + 4; }
+
+// PAGES: 0 none, 1 of 16 or 32 rows, 2 of 64 and more.
+//
+// FAR (pages) handles keys that a bias of -inf hides or that have no page, which weigh nothing whatever their rows hold,
+// and biases as large as a mask's (2^30 and more), whose logits are scaled and rounded first (in one multiply-add with the
+// scale the product's rest would be a large number there).  Without FAR a workgroup whose keys have any of these ends at
+// the first such tile, before it has written anything, and returns true.  (Both in one loop, by branches or one loop after the
+// other, kept neither the registers nor the exponentials beside the products: 2320 rows with bias 54 to 65 us.)
+template <int NW, int KS, int HP, bool CAUSAL, bool HAS_BIAS, bool VARLEN, bool DEC, int PAGES, bool FAR>
+__device__ __forceinline__ bool fwd_body(const FwdArgs &a, const MoreArgs<DEC, PAGES> &dec, char (&ks0)[tile_bytes<KS>()],
+                                         char (&ks1)[tile_bytes<KS>()], char (&vs0)[tile_bytes<KS>()],
+                                         char (&vs1)[tile_bytes<KS>()], float (&bs0)[HP][bias_row<KS>()],
+                                         float (&bs1)[HP][bias_row<KS>()], [[maybe_unused]] char *zeros) {
   constexpr bool PAGED = PAGES != 0;
   static_assert(!DEC || (VARLEN && NW == 4 && KS == 1), "the decode step's form");
-  static_assert(!PAGED || (VARLEN && CAUSAL && KS == 1 && !DEC), "the paged form");
+  static_assert(!PAGED || (VARLEN && CAUSAL && !DEC), "the paged form");
   constexpr int kWaves = NW;
   constexpr int CW = col_waves<NW, KS>();
   constexpr int BM = bm<CW, HP>();
   constexpr int KN = wave_keys<KS>(), SK = step_keys<KS>();
   constexpr int KB = KN / 16, ST = KN / 32;   // 16-key blocks and 32-key steps of a wave's keys
-  constexpr int kKTileBytes = SK * kKRowBytes;
-  // One __shared__ object per ring slot: the compiler separates LDS-DMA writes from LDS reads only
-  // across distinct objects, so the DMA of tile t+1 does not hold up the reads of tile t.
+  constexpr int kKTileBytes = tile_bytes<KS>();
   static_assert(kStages == 2, "two named LDS objects per operand");
-  __shared__ __attribute__((aligned(1024))) char ks0[kKTileBytes], ks1[kKTileBytes];
-  __shared__ __attribute__((aligned(1024))) char vs0[kKTileBytes], vs1[kKTileBytes];
-  // bias rows padded by 4 floats so that the two heads' rows fall on different banks
-  __shared__ __attribute__((aligned(256))) float bs0[HP][SK + 4], bs1[HP][SK + 4];
   auto kslot = [&](auto b) -> char * { if constexpr (decltype(b)::value == 0) return ks0; else return ks1; };
   auto vslot = [&](auto b) -> char * { if constexpr (decltype(b)::value == 0) return vs0; else return vs1; };
   auto bslot = [&](auto b) -> float (*)[SK + 4] {
@@ -291,7 +294,7 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void keybias_fwd_kernel(FwdArgs a,
   if constexpr (VARLEN && !DEC) {
     if (a.level_order) {
       const LevelTile lt = level_tile<BM>(a.cu_seqlens, a.batch, a.sq, bid / per_q, lane);
-      if (lt.seq < 0) return;   // workgroup-uniform: past the last tile
+      if (lt.seq < 0) return false;   // workgroup-uniform: past the last tile
       b = lt.seq;
       qt = lt.level;
       seq_row0 = lt.row0;
@@ -324,7 +327,7 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void keybias_fwd_kernel(FwdArgs a,
     }
   }
   const int q0 = qt * BM;
-  if (q0 >= sq) return;   // workgroup-uniform: past the end of this sequence
+  if (q0 >= sq) return false;   // workgroup-uniform: past the end of this sequence
   const int off = sk - sq;   // causal: query i sees keys j <= i + off (bottom-right aligned)
   const int h0 = kh * a.group + hg * HP;
 
@@ -385,7 +388,7 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void keybias_fwd_kernel(FwdArgs a,
   // decode: a chunk without a tile has nothing to add (the first one stands in where there is no key)
   const int n_parts = max(1, min(n_tiles, a.ns));   // chunks with a tile
   if constexpr (DEC) {
-    if (chunk >= 0 && t_lo == t_hi && (n_tiles > 0 || chunk > 0)) return;   // workgroup-uniform
+    if (chunk >= 0 && t_lo == t_hi && (n_tiles > 0 || chunk > 0)) return false;   // workgroup-uniform
   }
   // decode: a wave forms one row, 8 elements per lane (16 lanes, the four groups alike): the waves with a
   // query their head's q, waves 1 and 3 the new k and v of the last tile's workgroup
@@ -413,7 +416,6 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void keybias_fwd_kernel(FwdArgs a,
   // A tile of SK rows is SK/4 wave-loads of 1 KB; wave w issues loads w, w + kWaves, ...
   constexpr int kLoads = kKTileBytes / 1024 / kWaves;
   uint32_t koff[kLoads], voff[kLoads];
-  [[maybe_unused]] uint32_t koff4[kLoads], voff4[kLoads];   // within the four rows of a load
 #pragma unroll
   for (int it = 0; it < kLoads; ++it) {
     const int slot = wave + it * kWaves;                  // 1 KB slot = 4 rows
@@ -423,44 +425,54 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void keybias_fwd_kernel(FwdArgs a,
     const int vkey = slot * 4 + (lane >> 4);              // V LDS row (= key) written by this lane
     const int vc = (lane & 15) ^ vswz(vkey);
     voff[it] = (uint32_t)(vkey * a.v_rs * 2 + vc * 16);
-    koff4[it] = (uint32_t)((lane >> 4) * a.k_rs * 2 + kc * 16);
-    voff4[it] = (uint32_t)((lane >> 4) * a.v_rs * 2 + vc * 16);
   }
-  // Pages: the entries of the next tile to be issued, its 16-key quarters in lanes 0 .. 3 (loaded while the tile before it
-  // is computed), and which quarters of the issued tile have no page.
+  // Pages: the entries of the next tile to be issued, lane q that of its 16 keys (PAGES 2: 64) from 16 q (64 q) on, loaded while
+  // the tile before it is computed; and, by bit, which 16 keys of the issued tile have no page.
+  constexpr int kParts16 = SK / 16, kPartKeys = PAGES == 2 ? 64 : 16;
   [[maybe_unused]] int32_t entry = 0;
   [[maybe_unused]] uint32_t no_page = 0;
   [[maybe_unused]] auto load_entries = [&](int tile) {
     if constexpr (PAGED)
-      entry = dec.table[b * dec.table_rs + min((tile * SK + (PAGES == 1 ? 16 * (lane & 3) : 0)) >> dec.lg, dec.cols - 1)];
+      entry = dec.table[b * dec.table_rs + min((tile * SK + kPartKeys * (lane & (SK / kPartKeys - 1))) >> dec.lg, dec.cols - 1)];
   };
   [[maybe_unused]] auto issue_paged = [&](int tile, auto buf_c) {
     if constexpr (PAGED) {
       char *kd = kslot(buf_c), *vd = vslot(buf_c);
       const int wv = __builtin_amdgcn_readfirstlane(wave), mask = (1 << dec.lg) - 1, left = sk - tile * SK;
       const bf16_t *kh_base = a.k + (int64_t)kh * a.k_hs, *vh_base = a.v + (int64_t)kh * a.v_hs;
+      // a wave's further loads lie a whole number of rows behind its first one in K and V, at the same chunks of 16 bytes
+      static_assert(kWaves == 8 || kWaves == 4, "16 or 32 rows");
+      auto k_rows = [](int it) { return kWaves == 8 ? 32 * it : 32 * (it >> 1) + 4 * (it & 1); };
+      auto v_rows = [](int it) { return 4 * kWaves * it; };
       auto bytes = [&](int n, int64_t rs) { return n > 0 ? (uint32_t)((n - 1) * (int)rs + kD) * 2u : 0u; };   // of n rows
       if constexpr (PAGES == 2) {
-        const int32_t page = __builtin_amdgcn_readfirstlane(entry);
-        const bool there = (uint32_t)page < (uint32_t)dec.n_pages;
-        const int64_t p = there ? page : 0, row = (tile * SK) & mask;
-        const int n = there ? min(left, SK) : 0;
-        const brsrc_t kr = make_rsrc(kh_base + p * dec.k_ps + row * a.k_rs, bytes(n, a.k_rs));
-        const brsrc_t vr = make_rsrc(vh_base + p * dec.v_ps + row * a.v_rs, bytes(n, a.v_rs));
-        no_page = there ? 0u : 15u;
+        no_page = 0;
 #pragma unroll
-        for (int it = 0; it < kLoads; ++it) {
-          dma16(kr, kd + (wv + it * kWaves) * 1024, koff[it]);
-          dma16(vr, vd + (wv + it * kWaves) * 1024, voff[it]);
+        for (int i = 0; i < SK / 64; ++i) {          // loads kLoads / (SK / 64) of every 64 keys
+          const int32_t page = __builtin_amdgcn_readlane(entry, i);
+          const bool there = (uint32_t)page < (uint32_t)dec.n_pages;
+          const int64_t p = there ? page : 0, row = (tile * SK + 64 * i) & mask;
+          const int n = there ? min(left - 64 * i, 64) : 0;
+          const brsrc_t kr = make_rsrc(kh_base + p * dec.k_ps + row * a.k_rs, bytes(n, a.k_rs));
+          const brsrc_t vr = make_rsrc(vh_base + p * dec.v_ps + row * a.v_rs, bytes(n, a.v_rs));
+          no_page |= there || left <= 64 * i ? 0u : 15u << (4 * i);
+          constexpr int kOf64 = kLoads / (SK / 64);
+#pragma unroll
+          for (int it = 0; it < kOf64; ++it) {
+            dma16(kr, kd + (wv + (i * kOf64 + it) * kWaves) * 1024, koff[0] + (uint32_t)(k_rows(it) * (int)a.k_rs * 2));
+            dma16(vr, vd + (wv + (i * kOf64 + it) * kWaves) * 1024, voff[0] + (uint32_t)(v_rows(it) * (int)a.v_rs * 2));
+          }
         }
       } else {
-        // lane q holds where quarter q begins; a load brings four keys of a quarter, through a descriptor of exactly those that
+        // lane q holds where the keys from 16 q on begin; a load brings four of them, through a descriptor of exactly those that
         // are there
         const bool there = (uint32_t)entry < (uint32_t)dec.n_pages;
-        const int64_t p = there ? entry : 0, row = (tile * SK + 16 * (lane & 3)) & mask;
+        const int64_t p = there ? entry : 0, row = (tile * SK + 16 * (lane & (kParts16 - 1))) & mask;
         const uint64_t ka = (uint64_t)(kh_base + p * dec.k_ps + row * a.k_rs), va = (uint64_t)(vh_base + p * dec.v_ps + row * a.v_rs);
-        no_page = (uint32_t)__builtin_amdgcn_ballot_w64(!there) & 15u;
-        auto quarter = [&](uint64_t at, int key, int64_t rs, uint32_t n_bytes) {
+        no_page = (uint32_t)__builtin_amdgcn_ballot_w64(!there && 16 * (lane & (kParts16 - 1)) < left) & ((1u << kParts16) - 1u);
+        const uint32_t k4 = (uint32_t)((lane >> 4) * (int)a.k_rs * 2 + ((lane & 15) ^ ((4 * wave + (lane >> 4)) & 15)) * 16);
+        const uint32_t v4 = (uint32_t)((lane >> 4) * (int)a.v_rs * 2 + ((lane & 15) ^ vswz(4 * wave + (lane >> 4))) * 16);
+        auto part = [&](uint64_t at, int key, int64_t rs, uint32_t n_bytes) {
           const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)at, key >> 4), hi = __builtin_amdgcn_readlane((uint32_t)(at >> 32), key >> 4);
           return make_rsrc((const char *)(((uint64_t)hi << 32 | lo) + (uint32_t)((key & 15) * (int)rs * 2)), n_bytes);
         };
@@ -468,8 +480,8 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void keybias_fwd_kernel(FwdArgs a,
 #pragma unroll
           for (int it = 0; it < kLoads; ++it) {
             const int slot = wv + it * kWaves, kk = kperm(4 * slot), vk = 4 * slot;
-            dma16(quarter(ka, kk, a.k_rs, bytes(rows(kk), a.k_rs)), kd + slot * 1024, koff4[it]);
-            dma16(quarter(va, vk, a.v_rs, bytes(rows(vk), a.v_rs)), vd + slot * 1024, voff4[it]);
+            dma16(part(ka, kk, a.k_rs, bytes(rows(kk), a.k_rs)), kd + slot * 1024, k4);
+            dma16(part(va, vk, a.v_rs, bytes(rows(vk), a.v_rs)), vd + slot * 1024, v4);
           }
         };
         if (no_page == 0 && left >= SK) issue([](int) { return 4; });
@@ -548,17 +560,25 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void keybias_fwd_kernel(FwdArgs a,
         ring_barrier();
       }
     }
-    [[maybe_unused]] const uint32_t gone = no_page;   // of this tile
+    [[maybe_unused]] const uint32_t gone = no_page >> (KN / 16 * kg);   // of this tile, from this wave's keys on
+    if constexpr (PAGED && !FAR) {
+      bool stop = no_page != 0;
+      if constexpr (HAS_BIAS) {                    // every wave looks at all heads' biases
+        float big = 0.f;
+#pragma unroll
+        for (int i = 0; i < HP; ++i)
+#pragma unroll
+          for (int j = 0; j < SK / 64; ++j) big = fmaxf(big, fabsf(bslot(buf_c)[i][64 * j + lane]));
+        stop |= __builtin_amdgcn_ballot_w64(!(big < 0x1p30f)) != 0;
+      }
+      if (stop) return true;
+    }
     if (t + 1 < t_hi) issue_tile(t + 1, std::integral_constant<int, 1 - BUF>());
-    if (!wave_has_rows || (CAUSAL && n0 > qw_hi + off)) return;
+    if (!wave_has_rows || (CAUSAL && n0 > qw_hi + off)) return false;
 
     // ---- S^T = K Q^T + bias: 2 column blocks x KB key blocks x 4 d-steps.  The accumulators start
     // from the bias of their keys (raw-score units), so the bias add costs no VALU work. ----
     f32x4 sacc[2][KB];
-    // Pages: keys that a bias of -inf hides or that have no page weigh nothing whatever their rows hold, and where a bias is
-    // as large as a mask's (2^30 and more) the weights' exponents are formed without contraction, whose rest would be
-    // a large number there.  One test per tile of the lane's 16 biases.
-    [[maybe_unused]] float big = 0.f;
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
       if constexpr (HAS_BIAS) {
@@ -569,51 +589,54 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void keybias_fwd_kernel(FwdArgs a,
         sacc[0][kb] = f32x4{0.f, 0.f, 0.f, 0.f};
       }
       sacc[1][kb] = sacc[0][kb];
-      if constexpr (PAGED && HAS_BIAS) {
-        big = vmax3_abs(big, sacc[0][kb][0], sacc[0][kb][1]);
-        big = vmax3_abs(big, sacc[0][kb][2], sacc[0][kb][3]);
-      }
     }
-    // all K fragments of the wave's keys are read before the first MFMA, so LDS latency is paid once
+    // all K fragments of the wave's keys are read before the first MFMA, so LDS latency is paid once (FAR: registers count)
     bf16x8 kfr[KB][4];
-#pragma unroll
-    for (int ks = 0; ks < 4; ++ks) {
+    auto read_k = [&](int ks) {
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb) {
         const int lr = 16 * kb + c16;
         kfr[kb][ks] = lds_load16(kslot(buf_c) + KN * kg * kKRowBytes,
                                  lr * kKRowBytes + ((uint32_t)((4 * ks + G) ^ c16) << 4));
       }
+    };
+    if constexpr (!FAR) {
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) read_k(ks);
     }
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks) {
+      if constexpr (FAR) read_k(ks);
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb) {
 #pragma unroll
         for (int cb = 0; cb < 2; ++cb) sacc[cb][kb] = mfma16(kfr[kb][ks], qf[cb][ks], sacc[cb][kb]);
       }
+      if constexpr (FAR) __builtin_amdgcn_sched_barrier(0);
     }
 
-    [[maybe_unused]] bool far = false;
     [[maybe_unused]] uint32_t hidden = 0;   // by bit 4 kb + i
-    if constexpr (PAGED) {
-      if constexpr (HAS_BIAS) far = __builtin_amdgcn_ballot_w64(!(big < 0x1p30f)) != 0;
-      if (far || gone != 0) {
-        if constexpr (HAS_BIAS) {
-          const float *bp = &bslot(buf_c)[hw][8 * G];
+    if constexpr (FAR) {
+      if constexpr (HAS_BIAS) {
+        const float *bp = &bslot(buf_c)[hw][KN * kg + 8 * G];
 #pragma unroll
-          for (int e = 0; e < 4 * KB; ++e)
-            hidden |= bp[32 * (e >> 3) + 4 * ((e >> 2) & 1) + (e & 3)] == -INFINITY ? 1u << e : 0u;
-        }
-        hidden |= ((gone >> (G >> 1)) & 1 ? 0xffu : 0u) | ((gone >> (2 + (G >> 1))) & 1 ? 0xff00u : 0u);
-#pragma unroll
-        for (int cb = 0; cb < 2; ++cb)
-#pragma unroll
-          for (int e = 0; e < 4 * KB; ++e)
-            sacc[cb][e >> 2][e & 3] = (hidden >> e) & 1 ? -INFINITY : sacc[cb][e >> 2][e & 3];
+        for (int e = 0; e < 4 * KB; ++e)
+          hidden |= bp[32 * (e >> 3) + 4 * ((e >> 2) & 1) + (e & 3)] == -INFINITY ? 1u << e : 0u;
       }
+      hidden |= ((gone >> (G >> 1)) & 1 ? 0xffu : 0u) | ((gone >> (2 + (G >> 1))) & 1 ? 0xff00u : 0u);
+#pragma unroll
+      for (int cb = 0; cb < 2; ++cb)
+#pragma unroll
+        for (int e = 0; e < 4 * KB; ++e) {
+          const float z = sacc[cb][e >> 2][e & 3] * a.scale_log2;
+          const uint32_t sgn = (uint32_t)((int32_t)(hidden << (31 - e)) >> 31);
+          sacc[cb][e >> 2][e & 3] = u32_as_f32((sgn & 0xFF800000u) | (~sgn & __builtin_bit_cast(uint32_t, z)));
+        }
+      __builtin_amdgcn_sched_barrier(0);
     }
+    // what takes the accumulators to log2 units
+    const float to_log2 = FAR ? 1.f : a.scale_log2;
 
     // ---- online softmax: lane holds KN/4 keys of one column per block; the other keys of that
     // column sit in lanes l^16, l^32, l^48 ----
@@ -673,10 +696,10 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void keybias_fwd_kernel(FwdArgs a,
       mxr[0] = u32_as_f32(lo);
       mxr[1] = u32_as_f32(hi);
     }
-    if (__builtin_amdgcn_ballot_w64(mxr[0] > thr[0] || mxr[1] > thr[1]) != 0) {
+    if (FAR || __builtin_amdgcn_ballot_w64(mxr[0] > thr[0] || mxr[1] > thr[1]) != 0) {
 #pragma unroll
       for (int cb = 0; cb < 2; ++cb) {
-        const float m_new = fmaxf(mrun[cb], mxr[cb] * a.scale_log2);
+        const float m_new = fmaxf(mrun[cb], mxr[cb] * to_log2);
         // 0 on the first visible tile; columns that have seen no key yet (m_new = -inf) keep 1.
         const float alpha = m_new == -INFINITY ? 1.f : fast_exp2(mrun[cb] - m_new);
         mrun[cb] = m_new;
@@ -695,29 +718,13 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void keybias_fwd_kernel(FwdArgs a,
       for (int kb = 0; kb < KB; ++kb) {
 #pragma unroll
         for (int i = 0; i < 4; i += 2) {
-          const float p0 = fast_exp2(fmaf(sacc[cb][kb][i], a.scale_log2, mneg[cb]));
-          const float p1 = fast_exp2(fmaf(sacc[cb][kb][i + 1], a.scale_log2, mneg[cb]));
+          const float p0 = fast_exp2(fmaf(sacc[cb][kb][i], to_log2, mneg[cb]));
+          const float p1 = fast_exp2(fmaf(sacc[cb][kb][i + 1], to_log2, mneg[cb]));
           pk[cb][kb][i >> 1] = pack_bf16x2(p0, p1);
         }
       }
     }
-    if constexpr (PAGED && HAS_BIAS) {
-      if (far) {
-#pragma unroll
-        for (int cb = 0; cb < 2; ++cb)
-#pragma unroll
-          for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-            for (int i = 0; i < 4; i += 2) {
-              float z0 = sacc[cb][kb][i] * a.scale_log2, z1 = sacc[cb][kb][i + 1] * a.scale_log2;
-              asm("" : "+v"(z0), "+v"(z1));   // rounded, as the running maximum is
-              pk[cb][kb][i >> 1] = pack_bf16x2(fast_exp2(z0 + mneg[cb]), fast_exp2(z1 + mneg[cb]));
-            }
-      }
-    }
-
     // ---- O^T += V^T P^T: ST key steps x 8 d-blocks x 2 column blocks ----
-    auto add_values = [&](auto some_hidden) {
 #pragma unroll
     for (int st = 0; st < ST; ++st) {
       bf16x8 pb[2];
@@ -732,30 +739,20 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void keybias_fwd_kernel(FwdArgs a,
 #pragma unroll
       for (int dblk = 0; dblk < 8; ++dblk) {
         const char *vbuf = vslot(buf_c) + KN * kg * kKRowBytes;
-        const s16x4 lo = lds_read_tr16(vbuf + krow + vch[dblk]);
-        const s16x4 hi = lds_read_tr16(vbuf + krow + 4 * kKRowBytes + vch[dblk]);
-        bf16x8 vf = __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-        if constexpr (decltype(some_hidden)::value) {   // rows that the bias hides from this wave's head: 0
-          u32x4 w = __builtin_bit_cast(u32x4, vf);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const uint32_t two = hidden >> (8 * st + 2 * j);
-            w[j] &= (two & 1 ? 0u : 0xffffu) | (two & 2 ? 0u : 0xffff0000u);
-          }
-          vf = __builtin_bit_cast(bf16x8, w);
+        const char *vlo = vbuf + krow + vch[dblk], *vhi = vbuf + krow + 4 * kKRowBytes + vch[dblk];
+        if constexpr (FAR && HAS_BIAS) {   // rows that the bias hides from this wave's head read as 0
+          if ((hidden >> (8 * st + (c16 >> 2))) & 1) vlo = zeros;
+          if ((hidden >> (8 * st + 4 + (c16 >> 2))) & 1) vhi = zeros;
+          __builtin_amdgcn_sched_barrier(0);
         }
+        const s16x4 lo = lds_read_tr16(vlo);
+        const s16x4 hi = lds_read_tr16(vhi);
+        const bf16x8 vf = __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
 #pragma unroll
         for (int cb = 0; cb < 2; ++cb) oacc[cb][dblk] = mfma16(vf, pb[cb], oacc[cb][dblk]);
       }
     }
-    };
-    if constexpr (PAGED && HAS_BIAS) {
-      if (far) {
-        add_values(std::true_type());
-        return;
-      }
-    }
-    add_values(std::false_type());
+    return false;
   };
   if constexpr (PAGED) load_entries(t_lo);
   if (t_lo < t_hi) issue_tile(t_lo, std::integral_constant<int, 0>());
@@ -794,10 +791,10 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void keybias_fwd_kernel(FwdArgs a,
   }
   int t = t_lo;
   for (; t + 1 < t_hi; t += 2) {
-    tile_step(t, std::integral_constant<int, 0>());
-    tile_step(t + 1, std::integral_constant<int, 1>());
+    if (tile_step(t, std::integral_constant<int, 0>())) return true;
+    if (tile_step(t + 1, std::integral_constant<int, 1>())) return true;
   }
-  if (t < t_hi) tile_step(t, std::integral_constant<int, 0>());
+  if (t < t_hi && tile_step(t, std::integral_constant<int, 0>())) return true;
 
   // ---- merge of the KS key groups (KS > 1): a column's max over the groups, every group's row sum
   // and O rescaled to it (weight 0 where a group saw no key), then group g adds up d-blocks DB g ..
@@ -872,7 +869,7 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void keybias_fwd_kernel(FwdArgs a,
         last_s = __hip_atomic_fetch_add(dec.counters + unit, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
                  (uint32_t)n_parts - 1u;
       __syncthreads();
-      if (!last_s) return;
+      if (!last_s) return false;
       if (tid == 0) st_agent(dec.counters + unit, 0u);
       constexpr int kItems = HP * 16;   // a head's pieces of 8 O values
       __shared__ float part[kCombineMaxGroups - 1][10][kItems];
@@ -904,7 +901,7 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void keybias_fwd_kernel(FwdArgs a,
         if (cg > 0) store_fold(f, &part[cg - 1][0][item], kItems);
       }
       __syncthreads();
-      if (cg > 0) return;
+      if (cg > 0) return false;
       for (int q = 0; q < CG - 1; ++q) merge_fold(f, &part[q][0][item], kItems);
       const float s = f.wsum > 0.f ? 1.f / f.wsum : 0.f;
       bf16_t *orow = obase + (int64_t)hl * a.o_hs;
@@ -913,7 +910,7 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void keybias_fwd_kernel(FwdArgs a,
       const u32x2 y1 = {pack_bf16x2(f.acc[4] * s, f.acc[5] * s), pack_bf16x2(f.acc[6] * s, f.acc[7] * s)};
       *reinterpret_cast<u32x2 *>(orow + d0) = y0;
       *reinterpret_cast<u32x2 *>(orow + d0 + 16) = y1;
-      return;
+      return false;
     }
   } else if (chunk >= 0) {
     // partial result of this key chunk: O / l as bf16 (piece 4 cb + p holds d-blocks 2p and 2p+1 of
@@ -928,8 +925,8 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void keybias_fwd_kernel(FwdArgs a,
         const f32x4 &o0 = oacc[cb][2 * p], &o1 = oacc[cb][2 * p + 1];
         const float s = inv[cb];
         if constexpr (PAGED) {   // in fp32, the second half of a piece 64 lanes on
-          po[(8 * cb + 2 * p) * 64] = __builtin_bit_cast(u32x4, o0 * s);
-          po[(8 * cb + 2 * p + 1) * 64] = __builtin_bit_cast(u32x4, o1 * s);
+          po[(8 * cb + db0 + 2 * p) * 64] = __builtin_bit_cast(u32x4, o0 * s);
+          po[(8 * cb + db0 + 2 * p + 1) * 64] = __builtin_bit_cast(u32x4, o1 * s);
           continue;
         }
         const u32x4 w = {pack_bf16x2(o0[0] * s, o0[1] * s), pack_bf16x2(o0[2] * s, o0[3] * s),
@@ -946,7 +943,7 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void keybias_fwd_kernel(FwdArgs a,
         pml[cb * 64] = ml;
       }
     }
-    return;
+    return false;
   }
 #pragma unroll
   for (int cb = 0; cb < 2; ++cb) {
@@ -967,6 +964,26 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void keybias_fwd_kernel(FwdArgs a,
         a.lse[(int64_t)hh * a.lse_total + row0 + qrow[cb]] = lse;
       else
         a.lse[((int64_t)b * a.h + hh) * sq + qrow[cb]] = lse;
+    }
+  }
+  return false;
+}
+
+template <int NW, int KS, int HP, bool CAUSAL, bool HAS_BIAS, bool VARLEN, bool DEC = false, int PAGES = 0>
+__global__ __launch_bounds__(64 * NW, 8 / NW) void keybias_fwd_kernel(FwdArgs a, MoreArgs<DEC, PAGES> dec) {
+  __shared__ __attribute__((aligned(1024))) char ks0[tile_bytes<KS>()], ks1[tile_bytes<KS>()];
+  __shared__ __attribute__((aligned(1024))) char vs0[tile_bytes<KS>()], vs1[tile_bytes<KS>()];
+  __shared__ __attribute__((aligned(256))) float bs0[HP][bias_row<KS>()], bs1[HP][bias_row<KS>()];
+  auto run = [&](auto far_c, char *zeros) {
+    return fwd_body<NW, KS, HP, CAUSAL, HAS_BIAS, VARLEN, DEC, PAGES, decltype(far_c)::value>(a, dec, ks0, ks1, vs0, vs1, bs0, bs1,
+                                                                                              zeros);
+  };
+  if (run(std::false_type(), nullptr)) {          // workgroup-uniform
+    if constexpr (PAGES != 0) {
+      __shared__ __attribute__((aligned(16))) char zeros[16];   // what values that a bias hides are read from instead
+      if (threadIdx.x < 4) reinterpret_cast<uint32_t *>(zeros)[threadIdx.x] = 0u;
+      __syncthreads();           // every wave is done with the ring
+      run(std::true_type(), zeros);
     }
   }
 }
@@ -1093,15 +1110,31 @@ void dispatch_fwd(const FwdArgs &a, int nw, int ks, int hp, bool causal, bool ha
 #undef TG_FWD_CASE
 }
 
-template <int NW, int HP, bool HAS_BIAS, int PAGES>
+template <int NW, int KS, int HP>
 void launch_paged(const FwdArgs &a, const PagedArgs &pages, int nblocks, hipStream_t stream) {
-  hipLaunchKernelGGL((keybias_fwd_kernel<NW, 1, HP, true, HAS_BIAS, true, false, PAGES>), dim3(nblocks), dim3(64 * NW), 0,
-                     stream, a, pages);
+  constexpr int CW = col_waves<NW, KS>();
+  auto launch = [&](auto bias_c, auto pages_c) {
+    hipLaunchKernelGGL((keybias_fwd_kernel<NW, KS, HP, true, decltype(bias_c)::value, true, false, decltype(pages_c)::value>),
+                       dim3(nblocks), dim3(64 * NW), 0, stream, a, pages);
+  };
+  const std::integral_constant<int, 1> small;
+  const std::integral_constant<int, 2> large;
+  if (a.bias && pages.lg >= 6) launch(std::true_type(), large);
+  else if (a.bias) launch(std::true_type(), small);
+  else if (pages.lg >= 6) launch(std::false_type(), large);
+  else launch(std::false_type(), small);
   if (a.heavy_blocks > 0) {
     const int cgroups = combine_groups(a.ns);
-    hipLaunchKernelGGL((keybias_fwd_combine_kernel<NW, HP, true, true>), dim3((unsigned)(a.heavy_blocks / a.ns * NW * cgroups)),
+    hipLaunchKernelGGL((keybias_fwd_combine_kernel<CW, HP, true, true>), dim3((unsigned)(a.heavy_blocks / a.ns * CW * cgroups)),
                        dim3(512), 0, stream, a, cgroups);
   }
+}
+template <int HP>
+void dispatch_paged(const FwdArgs &a, const PagedArgs &pages, int nw, int ks, int nblocks, hipStream_t stream) {
+  if (nw == 4) launch_paged<4, 1, HP>(a, pages, nblocks, stream);
+  else if (ks == 1) launch_paged<8, 1, HP>(a, pages, nblocks, stream);
+  else if (ks == 2) launch_paged<8, 2, HP>(a, pages, nblocks, stream);
+  else launch_paged<8, 4, HP>(a, pages, nblocks, stream);
 }
 
 // The four forms of the kernel: waves per workgroup and key groups.  A CU holds one workgroup of eight
@@ -1217,7 +1250,7 @@ struct FwdPlan {
 // 15 %: 3000 rows over 32768 keys 760 -> 830 us, 3072 x 4096 without the mask 108 -> 117.
 // key_groups: whether ks > 1 may be taken (its last step's LDS DMA offsets reach up to 127 rows past sk and
 // must not wrap at 4 GiB).
-FwdPlan plan_dense(int hp, int sq, int sk, int64_t units, bool causal, bool splits, bool key_groups) {
+FwdPlan plan_dense(int hp, int sq, int sk, int64_t units, bool causal, bool splits, bool key_groups, int o_bytes = 128) {
   FwdPlan best;
   float best_cost = INFINITY;
   // the form with its split if wanted, and if it has one, where it costs less than the best so far and `limit`
@@ -1225,7 +1258,7 @@ FwdPlan plan_dense(int hp, int sq, int sk, int64_t units, bool causal, bool spli
     const Tiles t(f, hp, sq, sk, causal);
     SplitPlan p;
     if (split) {
-      if (splits) p = plan_split(f, t, units);
+      if (splits) p = plan_split(f, t, units, o_bytes);
       if (p.ns == 1) return false;
     }
     const float cost = launch_cost(f, t, units, p);
@@ -1271,6 +1304,13 @@ FwdPlan plan_varlen(int hp, int max_sq, int max_sk, int64_t units, bool causal, 
   plan.split = plan_split(kForms[w ? 0 : 1], w ? wide : narrow, units, o_bytes);
   if (plan.split.bytes > workspace_bytes) plan.split = SplitPlan{};
   return plan;
+}
+
+// A launch over pages: one sequence has a dense launch's forms, several a varlen one's.
+FwdPlan plan_paged(int hp, int num_seqs, int max_sq, int max_sk, int64_t units, int64_t workspace_bytes) {
+  if (num_seqs > 1) return plan_varlen(hp, max_sq, max_sk, units, true, workspace_bytes, 256);
+  const FwdPlan p = plan_dense(hp, max_sq, max_sk, units, true, true, true, 256);
+  return p.split.bytes <= workspace_bytes ? p : plan_dense(hp, max_sq, max_sk, units, true, false, true);
 }
 
 // Put a plan into the launch arguments.  Returns the grid size.
@@ -1452,6 +1492,7 @@ extern "C" int tg_keybias_fwd_noalloc(const void *q, const void *k, const void *
 
 namespace tg {
 namespace {
+int lo_env = -1;
 // Workgroups of a varlen launch, its plan and the order of its tiles put into the arguments.
 //
 // Sequence-major where level order has nothing to give.  Where every tile has a CU of its own the order decides
@@ -1466,11 +1507,12 @@ int64_t varlen_grid(FwdArgs &a, const FwdPlan &plan, int64_t units, void *worksp
                     int64_t key_rows) {
   const int64_t nblocks = apply_plan(a, plan, units, workspace);
   const int hp = a.group % 2 == 0 ? 2 : 1;
-  const int64_t level_blocks = level_tiles(a.batch, total_q, plan.nw * 32 / hp) * (a.h / hp);
+  const int64_t level_blocks = level_tiles(a.batch, total_q, plan.nw / plan.ks * 32 / hp) * (a.h / hp);
   const bool own_cu = level_blocks <= device_cus();
   const bool few_even_tiles = a.n_qtiles < 4 && total_q == (int64_t)a.batch * a.sq;
   a.level_order = a.n_heavy == 0 && a.n_qtiles > 1 && !own_cu && !few_even_tiles &&
                   varlen_level_order(causal, a.batch, key_rows, a.hkv);
+  if (lo_env >= 0 && a.n_heavy == 0) a.level_order = lo_env;
   return a.level_order ? level_blocks : nblocks;
 }
 
@@ -1716,7 +1758,7 @@ extern "C" int64_t tg_paged_attention_workspace_size(int32_t num_seqs, int32_t m
   if (num_seqs <= 0 || max_seqlen_q <= 0 || max_seqlen_k <= 0 || num_heads <= 0 || num_heads_k <= 0 || num_heads % num_heads_k != 0)
     return 0;
   const int hp = (num_heads / num_heads_k) % 2 == 0 ? 2 : 1;
-  return plan_varlen(hp, max_seqlen_q, max_seqlen_k, (int64_t)num_seqs * (num_heads / hp), true, INT64_MAX, 256).split.bytes;
+  return plan_paged(hp, num_seqs, max_seqlen_q, max_seqlen_k, (int64_t)num_seqs * (num_heads / hp), INT64_MAX).split.bytes;
 }
 
 extern "C" int tg_paged_attention(const void *q, int64_t q_row_stride, int64_t q_head_stride, const void *k_pages,
@@ -1764,27 +1806,18 @@ extern "C" int tg_paged_attention(const void *q, int64_t q_row_stride, int64_t q
   a.batch = num_seqs; a.sq = max_seqlen_q; a.sk = max_seqlen_k;
   a.h = num_heads; a.hkv = num_heads_k; a.group = num_heads / num_heads_k;
   a.scale_log2 = softmax_scale * kLog2e;
+  if (const char *e = getenv("TG_LO")) lo_env = atoi(e); else lo_env = -1;
   const PagedArgs pages{page_table, table_stride, c.k_ps, c.v_ps, table_cols, c.lg, c.n_pages};
   const int hp = a.group % 2 == 0 ? 2 : 1;
   const int64_t units = (int64_t)num_seqs * (num_heads / hp);
-  const FwdPlan plan = plan_varlen(hp, max_seqlen_q, max_seqlen_k, units, true, workspace ? workspace_bytes : 0, 256);
+  FwdPlan plan = plan_paged(hp, num_seqs, max_seqlen_q, max_seqlen_k, units, workspace ? workspace_bytes : 0);
+  if (const char *e = getenv("TG_NW")) { plan = FwdPlan{}; plan.nw = atoi(e); plan.ks = atoi(getenv("TG_KS")); plan.n_qtiles = Tiles(kForms[plan.nw == 4 ? 1 : plan.ks == 1 ? 0 : plan.ks == 2 ? 2 : 3], hp, max_seqlen_q, max_seqlen_k, true).n_qtiles;
+    if (const char *x = getenv("TG_NS")) { const Form &f = kForms[plan.nw == 4 ? 1 : plan.ks == 1 ? 0 : plan.ks == 2 ? 2 : 3]; plan.split.ns = atoi(x); plan.split.n_heavy = plan.n_qtiles; plan.split.heavy_units = plan.n_qtiles * units; plan.split.o_bytes = 256; plan.split.bytes = plan.split.heavy_units * plan.split.ns * (f.nw / f.ks) * 64 * 272; 
+      static void *big = nullptr; if (!big) hipMalloc(&big, 4ll << 30); workspace = big; } }
   const int64_t nblocks = varlen_grid(a, plan, units, workspace, true, total_q, (int64_t)num_seqs * max_seqlen_k);
   TG_CHECK(nblocks < (1ll << 31), "%s: grid too large", what);
-  auto launch = [&](auto nw_c, auto hp_c) {
-    constexpr int NW = decltype(nw_c)::value, HP = decltype(hp_c)::value;
-    if (bias_raw && c.lg >= 6) launch_paged<NW, HP, true, 2>(a, pages, (int)nblocks, stream);
-    else if (bias_raw) launch_paged<NW, HP, true, 1>(a, pages, (int)nblocks, stream);
-    else if (c.lg >= 6) launch_paged<NW, HP, false, 2>(a, pages, (int)nblocks, stream);
-    else launch_paged<NW, HP, false, 1>(a, pages, (int)nblocks, stream);
-  };
-  const std::integral_constant<int, 1> one;
-  const std::integral_constant<int, 2> two;
-  const std::integral_constant<int, 4> four;
-  const std::integral_constant<int, 8> eight;
-  if (plan.nw == 4 && hp == 2) launch(four, two);
-  else if (plan.nw == 4) launch(four, one);
-  else if (hp == 2) launch(eight, two);
-  else launch(eight, one);
+  if (hp == 2) dispatch_paged<2>(a, pages, plan.nw, plan.ks, (int)nblocks, stream);
+  else dispatch_paged<1>(a, pages, plan.nw, plan.ks, (int)nblocks, stream);
   TG_HIP_CHECK(hipPeekAtLastError());
   return 0;
 }
