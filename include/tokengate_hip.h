@@ -523,8 +523,8 @@ int tg_paged_append(const void *qkv, int64_t qkv_row_stride, const float *rope, 
  * only comes before have to be finite.  Weights in bf16, fp32 sums; workspace: tg_paged_attention_workspace_size bytes
  * for the key-range split of small launches (NULL or fewer bytes: no split), contents need no initialisation, shared by
  * stream-ordered calls.  max_seqlen_k < 2^24 and at most table_cols * page_rows. */
-int64_t tg_paged_attention_workspace_size(int32_t num_seqs, int32_t max_seqlen_q, int32_t max_seqlen_k, int32_t num_heads,
-                                          int32_t num_heads_k);
+int64_t tg_paged_attention_workspace_size(int32_t num_seqs, int32_t max_seqlen_q, int32_t max_seqlen_k, int32_t total_q,
+                                          int32_t num_heads, int32_t num_heads_k);
 int tg_paged_attention(const void *q, int64_t q_row_stride, int64_t q_head_stride, const void *k_pages,
                        int64_t k_page_stride, int64_t k_head_stride, int64_t k_row_stride, const void *v_pages,
                        int64_t v_page_stride, int64_t v_head_stride, int64_t v_row_stride, int32_t num_pages,

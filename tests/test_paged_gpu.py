@@ -273,12 +273,13 @@ def test_attention_masks_of_large_numbers(low):
     _attention([40], [150], 16, 8, 64, bias=bias, average=average)
 
 
-def test_attention_equals_contiguous():
-    """The bits of varlen_kv_attention where neither is split."""
+def test_attention_near_contiguous():
+    """varlen_kv_attention's outputs: both are within the tolerance of float64 (their key groups and chunks, and so the order
+    of their sums, may differ)."""
     from tokengate_amd import decoder as dec
     from tokengate_amd import paged as P
     g = _gen(3)
-    H, Hkv, page, new, used = 16, 8, 16, [200, 1300, 33], [900, 1300, 80]    # 504 workgroups: not split
+    H, Hkv, page, new, used = 16, 8, 16, [200, 1300, 33], [900, 1300, 80]
     table, n = table_of(g, used, page)
     cache = cache_of(g, n, Hkv, page)
     cu = _i32([0, 200, 1500, 1533])
@@ -290,7 +291,12 @@ def test_attention_equals_contiguous():
     q = normal(g, 1533, H, D)
     for bias in (None, _normal_bias(g, 3, H, 1300)):
         got = P.paged_attention(q, cache, table, cu, _i32(used), 1300, 1300, SCALE, bias)
-        assert torch.equal(got, dec.varlen_kv_attention(q, k, v, cu, start, _i32(used), 1300, 1300, SCALE, bias))
+        two = dec.varlen_kv_attention(q, k, v, cu, start, _i32(used), 1300, 1300, SCALE, bias)
+        for b, (m, u) in enumerate(zip(new, used)):
+            rows = slice(int(cu[b]), int(cu[b]) + m)
+            ref, mass = attend(q[rows], *keys_of(cache, table, b, u), SCALE, None if bias is None else bias[b, :, :u], u - m)
+            near(got[rows], ref, mass, BF)
+            near(two[rows], ref, mass, BF)
 
 
 # ---- one new token per sequence ---------------------------------------------------------------------------------------

@@ -74,7 +74,7 @@ SIGNATURES = {
     "tg_paged_begin": [vp, i64, vp, vp, vp, i32, vp, i64, i32, i32, i32, vp, vp, vp],
     "tg_paged_append": [vp, i64, vp, i64, i32, i32, i32, vp, vp, f32, vp, vp, vp, i64, i64, vp, vp, i64, i64, i64,
                         vp, i64, i64, i64, i32, i32, vp],
-    "tg_paged_attention_workspace_size": [i32, i32, i32, i32, i32],
+    "tg_paged_attention_workspace_size": [i32, i32, i32, i32, i32, i32],
     "tg_paged_attention": [vp, i64, i64, vp, i64, i64, i64, vp, i64, i64, i64, i32, i32, vp, i64, i32, vp, vp, i32, i32,
                            i32, i32, i32, i32, i32, vp, i64, i64, f32, vp, i64, i64, vp, i64, vp],
     "tg_paged_decode_attention_workspace_size": [i32, i32, i32, i32],

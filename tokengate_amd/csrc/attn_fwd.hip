@@ -118,7 +118,40 @@ struct PagedArgs {
   const int32_t *table;
   int64_t table_rs, k_ps, v_ps;
   int cols, lg, n_pages;
+  int order_chunk;   // tiles by the keys they read (key_tile), cut into chunks of at most so many key steps (0: FwdArgs' order)
 };
+
+// The tiles of n <= 64 sequences by the keys they read, most first: at level l (ROWS keys) the tiles that end there, of every
+// sequence that has one.  Tile i of the order, for every lane of the wave alike; seq < 0 past the end.  A tile's work is its
+// keys, which in a launch of prompt parts differ by the sequences' lengths, so that in a sequence's own order the
+// longest may begin last.
+struct KeyTile {
+  int seq, qt, row0, sq, sk;
+};
+template <int ROWS>
+__device__ __forceinline__ KeyTile key_tile(const int32_t *cu, const int32_t *used, int n, int max_q, int max_k, int i, int lane) {
+  const int row0 = lane < n ? cu[lane] : 0, sq = lane < n ? max(0, min(cu[lane + 1] - row0, max_q)) : 0;
+  const int sk = lane < n ? max(0, min(used[lane], max_k)) : 0;
+  const int nt = (sq + ROWS - 1) / ROWS, top = max(nt, (sk + ROWS - 1) / ROWS);
+  auto from = [&](int l) { return __builtin_amdgcn_readfirstlane(wave_sum_int(min(nt, max(0, top - l)))); };   // at level l and above
+  if (i >= from(0)) return KeyTile{-1, 0, 0, 0, 0};
+  int level = 0, hi = (max(max_q, max_k) + ROWS - 1) / ROWS, above = 0;   // from(level) > i >= above = from(hi)
+  while (hi - level > 1) {
+    const int mid = (level + hi) >> 1, t = from(mid);
+    if (t > i) {
+      level = mid;
+    } else {
+      hi = mid;
+      above = t;
+    }
+  }
+  const bool here = top > level && top - nt <= level;
+  const uint64_t m = __builtin_amdgcn_ballot_w64(here);
+  const int place = __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
+  const int s = (int)__builtin_ctzll(__builtin_amdgcn_ballot_w64(here && place == i - above));
+  return KeyTile{s, __builtin_amdgcn_readlane(nt, s) - (__builtin_amdgcn_readlane(top, s) - level),
+                 __builtin_amdgcn_readlane(row0, s), __builtin_amdgcn_readlane(sq, s), __builtin_amdgcn_readlane(sk, s)};
+}
 template <typename T>
 __device__ __forceinline__ void st_agent(T *p, T v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 template <typename T>
@@ -291,6 +324,8 @@ __device__ __forceinline__ bool fwd_body(const FwdArgs &a, const MoreArgs<DEC, P
   }
   int qt = a.n_qtiles - 1 - rank;
   [[maybe_unused]] int seq_row0 = 0, seq_len = 0;
+  [[maybe_unused]] bool by_keys = false;
+  if constexpr (PAGED) by_keys = dec.order_chunk > 0;
   if constexpr (VARLEN && !DEC) {
     if (a.level_order) {
       const LevelTile lt = level_tile<BM>(a.cu_seqlens, a.batch, a.sq, bid / per_q, lane);
@@ -299,6 +334,16 @@ __device__ __forceinline__ bool fwd_body(const FwdArgs &a, const MoreArgs<DEC, P
       qt = lt.level;
       seq_row0 = lt.row0;
       seq_len = lt.len;
+    } else if (by_keys) {
+      chunk = bid / per_q % a.ns;
+      const int i = bid / per_q / a.ns;
+      const KeyTile kt = key_tile<BM>(a.cu_seqlens, a.used_k, a.batch, a.sq, a.sk, i, lane);
+      if (kt.seq < 0) return false;
+      b = kt.seq;
+      qt = kt.qt;
+      seq_row0 = kt.row0;
+      seq_len = kt.sq;
+      hunit = (int64_t)i * per_q + x;
     } else {
       seq_row0 = a.cu_seqlens[b];
       seq_len = min(a.cu_seqlens[b + 1] - seq_row0, a.sq);   // rows past max_seqlen have no bias: not computed
@@ -381,9 +426,17 @@ __device__ __forceinline__ bool fwd_body(const FwdArgs &a, const MoreArgs<DEC, P
   const int n_tiles = kv_end > 0 ? (kv_end + SK - 1) / SK : 0;
   // key tiles [t_lo, t_hi) of this workgroup (a split tile's chunk covers its share of them)
   int t_lo = 0, t_hi = n_tiles;
+  int n_chunks = a.ns;
+  if constexpr (PAGED) {
+    if (by_keys) {
+      n_chunks = min(a.ns, max(1, (n_tiles + dec.order_chunk - 1) / dec.order_chunk));
+      if (chunk >= n_chunks) return false;         // workgroup-uniform
+      if (n_chunks == 1) chunk = -1;
+    }
+  }
   if (chunk >= 0) {
-    t_lo = (int)((int64_t)n_tiles * chunk / a.ns);
-    t_hi = (int)((int64_t)n_tiles * (chunk + 1) / a.ns);
+    t_lo = (int)((int64_t)n_tiles * chunk / n_chunks);
+    t_hi = (int)((int64_t)n_tiles * (chunk + 1) / n_chunks);
   }
   // decode: a chunk without a tile has nothing to add (the first one stands in where there is no key)
   const int n_parts = max(1, min(n_tiles, a.ns));   // chunks with a tile
@@ -924,6 +977,7 @@ __device__ __forceinline__ bool fwd_body(const FwdArgs &a, const MoreArgs<DEC, P
       for (int p = 0; p < DB / 2; ++p) {
         const f32x4 &o0 = oacc[cb][2 * p], &o1 = oacc[cb][2 * p + 1];
         const float s = inv[cb];
+        if (PAGED && !qvalid[cb]) continue;        // (the combine kernel reads valid rows only)
         if constexpr (PAGED) {   // in fp32, the second half of a piece 64 lanes on
           po[(8 * cb + db0 + 2 * p) * 64] = __builtin_bit_cast(u32x4, o0 * s);
           po[(8 * cb + db0 + 2 * p + 1) * 64] = __builtin_bit_cast(u32x4, o1 * s);
@@ -993,8 +1047,9 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void keybias_fwd_kernel(FwdArgs a,
 // tile; per piece, thread (group cg, lane) folds chunks cg, cg + CG, ... of its column and group 0
 // merges the CG partial results through LDS, so that a long chunk list (a decode row over a long
 // cache) is walked CG ways in parallel.
-template <int CW, int HP, bool VARLEN, bool PAGED = false>   // PAGED: partial results in fp32, no LSE
-__global__ __launch_bounds__(512) void keybias_fwd_combine_kernel(FwdArgs a, int CG) {
+// PAGED: partial results in fp32, no LSE; step: keys of a step
+template <int CW, int HP, bool VARLEN, bool PAGED = false, int step = 64>
+__global__ __launch_bounds__(512) void keybias_fwd_combine_kernel(FwdArgs a, int CG, int order_chunk) {
   constexpr int BM = bm<CW, HP>();
   // (m, wsum, acc[8]) of groups 1..CG-1 of each piece: PP * (CG - 1) < 8 slots
   __shared__ float part[kCombineMaxGroups - 1][10][64];
@@ -1011,12 +1066,22 @@ __global__ __launch_bounds__(512) void keybias_fwd_combine_kernel(FwdArgs a, int
   const int per_q = a.hkv * (a.group / HP);
   const int x = (int)(hunit % per_q), r2 = (int)(hunit / per_q);
   const int kh = x % a.hkv, hg = x / a.hkv;
-  const int b = VARLEN ? r2 / a.n_heavy : r2 % a.batch;
-  const int rank = VARLEN ? r2 % a.n_heavy : r2 / a.batch;
-  const int qt = a.n_qtiles - 1 - rank;
-  int sq = a.sq;
+  // (n_heavy 0: tiles by their keys)
+  const int b = VARLEN ? r2 / max(1, a.n_heavy) : r2 % a.batch;
+  const int rank = VARLEN ? r2 % max(1, a.n_heavy) : r2 / a.batch;
+  int qt = a.n_qtiles - 1 - rank;
+  int sq = a.sq, n_chunks = a.ns;
   int64_t row0 = 0;
-  if constexpr (VARLEN) {
+  if (PAGED && order_chunk > 0) {
+    const KeyTile kt = key_tile<BM>(a.cu_seqlens, a.used_k, a.batch, a.sq, a.sk, r2, lane);
+    if (kt.seq < 0) return;
+    row0 = kt.row0;
+    sq = kt.sq;
+    qt = kt.qt;
+    const int kv_end = min(kt.sk, (qt + 1) * BM + kt.sk - sq), n_tiles = kv_end > 0 ? (kv_end + step - 1) / step : 0;
+    n_chunks = min(a.ns, max(1, (n_tiles + order_chunk - 1) / order_chunk));
+    if (n_chunks == 1) return;   // written by the forward
+  } else if constexpr (VARLEN) {
     const int s0 = a.cu_seqlens[b], s1 = a.cu_seqlens[b + 1];
     row0 = s0;
     sq = min(s1 - s0, a.sq);
@@ -1033,7 +1098,7 @@ __global__ __launch_bounds__(512) void keybias_fwd_combine_kernel(FwdArgs a, int
   Fold f;
   if (valid) {
 #pragma unroll 4
-    for (int c = cg; c < a.ns; c += CG) {
+    for (int c = cg; c < n_chunks; c += CG) {
       const int64_t pw = pw0 + (int64_t)c * CW;
       const float2 mc = ml[pw * 128 + cb * 64 + lane];
       if constexpr (PAGED) {
@@ -1081,7 +1146,7 @@ void launch_fwd(const FwdArgs &a, int nblocks, hipStream_t stream) {
     const int cgroups = combine_groups(a.ns);   // workgroups of 512 threads per (split tile, column wave)
     const int64_t blocks = a.heavy_blocks / a.ns * CW * cgroups;
     hipLaunchKernelGGL((keybias_fwd_combine_kernel<CW, HP, VARLEN>), dim3((unsigned)blocks), dim3(512), 0, stream, a,
-                       cgroups);
+                       cgroups, 0);
   }
 }
 
@@ -1123,10 +1188,11 @@ void launch_paged(const FwdArgs &a, const PagedArgs &pages, int nblocks, hipStre
   else if (a.bias) launch(std::true_type(), small);
   else if (pages.lg >= 6) launch(std::false_type(), large);
   else launch(std::false_type(), small);
-  if (a.heavy_blocks > 0) {
+  if (a.ns > 1) {
     const int cgroups = combine_groups(a.ns);
-    hipLaunchKernelGGL((keybias_fwd_combine_kernel<CW, HP, true, true>), dim3((unsigned)(a.heavy_blocks / a.ns * CW * cgroups)),
-                       dim3(512), 0, stream, a, cgroups);
+    const int64_t split = (pages.order_chunk > 0 ? nblocks : a.heavy_blocks) / a.ns;
+    hipLaunchKernelGGL((keybias_fwd_combine_kernel<CW, HP, true, true, step_keys<KS>()>), dim3((unsigned)(split * CW * cgroups)),
+                       dim3(512), 0, stream, a, cgroups, pages.order_chunk);
   }
 }
 template <int HP>
@@ -1236,6 +1302,7 @@ float launch_cost(const Form &f, const Tiles &t, int64_t units, const SplitPlan 
 struct FwdPlan {
   int nw = 8, ks = 1, n_qtiles = 0;
   SplitPlan split;
+  int order_chunk = 0;   // pages: tiles by the keys they read, in chunks of so many steps (heavy_units: tiles)
 };
 
 // A dense launch's form and split.  Without key groups: eight waves where the grid gives at least two
@@ -1306,11 +1373,55 @@ FwdPlan plan_varlen(int hp, int max_sq, int max_sk, int64_t units, bool causal, 
   return plan;
 }
 
-// A launch over pages: one sequence has a dense launch's forms, several a varlen one's.
-FwdPlan plan_paged(int hp, int num_seqs, int max_sq, int max_sk, int64_t units, int64_t workspace_bytes) {
-  if (num_seqs > 1) return plan_varlen(hp, max_sq, max_sk, units, true, workspace_bytes, 256);
-  const FwdPlan p = plan_dense(hp, max_sq, max_sk, units, true, true, true, 256);
-  return p.split.bytes <= workspace_bytes ? p : plan_dense(hp, max_sq, max_sk, units, true, false, true);
+// A launch over pages.  One sequence has a dense launch's forms.  Up to 64 take their tiles by the keys they read (key_tile), in
+// the form, and cut into as many chunks, as an estimate finds quickest: the longest chunk, or the steps spread over the places
+// (the lengths behind the maxima are not known here: of a ragged batch's tiles 0.85 of the most, in 0.6 ns + 0.5 chunks),
+// and for chunks the second launch and its traffic, and, as two that share a CU end long before others do where they all fit at
+// once, 0.45 of one more round: 8 of 200 and 12000 165 us in 4 chunks, 122 in 8).  Sequences with many tiles each whose K/V outgrow the last-level
+// cache keep their own order (varlen_level_order's reason).
+// us of the varlen launch's plan / this one / the quickest of 16 forms with up to 32 chunks, 16 / 8 heads, ragged sequences x
+// rows x keys up to: 12 x 700 x 4099 225 / 178 / 161; 8 x 200 x 12000 177 / 122 / 115; 24 x 100 x 1500 50 / 35 / 35; 3 x 2500 x 8000
+// 305 / 235 / 216; 8 x 1000 x 1000 39 / 35 / 35; 4 x 512 x 512 25 / 18 / 18; 16 x 16 x 4000 43 / 41 / 41; 4 x 64 x 8000 34 / 38 / 34.
+FwdPlan plan_paged(int hp, int num_seqs, int max_sq, int max_sk, int64_t total_q, int num_heads, int num_heads_k,
+                   int64_t workspace_bytes) {
+  const int64_t heads = num_heads / hp, units = num_seqs * heads;
+  if (num_seqs == 1) {
+    const FwdPlan p = plan_dense(hp, max_sq, max_sk, units, true, true, true, 256);
+    return p.split.bytes <= workspace_bytes ? p : plan_dense(hp, max_sq, max_sk, units, true, false, true);
+  }
+  const int wide_tiles = Tiles(kForms[0], hp, max_sq, max_sk, true).n_qtiles;
+  if (num_seqs > 64 || (wide_tiles >= 8 && !varlen_small(num_seqs, (int64_t)num_seqs * max_sk, num_heads_k)))
+    return plan_varlen(hp, max_sq, max_sk, units, true, workspace_bytes, 256);
+  FwdPlan best;
+  float best_cost = INFINITY;
+  const bool ragged = total_q < (int64_t)num_seqs * max_sq;
+  for (const Form &f : kForms) {
+    if (f.ks == 4) continue;                       // never the quickest of these
+    const Tiles t(f, hp, max_sq, max_sk, true);
+    const int steps = std::max(1, (max_sk + t.step - 1) / t.step);
+    const int64_t tiles = level_tiles(num_seqs, total_q, t.bm) * heads, slots = (int64_t)device_cus() * (8 / f.nw);
+    for (int ns = 1; ns <= (f.nw == 4 ? 32 : 1) && (ns == 1 || steps >= 12 * ns); ns *= 2) {
+      const int chunk = (steps + ns - 1) / ns;
+      const int64_t bytes = ns > 1 ? tiles * ns * (f.nw / f.ks) * 64 * (256 + 2 * 8) : 0;
+      if (bytes > workspace_bytes || bytes > (256ll << 20)) break;
+      const float parts = ragged ? 0.6f * ns + 0.5f : (float)ns;   // of a tile
+      const float rounds = (float)tiles / (float)slots * (ns == 1 ? (ragged ? 0.85f : 1.f) : parts);
+      float cost = (f.full * chunk + f.group) * (ns == 1 ? std::max(1.f, rounds) : std::max(1.45f, rounds + 0.35f));
+      if (ns > 1) cost += f.combine + 2.f + (float)total_q * (float)num_heads * 1024.f * parts / 5e6f;   // written and read back at 5 TB/s
+      if (cost < best_cost) {
+        best_cost = cost;
+        best.nw = f.nw;
+        best.ks = f.ks;
+        best.n_qtiles = t.n_qtiles;
+        best.split.ns = ns;
+        best.split.heavy_units = tiles;
+        best.split.bytes = bytes;
+        best.split.o_bytes = 256;
+        best.order_chunk = chunk;
+      }
+    }
+  }
+  return best;
 }
 
 // Put a plan into the launch arguments.  Returns the grid size.
@@ -1492,7 +1603,6 @@ extern "C" int tg_keybias_fwd_noalloc(const void *q, const void *k, const void *
 
 namespace tg {
 namespace {
-int lo_env = -1;
 // Workgroups of a varlen launch, its plan and the order of its tiles put into the arguments.
 //
 // Sequence-major where level order has nothing to give.  Where every tile has a CU of its own the order decides
@@ -1512,7 +1622,6 @@ int64_t varlen_grid(FwdArgs &a, const FwdPlan &plan, int64_t units, void *worksp
   const bool few_even_tiles = a.n_qtiles < 4 && total_q == (int64_t)a.batch * a.sq;
   a.level_order = a.n_heavy == 0 && a.n_qtiles > 1 && !own_cu && !few_even_tiles &&
                   varlen_level_order(causal, a.batch, key_rows, a.hkv);
-  if (lo_env >= 0 && a.n_heavy == 0) a.level_order = lo_env;
   return a.level_order ? level_blocks : nblocks;
 }
 
@@ -1754,11 +1863,11 @@ extern "C" int tg_decode_attention(const void *qkv, int64_t qkv_row_stride, cons
 }
 
 extern "C" int64_t tg_paged_attention_workspace_size(int32_t num_seqs, int32_t max_seqlen_q, int32_t max_seqlen_k,
-                                                     int32_t num_heads, int32_t num_heads_k) {
-  if (num_seqs <= 0 || max_seqlen_q <= 0 || max_seqlen_k <= 0 || num_heads <= 0 || num_heads_k <= 0 || num_heads % num_heads_k != 0)
+                                                     int32_t total_q, int32_t num_heads, int32_t num_heads_k) {
+  if (num_seqs <= 0 || max_seqlen_q <= 0 || max_seqlen_k <= 0 || total_q <= 0 || num_heads <= 0 || num_heads_k <= 0 || num_heads % num_heads_k != 0)
     return 0;
   const int hp = (num_heads / num_heads_k) % 2 == 0 ? 2 : 1;
-  return plan_paged(hp, num_seqs, max_seqlen_q, max_seqlen_k, (int64_t)num_seqs * (num_heads / hp), INT64_MAX).split.bytes;
+  return plan_paged(hp, num_seqs, max_seqlen_q, max_seqlen_k, total_q, num_heads, num_heads_k, INT64_MAX).split.bytes;
 }
 
 extern "C" int tg_paged_attention(const void *q, int64_t q_row_stride, int64_t q_head_stride, const void *k_pages,
@@ -1806,15 +1915,21 @@ extern "C" int tg_paged_attention(const void *q, int64_t q_row_stride, int64_t q
   a.batch = num_seqs; a.sq = max_seqlen_q; a.sk = max_seqlen_k;
   a.h = num_heads; a.hkv = num_heads_k; a.group = num_heads / num_heads_k;
   a.scale_log2 = softmax_scale * kLog2e;
-  if (const char *e = getenv("TG_LO")) lo_env = atoi(e); else lo_env = -1;
-  const PagedArgs pages{page_table, table_stride, c.k_ps, c.v_ps, table_cols, c.lg, c.n_pages};
+  PagedArgs pages{page_table, table_stride, c.k_ps, c.v_ps, table_cols, c.lg, c.n_pages, 0};
   const int hp = a.group % 2 == 0 ? 2 : 1;
   const int64_t units = (int64_t)num_seqs * (num_heads / hp);
-  FwdPlan plan = plan_paged(hp, num_seqs, max_seqlen_q, max_seqlen_k, units, workspace ? workspace_bytes : 0);
-  if (const char *e = getenv("TG_NW")) { plan = FwdPlan{}; plan.nw = atoi(e); plan.ks = atoi(getenv("TG_KS")); plan.n_qtiles = Tiles(kForms[plan.nw == 4 ? 1 : plan.ks == 1 ? 0 : plan.ks == 2 ? 2 : 3], hp, max_seqlen_q, max_seqlen_k, true).n_qtiles;
-    if (const char *x = getenv("TG_NS")) { const Form &f = kForms[plan.nw == 4 ? 1 : plan.ks == 1 ? 0 : plan.ks == 2 ? 2 : 3]; plan.split.ns = atoi(x); plan.split.n_heavy = plan.n_qtiles; plan.split.heavy_units = plan.n_qtiles * units; plan.split.o_bytes = 256; plan.split.bytes = plan.split.heavy_units * plan.split.ns * (f.nw / f.ks) * 64 * 272; 
-      static void *big = nullptr; if (!big) hipMalloc(&big, 4ll << 30); workspace = big; } }
-  const int64_t nblocks = varlen_grid(a, plan, units, workspace, true, total_q, (int64_t)num_seqs * max_seqlen_k);
+  const FwdPlan plan = plan_paged(hp, num_seqs, max_seqlen_q, max_seqlen_k, total_q, num_heads, num_heads_k,
+                                  workspace ? workspace_bytes : 0);
+  int64_t nblocks;
+  if (plan.order_chunk > 0) {
+    pages.order_chunk = plan.order_chunk;
+    a.ns = plan.split.ns;
+    nblocks = plan.split.heavy_units * a.ns;
+    a.ws_o = static_cast<bf16_t *>(workspace);
+    a.ws_ml = reinterpret_cast<float *>(static_cast<char *>(workspace) + nblocks * (plan.nw / plan.ks) * 64 * plan.split.o_bytes);
+  } else {
+    nblocks = varlen_grid(a, plan, units, workspace, true, total_q, (int64_t)num_seqs * max_seqlen_k);
+  }
   TG_CHECK(nblocks < (1ll << 31), "%s: grid too large", what);
   if (hp == 2) dispatch_paged<2>(a, pages, plan.nw, plan.ks, (int)nblocks, stream);
   else dispatch_paged<1>(a, pages, plan.nw, plan.ks, (int)nblocks, stream);

@@ -212,7 +212,8 @@ def paged_attention(q: torch.Tensor, cache: PagedKV, page_table: torch.Tensor, c
         return out
     table = _table(what, page_table, n, max_k, cache.page_rows, dev)
     # (the size is of the current device's launch plan, as everything of the call)
-    ws, ws_ptr, ws_bytes = _lib.fwd_workspace("tg_paged_attention_workspace_size", q.device, n, int(max_q), int(max_k), H, Hkv)
+    ws, ws_ptr, ws_bytes = _lib.fwd_workspace("tg_paged_attention_workspace_size", q.device, n, int(max_q), int(max_k), T, H,
+                                              Hkv)
     _lib.call_on(dev, "tg_paged_attention", q.data_ptr(), q.stride(0) if T > 1 else H * HEAD_DIM,
                  q.stride(1) if H > 1 else HEAD_DIM, *cache._args, *table, cu, used, n, int(max_q), int(max_k), T, H, Hkv,
                  HEAD_DIM, *bias, float(scale), out.data_ptr(), out.stride(0) if T > 1 else H * HEAD_DIM,
