@@ -64,7 +64,8 @@ constexpr int kRounds = 2;
 struct SplitRule {
   int nseq, sets;                // sequences; kv heads times head sets
   int slots, least;              // workgroups that are resident at once; fewest tiles per chunk
-};
+  float per_root = 0.f;          // if positive: least times as many as this times the root of the longest's tiles, and at
+};                               // least 3 times, where that takes all of it
 struct Chunk {
   int seq, chunk, chunks, tiles, sk;
   int64_t start;
@@ -82,6 +83,9 @@ __device__ __forceinline__ int wave_scan(int x) {   // sum over the lanes up to 
   x = scan_step<0x118, 0xf>(x);
   x = scan_step<0x142, 0xa>(x);   // row_bcast 15: the first row's sum to the second, the third's to the fourth
   return scan_step<0x143, 0xc>(x);   // row_bcast 31: the first half's to the second
+}
+__device__ __forceinline__ int wave_max_int(int x) {   // of all lanes, in every lane (whole numbers below 2^24)
+  return (int)wave_max((float)x);
 }
 // ceil(n / T), n and T below 2^22: the quotient's float is off by less than 1 / T
 __device__ __forceinline__ int ceil_div(int n, float inv) { return (int)(((float)n - 0.5f) * inv) + 1; }
@@ -107,13 +111,23 @@ __device__ __forceinline__ Chunk find_chunk(const SplitRule &a, int q, int lane,
   };
   const float work = (float)count(1, true) * (float)a.sets, slots = (float)a.slots;
   float target = slots;
-  int T = max(a.least, (int)(work / target) + 1);
+  int least = a.least;
+  if (a.per_root > 0.f) {
+    int longest = 0;
+    for (int s0 = 0; s0 < a.nseq; s0 += 64) {
+      if (a.nseq > 64) read(s0 + lane);
+      longest = max(longest, wave_max_int(tiles));
+    }
+    if (a.nseq > 64) read(lane);
+    least = longest <= 3 * least ? max(least, longest) : least * max(1, (int)(a.per_root * __builtin_amdgcn_sqrtf((float)longest)));
+  }
+  int T = max(least, (int)(work / target) + 1);
   // (where not even an even cut of every sequence would fill one round, nothing is counted)
   for (int i = 0; i < 3 && work / (float)T + (float)a.nseq * (float)a.sets > slots; ++i) {
     const float over = (float)count(T, false) * (float)a.sets - slots;
     if (over <= 0.f) break;
     if (over > 0.75f * slots) {
-      T = max(a.least, (int)(work / (kRounds * slots)) + 1);
+      T = max(least, (int)(work / (kRounds * slots)) + 1);
       break;
     }
     target = fmaxf(target - over, 0.25f * slots);

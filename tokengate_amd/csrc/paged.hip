@@ -66,13 +66,15 @@ struct AppendArgs {
   PagePool c;
   int groups;                    // of 16 lanes per token
 };
-constexpr int kRowsPer = 4;
+constexpr int kRowsPer = 2;
 
+// (past the caches: the queries of a long prompt outgrow them, and a short one's stay in the last level)
+__device__ __forceinline__ void st16_stream(bf16_t *p, u32x4 v) { __builtin_nontemporal_store(v, reinterpret_cast<u32x4 *>(p)); }
 __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a) {
   const int j = threadIdx.x & 15;
-  const int64_t id = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
-  const int64_t t = id / a.groups;
-  const int sub = (int)(id - t * a.groups), rows = a.h + 2 * a.hkv;
+  const uint32_t id = blockIdx.x * 16 + (threadIdx.x >> 4);   // (below 2^32)
+  const int64_t t = id / (uint32_t)a.groups;
+  const int sub = (int)(id - (uint32_t)t * (uint32_t)a.groups), rows = a.h + 2 * a.hkv;
   if (t >= a.n) return;          // uniform over the 16 lanes
   const bf16_t *src = a.qkv + t * a.qkv_rs + 8 * j;
   u32x4 raw[kRowsPer];
@@ -99,7 +101,7 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a) {
     const int r = sub + i * a.groups;
     if (r >= rows) break;
     if (r >= a.h + a.hkv) {      // a value
-      if (keep) st16(a.c.v + page * a.c.v_ps + (r - a.h - a.hkv) * a.c.v_hs + off * a.c.v_rs + 8 * j, raw[i]);
+      if (keep) st16_stream(a.c.v + page * a.c.v_ps + (r - a.h - a.hkv) * a.c.v_hs + off * a.c.v_rs + 8 * j, raw[i]);
       continue;
     }
     const bool is_q = r < a.h;
@@ -109,8 +111,8 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a) {
     const float hs = is_q ? (float)(__bf16)((a.q_head_scale ? a.q_head_scale[r] : 1.f) * (a.q_row_scale ? a.q_row_scale[t] : 1.f))
                           : 1.f;
     norm_rope8(x, wf, a.eps, cs, j, hs, y);
-    if (is_q) st16(a.q + t * a.q_rs + r * a.q_hs + 8 * j, pack8(y));
-    else if (keep) st16(a.c.k + page * a.c.k_ps + (r - a.h) * a.c.k_hs + off * a.c.k_rs + 8 * j, pack8(y));
+    if (is_q) st16_stream(a.q + t * a.q_rs + r * a.q_hs + 8 * j, pack8(y));
+    else if (keep) st16_stream(a.c.k + page * a.c.k_ps + (r - a.h) * a.c.k_hs + off * a.c.k_rs + 8 * j, pack8(y));
   }
 }
 
@@ -152,12 +154,15 @@ struct PagedAttnArgs {
   int64_t out_rs;
   int nseq, sets;                // kv heads times head sets
   int slots, least;              // workgroups that are resident at once; fewest tiles per chunk
+  float per_root;                // and as many for the root of the longest's tiles
   uint32_t *counters;            // per unit: chunks arrived; zero between launches
   uint64_t *ml;                  // [workgroup][head]: running max (log2 units) and sum
   uint64_t *po;                  // [workgroup][head][64]: O, pairs of fp32
 };
 
 typedef float f32x4_u __attribute__((ext_vector_type(4), aligned(4)));
+// Waves of a workgroup, and workgroups that a CU holds.  4 / 8 / 12 waves (3 / 1 / 1 workgroups), 16 / 8 heads: one sequence of
+// 32 keys 5.8 / 7.0 / 7.2 us, 2320 10.2 / 12.8 / 13.3, 32769 31 / 32 / 33, 64 of 300 16.5 / 22.5 / 24.2, 64 x 4096 183 / 184 / 185.
 constexpr int kWaves = 4, kPerCu = 3;
 constexpr int kTile = 32;        // keys of a wave's step
 constexpr float kRescaleTau = 8.f;               // the running maximum moves only when a logit passes it by 2^8
@@ -173,7 +178,7 @@ __global__ __launch_bounds__(64 * kWaves, kPerCu) void paged_decode_kernel(Paged
   __shared__ __attribute__((aligned(16))) bf16_t new_x[2][kHeadDim];   // the new key and value
   __shared__ __attribute__((aligned(16))) float part_o[kWaves + 1][HP][kHeadDim], part_ml[kWaves + 1][HP][2];
 
-  const Chunk ck = find_chunk<kTile>({a.nseq, a.sets, a.slots, a.least}, blockIdx.x / a.sets, lane,
+  const Chunk ck = find_chunk<kTile>({a.nseq, a.sets, a.slots, a.least, a.per_root}, blockIdx.x / a.sets, lane,
                                      [&](int s) { return Keys{0, max(0, min(a.used[s], a.max_k))}; });
   if (ck.seq < 0) return;                        // workgroup-uniform: past the last chunk
   const int b = ck.seq, sk = ck.sk, nk = max(0, sk - 1);   // keys in the pages; the new one is apart
@@ -182,67 +187,30 @@ __global__ __launch_bounds__(64 * kWaves, kPerCu) void paged_decode_kernel(Paged
   const int32_t *const trow = a.table + b * a.table_rs;
   const int lg = a.c.lg, mask = (1 << lg) - 1;
   auto page_of = [&](int key) { return trow[min(key >> lg, a.cols - 1)]; };
-  const bool has_new = chunk == n_parts - 1 && sk > 0 && (uint32_t)page_of(nk) < (uint32_t)a.c.n_pages;
-
-  // ---- the rows to form: 16 lanes a row: query heads, then the new key and the new value ----
-  for (int r = tid >> 4; r < HP + 2; r += 4 * kWaves) {
-    if (r >= HP && !has_new) break;
+  // ---- loads of the rows to form, 16 lanes a row: query heads, then the new key and the new value.  They come before the
+  // tiles': loads complete in issue order, and the rows are formed while the tiles' are on their way ----
+  const bool last_chunk = chunk == n_parts - 1 && sk > 0;
+  struct Row {
+    u32x4 raw, norm_w;
+    f32x4 turn[4];
+    float scale;
+  };
+  auto load_row = [&](int r) {
+    Row x;
     const int head = r < HP ? h0 + min(r, nh - 1) : r == HP ? a.h + kh : a.h + a.hkv + kh;
-    const u32x4 raw = ld16(a.qkv + b * a.qkv_rs + (int64_t)head * kHeadDim + 8 * n16);
-    u32x4 y8 = raw;
-    if (r <= HP) {
-      const float *rp = a.rope + b * kHeadDim + 16 * (n16 & 7);
-      float x[8], wf[8], y[8], cs[8][2];
-      unpack8(raw, x);
-      unpack8(ld16((r < HP ? a.qw : a.kw) + 8 * n16), wf);
+    x.raw = ld16(a.qkv + b * a.qkv_rs + (int64_t)head * kHeadDim + 8 * n16);
+    x.norm_w = ld16((r < HP ? a.qw : a.kw) + 8 * n16);
+    const f32x4 *rp = reinterpret_cast<const f32x4 *>(a.rope + b * kHeadDim + 16 * (n16 & 7));
 #pragma unroll
-      for (int i = 0; i < 16; ++i) cs[i >> 1][i & 1] = rp[i];
-      const float hs = r < HP ? (float)(__bf16)((a.q_head_scale ? a.q_head_scale[head] : 1.f) * (a.q_row_scale ? a.q_row_scale[b] : 1.f))
-                              : 1.f;
-      norm_rope8(x, wf, a.eps, cs, n16, hs, y);
-      y8 = pack8(y);
-    }
-    if (r < HP) {
-      st16(&qs[r][8 * n16], y8);
-    } else {
-      st16(&new_x[r - HP][8 * n16], y8);
-      if (hg == 0) {
-        const int64_t page = page_of(nk), off = nk & mask;
-        st16((r == HP ? a.c.k + page * a.c.k_ps + kh * a.c.k_hs + off * a.c.k_rs
-                      : a.c.v + page * a.c.v_ps + kh * a.c.v_hs + off * a.c.v_rs) + 8 * n16, y8);
-      }
-    }
-  }
-  __syncthreads();
-  // ---- the new key: a part of its own, 16 lanes a head ----
-  if (has_new && wave == kWaves - 1) {
-    for (int i = G; i < HP; i += 4) {
-      float q[8], k[8], v[8], z = 0.f;
-      unpack8(*reinterpret_cast<const u32x4 *>(&qs[i][8 * n16]), q);
-      unpack8(*reinterpret_cast<const u32x4 *>(&new_x[0][8 * n16]), k);
-      unpack8(*reinterpret_cast<const u32x4 *>(&new_x[1][8 * n16]), v);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        z = fmaf(q[e], k[e], z);
-        part_o[kWaves][i][8 * n16 + e] = v[e];
-      }
-      z += dpp<0xB1>(z);
-      z += dpp<0x4E>(z);
-      z += dpp<0x141>(z);
-      z += dpp<0x140>(z);
-      const float bias = HAS_BIAS ? a.bias[(int64_t)b * a.bias_bs + (int64_t)(h0 + min(i, nh - 1)) * a.bias_hs + nk] : 0.f;
-      const bool hidden = bias == -INFINITY;
-      if (n16 == 0) {
-        part_ml[kWaves][i][0] = hidden ? -INFINITY : (z + bias) * a.scale_log2;
-        part_ml[kWaves][i][1] = hidden ? 0.f : 1.f;
-      }
-    }
-  }
-
-  bf16x8 qf[4];                  // lane (n, G): elements 32 i + 8 G .. + 7 of head n % HP
-#pragma unroll
-  for (int i = 0; i < 4; ++i) qf[i] = *reinterpret_cast<const bf16x8 *>(&qs[n16 & (HP - 1)][32 * i + 8 * G]);
-  const bool second = HP < 16 && (n16 & HP);     // this column holds the weights' second numbers
+    for (int i = 0; i < 4; ++i) x.turn[i] = rp[i];
+    x.scale = 1.f;
+    if (r < HP) x.scale = (float)(__bf16)((a.q_head_scale ? a.q_head_scale[head] : 1.f) * (a.q_row_scale ? a.q_row_scale[b] : 1.f));
+    return x;
+  };
+  const int rows = HP + (last_chunk ? 2 : 0), row0 = tid >> 4;
+  Row row;
+  if (row0 < rows) row = load_row(row0);
+  const int32_t new_page = page_of(nk);
 
   struct Tile {
     u32x4 k[2][4], v[8];
@@ -288,6 +256,71 @@ __global__ __launch_bounds__(64 * kWaves, kPerCu) void paged_decode_kernel(Paged
 #pragma unroll
     for (int j = 0; j < 8; ++j) l.v[j] = ld16(vbase + page * a.c.v_ps + (int64_t)((vk & mask) + j) * a.c.v_rs);
   };
+
+  Tile l;
+  auto first_loads = [&](int t) {
+    load_entries(t);
+    load_k(l, t);
+    load_v(l, t);
+    load_entries(t + kWaves);
+  };
+  int t = t_lo + wave;
+  if (t < t_hi) first_loads(t);
+
+  const bool has_new = last_chunk && (uint32_t)new_page < (uint32_t)a.c.n_pages;
+  for (int r = row0; r < rows; r += 4 * kWaves) {
+    if (r != row0) row = load_row(r);
+    u32x4 y8 = row.raw;
+    if (r <= HP) {
+      float x[8], wf[8], y[8], cs[8][2];
+      unpack8(row.raw, x);
+      unpack8(row.norm_w, wf);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) cs[i >> 1][i & 1] = row.turn[i >> 2][i & 3];
+      norm_rope8(x, wf, a.eps, cs, n16, row.scale, y);
+      y8 = pack8(y);
+    }
+    if (r < HP) {
+      st16(&qs[r][8 * n16], y8);
+    } else {
+      st16(&new_x[r - HP][8 * n16], y8);
+      if (hg == 0 && has_new) {
+        const int64_t page = new_page, off = nk & mask;
+        st16((r == HP ? a.c.k + page * a.c.k_ps + kh * a.c.k_hs + off * a.c.k_rs
+                      : a.c.v + page * a.c.v_ps + kh * a.c.v_hs + off * a.c.v_rs) + 8 * n16, y8);
+      }
+    }
+  }
+  __syncthreads();
+  // ---- the new key: a part of its own, 16 lanes a head ----
+  if (has_new && wave == kWaves - 1) {
+    for (int i = G; i < HP; i += 4) {
+      float q[8], k[8], v[8], z = 0.f;
+      unpack8(*reinterpret_cast<const u32x4 *>(&qs[i][8 * n16]), q);
+      unpack8(*reinterpret_cast<const u32x4 *>(&new_x[0][8 * n16]), k);
+      unpack8(*reinterpret_cast<const u32x4 *>(&new_x[1][8 * n16]), v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        z = fmaf(q[e], k[e], z);
+        part_o[kWaves][i][8 * n16 + e] = v[e];
+      }
+      z += dpp<0xB1>(z);
+      z += dpp<0x4E>(z);
+      z += dpp<0x141>(z);
+      z += dpp<0x140>(z);
+      const float bias = HAS_BIAS ? a.bias[(int64_t)b * a.bias_bs + (int64_t)(h0 + min(i, nh - 1)) * a.bias_hs + nk] : 0.f;
+      const bool hidden = bias == -INFINITY;
+      if (n16 == 0) {
+        part_ml[kWaves][i][0] = hidden ? -INFINITY : (z + bias) * a.scale_log2;
+        part_ml[kWaves][i][1] = hidden ? 0.f : 1.f;
+      }
+    }
+  }
+
+  bf16x8 qf[4];                  // lane (n, G): elements 32 i + 8 G .. + 7 of head n % HP
+#pragma unroll
+  for (int i = 0; i < 4; ++i) qf[i] = *reinterpret_cast<const bf16x8 *>(&qs[n16 & (HP - 1)][32 * i + 8 * G]);
+  const bool second = HP < 16 && (n16 & HP);     // this column holds the weights' second numbers
 
   f32x4 oacc[8];                 // lane (n, G): rows (columns of S^T) 4 G .. 4 G + 3, elements 8 n + e
   float mrun, lsum;
@@ -389,13 +422,6 @@ __global__ __launch_bounds__(64 * kWaves, kPerCu) void paged_decode_kernel(Paged
     }
     __builtin_amdgcn_sched_barrier(0);
   };
-  Tile l;
-  auto first_loads = [&](int t) {
-    load_entries(t);
-    load_k(l, t);
-    load_v(l, t);
-    load_entries(t + kWaves);
-  };
   auto clear = [&] {
 #pragma unroll
     for (int e = 0; e < 8; ++e) oacc[e] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -423,9 +449,7 @@ __global__ __launch_bounds__(64 * kWaves, kPerCu) void paged_decode_kernel(Paged
     return !__builtin_amdgcn_ballot_w64(!ok);
   };
   clear();
-  int t = t_lo + wave;
   if (t < t_hi) {
-    first_loads(t);
     for (; t + kWaves < t_hi; t += kWaves) step(l, t, std::false_type(), std::true_type(), 0.f);
     step(l, t, std::false_type(), std::false_type(), 0.f);
   }
@@ -551,6 +575,7 @@ __global__ __launch_bounds__(64 * kWaves, kPerCu) void paged_decode_kernel(Paged
 // Workgroups of a launch: units of (sequence, kv head, head set), cut into chunks on the device.
 struct DecodePlan {
   int hp, sets, slots, least;    // query heads of a workgroup: a power of two that holds the KV head's, at most 16
+  float per_root;                // see SplitRule
   int64_t grid, bytes;
 };
 // The counters' region is the same for every launch, so that no launch writes partial results where another counts;
@@ -561,8 +586,16 @@ DecodePlan plan_decode(int64_t num_seqs, int num_heads, int num_heads_k, int max
   const int group = num_heads / num_heads_k;
   for (p.hp = 1; p.hp < group && p.hp < 16;) p.hp *= 2;
   p.sets = num_heads_k * ((group + p.hp - 1) / p.hp);
-  p.slots = kPerCu * device_cus();
-  const int64_t units = num_seqs * p.sets, tiles = std::max(1, (max_k + kTile - 1) / kTile);
+  const int64_t units = num_seqs * p.sets;
+  // Few units: a workgroup per CU, whose longer chunks make fewer to merge (one sequence of 8192 / 32769 / 131072 keys with
+  // three per CU 17.7 / 34.3 / 100, with one 14.5 / 31.3 / 97 us; 2 of 8192 22.9 / 18.9); many, of uneven lengths, balance
+  // better over more (64 of up to 4099 132, over one per CU 131, two 150; 40 of up to 6000 108, 131, 109).
+  p.slots = (units < 128 ? 1 : kPerCu) * device_cus();
+  // Chunks of some of the four waves' steps, more for longer sequences, as the merge takes 0.1 us a chunk, with 8 and 16 heads 0.3:
+  // one of 8192 keys in 64 chunks 16.8, in 22 13.5, in 8 18; 8 of 8192 with 16 / 2 heads 31.5, 22.2, 19.5.  Up to 12 tiles
+  // are not cut (300 keys 8.9 in three chunks, 8.1 in one).
+  p.per_root = p.hp >= 8 ? 0.26f : 0.22f;
+  const int64_t tiles = std::max(1, (max_k + kTile - 1) / kTile);
   p.least = units <= kCounters ? kWaves : 1 << 22;
   p.grid = std::min<int64_t>(units * ((tiles + p.least - 1) / p.least), units + kRounds * p.slots);
   // counters, (max, sum), O
@@ -635,7 +668,7 @@ extern "C" int tg_paged_append(const void *qkv, int64_t qkv_row_stride, const fl
   a.slots = slots;
   a.groups = (num_heads + 2 * num_heads_k + kRowsPer - 1) / kRowsPer;
   const int64_t blocks = (n_tokens * a.groups + 15) / 16;
-  TG_CHECK(blocks < (1ll << 31), "%s: too many tokens", what);
+  TG_CHECK(blocks < (1ll << 28), "%s: too many tokens", what);
   hipLaunchKernelGGL(paged_append_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, a);
   TG_HIP_CHECK(hipGetLastError());
   return 0;
@@ -711,6 +744,7 @@ extern "C" int tg_paged_decode_attention(const void *qkv, int64_t qkv_row_stride
   a.sets = p.sets;
   a.slots = p.slots;
   a.least = p.least;
+  a.per_root = p.per_root;
   if (p.bytes > 0) {
     TG_CHECK(workspace != nullptr && workspace_bytes >= p.bytes, "%s: needs a workspace of %lld bytes (got %lld)", what,
              (long long)p.bytes, (long long)workspace_bytes);

@@ -339,23 +339,30 @@ __device__ __forceinline__ float wave_sum(float x) {
 // 8j+7 in x and their norm weights in wf, the rotate-half partner 8j+-64 sits in lane j^8; cs[e] is
 // (cos, sin) of frequency (8j + e) % 64.  y = hs * bf16(rotated), rounded by the caller.  The fused
 // multiply-adds are written out, so that every kernel that rotates a row gets the same bits.
+// (Exchanges within 16 lanes are data-parallel primitives: what __shfl_xor sends through the LDS crossbar.  After the first two
+// steps of the sum the lanes of a quad hold the same number, so a mirrored half row is as good as lane ^ 4.)
 constexpr int kHeadDim = 128;
+template <int CTRL>
+__device__ __forceinline__ float row16(float x) {
+  const int v = __builtin_bit_cast(int, x);
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(v, v, CTRL, 0xf, 0xf, true));
+}
 __device__ __forceinline__ void norm_rope8(float (&x)[8], const float (&wf)[8], float eps,
                                            const float (*cs)[2], int j, float hs, float (&y)[8]) {
   float ss = 0.f;
 #pragma unroll
   for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
-  ss += __shfl_xor(ss, 1);
-  ss += __shfl_xor(ss, 2);
-  ss += __shfl_xor(ss, 4);
-  ss += __shfl_xor(ss, 8);
+  ss += row16<0xB1>(ss);    // quad_perm 1 0 3 2
+  ss += row16<0x4E>(ss);    // quad_perm 2 3 0 1
+  ss += row16<0x141>(ss);   // row_half_mirror
+  ss += row16<0x128>(ss);   // row_ror 8
   const float rinv = rsqrtf(ss * (1.f / kHeadDim) + eps);
 #pragma unroll
   for (int e = 0; e < 8; ++e) x[e] = wf[e] * (x[e] * rinv);
   const float sgn = j < 8 ? -1.f : 1.f;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    const float p = __shfl_xor(x[e], 8);
+    const float p = row16<0x128>(x[e]);
     y[e] = hs * (float)(__bf16)fmaf(x[e], cs[e][0], sgn * p * cs[e][1]);
   }
 }
