@@ -19,6 +19,9 @@ later steps replay one captured HIP graph of the whole step (144 launches for 28
 and outputs are static device buffers; the first step runs eagerly and warms every kernel and
 library handle the capture records.
 
+After a prefill with page_rows the caches are in pages: each layer's launch is tg_paged_decode_attention over the group's
+page table, the same counters and steps otherwise.
+
 Two options leave the reference's decode.  With kv_bits 4 or 8 every layer's prompt rows are quantised
 into a cache of that many bits (kvquant.QuantKV; the prefill's bf16 caches may then be freed) and each
 layer's launch is tg_decode_attention_quant, which quantises the new rows on the way in.  With a Sampling
@@ -36,6 +39,7 @@ from tokengate_amd.decoder import (CacheGap, DecoderWeights, LayerKV, argmax_row
                                    linear_rows_norm_act, linear_rows_swiglu, logits_last, rmsnorm, sample_rows,
                                    sample_rows_workspace, silu_mul)
 from tokengate_amd.gate import ScoringHead
+from tokengate_amd.paged import PagedKV, paged_decode_attention, paged_decode_attention_workspace
 from tokengate_amd.kvquant import (QuantKV, decode_attention_quant, decode_attention_quant_workspace, kv_quantize)
 from tokengate_amd.prefill import PrefillResult
 
@@ -147,11 +151,16 @@ class DecodeState:
         cu_below = pf.cu_prompt if not prune_below_gate else pf.cu_kept
         self.kv_bits = kv_bits
         self.sampler = sampler
-        in_place = kv_bits == 16 and pf.decode_headroom >= max_new_tokens and pf.cache_above is not None \
+        self.paged = pf.pages_below is not None
+        if self.paged and (kv_bits != 16 or prune_below_gate):
+            raise ValueError("DecodeState: paged caches are decoded over as they are (kv_bits 16, not prune_below_gate)")
+        if self.paged and pf.decode_headroom < max_new_tokens:
+            raise ValueError("DecodeState: the prefill left pages for fewer new tokens than max_new_tokens")
+        in_place = self.paged or kv_bits == 16 and pf.decode_headroom >= max_new_tokens and pf.cache_above is not None \
             and pf.cache_below is not None
         gap = pf.decode_headroom if in_place else max_new_tokens
         self.in_place = in_place
-        self.kv: List[Union[LayerKV, QuantKV]] = []
+        self.kv: List[Union[LayerKV, QuantKV, PagedKV]] = []
         if kv_bits != 16:
             # where the prompt rows lie in the prefill's caches (None: back to back) and in these
             src = [c.rows_dev if pf.decode_headroom and c is not None else None for c in (pf.cache_below, pf.cache_above)]
@@ -195,7 +204,9 @@ class DecodeState:
         self.ssmax = pf.kept_ratio is not None
         # cache slots of the Phase-2 layers, the new token's included once a step has begun
         self.slots = h2d(torch.tensor([float(x) for x in pf.n_kept], dtype=torch.float32), dev) if self.ssmax else None
-        workspace = decode_attention_workspace if kv_bits == 16 else decode_attention_quant_workspace
+        self.tables = (pf.pages_below.table, pf.pages_above.table) if self.paged else None
+        workspace = paged_decode_attention_workspace if self.paged else decode_attention_workspace if kv_bits == 16 \
+            else decode_attention_quant_workspace
         self.att_ws = workspace(B, shape, max(self.cap_k), dev)
         self.rows_b = torch.arange(B, device=dev)
         self.steps = 0
@@ -270,13 +281,15 @@ class DecodeState:
             if not fused:
                 linear_rows(normed, lw.w_qkv, out=qkv)
             kv = self.kv[l]
-            rows = (self.seg_dev[g], self.used[g], self.cap_k[g], scale, self.att_ws, self.bias[j] if g else None,
+            rows = (self.used[g], self.cap_k[g], scale, self.att_ws, self.bias[j] if g else None,
                     self.qscale[j] if (g and self.qscale is not None) else None,
                     r_dec if (r_dec is not None and g) else None)
-            if self.kv_bits == 16:
-                decode_attention(qkv, rope, lw, s, kv.k, kv.v, *rows, out=att)
+            if self.paged:
+                paged_decode_attention(qkv, rope, lw, s, kv, self.tables[g], *rows, out=att)
+            elif self.kv_bits == 16:
+                decode_attention(qkv, rope, lw, s, kv.k, kv.v, self.seg_dev[g], *rows, out=att)
             else:
-                decode_attention_quant(qkv, rope, lw, s, kv, *rows, out=att)
+                decode_attention_quant(qkv, rope, lw, s, kv, self.seg_dev[g], *rows, out=att)
             linear_rows(att.view(B, -1), lw.w_o, out=hid)
             if fused:
                 if wide:

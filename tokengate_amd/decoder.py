@@ -324,15 +324,27 @@ class CacheGap:
 
 
 @dataclass
+class PageGeo:
+    """Where a packed batch's keys lie in paged caches (paged.PagedKV, one per layer): the page table, the keys of every
+    sequence with the packed rows, and what paged.paged_begin gives for these."""
+    table: torch.Tensor        # int32 (nseq, pages)
+    used: torch.Tensor         # int32 (nseq,)
+    max_k: int                 # host: most keys of a sequence
+    slots: torch.Tensor        # int32 (T,)
+    rope: torch.Tensor         # fp32 (T, 64, 2)
+
+
+@dataclass
 class Ragged:
     """Token geometry of a packed batch: rows of sequence b are cu[b] .. cu[b+1]-1.  With `cache`
     the layer's KV rows go to a cache with free rows after each sequence (CacheGap) and attention
-    reads its keys there."""
+    reads its keys there; with `pages` to the sequences' pages (then also over keys that came before)."""
     cu: List[int]
     cu_dev: torch.Tensor       # int32 (nseq + 1,) on the device
     positions: torch.Tensor    # int64 (T,) RoPE position of every row
     max_len: int
     cache: Optional[CacheGap] = None
+    pages: Optional[PageGeo] = None
 
     @property
     def total(self) -> int:
@@ -385,16 +397,18 @@ class Workspace:
 
 
 def run_layers(wts: DecoderWeights, layer_ids, x: torch.Tensor, geo: Ragged, ws: Workspace,
-               kv: List[Optional[LayerKV]], biases=None, q_scales=None, capture: Optional[list] = None,
+               kv: list, biases=None, q_scales=None, capture: Optional[list] = None,
                q_row_scale: Optional[torch.Tensor] = None, attn_only_last: bool = False) -> torch.Tensor:
     """Runs decoder layers `layer_ids` over the packed rows x (T, d) and returns the hidden state
-    after the last of them (T, d).  kv[i] receives layer i's cache rows.  biases[i] / q_scales[i]
+    after the last of them (T, d).  kv[i] receives layer i's cache rows (a LayerKV, with geo.pages a
+    paged.PagedKV).  biases[i] / q_scales[i]
     (optional): Phase-2 raw-unit key bias (nseq, H, >= max_len) and per-head query scale (H,)
     fp32 of layer i; q_row_scale (T,) fp32: a per-row query scale for every layer (the
     scaled-softmax ratio).  capture: optional list that receives each layer's input hidden state.
     attn_only_last: the last layer stops at its attention residual a = x + o_proj(attn) (the
     split gate layer's boundary, attn_only_forward of gate_forward.py:372-413); its MLP half is
     mlp_sublayer."""
+    from tokengate_amd.paged import paged_append, paged_attention      # (that module needs this one's types)
     shape = wts.shape
     T = geo.total
     if x.shape != (T, shape.d_model):
@@ -416,16 +430,21 @@ def run_layers(wts: DecoderWeights, layer_ids, x: torch.Tensor, geo: Ragged, ws:
         if capture is not None:
             capture.append(res.clone())
         torch.matmul(normed, lw.w_qkv.t(), out=qkv)
-        cg = geo.cache
-        q = qk_norm_rope(qkv, geo.positions, lw, shape, wts.inv_freq, kv[i].k, kv[i].v,
-                         q_scales[i] if q_scales is not None else None, q_row_scale,
-                         kv_rows=cg.rows_dev if cg is not None else None)
-        if cg is None:
-            varlen_attention(q, kv[i].k, kv[i].v, geo.cu_dev, geo.max_len, scale,
-                             biases[i] if biases is not None else None, out=attn, lse=lse)
+        cg, bias = geo.cache, biases[i] if biases is not None else None
+        if geo.pages is not None:
+            pg = geo.pages
+            q = paged_append(qkv, pg.rope, lw, shape, kv[i], pg.slots, q_scales[i] if q_scales is not None else None,
+                             q_row_scale, out=qkv[:, :shape.n_heads * shape.head_dim].unflatten(1, (shape.n_heads, shape.head_dim)))
+            paged_attention(q, kv[i], pg.table, geo.cu_dev, pg.used, geo.max_len, pg.max_k, scale, bias, out=attn)
         else:
-            varlen_kv_attention(q, kv[i].k, kv[i].v, geo.cu_dev, cg.seg_dev, cg.used_dev, geo.max_len,
-                                geo.max_len, scale, biases[i] if biases is not None else None, out=attn, lse=lse)
+            q = qk_norm_rope(qkv, geo.positions, lw, shape, wts.inv_freq, kv[i].k, kv[i].v,
+                             q_scales[i] if q_scales is not None else None, q_row_scale,
+                             kv_rows=cg.rows_dev if cg is not None else None)
+            if cg is None:
+                varlen_attention(q, kv[i].k, kv[i].v, geo.cu_dev, geo.max_len, scale, bias, out=attn, lse=lse)
+            else:
+                varlen_kv_attention(q, kv[i].k, kv[i].v, geo.cu_dev, cg.seg_dev, cg.used_dev, geo.max_len,
+                                    geo.max_len, scale, bias, out=attn, lse=lse)
         torch.matmul(attn.view(T, -1), lw.w_o.t(), out=hid)
         if attn_only_last and n_done == len(layer_ids) - 1:
             break

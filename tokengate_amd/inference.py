@@ -141,19 +141,20 @@ class TokenGateModel:
         return self.weights.device
 
     def prefill(self, ids: Sequence, max_kept_prefill_tokens=None, prune_below_gate: bool = False,
-                decode_headroom: int = 0):
+                decode_headroom: int = 0, page_rows: int = 0):
         """Gated prefill of already-split prompts: ids = [(clean_ids, start, end), ...];
-        decode_headroom: free cache rows left after each sequence for the decode to append to."""
+        decode_headroom: free cache rows left after each sequence for the decode to append to; page_rows: the
+        caches in pages of so many rows."""
         k = _NO_PRUNING if max_kept_prefill_tokens is None else max_kept_prefill_tokens
         return P.prefill_batch(self.weights, self.gate, [x[0] for x in ids], [x[1] for x in ids],
                                [x[2] for x in ids], self.gate_layer, k, prune_below_gate=prune_below_gate,
-                               decode_headroom=decode_headroom)
+                               decode_headroom=decode_headroom, page_rows=page_rows)
 
     @torch.no_grad()
     def generate(self, ids: Union[List[int], List[List[int]]], tokenizer=None, *, max_new_tokens: int = 20,
                  max_kept_prefill_tokens: Optional[int] = None, streamer=None,
                  prune_below_gate: bool = False, kv_bits: int = 16, temperature=0.0, top_k=0, top_p=1.0, min_p=0.0,
-                 seed: int = 0) -> GenerateOutput:
+                 seed: int = 0, page_rows: int = 0) -> GenerateOutput:
         """Gated prefill + greedy decode (TokenGateModel.generate, inference.py:85-124).  ids: one
         sequence or a batch, each carrying the state sentinels.  max_kept_prefill_tokens: the K of
         the paper (None keeps every state token); a list gives one K per sequence.  tokenizer:
@@ -162,12 +163,15 @@ class TokenGateModel:
         kv_bits: 16, or 8 or 4 for caches quantised after the prefill.  temperature (a number or one per
         sequence, as top_k, top_p and min_p): 0 everywhere is greedy decode, else tokens are sampled
         (decode.Sampling) from the random numbers that seed gives, and the result has their log
-        probabilities."""
+        probabilities.  page_rows: 0, or the rows of a page (a power of two from 16) for caches in pages
+        (paged.PagedKV), with kv_bits 16 and without prune_below_gate."""
         from tokengate_amd.decode import DecodeState, Sampling, TokenSampler
         if max_new_tokens < 1:
             raise ValueError("max_new_tokens must be positive")
         if kv_bits not in (4, 8, 16):
             raise ValueError(f"kv_bits must be 16, 8 or 4 (got {kv_bits})")
+        if page_rows and kv_bits != 16:
+            raise ValueError("page_rows: with kv_bits 16 only")
         if ids and isinstance(ids[0], int):
             ids = [ids]
         split = [split_state_span(list(seq)) for seq in ids]
@@ -177,7 +181,7 @@ class TokenGateModel:
         _sync()
         t0 = time.perf_counter()
         pf = self.prefill(split, max_kept_prefill_tokens, prune_below_gate,
-                          decode_headroom=max_new_tokens if max_new_tokens > 1 and kv_bits == 16 else 0)
+                          decode_headroom=max_new_tokens if max_new_tokens > 1 and kv_bits == 16 else 0, page_rows=page_rows)
         first = pf.first_tokens
         sampler, lps = None, None
         if sampled:

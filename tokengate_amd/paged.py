@@ -11,12 +11,12 @@ names none: its keys weigh nothing, and nothing is written to them.  Sequences m
 none of them appends to; which pages are free is the caller's to keep.  bf16, head_dim 128.
 """
 from dataclasses import dataclass
-from typing import Optional, Tuple
+from typing import List, Optional, Tuple
 
 import torch
 
 from tokengate_amd import _lib
-from tokengate_amd.decoder import DecoderShape, LayerWeights
+from tokengate_amd.decoder import DecoderShape, LayerWeights, PageGeo, h2d
 
 HEAD_DIM = 128
 
@@ -261,3 +261,27 @@ def paged_decode_attention(qkv: torch.Tensor, rope: torch.Tensor, lw: LayerWeigh
                  *cache._args, *table, used, int(max_k), *bias, float(scale), out.data_ptr(),
                  out.stride(0) if B > 1 else H * HEAD_DIM, workspace.data_ptr(), workspace.numel())
     return out
+
+
+def page_tables(lengths: List[int], room: int, page_rows: int, device) -> Tuple[torch.Tensor, int]:
+    """(page table, pages) of sequences of these lengths with room for `room` more keys each, one after the other."""
+    need = [(n + room + page_rows - 1) // page_rows for n in lengths]
+    table = torch.full((len(need), max(max(need), 1)), -1, dtype=torch.int32)
+    first = 0
+    for b, n in enumerate(need):
+        table[b, :n] = torch.arange(first, first + n, dtype=torch.int32)
+        first += n
+    return h2d(table, device), max(first, 1)
+
+
+def prompt_pages(cu: List[int], cu_dev: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, shape: DecoderShape,
+                 layers: int, room: int, page_rows: int) -> Tuple[PageGeo, List[PagedKV]]:
+    """Paged caches for `layers` layers of packed prompts cu[b] .. cu[b + 1] - 1 at these positions, with room for `room` more
+    keys each: the geometry for decoder.run_layers, and the caches."""
+    dev = positions.device
+    lens = [cu[b + 1] - cu[b] for b in range(len(cu) - 1)]
+    table, n_pages = page_tables(lens, room, page_rows, dev)
+    caches = [PagedKV.alloc(n_pages, shape.n_kv_heads, page_rows, dev) for _ in range(layers)]
+    used = h2d(torch.tensor(lens, dtype=torch.int32), dev)
+    slots, rope = paged_begin(positions, inv_freq, cu_dev, used, table, caches[0])
+    return PageGeo(table, used, max(lens), slots, rope), caches

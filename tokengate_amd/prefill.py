@@ -30,8 +30,9 @@ from typing import Dict, List, Optional, Sequence
 import torch
 
 from tokengate_amd import gate as G
-from tokengate_amd.decoder import (CacheGap, DecoderWeights, LayerKV, Ragged, Workspace, alloc_kv, argmax_rows, h2d,
+from tokengate_amd.decoder import (CacheGap, DecoderWeights, LayerKV, PageGeo, Ragged, Workspace, alloc_kv, argmax_rows, h2d,
                                    logits_last, mlp_sublayer, run_layers)
+from tokengate_amd.paged import prompt_pages
 
 
 @dataclass
@@ -57,6 +58,9 @@ class PrefillResult:
     cache_below: Optional[CacheGap] = None
     cache_above: Optional[CacheGap] = None
     phase2_bias_seq: Optional[torch.Tensor] = None
+    # with page_rows: kv holds paged.PagedKV, and these say where the sequences' keys lie in them
+    pages_below: Optional[PageGeo] = None
+    pages_above: Optional[PageGeo] = None
 
 
 def _cat_ids(ids_list: Sequence, device) -> torch.Tensor:
@@ -169,14 +173,17 @@ class Phase2Graphs:
 def prefill_batch(wts: DecoderWeights, head, ids_list: Sequence, art_starts: Sequence[int],
                   art_ends: Sequence[int], gate_layer: int, K, prune_below_gate: bool = False,
                   phase_timing: bool = False, capture: bool = False, mlp_rows: int = 131072,
-                  phase2_graphs: Optional[Phase2Graphs] = None, decode_headroom: int = 0) -> PrefillResult:
+                  phase2_graphs: Optional[Phase2Graphs] = None, decode_headroom: int = 0,
+                  page_rows: int = 0) -> PrefillResult:
     """ids_list: B prompts (lists of ints or 1-D tensors); the state span of prompt b is
     [art_starts[b], art_ends[b]); K: scalar or per-prompt list; head: gate.ScoringHead or
     gate.BranchHead (split gate layer).  phase2_graphs: replay Phase 2
     from captured graphs (captured on first use per geometry); the Phase-2 KV caches are then views
     of the graph's buffers, valid until its next replay.  decode_headroom: every layer's KV cache
     is laid out with that many free rows after each sequence (written there by the prefill's own
-    launches and the pack), so that decode appends in place.  Raises RuntimeError (after queueing
+    launches and the pack), so that decode appends in place.  page_rows: the caches are in pages of so
+    many rows (paged.PagedKV; a power of two from 16), decode_headroom more keys' among them; not with
+    prune_below_gate or phase2_graphs.  Raises RuntimeError (after queueing
     every launch, when the selection's launches have finished) if the keep-list selection reported
     an error: the result would be built on invalid keep lists."""
     shape = wts.shape
@@ -195,6 +202,10 @@ def prefill_batch(wts: DecoderWeights, head, ids_list: Sequence, art_starts: Seq
     gap = int(decode_headroom)
     if gap < 0:
         raise ValueError("decode_headroom must be >= 0")
+    if page_rows and (page_rows < 16 or page_rows > 65536 or page_rows & (page_rows - 1)):
+        raise ValueError(f"page_rows must be a power of two from 16 to 65536 (got {page_rows})")
+    if page_rows and (prune_below_gate or phase2_graphs is not None):
+        raise ValueError("page_rows: not with prune_below_gate or phase2_graphs")
     ev = [] if phase_timing else None
 
     def mark(name):
@@ -207,14 +218,18 @@ def prefill_batch(wts: DecoderWeights, head, ids_list: Sequence, art_starts: Seq
     mark("phase1")
     ids = _cat_ids(ids_list, dev)
     geo1 = Ragged.from_lengths(lens, dev)
-    if gap and not prune_below_gate:    # the Phase-1 caches are the decode caches of these layers
+    if gap and not prune_below_gate and not page_rows:    # the Phase-1 caches are the decode caches of these layers
         geo1.cache = CacheGap.build(geo1.cu, gap, dev)
     T = geo1.total
     x = torch.nn.functional.embedding(ids, wts.embed)
     ws1 = Workspace(shape, T, dev, mlp_rows=mlp_rows)
-    kv: List[Optional[LayerKV]] = [None] * n_layers
-    for i in range(gate_layer + 1):
-        kv[i] = alloc_kv(shape, geo1.kv_rows, dev)
+    kv: list = [None] * n_layers
+    if page_rows:
+        geo1.pages, kv[:gate_layer + 1] = prompt_pages(geo1.cu, geo1.cu_dev, geo1.positions, wts.inv_freq, shape, gate_layer + 1,
+                                                       gap, page_rows)
+    else:
+        for i in range(gate_layer + 1):
+            kv[i] = alloc_kv(shape, geo1.kv_rows, dev)
     split = bool(getattr(head, "split_gate_layer", False))
     h = run_layers(wts, range(gate_layer + 1), x, geo1, ws1, kv, capture=cap["phase1"] if cap else None,
                    attn_only_last=split)
@@ -282,7 +297,7 @@ def prefill_batch(wts: DecoderWeights, head, ids_list: Sequence, art_starts: Seq
     biases_all = bias_z[:, :, idx_d].permute(0, 2, 1, 3).contiguous()          # (L2, B, H, W)
     cu2_dev = h2d(torch.tensor(p.cu_kept, dtype=torch.int32), dev)
     above = list(range(gate_layer + 1, n_layers))
-    cache2 = None
+    cache2 = pages2 = None
     if phase2_graphs is not None and cap is None:
         h2, kv2 = phase2_graphs.run(wts, above, hs, kept_pos, cu2_dev, biases_all, q_head, mlp_rows, q_row,
                                     cu_kept=p.cu_kept, gap=gap)
@@ -291,12 +306,17 @@ def prefill_batch(wts: DecoderWeights, head, ids_list: Sequence, art_starts: Seq
         if gap:
             cache2 = CacheGap.build(p.cu_kept, gap, dev)
     else:
-        cache2 = CacheGap.build(p.cu_kept, gap, dev) if gap else None
+        cache2 = CacheGap.build(p.cu_kept, gap, dev) if gap and not page_rows else None
         geo2 = Ragged(p.cu_kept, cu2_dev, kept_pos, max_kept, cache=cache2)
         biases = {l: biases_all[j] for j, l in enumerate(above)}
         qs = {l: q_head[j] for j, l in enumerate(above)} if q_head is not None else None
-        for l in above:
-            kv[l] = alloc_kv(shape, geo2.kv_rows, dev)
+        if page_rows:
+            geo2.pages, kv[gate_layer + 1:] = prompt_pages(p.cu_kept, cu2_dev, kept_pos, wts.inv_freq, shape, len(above), gap,
+                                                           page_rows)
+            pages2 = geo2.pages
+        else:
+            for l in above:
+                kv[l] = alloc_kv(shape, geo2.kv_rows, dev)
         ws2 = ws2 if ws2 is not None else Workspace(shape, T2, dev, mlp_rows=mlp_rows)
         h2 = run_layers(wts, above, hs, geo2, ws2, kv, biases=biases, q_scales=qs,
                         capture=cap["phase2"] if cap else None, q_row_scale=q_row)
@@ -317,10 +337,10 @@ def prefill_batch(wts: DecoderWeights, head, ids_list: Sequence, art_starts: Seq
         cap.update(scores=scores, keep=keep, hs_packed=hs, h2=h2, logits=logits, biases_all=biases_all,
                    q_head=q_head, q_row=q_row)
     cache1 = None
-    if gap:
+    if gap and not page_rows:
         cache1 = geo1.cache if not prune_below_gate else CacheGap.build(p.cu_kept, gap, dev)
     return PrefillResult(first, logits, kept_pos, p.cu_kept, p.n_kept, p.k_clamped, kv, geo1.cu, kept_bias, ratio,
-                         bias_rows, phase_ms, cap, gap, cache1, cache2, biases_all if gap else None)
+                         bias_rows, phase_ms, cap, gap, cache1, cache2, biases_all if gap else None, geo1.pages, pages2)
 
 
 def ttft_ms(fn, reps: int = 5, warmup: int = 1) -> List[float]:
