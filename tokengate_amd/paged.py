@@ -19,6 +19,8 @@ from tokengate_amd import _lib
 from tokengate_amd.decoder import DecoderShape, LayerWeights, PageGeo, h2d
 
 HEAD_DIM = 128
+_I32, _F32, _BF16, _U8 = torch.int32, torch.float32, torch.bfloat16, torch.uint8
+_NO_BIAS = (None, 0, 0)
 
 
 def _apart(t: torch.Tensor) -> bool:
@@ -92,12 +94,14 @@ def _ints(what: str, name: str, t: torch.Tensor, n: int, dev: int) -> int:
 
 def _table(what: str, t: torch.Tensor, n_seqs: int, max_k: int, page_rows: int, dev: int) -> tuple:
     """(pointer, stride, columns) of a page table."""
-    if t.dtype is not torch.int32 or t.dim() != 2 or t.get_device() != dev or t.shape[0] < n_seqs or t.shape[1] < 1 \
-            or (t.stride(1) != 1 and t.shape[1] > 1):
+    if t.dtype is not _I32 or t.dim() != 2 or t.get_device() != dev:
         raise RuntimeError(f"{what}: page_table must be int32 (sequences, pages), rows contiguous, on the cache's device")
-    if t.shape[1] * page_rows < max_k:
+    (rows, cols), (rs, cs) = t.shape, t.stride()
+    if rows < n_seqs or cols < 1 or (cs != 1 and cols > 1):
+        raise RuntimeError(f"{what}: page_table must be int32 (sequences, pages), rows contiguous, on the cache's device")
+    if cols * page_rows < max_k:
         raise RuntimeError(f"{what}: page_table's columns hold fewer than max_k keys")
-    return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else t.shape[1], t.shape[1]
+    return t.data_ptr(), rs if rows > 1 else cols, cols
 
 
 def _floats(what: str, name: str, t: Optional[torch.Tensor], n: int, dev: int):
@@ -118,19 +122,18 @@ def _bias(what: str, t: Optional[torch.Tensor], n_seqs: int, n_heads: int, max_k
 
 
 def _qkv(what: str, qkv: torch.Tensor, shape: DecoderShape, cache: PagedKV) -> int:
-    H, Hkv = shape.n_heads, shape.n_kv_heads
-    if qkv.dtype is not torch.bfloat16 or qkv.dim() != 2 or qkv.shape[1] < (H + 2 * Hkv) * HEAD_DIM or qkv.stride(1) != 1:
+    width = (shape.n_heads + 2 * shape.n_kv_heads) * HEAD_DIM
+    if qkv.dtype is not _BF16 or qkv.dim() != 2 or qkv.shape[1] < width or qkv.stride(1) != 1:
         raise RuntimeError(f"{what}: qkv must be bf16 rows of every head's q, k and v")
-    if cache.n_kv_heads != Hkv or cache.device_index != qkv.get_device() or shape.head_dim != HEAD_DIM:
+    if cache.n_kv_heads != shape.n_kv_heads or cache.device_index != qkv.get_device() or shape.head_dim != HEAD_DIM:
         raise RuntimeError(f"{what}: the cache has other KV heads or is on another device")
-    return qkv.stride(0) if qkv.shape[0] > 1 else (H + 2 * Hkv) * HEAD_DIM
+    return qkv.stride(0) if qkv.shape[0] > 1 else width
 
 
-def _weights(what: str, lw: LayerWeights, dev: int) -> tuple:
+def _weights(what: str, lw: LayerWeights, dev: int) -> None:
     for t in (lw.q_norm, lw.k_norm):
-        if t.dtype is not torch.bfloat16 or not t.is_contiguous() or t.numel() != HEAD_DIM or t.get_device() != dev:
+        if t.dtype is not _BF16 or not t.is_contiguous() or t.numel() != HEAD_DIM or t.get_device() != dev:
             raise RuntimeError(f"{what}: norm weights must be contiguous bf16 (128,) on the cache's device")
-    return lw.q_norm.data_ptr(), lw.k_norm.data_ptr()
 
 
 def paged_begin(positions: torch.Tensor, inv_freq: torch.Tensor, cu_q: torch.Tensor, kv_used: torch.Tensor,
@@ -164,22 +167,31 @@ def paged_append(qkv: torch.Tensor, rope: torch.Tensor, lw: LayerWeights, shape:
     int32 = page * page_rows + row; a slot outside the cache writes none.  Returns the queries (T, H, 128): out, by
     default a new tensor; out may be qkv's own query columns (qkv[:, :H * 128].unflatten(1, (H, 128)): in place).  No two
     rows may name one slot."""
-    H, Hkv, dev = shape.n_heads, shape.n_kv_heads, cache.device_index
+    H, dev = shape.n_heads, cache.device_index
     rs = _qkv("paged_append", qkv, shape, cache)
     T = qkv.shape[0]
+    qw, kw = lw.q_norm, lw.k_norm
+    if not (slots.dtype is _I32 and slots.numel() >= T and slots.is_contiguous() and slots.get_device() == dev
+            and rope.dtype is _F32 and rope.numel() >= T * HEAD_DIM and rope.is_contiguous() and rope.get_device() == dev
+            and qw.dtype is _BF16 and kw.dtype is _BF16 and qw.numel() == HEAD_DIM and kw.numel() == HEAD_DIM
+            and qw.is_contiguous() and kw.is_contiguous() and qw.get_device() == dev and kw.get_device() == dev):
+        _ints("paged_append", "slots", slots, T, dev)
+        _floats("paged_append", "rope", rope, T * HEAD_DIM, dev)
+        _weights("paged_append", lw, dev)
+    qh = None if q_head_scale is None else _floats("paged_append", "q_head_scale", q_head_scale, H, dev)
+    qr = None if q_row_scale is None else _floats("paged_append", "q_row_scale", q_row_scale, T, dev)
     if out is None:
-        out = torch.empty((T, H, HEAD_DIM), dtype=torch.bfloat16, device=qkv.device)
-    elif out.dtype is not torch.bfloat16 or tuple(out.shape) != (T, H, HEAD_DIM) or out.stride(2) != 1 or out.get_device() != dev:
-        raise RuntimeError("paged_append: out must be bf16 (rows, H, 128), values contiguous, on the cache's device")
-    elif not _apart(out):
-        raise RuntimeError("paged_append: rows of out overlap")
-    ors, ohs = out.stride(0) if T > 1 else 0, out.stride(1) if H > 1 else HEAD_DIM
-    args = (_floats("paged_append", "rope", rope, T * HEAD_DIM, dev), _floats("paged_append", "q_head_scale", q_head_scale, H, dev),
-            _floats("paged_append", "q_row_scale", q_row_scale, T, dev), _ints("paged_append", "slots", slots, T, dev))
-    qw, kw = _weights("paged_append", lw, dev)
+        out = torch.empty((T, H, HEAD_DIM), dtype=_BF16, device=qkv.device)
+        ors, ohs = H * HEAD_DIM, HEAD_DIM
+    else:
+        if out.dtype is not _BF16 or tuple(out.shape) != (T, H, HEAD_DIM) or out.stride(2) != 1 or out.get_device() != dev:
+            raise RuntimeError("paged_append: out must be bf16 (rows, H, 128), values contiguous, on the cache's device")
+        if not _apart(out):
+            raise RuntimeError("paged_append: rows of out overlap")
+        ors, ohs = out.stride(0) if T > 1 else 0, out.stride(1) if H > 1 else HEAD_DIM
     if T:
-        _lib.call_on(dev, "tg_paged_append", qkv.data_ptr(), rs, args[0], T, H, Hkv, HEAD_DIM, qw, kw, shape.rms_eps, args[1],
-                     args[2], out.data_ptr(), ors, ohs, args[3], *cache._args)
+        _lib.call_on(dev, "tg_paged_append", qkv.data_ptr(), rs, rope.data_ptr(), T, H, shape.n_kv_heads, HEAD_DIM, qw.data_ptr(),
+                     kw.data_ptr(), shape.rms_eps, qh, qr, out.data_ptr(), ors, ohs, slots.data_ptr(), *cache._args)
     return out
 
 
@@ -237,29 +249,37 @@ def paged_decode_attention(qkv: torch.Tensor, rope: torch.Tensor, lw: LayerWeigh
     become key kv_used[b] - 1, and its query attends over keys 0 .. kv_used[b] - 1 (at most max_k); bias_raw (nseq, H,
     >= max_k) as decode_attention, -inf hides a key whatever its row holds.  A sequence of kv_used 0 (a free place of a
     padded batch) appends nothing and gets zeros.  No sequence may append a row that another one reads or appends."""
-    what, dev = "paged_decode_attention", cache.device_index
-    H, Hkv = shape.n_heads, shape.n_kv_heads
-    rs = _qkv(what, qkv, shape, cache)
+    dev, H, Hkv = cache.device_index, shape.n_heads, shape.n_kv_heads
+    rs = _qkv("paged_decode_attention", qkv, shape, cache)
     B = qkv.shape[0]
-    if out is None:
-        out = torch.empty((B, H, HEAD_DIM), dtype=torch.bfloat16, device=qkv.device)
-    elif out.dtype is not torch.bfloat16 or tuple(out.shape) != (B, H, HEAD_DIM) or out.stride()[1:] != (HEAD_DIM, 1) \
-            or out.get_device() != dev:
-        raise RuntimeError("paged_decode_attention: out must be bf16 (B, H, 128) rows on the cache's device")
-    used = _ints(what, "kv_used", kv_used, B, dev)
-    rope_p = _floats(what, "rope", rope, B * HEAD_DIM, dev)
-    qh = _floats(what, "q_head_scale", q_head_scale, H, dev)
-    qr = _floats(what, "q_row_scale", q_row_scale, B, dev)
-    bias = _bias(what, bias_raw, B, H, max_k, dev)
-    qw, kw = _weights(what, lw, dev)
-    if workspace.dtype is not torch.uint8 or not workspace.is_contiguous() or workspace.get_device() != dev:
+    qw, kw = lw.q_norm, lw.k_norm
+    # one test for what nearly every call passes; what does not pass it is looked at again for its message
+    if not (kv_used.dtype is _I32 and kv_used.numel() >= B and kv_used.is_contiguous() and kv_used.get_device() == dev
+            and rope.dtype is _F32 and rope.numel() >= B * HEAD_DIM and rope.is_contiguous() and rope.get_device() == dev
+            and qw.dtype is _BF16 and kw.dtype is _BF16 and qw.numel() == HEAD_DIM and kw.numel() == HEAD_DIM
+            and qw.is_contiguous() and kw.is_contiguous() and qw.get_device() == dev and kw.get_device() == dev
+            and workspace.dtype is _U8 and workspace.is_contiguous() and workspace.get_device() == dev):
+        _ints("paged_decode_attention", "kv_used", kv_used, B, dev)
+        _floats("paged_decode_attention", "rope", rope, B * HEAD_DIM, dev)
+        _weights("paged_decode_attention", lw, dev)
         raise RuntimeError("paged_decode_attention: workspace must be contiguous bytes on the cache's device")
+    qh = None if q_head_scale is None else _floats("paged_decode_attention", "q_head_scale", q_head_scale, H, dev)
+    qr = None if q_row_scale is None else _floats("paged_decode_attention", "q_row_scale", q_row_scale, B, dev)
+    bias = _NO_BIAS if bias_raw is None else _bias("paged_decode_attention", bias_raw, B, H, max_k, dev)
+    if out is None:
+        out = torch.empty((B, H, HEAD_DIM), dtype=_BF16, device=qkv.device)
+        ors = H * HEAD_DIM
+    else:
+        if out.dtype is not _BF16 or tuple(out.shape) != (B, H, HEAD_DIM) or out.stride(2) != 1 \
+                or (H > 1 and out.stride(1) != HEAD_DIM) or out.get_device() != dev:
+            raise RuntimeError("paged_decode_attention: out must be bf16 (B, H, 128) rows on the cache's device")
+        ors = out.stride(0) if B > 1 else H * HEAD_DIM
     if B == 0:
         return out
-    table = _table(what, page_table, B, max_k, cache.page_rows, dev)
-    _lib.call_on(dev, "tg_paged_decode_attention", qkv.data_ptr(), rs, rope_p, B, H, Hkv, HEAD_DIM, qw, kw, shape.rms_eps, qh, qr,
-                 *cache._args, *table, used, int(max_k), *bias, float(scale), out.data_ptr(),
-                 out.stride(0) if B > 1 else H * HEAD_DIM, workspace.data_ptr(), workspace.numel())
+    table = _table("paged_decode_attention", page_table, B, max_k, cache.page_rows, dev)
+    _lib.call_on(dev, "tg_paged_decode_attention", qkv.data_ptr(), rs, rope.data_ptr(), B, H, Hkv, HEAD_DIM, qw.data_ptr(),
+                 kw.data_ptr(), shape.rms_eps, qh, qr, *cache._args, *table, kv_used.data_ptr(), int(max_k), *bias, float(scale),
+                 out.data_ptr(), ors, workspace.data_ptr(), workspace.numel())
     return out
 
 
