@@ -350,6 +350,17 @@ __device__ __forceinline__ bool fwd_body(const FwdArgs &a, const MoreArgs<DEC, P
     }
   }
 
+  // Pages: the entries of the next tile to be issued, lane q that of its 16 keys (PAGES 2: 64) from 16 q (64 q) on, loaded while
+  // the tile before it is computed (the first tile's before anything else); and, by bit, which 16 keys of the issued tile
+  // have no page.
+  constexpr int kPartKeys = PAGES == 2 ? 64 : 16;
+  [[maybe_unused]] int32_t entry = 0;
+  [[maybe_unused]] uint32_t no_page = 0;
+  [[maybe_unused]] auto load_entries = [&](int tile) {
+    if constexpr (PAGED)
+      entry = dec.table[b * dec.table_rs + min((tile * SK + kPartKeys * (lane & (SK / kPartKeys - 1))) >> dec.lg, dec.cols - 1)];
+  };
+  if constexpr (PAGED) load_entries(0);
   int sq = a.sq, sk = a.sk;
   int64_t row0 = 0, krow0 = 0;
   if constexpr (DEC) {
@@ -479,15 +490,6 @@ __device__ __forceinline__ bool fwd_body(const FwdArgs &a, const MoreArgs<DEC, P
     const int vc = (lane & 15) ^ vswz(vkey);
     voff[it] = (uint32_t)(vkey * a.v_rs * 2 + vc * 16);
   }
-  // Pages: the entries of the next tile to be issued, lane q that of its 16 keys (PAGES 2: 64) from 16 q (64 q) on, loaded while
-  // the tile before it is computed; and, by bit, which 16 keys of the issued tile have no page.
-  constexpr int kParts16 = SK / 16, kPartKeys = PAGES == 2 ? 64 : 16;
-  [[maybe_unused]] int32_t entry = 0;
-  [[maybe_unused]] uint32_t no_page = 0;
-  [[maybe_unused]] auto load_entries = [&](int tile) {
-    if constexpr (PAGED)
-      entry = dec.table[b * dec.table_rs + min((tile * SK + kPartKeys * (lane & (SK / kPartKeys - 1))) >> dec.lg, dec.cols - 1)];
-  };
   [[maybe_unused]] auto issue_paged = [&](int tile, auto buf_c) {
     if constexpr (PAGED) {
       char *kd = kslot(buf_c), *vd = vslot(buf_c);
@@ -498,37 +500,39 @@ __device__ __forceinline__ bool fwd_body(const FwdArgs &a, const MoreArgs<DEC, P
       auto k_rows = [](int it) { return kWaves == 8 ? 32 * it : 32 * (it >> 1) + 4 * (it & 1); };
       auto v_rows = [](int it) { return 4 * kWaves * it; };
       auto bytes = [&](int n, int64_t rs) { return n > 0 ? (uint32_t)((n - 1) * (int)rs + kD) * 2u : 0u; };   // of n rows
+      // lane q holds where the keys from kPartKeys q on begin
+      const int part_row = kPartKeys * (lane & (SK / kPartKeys - 1));
+      const bool there = (uint32_t)entry < (uint32_t)dec.n_pages;
+      const int64_t p = there ? entry : 0, row = (tile * SK + part_row) & mask;
+      const uint64_t ka = (uint64_t)(kh_base + p * dec.k_ps + row * a.k_rs), va = (uint64_t)(vh_base + p * dec.v_ps + row * a.v_rs);
+      uint32_t gone = (uint32_t)__builtin_amdgcn_ballot_w64(!there && part_row < left) & ((1u << (SK / kPartKeys)) - 1u);
+      const bool all = gone == 0 && left >= SK;
+      auto part = [&](uint64_t at, int key, int64_t rs, uint32_t n_bytes) {   // from `key` on, of n_bytes
+        const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)at, key / kPartKeys);
+        const uint32_t hi = __builtin_amdgcn_readlane((uint32_t)(at >> 32), key / kPartKeys);
+        return make_rsrc((const char *)(((uint64_t)hi << 32 | lo) + (uint32_t)((key & (kPartKeys - 1)) * (int)rs * 2)), n_bytes);
+      };
+      auto is_gone = [&](int key) { return (gone >> (key / kPartKeys)) & 1; };
       if constexpr (PAGES == 2) {
-        no_page = 0;
-#pragma unroll
-        for (int i = 0; i < SK / 64; ++i) {          // loads kLoads / (SK / 64) of every 64 keys
-          const int32_t page = __builtin_amdgcn_readlane(entry, i);
-          const bool there = (uint32_t)page < (uint32_t)dec.n_pages;
-          const int64_t p = there ? page : 0, row = (tile * SK + 64 * i) & mask;
-          const int n = there ? min(left - 64 * i, 64) : 0;
-          const brsrc_t kr = make_rsrc(kh_base + p * dec.k_ps + row * a.k_rs, bytes(n, a.k_rs));
-          const brsrc_t vr = make_rsrc(vh_base + p * dec.v_ps + row * a.v_rs, bytes(n, a.v_rs));
-          no_page |= there || left <= 64 * i ? 0u : 15u << (4 * i);
+        auto issue = [&](auto rows) {              // rows(key): those of the 64 keys from `key` on that are there
           constexpr int kOf64 = kLoads / (SK / 64);
 #pragma unroll
-          for (int it = 0; it < kOf64; ++it) {
-            dma16(kr, kd + (wv + (i * kOf64 + it) * kWaves) * 1024, koff[0] + (uint32_t)(k_rows(it) * (int)a.k_rs * 2));
-            dma16(vr, vd + (wv + (i * kOf64 + it) * kWaves) * 1024, voff[0] + (uint32_t)(v_rows(it) * (int)a.v_rs * 2));
+          for (int i = 0; i < SK / 64; ++i) {      // loads kOf64 of every 64 keys
+            const brsrc_t kr = part(ka, 64 * i, 0, bytes(rows(64 * i), a.k_rs)), vr = part(va, 64 * i, 0, bytes(rows(64 * i), a.v_rs));
+#pragma unroll
+            for (int it = 0; it < kOf64; ++it) {
+              dma16(kr, kd + (wv + (i * kOf64 + it) * kWaves) * 1024, koff[0] + (uint32_t)(k_rows(it) * (int)a.k_rs * 2));
+              dma16(vr, vd + (wv + (i * kOf64 + it) * kWaves) * 1024, voff[0] + (uint32_t)(v_rows(it) * (int)a.v_rs * 2));
+            }
           }
-        }
+        };
+        if (all) issue([](int) { return 64; });
+        else issue([&](int key) { return is_gone(key) ? 0 : min(left - key, 64); });
+        gone = (gone & 1u ? 15u : 0u) | (gone & 2u ? 0xf0u : 0u);
       } else {
-        // lane q holds where the keys from 16 q on begin; a load brings four of them, through a descriptor of exactly those that
-        // are there
-        const bool there = (uint32_t)entry < (uint32_t)dec.n_pages;
-        const int64_t p = there ? entry : 0, row = (tile * SK + 16 * (lane & (kParts16 - 1))) & mask;
-        const uint64_t ka = (uint64_t)(kh_base + p * dec.k_ps + row * a.k_rs), va = (uint64_t)(vh_base + p * dec.v_ps + row * a.v_rs);
-        no_page = (uint32_t)__builtin_amdgcn_ballot_w64(!there && 16 * (lane & (kParts16 - 1)) < left) & ((1u << kParts16) - 1u);
+        // a load brings four keys, through a descriptor of exactly those that are there
         const uint32_t k4 = (uint32_t)((lane >> 4) * (int)a.k_rs * 2 + ((lane & 15) ^ ((4 * wave + (lane >> 4)) & 15)) * 16);
         const uint32_t v4 = (uint32_t)((lane >> 4) * (int)a.v_rs * 2 + ((lane & 15) ^ vswz(4 * wave + (lane >> 4))) * 16);
-        auto part = [&](uint64_t at, int key, int64_t rs, uint32_t n_bytes) {
-          const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)at, key >> 4), hi = __builtin_amdgcn_readlane((uint32_t)(at >> 32), key >> 4);
-          return make_rsrc((const char *)(((uint64_t)hi << 32 | lo) + (uint32_t)((key & 15) * (int)rs * 2)), n_bytes);
-        };
         auto issue = [&](auto rows) {              // rows(key): those of the four keys from `key` on that are there
 #pragma unroll
           for (int it = 0; it < kLoads; ++it) {
@@ -537,9 +541,10 @@ __device__ __forceinline__ bool fwd_body(const FwdArgs &a, const MoreArgs<DEC, P
             dma16(part(va, vk, a.v_rs, bytes(rows(vk), a.v_rs)), vd + slot * 1024, v4);
           }
         };
-        if (no_page == 0 && left >= SK) issue([](int) { return 4; });
-        else issue([&](int key) { return (no_page >> (key >> 4)) & 1 ? 0 : max(0, min(4, left - key)); });
+        if (all) issue([](int) { return 4; });
+        else issue([&](int key) { return is_gone(key) ? 0 : max(0, min(4, left - key)); });
       }
+      no_page = gone;
       load_entries(tile + 1);
     }
   };
@@ -807,7 +812,9 @@ __device__ __forceinline__ bool fwd_body(const FwdArgs &a, const MoreArgs<DEC, P
     }
     return false;
   };
-  if constexpr (PAGED) load_entries(t_lo);
+  if constexpr (PAGED) {
+    if (t_lo > 0) load_entries(t_lo);
+  }
   if (t_lo < t_hi) issue_tile(t_lo, std::integral_constant<int, 0>());
   if constexpr (DEC) {
     if (wave_has_rows || is_k) {
@@ -1407,6 +1414,7 @@ FwdPlan plan_paged(int hp, int num_seqs, int max_sq, int max_sk, int64_t total_q
       const float parts = ragged ? 0.6f * ns + 0.5f : (float)ns;   // of a tile
       const float rounds = (float)tiles / (float)slots * (ns == 1 ? (ragged ? 0.85f : 1.f) : parts);
       float cost = (f.full * chunk + f.group) * (ns == 1 ? std::max(1.f, rounds) : std::max(1.45f, rounds + 0.35f));
+      if (ns == 1 && f.nw == 4) cost *= 1.08f;   // (half the rows for each K/V tile: 12 x 700 x 4099 estimated 157 / 161 us, took 186 / 160)
       if (ns > 1) cost += f.combine + 2.f + (float)total_q * (float)num_heads * 1024.f * parts / 5e6f;   // written and read back at 5 TB/s
       if (cost < best_cost) {
         best_cost = cost;
