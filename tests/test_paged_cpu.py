@@ -135,3 +135,22 @@ def test_c_abi_refusals(ptr):
                cols=4, used=p, max_k=128, bias=None, b_s=0, b_h=0, scale=0.1, out=p, o_rs=2048, ws=p, ws_n=1 << 30, stream=None)
     for change, text in bad_pool + more + ((dict(o_rs=2040), "every head"), (dict(n=-1), "sequence count"), (dict(qkv=None), "null pointer")):
         assert text in _call("tg_paged_decode_attention", dec, **change), change
+
+
+def test_workspace_sizes():
+    """A workspace serves every smaller call; sizes that no call takes need none."""
+    from tokengate_amd import _lib
+    lib = _lib.load()
+    size = lib.tg_paged_decode_attention_workspace_size
+    for h, hkv in ((16, 8), (16, 1), (5, 5), (28, 4)):
+        for n in (1, 300, 5000, 1 << 20):
+            sizes = [size(b, h, hkv, n) for b in (1, 2, 8, 31, 64, 200, 1000, 2048, 5000, 60000)]
+            assert sizes == sorted(sizes)
+        assert [size(8, h, hkv, n) for n in (1, 200, 3000, 40000)] == sorted(size(8, h, hkv, n) for n in (1, 200, 3000, 40000))
+        assert size(0, h, hkv, 100) == size(-1, h, hkv, 100) == size(4, h, hkv, 0) == size(4, h, 0, 9) == size(4, 7, 3, 100) == 0
+    size = lib.tg_paged_attention_workspace_size
+    assert size(1, 33, 32769, 33, 16, 8) > 0 and size(1, 4096, 4096, 4096, 16, 8) >= 0
+    assert size(8, 2 ** 31 - 1, 6000, 160, 16, 8) == size(8, 160, 6000, 160, 16, 8)
+    for bad in ((0, 33, 900, 33, 16, 8), (1, 0, 900, 33, 16, 8), (1, 33, 0, 33, 16, 8), (1, 33, 900, 0, 16, 8), (1, 33, 900, 33, 15, 8),
+                (-1, 33, 900, 33, 16, 8), (1, 33, 900, 33, 16, 0)):
+        assert size(*bad) == 0

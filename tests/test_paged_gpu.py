@@ -216,6 +216,64 @@ def test_attention_whatever_unused_rows_hold(fill, page, bias):
     _attention([5, 70], [5, 777], 16, 8, page, bias=_normal_bias if bias else None, fill=fill)
 
 
+@pytest.mark.parametrize("new,used,H,Hkv,page,bias", [
+    ([1 + b % 23 for b in range(70)], [40 + 3 * b for b in range(70)], 16, 8, 16, True),
+    ([3] * 66, [1900 + b for b in range(66)], 4, 2, 64, True), ([b % 3 for b in range(300)], [b % 3 + b for b in range(300)], 5, 5, 32, False),
+    ([129] * 65, [700] * 65, 4, 4, 16, False)])
+def test_attention_of_many_sequences(new, used, H, Hkv, page, bias):
+    """More sequences than lanes; every sequence has keys of no page."""
+    def prepare(cache, table, _):
+        table[:, 1] = cache.n_pages
+    _attention(new, used, H, Hkv, page, bias=_normal_bias if bias else None, seed=len(new), prepare=prepare)
+
+
+@pytest.mark.parametrize("page,missing,masked", [(16, False, False), (64, True, False), (32, True, True), (128, False, True)])
+def test_attention_of_long_caches(page, missing, masked):
+    """Few rows over many keys, cut into chunks, some of them without a key that is seen."""
+    def bias(g, B, H, n):
+        x = _normal_bias(g, B, H, n)
+        if masked:
+            x[:, 1, 64:] = -math.inf
+            x[3, 2] = -math.inf
+            x[4, 3, ::2] = torch.finfo(torch.float32).min
+        return x
+
+    def prepare(cache, table, _):
+        if missing:
+            table[1, 3:], table[2, :40 * 16 // page], table[5, ::3] = -1, 2 ** 31 - 1, -7
+    used = [6000, 5999, 4100, 33, 5000, 3001, 128, 20]
+    _, _, _, out = _attention([20, 1, 33, 33, 7, 0, 40, 20], used, 8, 4, page, bias=bias, prepare=prepare)
+    if masked:
+        assert bool((out[54:87, 2] == 0).all())
+
+
+def test_attention_past_the_last_level_cache():
+    """Long prompt parts of sequences whose keys outgrow it."""
+    _attention([1100, 1030], [40000, 38001], 4, 4, 64, bias=_normal_bias)
+
+
+def test_attention_sizes_at_their_ends():
+    """A max_q far past every segment, a max_k of 0, one page table and one bias for all sequences."""
+    from tokengate_amd import paged as P
+    g = _gen(11)
+    H, Hkv, page, new, n = 8, 4, 32, [5, 40, 1], 70
+    table, n_pages = table_of(g, [n], page)
+    cache = cache_of(g, n_pages, Hkv, page)
+    q, cu, used = normal(g, 46, H, D), _i32([0, 5, 45, 46]), _i32([n] * 3)
+    bias = _normal_bias(g, 1, 1, n)
+    tables, biases = table.expand(3, -1), bias.expand(3, H, n)
+    a = P.paged_attention(q, cache, tables, cu, used, 40, n, SCALE, biases)
+    b = P.paged_attention(q, cache, tables, cu, used, 2 ** 31 - 1, n, SCALE, biases)
+    assert torch.equal(a, b)
+    k, v, there = keys_of(cache, table, 0, n)
+    for b, m in enumerate(new):
+        rows = slice(int(cu[b]), int(cu[b]) + m)
+        near(a[rows], *attend(q[rows], k, v, there, SCALE, bias[0].expand(H, n), n - m), BF)
+    assert bool((P.paged_attention(q, cache, tables, cu, used, 40, 0, SCALE) == 0).all())
+    assert P.paged_attention(q, cache, tables[:0], cu[:1], used[:0], 40, n, SCALE).shape == q.shape
+    assert P.paged_attention(q[:0], cache, tables, cu, used, 40, n, SCALE).shape == (0, H, D)
+
+
 def test_attention_more_queries_than_keys():
     """The first queries see no key: zeros."""
     _, _, _, out = _attention([20, 9], [6, 0], 16, 8, 16)
@@ -445,3 +503,46 @@ def test_decode_large_values(H, Hkv):
 def test_decode_more_keys_than_max():
     """kv_used past max_k: the first max_k keys, of which the last is the new one."""
     _decode([100, 70], 16, 8, 16, bias=_normal_bias, max_k=64)
+
+
+def test_decode_of_very_many_sequences():
+    """More units than the workspace has counters: none is cut, and the others' rows stay as they were."""
+    from tokengate_amd import paged as P
+    H, Hkv, page, B = 16, 8, 16, 2100
+    g = _gen(12)
+    shape, lw = shape_of(H, Hkv), weights(g)
+    used = [b % 5 for b in range(B)]
+    used[7] = 3000
+    table, n = table_of(g, [max(u, 1) if u < 99 else u for u in used], page)
+    cache = cache_of(g, n, Hkv, page)
+    qkv, rope = normal(g, B, (H + 2 * Hkv) * D), torch.rand(B, 64, 2, generator=g, device=DEV)
+    ws = P.paged_decode_attention_workspace(B, shape, 3000, DEV)
+    out = P.paged_decode_attention(qkv, rope, lw, shape, cache, table, _i32(used), 3000, SCALE, ws)
+    assert not bool(ws[:1 << 16].any())
+    few = list(range(40)) + list(range(B - 40, B))
+    q = P.paged_append(qkv, rope, lw, shape, cache, torch.full((B,), -1, dtype=torch.int32, device=DEV))
+    for b in few:
+        if used[b] == 0:
+            assert bool((out[b] == 0).all())
+            continue
+        near(out[b:b + 1], *attend(q[b:b + 1], *keys_of(cache, table, b, used[b]), SCALE), BF * BF, b)
+    few = _i32(few).long()                                       # the workspace serves a cut launch of fewer
+    a = P.paged_decode_attention(qkv[few], rope[few], lw, shape, cache, table[few], _i32(used)[few], 3000, SCALE, ws)
+    two = P.paged_decode_attention_workspace(80, shape, 3000, DEV)
+    assert torch.equal(a, P.paged_decode_attention(qkv[few], rope[few], lw, shape, cache, table[few], _i32(used)[few], 3000, SCALE, two))
+
+
+def test_decode_without_keys():
+    from tokengate_amd import paged as P
+    g = _gen(13)
+    H, Hkv, page = 16, 8, 16
+    shape, lw = shape_of(H, Hkv), weights(g)
+    cache = cache_of(g, 4, Hkv, page)
+    k0 = cache.k.clone()
+    qkv, rope = normal(g, 3, (H + 2 * Hkv) * D), torch.rand(3, 64, 2, generator=g, device=DEV)
+    ws = P.paged_decode_attention_workspace(3, shape, 0, DEV)
+    table = torch.zeros(3, 1, dtype=torch.int32, device=DEV)
+    assert bool((P.paged_decode_attention(qkv, rope, lw, shape, cache, table, _i32([0, 0, 0]), 16, SCALE, ws) == 0).all())
+    assert bool((P.paged_decode_attention(qkv, rope, lw, shape, cache, table, _i32([1, 2, 3]), 0, SCALE, ws) == 0).all())
+    assert P.paged_decode_attention(qkv[:0], rope, lw, shape, cache, table, _i32([]), 16, SCALE, ws).shape == (0, H, D)
+    assert torch.equal(cache.k, k0)

@@ -1875,7 +1875,7 @@ extern "C" int64_t tg_paged_attention_workspace_size(int32_t num_seqs, int32_t m
   if (num_seqs <= 0 || max_seqlen_q <= 0 || max_seqlen_k <= 0 || total_q <= 0 || num_heads <= 0 || num_heads_k <= 0 || num_heads % num_heads_k != 0)
     return 0;
   const int hp = (num_heads / num_heads_k) % 2 == 0 ? 2 : 1;
-  return plan_paged(hp, num_seqs, max_seqlen_q, max_seqlen_k, total_q, num_heads, num_heads_k, INT64_MAX).split.bytes;
+  return plan_paged(hp, num_seqs, std::min(max_seqlen_q, total_q), max_seqlen_k, total_q, num_heads, num_heads_k, INT64_MAX).split.bytes;
 }
 
 extern "C" int tg_paged_attention(const void *q, int64_t q_row_stride, int64_t q_head_stride, const void *k_pages,
@@ -1906,6 +1906,7 @@ extern "C" int tg_paged_attention(const void *q, int64_t q_row_stride, int64_t q
   TG_CHECK(softmax_scale > 0.f, "%s: softmax_scale must be positive", what);
   TG_CHECK(!bias_raw || (bias_seq_stride >= 0 && bias_head_stride >= 0), "%s: negative bias stride", what);
   if (num_seqs == 0 || max_seqlen_q == 0 || total_q == 0) return 0;
+  max_seqlen_q = std::min(max_seqlen_q, total_q);   // (no segment is longer)
   FwdArgs a{};
   a.q = static_cast<const bf16_t *>(q);
   a.k = c.k;

@@ -201,7 +201,8 @@ def paged_attention(q: torch.Tensor, cache: PagedKV, page_table: torch.Tensor, c
     """decoder.varlen_kv_attention over pages (tg_paged_attention): causal attention of every packed query segment cu_q[b]
     .. cu_q[b + 1] - 1 of q (T, H, 128), at most max_q rows, over keys 0 .. kv_used[b] - 1 of its sequence (at most max_k), the
     last query with the last key.  bias_raw (nseq, H, >= max_k) fp32 in raw-score units; -inf hides a key from a head
-    whatever its row holds.  Rows that see no key get zeros, rows of no segment keep what out holds."""
+    whatever its row holds; rows of keys that only come after a query have to be finite.  Rows that see no key get zeros, rows of no
+    segment keep what out holds."""
     what, dev, n = "paged_attention", cache.device_index, cu_q.numel() - 1
     if q.dtype is not torch.bfloat16 or q.dim() != 3 or q.shape[2] != HEAD_DIM or q.stride(2) != 1 or q.get_device() != dev:
         raise RuntimeError("paged_attention: q must be bf16 (rows, H, 128), values contiguous, on the cache's device")
