@@ -263,16 +263,19 @@ template <int KS> constexpr int bias_row() { return step_keys<KS>() + 4; }
 
 // PAGES: 0 none, 1 of 16 or 32 rows, 2 of 64 and more.
 //
-// FAR (pages) handles keys that a bias of -inf hides or that have no page, which weigh nothing whatever their rows hold,
-// and biases as large as a mask's (2^30 and more), whose logits are scaled and rounded first (in one multiply-add with the
-// scale the product's rest would be a large number there).  Without FAR a workgroup whose keys have any of these ends at
-// the first such tile, before it has written anything, and returns true.  (Both in one loop, by branches or one loop after the
-// other, kept neither the registers nor the exponentials beside the products: 2320 rows with bias 54 to 65 us.)
+// FAR (pages) hides keys whatever their rows hold: those of no page, and those with a bias of -inf, which elsewhere only adds
+// -inf to a logit that has to be finite, with the weight 0 for a value that has to be.  It also scales and rounds a logit before the
+// maximum is taken off (in one multiply-add with the scale the rest of a product that is 2^28 and more would be a large
+// number).  Without FAR a workgroup ends at the first tile with a key of no page, or behind the last one if its sums are not finite
+// or a maximum is that large, has written nothing and returns true.  (Both in one loop, by branches or one loop after the
+// other, kept neither the registers nor the exponentials beside the products: 2320 rows with bias 54 to 65 us.  A test of
+// every tile's biases cost 12 % at 8192 rows x 32768 keys.)
 template <int NW, int KS, int HP, bool CAUSAL, bool HAS_BIAS, bool VARLEN, bool DEC, int PAGES, bool FAR>
 __device__ __forceinline__ bool fwd_body(const FwdArgs &a, const MoreArgs<DEC, PAGES> &dec, char (&ks0)[tile_bytes<KS>()],
                                          char (&ks1)[tile_bytes<KS>()], char (&vs0)[tile_bytes<KS>()],
                                          char (&vs1)[tile_bytes<KS>()], float (&bs0)[HP][bias_row<KS>()],
-                                         float (&bs1)[HP][bias_row<KS>()], [[maybe_unused]] char *zeros) {
+                                         float (&bs1)[HP][bias_row<KS>()], [[maybe_unused]] char *zeros,
+                                         [[maybe_unused]] int *redo) {
   constexpr bool PAGED = PAGES != 0;
   static_assert(!DEC || (VARLEN && NW == 4 && KS == 1), "the decode step's form");
   static_assert(!PAGED || (VARLEN && CAUSAL && !DEC), "the paged form");
@@ -350,17 +353,21 @@ __device__ __forceinline__ bool fwd_body(const FwdArgs &a, const MoreArgs<DEC, P
     }
   }
 
-  // Pages: the entries of the next tile to be issued, lane q that of its 16 keys (PAGES 2: 64) from 16 q (64 q) on, loaded while
-  // the tile before it is computed (the first tile's before anything else); and, by bit, which 16 keys of the issued tile
-  // have no page.
-  constexpr int kPartKeys = PAGES == 2 ? 64 : 16;
+  // Pages: where 64 parts of 16 keys (PAGES 2: 64) begin in K and V is computed at once, by lane, for the next kBatch tiles; the
+  // entries of the batch after it are loaded meanwhile (the first ones before anything else).  Tile by tile, 8192 rows x
+  // 8192 keys of 64-row pages took 266 us, so 263 (16-row pages 292, 277).  parts_gone: by bit, which parts have no page;
+  // no_page: which 16 keys of the issued tile.
+  constexpr int kPartKeys = PAGES == 2 ? 64 : 16, kParts = SK / kPartKeys, kBatch = 64 / kParts;
   [[maybe_unused]] int32_t entry = 0;
+  [[maybe_unused]] uint64_t k_at = 0, v_at = 0, parts_gone = 0;
   [[maybe_unused]] uint32_t no_page = 0;
   [[maybe_unused]] auto load_entries = [&](int tile) {
-    if constexpr (PAGED)
-      entry = dec.table[b * dec.table_rs + min((tile * SK + kPartKeys * (lane & (SK / kPartKeys - 1))) >> dec.lg, dec.cols - 1)];
+    if constexpr (PAGED) entry = dec.table[b * dec.table_rs + min((tile * SK + kPartKeys * lane) >> dec.lg, dec.cols - 1)];
   };
   if constexpr (PAGED) load_entries(0);
+  if constexpr (PAGED && HAS_BIAS && !FAR) {
+    if (tid == 0) *redo = 0;                       // (the ring's first barrier is behind it)
+  }
   int sq = a.sq, sk = a.sk;
   int64_t row0 = 0, krow0 = 0;
   if constexpr (DEC) {
@@ -500,16 +507,21 @@ __device__ __forceinline__ bool fwd_body(const FwdArgs &a, const MoreArgs<DEC, P
       auto k_rows = [](int it) { return kWaves == 8 ? 32 * it : 32 * (it >> 1) + 4 * (it & 1); };
       auto v_rows = [](int it) { return 4 * kWaves * it; };
       auto bytes = [&](int n, int64_t rs) { return n > 0 ? (uint32_t)((n - 1) * (int)rs + kD) * 2u : 0u; };   // of n rows
-      // lane q holds where the keys from kPartKeys q on begin
-      const int part_row = kPartKeys * (lane & (SK / kPartKeys - 1));
-      const bool there = (uint32_t)entry < (uint32_t)dec.n_pages;
-      const int64_t p = there ? entry : 0, row = (tile * SK + part_row) & mask;
-      const uint64_t ka = (uint64_t)(kh_base + p * dec.k_ps + row * a.k_rs), va = (uint64_t)(vh_base + p * dec.v_ps + row * a.v_rs);
-      uint32_t gone = (uint32_t)__builtin_amdgcn_ballot_w64(!there && part_row < left) & ((1u << (SK / kPartKeys)) - 1u);
+      const int nth = (tile - t_lo) & (kBatch - 1);
+      if (nth == 0) {
+        const int key = tile * SK + kPartKeys * lane;
+        const bool there = (uint32_t)entry < (uint32_t)dec.n_pages;
+        const int64_t p = there ? entry : 0, row = key & mask;
+        k_at = (uint64_t)(kh_base + p * dec.k_ps + row * a.k_rs);
+        v_at = (uint64_t)(vh_base + p * dec.v_ps + row * a.v_rs);
+        parts_gone = __builtin_amdgcn_ballot_w64(!there && key < sk);
+        load_entries(tile + kBatch);
+      }
+      const uint32_t gone = (uint32_t)(parts_gone >> (kParts * nth)) & ((1u << kParts) - 1u);
       const bool all = gone == 0 && left >= SK;
       auto part = [&](uint64_t at, int key, int64_t rs, uint32_t n_bytes) {   // from `key` on, of n_bytes
-        const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)at, key / kPartKeys);
-        const uint32_t hi = __builtin_amdgcn_readlane((uint32_t)(at >> 32), key / kPartKeys);
+        const int q = kParts * nth + key / kPartKeys;
+        const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)at, q), hi = __builtin_amdgcn_readlane((uint32_t)(at >> 32), q);
         return make_rsrc((const char *)(((uint64_t)hi << 32 | lo) + (uint32_t)((key & (kPartKeys - 1)) * (int)rs * 2)), n_bytes);
       };
       auto is_gone = [&](int key) { return (gone >> (key / kPartKeys)) & 1; };
@@ -518,7 +530,7 @@ __device__ __forceinline__ bool fwd_body(const FwdArgs &a, const MoreArgs<DEC, P
           constexpr int kOf64 = kLoads / (SK / 64);
 #pragma unroll
           for (int i = 0; i < SK / 64; ++i) {      // loads kOf64 of every 64 keys
-            const brsrc_t kr = part(ka, 64 * i, 0, bytes(rows(64 * i), a.k_rs)), vr = part(va, 64 * i, 0, bytes(rows(64 * i), a.v_rs));
+            const brsrc_t kr = part(k_at, 64 * i, 0, bytes(rows(64 * i), a.k_rs)), vr = part(v_at, 64 * i, 0, bytes(rows(64 * i), a.v_rs));
 #pragma unroll
             for (int it = 0; it < kOf64; ++it) {
               dma16(kr, kd + (wv + (i * kOf64 + it) * kWaves) * 1024, koff[0] + (uint32_t)(k_rows(it) * (int)a.k_rs * 2));
@@ -528,7 +540,7 @@ __device__ __forceinline__ bool fwd_body(const FwdArgs &a, const MoreArgs<DEC, P
         };
         if (all) issue([](int) { return 64; });
         else issue([&](int key) { return is_gone(key) ? 0 : min(left - key, 64); });
-        gone = (gone & 1u ? 15u : 0u) | (gone & 2u ? 0xf0u : 0u);
+        no_page = (gone & 1u ? 15u : 0u) | (gone & 2u ? 0xf0u : 0u);
       } else {
         // a load brings four keys, through a descriptor of exactly those that are there
         const uint32_t k4 = (uint32_t)((lane >> 4) * (int)a.k_rs * 2 + ((lane & 15) ^ ((4 * wave + (lane >> 4)) & 15)) * 16);
@@ -537,15 +549,14 @@ __device__ __forceinline__ bool fwd_body(const FwdArgs &a, const MoreArgs<DEC, P
 #pragma unroll
           for (int it = 0; it < kLoads; ++it) {
             const int slot = wv + it * kWaves, kk = kperm(4 * slot), vk = 4 * slot;
-            dma16(part(ka, kk, a.k_rs, bytes(rows(kk), a.k_rs)), kd + slot * 1024, k4);
-            dma16(part(va, vk, a.v_rs, bytes(rows(vk), a.v_rs)), vd + slot * 1024, v4);
+            dma16(part(k_at, kk, a.k_rs, bytes(rows(kk), a.k_rs)), kd + slot * 1024, k4);
+            dma16(part(v_at, vk, a.v_rs, bytes(rows(vk), a.v_rs)), vd + slot * 1024, v4);
           }
         };
         if (all) issue([](int) { return 4; });
         else issue([&](int key) { return is_gone(key) ? 0 : max(0, min(4, left - key)); });
+        no_page = gone;
       }
-      no_page = gone;
-      load_entries(tile + 1);
     }
   };
   auto issue_tile = [&](int tile, auto buf_c) {
@@ -620,16 +631,7 @@ __device__ __forceinline__ bool fwd_body(const FwdArgs &a, const MoreArgs<DEC, P
     }
     [[maybe_unused]] const uint32_t gone = no_page >> (KN / 16 * kg);   // of this tile, from this wave's keys on
     if constexpr (PAGED && !FAR) {
-      bool stop = no_page != 0;
-      if constexpr (HAS_BIAS) {                    // every wave looks at all heads' biases
-        float big = 0.f;
-#pragma unroll
-        for (int i = 0; i < HP; ++i)
-#pragma unroll
-          for (int j = 0; j < SK / 64; ++j) big = fmaxf(big, fabsf(bslot(buf_c)[i][64 * j + lane]));
-        stop |= __builtin_amdgcn_ballot_w64(!(big < 0x1p30f)) != 0;
-      }
-      if (stop) return true;
+      if (no_page != 0) return true;
     }
     if (t + 1 < t_hi) issue_tile(t + 1, std::integral_constant<int, 1 - BUF>());
     if (!wave_has_rows || (CAUSAL && n0 > qw_hi + off)) return false;
@@ -770,16 +772,56 @@ __device__ __forceinline__ bool fwd_body(const FwdArgs &a, const MoreArgs<DEC, P
     }
     // P rounded to bf16 pairs (the B operand of P V and of the row-sum product)
     uint32_t pk[2][KB][2];
+    auto weigh = [&](int cb, int kb, int i) {
+      const float p0 = fast_exp2(fmaf(sacc[cb][kb][i], to_log2, mneg[cb]));
+      const float p1 = fast_exp2(fmaf(sacc[cb][kb][i + 1], to_log2, mneg[cb]));
+      pk[cb][kb][i >> 1] = pack_bf16x2(p0, p1);
+    };
+    auto step_weights = [&](int st, int cb) {
+      return __builtin_bit_cast(bf16x8, u32x4{pk[cb][2 * st][0], pk[cb][2 * st][1], pk[cb][2 * st + 1][0], pk[cb][2 * st + 1][1]});
+    };
+    const char *vbuf = vslot(buf_c) + KN * kg * kKRowBytes;
+    if constexpr (PAGED && !FAR) {
+      // The order that the compiler finds for the other forms, written out, as it doesn't beside a second pass: the first key
+      // step's weights, then products with the values of the next kAhead on their way and the second step's weights between:
+      // 8192 rows x 32768 keys 1665 to 1567 us (contiguous 1560), 2320 x 2320 with bias 46.5 to 43.3.
+      constexpr int kAhead = 4;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) weigh(e >> 2, (e >> 1) & 1, 2 * (e & 1));
+      s16x4 lo[kAhead], hi[kAhead];
+      auto read_v = [&](int n) {
+        const char *at = vbuf + 32 * (n >> 3) * kKRowBytes + vch[n & 7];
+        lo[n % kAhead] = lds_read_tr16(at);
+        hi[n % kAhead] = lds_read_tr16(at + 4 * kKRowBytes);
+      };
+#pragma unroll
+      for (int n = 0; n < kAhead; ++n) read_v(n);
+      __builtin_amdgcn_sched_barrier(0);
+      bf16x8 pb[2];
+#pragma unroll
+      for (int n = 0; n < 8 * ST; ++n) {
+        if (n % 8 == 0) {
+#pragma unroll
+          for (int cb = 0; cb < 2; ++cb) {
+            pb[cb] = step_weights(n >> 3, cb);
+            lacc[cb] = mfma16(ones, pb[cb], lacc[cb]);
+          }
+        }
+        const bf16x8 vf = __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo[n % kAhead], hi[n % kAhead], 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+        for (int cb = 0; cb < 2; ++cb) oacc[cb][n & 7] = mfma16(vf, pb[cb], oacc[cb][n & 7]);
+        if (n + kAhead < 8 * ST) read_v(n + kAhead);
+        if (n + 8 < 8 * ST) weigh(n >> 2, KB / 2 + ((n >> 1) & 1), 2 * (n & 1));
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      return false;
+    }
 #pragma unroll
     for (int cb = 0; cb < 2; ++cb) {
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb) {
 #pragma unroll
-        for (int i = 0; i < 4; i += 2) {
-          const float p0 = fast_exp2(fmaf(sacc[cb][kb][i], to_log2, mneg[cb]));
-          const float p1 = fast_exp2(fmaf(sacc[cb][kb][i + 1], to_log2, mneg[cb]));
-          pk[cb][kb][i >> 1] = pack_bf16x2(p0, p1);
-        }
+        for (int i = 0; i < 4; i += 2) weigh(cb, kb, i);
       }
     }
     // ---- O^T += V^T P^T: ST key steps x 8 d-blocks x 2 column blocks ----
@@ -787,16 +829,12 @@ __device__ __forceinline__ bool fwd_body(const FwdArgs &a, const MoreArgs<DEC, P
     for (int st = 0; st < ST; ++st) {
       bf16x8 pb[2];
 #pragma unroll
-      for (int cb = 0; cb < 2; ++cb) {
-        const u32x4 w = {pk[cb][2 * st][0], pk[cb][2 * st][1], pk[cb][2 * st + 1][0], pk[cb][2 * st + 1][1]};
-        pb[cb] = __builtin_bit_cast(bf16x8, w);
-      }
+      for (int cb = 0; cb < 2; ++cb) pb[cb] = step_weights(st, cb);
 #pragma unroll
       for (int cb = 0; cb < 2; ++cb) lacc[cb] = mfma16(ones, pb[cb], lacc[cb]);
       const uint32_t krow = (uint32_t)(32 * st * kKRowBytes);
 #pragma unroll
       for (int dblk = 0; dblk < 8; ++dblk) {
-        const char *vbuf = vslot(buf_c) + KN * kg * kKRowBytes;
         const char *vlo = vbuf + krow + vch[dblk], *vhi = vbuf + krow + 4 * kKRowBytes + vch[dblk];
         if constexpr (FAR && HAS_BIAS) {   // rows that the bias hides from this wave's head read as 0
           if ((hidden >> (8 * st + (c16 >> 2))) & 1) vlo = zeros;
@@ -855,6 +893,24 @@ __device__ __forceinline__ bool fwd_body(const FwdArgs &a, const MoreArgs<DEC, P
     if (tile_step(t + 1, std::integral_constant<int, 1>())) return true;
   }
   if (t < t_hi && tile_step(t, std::integral_constant<int, 0>())) return true;
+  if constexpr (PAGED && HAS_BIAS && !FAR) {
+    if (t_lo < t_hi) {
+      float rest = 0.f;                            // stays 0 where all are finite
+      bool far = false;
+#pragma unroll
+      for (int cb = 0; cb < 2; ++cb) {
+#pragma unroll
+        for (int d = 0; d < 8; ++d)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) rest = fmaf(oacc[cb][d][i], 0.f, rest);
+        rest = fmaf(lacc[cb][0], 0.f, rest);
+        far |= fabsf(mrun[cb]) >= 0x1p28f && mrun[cb] != -INFINITY;
+      }
+      if (__builtin_amdgcn_ballot_w64(far || rest != 0.f) != 0 && lane == 0) *redo = 1;
+      __syncthreads();
+      if (*redo != 0) return true;
+    }
+  }
 
   // ---- merge of the KS key groups (KS > 1): a column's max over the groups, every group's row sum
   // and O rescaled to it (weight 0 where a group saw no key), then group g adds up d-blocks DB g ..
@@ -1035,9 +1091,10 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void keybias_fwd_kernel(FwdArgs a,
   __shared__ __attribute__((aligned(1024))) char ks0[tile_bytes<KS>()], ks1[tile_bytes<KS>()];
   __shared__ __attribute__((aligned(1024))) char vs0[tile_bytes<KS>()], vs1[tile_bytes<KS>()];
   __shared__ __attribute__((aligned(256))) float bs0[HP][bias_row<KS>()], bs1[HP][bias_row<KS>()];
+  __shared__ int redo;
   auto run = [&](auto far_c, char *zeros) {
     return fwd_body<NW, KS, HP, CAUSAL, HAS_BIAS, VARLEN, DEC, PAGES, decltype(far_c)::value>(a, dec, ks0, ks1, vs0, vs1, bs0, bs1,
-                                                                                              zeros);
+                                                                                              zeros, &redo);
   };
   if (run(std::false_type(), nullptr)) {          // workgroup-uniform
     if constexpr (PAGES != 0) {
@@ -1387,7 +1444,7 @@ FwdPlan plan_varlen(int hp, int max_sq, int max_sk, int64_t units, bool causal, 
 // once, 0.45 of one more round: 8 of 200 and 12000 165 us in 4 chunks, 122 in 8).  Sequences with many tiles each whose K/V outgrow the last-level
 // cache keep their own order (varlen_level_order's reason).
 // us of the varlen launch's plan / this one / the quickest of 16 forms with up to 32 chunks, 16 / 8 heads, ragged sequences x
-// rows x keys up to: 12 x 700 x 4099 225 / 178 / 161; 8 x 200 x 12000 177 / 122 / 115; 24 x 100 x 1500 50 / 35 / 35; 3 x 2500 x 8000
+// rows x keys up to (with the kernel of an earlier step): 12 x 700 x 4099 225 / 161 / 161; 8 x 200 x 12000 177 / 122 / 115; 24 x 100 x 1500 50 / 35 / 35; 3 x 2500 x 8000
 // 305 / 235 / 216; 8 x 1000 x 1000 39 / 35 / 35; 4 x 512 x 512 25 / 18 / 18; 16 x 16 x 4000 43 / 41 / 41; 4 x 64 x 8000 34 / 38 / 34.
 FwdPlan plan_paged(int hp, int num_seqs, int max_sq, int max_sk, int64_t total_q, int num_heads, int num_heads_k,
                    int64_t workspace_bytes) {
