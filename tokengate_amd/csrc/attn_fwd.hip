@@ -261,7 +261,10 @@ template <int KS> constexpr int tile_bytes() { return step_keys<KS>() * kKRowByt
 // bias rows padded by 4 floats so that the two heads' rows fall on different banks
 template <int KS> constexpr int bias_row() { return step_keys<KS>() + 4; }
 
-// PAGES: 0 none, 1 of 16 or 32 rows, 2 of 64 and more.
+// PAGES: 0 none, 1 of 16 or 32 rows (a load's four keys through a descriptor of their own), 2 of 64 and more (64 keys through one).
+// us over contiguous K and V / pages of 64 rows / of 16, 16 / 8 heads, causal: 1024 x 1024 17.6 / 18.9 / 20.1, 2320 x 2320
+// 39.6 / 41.4 / 44.0, 8192 x 8192 243 / 250 / 260, 8192 x 32768 1580 / 1608 / 1650; with bias 39.8 / 43.3 / 45.7 and 1605 / 1656 / 1702.
+// The order of the pages, and rows of a head apart or together, make no difference.
 //
 // FAR (pages) hides keys whatever their rows hold: those of no page, and those with a bias of -inf, which elsewhere only adds
 // -inf to a logit that has to be finite, with the weight 0 for a value that has to be.  It also scales and rounds a logit before the
@@ -1441,11 +1444,12 @@ FwdPlan plan_varlen(int hp, int max_sq, int max_sk, int64_t units, bool causal, 
 // the form, and cut into as many chunks, as an estimate finds quickest: the longest chunk, or the steps spread over the places
 // (the lengths behind the maxima are not known here: of a ragged batch's tiles 0.85 of the most, in 0.6 ns + 0.5 chunks),
 // and for chunks the second launch and its traffic, and, as two that share a CU end long before others do where they all fit at
-// once, 0.45 of one more round: 8 of 200 and 12000 165 us in 4 chunks, 122 in 8).  Sequences with many tiles each whose K/V outgrow the last-level
-// cache keep their own order (varlen_level_order's reason).
+// once, 0.45 of one more round: 8 of 200 and 12000 165 us in 4 chunks, 122 in 8).  Sequences with many tiles each whose K/V
+// outgrow the last-level cache keep their own order (varlen_level_order's reason).
 // us of the varlen launch's plan / this one / the quickest of 16 forms with up to 32 chunks, 16 / 8 heads, ragged sequences x
-// rows x keys up to (with the kernel of an earlier step): 12 x 700 x 4099 225 / 161 / 161; 8 x 200 x 12000 177 / 122 / 115; 24 x 100 x 1500 50 / 35 / 35; 3 x 2500 x 8000
-// 305 / 235 / 216; 8 x 1000 x 1000 39 / 35 / 35; 4 x 512 x 512 25 / 18 / 18; 16 x 16 x 4000 43 / 41 / 41; 4 x 64 x 8000 34 / 38 / 34.
+// rows x keys up to (measured before the products' order was written out, which made all 5 % quicker): 12 x 700 x 4099
+// 225 / 161 / 161; 8 x 200 x 12000 177 / 122 / 115; 24 x 100 x 1500 50 / 35 / 35; 3 x 2500 x 8000 305 / 235 / 216;
+// 8 x 1000 x 1000 39 / 35 / 35; 4 x 512 x 512 25 / 18 / 18; 16 x 16 x 4000 43 / 41 / 41; 4 x 64 x 8000 34 / 38 / 34.
 FwdPlan plan_paged(int hp, int num_seqs, int max_sq, int max_sk, int64_t total_q, int num_heads, int num_heads_k,
                    int64_t workspace_bytes) {
   const int64_t heads = num_heads / hp, units = num_seqs * heads;

@@ -66,6 +66,9 @@ struct AppendArgs {
   PagePool c;
   int groups;                    // of 16 lanes per token
 };
+// Bound by bytes: q | k | v read and written once (32768 rows 98 .. 106 us, 5.2 .. 5.6 TB/s), few rows by the launch (8: 3.1).
+// Sixteen lanes take kRowsPer heads of a token, all loads ahead of the first product; with 1 / 2 / 4 heads 32768 rows take
+// 112 / 104 / 116 us, and 110 with two whose stores go through the caches.
 constexpr int kRowsPer = 2;
 
 // (past the caches: the queries of a long prompt outgrow them, and a short one's stay in the last level)
@@ -118,8 +121,11 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a) {
 
 // ---- attention of a decode step ---------------------------------------------------------------------
 //   z_j = scale (q . k_j + bias_j),   out = sum_j e^(z_j - m) v_j / sum_j e^(z_j - m)
-// One workgroup per (sequence, KV head and up to 16 of its query heads); a wave takes 32 keys at a time, straight from
-// the pages to registers in the layouts that the matrix cores read, so nothing waits at a barrier:
+// Units of (sequence, KV head, up to 16 of its query heads) are cut into chunks on the device, from the lengths themselves
+// (find_chunk); the last workgroup of a unit to arrive merges its chunks.  A wave takes 32 keys at a time, straight from the
+// pages to registers in the layouts that the matrix cores read, so nothing waits at a barrier.  Bound by the bytes of K and V
+// where there are many keys (8 of up to 131072 keys 441 us: 5.8 TB/s; 64 of up to 4099 131: 4.8), by dependent latencies where
+// there are few: lengths and pages, norms, one tile and the waves' merge take 5.8 us, 300 keys 8.0, 2320 10.4, 32769 31.
 //   * S^T = K Q^T (v_mfma_f32_16x16x32_bf16): A holds keys, lane (n, G) (n = lane % 16, G = lane / 16) elements 32 i + 8 G
 //     .. + 7 of key 8 (n / 4) + 4 t + n % 4 of instruction t (0, 1); B the query heads, head n % HP in column n.  So lane
 //     (n, G) ends up with the logits of keys 8 G .. 8 G + 7 of its head: in the order that the weights have as O's A.
