@@ -331,6 +331,50 @@ def test_attention_masks_of_large_numbers(low):
     _attention([40], [150], 16, 8, 64, bias=bias, average=average)
 
 
+@pytest.mark.parametrize("low", [torch.finfo(torch.float32).min, -1e30, -3e9, -math.inf])
+@pytest.mark.parametrize("new,used", [([40], [300]), ([200, 30, 5], [300, 250, 777])])
+def test_attention_masks_of_the_first_keys(low, new, used):
+    """Left padding: whole tiles of masked keys, and rows that see no other, before the ones that count.  (-3e9: a
+    maximum past 2^28.)"""
+    def bias(g, B, H, n):
+        x = _normal_bias(g, B, H, n)
+        x[:, ::3, :200] = low
+        return x
+    # a row that sees masked keys alone has their average, by weights that fp32 logits near 3e9 do not give
+    _attention(new, used, 6, 3, 64, bias=bias, average=[0, 3] if low == -3e9 else [])
+
+
+@pytest.mark.parametrize("new,used", [([50], [300]), ([300, 20], [300, 450]), ([17], [5000])])
+@pytest.mark.parametrize("H,Hkv", [(8, 4), (5, 5), (6, 2)])
+def test_attention_hidden_from_some_heads(new, used, H, Hkv):
+    """Keys hidden from some heads, with rows that are no numbers: the others' outputs are no numbers where they see one, and
+    these heads' are as if the rows were not there."""
+    from tokengate_amd import paged as P
+    g, page = _gen(21), 64
+    table, n = table_of(g, used, page)
+    cache = cache_of(g, n, Hkv, page)
+    bias = _normal_bias(g, len(used), H, max(used))
+    bad = [3, 70, 71, 200]
+    for b in range(len(used)):
+        bias[b, ::2, bad] = -math.inf
+        at = slots_of(table, page, [(b, j) for j in bad]).long()
+        cache.k[at[:2] // page, :, at[:2] % page] = math.nan
+        cache.v[at[2:] // page, :, at[2:] % page] = math.inf
+    cu = [0]
+    for x in new:
+        cu.append(cu[-1] + x)
+    q = normal(g, cu[-1], H, D)
+    out = P.paged_attention(q, cache, table, _i32(cu), _i32(used), max(new), max(used), SCALE, bias)
+    seen = list(range(0, H, 2))
+    clean = P.PagedKV(*(torch.where(t.isfinite(), t, torch.zeros_like(t)) for t in (cache.k, cache.v)))
+    for b, (m, u) in enumerate(zip(new, used)):
+        rows = slice(cu[b], cu[b] + m)
+        ref, mass = attend(q[rows], *keys_of(clean, table, b, u), SCALE, bias[b, :, :u], u - m)
+        near(out[rows][:, seen], ref[:, seen], mass[:, seen], BF, b)
+        if H > 1:
+            assert not bool(out[cu[b] + m - 1, 1].isfinite().all())
+
+
 def test_attention_near_contiguous():
     """varlen_kv_attention's outputs: both are within the tolerance of float64 (their key groups and chunks, and so the order
     of their sums, may differ)."""

@@ -210,9 +210,11 @@ struct Fold {
   float mmax = -INFINITY, wsum = 0.f;
   float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 };
-template <typename Value>   // value(e): the e-th of the chunk's eight
+// value(e): the e-th of the chunk's eight.  (A chunk without a key, l = 0, is left out; one whose l is no number is too, but
+// not over pages: there visible keys' not-a-numbers reach the output at every split, as without one.)
+template <bool PAGED = false, typename Value>
 __device__ __forceinline__ void fold_values(Fold &f, float2 mc, Value value) {
-  if (!(mc.y > 0.f)) return;
+  if (PAGED ? mc.y == 0.f : !(mc.y > 0.f)) return;
   if (mc.x > f.mmax) {
     const float sc = fast_exp2(f.mmax - mc.x);   // 0 while nothing has been added yet
     f.wsum *= sc;
@@ -229,9 +231,10 @@ __device__ __forceinline__ void fold_chunk(Fold &f, float2 mc, u32x4 pv) {
   fold_values(f, mc, [&](int e) { return u32_as_f32(e & 1 ? pv[e >> 1] & 0xffff0000u : pv[e >> 1] << 16); });
 }
 // p: another group's (mmax, wsum, acc), `stride` floats apart
+template <bool PAGED = false>
 __device__ __forceinline__ void merge_fold(Fold &f, const float *p, int stride) {
   const float m2 = p[0], w2 = p[stride];
-  if (!(w2 > 0.f)) return;
+  if (PAGED ? w2 == 0.f : !(w2 > 0.f)) return;
   const float mn = fmaxf(f.mmax, m2);
   const float s1 = fast_exp2(f.mmax - mn), s2 = fast_exp2(m2 - mn);   // s1 = 0 if mmax = -inf
   f.wsum = f.wsum * s1 + w2 * s2;
@@ -1171,7 +1174,7 @@ __global__ __launch_bounds__(512) void keybias_fwd_combine_kernel(FwdArgs a, int
       if constexpr (PAGED) {
         const f32x4 *pf = reinterpret_cast<const f32x4 *>(po) + pw * (16 * 64) + 2 * j * 64 + lane;
         const f32x4 v0 = pf[0], v1 = pf[64];
-        fold_values(f, mc, [&](int e) { return e < 4 ? v0[e & 3] : v1[e & 3]; });
+        fold_values<true>(f, mc, [&](int e) { return e < 4 ? v0[e & 3] : v1[e & 3]; });
       } else {
         const u32x4 pv = po[pw * (8 * 64) + j * 64 + lane];
         fold_chunk(f, mc, pv);
@@ -1181,7 +1184,7 @@ __global__ __launch_bounds__(512) void keybias_fwd_combine_kernel(FwdArgs a, int
   if (cg > 0) store_fold(f, &mypart[cg - 1][0][lane], 64);
   __syncthreads();
   if (cg > 0 || !valid) return;
-  for (int q = 0; q < CG - 1; ++q) merge_fold(f, &mypart[q][0][lane], 64);
+  for (int q = 0; q < CG - 1; ++q) merge_fold<PAGED>(f, &mypart[q][0][lane], 64);
   const float wsum = f.wsum, mmax = f.mmax;
   const float (&acc)[8] = f.acc;
   const float inv = wsum > 0.f ? 1.f / wsum : 0.f;
