@@ -75,6 +75,7 @@ SIGNATURES = {
     "tg_paged_append": [vp, i64, vp, i64, i32, i32, i32, vp, vp, f32, vp, vp, vp, i64, i64, vp, vp, i64, i64, i64,
                         vp, i64, i64, i64, i32, i32, vp],
     "tg_paged_attention_workspace_size": [i32, i32, i32, i32, i32, i32],
+    "tg_paged_attention_plan": [i32, i32, i32, i32, i32, i32, i64, vp],
     "tg_paged_attention": [vp, i64, i64, vp, i64, i64, i64, vp, i64, i64, i64, i32, i32, vp, i64, i32, vp, vp, i32, i32,
                            i32, i32, i32, i32, i32, vp, i64, i64, f32, vp, i64, i64, vp, i64, vp],
     "tg_paged_decode_attention_workspace_size": [i32, i32, i32, i32],
@@ -149,6 +150,16 @@ def fwd_plan(B, Sq, Sk, H, Hkv, causal, workspace_bytes):
     """(waves, key groups, chunks, split tiles, tiles) of a dense forward (tg_keybias_fwd_plan)."""
     plan = (C.c_int32 * 5)()
     call("tg_keybias_fwd_plan", B, Sq, Sk, H, Hkv, int(causal), int(workspace_bytes), plan)
+    return tuple(plan)
+
+
+def paged_plan(n_seqs, max_q, max_k, total_q, H, Hkv, workspace_bytes=None):
+    """(waves, key groups, chunks, split tiles, tiles, order) of tg_paged_attention (tg_paged_attention_plan); by default with
+    the workspace that it asks for."""
+    if workspace_bytes is None:
+        workspace_bytes = load().tg_paged_attention_workspace_size(n_seqs, max_q, max_k, total_q, H, Hkv)
+    plan = (C.c_int32 * 6)()
+    call("tg_paged_attention_plan", n_seqs, max_q, max_k, total_q, H, Hkv, int(workspace_bytes), plan)
     return tuple(plan)
 
 

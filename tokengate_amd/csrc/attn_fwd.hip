@@ -1934,6 +1934,22 @@ extern "C" int tg_decode_attention(const void *qkv, int64_t qkv_row_stride, cons
   return 0;
 }
 
+namespace tg {
+namespace {
+// The plan of a launch over pages, put into its arguments (sizes and heads are in them).  Returns the grid size.
+int64_t paged_grid(FwdArgs &a, PagedArgs &pages, FwdPlan &plan, int64_t workspace_bytes) {
+  const int hp = a.group % 2 == 0 ? 2 : 1;
+  const int64_t units = (int64_t)a.batch * (a.h / hp);
+  plan = plan_paged(hp, a.batch, a.sq, a.sk, a.lse_total, a.h, a.hkv, workspace_bytes);
+  if (plan.order_chunk == 0) return varlen_grid(a, plan, units, nullptr, true, a.lse_total, (int64_t)a.batch * a.sk);
+  pages.order_chunk = plan.order_chunk;
+  a.n_qtiles = plan.n_qtiles;                     // (the kernel divides by it before it looks its tile up)
+  a.ns = plan.split.ns;
+  return plan.split.heavy_units * a.ns;
+}
+}  // namespace
+}  // namespace tg
+
 extern "C" int64_t tg_paged_attention_workspace_size(int32_t num_seqs, int32_t max_seqlen_q, int32_t max_seqlen_k,
                                                      int32_t total_q, int32_t num_heads, int32_t num_heads_k) {
   if (num_seqs <= 0 || max_seqlen_q <= 0 || max_seqlen_k <= 0 || total_q <= 0 || num_heads <= 0 || num_heads_k <= 0 || num_heads % num_heads_k != 0)
@@ -1989,23 +2005,38 @@ extern "C" int tg_paged_attention(const void *q, int64_t q_row_stride, int64_t q
   a.h = num_heads; a.hkv = num_heads_k; a.group = num_heads / num_heads_k;
   a.scale_log2 = softmax_scale * kLog2e;
   PagedArgs pages{page_table, table_stride, c.k_ps, c.v_ps, table_cols, c.lg, c.n_pages, 0};
-  const int hp = a.group % 2 == 0 ? 2 : 1;
-  const int64_t units = (int64_t)num_seqs * (num_heads / hp);
-  const FwdPlan plan = plan_paged(hp, num_seqs, max_seqlen_q, max_seqlen_k, total_q, num_heads, num_heads_k,
-                                  workspace ? workspace_bytes : 0);
-  int64_t nblocks;
-  if (plan.order_chunk > 0) {
-    pages.order_chunk = plan.order_chunk;
-    a.ns = plan.split.ns;
-    nblocks = plan.split.heavy_units * a.ns;
+  FwdPlan plan;
+  const int64_t nblocks = paged_grid(a, pages, plan, workspace ? workspace_bytes : 0);
+  if (workspace) {
     a.ws_o = static_cast<bf16_t *>(workspace);
-    a.ws_ml = reinterpret_cast<float *>(static_cast<char *>(workspace) + nblocks * (plan.nw / plan.ks) * 64 * plan.split.o_bytes);
-  } else {
-    nblocks = varlen_grid(a, plan, units, workspace, true, total_q, (int64_t)num_seqs * max_seqlen_k);
+    a.ws_ml = reinterpret_cast<float *>(static_cast<char *>(workspace) +
+                                        plan.split.heavy_units * a.ns * (plan.nw / plan.ks) * 64 * plan.split.o_bytes);
   }
   TG_CHECK(nblocks < (1ll << 31), "%s: grid too large", what);
-  if (hp == 2) dispatch_paged<2>(a, pages, plan.nw, plan.ks, (int)nblocks, stream);
+  if (a.group % 2 == 0) dispatch_paged<2>(a, pages, plan.nw, plan.ks, (int)nblocks, stream);
   else dispatch_paged<1>(a, pages, plan.nw, plan.ks, (int)nblocks, stream);
   TG_HIP_CHECK(hipPeekAtLastError());
+  return 0;
+}
+
+extern "C" int tg_paged_attention_plan(int32_t num_seqs, int32_t max_seqlen_q, int32_t max_seqlen_k, int32_t total_q,
+                                       int32_t num_heads, int32_t num_heads_k, int64_t workspace_bytes, int32_t plan[6]) {
+  clear_error();
+  TG_CHECK(plan != nullptr && num_seqs > 0 && max_seqlen_q > 0 && max_seqlen_k >= 0 && total_q > 0 && num_heads_k > 0 &&
+               num_heads > 0 && num_heads % num_heads_k == 0 && workspace_bytes >= 0,
+           "paged_attention_plan: bad sizes");
+  FwdArgs a{};
+  a.batch = num_seqs; a.sq = std::min(max_seqlen_q, total_q); a.sk = max_seqlen_k;
+  a.lse_total = total_q;
+  a.h = num_heads; a.hkv = num_heads_k; a.group = num_heads / num_heads_k;
+  PagedArgs pages{};
+  FwdPlan p;
+  paged_grid(a, pages, p, workspace_bytes);
+  plan[0] = p.nw;
+  plan[1] = p.ks;
+  plan[2] = a.ns;
+  plan[3] = a.n_heavy;
+  plan[4] = a.n_qtiles;
+  plan[5] = pages.order_chunk > 0 ? 2 : a.level_order;
   return 0;
 }
