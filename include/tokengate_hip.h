@@ -527,8 +527,8 @@ int64_t tg_paged_attention_workspace_size(int32_t num_seqs, int32_t max_seqlen_q
                                           int32_t num_heads, int32_t num_heads_k);
 /* The form that tg_paged_attention takes for these sizes and this workspace on the current device, without a launch: plan[0] waves
  * per workgroup, [1] key groups among them, [2] chunks that a split tile's keys are cut into (1: no split), [3] tiles of
- * every sequence that are split (order 2: any, by their keys), [4] tiles of the longest sequence, [5] the tiles' order: 0 each
- * sequence's own, longest first, 1 level by level over the sequences, 2 by the keys they read. */
+ * every sequence that are split ([5] = 1: any, by their keys), [4] tiles of the longest sequence, [5] the tiles' order: 0 each
+ * sequence's own, longest first, 1 by the keys they read. */
 int tg_paged_attention_plan(int32_t num_seqs, int32_t max_seqlen_q, int32_t max_seqlen_k, int32_t total_q, int32_t num_heads,
                             int32_t num_heads_k, int64_t workspace_bytes, int32_t plan[6]);
 int tg_paged_attention(const void *q, int64_t q_row_stride, int64_t q_head_stride, const void *k_pages,

@@ -2,6 +2,7 @@
 them the tests on the GPU reach."""
 import pytest
 
+from paged_forms import FORMS
 from tokengate_amd import _lib
 
 # sequences, longest segment, most keys, rows, heads, KV heads
@@ -16,7 +17,7 @@ def test_tiles_of_every_launch():
         for ws in (None, 0):
             waves, groups, chunks, split, tiles, order = _lib.paged_plan(*s, workspace_bytes=ws)
             assert tiles >= 1 and 0 <= split <= tiles and (split < tiles or order == 0), (s, ws)
-            assert chunks >= 1 and (ws is None or chunks == 1) and waves % groups == 0, (s, ws)
+            assert order in (0, 1) and chunks >= 1 and (ws is None or chunks == 1) and waves % groups == 0, (s, ws)
 
 
 def test_bad_sizes():
@@ -24,3 +25,25 @@ def test_bad_sizes():
               (1, 8, 8, 8, 2, 1, -1)):
         with pytest.raises(RuntimeError, match="bad sizes"):
             _lib.paged_plan(*s)
+
+
+@pytest.mark.parametrize("form", FORMS, ids=[f.name for f in FORMS])
+def test_which_launch_a_shape_takes(form):
+    """The kernel that test_paged_forms_gpu.py's shapes are named for."""
+    n = len(form.new)
+    waves, groups, chunks, _, _, order = _lib.paged_plan(n, max(form.new), max(form.used), sum(form.new) + 2, form.H, form.Hkv)
+    assert (waves, groups, chunks > 1, order) == (form.waves, form.groups, form.split, form.by_keys)
+
+
+def test_every_launch_has_a_shape():
+    """Every form that any of many sizes takes, for one query head of a workgroup and for two."""
+    def kernel(H, Hkv, plan):
+        return plan[0], plan[1], plan[2] > 1, plan[5], 1 + ((H // Hkv) % 2 == 0)
+    taken = set()
+    for n in (1, 2, 5, 12, 20, 40, 64, 65, 100):
+        for q in (1, 16, 33, 100, 130, 200, 700, 1030, 1500, 2320, 8192):
+            for k in (q, 2 * q, 1000, 4100, 9000, 20000, 32769, 40000):
+                if k >= q:
+                    for H, Hkv in ((16, 8), (8, 4), (4, 4), (5, 5), (1, 1), (2, 1)):
+                        taken.update(kernel(H, Hkv, _lib.paged_plan(n, q, k, rows, H, Hkv)) for rows in (n * q, q + (n - 1) * q // 2))
+    assert taken == {(f.waves, f.groups, f.split, f.by_keys, 1 + ((f.H // f.Hkv) % 2 == 0)) for f in FORMS}

@@ -2037,6 +2037,6 @@ extern "C" int tg_paged_attention_plan(int32_t num_seqs, int32_t max_seqlen_q, i
   plan[2] = a.ns;
   plan[3] = a.n_heavy;
   plan[4] = a.n_qtiles;
-  plan[5] = pages.order_chunk > 0 ? 2 : a.level_order;
+  plan[5] = pages.order_chunk > 0;
   return 0;
 }
