@@ -261,6 +261,44 @@ def test_prefill_and_decode(cuda, page, ssmax):
         b_.step(cur)
 
 
+@pytest.mark.parametrize("page", [16, 64])
+def test_decode_appends_alike(cuda, page):
+    """Every key and value of every layer, the appended ones too, after decode steps taken eagerly and replayed; and what the steps
+    appended has replaced what the pages held."""
+    from tokengate_amd import decode as D_
+    m = _model(cuda)
+    steps = 4
+    pfs = [_prefill(m, steps, page) for _ in range(2)]
+    tables = [(pf.pages_below if l <= m.gate_layer else pf.pages_above).table for pf in pfs for l in range(len(pf.kv))]
+    lengths = [[cu[b + 1] - cu[b] for b in range(3)] for cu in (pfs[0].cu_prompt, pfs[0].cu_kept)]
+    layers = len(pfs[0].kv)
+
+    def rows(i, l, b, n):
+        k, v, there = keys_of(pfs[i].kv[l], tables[i * layers + l], b, n)
+        assert bool(there.all())
+        return k, v
+
+    for i in range(2):
+        for l in range(layers):                                  # no number where the steps are to write
+            table, c = tables[i * layers + l], pfs[i].kv[l]
+            for b in range(3):
+                n = lengths[l > m.gate_layer][b]
+                for j in range(n, n + steps):
+                    c.k[table[b, j // page], :, j % page] = float("nan")
+                    c.v[table[b, j // page], :, j % page] = float("nan")
+    states = [D_.DecodeState(m.weights, m.gate, m.gate_layer, pf, steps, graph=g) for pf, g in zip(pfs, (False, True))]
+    cur = pfs[0].first_tokens
+    for _ in range(steps):
+        nxt = [s.step(cur) for s in states]
+        assert torch.equal(states[0].last_logits, states[1].last_logits)
+        cur = nxt[0]
+    for l in range(layers):
+        for b in range(3):
+            n = lengths[l > m.gate_layer][b] + steps
+            for x, y in zip(rows(0, l, b, n), rows(1, l, b, n)):
+                assert bool(x.isfinite().all()) and torch.equal(x, y), (l, b)
+
+
 def test_generate(cuda):
     m = _model(cuda)
     prompts = _prompts([300, 90], [(10, 250), (0, 60)], 7)
