@@ -89,6 +89,23 @@ def test_python_refusals():
             call()
 
 
+def test_sizes_past_32_bits():
+    """A table may hold more keys than a call takes: such a max_k is refused, as the C entries do, and not cut to 32 bits."""
+    from tokengate_amd import decoder as dec
+    from tokengate_amd import paged as P
+    c = _cache(1, 1, 65536)
+    i32 = lambda *n: torch.zeros(*n, dtype=torch.int32)
+    shape, w = dec.DecoderShape(n_layers=1, n_heads=1, n_kv_heads=1), torch.ones(128, dtype=BF)
+    lw = dec.LayerWeights(None, None, w, w, None, None, None, None)
+    table = i32(1, 65537)
+    for max_k in (1 << 24, 2 ** 32 + 5, -1, -2 ** 32):
+        with pytest.raises(RuntimeError, match="max_k must be in"):
+            P.paged_attention(torch.zeros(1, 1, 128, dtype=BF), c, table, i32(2), i32(1), 1, max_k, 0.1)
+        with pytest.raises(RuntimeError, match="max_k must be in"):
+            P.paged_decode_attention(torch.zeros(1, 384, dtype=BF), torch.zeros(1, 64, 2), lw, shape, c, table, i32(1), max_k, 0.1,
+                                     torch.zeros(16, dtype=torch.uint8))
+
+
 def _call(name, good, **change):
     """The error of a C call whose arguments are `good` but for `change`, made before anything is launched."""
     from tokengate_amd import _lib

@@ -274,6 +274,19 @@ def test_attention_sizes_at_their_ends():
     assert P.paged_attention(q[:0], cache, tables, cu, used, 40, n, SCALE).shape == (0, H, D)
 
 
+@pytest.mark.parametrize("max_q", [2 ** 31, 2 ** 32 + 3, 2 ** 40])
+def test_attention_max_q_past_32_bits(max_q):
+    """Any max_q past the rows is their count."""
+    from tokengate_amd import paged as P
+    g = _gen(14)
+    H, Hkv, page = 8, 4, 32
+    table, n_pages = table_of(g, [90, 33], page)
+    cache = cache_of(g, n_pages, Hkv, page)
+    q, cu, used = normal(g, 45, H, D), _i32([0, 40, 45]), _i32([90, 33])
+    a = P.paged_attention(q, cache, table, cu, used, 40, 90, SCALE, out=torch.full_like(q, 7.0))
+    assert torch.equal(a, P.paged_attention(q, cache, table, cu, used, max_q, 90, SCALE, out=torch.full_like(q, 7.0)))
+
+
 def test_attention_more_queries_than_keys():
     """The first queries see no key: zeros."""
     _, _, _, out = _attention([20, 9], [6, 0], 16, 8, 16)

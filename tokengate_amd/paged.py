@@ -92,6 +92,13 @@ def _ints(what: str, name: str, t: torch.Tensor, n: int, dev: int) -> int:
     return t.data_ptr()
 
 
+def _max_k(what: str, max_k: int) -> int:
+    n = int(max_k)                               # (the call takes 32 bits: a larger number would be cut)
+    if not 0 <= n < 1 << 24:
+        raise RuntimeError(f"{what}: max_k must be in 0..2^24 - 1 (got {max_k})")
+    return n
+
+
 def _table(what: str, t: torch.Tensor, n_seqs: int, max_k: int, page_rows: int, dev: int) -> tuple:
     """(pointer, stride, columns) of a page table."""
     if t.dtype is not _I32 or t.dim() != 2 or t.get_device() != dev:
@@ -199,10 +206,10 @@ def paged_attention(q: torch.Tensor, cache: PagedKV, page_table: torch.Tensor, c
                     max_q: int, max_k: int, scale: float, bias_raw: Optional[torch.Tensor] = None,
                     out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """decoder.varlen_kv_attention over pages (tg_paged_attention): causal attention of every packed query segment cu_q[b]
-    .. cu_q[b + 1] - 1 of q (T, H, 128), at most max_q rows, over keys 0 .. kv_used[b] - 1 of its sequence (at most max_k), the
-    last query with the last key.  bias_raw (nseq, H, >= max_k) fp32 in raw-score units; -inf hides a key from a head
-    whatever its row holds; rows of keys that only come after a query have to be finite.  Rows that see no key get zeros, rows of no
-    segment keep what out holds."""
+    .. cu_q[b + 1] - 1 of q (T, H, 128), at most max_q rows (any number past T is T), over keys 0 .. kv_used[b] - 1 of its
+    sequence (at most max_k), the last query with the last key.  bias_raw (nseq, H, >= max_k) fp32 in raw-score units; -inf
+    hides a key from a head whatever its row holds; rows of keys that only come after a query have to be finite.  Rows that
+    see no key get zeros, rows of no segment keep what out holds."""
     what, dev, n = "paged_attention", cache.device_index, cu_q.numel() - 1
     if q.dtype is not torch.bfloat16 or q.dim() != 3 or q.shape[2] != HEAD_DIM or q.stride(2) != 1 or q.get_device() != dev:
         raise RuntimeError("paged_attention: q must be bf16 (rows, H, 128), values contiguous, on the cache's device")
@@ -220,15 +227,17 @@ def paged_attention(q: torch.Tensor, cache: PagedKV, page_table: torch.Tensor, c
         raise RuntimeError("paged_attention: rows of out overlap")
     cu = _ints(what, "cu_q", cu_q, n + 1, dev)
     used = _ints(what, "kv_used", kv_used, n, dev)
+    max_k, max_q = _max_k(what, max_k), min(int(max_q), T)
+    if max_q < 0:
+        raise RuntimeError(f"{what}: max_q must not be negative (got {max_q})")
     bias = _bias(what, bias_raw, n, H, max_k, dev)
     if n == 0 or T == 0:
         return out
     table = _table(what, page_table, n, max_k, cache.page_rows, dev)
     # (the size is of the current device's launch plan, as everything of the call)
-    ws, ws_ptr, ws_bytes = _lib.fwd_workspace("tg_paged_attention_workspace_size", q.device, n, int(max_q), int(max_k), T, H,
-                                              Hkv)
+    ws, ws_ptr, ws_bytes = _lib.fwd_workspace("tg_paged_attention_workspace_size", q.device, n, max_q, max_k, T, H, Hkv)
     _lib.call_on(dev, "tg_paged_attention", q.data_ptr(), q.stride(0) if T > 1 else H * HEAD_DIM,
-                 q.stride(1) if H > 1 else HEAD_DIM, *cache._args, *table, cu, used, n, int(max_q), int(max_k), T, H, Hkv,
+                 q.stride(1) if H > 1 else HEAD_DIM, *cache._args, *table, cu, used, n, max_q, max_k, T, H, Hkv,
                  HEAD_DIM, *bias, float(scale), out.data_ptr(), out.stride(0) if T > 1 else H * HEAD_DIM,
                  out.stride(1) if H > 1 else HEAD_DIM, ws_ptr, ws_bytes)
     return out
@@ -237,7 +246,8 @@ def paged_attention(q: torch.Tensor, cache: PagedKV, page_table: torch.Tensor, c
 def paged_decode_attention_workspace(n_seqs: int, shape: DecoderShape, max_k: int, device) -> torch.Tensor:
     """Zeroed workspace for paged_decode_attention calls of up to n_seqs sequences and max_k keys (its counters stay zero
     between calls), for one stream: calls that may overlap need one each."""
-    n = int(_lib.load().tg_paged_decode_attention_workspace_size(n_seqs, shape.n_heads, shape.n_kv_heads, int(max_k)))
+    n = int(_lib.load().tg_paged_decode_attention_workspace_size(n_seqs, shape.n_heads, shape.n_kv_heads,
+                                                                 _max_k("paged_decode_attention_workspace", max_k)))
     return torch.zeros(max(n, 16), dtype=torch.uint8, device=device)
 
 
@@ -266,6 +276,7 @@ def paged_decode_attention(qkv: torch.Tensor, rope: torch.Tensor, lw: LayerWeigh
         raise RuntimeError("paged_decode_attention: workspace must be contiguous bytes on the cache's device")
     qh = None if q_head_scale is None else _floats("paged_decode_attention", "q_head_scale", q_head_scale, H, dev)
     qr = None if q_row_scale is None else _floats("paged_decode_attention", "q_row_scale", q_row_scale, B, dev)
+    max_k = _max_k("paged_decode_attention", max_k)
     bias = _NO_BIAS if bias_raw is None else _bias("paged_decode_attention", bias_raw, B, H, max_k, dev)
     if out is None:
         out = torch.empty((B, H, HEAD_DIM), dtype=_BF16, device=qkv.device)
@@ -279,7 +290,7 @@ def paged_decode_attention(qkv: torch.Tensor, rope: torch.Tensor, lw: LayerWeigh
         return out
     table = _table("paged_decode_attention", page_table, B, max_k, cache.page_rows, dev)
     _lib.call_on(dev, "tg_paged_decode_attention", qkv.data_ptr(), rs, rope.data_ptr(), B, H, Hkv, HEAD_DIM, qw.data_ptr(),
-                 kw.data_ptr(), shape.rms_eps, qh, qr, *cache._args, *table, kv_used.data_ptr(), int(max_k), *bias, float(scale),
+                 kw.data_ptr(), shape.rms_eps, qh, qr, *cache._args, *table, kv_used.data_ptr(), max_k, *bias, float(scale),
                  out.data_ptr(), ors, workspace.data_ptr(), workspace.numel())
     return out
 
