@@ -45,3 +45,15 @@ def test_form_with_hidden_keys(form, page, bias):
             table[s, n // 3:n // 3 + n // 8] = cache.n_pages
 
     _attention(form.new, form.used, form.H, form.Hkv, page, bias=hide if bias else None, seed=page + 1, prepare=prepare)
+
+
+@forms
+@pages
+@pytest.mark.parametrize("bias", [False, True])
+def test_form_with_large_values(form, page, bias):
+    """Values near the largest float, of one sign in a KV head so that their sums grow with the keys: outputs are averages of
+    them, and finite."""
+    def prepare(cache, table, _):
+        cache.v.copy_((cache.v.abs() * 1.5e38).clamp(max=3.3e38))
+        cache.v[:, 1::2].neg_()
+    _attention(form.new, form.used, form.H, form.Hkv, page, bias=_normal_bias if bias else None, seed=page + 2, prepare=prepare)

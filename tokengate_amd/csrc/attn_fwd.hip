@@ -211,10 +211,20 @@ struct Fold {
   float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 };
 // value(e): the e-th of the chunk's eight.  (A chunk without a key, l = 0, is left out; one whose l is no number is too, but
-// not over pages: there visible keys' not-a-numbers reach the output at every split, as without one.)
+// not over pages: there visible keys' not-a-numbers reach the output at every split, as without one.  Over pages, too, acc is
+// the average so far, by weights that add up to 1, and not the sum, which values near the largest float take past it.)
 template <bool PAGED = false, typename Value>
 __device__ __forceinline__ void fold_values(Fold &f, float2 mc, Value value) {
   if (PAGED ? mc.y == 0.f : !(mc.y > 0.f)) return;
+  if constexpr (PAGED) {
+    const float m = fmaxf(f.mmax, mc.x), before = f.wsum * fast_exp2(f.mmax - m), w = mc.y * fast_exp2(mc.x - m);
+    const float r = __builtin_amdgcn_rcpf(before + w);   // (1 at least: the largest maximum's l is)
+    f.wsum = before + w;
+    f.mmax = m;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f.acc[e] = f.acc[e] * (before * r) + value(e) * (w * r);
+    return;
+  }
   if (mc.x > f.mmax) {
     const float sc = fast_exp2(f.mmax - mc.x);   // 0 while nothing has been added yet
     f.wsum *= sc;
@@ -236,8 +246,14 @@ __device__ __forceinline__ void merge_fold(Fold &f, const float *p, int stride) 
   const float m2 = p[0], w2 = p[stride];
   if (PAGED ? w2 == 0.f : !(w2 > 0.f)) return;
   const float mn = fmaxf(f.mmax, m2);
-  const float s1 = fast_exp2(f.mmax - mn), s2 = fast_exp2(m2 - mn);   // s1 = 0 if mmax = -inf
+  float s1 = fast_exp2(f.mmax - mn), s2 = fast_exp2(m2 - mn);   // s1 = 0 if mmax = -inf
+  const float before = f.wsum;
   f.wsum = f.wsum * s1 + w2 * s2;
+  if constexpr (PAGED) {
+    const float r = __builtin_amdgcn_rcpf(f.wsum);
+    s1 *= before * r;
+    s2 *= w2 * r;
+  }
 #pragma unroll
   for (int i = 0; i < 8; ++i) f.acc[i] = f.acc[i] * s1 + p[(2 + i) * stride] * s2;
   f.mmax = mn;
@@ -272,10 +288,12 @@ template <int KS> constexpr int bias_row() { return step_keys<KS>() + 4; }
 // FAR (pages) hides keys whatever their rows hold: those of no page, and those with a bias of -inf, which elsewhere only adds
 // -inf to a logit that has to be finite, with the weight 0 for a value that has to be.  It also scales and rounds a logit before the
 // maximum is taken off (in one multiply-add with the scale the rest of a product that is 2^28 and more would be a large
-// number).  Without FAR a workgroup ends at the first tile with a key of no page, or behind the last one if its sums are not finite
-// or a maximum is that large, has written nothing and returns true.  (Both in one loop, by branches or one loop after the
-// other, kept neither the registers nor the exponentials beside the products: 2320 rows with bias 54 to 65 us.  A test of
-// every tile's biases cost 12 % at 8192 rows x 32768 keys.)
+// number), and its weights are 2^-kFarLift of the others': sums of up to 2^24 values near the largest float stay finite, while
+// weights below 2^-94 of a row's largest, and products below 2^-126, count as 0.  Without FAR a workgroup ends at the first tile with
+// a key of no page, or behind the last one if its sums are not below 2^100 or a maximum is that large, has written nothing and
+// returns true.  (Both in one loop, by branches or one loop after the other, kept neither the registers nor the exponentials
+// beside the products: 2320 rows with bias 54 to 65 us.  A test of every tile's biases cost 12 % at 8192 rows x 32768 keys.)
+constexpr float kFarLift = 32.f;
 template <int NW, int KS, int HP, bool CAUSAL, bool HAS_BIAS, bool VARLEN, bool DEC, int PAGES, bool FAR>
 __device__ __forceinline__ bool fwd_body(const FwdArgs &a, const MoreArgs<DEC, PAGES> &dec, char (&ks0)[tile_bytes<KS>()],
                                          char (&ks1)[tile_bytes<KS>()], char (&vs0)[tile_bytes<KS>()],
@@ -371,7 +389,7 @@ __device__ __forceinline__ bool fwd_body(const FwdArgs &a, const MoreArgs<DEC, P
     if constexpr (PAGED) entry = dec.table[b * dec.table_rs + min((tile * SK + kPartKeys * lane) >> dec.lg, dec.cols - 1)];
   };
   if constexpr (PAGED) load_entries(0);
-  if constexpr (PAGED && HAS_BIAS && !FAR) {
+  if constexpr (PAGED && !FAR) {
     if (tid == 0) *redo = 0;                       // (the ring's first barrier is behind it)
   }
   int sq = a.sq, sk = a.sk;
@@ -703,6 +721,7 @@ __device__ __forceinline__ bool fwd_body(const FwdArgs &a, const MoreArgs<DEC, P
     }
     // what takes the accumulators to log2 units
     const float to_log2 = FAR ? 1.f : a.scale_log2;
+    constexpr float lift = FAR ? kFarLift : 0.f;   // (x - 0 is x)
 
     // ---- online softmax: lane holds KN/4 keys of one column per block; the other keys of that
     // column sit in lanes l^16, l^32, l^48 ----
@@ -779,8 +798,8 @@ __device__ __forceinline__ bool fwd_body(const FwdArgs &a, const MoreArgs<DEC, P
     // P rounded to bf16 pairs (the B operand of P V and of the row-sum product)
     uint32_t pk[2][KB][2];
     auto weigh = [&](int cb, int kb, int i) {
-      const float p0 = fast_exp2(fmaf(sacc[cb][kb][i], to_log2, mneg[cb]));
-      const float p1 = fast_exp2(fmaf(sacc[cb][kb][i + 1], to_log2, mneg[cb]));
+      const float p0 = fast_exp2(fmaf(sacc[cb][kb][i], to_log2, mneg[cb]) - lift);
+      const float p1 = fast_exp2(fmaf(sacc[cb][kb][i + 1], to_log2, mneg[cb]) - lift);
       pk[cb][kb][i >> 1] = pack_bf16x2(p0, p1);
     };
     auto step_weights = [&](int st, int cb) {
@@ -899,20 +918,20 @@ __device__ __forceinline__ bool fwd_body(const FwdArgs &a, const MoreArgs<DEC, P
     if (tile_step(t + 1, std::integral_constant<int, 1>())) return true;
   }
   if (t < t_hi && tile_step(t, std::integral_constant<int, 0>())) return true;
-  if constexpr (PAGED && HAS_BIAS && !FAR) {
+  if constexpr (PAGED && !FAR) {
     if (t_lo < t_hi) {
-      float rest = 0.f;                            // stays 0 where all are finite
+      float rest = 0.f;                            // finite where all are below 2^94, not where one is 2^100
       bool far = false;
 #pragma unroll
       for (int cb = 0; cb < 2; ++cb) {
 #pragma unroll
         for (int d = 0; d < 8; ++d)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) rest = fmaf(oacc[cb][d][i], 0.f, rest);
-        rest = fmaf(lacc[cb][0], 0.f, rest);
+          for (int i = 0; i < 4; ++i) rest = fmaf(oacc[cb][d][i], 0x1p28f, rest);
+        rest = fmaf(lacc[cb][0], 0x1p28f, rest);
         far |= fabsf(mrun[cb]) >= 0x1p28f && mrun[cb] != -INFINITY;
       }
-      if (__builtin_amdgcn_ballot_w64(far || rest != 0.f) != 0 && lane == 0) *redo = 1;
+      if (__builtin_amdgcn_ballot_w64(far || !(fabsf(rest) < INFINITY)) != 0 && lane == 0) *redo = 1;
       __syncthreads();
       if (*redo != 0) return true;
     }
@@ -959,6 +978,7 @@ __device__ __forceinline__ bool fwd_body(const FwdArgs &a, const MoreArgs<DEC, P
   for (int cb = 0; cb < 2; ++cb) {
     l[cb] = lacc[cb][0];
     inv[cb] = l[cb] > 0.f ? 1.f / l[cb] : 0.f;
+    if constexpr (FAR) l[cb] *= __builtin_exp2f(kFarLift);   // as the other chunks'
   }
   if constexpr (DEC) {
     if (chunk >= 0) {
@@ -1187,7 +1207,7 @@ __global__ __launch_bounds__(512) void keybias_fwd_combine_kernel(FwdArgs a, int
   for (int q = 0; q < CG - 1; ++q) merge_fold<PAGED>(f, &mypart[q][0][lane], 64);
   const float wsum = f.wsum, mmax = f.mmax;
   const float (&acc)[8] = f.acc;
-  const float inv = wsum > 0.f ? 1.f / wsum : 0.f;
+  const float inv = PAGED ? 1.f : wsum > 0.f ? 1.f / wsum : 0.f;
   const int h0 = kh * a.group + hg * HP;
   bf16_t *orow = a.o + (VARLEN ? row0 * a.o_rs : (int64_t)b * a.o_bs) + (int64_t)qrow * a.o_rs +
                  (int64_t)(h0 + hl) * a.o_hs;
