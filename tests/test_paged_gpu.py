@@ -4,6 +4,7 @@ bf16, p (1 + d) with |d| <= 2^-8, and as their sum is of the same numbers the ou
 (sum p |v| + |out|); paged_decode_attention's weights are two bf16 numbers, 2^-16; logits from fp32 sums move a weight by
 their own error, 2^-12 here."""
 import math
+import sys
 
 import pytest
 import torch
@@ -344,6 +345,22 @@ def test_attention_masks_of_large_numbers(low):
     _attention([40], [150], 16, 8, 64, bias=bias, average=average)
 
 
+@pytest.mark.parametrize("scale", [0.7, 1.0, 1.5])
+@pytest.mark.parametrize("new,used", [([1], [150]), ([40], [150]), ([200, 30, 5], [300, 250, 777]), ([20, 3], [6000, 20]), ([33], [9000])])
+def test_attention_masks_past_the_range_when_scaled(monkeypatch, new, used, scale):
+    """The lowest float times a scale of log2(e) of its own passes fp32's range: a row that sees nothing else still has the
+    average of its values."""
+    def bias(g, B, H, n):
+        x = torch.zeros(B, H, n, device=DEV)
+        x[:, ::2, 10:90] = torch.finfo(torch.float32).min
+        x[:, 1] = torch.finfo(torch.float32).min
+        x[0, 3, ::2], x[0, 3, 1::2] = -math.inf, torch.finfo(torch.float32).min
+        return x
+    monkeypatch.setattr(sys.modules[__name__], "SCALE", scale)
+    _attention(new, used, 8, 4, 64, bias=bias)
+    _attention(new, used, 5, 5, 16, bias=bias)
+
+
 @pytest.mark.parametrize("low", [torch.finfo(torch.float32).min, -1e30, -3e9, -math.inf])
 @pytest.mark.parametrize("new,used", [([40], [300]), ([200, 30, 5], [300, 250, 777])])
 def test_attention_masks_of_the_first_keys(low, new, used):
@@ -546,6 +563,19 @@ def test_decode_masks_of_large_numbers(low):
         x[:, 1] = low
         return x
     _decode([150, 15], 16, 8, 16, bias=bias)
+
+
+@pytest.mark.parametrize("scale", [0.7, 1.0, 1.5])
+@pytest.mark.parametrize("H,Hkv", [(16, 8), (5, 5), (16, 1)])
+def test_decode_masks_past_the_range_when_scaled(monkeypatch, H, Hkv, scale):
+    def bias(g, B, H, n):
+        x = torch.zeros(B, H, n, device=DEV)
+        x[:, ::2, 10:90] = torch.finfo(torch.float32).min
+        x[:, 1] = torch.finfo(torch.float32).min
+        x[0, 3, ::2], x[0, 3, 1::2] = -math.inf, torch.finfo(torch.float32).min
+        return x
+    monkeypatch.setattr(sys.modules[__name__], "SCALE", scale)
+    _decode([150, 15, 6000, 1], H, Hkv, 16, bias=bias)
 
 
 @pytest.mark.parametrize("H,Hkv", [(16, 8), (16, 1)])

@@ -713,7 +713,7 @@ __device__ __forceinline__ bool fwd_body(const FwdArgs &a, const MoreArgs<DEC, P
       for (int cb = 0; cb < 2; ++cb)
 #pragma unroll
         for (int e = 0; e < 4 * KB; ++e) {
-          const float z = sacc[cb][e >> 2][e & 3] * a.scale_log2;
+          const float z = HAS_BIAS ? in_range(sacc[cb][e >> 2][e & 3] * a.scale_log2) : sacc[cb][e >> 2][e & 3] * a.scale_log2;
           const uint32_t sgn = (uint32_t)((int32_t)(hidden << (31 - e)) >> 31);
           sacc[cb][e >> 2][e & 3] = u32_as_f32((sgn & 0xFF800000u) | (~sgn & __builtin_bit_cast(uint32_t, z)));
         }
@@ -930,6 +930,8 @@ __device__ __forceinline__ bool fwd_body(const FwdArgs &a, const MoreArgs<DEC, P
           for (int i = 0; i < 4; ++i) rest = fmaf(oacc[cb][d][i], 0x1p28f, rest);
         rest = fmaf(lacc[cb][0], 0x1p28f, rest);
         far |= fabsf(mrun[cb]) >= 0x1p28f && mrun[cb] != -INFINITY;
+        // a mask's lowest float, scaled past fp32's range: all that the row has, if its maximum is of nothing
+        if constexpr (HAS_BIAS) far |= a.scale_log2 > 1.f && qvalid[cb] && mrun[cb] == -INFINITY;
       }
       if (__builtin_amdgcn_ballot_w64(far || !(fabsf(rest) < INFINITY)) != 0 && lane == 0) *redo = 1;
       __syncthreads();

@@ -14,6 +14,10 @@ struct PagePool {
   int n_pages, lg;               // a page has 1 << lg rows
 };
 
+// A logit that its scale took below fp32's range (a mask's lowest float, at scales above ln 2) is the lowest float, so that it
+// weighs nothing beside others, but is not hidden.  (A not-a-number stays one.)
+__device__ __forceinline__ float in_range(float z) { return z < -3.402823466e38f ? -3.402823466e38f : z; }
+
 inline int check_pool(const char *what, const void *k, const void *v, const int64_t (&ks)[3], const int64_t (&vs)[3],
                       int32_t num_pages, int32_t page_rows, int32_t num_heads_k, int32_t head_dim, PagePool *p) {
   TG_CHECK(head_dim == kHeadDim, "%s: head_dim must be 128", what);

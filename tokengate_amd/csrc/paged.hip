@@ -317,7 +317,7 @@ __global__ __launch_bounds__(64 * kWaves, kPerCu) void paged_decode_kernel(Paged
       const float bias = HAS_BIAS ? a.bias[(int64_t)b * a.bias_bs + (int64_t)(h0 + min(i, nh - 1)) * a.bias_hs + nk] : 0.f;
       const bool hidden = bias == -INFINITY;
       if (n16 == 0) {
-        part_ml[kWaves][i][0] = hidden ? -INFINITY : (z + bias) * a.scale_log2;
+        part_ml[kWaves][i][0] = hidden ? -INFINITY : HAS_BIAS ? in_range((z + bias) * a.scale_log2) : z * a.scale_log2;
         part_ml[kWaves][i][1] = hidden ? 0.f : 1.f;
       }
     }
@@ -343,6 +343,7 @@ __global__ __launch_bounds__(64 * kWaves, kPerCu) void paged_decode_kernel(Paged
     for (int j = 0; j < 8; ++j) {
       z[j] = (HAS_BIAS ? s[j >> 2][j & 3] + l.bias[j] : s[j >> 2][j & 3]) * a.scale_log2;
       asm("" : "+v"(z[j]));   // rounded: contracted into z - m below, a bias near the lowest float leaves the rounding's rest
+      if constexpr (HAS_BIAS) z[j] = in_range(z[j]);
       if (j >= l.valid) z[j] = -INFINITY;
       if constexpr (HAS_BIAS) z[j] = l.bias[j] == -INFINITY ? -INFINITY : z[j];   // hidden, whatever the row holds
       most = fmaxf(most, z[j]);
