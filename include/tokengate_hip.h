@@ -519,10 +519,9 @@ int tg_paged_append(const void *qkv, int64_t qkv_row_stride, const float *rope, 
 /* Causal attention of every packed query segment over its sequence's pages: query i of n_q = cu_seqlens_q[b + 1] -
  * cu_seqlens_q[b] (at most max_seqlen_q) sees keys j <= i + n_k - n_q of n_k = min(kv_used[b], max_seqlen_k), logits softmax_scale *
  * (q . k_j + bias_raw[b, h, j]), those below fp32's range its lowest number.  Rows that see no key get zeros; rows of no sequence
- * keep what out holds.  A bias of -inf hides a
- * key from the head whatever its row holds, as does an entry that names no page; the rows of keys that a query
- * only comes before have to be finite.  Weights in bf16, fp32 sums (where these pass 2^94 the tile is taken again with weights
- * 2^-32 as large, so that finite values have finite averages); workspace: tg_paged_attention_workspace_size bytes
+ * keep what out holds.  A bias of -inf hides a key from the head whatever its row holds, as does an entry that names no page; the
+ * rows of keys that a query only comes before have to be finite.  Weights in bf16, fp32 sums (where these pass 2^94 the tile is
+ * taken again with weights 2^-32 as large, so that finite values have finite averages); workspace: tg_paged_attention_workspace_size bytes
  * for the key-range split of small launches (NULL or fewer bytes: no split), contents need no initialisation, shared by
  * stream-ordered calls.  max_seqlen_k < 2^24 and at most table_cols * page_rows. */
 int64_t tg_paged_attention_workspace_size(int32_t num_seqs, int32_t max_seqlen_q, int32_t max_seqlen_k, int32_t total_q,

@@ -281,9 +281,9 @@ template <int KS> constexpr int tile_bytes() { return step_keys<KS>() * kKRowByt
 template <int KS> constexpr int bias_row() { return step_keys<KS>() + 4; }
 
 // PAGES: 0 none, 1 of 16 or 32 rows (a load's four keys through a descriptor of their own), 2 of 64 and more (64 keys through one).
-// us over contiguous K and V / pages of 64 rows / of 16, 16 / 8 heads, causal: 1024 x 1024 17.6 / 18.9 / 20.1, 2320 x 2320
-// 39.6 / 41.4 / 44.0, 8192 x 8192 243 / 250 / 260, 8192 x 32768 1580 / 1608 / 1650; with bias 39.8 / 43.3 / 45.7 and 1605 / 1656 / 1702.
-// The order of the pages, and rows of a head apart or together, make no difference.
+// us over contiguous K and V / pages of 64 rows / of 16, 16 / 8 heads, causal: 1024 x 1024 16.5 / 18.4 / 19.4, 2320 x 2320
+// 38.1 / 41.3 / 43.6, 8192 x 8192 237 / 246 / 255, 8192 x 32768 1521 / 1567 / 1619; with bias 16.8 / 19.0 / 20.2, 39.2 / 42.9 / 45.6,
+// 241 / 253 / 262 and 1560 / 1615 / 1664.  The order of the pages, and rows of a head apart or together, make no difference.
 //
 // FAR (pages) hides keys whatever their rows hold: those of no page, and those with a bias of -inf, which elsewhere only adds
 // -inf to a logit that has to be finite, with the weight 0 for a value that has to be.  It also scales and rounds a logit before the
@@ -293,6 +293,8 @@ template <int KS> constexpr int bias_row() { return step_keys<KS>() + 4; }
 // a key of no page, or behind the last one if its sums are not below 2^100 or a maximum is that large, has written nothing and
 // returns true.  (Both in one loop, by branches or one loop after the other, kept neither the registers nor the exponentials
 // beside the products: 2320 rows with bias 54 to 65 us.  A test of every tile's biases cost 12 % at 8192 rows x 32768 keys.)
+// Both share one allocation of registers: biased forms hold 256 (key groups of four 223 to 229), with key groups of two up to 2
+// more in scratch, and 46 to 69 scalar ones in vector lanes; unbiased ones 199 to 247, none in scratch, 26 to 41.
 constexpr float kFarLift = 32.f;
 template <int NW, int KS, int HP, bool CAUSAL, bool HAS_BIAS, bool VARLEN, bool DEC, int PAGES, bool FAR>
 __device__ __forceinline__ bool fwd_body(const FwdArgs &a, const MoreArgs<DEC, PAGES> &dec, char (&ks0)[tile_bytes<KS>()],
@@ -379,7 +381,8 @@ __device__ __forceinline__ bool fwd_body(const FwdArgs &a, const MoreArgs<DEC, P
 
   // Pages: where 64 parts of 16 keys (PAGES 2: 64) begin in K and V is computed at once, by lane, for the next kBatch tiles; the
   // entries of the batch after it are loaded meanwhile (the first ones before anything else).  Tile by tile, 8192 rows x
-  // 8192 keys of 64-row pages took 266 us, so 263 (16-row pages 292, 277).  parts_gone: by bit, which parts have no page;
+  // 8192 keys of 64-row pages took 266 us, so 263 (16-row pages 292, 277; both
+  // before the products' order below was written out).  parts_gone: by bit, which parts have no page;
   // no_page: which 16 keys of the issued tile.
   constexpr int kPartKeys = PAGES == 2 ? 64 : 16, kParts = SK / kPartKeys, kBatch = 64 / kParts;
   [[maybe_unused]] int32_t entry = 0;
@@ -795,7 +798,8 @@ __device__ __forceinline__ bool fwd_body(const FwdArgs &a, const MoreArgs<DEC, P
         for (int d = 0; d < 8; ++d) oacc[cb][d] *= alpha;
       }
     }
-    // P rounded to bf16 pairs (the B operand of P V and of the row-sum product)
+    // P rounded to bf16 pairs (the B operand of P V and of the row-sum product): a relative error of 2^-8 that the row sum, of the
+    // same numbers, has too.  Two bf16 numbers a weight would be half again as many matrix instructions.
     uint32_t pk[2][KB][2];
     auto weigh = [&](int cb, int kb, int i) {
       const float p0 = fast_exp2(fmaf(sacc[cb][kb][i], to_log2, mneg[cb]) - lift);
@@ -1467,14 +1471,17 @@ FwdPlan plan_varlen(int hp, int max_sq, int max_sk, int64_t units, bool causal, 
 
 // A launch over pages.  One sequence has a dense launch's forms.  Up to 64 take their tiles by the keys they read (key_tile), in
 // the form, and cut into as many chunks, as an estimate finds quickest: the longest chunk, or the steps spread over the places
-// (the lengths behind the maxima are not known here: of a ragged batch's tiles 0.85 of the most, in 0.6 ns + 0.5 chunks),
+// (the lengths behind the maxima are not known here: of a ragged batch's tiles 0.85 of the most, in 0.6 ns + 0.5 chunks, ragged
+// where the rows are fewer than so many of the longest: parts of one size over contexts of many lengths count as even),
 // and for chunks the second launch and its traffic, and, as two that share a CU end long before others do where they all fit at
 // once, 0.45 of one more round: 8 of 200 and 12000 165 us in 4 chunks, 122 in 8).  Sequences with many tiles each whose K/V
-// outgrow the last-level cache keep their own order (varlen_level_order's reason).
+// outgrow the last-level cache keep their own order (varlen_level_order's reason; us in it / by the keys they read, 12 x 1024 rows
+// of 8192 keys: alike 708 / 749, ragged 374 / 368; 32 x 1024 x 8192 1891 / 2255, 824 / 821; but 12 x 1024 x 4099 364 / 346, 194 / 165).
 // us of the varlen launch's plan / this one / the quickest of 16 forms with up to 32 chunks, 16 / 8 heads, ragged sequences x
 // rows x keys up to (measured before the products' order was written out, which made all 5 % quicker): 12 x 700 x 4099
 // 225 / 161 / 161; 8 x 200 x 12000 177 / 122 / 115; 24 x 100 x 1500 50 / 35 / 35; 3 x 2500 x 8000 305 / 235 / 216;
-// 8 x 1000 x 1000 39 / 35 / 35; 4 x 512 x 512 25 / 18 / 18; 16 x 16 x 4000 43 / 41 / 41; 4 x 64 x 8000 34 / 38 / 34.
+// 8 x 1000 x 1000 39 / 35 / 35; 4 x 512 x 512 25 / 18 / 18; 16 x 16 x 4000 43 / 41 / 41; 4 x 64 x 8000 34 / 38 / 34.  This one now, with
+// pages of 64 rows / 16: 140 / 148; 112 / 120; 32 / 34; 215 / 225; 33 / 34; 18 / 18; 38 / 40; 36 / 38.
 FwdPlan plan_paged(int hp, int num_seqs, int max_sq, int max_sk, int64_t total_q, int num_heads, int num_heads_k,
                    int64_t workspace_bytes) {
   const int64_t heads = num_heads / hp, units = num_seqs * heads;

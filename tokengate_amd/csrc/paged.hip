@@ -12,7 +12,8 @@ namespace {
 
 // ---- start of a step: the packed rows' slots and rotary table -----------------------------------------
 // One wave a row.  The row's sequence is the last one that begins at or before it (a bisection over cu_seqlens, whose
-// values the lanes read alike).  Angles as tg_decode_begin's and tg_qk_norm_rope's: position * inv_freq in fp32.
+// values the lanes read alike).  Angles as tg_decode_begin's and tg_qk_norm_rope's: position * inv_freq in fp32.  8 rows take the
+// launch (2.3 us); 32768 rows 8.4 us, 2.8 of them for the bytes (17 MB, nearly all written), the rest sines and cosines.
 struct BeginArgs {
   const int64_t *pos;
   int64_t n;
@@ -66,7 +67,7 @@ struct AppendArgs {
   PagePool c;
   int groups;                    // of 16 lanes per token
 };
-// Bound by bytes: q | k | v read and written once (32768 rows 98 .. 106 us, 5.2 .. 5.6 TB/s), few rows by the launch (8: 3.1).
+// Bound by bytes: q | k | v read and written once (32768 rows 101 .. 103 us, 5.4 TB/s), few rows by the launch (8: 3.1).
 // Sixteen lanes take kRowsPer heads of a token, all loads ahead of the first product; with 1 / 2 / 4 heads 32768 rows take
 // 112 / 104 / 116 us, and 110 with two whose stores go through the caches.
 constexpr int kRowsPer = 2;
@@ -125,17 +126,19 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a) {
 // (find_chunk); the last workgroup of a unit to arrive merges its chunks.  A wave takes 32 keys at a time, straight from the
 // pages to registers in the layouts that the matrix cores read, so nothing waits at a barrier.  Bound by the bytes of K and V
 // where there are many keys (8 of up to 131072 keys 441 us: 5.8 TB/s; 64 of up to 4099 131: 4.8), by dependent latencies where
-// there are few: lengths and pages, norms, one tile and the waves' merge take 5.8 us, 300 keys 8.0, 2320 10.4, 32769 31.
+// there are few: lengths and pages, norms, one tile and the waves' merge take 5.8 us, 300 keys 8.0, 2320 10.4, 32769 31 (27 where
+// they are in the last-level cache).
 //   * S^T = K Q^T (v_mfma_f32_16x16x32_bf16): A holds keys, lane (n, G) (n = lane % 16, G = lane / 16) elements 32 i + 8 G
 //     .. + 7 of key 8 (n / 4) + 4 t + n % 4 of instruction t (0, 1); B the query heads, head n % HP in column n.  So lane
 //     (n, G) ends up with the logits of keys 8 G .. 8 G + 7 of its head: in the order that the weights have as O's A.
 //   * O = P V: a lane reads 16 bytes (elements 8 n .. 8 n + 7) of keys 8 G .. 8 G + 7; instruction e takes element 8 n + e of
 //     the eight, one byte permutation per two.
-//   * A weight is two bf16 numbers, 16 bits together (relative error 2^-17; rounded to one it would be 2^-9, as much as
+//   * A weight is two bf16 numbers, 16 bits together (relative error 2^-17; rounded to one it would be 2^-8, as much as
 //     the output's own rounding): columns repeat the heads, and every other repetition holds the second numbers.  With 16
 //     heads there is no repetition, and the second numbers are a second product.
 //   * The new key is not in the tiles: it is a part of its own beside the waves', from registers.
-//   * Keys past the sequence's last, or of no page, are of weight 0 and their values 0, whatever the rows hold.  A key that a
+//   * Keys past the sequence's last, or of no page (page 0's rows are read in their place), are of weight 0 and their values 0,
+//     whatever the rows hold.  A key that a
 //     bias of -inf hides from a head may hold anything too: a wave whose sums are not finite takes its tiles once more,
 //     each head by itself with the rows it does not see left out, and with weights 2^-64 of these (values near the largest
 //     float pass fp32's range in the first sums).
